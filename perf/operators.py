@@ -130,7 +130,8 @@ def prepare(case, seed):
         qkv = _randn(g, b, n, h + 2 * hk, d, dtype=dtype)
         q, k, v = (t.transpose(1, 2) for t in qkv.split([h, hk, hk], dim=2))
         s["q"], s["k"], s["v"] = (t.detach().requires_grad_(case["train"]) for t in (q, k, v))
-        s["rel_bias"] = _randn(g, h, 2 * case["r_max"] + 1, std=0.5).requires_grad_(case["train"]) if case["r_max"] else None
+        # the learned bias in the type of the projections, as a layer cast to 16 bits has it
+        s["rel_bias"] = _randn(g, h, 2 * case["r_max"] + 1, dtype=dtype, std=0.5).requires_grad_(case["train"]) if case["r_max"] else None
         s["mask"] = None
         if case["pad"]:
             s["mask"] = torch.ones(b, n, dtype=torch.bool, device="cuda")
@@ -262,7 +263,7 @@ def _plain_attn(s):
         by_offset = skewed.sum(1, dtype=torch.float64)   # column c: j - i = n - 1 - c
         at = torch.arange(n - 1, -n, -1, device=q.device).clamp_(-s["r_max"], s["r_max"]) + s["r_max"]
         db = torch.zeros(s["heads"], 2 * s["r_max"] + 1, dtype=torch.float64, device=q.device)
-        out.append(db.index_add_(1, at, by_offset).float())
+        out.append(db.index_add_(1, at, by_offset).to(s["q"].dtype))
     return tuple(out)
 
 
