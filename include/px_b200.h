@@ -156,7 +156,8 @@ PX_API int32_t px_trimul_contract(const px_f16* a, const px_f16* b, px_f16* x, i
 #define PX_FAMILY_MSA_TRANSITION 13
 #define PX_FAMILY_MSA_AVERAGE 14
 #define PX_FAMILY_MSA_ROWS 15
-#define PX_N_FAMILIES 16
+#define PX_FAMILY_RELPOS 16
+#define PX_N_FAMILIES 17
 PX_API int32_t px_device_error_flags(uint32_t* flags);
 PX_API int32_t px_device_error_detail(uint32_t* flags, uint32_t* detail);
 /* Limit of every bounded wait on the current device, in SM clock cycles (default 2^28, about 0.14 s); cycles <= 0
@@ -382,6 +383,31 @@ PX_API int32_t px_opm_out(const px_f16* x, const px_f16* w_out, const float* bia
  * and backward), whose mask comes from a counter-based generator inside the kernel; here the caller draws it. */
 PX_API int32_t px_scale_add_rowwise(const void* residual, const void* x, const void* mask, void* out, int64_t batches,
                              int64_t rows, int64_t cd, int32_t dtype, void* stream);
+
+/* ---- Dropout from a counter-based generator, with the residual add (training path) -----------
+ * out[o][s][i] = residual[o][s][i] + keep(o, i) x[o][s][i] / (1 - p) for tensors [outer][shared][inner] of one type (PX_F32, PX_BF16,
+ * PX_F16); residual NULL: the product alone (the gradient with respect to x for a given gradient of out).  out may be x or residual.
+ * keep(e) = word e mod 4 of Philox4x32-10 with key `seed` and counter (e / 4, offset), both 64-bit, is at least round(p 2^32), e = o inner + i:
+ * a function of seed, offset and place, so that no mask is stored.  A dropped element gives the residual (or 0) whatever x holds; 0 <= p <= 1.
+ * state: NULL, or two device words (seed, offset) that the kernel reads in place of the arguments, so that a captured call draws anew
+ * when they change; used: NULL, or two device words that receive what the call used (not `state` itself).
+ * Stands in for the in-kernel generator of protenix/model/modules/fused_ops.py:40-187 and for the Dropout modules of
+ * protenix/model/triangular/layers.py (shared axis: batch_dim). */
+PX_API int32_t px_dropout_add(const void* residual, const void* x, void* out, int64_t outer, int64_t shared, int64_t inner, double p,
+                       int64_t seed, int64_t offset, const int64_t* state, int64_t* used, int32_t dtype, void* stream);
+
+/* ---- Relative position encoding of token pairs, and the gradient of its weight ---------------
+ * z[b][i][j][:] = W onehot(buckets of (i, j)), features [batch][n], W fp32 [c][4 r_max + 2 s_max + 7] (columns: residue
+ * offsets, token offsets, same entity, copy offsets, as the reference concatenates them), z PX_F32, PX_BF16 or PX_F16 [batch][n][n][c].
+ * The gradient dw (fp32, like W) is a sum over the pairs of each bucket in a fixed order.  c a multiple of 8,
+ * 4 r_max + 2 s_max + 5 <= 380.  Replace RelativePositionEncoding (protenix/model/modules/embedders.py) and its autograd. */
+PX_API int64_t px_relpos_workspace_bytes(int64_t batch, int64_t n, int64_t c, int32_t r_max, int32_t s_max);
+PX_API int32_t px_relpos_fwd(const int64_t* asym_id, const int64_t* residue_index, const int64_t* entity_id, const int64_t* token_index,
+                      const int64_t* sym_id, const float* w, void* z, int64_t batch, int64_t n, int64_t c, int32_t r_max,
+                      int32_t s_max, int32_t dtype, void* stream);
+PX_API int32_t px_relpos_bwd(const int64_t* asym_id, const int64_t* residue_index, const int64_t* entity_id, const int64_t* token_index,
+                      const int64_t* sym_id, const void* dz, float* dw, void* workspace, int64_t workspace_bytes, int64_t batch,
+                      int64_t n, int64_t c, int32_t r_max, int32_t s_max, int32_t dtype, void* stream);
 
 /* ---- Exchange between the GPUs of one box (row-sharded path) ------------------------------
  * No counterpart in the reference (which runs the Pairformer on one GPU).  A peer buffer is a

@@ -1,6 +1,7 @@
 """B200-native (sm_100a) Pairformer pair-representation forward path behind the module API of
 bytedance/Protenix.  One code path: hand-written CUDA kernels reached through a C ABI
 (``include/px_b200.h``); nothing falls back to the CPU or to another back-end."""
+from .embedders import RelativePositionEncoding, relative_position_encoding
 from .layer_norm import FusedLayerNorm, LayerNorm
 from .msa import OuterProductMean
 from .pairformer import PairformerBlock, PairformerStack
@@ -10,7 +11,7 @@ from .transformer import AttentionPairBias
 from .triangular import (OpenfoldLinear, TriangleAttention, TriangleAttentionEndingNode,
                          TriangleAttentionStartingNode, TriangleMultiplicationIncoming,
                          TriangleMultiplicationOutgoing, TriangleMultiplicativeUpdate)
-from .fused_ops import dropout_add_rowwise
+from .fused_ops import dropout_add, dropout_add_rowwise
 from .weights import weights_changed
 
 __all__ = [
@@ -18,6 +19,6 @@ __all__ = [
     "AttentionPairBias", "OpenfoldLinear", "TriangleAttention", "TriangleAttentionEndingNode",
     "TriangleAttentionStartingNode", "TriangleMultiplicationIncoming", "TriangleMultiplicationOutgoing",
     "TriangleMultiplicativeUpdate", "dropout_add_rowwise", "RecyclingTrunk", "OuterProductMean",
-    "weights_changed",
+    "weights_changed", "dropout_add", "RelativePositionEncoding", "relative_position_encoding",
 ]
 __version__ = "0.1.0"

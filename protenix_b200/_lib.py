@@ -7,7 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_char_p, c_float, c_int32, c_int64, c_void_p
+from ctypes import c_char_p, c_double, c_float, c_int32, c_int64, c_void_p
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 # PX_B200_LIB names another build of the same library (e.g. one compiled with different options)
@@ -15,7 +15,7 @@ LIB_PATH = os.environ.get("PX_B200_LIB") or os.path.join(HERE, "libpx_b200.so")
 
 PX_F32, PX_BF16, PX_F16 = 0, 1, 2
 
-P, I32, I64, F = c_void_p, c_int32, c_int64, c_float
+P, I32, I64, F, D = c_void_p, c_int32, c_int64, c_float, c_double
 
 # name -> (restype, argtypes); mirrors include/px_b200.h declaration by declaration
 SIGNATURES = {
@@ -80,6 +80,10 @@ SIGNATURES = {
     "px_single_finish": (I32, [P, P, I32, P, P, P, P, P, I64, I64, F, P]),
     "px_recycle_update": (I32, [P, P, P, I32, P, P, P, I64, F, P]),
     "px_scale_add_rowwise": (I32, [P, P, P, P, I64, I64, I64, I32, P]),
+    "px_dropout_add": (I32, [P, P, P, I64, I64, I64, D, I64, I64, P, P, I32, P]),
+    "px_relpos_workspace_bytes": (I64, [I64, I64, I64, I32, I32]),
+    "px_relpos_fwd": (I32, [P, P, P, P, P, P, P, I64, I64, I64, I32, I32, I32, P]),
+    "px_relpos_bwd": (I32, [P, P, P, P, P, P, P, P, I64, I64, I64, I64, I32, I32, I32, P]),
     "px_opm_outer": (I32, [P, P, P, I64, I64, I64, P]),
     "px_opm_out": (I32, [P, P, P, P, P, P, I32, I64, I64, I32, P]),
     "px_peer_alloc": (I32, [I64, P, P]),

@@ -1,0 +1,331 @@
+// Relative position encoding of token pairs (RelativePositionEncoding of the reference's input embedder; AlphaFold 3, algorithm 3):
+//   z[i][j][:] = W_pos[bp] + W_tok[bt] + [same entity] W_ent + W_chain[bc]           rows of W^T, W = [c][4 r + 2 s + 7]
+//   bp = same chain ? clip(residue_i - residue_j + r, 0, 2 r) : 2 r + 1
+//   bt = same chain and residue ? clip(token_i - token_j + r, 0, 2 r) : 2 r + 1
+//   bc = same entity ? clip(copy_i - copy_j + s, 0, 2 s) : 2 s + 1
+// and the gradient of W: sums of dz over the pairs of a bucket.  The one-hot matrix never exists.
+//
+// Two table rows make a pair: bt differs from 2 r + 1 only where bp = r, and the entity's flag follows from bc, so there are
+// 4 r + 3 sums W_pos + W_tok and 2 s + 2 sums W_chain + W_ent (both tables 70 KB of shared memory for r = 32, s = 2 and 128 channels).
+//
+// Forward: memory-bound writer, a warp takes 32 neighbouring pairs of a row; a lane finds one pair's two rows, then the warp
+// writes pair after pair, 4 channels a lane, and looks the rows up again only where they change (most neighbours are far apart or in
+// another chain: clipped alike).
+//
+// Backward: memory-bound reader.  A block of two warps (64 channels each, two a lane) reads a run of pairs through a ring of bulk copies and
+// holds sums of its own for every table row in shared memory, so there are no atomics and a call gives the same bits every time.  A lane adds up neighbours with
+// the same rows in registers and goes to the shared sums only where they change.  The blocks' sums, folded to the columns of W, are
+// added up in their order by a second kernel.
+#include "px_tcgen05.cuh"
+
+namespace px {
+
+constexpr int kRpChunk = 128;           // channels a block handles
+constexpr int kRpMaxRows = 380;         // rows of both tables together: what shared memory holds beside the backward pass's ring
+constexpr int kRpPairs = 32;            // pairs of a warp's step, and of a backward stage of 16-bit values
+constexpr int kRpStages = 4;
+constexpr int kRpStageBytes = 8192;
+
+struct RelposArgs {
+  const long long *asym, *residue, *entity, *token, *sym;      // [batch][n]
+  long long n, pairs;                    // tokens; pairs of all batches
+  int c, r, s;                           // channels and clipping distances
+  __host__ __device__ int rows1() const { return 4 * r + 3; }
+  __host__ __device__ int rows2() const { return 2 * s + 2; }
+  __host__ __device__ int columns() const { return 4 * r + 2 * s + 7; }
+};
+
+__device__ __forceinline__ int clip_to(long long d, int r) {      // in 0 .. 2 r
+  return d < -(long long)r ? 0 : d > (long long)r ? 2 * r : (int)d + r;
+}
+// The table rows of a pair: the first table's in the low half, the second's in the high half.  (Differences wrap as the tensor ones do.)
+__device__ __forceinline__ uint32_t relpos_code(const RelposArgs& a, long long at_i, long long at_j) {
+  const auto less = [&](const long long* v) { return (long long)((unsigned long long)__ldg(v + at_i) - (unsigned long long)__ldg(v + at_j)); };
+  const bool chain = less(a.asym) == 0, entity = less(a.entity) == 0;
+  const long long dr = less(a.residue);
+  int first = 2 * a.r + 1;
+  if (chain) first = dr == 0 ? 2 * a.r + 2 + clip_to(less(a.token), a.r) : clip_to(dr, a.r);
+  const int second = entity ? clip_to(less(a.sym), a.s) : 2 * a.s + 1;
+  return (uint32_t)first | (uint32_t)second << 16;
+}
+
+template <typename T>
+__device__ __forceinline__ void store4(T* p, float4 v);
+template <>
+__device__ __forceinline__ void store4<float>(float* p, float4 v) { __stcs(reinterpret_cast<float4*>(p), v); }
+template <>
+__device__ __forceinline__ void store4<bf16>(bf16* p, float4 v) {
+  __stcs(reinterpret_cast<uint2*>(p), make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w)));
+}
+template <>
+__device__ __forceinline__ void store4<__half>(__half* p, float4 v) {
+  const __half2 lo = __floats2half2_rn(v.x, v.y), hi = __floats2half2_rn(v.z, v.w);
+  __stcs(reinterpret_cast<uint2*>(p), make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi)));
+}
+
+constexpr int kRpFwdThreads = 512;
+constexpr int kRpPitch = kRpChunk + 4;   // floats of a table row: rows 16 bytes apart in the banks while the tables are laid out
+
+template <typename T>
+__global__ void __launch_bounds__(kRpFwdThreads) relpos_fwd_kernel(RelposArgs a, const float* __restrict__ w, T* __restrict__ z) {
+  extern __shared__ __align__(16) float rp_table[];
+  const int c0 = blockIdx.y * kRpChunk, channels = min(kRpChunk, a.c - c0), t = a.columns();
+  const int rows1 = a.rows1(), rows2 = a.rows2(), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int pos = 0, tok = 2 * a.r + 2, ent = 4 * a.r + 4, chain = ent + 1;      // first columns of the four parts of W
+  for (int ch = warp; ch < channels; ch += kRpFwdThreads / 32) {
+    const float* row = w + (long long)(c0 + ch) * t;
+    for (int k = lane; k < rows1 + rows2; k += 32) {
+      float v;
+      if (k < tok) v = row[pos + k] + row[tok + 2 * a.r + 1];
+      else if (k < rows1) v = row[pos + a.r] + row[tok + k - tok];
+      else v = row[chain + k - rows1] + (k - rows1 < 2 * a.s + 1 ? row[ent] : 0.f);
+      rp_table[k * kRpPitch + ch] = v;
+    }
+  }
+  __syncthreads();
+  const long long strips = (a.n + kRpPairs - 1) / kRpPairs, rows = a.pairs / a.n;
+  const long long warps = (long long)gridDim.x * (kRpFwdThreads / 32);
+  const bool mine = 4 * lane < channels;
+  for (long long u = (long long)blockIdx.x * (kRpFwdThreads / 32) + warp; u < rows * strips; u += warps) {
+    const long long i = u / strips, j0 = (u - i * strips) * kRpPairs, first = i / a.n * a.n;     // i counts the rows of all batches
+    const int count = (int)min((long long)kRpPairs, a.n - j0);
+    const uint32_t code = relpos_code(a, i, first + j0 + min(lane, count - 1));
+    T* out = z + (i * a.n + j0) * a.c + c0 + 4 * lane;
+    uint32_t have = 0xffffffffu;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int k = 0; k < count; ++k) {
+      const uint32_t now = __shfl_sync(0xffffffffu, code, k);
+      if (now != have) {
+        have = now;
+        const float4 p = *reinterpret_cast<const float4*>(rp_table + (now & 0xffffu) * kRpPitch + 4 * lane);
+        const float4 q = *reinterpret_cast<const float4*>(rp_table + (rows1 + (now >> 16)) * kRpPitch + 4 * lane);
+        v = make_float4(p.x + q.x, p.y + q.y, p.z + q.z, p.w + q.w);
+      }
+      if (mine) store4(out + (long long)k * a.c, v);
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ float2 load2(const T* p);
+template <>
+__device__ __forceinline__ float2 load2<float>(const float* p) { return *reinterpret_cast<const float2*>(p); }
+template <>
+__device__ __forceinline__ float2 load2<bf16>(const bf16* p) { return unpack_bf16x2(*reinterpret_cast<const uint32_t*>(p)); }
+template <>
+__device__ __forceinline__ float2 load2<__half>(const __half* p) { return unpack_f16x2(*reinterpret_cast<const uint32_t*>(p)); }
+
+__device__ __forceinline__ void bulk_load(void* to, const void* from, uint32_t bytes, uint64_t* bar) {      // multiples of 16 bytes
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(smem_u32(to)), "l"(from),
+               "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+// Block b adds up the pairs [b * per, (b + 1) * per) of its channels; partial: [chunk][block][columns][kRpChunk].
+template <typename T>
+__global__ void __launch_bounds__(64) relpos_bwd_kernel(RelposArgs a, const T* __restrict__ dz, float* __restrict__ partial, long long per) {
+  constexpr int kPairs = kRpStageBytes / (kRpChunk * (int)sizeof(T));      // of a stage: 16 (fp32) or 32
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  __shared__ uint64_t full[kRpStages];
+  T* stage = reinterpret_cast<T*>(smem_raw);
+  float* sums = reinterpret_cast<float*>(smem_raw + kRpStages * kRpStageBytes);
+  const int c0 = blockIdx.y * kRpChunk, channels = min(kRpChunk, a.c - c0), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int rows1 = a.rows1(), rows = rows1 + a.rows2();
+  const long long begin = (long long)blockIdx.x * per, end = min(begin + per, a.pairs);
+  const int steps = (int)((end - begin + kPairs - 1) / kPairs);
+  if (threadIdx.x == 0) {
+    for (int k = 0; k < kRpStages; ++k) mbar_init(&full[k], 1);
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+  }
+  // the parts of a stage that no copy reaches (channels and pairs beyond the last) are added up as zeros
+  for (int k = threadIdx.x; k < kRpStages * kRpStageBytes / 16; k += 64) reinterpret_cast<uint4*>(smem_raw)[k] = make_uint4(0u, 0u, 0u, 0u);
+  for (int k = threadIdx.x; k < rows * kRpChunk / 4; k += 64) reinterpret_cast<float4*>(sums)[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+  asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+  __syncthreads();
+  const auto fetch = [&](int step) {              // one thread
+    const long long p0 = begin + (long long)step * kPairs;
+    const int count = (int)min((long long)kPairs, end - p0), b = step % kRpStages;
+    const uint32_t bytes = (uint32_t)(channels * sizeof(T));
+    T* to = stage + b * (kRpStageBytes / (int)sizeof(T));
+    mbar_expect_tx(&full[b], bytes * count);
+    if (a.c == kRpChunk) {
+      bulk_load(to, dz + p0 * a.c, bytes * count, &full[b]);
+    } else {
+      for (int k = 0; k < count; ++k) bulk_load(to + k * kRpChunk, dz + (p0 + k) * a.c + c0, bytes, &full[b]);
+    }
+  };
+  if (threadIdx.x == 0)
+    for (int k = 0; k < kRpStages - 1 && k < steps; ++k) fetch(k);
+  float2* const mine = reinterpret_cast<float2*>(sums) + 32 * warp + lane;       // row k: mine[k * kRpChunk / 2]
+  int row1 = -1, row2 = -1;                        // what the running sums belong to
+  float2 run1 = make_float2(0.f, 0.f), run2 = run1;
+  const auto flush = [&](int row, float2& run) {
+    if (row >= 0) {
+      float2* const p = mine + row * (kRpChunk / 2);
+      const float2 v = *p;
+      *p = make_float2(v.x + run.x, v.y + run.y);
+    }
+    run = make_float2(0.f, 0.f);
+  };
+  bool ok = true;
+  for (int step = 0; step < steps; ++step) {
+    const long long p0 = begin + (long long)step * kPairs;
+    const int count = (int)min((long long)kPairs, end - p0), b = step % kRpStages;
+    const long long p = p0 + min(lane, count - 1), i = p / a.n;
+    const uint32_t code = relpos_code(a, i, i / a.n * a.n + (p - i * a.n));
+    ok = mbar_wait_warp(&full[b], (step / kRpStages) & 1, 1u);
+    ok = __syncthreads_and(ok) != 0;               // both warps are through with the stage that is filled next
+    if (!ok) break;
+    if (threadIdx.x == 0 && step + kRpStages - 1 < steps) fetch(step + kRpStages - 1);
+    const T* from = stage + b * (kRpStageBytes / (int)sizeof(T)) + 2 * (32 * warp + lane);
+    if (count == kPairs && __all_sync(0xffffffffu, code == ((uint32_t)row1 | (uint32_t)row2 << 16))) {
+      float2 t[4];
+#pragma unroll
+      for (int k = 0; k < kPairs; ++k) {
+        const float2 v = load2(from + k * kRpChunk);
+        t[k & 3] = k < 4 ? v : make_float2(t[k & 3].x + v.x, t[k & 3].y + v.y);
+      }
+      const float x = (t[0].x + t[1].x) + (t[2].x + t[3].x), y = (t[0].y + t[1].y) + (t[2].y + t[3].y);
+      run1.x += x, run1.y += y, run2.x += x, run2.y += y;
+    } else {
+#pragma unroll 4
+      for (int k = 0; k < count; ++k) {
+        const uint32_t now = __shfl_sync(0xffffffffu, code, k);
+        const float2 v = load2(from + k * kRpChunk);
+        if ((int)(now & 0xffffu) != row1) {
+          flush(row1, run1);
+          row1 = (int)(now & 0xffffu);
+        }
+        if ((int)(now >> 16) != row2) {
+          flush(row2 >= 0 ? rows1 + row2 : -1, run2);
+          row2 = (int)(now >> 16);
+        }
+        run1.x += v.x, run1.y += v.y, run2.x += v.x, run2.y += v.y;
+      }
+    }
+  }
+  flush(row1, run1);
+  flush(row2 >= 0 ? rows1 + row2 : -1, run2);
+  __syncthreads();
+  // the columns of W: a table row counts for its position and its token column, a copy row for its own and, unless the entities differ, the entity's
+  const int t = a.columns(), tok = 2 * a.r + 2, ent = 4 * a.r + 4;
+  float* out = partial + ((long long)blockIdx.y * gridDim.x + blockIdx.x) * t * kRpChunk + 2 * (32 * warp + lane);
+  const auto range = [&](int from, int to) {
+    float2 v = make_float2(0.f, 0.f);
+    for (int k = from; k < to; ++k) {
+      const float2 m = mine[k * (kRpChunk / 2)];
+      v.x += m.x, v.y += m.y;
+    }
+    return v;
+  };
+  for (int k = 0; k < t; ++k) {
+    float2 v;
+    if (k < ent - 1) v = range(k, k + 1);
+    else if (k == ent - 1) v = range(0, tok);
+    else if (k == ent) v = range(rows1, rows1 + 2 * a.s + 1);
+    else v = range(rows1 + k - ent - 1, rows1 + k - ent);
+    if (k == a.r) {                                // pairs of one residue, whatever their tokens
+      const float2 m = range(tok, rows1);
+      v.x += m.x, v.y += m.y;
+    }
+    *reinterpret_cast<float2*>(out + (long long)k * kRpChunk) = v;
+  }
+}
+
+// dw[c][t] = the blocks' sums, in their order: eight slices of the blocks, each added up by one thread a channel, then the slices.
+__global__ void __launch_bounds__(8 * kRpChunk) relpos_reduce_kernel(const float* __restrict__ partial, float* __restrict__ dw, int blocks, int t,
+                                                                     int c) {
+  __shared__ float slice[8][kRpChunk];
+  const int k = blockIdx.x, chunk = blockIdx.y, ch = threadIdx.x % kRpChunk, s = threadIdx.x / kRpChunk;
+  const float* p = partial + ((long long)chunk * blocks * t + k) * kRpChunk + ch;
+  float v = 0.f;
+#pragma unroll 8
+  for (int b = s; b < blocks; b += 8) v += p[(long long)b * t * kRpChunk];
+  slice[s][ch] = v;
+  __syncthreads();
+  if (s == 0 && chunk * kRpChunk + ch < c) {
+    float sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum += slice[e][ch];
+    dw[(long long)(chunk * kRpChunk + ch) * t + k] = sum;
+  }
+}
+
+PX_DEFINE_FAMILY_HOOKS(relpos)
+
+static bool relpos_sizes(int64_t batch, int64_t n, int64_t c, int32_t r, int32_t s) {
+  return batch >= 0 && n >= 0 && c > 0 && r >= 0 && s >= 0 && n < (1 << 24) && batch < (1 << 24) && c < (1 << 16);
+}
+static bool relpos_fits(int64_t c, int32_t r, int32_t s) {
+  return c % 8 == 0 && r <= kRpMaxRows && s <= kRpMaxRows && 4 * r + 2 * s + 5 <= kRpMaxRows;
+}
+// Blocks of the backward pass: two an SM, and no more than leave each some hundreds of pairs, since each brings sums of its own.
+static int64_t relpos_blocks(int64_t pairs) { return std::max<int64_t>(1, std::min<int64_t>(2 * sm_count(), pairs / 256)); }
+
+}  // namespace px
+
+using namespace px;
+
+extern "C" int64_t px_relpos_workspace_bytes(int64_t batch, int64_t n, int64_t c, int32_t r_max, int32_t s_max) {
+  if (!relpos_sizes(batch, n, c, r_max, s_max) || !relpos_fits(c, r_max, s_max)) return 0;
+  return relpos_blocks(batch * n * n) * ((c + kRpChunk - 1) / kRpChunk) * (4 * r_max + 2 * s_max + 7) * kRpChunk * 4;
+}
+
+extern "C" int32_t px_relpos_fwd(const int64_t* asym_id, const int64_t* residue_index, const int64_t* entity_id, const int64_t* token_index,
+                                 const int64_t* sym_id, const float* w, void* z, int64_t batch, int64_t n, int64_t c, int32_t r_max,
+                                 int32_t s_max, int32_t dtype, void* stream) {
+  if (!relpos_sizes(batch, n, c, r_max, s_max)) return PX_ERR_BAD_ARG;
+  if (!relpos_fits(c, r_max, s_max) || (dtype != PX_F32 && dtype != PX_BF16 && dtype != PX_F16)) return PX_ERR_UNSUPPORTED;
+  if (batch == 0 || n == 0) return PX_OK;
+  if (!asym_id || !residue_index || !entity_id || !token_index || !sym_id || !w || !z || ((uintptr_t)z & 15)) return PX_ERR_BAD_ARG;
+  const RelposArgs a = {(const long long*)asym_id, (const long long*)residue_index, (const long long*)entity_id, (const long long*)token_index,
+                        (const long long*)sym_id, n, batch * n * n, (int)c, r_max, s_max};
+  const size_t smem = (size_t)(a.rows1() + a.rows2()) * kRpPitch * 4;
+  const int64_t strips = batch * n * ((n + kRpPairs - 1) / kRpPairs), per = kRpFwdThreads / 32;
+  const int64_t room = sm_count() * std::max<int64_t>(1, std::min<int64_t>(4, (int64_t)(227 << 10) / (int64_t)(smem + 1024)));
+  const dim3 grid((unsigned)std::min((strips + per - 1) / per, room), (unsigned)((c + kRpChunk - 1) / kRpChunk));
+  static SmemLimit limit[3];
+  const auto go = [&](auto* kernel, auto* out) {
+    if (!limit[dtype].set(kernel, (size_t)kRpMaxRows * kRpPitch * 4)) return false;
+    kernel<<<grid, kRpFwdThreads, smem, (cudaStream_t)stream>>>(a, w, out);
+    return cudaGetLastError() == cudaSuccess;
+  };
+  const bool done = dtype == PX_F32    ? go(relpos_fwd_kernel<float>, (float*)z)
+                    : dtype == PX_BF16 ? go(relpos_fwd_kernel<bf16>, (bf16*)z)
+                                       : go(relpos_fwd_kernel<__half>, (__half*)z);
+  return done ? PX_OK : PX_ERR_LAUNCH;
+}
+
+extern "C" int32_t px_relpos_bwd(const int64_t* asym_id, const int64_t* residue_index, const int64_t* entity_id, const int64_t* token_index,
+                                 const int64_t* sym_id, const void* dz, float* dw, void* workspace, int64_t workspace_bytes, int64_t batch,
+                                 int64_t n, int64_t c, int32_t r_max, int32_t s_max, int32_t dtype, void* stream) {
+  if (!relpos_sizes(batch, n, c, r_max, s_max)) return PX_ERR_BAD_ARG;
+  if (!relpos_fits(c, r_max, s_max) || (dtype != PX_F32 && dtype != PX_BF16 && dtype != PX_F16)) return PX_ERR_UNSUPPORTED;
+  if (!dw) return PX_ERR_BAD_ARG;
+  const cudaStream_t st = (cudaStream_t)stream;
+  const RelposArgs a = {(const long long*)asym_id, (const long long*)residue_index, (const long long*)entity_id, (const long long*)token_index,
+                        (const long long*)sym_id, n, batch * n * n, (int)c, r_max, s_max};
+  if (batch == 0 || n == 0)
+    return cudaMemsetAsync(dw, 0, (size_t)c * a.columns() * 4, st) == cudaSuccess ? PX_OK : PX_ERR_LAUNCH;
+  if (!asym_id || !residue_index || !entity_id || !token_index || !sym_id || !dz || !workspace || ((uintptr_t)dz & 15) ||
+      ((uintptr_t)workspace & 15))
+    return PX_ERR_BAD_ARG;
+  if (workspace_bytes < px_relpos_workspace_bytes(batch, n, c, r_max, s_max)) return PX_ERR_WORKSPACE;
+  const int64_t most = relpos_blocks(a.pairs), per = ((a.pairs + most - 1) / most + kRpPairs - 1) / kRpPairs * kRpPairs;
+  const int blocks = (int)((a.pairs + per - 1) / per);
+  const unsigned chunks = (unsigned)((c + kRpChunk - 1) / kRpChunk);
+  const size_t fixed = (size_t)kRpStages * kRpStageBytes, smem = fixed + (size_t)(a.rows1() + a.rows2()) * kRpChunk * 4;
+  static SmemLimit limit[3];
+  const auto go = [&](auto* kernel, auto* in) {
+    if (!limit[dtype].set(kernel, fixed + (size_t)kRpMaxRows * kRpChunk * 4)) return false;
+    kernel<<<dim3((unsigned)blocks, chunks), 64, smem, st>>>(a, in, (float*)workspace, per);
+    return cudaGetLastError() == cudaSuccess;
+  };
+  const bool done = dtype == PX_F32    ? go(relpos_bwd_kernel<float>, (const float*)dz)
+                    : dtype == PX_BF16 ? go(relpos_bwd_kernel<bf16>, (const bf16*)dz)
+                                       : go(relpos_bwd_kernel<__half>, (const __half*)dz);
+  if (!done) return PX_ERR_LAUNCH;
+  relpos_reduce_kernel<<<dim3((unsigned)a.columns(), chunks), 8 * kRpChunk, 0, st>>>((const float*)workspace, dw, blocks, a.columns(), (int)c);
+  return cudaGetLastError() == cudaSuccess ? PX_OK : PX_ERR_LAUNCH;
+}

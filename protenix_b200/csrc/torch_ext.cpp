@@ -18,6 +18,7 @@
 #include <ATen/ops/full.h>
 #include <ATen/ops/mm.h>
 #include <ATen/ops/ones.h>
+#include <ATen/ops/stack.h>
 #include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -58,7 +59,8 @@ constexpr int64_t kCz = 128, kCs = 384, kHeadsSingle = 16, kHeads = 4, kHeadDim 
   X(px_pair_bias_folded_bytes) X(px_pair_bias_fold) X(px_pair_bias_proj_folded) X(px_single_weights_bytes)               \
   X(px_single_workspace_bytes) X(px_single_prepare) X(px_single_project) X(px_single_finish) X(px_opm_outer)             \
   X(px_opm_out) X(px_msa_opm_prep) X(px_msa_values) X(px_msa_weights) X(px_msa_average) X(px_msa_gate_out)               \
-  X(px_msa_rows_weights_bytes) X(px_msa_rows_prepare) X(px_msa_transition_weights_bytes) X(px_msa_transition_prepare) X(px_msa_transition)
+  X(px_msa_rows_weights_bytes) X(px_msa_rows_prepare) X(px_msa_transition_weights_bytes) X(px_msa_transition_prepare) X(px_msa_transition) \
+  X(px_dropout_add) X(px_relpos_workspace_bytes) X(px_relpos_fwd) X(px_relpos_bwd)
 struct Abi {
 #define X(f) decltype(&::f) f = nullptr;
   PX_FUNCTIONS(X)
@@ -1004,12 +1006,16 @@ Tensor dropout_add(const Tensor& residual, const Tensor& x, double p) {
   return DropoutAddFunction::apply(residual, x, mask);
 }
 
+#include "torch_training.h"
+
 }  // namespace
 
 PYBIND11_MODULE(_C, m) {
   m.def("bind_library", &bind_library);
   m.def("layer_norm", &layer_norm);
   m.def("dropout_add", &dropout_add);
+  m.def("counter_dropout_add", &counter_dropout_add);
+  m.def("relative_position_encoding", &relative_position_encoding);
   py::class_<Params, std::shared_ptr<Params>>(m, "Params")
       .def(py::init<std::string, py::object, py::list, py::list, py::list>())
       .def("current", &Params::current)
