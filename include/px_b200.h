@@ -157,7 +157,8 @@ PX_API int32_t px_trimul_contract(const px_f16* a, const px_f16* b, px_f16* x, i
 #define PX_FAMILY_MSA_AVERAGE 14
 #define PX_FAMILY_MSA_ROWS 15
 #define PX_FAMILY_RELPOS 16
-#define PX_N_FAMILIES 17
+#define PX_FAMILY_WINDOW 17
+#define PX_N_FAMILIES 18
 PX_API int32_t px_device_error_flags(uint32_t* flags);
 PX_API int32_t px_device_error_detail(uint32_t* flags, uint32_t* detail);
 /* Limit of every bounded wait on the current device, in SM clock cycles (default 2^28, about 0.14 s); cycles <= 0
@@ -408,6 +409,36 @@ PX_API int32_t px_relpos_fwd(const int64_t* asym_id, const int64_t* residue_inde
 PX_API int32_t px_relpos_bwd(const int64_t* asym_id, const int64_t* residue_index, const int64_t* entity_id, const int64_t* token_index,
                       const int64_t* sym_id, const void* dz, float* dw, void* workspace, int64_t workspace_bytes, int64_t batch,
                       int64_t n, int64_t c, int32_t r_max, int32_t s_max, int32_t dtype, void* stream);
+
+/* ---- Attention with a sliding window (sequence-local attention; forward and backward) ---------
+ * o_i = sum over visible j of softmax_j(scale q_i . k_j + bias[head][clip(j - i, -r_max, r_max) + r_max]) v_j; key j is visible to query i when
+ * j <= i + right, j >= i - left or j < sinks, and mask[j] is not zero.  A query that sees nothing gives 0 and takes part in no gradient.
+ * Rows q, o [batch][heads][n][d], k, v [batch][kv_heads][n][d] with the strides of px_rows; query head h uses key head h / (heads /
+ * kv_heads).  PX_BF16 or PX_F16; d a multiple of 8 up to 128; products of 16-bit operands, everything else fp32.  What masked keys and
+ * queries that see nothing hold (NaN included) has no influence.  lse: px_window_lse_floats() floats that the backward pass reads, or NULL.
+ * px_window_bwd writes those of dq, dk, dv (types and shapes of q, k, v) and dbias (bias_dtype) that are not NULL; sums have a fixed
+ * order.  Workspace aligned to 256 bytes.  Stands in for the local attention of protenix/model/modules/primitives.py
+ * (n_queries / n_keys) where the window moves with the query, not with its block. */
+typedef struct {
+  void* data;
+  int64_t batch, head, row; /* strides in elements, multiples of 8; ignored for an axis of length one */
+} px_rows;
+typedef struct {
+  int64_t batch, heads, kv_heads, n, d;
+  int64_t left, right, sinks;
+  int64_t r_max;       /* clipping distance of the bias, at most 256; negative: no bias */
+  const void* bias;    /* [heads][2 r_max + 1] */
+  const uint8_t* mask; /* [batch][n], or NULL */
+  float scale;         /* positive and finite */
+  int32_t dtype, bias_dtype;
+} px_window;
+PX_API int64_t px_window_lse_floats(int64_t batch, int64_t heads, int64_t n);
+PX_API int32_t px_window_fwd(const px_window* w, const px_rows* q, const px_rows* k, const px_rows* v, const px_rows* o, float* lse,
+                      void* stream);
+PX_API int64_t px_window_workspace_bytes(const px_window* w, int32_t bias_grad);
+PX_API int32_t px_window_bwd(const px_window* w, const px_rows* q, const px_rows* k, const px_rows* v, const px_rows* o, const px_rows* dout,
+                      const float* lse, const px_rows* dq, const px_rows* dk, const px_rows* dv, void* dbias, void* workspace,
+                      int64_t workspace_bytes, void* stream);
 
 /* ---- Exchange between the GPUs of one box (row-sharded path) ------------------------------
  * No counterpart in the reference (which runs the Pairformer on one GPU).  A peer buffer is a

@@ -12,6 +12,7 @@ from .triangular import (OpenfoldLinear, TriangleAttention, TriangleAttentionEnd
                          TriangleAttentionStartingNode, TriangleMultiplicationIncoming,
                          TriangleMultiplicationOutgoing, TriangleMultiplicativeUpdate)
 from .fused_ops import dropout_add, dropout_add_rowwise
+from .window_attention import window_attention
 from .weights import weights_changed
 
 __all__ = [
@@ -20,5 +21,6 @@ __all__ = [
     "TriangleAttentionStartingNode", "TriangleMultiplicationIncoming", "TriangleMultiplicationOutgoing",
     "TriangleMultiplicativeUpdate", "dropout_add_rowwise", "RecyclingTrunk", "OuterProductMean",
     "weights_changed", "dropout_add", "RelativePositionEncoding", "relative_position_encoding",
+    "window_attention",
 ]
 __version__ = "0.1.0"

@@ -1,0 +1,153 @@
+// What the kernels of windowed attention share (window_attention.cu, px_window_bwd.cuh): the geometry of the window, the
+// tiles, the learned bias.
+#pragma once
+#include <math_constants.h>
+
+#include "px_tcgen05.cuh"
+
+namespace px {
+
+constexpr int kWRows = 128;      // rows a CTA owns: queries (forward, dQ) or keys (dK, dV)
+constexpr int kWCols = 64;       // keys or queries of a streamed tile
+constexpr int kWMaxR = 256;      // largest clipping distance of the learned bias
+
+// A call, as the kernels see it.  left, right and sinks are at most n.
+struct WindowArgs {
+  int n, d, heads, kv_heads, group, tiles;     // group: heads / kv_heads; tiles of kWRows rows
+  int left, right, sinks, r;                   // r < 0: no bias
+  int npad;                                    // row statistics are [batch * heads][npad]
+  float c;                                     // scale * log2(e)
+  const uint8_t* mask;                         // [batch][n] or NULL
+  const void* bias;                            // [heads][2 r + 1]
+  int bias_type;
+};
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z, int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];\n"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
+// A tile of `rows` rows as panels of 64 elements (128 bytes, 128-byte swizzle), one behind the other.  Elements beyond d and rows beyond n
+// arrive as zeros.
+template <int kPanels>
+__device__ __forceinline__ void load_rows(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int rows, int row0, int head, int batch) {
+#pragma unroll
+  for (int p = 0; p < kPanels; ++p) tma_load_4d(dst + p * rows * 128, map, bar, 64 * p, row0, head, batch);
+}
+
+// D[128][rows of B] = A B^T over d, both K-major panels of 64 (one lane).
+__device__ __forceinline__ void mma_rows(uint32_t d_tmem, uint32_t a, uint32_t b, int b_rows, int steps, uint32_t idesc) {
+  for (int ks = 0; ks < steps; ++ks) {
+    const uint32_t panel = ks >> 2, at = 2 * (ks & 3);
+    umma_bf16(d_tmem, umma_desc_sw128(a + panel * (kWRows * 128)) + at, umma_desc_sw128(b + panel * b_rows * 128) + at, idesc, ks > 0);
+  }
+}
+// D[128][d] += A[128][kWCols] B with A in tensor memory and B the streamed tile [kWCols][d], read along its rows (one lane).
+__device__ __forceinline__ void mma_streamed(uint32_t d_tmem, uint32_t a_tmem, uint32_t b, uint32_t idesc, bool first) {
+#pragma unroll
+  for (int ks = 0; ks < kWCols / 16; ++ks)
+    umma_bf16_ts(d_tmem, a_tmem + 8 * ks, umma_desc_mn_sw128(b + ks * 2048, kWCols * 128, 1024), idesc, !first || ks > 0);
+}
+
+// Streamed key tiles of the queries [q0, q0 + 128): the first tiles as far as they hold sinks, then those of the window.
+struct KeyTiles {
+  int sink, first, count;
+  __device__ __forceinline__ KeyTiles(const WindowArgs& a, int q0) {
+    const int lo = max(0, q0 - a.left), hi = min(a.n - 1, q0 + kWRows - 1 + a.right);
+    first = lo / kWCols;
+    sink = min((a.sinks + kWCols - 1) / kWCols, first);
+    count = sink + hi / kWCols - first + 1;
+  }
+  __device__ __forceinline__ int key(int t) const { return (t < sink ? t : first + t - sink) * kWCols; }
+};
+
+__device__ __forceinline__ uint64_t bits_between(int from, int to) {     // bits from .. to, both cut to 0 .. 63
+  from = max(from, 0), to = min(to, 63);
+  return from > to ? 0ull : (~0ull << from) & (~0ull >> (63 - to));
+}
+// Bit c: key k0 + c exists and is not masked (whole warp).
+__device__ __forceinline__ uint64_t key_bits(const WindowArgs& a, int batch, int k0, int lane) {
+  uint64_t w = bits_between(0, a.n - 1 - k0);
+  if (a.mask) {
+    const uint8_t* m = a.mask + (size_t)batch * a.n + k0;
+    const unsigned lo = __ballot_sync(0xffffffffu, k0 + lane < a.n && __ldg(m + min(lane, a.n - 1 - k0)) != 0);
+    const unsigned hi = __ballot_sync(0xffffffffu, k0 + 32 + lane < a.n && __ldg(m + min(32 + lane, a.n - 1 - k0)) != 0);
+    w = (uint64_t)hi << 32 | lo;
+  }
+  return w;
+}
+// Whether the queries [q0, q0 + 128) see all of the keys [k0, k0 + 64), as far as the window goes.
+__device__ __forceinline__ bool window_covers(const WindowArgs& a, int q0, int k0) {
+  return k0 + kWCols - 1 <= q0 + a.right && (k0 >= q0 + kWRows - 1 - a.left || k0 + kWCols <= a.sinks);
+}
+// Bit c: query i sees key k0 + c.
+__device__ __forceinline__ uint64_t visible_bits(const WindowArgs& a, int i, int k0, uint64_t keys) {
+  const int hi = i + a.right - k0;
+  return (bits_between(i - a.left - k0, hi) | bits_between(0, min(a.sinks - 1 - k0, hi))) & keys;
+}
+
+// The learned bias of one head times log2(e), by offset j - i and continued beyond +-r far enough that every offset of a tile that reaches into
+// (-r, r) has its place: at(offset) for |offset| < r + kWRows + kWCols.
+constexpr int kWBiasBeyond = kWRows + kWCols;
+__host__ __device__ constexpr int bias_floats(int r) { return r < 0 ? 0 : 2 * r + 1 + 2 * kWBiasBeyond; }
+__device__ __forceinline__ float bias_value(const WindowArgs& a, int head, int bucket) {
+  const size_t at = (size_t)head * (2 * a.r + 1) + bucket;
+  const float v = a.bias_type == PX_F32    ? __ldg((const float*)a.bias + at)
+                  : a.bias_type == PX_BF16 ? __bfloat162float(__ldg((const bf16*)a.bias + at))
+                                           : __half2float(__ldg((const __half*)a.bias + at));
+  return v * kLog2e;
+}
+__device__ __forceinline__ void bias_fill(const WindowArgs& a, int head, float* to) {
+  for (int k = threadIdx.x; k < bias_floats(a.r); k += blockDim.x) to[k] = bias_value(a, head, min(max(k - kWBiasBeyond, 0), 2 * a.r));
+}
+// Whether offsets lowest .. highest are all clipped, and to which side.
+__device__ __forceinline__ bool clipped_low(const WindowArgs& a, int highest) { return highest <= -a.r; }
+__device__ __forceinline__ bool clipped_high(const WindowArgs& a, int lowest) { return lowest >= a.r; }
+
+// Row `row` of a streamed tile in shared memory becomes zeros (its `half` of the 128 bytes of each panel).  What a product weights with zero must be
+// finite: masked keys and rows that see nothing may hold anything.
+template <int kPanels>
+__device__ __forceinline__ void clear_row(unsigned char* tile, int row, int part, int parts) {
+#pragma unroll
+  for (int p = 0; p < kPanels; ++p)
+    for (int k = part * (8 / parts); k < (part + 1) * (8 / parts); ++k)
+      *reinterpret_cast<uint4*>(tile + p * kWCols * 128 + row * 128 + k * 16) = make_uint4(0u, 0u, 0u, 0u);
+}
+// Barrier of `threads` threads that tells whether `ok` held for all: they leave a loop together after one of their waits ran out.
+__device__ __forceinline__ bool barrier_all(int id, int threads, bool ok) {
+  int all;
+  asm volatile("{\n .reg .pred p, q;\n setp.ne.b32 p, %1, 0;\n barrier.cta.red.and.pred q, %2, %3, p;\n selp.b32 %0, 1, 0, q;\n}\n"
+               : "=r"(all)
+               : "r"((int)ok), "r"(id), "r"(threads)
+               : "memory");
+  return all != 0;
+}
+__device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
+
+// 8 values of a row as 16 bytes.
+template <bool kF16>
+__device__ __forceinline__ void store8(void* to, const uint32_t* v, float scale) {
+  uint4 w;
+  uint32_t* o = reinterpret_cast<uint32_t*>(&w);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o[e] = pack16x2<kF16>(__uint_as_float(v[2 * e]) * scale, __uint_as_float(v[2 * e + 1]) * scale);
+  *reinterpret_cast<uint4*>(to) = w;
+}
+
+__device__ __forceinline__ void tmem_alloc(uint32_t* base, uint32_t cols) {      // whole warp
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(base)), "r"(cols) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+}
+__device__ __forceinline__ void tmem_free(uint32_t base, uint32_t cols) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(base), "r"(cols) : "memory");
+}
+
+// Rows of 16-bit values in global memory: strides in elements.
+struct RowsOut {
+  uint16_t* data;
+  long long batch, head, row;
+  __device__ __forceinline__ uint16_t* at(int b, int h, int i) const { return data + b * batch + h * head + i * row; }
+};
+
+}  // namespace px

@@ -116,12 +116,6 @@ __device__ __forceinline__ float2 load2<bf16>(const bf16* p) { return unpack_bf1
 template <>
 __device__ __forceinline__ float2 load2<__half>(const __half* p) { return unpack_f16x2(*reinterpret_cast<const uint32_t*>(p)); }
 
-__device__ __forceinline__ void bulk_load(void* to, const void* from, uint32_t bytes, uint64_t* bar) {      // multiples of 16 bytes
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(smem_u32(to)), "l"(from),
-               "r"(bytes), "r"(smem_u32(bar))
-               : "memory");
-}
-
 // Block b adds up the pairs [b * per, (b + 1) * per) of its channels; partial: [chunk][block][columns][kRpChunk].
 template <typename T>
 __global__ void __launch_bounds__(64) relpos_bwd_kernel(RelposArgs a, const T* __restrict__ dz, float* __restrict__ partial, long long per) {

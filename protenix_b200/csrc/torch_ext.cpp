@@ -10,6 +10,7 @@
 // px_b200.h, whose functions are taken from the library handle that the Python side has loaded.  Workspaces come from the
 // caching allocator on each call.
 #include <ATen/ATen.h>
+#include <ATen/ExpandUtils.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/CUDAEvent.h>
 #include <ATen/ops/dropout.h>
@@ -30,6 +31,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <mutex>
 #include <stdexcept>
 #include <string>
@@ -60,7 +62,8 @@ constexpr int64_t kCz = 128, kCs = 384, kHeadsSingle = 16, kHeads = 4, kHeadDim 
   X(px_single_workspace_bytes) X(px_single_prepare) X(px_single_project) X(px_single_finish) X(px_opm_outer)             \
   X(px_opm_out) X(px_msa_opm_prep) X(px_msa_values) X(px_msa_weights) X(px_msa_average) X(px_msa_gate_out)               \
   X(px_msa_rows_weights_bytes) X(px_msa_rows_prepare) X(px_msa_transition_weights_bytes) X(px_msa_transition_prepare) X(px_msa_transition) \
-  X(px_dropout_add) X(px_relpos_workspace_bytes) X(px_relpos_fwd) X(px_relpos_bwd)
+  X(px_dropout_add) X(px_relpos_workspace_bytes) X(px_relpos_fwd) X(px_relpos_bwd) X(px_window_lse_floats) \
+  X(px_window_fwd) X(px_window_workspace_bytes) X(px_window_bwd)
 struct Abi {
 #define X(f) decltype(&::f) f = nullptr;
   PX_FUNCTIONS(X)
@@ -1014,6 +1017,7 @@ PYBIND11_MODULE(_C, m) {
   m.def("bind_library", &bind_library);
   m.def("layer_norm", &layer_norm);
   m.def("dropout_add", &dropout_add);
+  m.def("window_attention", &window_attention);
   m.def("counter_dropout_add", &counter_dropout_add);
   m.def("relative_position_encoding", &relative_position_encoding);
   py::class_<Params, std::shared_ptr<Params>>(m, "Params")

@@ -1,4 +1,4 @@
-// The host path of the training operators: dropout-add from a counter-based generator, relative position encoding.
+// The host path of the training operators: dropout-add from a counter-based generator, relative position encoding, windowed attention.
 // Part of torch_ext.cpp (inside its unnamed namespace).  Each is an autograd function whose two directions are launches of the
 // C ABI.  Gradients are computed in kernels, so the ones that are not linear in what they differentiate have no second derivative: a
 // backward pass that is asked to build a graph is refused.
@@ -173,4 +173,140 @@ Tensor relative_position_encoding(const Tensor& weight, const std::vector<Tensor
   const Tensor z = at::GradMode::is_enabled() && weight.requires_grad() ? RelposFunction::apply(weight, ids, batch, n, r, s, type)
                                                                         : RelposFunction::run(weight, ids, {batch, n, weight.size(0), r, s, type});
   return z.view(shape);
+}
+
+// ---- attention with a sliding window ---------------------------------------------------------------------------------
+struct WindowCall {
+  int64_t left, right, sinks;
+  double scale;
+};
+
+// [B, H, N, D] as the kernels address it: rows of neighbouring elements, 16-byte aligned, positive strides that are multiples of 16 bytes.
+Tensor rows_fitted(const Tensor& t) {
+  bool fits = t.size(3) <= 1 || t.stride(3) == 1;
+  for (int i = 0; i < 3; ++i) fits = fits && (t.size(i) <= 1 || (t.stride(i) > 0 && t.stride(i) % 8 == 0));
+  if (fits && ((uintptr_t)t.data_ptr() & 15) == 0) return t;
+  const Tensor c = t.contiguous();
+  return ((uintptr_t)c.data_ptr() & 15) == 0 ? c : c.clone();
+}
+px_rows rows_of(const Tensor& t) { return {t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)}; }
+// A tensor of t's shape whose heads lie inside the rows where t's do, so that what follows (a projection of all heads) needs no copy.
+Tensor rows_like(const Tensor& t) {
+  const bool inside = t.size(1) > 1 && t.size(2) > 1 && t.stride(1) < t.stride(2);
+  return inside ? at::empty({t.size(0), t.size(2), t.size(1), t.size(3)}, t.options()).transpose(1, 2) : at::empty(t.sizes(), t.options());
+}
+px_window window_of(const Tensor& q, const Tensor& k, const Tensor& bias, const Tensor& mask, const WindowCall& c) {
+  px_window w = {};
+  w.batch = q.size(0), w.heads = q.size(1), w.kv_heads = k.size(1), w.n = q.size(2), w.d = q.size(3);
+  w.left = c.left, w.right = c.right, w.sinks = c.sinks;
+  w.r_max = bias.defined() ? (bias.size(1) - 1) / 2 : -1;
+  w.bias = bias.defined() ? bias.data_ptr() : nullptr;
+  w.bias_dtype = bias.defined() ? dtype_code(bias, "rel_bias") : PX_F32;
+  w.mask = mask.defined() ? (const uint8_t*)mask.data_ptr() : nullptr;
+  w.scale = (float)c.scale;
+  w.dtype = dtype_code(q, "q");
+  return w;
+}
+Tensor window_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& bias, const Tensor& mask, const WindowCall& c, Tensor* lse) {
+  const Tensor o = rows_like(q);
+  const px_window w = window_of(q, k, bias, mask, c);
+  if (lse) *lse = at::empty({abi.px_window_lse_floats(w.batch, w.heads, w.n)}, q.options().dtype(at::kFloat));
+  const px_rows rq = rows_of(q), rk = rows_of(k), rv = rows_of(v), ro = rows_of(o);
+  const cudaStream_t st = at::cuda::getCurrentCUDAStream();
+  launch("px_window_fwd", st, [&] { return abi.px_window_fwd(&w, &rq, &rk, &rv, &ro, lse ? (float*)lse->data_ptr() : nullptr, st); });
+  return o;
+}
+
+struct WindowFunction : torch::autograd::Function<WindowFunction> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& q_, const Tensor& k_, const Tensor& v_, const OptTensor& bias_,
+                        const OptTensor& mask_, int64_t left, int64_t right, int64_t sinks, double scale) {
+    c10::cuda::CUDAGuard guard(q_.device());
+    const Tensor q = rows_fitted(q_), k = rows_fitted(k_), v = rows_fitted(v_);
+    const Tensor bias = has(bias_) ? bias_->contiguous() : Tensor(), mask = has(mask_) ? *mask_ : Tensor();
+    Tensor lse;
+    const Tensor o = window_forward(q, k, v, bias, mask, {left, right, sinks, scale}, &lse);
+    ctx->save_for_backward({q, k, v, o, lse, bias, mask});
+    ctx->saved_data["window"] = c10::List<int64_t>({left, right, sinks});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["f"] = (int64_t)q_.requires_grad() | (int64_t)k_.requires_grad() << 1 | (int64_t)v_.requires_grad() << 2 |
+                           (int64_t)(has(bias_) && bias_->requires_grad()) << 3;
+    return o;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    first_derivative_only("window_attention");
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &o = saved[3], &lse = saved[4], &bias = saved[5], &mask = saved[6];
+    c10::cuda::CUDAGuard guard(q.device());
+    const auto at3 = ctx->saved_data["window"].toIntVector();
+    const int64_t f = ctx->saved_data["f"].toInt();
+    const px_window w = window_of(q, k, bias, mask, {at3[0], at3[1], at3[2], ctx->saved_data["scale"].toDouble()});
+    const Tensor dout = rows_fitted(grads[0]);
+    Tensor dq, dk, dv, dbias;
+    if (f & 1) dq = rows_like(q);
+    if (f & 2) dk = rows_like(k);
+    if (f & 4) dv = rows_like(v);
+    if (f & 8) dbias = at::empty_like(bias);
+    const int64_t bytes = abi.px_window_workspace_bytes(&w, f >> 3 & 1);
+    const Tensor ws = bytes_like(q, bytes);
+    const auto opt = [](const Tensor& t) { return t.defined() ? rows_of(t) : px_rows{}; };
+    const px_rows rq = rows_of(q), rk = rows_of(k), rv = rows_of(v), ro = rows_of(o), rg = rows_of(dout), gq = opt(dq), gk = opt(dk), gv = opt(dv);
+    const cudaStream_t st = at::cuda::getCurrentCUDAStream();
+    launch("px_window_bwd", st, [&] {
+      return abi.px_window_bwd(&w, &rq, &rk, &rv, &ro, &rg, (const float*)lse.data_ptr(), dq.defined() ? &gq : nullptr,
+                               dk.defined() ? &gk : nullptr, dv.defined() ? &gv : nullptr, dbias.defined() ? dbias.data_ptr() : nullptr,
+                               ws.data_ptr(), bytes, st);
+    });
+    return {dq, dk, dv, dbias, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Tensor window_attention(const Tensor& q, const Tensor& k, const Tensor& v, int64_t left, int64_t right, int64_t sinks, const OptTensor& bias,
+                        const OptTensor& mask, const c10::optional<double>& scale_) {
+  need_cuda(q, "q");
+  if (q.scalar_type() != at::kBFloat16 && q.scalar_type() != at::kHalf) fail("q, k and v must be bfloat16 or float16");
+  if (q.dim() < 3) fail("q must be [..., H, N, D], got " + shape_of(q));
+  const int64_t h = q.size(-3), n = q.size(-2), d = q.size(-1);
+  for (const auto& [t, name] : {std::pair<const Tensor&, const char*>(k, "k"), std::pair<const Tensor&, const char*>(v, "v")}) {
+    need_on(t, q.device(), name);
+    if (t.scalar_type() != q.scalar_type()) fail(std::string(name) + " must have the type of q");
+    if (t.dim() != q.dim() || t.sizes() != k.sizes() || t.size(-2) != n || t.size(-1) != d || t.size(-3) < 1 || h % t.size(-3) != 0 ||
+        !t.sizes().slice(0, t.dim() - 3).equals(q.sizes().slice(0, q.dim() - 3)))
+      fail("k and v must be [..., H_kv, N, D] with the batch axes, N and D of q and H_kv a divisor of H; got " + shape_of(q) + ", " +
+           shape_of(k) + " and " + shape_of(v));
+  }
+  if (h < 1 || d < 8 || d > 128 || d % 8 != 0) fail("the kernels handle head sizes of 8 to 128 in steps of 8, got " + shape_of(q));
+  if (n > (1 << 24)) fail("at most 2^24 rows");
+  if (left < 0 || right < 0 || sinks < 0) fail("window and sinks must not be negative");
+  const double scale = scale_.has_value() ? *scale_ : 1.0 / std::sqrt((double)d);
+  if (!(scale > 0.0) || !((float)scale > 0.f) || !((float)scale <= 3.0e38f)) fail("scale must be positive and finite");
+  int64_t batch = 1;
+  for (int64_t i = 0; i < q.dim() - 3; ++i) batch *= q.size(i);
+  if (batch > 65535 || h > 65535) fail("at most 65535 samples and heads");
+  if (has(bias)) {
+    need_on(*bias, q.device(), "rel_bias");
+    if (bias->dim() != 2 || bias->size(0) != h || bias->size(1) % 2 != 1 || bias->size(1) > 513)
+      fail("rel_bias must be [H, 2 r + 1] with r at most 256, got " + shape_of(*bias));
+    if (bias->scalar_type() != at::kFloat && bias->scalar_type() != q.scalar_type()) fail("rel_bias must be float32 or of the type of q");
+  }
+  c10::cuda::CUDAGuard guard(q.device());
+  OptTensor m;
+  if (has(mask)) {
+    need_on(*mask, q.device(), "mask");
+    auto want = q.sizes().slice(0, q.dim() - 3).vec();
+    want.push_back(n);
+    if (mask->dim() < 1 || !at::is_expandable_to(mask->sizes(), want)) fail("mask must be [..., N] over the batch axes of q, got " + shape_of(*mask));
+    const Tensor truth = mask->scalar_type() == at::kBool ? mask->detach() : mask->detach().ne(0);
+    m = truth.expand(want).reshape({batch, n}).contiguous();
+  }
+  const auto four = [&](const Tensor& t) { return t.reshape({batch, t.size(-3), n, d}); };
+  const Tensor q4 = four(q), k4 = four(k), v4 = four(v);
+  const auto wants = [](const Tensor& t) { return t.requires_grad(); };
+  Tensor o;
+  if (at::GradMode::is_enabled() && (wants(q) || wants(k) || wants(v) || (has(bias) && wants(*bias)))) {
+    o = WindowFunction::apply(q4, k4, v4, bias, m, left, right, sinks, scale);
+  } else {
+    const Tensor b = has(bias) ? bias->contiguous() : Tensor();
+    o = window_forward(rows_fitted(q4), rows_fitted(k4), rows_fitted(v4), b, m.has_value() ? *m : Tensor(), {left, right, sinks, scale}, nullptr);
+  }
+  return o.reshape(q.sizes());
 }
