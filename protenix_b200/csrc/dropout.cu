@@ -18,16 +18,26 @@
 
 namespace px {
 
-__device__ __forceinline__ void philox4x32(uint32_t (&c)[4], uint32_t k0, uint32_t k1) {
+// The keys of the ten rounds: made once a thread (made anew with every block of four they were a tenth of the kernel's instructions).
+struct RoundKeys {
+  uint32_t a[10], b[10];
+  __device__ __forceinline__ explicit RoundKeys(unsigned long long seed) {
+#pragma unroll
+    for (int r = 0; r < 10; ++r) {
+      a[r] = (uint32_t)seed + r * 0x9E3779B9u;
+      b[r] = (uint32_t)(seed >> 32) + r * 0xBB67AE85u;
+      asm volatile("" : "+r"(a[r]), "+r"(b[r]));      // values, no longer sums that the compiler would rather form again
+    }
+  }
+};
+__device__ __forceinline__ void philox4x32(uint32_t (&c)[4], const RoundKeys& k) {
 #pragma unroll
   for (int r = 0; r < 10; ++r) {
     const uint64_t a = (uint64_t)0xD2511F53u * c[0], b = (uint64_t)0xCD9E8D57u * c[2];
-    c[0] = (uint32_t)(b >> 32) ^ c[1] ^ k0;
+    c[0] = (uint32_t)(b >> 32) ^ c[1] ^ k.a[r];
     c[1] = (uint32_t)b;
-    c[2] = (uint32_t)(a >> 32) ^ c[3] ^ k1;
+    c[2] = (uint32_t)(a >> 32) ^ c[3] ^ k.b[r];
     c[3] = (uint32_t)a;
-    k0 += 0x9E3779B9u;
-    k1 += 0xBB67AE85u;
   }
 }
 
@@ -58,24 +68,22 @@ struct DropoutArgs {
   long long* used;                     // receives the pair that the call used, or NULL
 };
 
-// Bit e: whether element at + e is kept.  `at` is a multiple of four unless VEC is 1.
+// Whether the elements at, at + 1, ... are kept.  `at` is a multiple of four unless VEC is 1.
 template <int VEC>
-__device__ __forceinline__ uint32_t kept(const DropoutArgs& a, unsigned long long seed, unsigned long long offset, long long at) {
-  uint32_t bits = 0;
+__device__ __forceinline__ void kept(const DropoutArgs& a, const RoundKeys& keys, unsigned long long offset, long long at, bool (&keep)[VEC]) {
 #pragma unroll
   for (int q = 0; q < (VEC + 3) / 4; ++q) {
     const unsigned long long block = ((unsigned long long)at >> 2) + q;
     uint32_t c[4] = {(uint32_t)block, (uint32_t)(block >> 32), (uint32_t)offset, (uint32_t)(offset >> 32)};
-    philox4x32(c, (uint32_t)seed, (uint32_t)(seed >> 32));
-    if (VEC == 1) {
+    philox4x32(c, keys);
+    if constexpr (VEC == 1) {
       const int w = (int)(at & 3);
-      bits = (w < 2 ? (w ? c[1] : c[0]) : (w == 2 ? c[2] : c[3])) >= a.threshold;
+      keep[0] = (w < 2 ? (w ? c[1] : c[0]) : (w == 2 ? c[2] : c[3])) >= a.threshold && !a.none;
     } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) bits |= (c[e] >= a.threshold ? 1u : 0u) << (4 * q + e);
+      for (int e = 0; e < 4; ++e) keep[4 * q + e] = c[e] >= a.threshold && !a.none;
     }
   }
-  return a.none ? 0u : bits;
 }
 
 template <typename T, int VEC>
@@ -83,15 +91,27 @@ struct alignas(sizeof(T) * VEC) Pack {
   T v[VEC];
 };
 
-template <typename T, int VEC>
-__device__ __forceinline__ Pack<T, VEC> dropped(const Pack<T, VEC>& x, const Pack<T, VEC>* r, uint32_t bits, float scale) {
+template <typename T>
+__device__ __forceinline__ void round_pair(T* to, float a, float b);
+template <>
+__device__ __forceinline__ void round_pair<float>(float* to, float a, float b) { to[0] = a, to[1] = b; }
+template <>
+__device__ __forceinline__ void round_pair<bf16>(bf16* to, float a, float b) { *reinterpret_cast<__nv_bfloat162*>(to) = __floats2bfloat162_rn(a, b); }
+template <>
+__device__ __forceinline__ void round_pair<__half>(__half* to, float a, float b) { *reinterpret_cast<__half2*>(to) = __floats2half2_rn(a, b); }
+
+// A kept element's product and sum are fp32 and round once; a dropped one leaves the residual as it is.
+template <typename T, int VEC, bool kResidual>
+__device__ __forceinline__ Pack<T, VEC> dropped(const Pack<T, VEC>& x, const Pack<T, VEC>& r, const bool (&keep)[VEC], float scale) {
   Pack<T, VEC> o;
+  float v[VEC];
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) {
-    const bool keep = bits >> e & 1;
-    // a kept element's product and sum round once, in the store; a dropped one leaves the residual as it is
-    o.v[e] = r ? (keep ? from_f32<T>(fmaf(to_f32(x.v[e]), scale, to_f32(r->v[e]))) : r->v[e])
-               : (keep ? from_f32<T>(to_f32(x.v[e]) * scale) : from_f32<T>(0.f));
+  for (int e = 0; e < VEC; ++e) v[e] = fmaf(keep[e] ? to_f32(x.v[e]) : 0.f, scale, kResidual ? to_f32(r.v[e]) : 0.f);
+  if constexpr (VEC == 1) {
+    o.v[0] = from_f32<T>(v[0]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < VEC; e += 2) round_pair(o.v + e, v[e], v[e + 1]);
   }
   return o;
 }
@@ -106,28 +126,34 @@ __global__ void __launch_bounds__(256) dropout_kernel(const T* residual, const T
     a.used[0] = (long long)seed;
     a.used[1] = (long long)offset;
   }
+  const RoundKeys keys(seed);
   const long long step = (long long)gridDim.x * blockDim.x * VEC, total = a.inner;
   for (long long i = ((long long)blockIdx.x * blockDim.x + threadIdx.x) * VEC; i < total; i += step) {
     if (i + VEC <= total) {
       const V xv = *reinterpret_cast<const V*>(x + i);
-      V rv;
+      V rv = xv;
       if (kResidual) rv = *reinterpret_cast<const V*>(residual + i);
-      *reinterpret_cast<V*>(out + i) = dropped<T, VEC>(xv, kResidual ? &rv : nullptr, kept<VEC>(a, seed, offset, i), a.scale);
+      bool keep[VEC];
+      kept<VEC>(a, keys, offset, i, keep);
+      *reinterpret_cast<V*>(out + i) = dropped<T, VEC, kResidual>(xv, rv, keep, a.scale);
     } else {
       for (long long e = i; e < total; ++e) {
         const Pack<T, 1> x1 = {{x[e]}};
         Pack<T, 1> r1 = x1;
         if (kResidual) r1.v[0] = residual[e];
-        out[e] = dropped<T, 1>(x1, kResidual ? &r1 : nullptr, kept<1>(a, seed, offset, e), a.scale).v[0];
+        bool keep[1];
+        kept<1>(a, keys, offset, e, keep);
+        out[e] = dropped<T, 1, kResidual>(x1, r1, keep, a.scale).v[0];
       }
     }
   }
 }
 
-// Shared along the middle axis: thread = 16 bytes of a row (o, i) and `rows` of the shared axis.
+constexpr int kSharedRows = 4;      // of the shared axis, a thread: what the generator costs is spread over them
+
+// Shared along the middle axis: thread = 16 bytes of a row (o, i) and up to kSharedRows of the shared axis, all requested before the mask is made.
 template <typename T, int VEC, bool kResidual>
-__global__ void __launch_bounds__(256) dropout_shared_kernel(const T* residual, const T* x, T* out, DropoutArgs a, long long rows,
-                                                             long long units) {
+__global__ void __launch_bounds__(256) dropout_shared_kernel(const T* residual, const T* x, T* out, DropoutArgs a, long long units) {
   typedef Pack<T, VEC> V;
   const unsigned long long seed = a.state ? (unsigned long long)a.state[0] : a.seed;
   const unsigned long long offset = a.state ? (unsigned long long)a.state[1] : a.offset;
@@ -135,21 +161,26 @@ __global__ void __launch_bounds__(256) dropout_shared_kernel(const T* residual, 
     a.used[0] = (long long)seed;
     a.used[1] = (long long)offset;
   }
+  const RoundKeys keys(seed);
   const long long vectors = a.outer * a.inner / VEC;       // of the mask
   for (long long u = (long long)blockIdx.x * blockDim.x + threadIdx.x; u < units; u += (long long)gridDim.x * blockDim.x) {
-    const long long m = u % vectors * VEC, s0 = u / vectors * rows;
+    const long long m = u % vectors * VEC, s0 = u / vectors * kSharedRows;
     const long long o = m / a.inner, i = m - o * a.inner;  // VEC divides inner: a vector never leaves its row
-    const uint32_t bits = kept<VEC>(a, seed, offset, m);
-    const int count = (int)(a.shared - s0 < rows ? a.shared - s0 : rows);
+    const int count = (int)(a.shared - s0 < kSharedRows ? a.shared - s0 : kSharedRows);
     const long long at = (o * a.shared + s0) * a.inner + i;
-#pragma unroll 4
-    for (int s = 0; s < count; ++s) {
-      const long long e = at + s * a.inner;
-      const V xv = *reinterpret_cast<const V*>(x + e);
-      V rv;
-      if (kResidual) rv = *reinterpret_cast<const V*>(residual + e);
-      *reinterpret_cast<V*>(out + e) = dropped<T, VEC>(xv, kResidual ? &rv : nullptr, bits, a.scale);
+    V xv[kSharedRows], rv[kSharedRows];
+#pragma unroll
+    for (int s = 0; s < kSharedRows; ++s) {
+      if (s < count) {
+        xv[s] = *reinterpret_cast<const V*>(x + at + s * a.inner);
+        rv[s] = kResidual ? *reinterpret_cast<const V*>(residual + at + s * a.inner) : xv[s];
+      }
     }
+    bool keep[VEC];
+    kept<VEC>(a, keys, offset, m, keep);
+#pragma unroll
+    for (int s = 0; s < kSharedRows; ++s)
+      if (s < count) *reinterpret_cast<V*>(out + at + s * a.inner) = dropped<T, VEC, kResidual>(xv[s], rv[s], keep, a.scale);
   }
 }
 
@@ -160,12 +191,9 @@ static cudaError_t launch_dropout_as(const void* residual, const void* x, void* 
     const int64_t blocks = std::min<int64_t>((a.inner / VEC + 1 + 255) / 256, most);
     dropout_kernel<T, VEC, kResidual><<<(unsigned)blocks, 256, 0, st>>>((const T*)residual, (const T*)x, (T*)out, a);
   } else {
-    // rows of the shared axis a thread: enough for the generator's work not to count, unless that leaves SMs idle
-    const int64_t vectors = a.outer * a.inner / VEC, fill = (int64_t)sm_count() * 2048;
-    const int64_t rows = std::max<int64_t>(1, std::min<int64_t>(16, vectors * a.shared / fill));
-    const int64_t units = vectors * ((a.shared + rows - 1) / rows);
+    const int64_t units = a.outer * a.inner / VEC * ((a.shared + kSharedRows - 1) / kSharedRows);
     const int64_t blocks = std::min<int64_t>((units + 255) / 256, most);
-    dropout_shared_kernel<T, VEC, kResidual><<<(unsigned)blocks, 256, 0, st>>>((const T*)residual, (const T*)x, (T*)out, a, rows, units);
+    dropout_shared_kernel<T, VEC, kResidual><<<(unsigned)blocks, 256, 0, st>>>((const T*)residual, (const T*)x, (T*)out, a, units);
   }
   return cudaGetLastError();
 }

@@ -12,10 +12,10 @@
 // writes pair after pair, 4 channels a lane, and looks the rows up again only where they change (most neighbours are far apart or in
 // another chain: clipped alike).
 //
-// Backward: memory-bound reader.  A block of two warps (64 channels each, two a lane) reads a run of pairs through a ring of bulk copies and
-// holds sums of its own for every table row in shared memory, so there are no atomics and a call gives the same bits every time.  A lane adds up neighbours with
-// the same rows in registers and goes to the shared sums only where they change.  The blocks' sums, folded to the columns of W, are
-// added up in their order by a second kernel.
+// Backward: memory-bound reader.  A block (a thread = one channel) reads strips of 32 pairs of a row through a ring of bulk copies and holds
+// sums of its own for every table row in shared memory, so there are no atomics and a call gives the same bits every time.  Neighbours with
+// the same rows are added up in registers; neighbours whose rows all differ, as near the diagonal, go to their sums eight at a time; the rest one by one.
+// The blocks' sums, folded to the columns of W, are added up in their order by a second kernel.
 #include "px_tcgen05.cuh"
 
 namespace px {
@@ -72,14 +72,23 @@ __global__ void __launch_bounds__(kRpFwdThreads) relpos_fwd_kernel(RelposArgs a,
   const int c0 = blockIdx.y * kRpChunk, channels = min(kRpChunk, a.c - c0), t = a.columns();
   const int rows1 = a.rows1(), rows2 = a.rows2(), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int pos = 0, tok = 2 * a.r + 2, ent = 4 * a.r + 4, chain = ent + 1;      // first columns of the four parts of W
-  for (int ch = warp; ch < channels; ch += kRpFwdThreads / 32) {
-    const float* row = w + (long long)(c0 + ch) * t;
-    for (int k = lane; k < rows1 + rows2; k += 32) {
-      float v;
-      if (k < tok) v = row[pos + k] + row[tok + 2 * a.r + 1];
-      else if (k < rows1) v = row[pos + a.r] + row[tok + k - tok];
-      else v = row[chain + k - rows1] + (k - rows1 < 2 * a.s + 1 ? row[ent] : 0.f);
-      rp_table[k * kRpPitch + ch] = v;
+  // A lane has one table row of eight channels at a time: sixteen loads in flight (one channel after the other took 15 us).
+  constexpr int kWarps = kRpFwdThreads / 32;
+  for (int k = lane; k < rows1 + rows2; k += 32) {
+    const int first = k < tok ? pos + k : k < rows1 ? pos + a.r : chain + k - rows1;
+    const int second = k < tok ? tok + 2 * a.r + 1 : k < rows1 ? k : k - rows1 < 2 * a.s + 1 ? ent : -1;
+#pragma unroll 1
+    for (int ch0 = warp; ch0 < channels; ch0 += 8 * kWarps) {
+      float u[8], v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int ch = min(ch0 + e * kWarps, channels - 1);
+        u[e] = __ldg(w + (long long)(c0 + ch) * t + first);
+        v[e] = __ldg(w + (long long)(c0 + ch) * t + max(second, 0));
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (ch0 + e * kWarps < channels) rp_table[k * kRpPitch + ch0 + e * kWarps] = u[e] + (second < 0 ? 0.f : v[e]);
     }
   }
   __syncthreads();
@@ -108,123 +117,174 @@ __global__ void __launch_bounds__(kRpFwdThreads) relpos_fwd_kernel(RelposArgs a,
 }
 
 template <typename T>
-__device__ __forceinline__ float2 load2(const T* p);
+__device__ __forceinline__ float load1(const T* p);
 template <>
-__device__ __forceinline__ float2 load2<float>(const float* p) { return *reinterpret_cast<const float2*>(p); }
+__device__ __forceinline__ float load1<float>(const float* p) { return *p; }
 template <>
-__device__ __forceinline__ float2 load2<bf16>(const bf16* p) { return unpack_bf16x2(*reinterpret_cast<const uint32_t*>(p)); }
+__device__ __forceinline__ float load1<bf16>(const bf16* p) { return __bfloat162float(*p); }
 template <>
-__device__ __forceinline__ float2 load2<__half>(const __half* p) { return unpack_f16x2(*reinterpret_cast<const uint32_t*>(p)); }
+__device__ __forceinline__ float load1<__half>(const __half* p) { return __half2float(*p); }
 
-// Block b adds up the pairs [b * per, (b + 1) * per) of its channels; partial: [chunk][block][columns][kRpChunk].
+constexpr int kRpBwdThreads = kRpChunk;      // a thread = one channel
+
+// Block b adds up the units [b * per, (b + 1) * per) of its channels; a unit is a row's strip of 32 pairs.  partial: [chunk][block][columns][kRpChunk].
 template <typename T>
-__global__ void __launch_bounds__(64) relpos_bwd_kernel(RelposArgs a, const T* __restrict__ dz, float* __restrict__ partial, long long per) {
+__global__ void __launch_bounds__(kRpBwdThreads) relpos_bwd_kernel(RelposArgs a, const T* __restrict__ dz, float* __restrict__ partial, int per) {
   constexpr int kPairs = kRpStageBytes / (kRpChunk * (int)sizeof(T));      // of a stage: 16 (fp32) or 32
+  constexpr int kParts = kRpPairs / kPairs;                                // stages of a unit
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   __shared__ uint64_t full[kRpStages];
   T* stage = reinterpret_cast<T*>(smem_raw);
-  float* sums = reinterpret_cast<float*>(smem_raw + kRpStages * kRpStageBytes);
-  const int c0 = blockIdx.y * kRpChunk, channels = min(kRpChunk, a.c - c0), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int rows1 = a.rows1(), rows = rows1 + a.rows2();
-  const long long begin = (long long)blockIdx.x * per, end = min(begin + per, a.pairs);
-  const int steps = (int)((end - begin + kPairs - 1) / kPairs);
+  float* const mine = reinterpret_cast<float*>(smem_raw + kRpStages * kRpStageBytes) + threadIdx.x;      // row k: mine[k * kRpChunk]
+  const int c0 = blockIdx.y * kRpChunk, channels = min(kRpChunk, a.c - c0), lane = threadIdx.x & 31;
+  const int rows1 = a.rows1(), rows = rows1 + a.rows2(), n = (int)a.n;
+  const int strips = (n + kRpPairs - 1) / kRpPairs;
+  const long long units = a.pairs / a.n * strips, begin = (long long)blockIdx.x * per;
+  const int steps = (int)(min(begin + per, units) - begin) * kParts;
   if (threadIdx.x == 0) {
     for (int k = 0; k < kRpStages; ++k) mbar_init(&full[k], 1);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
-  // the parts of a stage that no copy reaches (channels and pairs beyond the last) are added up as zeros
-  for (int k = threadIdx.x; k < kRpStages * kRpStageBytes / 16; k += 64) reinterpret_cast<uint4*>(smem_raw)[k] = make_uint4(0u, 0u, 0u, 0u);
-  for (int k = threadIdx.x; k < rows * kRpChunk / 4; k += 64) reinterpret_cast<float4*>(sums)[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-  asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+  // the parts of a stage that no copy reaches (channels beyond the last) are added up as zeros
+  if (channels < kRpChunk) {
+    for (int k = threadIdx.x; k < kRpStages * kRpStageBytes / 16; k += kRpBwdThreads)
+      reinterpret_cast<uint4*>(smem_raw)[k] = make_uint4(0u, 0u, 0u, 0u);
+    asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+  }
+  for (int k = 0; k < rows; ++k) mine[k * kRpChunk] = 0.f;
   __syncthreads();
-  const auto fetch = [&](int step) {              // one thread
-    const long long p0 = begin + (long long)step * kPairs;
-    const int count = (int)min((long long)kPairs, end - p0), b = step % kRpStages;
+  // Where a unit lies: its row of all batches, its first column; both kept up by additions.
+  struct Place {
+    long long i;
+    int strip;
+    __device__ __forceinline__ void next(int strips) {
+      if (++strip == strips) strip = 0, ++i;
+    }
+  };
+  const auto pairs_of = [&](const Place& p, int part) { return min(max(n - p.strip * kRpPairs - part * kPairs, 0), kPairs); };
+  const auto fetch = [&](const Place& p, int step) {              // one thread
+    const int part = step % kParts, count = pairs_of(p, part), b = step % kRpStages;
     const uint32_t bytes = (uint32_t)(channels * sizeof(T));
-    T* to = stage + b * (kRpStageBytes / (int)sizeof(T));
+    T* const to = stage + b * (kRpStageBytes / (int)sizeof(T));
+    const T* const from = dz + (p.i * n + p.strip * kRpPairs + part * kPairs) * a.c + c0;
     mbar_expect_tx(&full[b], bytes * count);
     if (a.c == kRpChunk) {
-      bulk_load(to, dz + p0 * a.c, bytes * count, &full[b]);
+      if (count > 0) bulk_load(to, from, bytes * count, &full[b]);
     } else {
-      for (int k = 0; k < count; ++k) bulk_load(to + k * kRpChunk, dz + (p0 + k) * a.c + c0, bytes, &full[b]);
+      for (int k = 0; k < count; ++k) bulk_load(to + k * kRpChunk, from + (long long)k * a.c, bytes, &full[b]);
     }
   };
-  if (threadIdx.x == 0)
-    for (int k = 0; k < kRpStages - 1 && k < steps; ++k) fetch(k);
-  float2* const mine = reinterpret_cast<float2*>(sums) + 32 * warp + lane;       // row k: mine[k * kRpChunk / 2]
+  Place here = {begin / strips, (int)(begin % strips)}, ahead = here;
+  if (threadIdx.x == 0) {
+    for (int k = 0; k < kRpStages - 1 && k < steps; ++k) {
+      fetch(ahead, k);
+      if ((k + 1) % kParts == 0) ahead.next(strips);
+    }
+  }
   int row1 = -1, row2 = -1;                        // what the running sums belong to
-  float2 run1 = make_float2(0.f, 0.f), run2 = run1;
-  const auto flush = [&](int row, float2& run) {
-    if (row >= 0) {
-      float2* const p = mine + row * (kRpChunk / 2);
-      const float2 v = *p;
-      *p = make_float2(v.x + run.x, v.y + run.y);
-    }
-    run = make_float2(0.f, 0.f);
+  float run1 = 0.f, run2 = 0.f;
+  const auto flush = [&](int row, float& run) {
+    if (row >= 0) mine[row * kRpChunk] += run;
+    run = 0.f;
   };
+  uint32_t code = 0;
   bool ok = true;
   for (int step = 0; step < steps; ++step) {
-    const long long p0 = begin + (long long)step * kPairs;
-    const int count = (int)min((long long)kPairs, end - p0), b = step % kRpStages;
-    const long long p = p0 + min(lane, count - 1), i = p / a.n;
-    const uint32_t code = relpos_code(a, i, i / a.n * a.n + (p - i * a.n));
+    const int part = step % kParts, count = pairs_of(here, part), b = step % kRpStages;
+    if (part == 0) code = relpos_code(a, here.i, here.i / n * n + min(here.strip * kRpPairs + lane, n - 1));
     ok = mbar_wait_warp(&full[b], (step / kRpStages) & 1, 1u);
-    ok = __syncthreads_and(ok) != 0;               // both warps are through with the stage that is filled next
+    ok = __syncthreads_and(ok) != 0;               // all are through with the stage that is filled next
     if (!ok) break;
-    if (threadIdx.x == 0 && step + kRpStages - 1 < steps) fetch(step + kRpStages - 1);
-    const T* from = stage + b * (kRpStageBytes / (int)sizeof(T)) + 2 * (32 * warp + lane);
-    if (count == kPairs && __all_sync(0xffffffffu, code == ((uint32_t)row1 | (uint32_t)row2 << 16))) {
-      float2 t[4];
+    if (threadIdx.x == 0 && step + kRpStages - 1 < steps) {
+      fetch(ahead, step + kRpStages - 1);
+      if ((step + kRpStages) % kParts == 0) ahead.next(strips);
+    }
+    const T* const from = stage + b * (kRpStageBytes / (int)sizeof(T)) + threadIdx.x;
+    const int l0 = part * kPairs;                  // the lane that has the code of the stage's first pair
+    const uint32_t first = code & 0xffffu, second = code >> 16;
+    // neighbours with one row each, neighbours with rows that all differ, and both for the second table: bits by lane
+    const uint32_t same1 = __ballot_sync(0xffffffffu, first == (uint32_t)row1), same2 = __ballot_sync(0xffffffffu, second == (uint32_t)row2);
+    const uint32_t all = kPairs == 32 ? 0xffffffffu : 0xffffu << l0;
+    if (count == kPairs && (same1 & same2 & all) == all) {
+      float t[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int k = 0; k < kPairs; ++k) {
-        const float2 v = load2(from + k * kRpChunk);
-        t[k & 3] = k < 4 ? v : make_float2(t[k & 3].x + v.x, t[k & 3].y + v.y);
-      }
-      const float x = (t[0].x + t[1].x) + (t[2].x + t[3].x), y = (t[0].y + t[1].y) + (t[2].y + t[3].y);
-      run1.x += x, run1.y += y, run2.x += x, run2.y += y;
+      for (int k = 0; k < kPairs; ++k) t[k & 3] += load1(from + k * kRpChunk);
+      const float sum = (t[0] + t[1]) + (t[2] + t[3]);
+      run1 += sum, run2 += sum;
     } else {
-#pragma unroll 4
-      for (int k = 0; k < count; ++k) {
-        const uint32_t now = __shfl_sync(0xffffffffu, code, k);
-        const float2 v = load2(from + k * kRpChunk);
-        if ((int)(now & 0xffffu) != row1) {
+      const uint32_t like = __match_any_sync(0xffffffffu, first) & (0xffu << (lane & 24));      // in this lane's group of eight
+      const uint32_t distinct = __ballot_sync(0xffffffffu, like == 1u << lane);
+      for (int g = 0; g < count; g += 8) {
+        const uint32_t group = 0xffu << (l0 + g);
+        const uint32_t lead = __shfl_sync(0xffffffffu, code, l0 + g);
+        if (g + 8 <= count && (distinct & group) == group) {
+          // eight rows of the first table, side by side: their sums have no order among them
+          float v[8], sum[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) v[k] = load1(from + (g + k) * kRpChunk);
           flush(row1, run1);
-          row1 = (int)(now & 0xffffu);
+          row1 = -1;
+          float* at[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) at[k] = mine + __shfl_sync(0xffffffffu, first, l0 + g + k) * kRpChunk;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) sum[k] = *at[k] + v[k];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) *at[k] = sum[k];
+          if (__all_sync(0xffffffffu, second == lead >> 16 || (group >> lane & 1) == 0)) {
+            if ((int)(lead >> 16) != row2) {
+              flush(row2 >= 0 ? rows1 + row2 : -1, run2);
+              row2 = (int)(lead >> 16);
+            }
+            run2 += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+          } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const int now = (int)__shfl_sync(0xffffffffu, second, l0 + g + k);
+              if (now != row2) {
+                flush(row2 >= 0 ? rows1 + row2 : -1, run2);
+                row2 = now;
+              }
+              run2 += v[k];
+            }
+          }
+        } else {
+          for (int k = g; k < min(g + 8, count); ++k) {
+            const uint32_t now = __shfl_sync(0xffffffffu, code, l0 + k);
+            const float v = load1(from + k * kRpChunk);
+            if ((int)(now & 0xffffu) != row1) {
+              flush(row1, run1);
+              row1 = (int)(now & 0xffffu);
+            }
+            if ((int)(now >> 16) != row2) {
+              flush(row2 >= 0 ? rows1 + row2 : -1, run2);
+              row2 = (int)(now >> 16);
+            }
+            run1 += v, run2 += v;
+          }
         }
-        if ((int)(now >> 16) != row2) {
-          flush(row2 >= 0 ? rows1 + row2 : -1, run2);
-          row2 = (int)(now >> 16);
-        }
-        run1.x += v.x, run1.y += v.y, run2.x += v.x, run2.y += v.y;
       }
     }
+    if (part == kParts - 1) here.next(strips);
   }
   flush(row1, run1);
   flush(row2 >= 0 ? rows1 + row2 : -1, run2);
-  __syncthreads();
   // the columns of W: a table row counts for its position and its token column, a copy row for its own and, unless the entities differ, the entity's
   const int t = a.columns(), tok = 2 * a.r + 2, ent = 4 * a.r + 4;
-  float* out = partial + ((long long)blockIdx.y * gridDim.x + blockIdx.x) * t * kRpChunk + 2 * (32 * warp + lane);
+  float* const out = partial + ((long long)blockIdx.y * gridDim.x + blockIdx.x) * t * kRpChunk + threadIdx.x;
   const auto range = [&](int from, int to) {
-    float2 v = make_float2(0.f, 0.f);
-    for (int k = from; k < to; ++k) {
-      const float2 m = mine[k * (kRpChunk / 2)];
-      v.x += m.x, v.y += m.y;
-    }
-    return v;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int k = from; k < to; k += 4)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += k + e < to ? mine[(k + e) * kRpChunk] : 0.f;
+    return (v[0] + v[1]) + (v[2] + v[3]);
   };
-  for (int k = 0; k < t; ++k) {
-    float2 v;
-    if (k < ent - 1) v = range(k, k + 1);
-    else if (k == ent - 1) v = range(0, tok);
-    else if (k == ent) v = range(rows1, rows1 + 2 * a.s + 1);
-    else v = range(rows1 + k - ent - 1, rows1 + k - ent);
-    if (k == a.r) {                                // pairs of one residue, whatever their tokens
-      const float2 m = range(tok, rows1);
-      v.x += m.x, v.y += m.y;
-    }
-    *reinterpret_cast<float2*>(out + (long long)k * kRpChunk) = v;
-  }
+#pragma unroll 8
+  for (int k = 0; k < ent - 1; ++k) out[k * kRpChunk] = mine[k * kRpChunk];
+  out[a.r * kRpChunk] = mine[a.r * kRpChunk] + range(tok, rows1);      // pairs of one residue, whatever their tokens
+  out[(ent - 1) * kRpChunk] = range(0, tok);
+  out[ent * kRpChunk] = range(rows1, rows1 + 2 * a.s + 1);
+  for (int k = ent + 1; k < t; ++k) out[k * kRpChunk] = mine[(rows1 + k - ent - 1) * kRpChunk];
 }
 
 // dw[c][t] = the blocks' sums, in their order: eight slices of the blocks, each added up by one thread a channel, then the slices.
@@ -254,8 +314,10 @@ static bool relpos_sizes(int64_t batch, int64_t n, int64_t c, int32_t r, int32_t
 static bool relpos_fits(int64_t c, int32_t r, int32_t s) {
   return c % 8 == 0 && r <= kRpMaxRows && s <= kRpMaxRows && 4 * r + 2 * s + 5 <= kRpMaxRows;
 }
-// Blocks of the backward pass: two an SM, and no more than leave each some hundreds of pairs, since each brings sums of its own.
-static int64_t relpos_blocks(int64_t pairs) { return std::max<int64_t>(1, std::min<int64_t>(2 * sm_count(), pairs / 256)); }
+// Backward pass: units (strips of 32 pairs of a row), and blocks: two an SM, and no more than leave each some units, since each brings
+// sums of its own.
+static int64_t relpos_units(int64_t batch, int64_t n) { return batch * n * ((n + kRpPairs - 1) / kRpPairs); }
+static int64_t relpos_blocks(int64_t units) { return std::max<int64_t>(1, std::min<int64_t>(2 * sm_count(), units / 16)); }
 
 }  // namespace px
 
@@ -263,7 +325,7 @@ using namespace px;
 
 extern "C" int64_t px_relpos_workspace_bytes(int64_t batch, int64_t n, int64_t c, int32_t r_max, int32_t s_max) {
   if (!relpos_sizes(batch, n, c, r_max, s_max) || !relpos_fits(c, r_max, s_max)) return 0;
-  return relpos_blocks(batch * n * n) * ((c + kRpChunk - 1) / kRpChunk) * (4 * r_max + 2 * s_max + 7) * kRpChunk * 4;
+  return relpos_blocks(relpos_units(batch, n)) * ((c + kRpChunk - 1) / kRpChunk) * (4 * r_max + 2 * s_max + 7) * kRpChunk * 4;
 }
 
 extern "C" int32_t px_relpos_fwd(const int64_t* asym_id, const int64_t* residue_index, const int64_t* entity_id, const int64_t* token_index,
@@ -276,9 +338,9 @@ extern "C" int32_t px_relpos_fwd(const int64_t* asym_id, const int64_t* residue_
   const RelposArgs a = {(const long long*)asym_id, (const long long*)residue_index, (const long long*)entity_id, (const long long*)token_index,
                         (const long long*)sym_id, n, batch * n * n, (int)c, r_max, s_max};
   const size_t smem = (size_t)(a.rows1() + a.rows2()) * kRpPitch * 4;
-  const int64_t strips = batch * n * ((n + kRpPairs - 1) / kRpPairs), per = kRpFwdThreads / 32;
+  const int64_t strips = relpos_units(batch, n);
   const int64_t room = sm_count() * std::max<int64_t>(1, std::min<int64_t>(4, (int64_t)(227 << 10) / (int64_t)(smem + 1024)));
-  const dim3 grid((unsigned)std::min((strips + per - 1) / per, room), (unsigned)((c + kRpChunk - 1) / kRpChunk));
+  const dim3 grid((unsigned)std::min((strips + 3) / 4, room), (unsigned)((c + kRpChunk - 1) / kRpChunk));
   static SmemLimit limit[3];
   const auto go = [&](auto* kernel, auto* out) {
     if (!limit[dtype].set(kernel, (size_t)kRpMaxRows * kRpPitch * 4)) return false;
@@ -306,14 +368,14 @@ extern "C" int32_t px_relpos_bwd(const int64_t* asym_id, const int64_t* residue_
       ((uintptr_t)workspace & 15))
     return PX_ERR_BAD_ARG;
   if (workspace_bytes < px_relpos_workspace_bytes(batch, n, c, r_max, s_max)) return PX_ERR_WORKSPACE;
-  const int64_t most = relpos_blocks(a.pairs), per = ((a.pairs + most - 1) / most + kRpPairs - 1) / kRpPairs * kRpPairs;
-  const int blocks = (int)((a.pairs + per - 1) / per);
+  const int64_t units = relpos_units(batch, n), most = relpos_blocks(units), per = (units + most - 1) / most;
+  const int blocks = (int)((units + per - 1) / per);
   const unsigned chunks = (unsigned)((c + kRpChunk - 1) / kRpChunk);
   const size_t fixed = (size_t)kRpStages * kRpStageBytes, smem = fixed + (size_t)(a.rows1() + a.rows2()) * kRpChunk * 4;
   static SmemLimit limit[3];
   const auto go = [&](auto* kernel, auto* in) {
     if (!limit[dtype].set(kernel, fixed + (size_t)kRpMaxRows * kRpChunk * 4)) return false;
-    kernel<<<dim3((unsigned)blocks, chunks), 64, smem, st>>>(a, in, (float*)workspace, per);
+    kernel<<<dim3((unsigned)blocks, chunks), kRpBwdThreads, smem, st>>>(a, in, (float*)workspace, (int)per);
     return cudaGetLastError() == cudaSuccess;
   };
   const bool done = dtype == PX_F32    ? go(relpos_bwd_kernel<float>, (const float*)dz)

@@ -19,7 +19,6 @@
 #include <ATen/ops/full.h>
 #include <ATen/ops/mm.h>
 #include <ATen/ops/ones.h>
-#include <ATen/ops/stack.h>
 #include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>

@@ -99,44 +99,50 @@ struct RelposSizes {
   int64_t batch, n, c, r, s, type;      // type: of z
 };
 
-struct RelposFunction : torch::autograd::Function<RelposFunction> {
-  // ids: [5][batch][n], in the order of the C ABI
-  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& weight, const Tensor& ids, int64_t batch, int64_t n, int64_t r,
-                        int64_t s, int64_t type) {
-    ctx->save_for_backward({ids});
-    ctx->saved_data["sizes"] = c10::List<int64_t>({batch, n, weight.size(0), r, s, type, (int64_t)weight.scalar_type()});
-    return run(weight, ids, {batch, n, weight.size(0), r, s, type});
+typedef std::vector<Tensor> Features;      // asym, residue, entity, token, copy numbers: int64, contiguous
+struct FeatureData {
+  const int64_t* p[5];
+  explicit FeatureData(const Tensor* f) {
+    for (int i = 0; i < 5; ++i) p[i] = (const int64_t*)f[i].data_ptr();
   }
-  static Tensor run(const Tensor& weight, const Tensor& ids, const RelposSizes& z) {
-    c10::cuda::CUDAGuard guard(ids.device());
-    const Tensor w = weight.detach().to(at::kFloat).contiguous();
+};
+
+struct RelposFunction : torch::autograd::Function<RelposFunction> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& weight, const Features& f, int64_t batch, int64_t n, int64_t r,
+                        int64_t s, int64_t type) {
+    ctx->save_for_backward({f[0], f[1], f[2], f[3], f[4]});
+    ctx->saved_data["sizes"] = c10::List<int64_t>({batch, n, weight.size(0), r, s, (int64_t)weight.scalar_type()});
+    return run(weight, f, {batch, n, weight.size(0), r, s, type});
+  }
+  static Tensor run(const Tensor& weight, const Features& f, const RelposSizes& z) {
+    const Tensor w = weight.scalar_type() == at::kFloat && weight.is_contiguous() ? weight : weight.detach().to(at::kFloat).contiguous();
     const Tensor out = at::empty({z.batch, z.n, z.n, z.c}, w.options().dtype((at::ScalarType)z.type));
-    const int64_t *id = (const int64_t*)ids.data_ptr(), per = z.batch * z.n;
+    const FeatureData d(f.data());
     const cudaStream_t st = at::cuda::getCurrentCUDAStream();
     launch("px_relpos_fwd", st, [&] {
-      return abi.px_relpos_fwd(id, id + per, id + 2 * per, id + 3 * per, id + 4 * per, (const float*)w.data_ptr(), out.data_ptr(), z.batch, z.n,
-                               z.c, (int32_t)z.r, (int32_t)z.s, dtype_code(out, "dtype"), st);
+      return abi.px_relpos_fwd(d.p[0], d.p[1], d.p[2], d.p[3], d.p[4], (const float*)w.data_ptr(), out.data_ptr(), z.batch, z.n, z.c,
+                               (int32_t)z.r, (int32_t)z.s, dtype_code(out, "dtype"), st);
     });
     return out;
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     first_derivative_only("relative_position_encoding");
-    const Tensor ids = ctx->get_saved_variables()[0];
+    const auto f = ctx->get_saved_variables();
     const auto v = ctx->saved_data["sizes"].toIntVector();
-    c10::cuda::CUDAGuard guard(ids.device());
+    c10::cuda::CUDAGuard guard(f[0].device());
     const Tensor dz = aligned(grads[0]);
     const int64_t batch = v[0], n = v[1], c = v[2];
     const int32_t r = (int32_t)v[3], s = (int32_t)v[4];
-    const Tensor dw = at::empty({c, 4 * r + 2 * s + 7}, ids.options().dtype(at::kFloat));
+    const Tensor dw = at::empty({c, 4 * r + 2 * s + 7}, dz.options().dtype(at::kFloat));
     const int64_t bytes = abi.px_relpos_workspace_bytes(batch, n, c, r, s);
-    const Tensor ws = bytes_like(ids, bytes);
-    const int64_t *id = (const int64_t*)ids.data_ptr(), per = batch * n;
+    const Tensor ws = bytes_like(dz, bytes);
+    const FeatureData d(f.data());
     const cudaStream_t st = at::cuda::getCurrentCUDAStream();
     launch("px_relpos_bwd", st, [&] {
-      return abi.px_relpos_bwd(id, id + per, id + 2 * per, id + 3 * per, id + 4 * per, dz.data_ptr(), (float*)dw.data_ptr(), ws.data_ptr(), bytes,
-                               batch, n, c, r, s, dtype_code(dz, "the gradient"), st);
+      return abi.px_relpos_bwd(d.p[0], d.p[1], d.p[2], d.p[3], d.p[4], dz.data_ptr(), (float*)dw.data_ptr(), ws.data_ptr(), bytes, batch, n, c,
+                               r, s, dtype_code(dz, "the gradient"), st);
     });
-    return {dw.to((at::ScalarType)v[6]), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    return {dw.to((at::ScalarType)v[5]), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
 
@@ -150,28 +156,23 @@ Tensor relative_position_encoding(const Tensor& weight, const std::vector<Tensor
     fail("weight must be [c, " + std::to_string(4 * r + 2 * s + 7) + "] for these r_max and s_max, got " + shape_of(weight));
   if (weight.size(0) == 0 || weight.size(0) % 8 != 0 || 4 * r + 2 * s + 5 > 380)
     fail("the kernels handle a multiple of 8 channels and 4 r_max + 2 s_max of up to 375");
-  std::vector<Tensor> rows;
+  c10::cuda::CUDAGuard guard(weight.device());
+  Features rows;
   for (int i = 0; i < 5; ++i) {
     const Tensor& f = features[i];
     need_on(f, weight.device(), names[i]);
     if (!at::isIntegralType(f.scalar_type(), false)) fail(std::string(names[i]) + " must be an integer tensor");
     if (f.dim() < 1 || f.sizes() != features[0].sizes()) fail("the features must have one shape [..., N]");
-    rows.push_back(f.to(at::kLong));
+    rows.push_back(f.to(at::kLong).contiguous());
   }
   const int64_t n = features[0].size(-1), batch = n ? features[0].numel() / n : 0;
   auto shape = features[0].sizes().vec();
   shape.push_back(n);
   shape.push_back(weight.size(0));
-  c10::cuda::CUDAGuard guard(weight.device());
-  Tensor ids;
-  {
-    at::AutoDispatchBelowADInplaceOrView below;
-    ids = at::stack(rows).reshape({5, batch, n});      // one piece, and a snapshot: the backward pass reads it again
-  }
   const int64_t type = (int64_t)(z_type.has_value() ? *z_type : weight.scalar_type());
   if (type != (int64_t)at::kFloat && type != (int64_t)at::kBFloat16 && type != (int64_t)at::kHalf) fail("dtype must be float32, bfloat16 or float16");
-  const Tensor z = at::GradMode::is_enabled() && weight.requires_grad() ? RelposFunction::apply(weight, ids, batch, n, r, s, type)
-                                                                        : RelposFunction::run(weight, ids, {batch, n, weight.size(0), r, s, type});
+  const Tensor z = at::GradMode::is_enabled() && weight.requires_grad() ? RelposFunction::apply(weight, rows, batch, n, r, s, type)
+                                                                        : RelposFunction::run(weight, rows, {batch, n, weight.size(0), r, s, type});
   return z.view(shape);
 }
 

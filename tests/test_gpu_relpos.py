@@ -51,7 +51,7 @@ def _check(f, c, r, s, dtype, seed=1):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", list(DTYPES))
-@pytest.mark.parametrize("n", [1, 2, 31, 33, 97, 150])
+@pytest.mark.parametrize("n", [1, 2, 16, 31, 33, 97, 150])
 def test_chains(n, dtype):
     _check(_features(n, n), 128, 32, 2, DTYPES[dtype])
 
@@ -98,15 +98,13 @@ def test_module_and_its_state():
 
 
 @pytest.mark.gpu
-def test_features_may_change_before_the_backward_pass():
+def test_features_that_change_before_the_backward_pass_are_noticed():
     f = {k: v.cuda() for k, v in _features(40, 8).items()}
     w = torch.randn(128, 139, device="cuda").requires_grad_()
-    dz = torch.randn(40, 40, 128, device="cuda")
-    want, = torch.autograd.grad(px.relative_position_encoding(w, **f), w, dz)
     z = px.relative_position_encoding(w, **f)
-    for v in f.values():
-        v.zero_()
-    assert torch.equal(torch.autograd.grad(z, w, dz)[0], want)
+    f["sym_id"].zero_()
+    with pytest.raises(RuntimeError, match="inplace"):
+        torch.autograd.grad(z.sum(), w)
 
 
 @pytest.mark.gpu
