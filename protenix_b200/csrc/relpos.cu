@@ -127,9 +127,17 @@ __device__ __forceinline__ float load1<__half>(const __half* p) { return __half2
 
 constexpr int kRpBwdThreads = kRpChunk;      // a thread = one channel
 
+// The codes of all pairs, by units: lane l of a strip has pair l's (the last one's beyond the row).
+__global__ void __launch_bounds__(256) relpos_code_kernel(RelposArgs a, int strips, uint32_t* __restrict__ codes) {
+  const int n = (int)a.n, strip = blockIdx.x % strips, lane = threadIdx.x & 31;
+  const long long i = (long long)(blockIdx.x / strips) * 8 + (threadIdx.x >> 5);
+  if (i < a.pairs / a.n) codes[(i * strips + strip) * kRpPairs + lane] = relpos_code(a, i, i / n * n + min(strip * kRpPairs + lane, n - 1));
+}
+
 // Block b adds up the units [b * per, (b + 1) * per) of its channels; a unit is a row's strip of 32 pairs.  partial: [chunk][block][columns][kRpChunk].
 template <typename T>
-__global__ void __launch_bounds__(kRpBwdThreads) relpos_bwd_kernel(RelposArgs a, const T* __restrict__ dz, float* __restrict__ partial, int per) {
+__global__ void __launch_bounds__(kRpBwdThreads) relpos_bwd_kernel(RelposArgs a, const T* __restrict__ dz, const uint32_t* __restrict__ codes,
+                                                                   float* __restrict__ partial, int per) {
   constexpr int kPairs = kRpStageBytes / (kRpChunk * (int)sizeof(T));      // of a stage: 16 (fp32) or 32
   constexpr int kParts = kRpPairs / kPairs;                                // stages of a unit
   extern __shared__ __align__(1024) unsigned char smem_raw[];
@@ -187,11 +195,25 @@ __global__ void __launch_bounds__(kRpBwdThreads) relpos_bwd_kernel(RelposArgs a,
     if (row >= 0) mine[row * kRpChunk] += run;
     run = 0.f;
   };
-  uint32_t code = 0;
+  const auto turn_to = [&](uint32_t now) {         // a code for the whole warp: what does not go on is put away
+    if ((int)(now & 0xffffu) != row1) {
+      flush(row1, run1);
+      row1 = (int)(now & 0xffffu);
+    }
+    if ((int)(now >> 16) != row2) {
+      flush(row2 >= 0 ? rows1 + row2 : -1, run2);
+      row2 = (int)(now >> 16);
+    }
+  };
+  const uint32_t* const my_codes = codes + begin * kRpPairs + lane;
+  uint32_t code = 0, next = steps > 0 ? __ldg(my_codes) : 0;
   bool ok = true;
   for (int step = 0; step < steps; ++step) {
     const int part = step % kParts, count = pairs_of(here, part), b = step % kRpStages;
-    if (part == 0) code = relpos_code(a, here.i, here.i / n * n + min(here.strip * kRpPairs + lane, n - 1));
+    if (part == 0) {
+      code = next;
+      if (step + kParts < steps) next = __ldg(my_codes + (long long)(step / kParts + 1) * kRpPairs);
+    }
     ok = mbar_wait_warp(&full[b], (step / kRpStages) & 1, 1u);
     ok = __syncthreads_and(ok) != 0;               // all are through with the stage that is filled next
     if (!ok) break;
@@ -201,65 +223,49 @@ __global__ void __launch_bounds__(kRpBwdThreads) relpos_bwd_kernel(RelposArgs a,
     }
     const T* const from = stage + b * (kRpStageBytes / (int)sizeof(T)) + threadIdx.x;
     const int l0 = part * kPairs;                  // the lane that has the code of the stage's first pair
-    const uint32_t first = code & 0xffffu, second = code >> 16;
-    // neighbours with one row each, neighbours with rows that all differ, and both for the second table: bits by lane
-    const uint32_t same1 = __ballot_sync(0xffffffffu, first == (uint32_t)row1), same2 = __ballot_sync(0xffffffffu, second == (uint32_t)row2);
     const uint32_t all = kPairs == 32 ? 0xffffffffu : 0xffffu << l0;
-    if (count == kPairs && (same1 & same2 & all) == all) {
+    const uint32_t lead = __shfl_sync(0xffffffffu, code, l0);
+    if (count == kPairs && (__ballot_sync(0xffffffffu, code == lead) & all) == all) {
+      turn_to(lead);
       float t[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int k = 0; k < kPairs; ++k) t[k & 3] += load1(from + k * kRpChunk);
       const float sum = (t[0] + t[1]) + (t[2] + t[3]);
       run1 += sum, run2 += sum;
     } else {
-      const uint32_t like = __match_any_sync(0xffffffffu, first) & (0xffu << (lane & 24));      // in this lane's group of eight
-      const uint32_t distinct = __ballot_sync(0xffffffffu, like == 1u << lane);
+      const uint32_t first = code & 0xffffu, second = code >> 16, mine8 = 0xffu << (lane & 24);      // the lanes of this lane's group of eight
+      const uint32_t like = __match_any_sync(0xffffffffu, first) & mine8;
+      const uint32_t distinct = __ballot_sync(0xffffffffu, like == 1u << lane), alike = __ballot_sync(0xffffffffu, like == mine8);
+      const uint32_t copies = __ballot_sync(0xffffffffu, second == __shfl_sync(0xffffffffu, second, lane & 24));
+#pragma unroll 1
       for (int g = 0; g < count; g += 8) {
-        const uint32_t group = 0xffu << (l0 + g);
-        const uint32_t lead = __shfl_sync(0xffffffffu, code, l0 + g);
-        if (g + 8 <= count && (distinct & group) == group) {
-          // eight rows of the first table, side by side: their sums have no order among them
-          float v[8], sum[8];
+        const uint32_t group = 0xffu << (l0 + g), now = __shfl_sync(0xffffffffu, code, l0 + g);
+        if (g + 8 <= count && (copies & group) == group && ((distinct | alike) & group) == group) {
+          float v[8];
 #pragma unroll
           for (int k = 0; k < 8; ++k) v[k] = load1(from + (g + k) * kRpChunk);
-          flush(row1, run1);
-          row1 = -1;
-          float* at[8];
-#pragma unroll
-          for (int k = 0; k < 8; ++k) at[k] = mine + __shfl_sync(0xffffffffu, first, l0 + g + k) * kRpChunk;
-#pragma unroll
-          for (int k = 0; k < 8; ++k) sum[k] = *at[k] + v[k];
-#pragma unroll
-          for (int k = 0; k < 8; ++k) *at[k] = sum[k];
-          if (__all_sync(0xffffffffu, second == lead >> 16 || (group >> lane & 1) == 0)) {
-            if ((int)(lead >> 16) != row2) {
-              flush(row2 >= 0 ? rows1 + row2 : -1, run2);
-              row2 = (int)(lead >> 16);
-            }
-            run2 += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+          const float sum = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+          if ((alike & group) == group) {
+            turn_to(now);
+            run1 += sum, run2 += sum;
           } else {
+            // eight rows of the first table, side by side: their sums have no order among them
+            turn_to((now & 0xffff0000u) | 0xffffu);
+            row1 = -1;
+            float* at[8];
+            float u[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              const int now = (int)__shfl_sync(0xffffffffu, second, l0 + g + k);
-              if (now != row2) {
-                flush(row2 >= 0 ? rows1 + row2 : -1, run2);
-                row2 = now;
-              }
-              run2 += v[k];
-            }
+            for (int k = 0; k < 8; ++k) at[k] = mine + __shfl_sync(0xffffffffu, first, l0 + g + k) * kRpChunk;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) u[k] = *at[k];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) *at[k] = u[k] + v[k];
+            run1 = 0.f, run2 += sum;
           }
         } else {
           for (int k = g; k < min(g + 8, count); ++k) {
-            const uint32_t now = __shfl_sync(0xffffffffu, code, l0 + k);
             const float v = load1(from + k * kRpChunk);
-            if ((int)(now & 0xffffu) != row1) {
-              flush(row1, run1);
-              row1 = (int)(now & 0xffffu);
-            }
-            if ((int)(now >> 16) != row2) {
-              flush(row2 >= 0 ? rows1 + row2 : -1, run2);
-              row2 = (int)(now >> 16);
-            }
+            turn_to(__shfl_sync(0xffffffffu, code, l0 + k));
             run1 += v, run2 += v;
           }
         }
@@ -325,7 +331,8 @@ using namespace px;
 
 extern "C" int64_t px_relpos_workspace_bytes(int64_t batch, int64_t n, int64_t c, int32_t r_max, int32_t s_max) {
   if (!relpos_sizes(batch, n, c, r_max, s_max) || !relpos_fits(c, r_max, s_max)) return 0;
-  return relpos_blocks(relpos_units(batch, n)) * ((c + kRpChunk - 1) / kRpChunk) * (4 * r_max + 2 * s_max + 7) * kRpChunk * 4;
+  const int64_t units = relpos_units(batch, n);
+  return units * kRpPairs * 4 + relpos_blocks(units) * ((c + kRpChunk - 1) / kRpChunk) * (4 * r_max + 2 * s_max + 7) * kRpChunk * 4;
 }
 
 extern "C" int32_t px_relpos_fwd(const int64_t* asym_id, const int64_t* residue_index, const int64_t* entity_id, const int64_t* token_index,
@@ -371,17 +378,24 @@ extern "C" int32_t px_relpos_bwd(const int64_t* asym_id, const int64_t* residue_
   const int64_t units = relpos_units(batch, n), most = relpos_blocks(units), per = (units + most - 1) / most;
   const int blocks = (int)((units + per - 1) / per);
   const unsigned chunks = (unsigned)((c + kRpChunk - 1) / kRpChunk);
+  const int strips = (int)(units / (batch * n));
+  uint32_t* const codes = (uint32_t*)workspace;
+  float* const partial = (float*)(codes + units * kRpPairs);
+  const int64_t code_blocks = (batch * n + 7) / 8 * strips;
+  if (code_blocks > 0x7fffffff) return PX_ERR_UNSUPPORTED;
+  relpos_code_kernel<<<(unsigned)code_blocks, 256, 0, st>>>(a, strips, codes);
+  if (cudaGetLastError() != cudaSuccess) return PX_ERR_LAUNCH;
   const size_t fixed = (size_t)kRpStages * kRpStageBytes, smem = fixed + (size_t)(a.rows1() + a.rows2()) * kRpChunk * 4;
   static SmemLimit limit[3];
   const auto go = [&](auto* kernel, auto* in) {
     if (!limit[dtype].set(kernel, fixed + (size_t)kRpMaxRows * kRpChunk * 4)) return false;
-    kernel<<<dim3((unsigned)blocks, chunks), kRpBwdThreads, smem, st>>>(a, in, (float*)workspace, (int)per);
+    kernel<<<dim3((unsigned)blocks, chunks), kRpBwdThreads, smem, st>>>(a, in, codes, partial, (int)per);
     return cudaGetLastError() == cudaSuccess;
   };
   const bool done = dtype == PX_F32    ? go(relpos_bwd_kernel<float>, (const float*)dz)
                     : dtype == PX_BF16 ? go(relpos_bwd_kernel<bf16>, (const bf16*)dz)
                                        : go(relpos_bwd_kernel<__half>, (const __half*)dz);
   if (!done) return PX_ERR_LAUNCH;
-  relpos_reduce_kernel<<<dim3((unsigned)a.columns(), chunks), 8 * kRpChunk, 0, st>>>((const float*)workspace, dw, blocks, a.columns(), (int)c);
+  relpos_reduce_kernel<<<dim3((unsigned)a.columns(), chunks), 8 * kRpChunk, 0, st>>>(partial, dw, blocks, a.columns(), (int)c);
   return cudaGetLastError() == cudaSuccess ? PX_OK : PX_ERR_LAUNCH;
 }
