@@ -81,9 +81,10 @@ SIGNATURES = {
     "px_recycle_update": (I32, [P, P, P, I32, P, P, P, I64, F, P]),
     "px_scale_add_rowwise": (I32, [P, P, P, P, I64, I64, I64, I32, P]),
     "px_dropout_add": (I32, [P, P, P, I64, I64, I64, D, I64, I64, P, P, I32, P]),
+    "px_relpos_codes_bytes": (I64, [I64, I64]),
     "px_relpos_workspace_bytes": (I64, [I64, I64, I64, I32, I32]),
-    "px_relpos_fwd": (I32, [P, P, P, P, P, P, P, I64, I64, I64, I32, I32, I32, P]),
-    "px_relpos_bwd": (I32, [P, P, P, P, P, P, P, P, I64, I64, I64, I64, I32, I32, I32, P]),
+    "px_relpos_fwd": (I32, [P, P, P, P, P, P, P, P, I64, I64, I64, I32, I32, I32, P]),
+    "px_relpos_bwd": (I32, [P, P, P, P, I64, I64, I64, I64, I32, I32, I32, P]),
     "px_window_lse_floats": (I64, [I64, I64, I64]),
     "px_window_fwd": (I32, [P, P, P, P, P, P, P]),
     "px_window_workspace_bytes": (I64, [P, I32]),

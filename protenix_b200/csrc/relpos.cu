@@ -8,9 +8,9 @@
 // Two table rows make a pair: bt differs from 2 r + 1 only where bp = r, and the entity's flag follows from bc, so there are
 // 4 r + 3 sums W_pos + W_tok and 2 s + 2 sums W_chain + W_ent (both tables 70 KB of shared memory for r = 32, s = 2 and 128 channels).
 //
-// Forward: memory-bound writer, a warp takes 32 neighbouring pairs of a row; a lane finds one pair's two rows, then the warp
-// writes pair after pair, 4 channels a lane, and looks the rows up again only where they change (most neighbours are far apart or in
-// another chain: clipped alike).
+// Forward: memory-bound writer, a warp takes 32 neighbouring pairs of a row; a lane finds one pair's two rows (a code, kept for the
+// backward pass: 4 bytes beside the pair's 256 or 512), then the warp writes pair after pair, 4 channels a lane, and looks the rows up again only
+// where they change (most neighbours are far apart or in another chain: clipped alike).
 //
 // Backward: memory-bound reader.  A block (a thread = one channel) reads strips of 32 pairs of a row through a ring of bulk copies and holds
 // sums of its own for every table row in shared memory, so there are no atomics and a call gives the same bits every time.  Neighbours with
@@ -63,42 +63,55 @@ __device__ __forceinline__ void store4<__half>(__half* p, float4 v) {
   __stcs(reinterpret_cast<uint2*>(p), make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi)));
 }
 
-constexpr int kRpFwdThreads = 512;
-constexpr int kRpPitch = kRpChunk + 4;   // floats of a table row: rows 16 bytes apart in the banks while the tables are laid out
+constexpr int kRpFwdThreads = 1024;      // one block an SM
 
+// codes: what relpos_bwd_kernel reads, [row of all batches][strip][32] (the last pair's beyond the row), or NULL.  slice: channels of W that are
+// brought into shared memory at a time, all of them unless the tables are large.
 template <typename T>
-__global__ void __launch_bounds__(kRpFwdThreads) relpos_fwd_kernel(RelposArgs a, const float* __restrict__ w, T* __restrict__ z) {
-  extern __shared__ __align__(16) float rp_table[];
+__global__ void __launch_bounds__(kRpFwdThreads) relpos_fwd_kernel(RelposArgs a, const float* __restrict__ w, T* __restrict__ z,
+                                                                   uint32_t* __restrict__ codes, int slice) {
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  __shared__ uint64_t full;
   const int c0 = blockIdx.y * kRpChunk, channels = min(kRpChunk, a.c - c0), t = a.columns();
-  const int rows1 = a.rows1(), rows2 = a.rows2(), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int pos = 0, tok = 2 * a.r + 2, ent = 4 * a.r + 4, chain = ent + 1;      // first columns of the four parts of W
-  // A lane has one table row of eight channels at a time: sixteen loads in flight (one channel after the other took 15 us).
-  constexpr int kWarps = kRpFwdThreads / 32;
-  for (int k = lane; k < rows1 + rows2; k += 32) {
-    const int first = k < tok ? pos + k : k < rows1 ? pos + a.r : chain + k - rows1;
-    const int second = k < tok ? tok + 2 * a.r + 1 : k < rows1 ? k : k - rows1 < 2 * a.s + 1 ? ent : -1;
-#pragma unroll 1
-    for (int ch0 = warp; ch0 < channels; ch0 += 8 * kWarps) {
-      float u[8], v[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int ch = min(ch0 + e * kWarps, channels - 1);
-        u[e] = __ldg(w + (long long)(c0 + ch) * t + first);
-        v[e] = __ldg(w + (long long)(c0 + ch) * t + max(second, 0));
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (ch0 + e * kWarps < channels) rp_table[k * kRpPitch + ch0 + e * kWarps] = u[e] + (second < 0 ? 0.f : v[e]);
-    }
+  const int rows1 = a.rows1(), rows = rows1 + a.rows2(), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tok = 2 * a.r + 2, ent = 4 * a.r + 4, chain = ent + 1;      // first columns of the parts of W behind the first
+  float* const table = reinterpret_cast<float*>(smem_raw);              // [rows][kRpChunk]
+  float* const part = table + rows * kRpChunk;                          // [slice][t]
+  if (threadIdx.x == 0) {
+    mbar_init(&full, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
   __syncthreads();
-  const long long strips = (a.n + kRpPairs - 1) / kRpPairs, rows = a.pairs / a.n;
-  const long long warps = (long long)gridDim.x * (kRpFwdThreads / 32);
+  bool ok = true;
+  for (int s0 = 0, k = 0; s0 < channels; s0 += slice, ++k) {
+    const int count = min(slice, channels - s0);
+    if (threadIdx.x == 0) {
+      mbar_expect_tx(&full, (uint32_t)(count * t * 4));
+      bulk_load(part, w + (long long)(c0 + s0) * t, (uint32_t)(count * t * 4), &full);
+    }
+    ok = mbar_wait(&full, k & 1, 2u) && ok;
+    // A lane = a channel: t is odd, so neither side of this transposition meets a bank twice.
+    for (int u = threadIdx.x; u < rows * kRpChunk; u += kRpFwdThreads) {
+      const int ch = u % kRpChunk, row = u / kRpChunk;
+      if (ch < count) {
+        const float* const f = part + ch * t;
+        const float v = row < tok     ? f[row] + f[tok + 2 * a.r + 1]
+                        : row < rows1 ? f[a.r] + f[row]
+                                      : f[chain + row - rows1] + (row - rows1 < 2 * a.s + 1 ? f[ent] : 0.f);
+        table[row * kRpChunk + s0 + ch] = v;
+      }
+    }
+    ok = __syncthreads_and(ok) != 0;
+  }
+  if (!ok) return;
+  const int strips = (int)((a.n + kRpPairs - 1) / kRpPairs);
+  const long long units = a.pairs / a.n * strips, warps = (long long)gridDim.x * (kRpFwdThreads / 32);
   const bool mine = 4 * lane < channels;
-  for (long long u = (long long)blockIdx.x * (kRpFwdThreads / 32) + warp; u < rows * strips; u += warps) {
-    const long long i = u / strips, j0 = (u - i * strips) * kRpPairs, first = i / a.n * a.n;     // i counts the rows of all batches
-    const int count = (int)min((long long)kRpPairs, a.n - j0);
-    const uint32_t code = relpos_code(a, i, first + j0 + min(lane, count - 1));
+  for (long long u = (long long)warp * gridDim.x + blockIdx.x; u < units; u += warps) {      // the blocks have equal shares, however few units there are
+    const long long i = u / strips;                                      // counts the rows of all batches
+    const int j0 = (int)(u - i * strips) * kRpPairs, count = (int)min((long long)kRpPairs, a.n - j0);
+    const uint32_t code = relpos_code(a, i, i / a.n * a.n + j0 + min(lane, count - 1));
+    if (codes && blockIdx.y == 0) codes[u * kRpPairs + lane] = code;
     T* out = z + (i * a.n + j0) * a.c + c0 + 4 * lane;
     uint32_t have = 0xffffffffu;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -107,8 +120,8 @@ __global__ void __launch_bounds__(kRpFwdThreads) relpos_fwd_kernel(RelposArgs a,
       const uint32_t now = __shfl_sync(0xffffffffu, code, k);
       if (now != have) {
         have = now;
-        const float4 p = *reinterpret_cast<const float4*>(rp_table + (now & 0xffffu) * kRpPitch + 4 * lane);
-        const float4 q = *reinterpret_cast<const float4*>(rp_table + (rows1 + (now >> 16)) * kRpPitch + 4 * lane);
+        const float4 p = *reinterpret_cast<const float4*>(table + (now & 0xffffu) * kRpChunk + 4 * lane);
+        const float4 q = *reinterpret_cast<const float4*>(table + (rows1 + (now >> 16)) * kRpChunk + 4 * lane);
         v = make_float4(p.x + q.x, p.y + q.y, p.z + q.z, p.w + q.w);
       }
       if (mine) store4(out + (long long)k * a.c, v);
@@ -127,16 +140,9 @@ __device__ __forceinline__ float load1<__half>(const __half* p) { return __half2
 
 constexpr int kRpBwdThreads = kRpChunk;      // a thread = one channel
 
-// The codes of all pairs, by units: lane l of a strip has pair l's (the last one's beyond the row).
-__global__ void __launch_bounds__(256) relpos_code_kernel(RelposArgs a, int strips, uint32_t* __restrict__ codes) {
-  const int n = (int)a.n, strip = blockIdx.x % strips, lane = threadIdx.x & 31;
-  const long long i = (long long)(blockIdx.x / strips) * 8 + (threadIdx.x >> 5);
-  if (i < a.pairs / a.n) codes[(i * strips + strip) * kRpPairs + lane] = relpos_code(a, i, i / n * n + min(strip * kRpPairs + lane, n - 1));
-}
-
 // Block b adds up the units [b * per, (b + 1) * per) of its channels; a unit is a row's strip of 32 pairs.  partial: [chunk][block][columns][kRpChunk].
 template <typename T>
-__global__ void __launch_bounds__(kRpBwdThreads) relpos_bwd_kernel(RelposArgs a, const T* __restrict__ dz, const uint32_t* __restrict__ codes,
+__global__ void __launch_bounds__(kRpBwdThreads, 2) relpos_bwd_kernel(RelposArgs a, const T* __restrict__ dz, const uint32_t* __restrict__ codes,
                                                                    float* __restrict__ partial, int per) {
   constexpr int kPairs = kRpStageBytes / (kRpChunk * (int)sizeof(T));      // of a stage: 16 (fp32) or 32
   constexpr int kParts = kRpPairs / kPairs;                                // stages of a unit
@@ -215,7 +221,9 @@ __global__ void __launch_bounds__(kRpBwdThreads) relpos_bwd_kernel(RelposArgs a,
       if (step + kParts < steps) next = __ldg(my_codes + (long long)(step / kParts + 1) * kRpPairs);
     }
     ok = mbar_wait_warp(&full[b], (step / kRpStages) & 1, 1u);
-    ok = __syncthreads_and(ok) != 0;               // all are through with the stage that is filled next
+    // All are through with the stage that is filled next.  (Barriers of the four warps' own, asked by a fifth warp or by the first, let them drift apart and
+    // took 172 and 200 us at 1501 tokens where this takes 158.)
+    ok = __syncthreads_and(ok) != 0;
     if (!ok) break;
     if (threadIdx.x == 0 && step + kRpStages - 1 < steps) {
       fetch(ahead, step + kRpStages - 1);
@@ -332,26 +340,31 @@ using namespace px;
 extern "C" int64_t px_relpos_workspace_bytes(int64_t batch, int64_t n, int64_t c, int32_t r_max, int32_t s_max) {
   if (!relpos_sizes(batch, n, c, r_max, s_max) || !relpos_fits(c, r_max, s_max)) return 0;
   const int64_t units = relpos_units(batch, n);
-  return units * kRpPairs * 4 + relpos_blocks(units) * ((c + kRpChunk - 1) / kRpChunk) * (4 * r_max + 2 * s_max + 7) * kRpChunk * 4;
+  return relpos_blocks(units) * ((c + kRpChunk - 1) / kRpChunk) * (4 * r_max + 2 * s_max + 7) * kRpChunk * 4;
+}
+
+extern "C" int64_t px_relpos_codes_bytes(int64_t batch, int64_t n) {
+  return relpos_sizes(batch, n, 8, 0, 0) && n > 0 ? relpos_units(batch, n) * kRpPairs * 4 : 0;
 }
 
 extern "C" int32_t px_relpos_fwd(const int64_t* asym_id, const int64_t* residue_index, const int64_t* entity_id, const int64_t* token_index,
-                                 const int64_t* sym_id, const float* w, void* z, int64_t batch, int64_t n, int64_t c, int32_t r_max,
-                                 int32_t s_max, int32_t dtype, void* stream) {
+                                 const int64_t* sym_id, const float* w, void* z, uint32_t* codes, int64_t batch, int64_t n, int64_t c,
+                                 int32_t r_max, int32_t s_max, int32_t dtype, void* stream) {
   if (!relpos_sizes(batch, n, c, r_max, s_max)) return PX_ERR_BAD_ARG;
   if (!relpos_fits(c, r_max, s_max) || (dtype != PX_F32 && dtype != PX_BF16 && dtype != PX_F16)) return PX_ERR_UNSUPPORTED;
   if (batch == 0 || n == 0) return PX_OK;
-  if (!asym_id || !residue_index || !entity_id || !token_index || !sym_id || !w || !z || ((uintptr_t)z & 15)) return PX_ERR_BAD_ARG;
+  if (!asym_id || !residue_index || !entity_id || !token_index || !sym_id || !w || !z || (((uintptr_t)z | (uintptr_t)w) & 15)) return PX_ERR_BAD_ARG;
   const RelposArgs a = {(const long long*)asym_id, (const long long*)residue_index, (const long long*)entity_id, (const long long*)token_index,
                         (const long long*)sym_id, n, batch * n * n, (int)c, r_max, s_max};
-  const size_t smem = (size_t)(a.rows1() + a.rows2()) * kRpPitch * 4;
-  const int64_t strips = relpos_units(batch, n);
-  const int64_t room = sm_count() * std::max<int64_t>(1, std::min<int64_t>(4, (int64_t)(227 << 10) / (int64_t)(smem + 1024)));
-  const dim3 grid((unsigned)std::min((strips + 3) / 4, room), (unsigned)((c + kRpChunk - 1) / kRpChunk));
+  constexpr size_t kRoom = (size_t)226 << 10;
+  const size_t table = (size_t)(a.rows1() + a.rows2()) * kRpChunk * 4, row = (size_t)a.columns() * 4;
+  const int slice = (int)std::min<size_t>(kRpChunk, (kRoom - table) / row / 8 * 8);      // at least 8: see kRpMaxRows
+  // a few strips a block at least, one block an SM at most
+  const dim3 grid((unsigned)std::min<int64_t>((relpos_units(batch, n) + 3) / 4, sm_count()), (unsigned)((c + kRpChunk - 1) / kRpChunk));
   static SmemLimit limit[3];
   const auto go = [&](auto* kernel, auto* out) {
-    if (!limit[dtype].set(kernel, (size_t)kRpMaxRows * kRpPitch * 4)) return false;
-    kernel<<<grid, kRpFwdThreads, smem, (cudaStream_t)stream>>>(a, w, out);
+    if (!limit[dtype].set(kernel, kRoom)) return false;
+    kernel<<<grid, kRpFwdThreads, table + slice * row, (cudaStream_t)stream>>>(a, w, out, codes, slice);
     return cudaGetLastError() == cudaSuccess;
   };
   const bool done = dtype == PX_F32    ? go(relpos_fwd_kernel<float>, (float*)z)
@@ -360,31 +373,21 @@ extern "C" int32_t px_relpos_fwd(const int64_t* asym_id, const int64_t* residue_
   return done ? PX_OK : PX_ERR_LAUNCH;
 }
 
-extern "C" int32_t px_relpos_bwd(const int64_t* asym_id, const int64_t* residue_index, const int64_t* entity_id, const int64_t* token_index,
-                                 const int64_t* sym_id, const void* dz, float* dw, void* workspace, int64_t workspace_bytes, int64_t batch,
+extern "C" int32_t px_relpos_bwd(const uint32_t* codes, const void* dz, float* dw, void* workspace, int64_t workspace_bytes, int64_t batch,
                                  int64_t n, int64_t c, int32_t r_max, int32_t s_max, int32_t dtype, void* stream) {
   if (!relpos_sizes(batch, n, c, r_max, s_max)) return PX_ERR_BAD_ARG;
   if (!relpos_fits(c, r_max, s_max) || (dtype != PX_F32 && dtype != PX_BF16 && dtype != PX_F16)) return PX_ERR_UNSUPPORTED;
   if (!dw) return PX_ERR_BAD_ARG;
   const cudaStream_t st = (cudaStream_t)stream;
-  const RelposArgs a = {(const long long*)asym_id, (const long long*)residue_index, (const long long*)entity_id, (const long long*)token_index,
-                        (const long long*)sym_id, n, batch * n * n, (int)c, r_max, s_max};
+  const RelposArgs a = {nullptr, nullptr, nullptr, nullptr, nullptr, n, batch * n * n, (int)c, r_max, s_max};
   if (batch == 0 || n == 0)
     return cudaMemsetAsync(dw, 0, (size_t)c * a.columns() * 4, st) == cudaSuccess ? PX_OK : PX_ERR_LAUNCH;
-  if (!asym_id || !residue_index || !entity_id || !token_index || !sym_id || !dz || !workspace || ((uintptr_t)dz & 15) ||
-      ((uintptr_t)workspace & 15))
-    return PX_ERR_BAD_ARG;
+  if (!codes || !dz || !workspace || (((uintptr_t)dz | (uintptr_t)workspace) & 15)) return PX_ERR_BAD_ARG;
   if (workspace_bytes < px_relpos_workspace_bytes(batch, n, c, r_max, s_max)) return PX_ERR_WORKSPACE;
   const int64_t units = relpos_units(batch, n), most = relpos_blocks(units), per = (units + most - 1) / most;
   const int blocks = (int)((units + per - 1) / per);
   const unsigned chunks = (unsigned)((c + kRpChunk - 1) / kRpChunk);
-  const int strips = (int)(units / (batch * n));
-  uint32_t* const codes = (uint32_t*)workspace;
-  float* const partial = (float*)(codes + units * kRpPairs);
-  const int64_t code_blocks = (batch * n + 7) / 8 * strips;
-  if (code_blocks > 0x7fffffff) return PX_ERR_UNSUPPORTED;
-  relpos_code_kernel<<<(unsigned)code_blocks, 256, 0, st>>>(a, strips, codes);
-  if (cudaGetLastError() != cudaSuccess) return PX_ERR_LAUNCH;
+  float* const partial = (float*)workspace;
   const size_t fixed = (size_t)kRpStages * kRpStageBytes, smem = fixed + (size_t)(a.rows1() + a.rows2()) * kRpChunk * 4;
   static SmemLimit limit[3];
   const auto go = [&](auto* kernel, auto* in) {

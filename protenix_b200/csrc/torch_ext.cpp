@@ -61,7 +61,7 @@ constexpr int64_t kCz = 128, kCs = 384, kHeadsSingle = 16, kHeads = 4, kHeadDim 
   X(px_single_workspace_bytes) X(px_single_prepare) X(px_single_project) X(px_single_finish) X(px_opm_outer)             \
   X(px_opm_out) X(px_msa_opm_prep) X(px_msa_values) X(px_msa_weights) X(px_msa_average) X(px_msa_gate_out)               \
   X(px_msa_rows_weights_bytes) X(px_msa_rows_prepare) X(px_msa_transition_weights_bytes) X(px_msa_transition_prepare) X(px_msa_transition) \
-  X(px_dropout_add) X(px_relpos_workspace_bytes) X(px_relpos_fwd) X(px_relpos_bwd) X(px_window_lse_floats) \
+  X(px_dropout_add) X(px_relpos_codes_bytes) X(px_relpos_workspace_bytes) X(px_relpos_fwd) X(px_relpos_bwd) X(px_window_lse_floats) \
   X(px_window_fwd) X(px_window_workspace_bytes) X(px_window_bwd)
 struct Abi {
 #define X(f) decltype(&::f) f = nullptr;

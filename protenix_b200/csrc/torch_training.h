@@ -100,47 +100,47 @@ struct RelposSizes {
 };
 
 typedef std::vector<Tensor> Features;      // asym, residue, entity, token, copy numbers: int64, contiguous
-struct FeatureData {
-  const int64_t* p[5];
-  explicit FeatureData(const Tensor* f) {
-    for (int i = 0; i < 5; ++i) p[i] = (const int64_t*)f[i].data_ptr();
-  }
-};
+
+// codes: receives the buckets of the pairs, for the backward pass (NULL: not wanted)
+Tensor relpos_forward(const Tensor& weight, const Features& f, const RelposSizes& z, Tensor* codes) {
+  const Tensor w = aligned(weight.scalar_type() == at::kFloat ? weight : weight.to(at::kFloat));
+  const Tensor out = at::empty({z.batch, z.n, z.n, z.c}, w.options().dtype((at::ScalarType)z.type));
+  if (codes) *codes = bytes_like(w, abi.px_relpos_codes_bytes(z.batch, z.n));
+  const int64_t* id[5];
+  for (int i = 0; i < 5; ++i) id[i] = (const int64_t*)f[i].data_ptr();
+  const cudaStream_t st = at::cuda::getCurrentCUDAStream();
+  launch("px_relpos_fwd", st, [&] {
+    return abi.px_relpos_fwd(id[0], id[1], id[2], id[3], id[4], (const float*)w.data_ptr(), out.data_ptr(),
+                             codes ? (uint32_t*)codes->data_ptr() : nullptr, z.batch, z.n, z.c, (int32_t)z.r, (int32_t)z.s,
+                             dtype_code(out, "dtype"), st);
+  });
+  return out;
+}
 
 struct RelposFunction : torch::autograd::Function<RelposFunction> {
   static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& weight, const Features& f, int64_t batch, int64_t n, int64_t r,
                         int64_t s, int64_t type) {
-    ctx->save_for_backward({f[0], f[1], f[2], f[3], f[4]});
+    Tensor codes;
+    const Tensor z = relpos_forward(weight, f, {batch, n, weight.size(0), r, s, type}, &codes);
+    ctx->save_for_backward({codes});
     ctx->saved_data["sizes"] = c10::List<int64_t>({batch, n, weight.size(0), r, s, (int64_t)weight.scalar_type()});
-    return run(weight, f, {batch, n, weight.size(0), r, s, type});
-  }
-  static Tensor run(const Tensor& weight, const Features& f, const RelposSizes& z) {
-    const Tensor w = weight.scalar_type() == at::kFloat && weight.is_contiguous() ? weight : weight.detach().to(at::kFloat).contiguous();
-    const Tensor out = at::empty({z.batch, z.n, z.n, z.c}, w.options().dtype((at::ScalarType)z.type));
-    const FeatureData d(f.data());
-    const cudaStream_t st = at::cuda::getCurrentCUDAStream();
-    launch("px_relpos_fwd", st, [&] {
-      return abi.px_relpos_fwd(d.p[0], d.p[1], d.p[2], d.p[3], d.p[4], (const float*)w.data_ptr(), out.data_ptr(), z.batch, z.n, z.c,
-                               (int32_t)z.r, (int32_t)z.s, dtype_code(out, "dtype"), st);
-    });
-    return out;
+    return z;
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     first_derivative_only("relative_position_encoding");
-    const auto f = ctx->get_saved_variables();
+    const Tensor codes = ctx->get_saved_variables()[0];
     const auto v = ctx->saved_data["sizes"].toIntVector();
-    c10::cuda::CUDAGuard guard(f[0].device());
+    c10::cuda::CUDAGuard guard(codes.device());
     const Tensor dz = aligned(grads[0]);
     const int64_t batch = v[0], n = v[1], c = v[2];
     const int32_t r = (int32_t)v[3], s = (int32_t)v[4];
     const Tensor dw = at::empty({c, 4 * r + 2 * s + 7}, dz.options().dtype(at::kFloat));
     const int64_t bytes = abi.px_relpos_workspace_bytes(batch, n, c, r, s);
     const Tensor ws = bytes_like(dz, bytes);
-    const FeatureData d(f.data());
     const cudaStream_t st = at::cuda::getCurrentCUDAStream();
     launch("px_relpos_bwd", st, [&] {
-      return abi.px_relpos_bwd(d.p[0], d.p[1], d.p[2], d.p[3], d.p[4], dz.data_ptr(), (float*)dw.data_ptr(), ws.data_ptr(), bytes, batch, n, c,
-                               r, s, dtype_code(dz, "the gradient"), st);
+      return abi.px_relpos_bwd((const uint32_t*)codes.data_ptr(), dz.data_ptr(), (float*)dw.data_ptr(), ws.data_ptr(), bytes, batch, n, c, r, s,
+                               dtype_code(dz, "the gradient"), st);
     });
     return {dw.to((at::ScalarType)v[5]), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
   }
@@ -172,7 +172,7 @@ Tensor relative_position_encoding(const Tensor& weight, const std::vector<Tensor
   const int64_t type = (int64_t)(z_type.has_value() ? *z_type : weight.scalar_type());
   if (type != (int64_t)at::kFloat && type != (int64_t)at::kBFloat16 && type != (int64_t)at::kHalf) fail("dtype must be float32, bfloat16 or float16");
   const Tensor z = at::GradMode::is_enabled() && weight.requires_grad() ? RelposFunction::apply(weight, rows, batch, n, r, s, type)
-                                                                        : RelposFunction::run(weight, rows, {batch, n, weight.size(0), r, s, type});
+                                                                        : relpos_forward(weight, rows, {batch, n, weight.size(0), r, s, type}, nullptr);
   return z.view(shape);
 }
 
