@@ -8,7 +8,7 @@
 namespace px {
 
 constexpr int kWRows = 128;      // rows a CTA owns: queries (forward, dQ) or keys (dK, dV)
-constexpr int kWCols = 64;       // keys or queries of a streamed tile
+constexpr int kWCols = 64;       // keys or queries of a streamed tile of the backward pass
 constexpr int kWMaxR = 256;      // largest clipping distance of the learned bias
 
 // A call, as the kernels see it.  left, right and sinks are at most n.
@@ -43,53 +43,53 @@ __device__ __forceinline__ void mma_rows(uint32_t d_tmem, uint32_t a, uint32_t b
     umma_bf16(d_tmem, umma_desc_sw128(a + panel * (kWRows * 128)) + at, umma_desc_sw128(b + panel * b_rows * 128) + at, idesc, ks > 0);
   }
 }
-// D[128][d] += A[128][kWCols] B with A in tensor memory and B the streamed tile [kWCols][d], read along its rows (one lane).
+// D[128][d] += A[128][kKT] B with A in tensor memory and B the streamed tile [kKT][d], read along its rows (one lane).
+template <int kKT>
 __device__ __forceinline__ void mma_streamed(uint32_t d_tmem, uint32_t a_tmem, uint32_t b, uint32_t idesc, bool first) {
 #pragma unroll
-  for (int ks = 0; ks < kWCols / 16; ++ks)
-    umma_bf16_ts(d_tmem, a_tmem + 8 * ks, umma_desc_mn_sw128(b + ks * 2048, kWCols * 128, 1024), idesc, !first || ks > 0);
+  for (int ks = 0; ks < kKT / 16; ++ks)
+    umma_bf16_ts(d_tmem, a_tmem + 8 * ks, umma_desc_mn_sw128(b + ks * 2048, kKT * 128, 1024), idesc, !first || ks > 0);
 }
 
 // Streamed key tiles of the queries [q0, q0 + 128): the first tiles as far as they hold sinks, then those of the window.
+template <int kKT>
 struct KeyTiles {
   int sink, first, count;
   __device__ __forceinline__ KeyTiles(const WindowArgs& a, int q0) {
     const int lo = max(0, q0 - a.left), hi = min(a.n - 1, q0 + kWRows - 1 + a.right);
-    first = lo / kWCols;
-    sink = min((a.sinks + kWCols - 1) / kWCols, first);
-    count = sink + hi / kWCols - first + 1;
+    first = lo / kKT;
+    sink = min((a.sinks + kKT - 1) / kKT, first);
+    count = sink + hi / kKT - first + 1;
   }
-  __device__ __forceinline__ int key(int t) const { return (t < sink ? t : first + t - sink) * kWCols; }
+  __device__ __forceinline__ int key(int t) const { return (t < sink ? t : first + t - sink) * kKT; }
 };
 
-__device__ __forceinline__ uint64_t bits_between(int from, int to) {     // bits from .. to, both cut to 0 .. 63
-  from = max(from, 0), to = min(to, 63);
-  return from > to ? 0ull : (~0ull << from) & (~0ull >> (63 - to));
+// Bits from .. to of a word, both cut to 0 .. 31.
+__device__ __forceinline__ uint32_t bits_between(int from, int to) {
+  from = max(from, 0), to = min(to, 31);
+  return from > to ? 0u : (0xffffffffu << from) & (0xffffffffu >> (31 - to));
 }
 // Bit c: key k0 + c exists and is not masked (whole warp).
-__device__ __forceinline__ uint64_t key_bits(const WindowArgs& a, int batch, int k0, int lane) {
-  uint64_t w = bits_between(0, a.n - 1 - k0);
-  if (a.mask) {
-    const uint8_t* m = a.mask + (size_t)batch * a.n + k0;
-    const unsigned lo = __ballot_sync(0xffffffffu, k0 + lane < a.n && __ldg(m + min(lane, a.n - 1 - k0)) != 0);
-    const unsigned hi = __ballot_sync(0xffffffffu, k0 + 32 + lane < a.n && __ldg(m + min(32 + lane, a.n - 1 - k0)) != 0);
-    w = (uint64_t)hi << 32 | lo;
-  }
-  return w;
-}
-// Whether the queries [q0, q0 + 128) see all of the keys [k0, k0 + 64), as far as the window goes.
-__device__ __forceinline__ bool window_covers(const WindowArgs& a, int q0, int k0) {
-  return k0 + kWCols - 1 <= q0 + a.right && (k0 >= q0 + kWRows - 1 - a.left || k0 + kWCols <= a.sinks);
+__device__ __forceinline__ uint32_t key_bits(const WindowArgs& a, int batch, int k0, int lane) {
+  if (!a.mask) return bits_between(0, a.n - 1 - k0);
+  return __ballot_sync(0xffffffffu, k0 + lane < a.n && __ldg(a.mask + (size_t)batch * a.n + min(k0 + lane, a.n - 1)) != 0);
 }
 // Bit c: query i sees key k0 + c.
-__device__ __forceinline__ uint64_t visible_bits(const WindowArgs& a, int i, int k0, uint64_t keys) {
+__device__ __forceinline__ uint32_t visible_bits(const WindowArgs& a, int i, int k0, uint32_t keys) {
   const int hi = i + a.right - k0;
   return (bits_between(i - a.left - k0, hi) | bits_between(0, min(a.sinks - 1 - k0, hi))) & keys;
 }
+// What a block of 32 queries from q0 and 32 keys from k0 is, as far as the window goes: out of sight, or seen by all of the queries.
+__device__ __forceinline__ bool block_dead(const WindowArgs& a, int q0, int k0) {
+  return k0 > q0 + 31 + a.right || (k0 + 31 < q0 - a.left && k0 >= a.sinks);
+}
+__device__ __forceinline__ bool block_whole(const WindowArgs& a, int q0, int k0) {
+  return k0 + 31 <= q0 + a.right && (k0 >= q0 + 31 - a.left || k0 + 32 <= a.sinks);
+}
 
-// The learned bias of one head times log2(e), by offset j - i and continued beyond +-r far enough that every offset of a tile that reaches into
-// (-r, r) has its place: at(offset) for |offset| < r + kWRows + kWCols.
-constexpr int kWBiasBeyond = kWRows + kWCols;
+// The learned bias of one head times log2(e), by offset j - i and continued beyond +-r far enough that every offset of a block of 32 x 32 that reaches
+// into (-r, r) has its place.
+constexpr int kWBiasBeyond = 64;
 __host__ __device__ constexpr int bias_floats(int r) { return r < 0 ? 0 : 2 * r + 1 + 2 * kWBiasBeyond; }
 __device__ __forceinline__ float bias_value(const WindowArgs& a, int head, int bucket) {
   const size_t at = (size_t)head * (2 * a.r + 1) + bucket;
@@ -101,18 +101,46 @@ __device__ __forceinline__ float bias_value(const WindowArgs& a, int head, int b
 __device__ __forceinline__ void bias_fill(const WindowArgs& a, int head, float* to) {
   for (int k = threadIdx.x; k < bias_floats(a.r); k += blockDim.x) to[k] = bias_value(a, head, min(max(k - kWBiasBeyond, 0), 2 * a.r));
 }
-// Whether offsets lowest .. highest are all clipped, and to which side.
-__device__ __forceinline__ bool clipped_low(const WindowArgs& a, int highest) { return highest <= -a.r; }
-__device__ __forceinline__ bool clipped_high(const WindowArgs& a, int lowest) { return lowest >= a.r; }
+// How the bias meets a block of 32 queries from q0 and 32 keys from k0: `near`, by offset; otherwise one number, `flat` (the offsets are all clipped
+// to the same side, or there is no bias).
+struct BlockBias {
+  bool near, low;
+  float flat;
+  __device__ __forceinline__ BlockBias(const WindowArgs& a, const float* bias, int q0, int k0) {
+    low = k0 + 31 - q0 <= -a.r;
+    const bool high = k0 - q0 - 31 >= a.r;
+    near = a.r >= 0 && !low && !high;
+    flat = a.r < 0 ? 0.f : low ? bias[0] : bias[2 * a.r + 2 * kWBiasBeyond];
+  }
+};
+// The values of row i (query) from key k0 on: [0], [1], ...
+__device__ __forceinline__ const float* bias_row(const WindowArgs& a, const float* bias, int i, int k0) {
+  return bias + (k0 - i + a.r + kWBiasBeyond);
+}
 
-// Row `row` of a streamed tile in shared memory becomes zeros (its `half` of the 128 bytes of each panel).  What a product weights with zero must be
-// finite: masked keys and rows that see nothing may hold anything.
-template <int kPanels>
+// Row `row` of a streamed tile of kKT rows in shared memory becomes zeros (part `part` of the 128 bytes of each panel).  What a product weights with
+// zero must be finite: masked keys and rows that see nothing may hold anything.
+template <int kPanels, int kKT>
 __device__ __forceinline__ void clear_row(unsigned char* tile, int row, int part, int parts) {
 #pragma unroll
   for (int p = 0; p < kPanels; ++p)
     for (int k = part * (8 / parts); k < (part + 1) * (8 / parts); ++k)
-      *reinterpret_cast<uint4*>(tile + p * kWCols * 128 + row * 128 + k * 16) = make_uint4(0u, 0u, 0u, 0u);
+      *reinterpret_cast<uint4*>(tile + p * kKT * 128 + row * 128 + k * 16) = make_uint4(0u, 0u, 0u, 0u);
+}
+__device__ __forceinline__ float max3f(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float max32(const float* s) {
+  float m[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    m[k] = max3f(s[8 * k], s[8 * k + 1], s[8 * k + 2]);
+    m[k] = max3f(m[k], s[8 * k + 3], s[8 * k + 4]);
+    m[k] = max3f(m[k], s[8 * k + 5], s[8 * k + 6]);
+  }
+  return max3f(max3f(m[0], m[1], s[7]), max3f(m[2], m[3], s[15]), fmaxf(s[23], s[31]));
 }
 // Barrier of `threads` threads that tells whether `ok` held for all: they leave a loop together after one of their waits ran out.
 __device__ __forceinline__ bool barrier_all(int id, int threads, bool ok) {

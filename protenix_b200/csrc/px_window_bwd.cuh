@@ -19,8 +19,8 @@ namespace px {
 constexpr int kWBwdThreads = 288;
 
 struct WindowBwdArgs {
-  const float* lse;              // [batch * heads][npad], base 2; +inf for rows that see nothing and beyond the last
-  float* delta;                  // the same shape
+  const float* nlse;             // [batch * heads][npad], base 2, negative; -inf for rows that see nothing and beyond the last
+  float* ndelta;                 // -delta, the same shape
   float* dbias;                  // partial sums [batch * heads * tiles][2 r + 1] or NULL
   float* sinks;                  // partial sums [batch * kv_heads][sink_tiles][1 + chunks][2][128][dn] (dK, dV)
   float scale;
@@ -28,29 +28,34 @@ struct WindowBwdArgs {
 };
 
 struct WindowBwdBars {
-  uint64_t own_full, first_full[2], second_full[2], ready, given, done;      // streamed operands; S and dP; P and dS; the products with them
+  // streamed operands; S and dP, complete and in registers; P and dS; the products with them
+  uint64_t own_full, first_full[2], second_full[2], ready, taken, given, done;
   uint32_t tmem_base;
 };
 
 // ---- dQ, delta, dbias ------------------------------------------------------------------------------------------------
-// TMEM: S (64) | dP (64) | dQ (64 or 128); dS in the place of S.
-template <int kPanels>
+// TMEM: S (64) | dP (64) | dS (32) | dQ (64): the next S and dP are made while this dS is.  Heads beyond 64: S | dP | dQ (128), dS in the place of S.
+// kD: the head size that there is room for, 64 or 128.
+template <int kD>
 struct WindowDqLayout {
-  static constexpr int stages = kPanels == 1 ? 2 : 1, tile = kPanels * kWCols * 128;
-  static constexpr int q = 0, dout = kPanels * kWRows * 128, k = 2 * dout, v = k + stages * tile, bars = v + stages * tile;
+  static constexpr int panels = kD / 64, stages = kD == 64 ? 2 : 1, tile = panels * kWCols * 128;
+  static constexpr bool ahead = kD == 64;
+  static constexpr int cols = 256, col_ds = ahead ? 2 * kWCols : 0, col_q = ahead ? 2 * kWCols + kWCols / 2 : 2 * kWCols;
+  static_assert(col_q + kD <= cols, "tensor memory of a CTA");
+  static constexpr int q = 0, dout = panels * kWRows * 128, k = 2 * dout, v = k + stages * tile, bars = v + stages * tile;
   static constexpr int part = bars + 128, bias = part + 2 * kWRows * 4;
   static constexpr int bytes(int r, bool grad) { return bias + bias_floats(r) * 4 * (grad ? 9 : 1) + (grad ? 8 * 32 * 4 : 0); }
 };
 static_assert(sizeof(WindowBwdBars) <= 128, "room for the barriers");
 
-template <bool kF16, int kPanels, bool kBiasGrad>
+template <bool kF16, int kD, bool kBiasGrad>
 __global__ void __launch_bounds__(kWBwdThreads, 2)
 window_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do, const __grid_constant__ CUtensorMap map_k,
                  const __grid_constant__ CUtensorMap map_v, const WindowArgs a, const WindowBwdArgs g, const RowsOut dout, const RowsOut o,
                  const RowsOut dq) {
-  typedef WindowDqLayout<kPanels> L;
-  constexpr uint32_t kCols = 256;
-  constexpr int kStages = L::stages;
+  typedef WindowDqLayout<kD> L;
+  constexpr uint32_t kCols = L::cols;
+  constexpr int kStages = L::stages, kPanels = L::panels;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* sm = smem_aligned(smem_raw);
   WindowBwdBars& bars = *reinterpret_cast<WindowBwdBars*>(sm + L::bars);
@@ -58,7 +63,7 @@ window_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   float* const bias = reinterpret_cast<float*>(sm + L::bias);
   const int warp = warp_index(), lane = threadIdx.x & 31;
   const int q0 = (int)(blockIdx.x % a.tiles) * kWRows, bh = blockIdx.x / a.tiles, head = bh % a.heads, batch = bh / a.heads;
-  const KeyTiles tiles(a, q0);
+  const KeyTiles<kWCols> tiles(a, q0);
 
   const bool skip = cta_begin();
   if (threadIdx.x == 0) {
@@ -69,6 +74,7 @@ window_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       mbar_init(&bars.second_full[s], 1);
     }
     mbar_init(&bars.ready, 1);
+    mbar_init(&bars.taken, 8);
     mbar_init(&bars.given, 8);
     mbar_init(&bars.done, 1);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
@@ -81,8 +87,8 @@ window_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     bias_fill(a, head, bias);
     if (kBiasGrad)
       for (int k = threadIdx.x; k < 8 * ext; k += kWBwdThreads) bias[ext + k] = 0.f;
+    __syncthreads();
   }
-  __syncthreads();
 
   float low = 0.f, high = 0.f;                     // sums of dS over offsets that are clipped
   if (warp == 8) {
@@ -120,24 +126,38 @@ window_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     __syncwarp();
     bool ok = mbar_wait_warp(&bars.own_full, 0, 1u) && issue(0);
     for (int t = 0; t < tiles.count && ok; ++t) {
-      ok = mbar_wait_warp(&bars.given, t & 1, 8u);            // dS(t) is there; S(t) and dP(t) are complete: V's tile is free
+      ok = mbar_wait_warp(&bars.taken, t & 1, 8u);            // S(t) and dP(t) are complete and in registers: V's tile is free
+      if (!ok) break;
+      if (t + kStages < tiles.count && elect_lane()) load(t + kStages, bars.second_full, &map_v, v_at);
+      __syncwarp();
+      if (L::ahead) {
+        if (t > 0 && t + 1 < tiles.count) {                   // K's tile of the step before is free
+          ok = mbar_wait_warp(&bars.done, (t - 1) & 1, 16u);
+          if (!ok) break;
+          if (elect_lane()) load(t + 1, bars.first_full, &map_k, k_at);
+          __syncwarp();
+        }
+        if (t + 1 < tiles.count && !(ok = issue(t + 1))) break;
+      }
+      ok = mbar_wait_warp(&bars.given, t & 1, 8u);
       if (!ok) break;
       tc_fence_after();
       if (elect_lane()) {
-        mma_streamed(tmem + 2 * kWCols, tmem, k_at + (t % kStages) * L::tile, idesc_q, t == 0);
+        mma_streamed<kWCols>(tmem + L::col_q, tmem + L::col_ds, k_at + (t % kStages) * L::tile, idesc_q, t == 0);
         umma_commit(&bars.done);
-        if (t + kStages < tiles.count) load(t + kStages, bars.second_full, &map_v, v_at);
       }
       __syncwarp();
-      ok = mbar_wait_warp(&bars.done, t & 1, 16u);            // K's tile and the place of S are free
-      if (!ok) break;
-      if (t + kStages < tiles.count && elect_lane()) load(t + kStages, bars.first_full, &map_k, k_at);
-      __syncwarp();
-      if (t + 1 < tiles.count) ok = issue(t + 1);
+      if (!L::ahead) {
+        ok = mbar_wait_warp(&bars.done, t & 1, 16u);          // K's tile and the place of S are free
+        if (!ok) break;
+        if (t + 1 < tiles.count && elect_lane()) load(t + 1, bars.first_full, &map_k, k_at);
+        __syncwarp();
+        if (t + 1 < tiles.count) ok = issue(t + 1);
+      }
     }
   } else {
     // ------------------------------------------------------------------ one query row x 32 keys a thread
-    const int quarter = warp & 3, half = warp >> 2, row = 32 * quarter + lane, i = q0 + row;
+    const int quarter = warp & 3, half = warp >> 2, row = 32 * quarter + lane, i = q0 + row, qw = q0 + 32 * quarter;
     const uint32_t t_lane = tmem + ((uint32_t)(32 * quarter) << 16);
     // delta = dO . O, each thread over its half of the 16-byte pieces of the row
     float sum = 0.f;
@@ -155,63 +175,82 @@ window_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     }
     part[half * kWRows + row] = sum;
     asm volatile("bar.sync 1, 256;\n" ::: "memory");
-    const float delta = part[row] + part[kWRows + row];
-    if (half == 0) g.delta[(size_t)bh * a.npad + i] = delta;      // 0 beyond the last row
-    const float lse = g.lse[(size_t)bh * a.npad + i];
+    const float ndelta = -(part[row] + part[kWRows + row]);
+    if (half == 0) g.ndelta[(size_t)bh * a.npad + i] = ndelta;      // 0 beyond the last row
+    const float nlse = g.nlse[(size_t)bh * a.npad + i];
     float* const sums = bias + ext * (1 + warp);                   // by offset, as the bias lies
     float* const stage = bias + ext * 9 + 32 * warp;
     bool ok = true;
     for (int t = 0; t < tiles.count; ++t) {
       const int k0 = tiles.key(t), kh = k0 + 32 * half;
-      const uint64_t keys = key_bits(a, batch, k0, lane);
-      const bool whole = keys == ~0ull && window_covers(a, q0, k0);
+      const uint32_t keys = key_bits(a, batch, kh, lane);
+      const bool dead = keys == 0 || block_dead(a, qw, kh);
+      // masked keys of the tile: their rows of K become zeros, those of this half by its four warps
+      const bool hidden = keys != bits_between(0, a.n - 1 - kh);
       ok = mbar_wait(&bars.ready, t & 1, 32u);
       __syncwarp();
       tc_fence_after();
       float s[32], d[32];
-      tmem_ld32(t_lane + 32 * half, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
-      tmem_ld32(t_lane + kWCols + 32 * half, *reinterpret_cast<uint32_t(*)[32]>(&d[0]));
-      tmem_wait_ld();
-      // all of S has to be read before any of dS goes where it lies
+      uint32_t w[16];
+      if (!dead) {
+        tmem_ld32(t_lane + 32 * half, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
+        tmem_ld32(t_lane + kWCols + 32 * half, *reinterpret_cast<uint32_t(*)[32]>(&d[0]));
+        tmem_wait_ld();
+      }
       tc_fence_before();
-      ok = barrier_all(2 + quarter, 64, ok);
+      // where dS goes to the place of S, all of S has to be read before
+      ok = L::ahead ? __all_sync(0xffffffffu, ok) != 0 : barrier_all(2 + quarter, 64, ok);
       if (!ok) break;
-      tc_fence_after();
-      const int lowest = kh - (q0 + 32 * quarter + 31), highest = kh + 31 - (q0 + 32 * quarter);      // offsets of this warp's block
-      const bool flat_low = a.r >= 0 && clipped_low(a, highest), flat_high = a.r >= 0 && clipped_high(a, lowest);
-      const bool near = a.r >= 0 && !flat_low && !flat_high;
-      const float shift = (flat_low ? bias[0] : flat_high ? bias[ext - 1] : 0.f) - lse;
-      if (near) {
-        const float* b = bias + (kh - i + a.r + kWBiasBeyond);
+      if (lane == 0) mbar_arrive(&bars.taken);
+      const BlockBias bb(a, bias, qw, kh);
+      if (!dead) {
+        const float shift = nlse + bb.flat;
+        if (bb.near) {
+          const float* const y = bias_row(a, bias, i, kh);
 #pragma unroll
-        for (int c = 0; c < 32; ++c) s[c] = fast_exp2(fmaf(s[c], a.c, shift + b[c]));
+          for (int c = 0; c < 32; c += 2) {
+            float y0 = y[c], y1 = y[c + 1];
+            add2(y0, y1, nlse, nlse);
+            fma2(s[c], s[c + 1], s[c], s[c + 1], a.c, a.c, y0, y1);
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < 32; c += 2) fma2(s[c], s[c + 1], s[c], s[c + 1], a.c, a.c, shift, shift);
+        }
+#pragma unroll
+        for (int c = 0; c < 32; c += 2) {
+          add2(d[c], d[c + 1], ndelta, ndelta);
+          mul2(d[c], d[c + 1], fast_exp2(s[c]), fast_exp2(s[c + 1]));
+        }
+        if (keys != 0xffffffffu || !block_whole(a, qw, kh)) {
+          const uint32_t seen = visible_bits(a, i, kh, keys);
+#pragma unroll
+          for (int c = 0; c < 32; ++c) d[c] = (seen >> c & 1u) ? d[c] : 0.f;
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) w[e] = pack16x2<kF16>(d[2 * e], d[2 * e + 1]);
       } else {
 #pragma unroll
-        for (int c = 0; c < 32; ++c) s[c] = fast_exp2(fmaf(s[c], a.c, shift));
+        for (int e = 0; e < 16; ++e) w[e] = 0u;
       }
-#pragma unroll
-      for (int c = 0; c < 32; ++c) d[c] = s[c] * (d[c] - delta);
-      if (!whole) {
-        const uint32_t seen = (uint32_t)(visible_bits(a, i, k0, keys) >> (32 * half));
-#pragma unroll
-        for (int c = 0; c < 32; ++c) d[c] = (seen >> c & 1u) ? d[c] : 0.f;
+      if (L::ahead && t > 0) {                      // the product before has read its dS
+        ok = mbar_wait(&bars.done, (t - 1) & 1, 64u);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
       }
-      uint32_t w[16];
-#pragma unroll
-      for (int e = 0; e < 16; ++e) w[e] = pack16x2<kF16>(d[2 * e], d[2 * e + 1]);
-      tmem_st16(t_lane + 16 * half, w);
-      if (keys != bits_between(0, a.n - 1 - k0)) {  // masked keys: their rows of K
+      tc_fence_after();
+      tmem_st16(t_lane + L::col_ds + 16 * half, w);
+      if (hidden) {
         mbar_wait(&bars.first_full[t % kStages], (t / kStages) & 1, 128u);      // complete: S(t) is; orders these writes behind the copy's
-        const int r64 = threadIdx.x & 63;
-        if (!(keys >> r64 & 1)) clear_row<kPanels>(sm + L::k + (t % kStages) * L::tile, r64, threadIdx.x >> 6, 4);
+        if (!(keys >> lane & 1)) clear_row<kPanels, kWCols>(sm + L::k + (t % kStages) * L::tile, 32 * half + lane, quarter, 4);
         fence_async_shared();
       }
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars.given);
-      if (kBiasGrad) {
-        if (near) {
+      if (kBiasGrad && !dead) {
+        if (bb.near) {
           // Sums along the diagonals of a 32 x 32 block: the running sum moves one lane on with each column, and leaves by the last lane.
           float run = 0.f;
 #pragma unroll
@@ -221,17 +260,17 @@ window_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             if (lane == 31) stage[c] = run;         // offset c - 31 of the block is complete
           }
           __syncwarp();
-          float* const at = sums + (kh - (q0 + 32 * quarter) + a.r + kWBiasBeyond);
+          float* const at = sums + (kh - qw + a.r + kWBiasBeyond);
           at[lane - 31] += stage[lane];
           __syncwarp();
           if (lane < 31) at[31 - lane] += run;
           __syncwarp();
         } else {
-          float v = 0.f;
+          float v0 = 0.f, v1 = 0.f;
 #pragma unroll
-          for (int c = 0; c < 32; ++c) v += d[c];
-          if (flat_low) low += v;
-          else high += v;
+          for (int c = 0; c < 32; c += 2) add2(v0, v1, d[c], d[c + 1]);
+          if (bb.low) low += v0 + v1;
+          else high += v0 + v1;
         }
       }
     }
@@ -242,7 +281,7 @@ window_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       uint16_t* const out = dq.at(batch, head, i);
       for (int c = 16 * half; c < a.d; c += 32) {
         uint32_t x[16];
-        tmem_ld16(t_lane + 2 * kWCols + c, x);
+        tmem_ld16(t_lane + L::col_q + c, x);
         tmem_wait_ld();
         if (i < a.n) {
           store8<kF16>(out + c, x, g.scale);
@@ -266,19 +305,26 @@ window_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     float* const out = g.dbias + (size_t)blockIdx.x * (2 * a.r + 1);
     for (int b = threadIdx.x; b < 2 * a.r + 1; b += kWBwdThreads) {
       float v = 0.f;
-      for (int k = 0; k < 8; ++k) {
-        const float* const s = bias + ext * (1 + k);
-        v += s[b + kWBiasBeyond];
-        if (b == 0) {
-          for (int e = 0; e < kWBiasBeyond; ++e) v += s[e];
-          v += part[k];
-        }
-        if (b == 2 * a.r) {
-          for (int e = b + kWBiasBeyond + 1; e < ext; ++e) v += s[e];
-          v += part[8 + k];
-        }
-      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v += bias[ext * (1 + k) + b + kWBiasBeyond];
       out[b] = v;
+    }
+    // the two ends: what lies beyond them, a warp each
+    if (warp < 2) {
+      __syncwarp();
+      float v = 0.f;
+      for (int k = 0; k < 8; ++k) {
+        const float* const s = bias + ext * (1 + k) + (warp == 0 ? 0 : 2 * a.r + 1 + kWBiasBeyond);
+        for (int e = lane; e < kWBiasBeyond; e += 32) v += s[e];
+        if (lane == k) v += part[8 * warp + k];
+      }
+      v = warp_sum(v);
+      if (lane == 0) part[32 + warp] = v;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      out[0] += part[32];
+      out[2 * a.r] += part[33];
     }
   }
 }
@@ -306,11 +352,17 @@ __global__ void __launch_bounds__(1024) window_dbias_kernel(const float* __restr
 }
 
 // ---- dK, dV ----------------------------------------------------------------------------------------------------------
-// TMEM: S^T (64) | dP^T (64) | dV | dK (64 or 128 each); P^T and dS^T in the places of S^T and dP^T.
-template <int kPanels>
+// TMEM, heads up to 32: S^T (64) | dP^T (64) | P^T (32) | dS^T (32) | dV (32) | dK (32), two CTAs an SM; beyond 64 the same with dV and dK of 128 and one CTA.
+// The next S^T and dP^T are made while these P^T and dS^T are.  Heads of 33 to 64: S^T | dP^T | dV (64) | dK (64), P^T and dS^T in the places of S^T and dP^T.
+template <int kD>
 struct WindowDkvLayout {
-  static constexpr int tile = kPanels * kWCols * 128, stat = 2 * kWCols * 4;
-  static constexpr int k = 0, v = kPanels * kWRows * 128, q = 2 * v, dout = q + 2 * tile, stats = dout + 2 * tile, bars = stats + 2 * stat;
+  static constexpr int panels = kD > 64 ? 2 : 1, tile = panels * kWCols * 128, stat = 2 * kWCols * 4;
+  static constexpr bool ahead = kD != 64;
+  static constexpr int cols = kD == 128 ? 512 : 256, ctas = kD == 128 ? 1 : 2;
+  static constexpr int col_p = ahead ? 2 * kWCols : 0, col_ds = ahead ? col_p + kWCols / 2 : kWCols;
+  static constexpr int col_v = ahead ? 3 * kWCols : 2 * kWCols, col_k = col_v + kD;
+  static_assert(col_k + kD <= cols, "tensor memory of a CTA");
+  static constexpr int k = 0, v = panels * kWRows * 128, q = 2 * v, dout = q + 2 * tile, stats = dout + 2 * tile, bars = stats + 2 * stat;
   static constexpr int bias = bars + 128;
   static constexpr int bytes(int r) { return bias + bias_floats(r) * 4; }
 };
@@ -318,20 +370,25 @@ struct WindowDkvLayout {
 // The queries of one CTA: streamed tiles first .. first + count - 1 of `per` a head, over the heads of the group.
 struct QueryTiles {
   int first, per, begin, count;      // begin: the first of the items head-of-group * per + tile
-  __device__ __forceinline__ int query(int it) const { return (first + (begin + it) % per) * kWCols; }
-  __device__ __forceinline__ int member(int it) const { return (begin + it) / per; }
+};
+struct QueryItem {                   // one of them, stepped along
+  int tile, member;
+  __device__ __forceinline__ explicit QueryItem(const QueryTiles& t) : tile(t.begin % t.per), member(t.begin / t.per) {}
+  __device__ __forceinline__ void next(const QueryTiles& t) {
+    if (++tile == t.per) tile = 0, ++member;
+  }
 };
 __host__ __device__ __forceinline__ int last_of_window(int n, int left, int k0) {      // last streamed tile of the window of 128 keys
   return (k0 + kWRows - 1 + left < n - 1 ? k0 + kWRows - 1 + left : n - 1) / kWCols;
 }
 
-template <bool kF16, int kPanels>
-__global__ void __launch_bounds__(kWBwdThreads, kPanels == 1 ? 2 : 1)
+template <bool kF16, int kD>
+__global__ void __launch_bounds__(kWBwdThreads, WindowDkvLayout<kD>::ctas)
 window_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do, const __grid_constant__ CUtensorMap map_k,
                   const __grid_constant__ CUtensorMap map_v, const WindowArgs a, const WindowBwdArgs g, const RowsOut dk, const RowsOut dv) {
-  typedef WindowDkvLayout<kPanels> L;
-  constexpr uint32_t kCols = kPanels == 1 ? 256 : 512;
-  constexpr int kAcc = 64 * kPanels;             // columns of an accumulator
+  typedef WindowDkvLayout<kD> L;
+  constexpr uint32_t kCols = L::cols;
+  constexpr int kPanels = L::panels;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* sm = smem_aligned(smem_raw);
   WindowBwdBars& bars = *reinterpret_cast<WindowBwdBars*>(sm + L::bars);
@@ -364,6 +421,7 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       mbar_init(&bars.second_full[s], 1);
     }
     mbar_init(&bars.ready, 1);
+    mbar_init(&bars.taken, 8);
     mbar_init(&bars.given, 8);
     mbar_init(&bars.done, 1);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
@@ -380,14 +438,15 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     const uint32_t k_at = smem_u32(sm), v_at = smem_u32(sm + L::v), q_at = smem_u32(sm + L::q), do_at = smem_u32(sm + L::dout);
     const uint32_t idesc_s = umma_idesc_16(128, kWCols, kF16, kF16), idesc_d = umma_idesc_16(128, (a.d + 15) & ~15, kF16, kF16, false, true);
     const int steps = (a.d + 15) / 16;
-    const auto load = [&](int t) {      // one lane: Q, dO and the rows' statistics
-      const int s = t & 1, head = kv * a.group + tiles.member(t), q0 = tiles.query(t);
+    QueryItem coming(tiles);
+    const auto load = [&](int s) {      // one lane: Q, dO and the rows' statistics of the item that comes next
+      const int head = kv * a.group + coming.member, q0 = (tiles.first + coming.tile) * kWCols;
       mbar_expect_tx(&bars.first_full[s], 2 * L::tile + L::stat);
       load_rows<kPanels>(q_at + s * L::tile, &map_q, &bars.first_full[s], kWCols, q0, head, batch);
       load_rows<kPanels>(do_at + s * L::tile, &map_do, &bars.first_full[s], kWCols, q0, head, batch);
       const size_t row = (size_t)(batch * a.heads + head) * a.npad + q0;
-      bulk_load(sm + L::stats + s * L::stat, g.lse + row, kWCols * 4, &bars.first_full[s]);
-      bulk_load(sm + L::stats + s * L::stat + kWCols * 4, g.delta + row, kWCols * 4, &bars.first_full[s]);
+      bulk_load(sm + L::stats + s * L::stat, g.nlse + row, kWCols * 4, &bars.first_full[s]);
+      bulk_load(sm + L::stats + s * L::stat + kWCols * 4, g.ndelta + row, kWCols * 4, &bars.first_full[s]);
     };
     const auto issue = [&](int t) {
       const int s = t & 1;
@@ -407,116 +466,163 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         mbar_expect_tx(&bars.own_full, 2 * kPanels * kWRows * 128);
         load_rows<kPanels>(k_at, &map_k, &bars.own_full, kWRows, k0, kv, batch);
         load_rows<kPanels>(v_at, &map_v, &bars.own_full, kWRows, k0, kv, batch);
-        for (int t = 0; t < 2 && t < tiles.count; ++t) load(t);
       }
       __syncwarp();
+      for (int t = 0; t < 2 && t < tiles.count; ++t) {
+        if (elect_lane()) load(t);
+        __syncwarp();
+        coming.next(tiles);
+      }
       ok = mbar_wait_warp(&bars.own_full, 0, 1u) && issue(0);
     }
     for (int t = 0; t < tiles.count && ok; ++t) {
+      if (L::ahead) {
+        ok = mbar_wait_warp(&bars.taken, t & 1, 8u);
+        if (!ok) break;
+        if (t > 0 && t + 1 < tiles.count) {                   // the streamed tile of the step before is free
+          ok = mbar_wait_warp(&bars.done, (t - 1) & 1, 16u);
+          if (!ok) break;
+          if (elect_lane()) load((t + 1) & 1);
+          __syncwarp();
+          coming.next(tiles);
+        }
+        if (t + 1 < tiles.count && !(ok = issue(t + 1))) break;
+      }
       ok = mbar_wait_warp(&bars.given, t & 1, 8u);
       if (!ok) break;
       tc_fence_after();
       if (elect_lane()) {
         const int s = t & 1;
-        mma_streamed(tmem + 2 * kWCols, tmem, do_at + s * L::tile, idesc_d, t == 0);
-        mma_streamed(tmem + 2 * kWCols + kAcc, tmem + kWCols, q_at + s * L::tile, idesc_d, t == 0);
+        mma_streamed<kWCols>(tmem + L::col_v, tmem + L::col_p, do_at + s * L::tile, idesc_d, t == 0);
+        mma_streamed<kWCols>(tmem + L::col_k, tmem + L::col_ds, q_at + s * L::tile, idesc_d, t == 0);
         umma_commit(&bars.done);
       }
       __syncwarp();
-      ok = mbar_wait_warp(&bars.done, t & 1, 16u);            // the streamed tile and the places of S^T and dP^T are free
-      if (!ok) break;
-      if (t + 2 < tiles.count && elect_lane()) load(t + 2);
-      __syncwarp();
-      if (t + 1 < tiles.count) ok = issue(t + 1);
+      if (!L::ahead) {
+        ok = mbar_wait_warp(&bars.done, t & 1, 16u);          // the streamed tile and the places of S^T and dP^T are free
+        if (!ok) break;
+        if (t + 2 < tiles.count) {
+          if (elect_lane()) load(t & 1);
+          __syncwarp();
+          coming.next(tiles);
+        }
+        if (t + 1 < tiles.count) ok = issue(t + 1);
+      }
     }
   } else {
     // ------------------------------------------------------------------ one key row x 32 queries a thread
-    const int quarter = warp & 3, half = warp >> 2, row = 32 * quarter + lane, j = k0 + row;
+    const int quarter = warp & 3, half = warp >> 2, row = 32 * quarter + lane, j = k0 + row, kw = k0 + 32 * quarter;
     const uint32_t t_lane = tmem + ((uint32_t)(32 * quarter) << 16);
     bool ok = true;
     int filled = -1;                               // the group's head whose bias is in shared memory
-    const int wide = a.r >= 0 && a.group > 1;      // the bias changes on the way: all eight warps keep together
-    for (int t = 0; t < tiles.count; ++t) {
-      const int q0 = tiles.query(t), qh = q0 + 32 * half, s = t & 1, member = tiles.member(t);
-      if (a.r >= 0 && member != filled) {
+    const bool wide = a.r >= 0 && a.group > 1;     // the bias changes on the way: all eight warps keep together
+    QueryItem now(tiles);
+    for (int t = 0; t < tiles.count; ++t, now.next(tiles)) {
+      const int qh = (tiles.first + now.tile) * kWCols + 32 * half, s = t & 1;
+      if (a.r >= 0 && now.member != filled) {
         // all are past the tile before (barrier below), but not all are through with it
         asm volatile("bar.sync 1, 256;\n" ::: "memory");
         for (int k = threadIdx.x; k < bias_floats(a.r); k += 256)
-          bias[k] = bias_value(a, kv * a.group + member, min(max(k - kWBiasBeyond, 0), 2 * a.r));
+          bias[k] = bias_value(a, kv * a.group + now.member, min(max(k - kWBiasBeyond, 0), 2 * a.r));
         asm volatile("bar.sync 1, 256;\n" ::: "memory");
-        filled = member;
+        filled = now.member;
       }
+      const bool dead = qh >= a.n || block_dead(a, qh, kw);
       ok = mbar_wait(&bars.ready, t & 1, 32u);
       // the statistics came with the operands; this wait only makes the copy's writes visible here
       ok = mbar_wait(&bars.first_full[s], (t >> 1) & 1, 64u) && ok;
       __syncwarp();
       tc_fence_after();
       float p[32], d[32];
-      tmem_ld32(t_lane + 32 * half, *reinterpret_cast<uint32_t(*)[32]>(&p[0]));
-      tmem_ld32(t_lane + kWCols + 32 * half, *reinterpret_cast<uint32_t(*)[32]>(&d[0]));
-      tmem_wait_ld();
+      if (!dead) {
+        tmem_ld32(t_lane + 32 * half, *reinterpret_cast<uint32_t(*)[32]>(&p[0]));
+        tmem_ld32(t_lane + kWCols + 32 * half, *reinterpret_cast<uint32_t(*)[32]>(&d[0]));
+        tmem_wait_ld();
+      }
       tc_fence_before();
-      ok = barrier_all(wide ? 1 : 2 + quarter, wide ? 256 : 64, ok);      // both halves have read what is overwritten below
+      // where P^T and dS^T go to the places of S^T and dP^T, both halves have to have read these
+      if (L::ahead && !wide) ok = __all_sync(0xffffffffu, ok) != 0;
+      else ok = barrier_all(wide ? 1 : 2 + quarter, wide ? 256 : 64, ok);
       if (!ok) break;
-      tc_fence_after();
-      const float4* const lse4 = reinterpret_cast<const float4*>(sm + L::stats + s * L::stat) + 8 * half;
-      const float4* const delta4 = lse4 + kWCols / 4;
-      const int lowest = k0 + 32 * quarter - (qh + 31), highest = k0 + 32 * quarter + 31 - qh;
-      const bool flat_low = a.r >= 0 && clipped_low(a, highest), flat_high = a.r >= 0 && clipped_high(a, lowest);
-      const float flat = flat_low ? bias[0] : flat_high ? bias[bias_floats(a.r) - 1] : 0.f;
-      const bool near = a.r >= 0 && !flat_low && !flat_high;
-      const float* const b = bias + (near ? j - qh + a.r + kWBiasBeyond : 0);
-      const bool whole = !any_masked && k0 + kWRows - 1 <= q0 + a.right && q0 + kWCols - 1 <= k0 + a.left && q0 + kWCols <= a.n;
-#pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        const float4 l4 = lse4[c], e4 = delta4[c];
-        const float l[4] = {l4.x, l4.y, l4.z, l4.w}, e[4] = {e4.x, e4.y, e4.z, e4.w};
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const float add = (near ? b[-(4 * c + x)] : flat) - l[x];
-          p[4 * c + x] = fast_exp2(fmaf(p[4 * c + x], a.c, add));
-          d[4 * c + x] = p[4 * c + x] * (d[4 * c + x] - e[x]);
-        }
-      }
-      bool nothing = false;                        // a query of this tile that sees nothing: its rows of Q and dO may hold anything
-      if (!whole) {
-        // queries j - right .. j + left, all from j - right on for a sink, none for a masked key
-        const int from = j - a.right - qh, to = masked ? -1 : j < a.sinks ? 31 : min(31, j + a.left - qh);
-        const uint32_t seen = (uint32_t)bits_between(from, to);
-#pragma unroll
-        for (int c = 0; c < 32; ++c) {
-          const bool see = seen >> c & 1u;
-          p[c] = see ? p[c] : 0.f;
-          d[c] = see ? d[c] : 0.f;
-        }
-      }
-      {
-        const float* const all = reinterpret_cast<const float*>(sm + L::stats + s * L::stat);
-        nothing = __any_sync(0xffffffffu, all[lane] == CUDART_INF_F || all[32 + lane] == CUDART_INF_F);
-        if (nothing) {
+      if (L::ahead && lane == 0) mbar_arrive(&bars.taken);
+      uint32_t wp[16], wd[16];
+      if (!dead) {
+        const float4* const nlse4 = reinterpret_cast<const float4*>(sm + L::stats + s * L::stat) + 8 * half;
+        const float4* const ndelta4 = nlse4 + kWCols / 4;
+        const BlockBias bb(a, bias, qh, kw);
+        if (bb.near) {
+          const float* const y = bias_row(a, bias, qh, j);      // of query qh + c: y[-c]
 #pragma unroll
           for (int c = 0; c < 8; ++c) {
-            const float4 l4 = lse4[c];
-            const float l[4] = {l4.x, l4.y, l4.z, l4.w};
-#pragma unroll
-            for (int x = 0; x < 4; ++x)
-              if (l[x] == CUDART_INF_F) p[4 * c + x] = d[4 * c + x] = 0.f;
+            float4 l4 = nlse4[c];
+            add2(l4.x, l4.y, y[-4 * c], y[-4 * c - 1]);
+            add2(l4.z, l4.w, y[-4 * c - 2], y[-4 * c - 3]);
+            fma2(p[4 * c], p[4 * c + 1], p[4 * c], p[4 * c + 1], a.c, a.c, l4.x, l4.y);
+            fma2(p[4 * c + 2], p[4 * c + 3], p[4 * c + 2], p[4 * c + 3], a.c, a.c, l4.z, l4.w);
           }
-          const int r64 = threadIdx.x & 63;
-          if (all[r64] == CUDART_INF_F) {
-            clear_row<kPanels>(sm + L::q + s * L::tile, r64, threadIdx.x >> 6, 4);
-            clear_row<kPanels>(sm + L::dout + s * L::tile, r64, threadIdx.x >> 6, 4);
+        } else {
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            float4 l4 = nlse4[c];
+            add2(l4.x, l4.y, bb.flat, bb.flat);
+            add2(l4.z, l4.w, bb.flat, bb.flat);
+            fma2(p[4 * c], p[4 * c + 1], p[4 * c], p[4 * c + 1], a.c, a.c, l4.x, l4.y);
+            fma2(p[4 * c + 2], p[4 * c + 3], p[4 * c + 2], p[4 * c + 3], a.c, a.c, l4.z, l4.w);
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          const float4 e4 = ndelta4[c];
+          add2(d[4 * c], d[4 * c + 1], e4.x, e4.y);
+          add2(d[4 * c + 2], d[4 * c + 3], e4.z, e4.w);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) p[4 * c + x] = fast_exp2(p[4 * c + x]);
+          mul2(d[4 * c], d[4 * c + 1], p[4 * c], p[4 * c + 1]);
+          mul2(d[4 * c + 2], d[4 * c + 3], p[4 * c + 2], p[4 * c + 3]);
+        }
+        if (any_masked || !block_whole(a, qh, kw)) {
+          // queries j - right .. j + left, all from j - right on for a sink, none for a masked key
+          const int from = j - a.right - qh, to = masked ? -1 : j < a.sinks ? 31 : j + a.left - qh;
+          const uint32_t seen = bits_between(from, to);
+#pragma unroll
+          for (int c = 0; c < 32; ++c) {
+            const bool see = seen >> c & 1u;
+            p[c] = see ? p[c] : 0.f;
+            d[c] = see ? d[c] : 0.f;
+          }
+        }
+      }
+      if (a.mask) {
+        // queries that see nothing: whatever their rows of Q and dO hold becomes zeros; those of this half by its four warps
+        const float* const mine = reinterpret_cast<const float*>(sm + L::stats + s * L::stat) + 32 * half;
+        const uint32_t nothing = __ballot_sync(0xffffffffu, mine[lane] == -CUDART_INF_F);
+        if (nothing) {
+          if (!dead) {
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+              if (nothing >> c & 1u) p[c] = d[c] = 0.f;
+          }
+          if (nothing >> lane & 1u) {
+            clear_row<kPanels, kWCols>(sm + L::q + s * L::tile, 32 * half + lane, quarter, 4);
+            clear_row<kPanels, kWCols>(sm + L::dout + s * L::tile, 32 * half + lane, quarter, 4);
           }
           fence_async_shared();
         }
       }
-      uint32_t w[16];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) w[e] = pack16x2<kF16>(p[2 * e], p[2 * e + 1]);
-      tmem_st16(t_lane + 16 * half, w);
-#pragma unroll
-      for (int e = 0; e < 16; ++e) w[e] = pack16x2<kF16>(d[2 * e], d[2 * e + 1]);
-      tmem_st16(t_lane + kWCols + 16 * half, w);
+      for (int e = 0; e < 16; ++e) {
+        wp[e] = dead ? 0u : pack16x2<kF16>(p[2 * e], p[2 * e + 1]);
+        wd[e] = dead ? 0u : pack16x2<kF16>(d[2 * e], d[2 * e + 1]);
+      }
+      if (L::ahead && t > 0) {                      // the products before have read their P^T and dS^T
+        ok = mbar_wait(&bars.done, (t - 1) & 1, 64u);
+        if (!wide) ok = __all_sync(0xffffffffu, ok) != 0;
+        else ok = barrier_all(1, 256, ok);
+        if (!ok) break;
+      }
+      tc_fence_after();
+      tmem_st16(t_lane + L::col_p + 16 * half, wp);
+      tmem_st16(t_lane + L::col_ds + 16 * half, wd);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -540,7 +646,7 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         for (int c = 16 * half; c < a.d; c += 32) {
           uint32_t x[16];
           if (tiles.count > 0) {
-            tmem_ld16(t_lane + 2 * kWCols + (which ? 0 : kAcc) + c, x);
+            tmem_ld16(t_lane + (which ? L::col_v : L::col_k) + c, x);
             tmem_wait_ld();
           } else {
 #pragma unroll

@@ -26,32 +26,37 @@ constexpr float kWRescaleGap = 8.0f;
 constexpr int kWFwdThreads = 160;
 
 struct WindowFwdBars {
-  uint64_t q_full, k_full[2], v_full[2], s_full, p_ready, pv_done;
+  uint64_t q_full, k_full[2], v_full[2], s_full, s_free, p_ready, pv_done;
   uint32_t tmem_base;
-};
-
-template <int kPanels>
-struct WindowFwdLayout {
-  static constexpr int q = 0, tile = kPanels * kWCols * 128;
-  static constexpr int k = kPanels * kWRows * 128, v = k + 2 * tile, bars = v + 2 * tile;
-  static constexpr int bias = bars + 128;
-  static constexpr int bytes(int r) { return bias + bias_floats(r) * 4; }
 };
 static_assert(sizeof(WindowFwdBars) <= 128, "room for the barriers");
 
-template <bool kF16, int kPanels>
-__global__ void __launch_bounds__(kWFwdThreads, kPanels == 1 ? 4 : 2)
+// kD: the head size that the accumulator has room for, 32, 64 or 128.
+template <int kD>
+struct WindowFwdLayout {
+  static constexpr int panels = kD > 64 ? 2 : 1, keys = kD == 64 ? 128 : 64, ctas = kD == 32 ? 4 : 2;
+  static constexpr int cols = kD == 32 ? 128 : 256, col_p = keys, col_o = keys + keys / 2;      // S | P | O
+  static_assert(col_o + kD <= cols, "tensor memory of a CTA");
+  static constexpr int q = 0, tile = panels * keys * 128;
+  static constexpr int k = panels * kWRows * 128, v = k + 2 * tile, bars = v + 2 * tile;
+  static constexpr int bias = bars + 128;
+  static constexpr int bytes(int r) { return bias + bias_floats(r) * 4; }
+};
+
+template <bool kF16, int kD>
+__global__ void __launch_bounds__(kWFwdThreads, WindowFwdLayout<kD>::ctas)
 window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                  const WindowArgs a, const RowsOut o, float* __restrict__ lse) {
-  typedef WindowFwdLayout<kPanels> L;
-  constexpr uint32_t kCols = kPanels == 1 ? 128 : 256;
+                  const WindowArgs a, const RowsOut o, float* __restrict__ nlse) {
+  typedef WindowFwdLayout<kD> L;
+  constexpr uint32_t kCols = L::cols;
+  constexpr int kPanels = L::panels, kKT = L::keys, kBlocks = kKT / 32;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* sm = smem_aligned(smem_raw);
   WindowFwdBars& bars = *reinterpret_cast<WindowFwdBars*>(sm + L::bars);
   float* const bias = reinterpret_cast<float*>(sm + L::bias);
   const int warp = warp_index(), lane = threadIdx.x & 31;
   const int q0 = (int)(blockIdx.x % a.tiles) * kWRows, bh = blockIdx.x / a.tiles, head = bh % a.heads, batch = bh / a.heads;
-  const KeyTiles tiles(a, q0);
+  const KeyTiles<kKT> tiles(a, q0);
 
   const bool skip = cta_begin();
   if (threadIdx.x == 0) {
@@ -62,6 +67,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       mbar_init(&bars.v_full[s], 1);
     }
     mbar_init(&bars.s_full, 1);
+    mbar_init(&bars.s_free, 4);
     mbar_init(&bars.p_ready, 4);
     mbar_init(&bars.pv_done, 1);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
@@ -69,27 +75,29 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   if (warp == 4) tmem_alloc(&bars.tmem_base, kCols);
   if (!cta_ready(skip, warp == 4, bars.tmem_base, kCols)) return;
   const uint32_t tmem = bars.tmem_base;
-  if (a.r >= 0) bias_fill(a, head, bias);
-  __syncthreads();
+  if (a.r >= 0) {
+    bias_fill(a, head, bias);
+    __syncthreads();
+  }
 
   if (warp == 4) {
     // ------------------------------------------------------------------ copies and products
     const int kv = head / a.group;
     const uint32_t q_at = smem_u32(sm), k_at = smem_u32(sm + L::k), v_at = smem_u32(sm + L::v);
-    const uint32_t idesc_s = umma_idesc_16(128, kWCols, kF16, kF16), idesc_o = umma_idesc_16(128, (a.d + 15) & ~15, kF16, kF16, false, true);
+    const uint32_t idesc_s = umma_idesc_16(128, kKT, kF16, kF16), idesc_o = umma_idesc_16(128, (a.d + 15) & ~15, kF16, kF16, false, true);
     const auto load_k = [&](int t) {      // one lane
       mbar_expect_tx(&bars.k_full[t & 1], L::tile);
-      load_rows<kPanels>(k_at + (t & 1) * L::tile, &map_k, &bars.k_full[t & 1], kWCols, tiles.key(t), kv, batch);
+      load_rows<kPanels>(k_at + (t & 1) * L::tile, &map_k, &bars.k_full[t & 1], kKT, tiles.key(t), kv, batch);
     };
     const auto load_v = [&](int t) {
       mbar_expect_tx(&bars.v_full[t & 1], L::tile);
-      load_rows<kPanels>(v_at + (t & 1) * L::tile, &map_v, &bars.v_full[t & 1], kWCols, tiles.key(t), kv, batch);
+      load_rows<kPanels>(v_at + (t & 1) * L::tile, &map_v, &bars.v_full[t & 1], kKT, tiles.key(t), kv, batch);
     };
     const auto issue_s = [&](int t) {
       if (!mbar_wait_warp(&bars.k_full[t & 1], (t >> 1) & 1, 2u)) return false;
       tc_fence_after();
       if (elect_lane()) {
-        mma_rows(tmem, q_at, k_at + (t & 1) * L::tile, kWCols, (a.d + 15) / 16, idesc_s);
+        mma_rows(tmem, q_at, k_at + (t & 1) * L::tile, kKT, (a.d + 15) / 16, idesc_s);
         umma_commit(&bars.s_full);
       }
       __syncwarp();
@@ -106,78 +114,108 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     __syncwarp();
     bool ok = mbar_wait_warp(&bars.q_full, 0, 1u) && issue_s(0);
     for (int t = 0; t < tiles.count && ok; ++t) {
-      ok = mbar_wait_warp(&bars.p_ready, t & 1, 4u);          // S(t) is complete and read: its K tile is free
+      ok = mbar_wait_warp(&bars.s_free, t & 1, 4u);           // S(t) is complete and in registers: its K tile and its place are free
       if (!ok) break;
       if (t + 2 < tiles.count && elect_lane()) load_k(t + 2);
       __syncwarp();
-      ok = mbar_wait_warp(&bars.v_full[t & 1], (t >> 1) & 1, 8u);
+      if (t + 1 < tiles.count && !(ok = issue_s(t + 1))) break;
+      if (t > 0 && t + 1 < tiles.count) {                     // the V tile of the step before is free
+        ok = mbar_wait_warp(&bars.pv_done, (t - 1) & 1, 16u);
+        if (!ok) break;
+        if (elect_lane()) load_v(t + 1);
+        __syncwarp();
+      }
+      ok = mbar_wait_warp(&bars.p_ready, t & 1, 8u) && mbar_wait_warp(&bars.v_full[t & 1], (t >> 1) & 1, 8u);
       if (!ok) break;
       tc_fence_after();
       if (elect_lane()) {
-        mma_streamed(tmem + kWCols, tmem, v_at + (t & 1) * L::tile, idesc_o, t == 0);
+        mma_streamed<kKT>(tmem + L::col_o, tmem + L::col_p, v_at + (t & 1) * L::tile, idesc_o, t == 0);
         umma_commit(&bars.pv_done);
       }
       __syncwarp();
-      ok = mbar_wait_warp(&bars.pv_done, t & 1, 16u);         // P, which lies where the next S goes, has been read
-      if (!ok) break;
-      if (t + 2 < tiles.count && elect_lane()) load_v(t + 2);
-      __syncwarp();
-      if (t + 1 < tiles.count) ok = issue_s(t + 1);
     }
   } else {
     // ------------------------------------------------------------------ one query row a thread
-    const int row = threadIdx.x, i = q0 + row;
-    const uint32_t t_s = tmem + ((uint32_t)(32 * warp) << 16), t_o = t_s + kWCols;
-    float m = -CUDART_INF_F, l = 0.f;
+    const int row = threadIdx.x, i = q0 + row, qw = q0 + 32 * warp;
+    const uint32_t t_s = tmem + ((uint32_t)(32 * warp) << 16), t_p = t_s + L::col_p, t_o = t_s + L::col_o;
+    float m = -CUDART_INF_F, l0 = 0.f, l1 = 0.f;
     bool ok = true;
     for (int t = 0; t < tiles.count; ++t) {
       const int k0 = tiles.key(t);
-      const uint64_t keys = key_bits(a, batch, k0, lane);
-      const bool whole = keys == ~0ull && window_covers(a, q0, k0);
+      uint32_t keys[kBlocks];
+      bool dead[kBlocks], hidden = false;
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b) {
+        keys[b] = key_bits(a, batch, k0 + 32 * b, lane);
+        dead[b] = keys[b] == 0 || block_dead(a, qw, k0 + 32 * b);
+        hidden = hidden || keys[b] != bits_between(0, a.n - 1 - (k0 + 32 * b));
+      }
       ok = mbar_wait(&bars.s_full, t & 1, 32u);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
-      float s[kWCols];
-      tmem_ld32(t_s, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
-      tmem_ld32(t_s + 32, *reinterpret_cast<uint32_t(*)[32]>(&s[32]));
+      float s[kKT];
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b) tmem_ld32(t_s + 32 * b, *reinterpret_cast<uint32_t(*)[32]>(&s[32 * b]));
       tmem_wait_ld();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars.s_free);
       // logits = s * mul + add, in base 2
-      float mul = a.c, add = 0.f;
-      if (a.r >= 0) {
-        if (clipped_low(a, k0 + kWCols - 1 - q0)) {
-          add = bias[0];
-        } else if (clipped_high(a, k0 - q0 - (kWRows - 1))) {
-          add = bias[bias_floats(a.r) - 1];
-        } else {
-          const float* b = bias + (k0 - i + a.r + kWBiasBeyond);
+      float mul[kBlocks], add[kBlocks], mt = -CUDART_INF_F;
 #pragma unroll
-          for (int c = 0; c < kWCols; ++c) s[c] = fmaf(s[c], mul, b[c]);
-          mul = 1.f;
+      for (int b = 0; b < kBlocks; ++b) {
+        if (dead[b]) continue;
+        const int kb = k0 + 32 * b;
+        float* const x = s + 32 * b;
+        const BlockBias bb(a, bias, qw, kb);
+        mul[b] = a.c, add[b] = bb.flat;
+        if (bb.near) {
+          const float* const y = bias_row(a, bias, i, kb);
+#pragma unroll
+          for (int c = 0; c < 32; c += 2) fma2(x[c], x[c + 1], x[c], x[c + 1], a.c, a.c, y[c], y[c + 1]);
+          mul[b] = 1.f, add[b] = 0.f;
         }
-      }
-      if (!whole) {
-        const uint64_t seen = visible_bits(a, i, k0, keys);
-        const uint32_t lo = (uint32_t)seen, hi = (uint32_t)(seen >> 32);
+        if (keys[b] != 0xffffffffu || !block_whole(a, qw, kb)) {
+          const uint32_t seen = visible_bits(a, i, kb, keys[b]);
 #pragma unroll
-        for (int c = 0; c < kWCols; ++c) s[c] = ((c < 32 ? lo : hi) >> (c & 31) & 1u) ? s[c] : -CUDART_INF_F;
+          for (int c = 0; c < 32; ++c) x[c] = (seen >> c & 1u) ? x[c] : -CUDART_INF_F;
+        }
+        mt = fmaxf(mt, fmaf(max32(x), mul[b], add[b]));
       }
-      float mq[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        mq[k] = s[16 * k];
-#pragma unroll
-        for (int e = 1; e < 16; ++e) mq[k] = fmaxf(mq[k], s[16 * k + e]);
-      }
-      const float mt = fmaf(fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3])), mul, add);
       const bool up = mt > m + kWRescaleGap;
       const bool move = __any_sync(0xffffffffu, up) && t > 0;      // the first product overwrites O
       const float m_old = m;
       m = up ? mt : m;
-      const float shift = add - (m == -CUDART_INF_F ? 0.f : m);
-      if (move) {                                                   // O is at rest: S(t) was issued after P V (t - 1) was complete
+      const float shift = m == -CUDART_INF_F ? 0.f : -m;
+      float r0 = 0.f, r1 = 0.f;
+      uint32_t w[kKT / 2];
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b) {
+        if (dead[b]) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) w[16 * b + e] = 0u;
+          continue;
+        }
+        const float sh = add[b] + shift;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          float p0 = s[32 * b + 2 * e], p1 = s[32 * b + 2 * e + 1];
+          fma2(p0, p1, p0, p1, mul[b], mul[b], sh, sh);
+          p0 = fast_exp2(p0), p1 = fast_exp2(p1);
+          add2(r0, r1, p0, p1);
+          w[16 * b + e] = pack16x2<kF16>(p0, p1);
+        }
+      }
+      if (t > 0) {                                                  // P and O are at rest
+        ok = mbar_wait(&bars.pv_done, (t - 1) & 1, 128u);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+      }
+      if (move) {
         const float alpha = up ? fast_exp2(m_old - m) : 1.f;
-        l *= alpha;
+        l0 *= alpha, l1 *= alpha;
         for (int c = 0; c < a.d; c += 16) {
           uint32_t x[16];
           tmem_ld16(t_o + c, x);
@@ -187,23 +225,18 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           tmem_st16(t_o + c, x);
         }
       }
-      float l0 = 0.f, l1 = 0.f;
+      add2(l0, l1, r0, r1);
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        uint32_t w[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float p0 = fast_exp2(fmaf(s[32 * k + 2 * e], mul, shift)), p1 = fast_exp2(fmaf(s[32 * k + 2 * e + 1], mul, shift));
-          add2(l0, l1, p0, p1);
-          w[e] = pack16x2<kF16>(p0, p1);
-        }
-        tmem_st16(t_s + 16 * k, w);
-      }
-      l += l0 + l1;
-      if (keys != bits_between(0, a.n - 1 - k0)) {                  // masked keys: their rows of V, by one thread of each half
+      for (int b = 0; b < kBlocks; ++b) tmem_st16(t_p + 16 * b, *reinterpret_cast<const uint32_t(*)[16]>(&w[16 * b]));
+      if (hidden) {                                                 // masked keys: their rows of V
         ok = mbar_wait_warp(&bars.v_full[t & 1], (t >> 1) & 1, 64u);
         if (!ok) break;
-        if (!(keys >> (row & 63) & 1)) clear_row<kPanels>(sm + L::v + (t & 1) * L::tile, row & 63, row >> 6, 2);
+        constexpr int kParts = 128 / kKT;
+        const int r = row % kKT;
+        uint32_t word = keys[0];
+#pragma unroll
+        for (int b = 1; b < kBlocks; ++b) word = r >> 5 == b ? keys[b] : word;
+        if (!(word >> (r & 31) & 1)) clear_row<kPanels, kKT>(sm + L::v + (t & 1) * L::tile, r, row / kKT, kParts);
         fence_async_shared();
       }
       tmem_wait_st();
@@ -215,7 +248,8 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     ok = __all_sync(0xffffffffu, ok);
     if (ok) {
       tc_fence_after();
-      const bool empty = !(l > 0.f) && m == -CUDART_INF_F;
+      const float l = l0 + l1;
+      const bool empty = m == -CUDART_INF_F;
       const float inv = empty ? 0.f : 1.f / l;
       uint16_t* const out = o.at(batch, head, i);
       for (int c = 0; c < a.d; c += 16) {
@@ -228,7 +262,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         }
       }
       // Rows that see nothing, and those beyond the last, have weights of zero in the backward pass.
-      if (lse) lse[(size_t)bh * a.npad + i] = i < a.n && !empty ? m + log2f(l) : CUDART_INF_F;
+      if (nlse) nlse[(size_t)bh * a.npad + i] = i < a.n && !empty ? -(m + log2f(l)) : -CUDART_INF_F;
     }
   }
   tc_fence_before();
@@ -295,13 +329,16 @@ static WindowArgs window_args(const px_window& w) {
   return a;
 }
 
-template <bool kF16, int kPanels>
-static bool launch_window_fwd(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const WindowArgs& a, const RowsOut& o, float* lse,
-                              int64_t blocks, cudaStream_t st) {
-  typedef WindowFwdLayout<kPanels> L;
+template <bool kF16, int kD>
+static bool launch_window_fwd(const px_window& w, const px_rows& q, const px_rows& k, const px_rows& v, const WindowArgs& a, const RowsOut& o,
+                              float* lse, cudaStream_t st) {
+  typedef WindowFwdLayout<kD> L;
+  CUtensorMap mq, mk, mv;
+  if (!rows_map(&mq, q, w, w.heads, kWRows) || !rows_map(&mk, k, w, w.kv_heads, L::keys) || !rows_map(&mv, v, w, w.kv_heads, L::keys)) return false;
   static SmemLimit limit;
-  if (!limit.set(window_fwd_kernel<kF16, kPanels>, L::bytes(kWMaxR) + 1024)) return false;
-  return launch_pdl(window_fwd_kernel<kF16, kPanels>, dim3((unsigned)blocks), kWFwdThreads, (size_t)L::bytes(a.r) + 1024, st, mq, mk, mv, a, o, lse);
+  if (!limit.set(window_fwd_kernel<kF16, kD>, L::bytes(kWMaxR) + 1024)) return false;
+  return launch_pdl(window_fwd_kernel<kF16, kD>, dim3((unsigned)((int64_t)a.tiles * w.heads * w.batch)), kWFwdThreads, (size_t)L::bytes(a.r) + 1024,
+                    st, mq, mk, mv, a, o, lse);
 }
 
 }  // namespace px
@@ -317,13 +354,12 @@ extern "C" int32_t px_window_fwd(const px_window* w, const px_rows* q, const px_
   if (w->batch == 0 || w->n == 0) return PX_OK;
   if (!rows_fit(q, *w, w->heads) || !rows_fit(k, *w, w->kv_heads) || !rows_fit(v, *w, w->kv_heads) || !rows_fit(o, *w, w->heads))
     return PX_ERR_BAD_ARG;
-  CUtensorMap mq, mk, mv;
-  if (!have_context() || !rows_map(&mq, *q, *w, w->heads, kWRows) || !rows_map(&mk, *k, *w, w->kv_heads, kWCols) || !rows_map(&mv, *v, *w, w->kv_heads, kWCols))
-    return PX_ERR_LAUNCH;
-  const WindowArgs a = window_args(*w);
-  const auto go = w->dtype == PX_F16 ? (w->d <= 64 ? launch_window_fwd<true, 1> : launch_window_fwd<true, 2>)
-                                     : (w->d <= 64 ? launch_window_fwd<false, 1> : launch_window_fwd<false, 2>);
-  return go(mq, mk, mv, a, rows_out(o), lse, (int64_t)a.tiles * w->heads * w->batch, (cudaStream_t)stream) ? PX_OK : PX_ERR_LAUNCH;
+  if (!have_context()) return PX_ERR_LAUNCH;
+  const auto go = w->dtype == PX_F16 ? (w->d <= 32 ? launch_window_fwd<true, 32> : w->d <= 64 ? launch_window_fwd<true, 64> : launch_window_fwd<true, 128>)
+                                     : (w->d <= 32   ? launch_window_fwd<false, 32>
+                                        : w->d <= 64 ? launch_window_fwd<false, 64>
+                                                     : launch_window_fwd<false, 128>);
+  return go(*w, *q, *k, *v, window_args(*w), rows_out(o), lse, (cudaStream_t)stream) ? PX_OK : PX_ERR_LAUNCH;
 }
 
 namespace px {
@@ -353,33 +389,44 @@ static WindowSpace window_space(const px_window& w, const WindowArgs& a, bool bi
   return s;
 }
 
-template <bool kF16, int kPanels, bool kBiasGrad>
+// q, dO, k, v as a kernel cuts them that owns 128 rows of queries (own_q) or keys and streams the others.
+static bool bwd_maps(CUtensorMap* m, const px_window& w, const px_rows& q, const px_rows& dout, const px_rows& k, const px_rows& v, bool own_q) {
+  const uint32_t rq = own_q ? kWRows : kWCols, rk = own_q ? kWCols : kWRows;
+  return rows_map(&m[0], q, w, w.heads, rq) && rows_map(&m[1], dout, w, w.heads, rq) && rows_map(&m[2], k, w, w.kv_heads, rk) &&
+         rows_map(&m[3], v, w, w.kv_heads, rk);
+}
+template <bool kF16, int kD, bool kBiasGrad>
 static bool launch_window_dq(const CUtensorMap* m, const WindowArgs& a, const WindowBwdArgs& g, const RowsOut& dout, const RowsOut& o,
                              const RowsOut& dq, int64_t blocks, cudaStream_t st) {
-  typedef WindowDqLayout<kPanels> L;
+  typedef WindowDqLayout<kD> L;
   static SmemLimit limit;
-  const auto kernel = window_dq_kernel<kF16, kPanels, kBiasGrad>;
+  const auto kernel = window_dq_kernel<kF16, kD, kBiasGrad>;
   if (!limit.set(kernel, L::bytes(kWMaxR, kBiasGrad) + 1024)) return false;
   return launch_pdl(kernel, dim3((unsigned)blocks), kWBwdThreads, (size_t)L::bytes(a.r, kBiasGrad) + 1024, st, m[0], m[1], m[2], m[3], a, g, dout, o,
                     dq);
 }
-template <bool kF16, int kPanels>
+template <bool kF16, int kD>
 static bool launch_window_dkv(const CUtensorMap* m, const WindowArgs& a, const WindowBwdArgs& g, const RowsOut& dk, const RowsOut& dv, int64_t blocks,
                               cudaStream_t st) {
-  typedef WindowDkvLayout<kPanels> L;
+  typedef WindowDkvLayout<kD> L;
   static SmemLimit limit;
-  const auto kernel = window_dkv_kernel<kF16, kPanels>;
+  const auto kernel = window_dkv_kernel<kF16, kD>;
   if (!limit.set(kernel, L::bytes(kWMaxR) + 1024)) return false;
   return launch_pdl(kernel, dim3((unsigned)blocks), kWBwdThreads, (size_t)L::bytes(a.r) + 1024, st, m[0], m[1], m[2], m[3], a, g, dk, dv);
 }
 
-template <bool kF16, int kPanels>
-static bool window_bwd(const px_window& w, const CUtensorMap* own_q, const CUtensorMap* own_k, const WindowArgs& a, const WindowBwdArgs& g,
-                       const RowsOut& dout, const RowsOut& o, const RowsOut& dq, const RowsOut& dk, const RowsOut& dv, void* dbias, cudaStream_t st) {
+struct BwdRows {
+  const px_rows *q, *k, *v, *o, *dout, *dq, *dk, *dv;
+};
+template <bool kF16>
+static bool window_bwd(const px_window& w, const BwdRows& x, const WindowArgs& a, const WindowBwdArgs& g, void* dbias, cudaStream_t st) {
   const int64_t blocks = (int64_t)a.tiles * w.heads * w.batch;
-  if (!(dbias ? launch_window_dq<kF16, kPanels, true>(own_q, a, g, dout, o, dq, blocks, st)
-              : launch_window_dq<kF16, kPanels, false>(own_q, a, g, dout, o, dq, blocks, st)))
-    return false;
+  const RowsOut dout = rows_out(x.dout), o = rows_out(x.o), dq = rows_out(x.dq), dk = rows_out(x.dk), dv = rows_out(x.dv);
+  CUtensorMap m[4];
+  if (!bwd_maps(m, w, *x.q, *x.dout, *x.k, *x.v, true)) return false;
+  const auto go_q = w.d <= 64 ? (dbias ? launch_window_dq<kF16, 64, true> : launch_window_dq<kF16, 64, false>)
+                              : (dbias ? launch_window_dq<kF16, 128, true> : launch_window_dq<kF16, 128, false>);
+  if (!go_q(m, a, g, dout, o, dq, blocks, st)) return false;
   if (dbias) {
     const int buckets = 2 * a.r + 1;
     window_dbias_kernel<<<dim3((unsigned)((buckets + 31) / 32), (unsigned)w.heads), 1024, 0, st>>>(g.dbias, dbias, a.bias_type, (int)w.batch, a.heads,
@@ -387,7 +434,9 @@ static bool window_bwd(const px_window& w, const CUtensorMap* own_q, const CUten
     if (cudaGetLastError() != cudaSuccess) return false;
   }
   if (!dk.data && !dv.data) return true;
-  if (!launch_window_dkv<kF16, kPanels>(own_k, a, g, dk, dv, (int64_t)(a.tiles + g.sink_tiles * g.chunks) * w.kv_heads * w.batch, st)) return false;
+  if (!bwd_maps(m, w, *x.q, *x.dout, *x.k, *x.v, false)) return false;
+  const auto go_kv = w.d <= 32 ? launch_window_dkv<kF16, 32> : w.d <= 64 ? launch_window_dkv<kF16, 64> : launch_window_dkv<kF16, 128>;
+  if (!go_kv(m, a, g, dk, dv, (int64_t)(a.tiles + g.sink_tiles * g.chunks) * w.kv_heads * w.batch, st)) return false;
   if (g.chunks > 0) {
     const int rows = a.n < g.sink_tiles * kWRows ? a.n : g.sink_tiles * kWRows;
     const int64_t per = (2 * (int64_t)rows * (a.d / 8) + 255) / 256;
@@ -423,21 +472,16 @@ extern "C" int32_t px_window_bwd(const px_window* w, const px_rows* q, const px_
   const WindowArgs a = window_args(*w);
   const WindowSpace space = window_space(*w, a, dbias != nullptr);
   if (workspace_bytes < space.total) return PX_ERR_WORKSPACE;
-  CUtensorMap own_q[4], own_k[4];      // q, dO, k, v as the two kernels cut them
-  if (!have_context() || !rows_map(&own_q[0], *q, *w, w->heads, kWRows) || !rows_map(&own_q[1], *dout, *w, w->heads, kWRows) ||
-      !rows_map(&own_q[2], *k, *w, w->kv_heads, kWCols) || !rows_map(&own_q[3], *v, *w, w->kv_heads, kWCols) ||
-      !rows_map(&own_k[0], *q, *w, w->heads, kWCols) || !rows_map(&own_k[1], *dout, *w, w->heads, kWCols) ||
-      !rows_map(&own_k[2], *k, *w, w->kv_heads, kWRows) || !rows_map(&own_k[3], *v, *w, w->kv_heads, kWRows))
-    return PX_ERR_LAUNCH;
+  if (!have_context()) return PX_ERR_LAUNCH;
   WindowBwdArgs g = {};
   unsigned char* const ws = (unsigned char*)workspace;
-  g.lse = lse;
-  g.delta = (float*)(ws + space.delta);
+  g.nlse = lse;
+  g.ndelta = (float*)(ws + space.delta);
   g.dbias = (float*)(ws + space.dbias);
   g.sinks = (float*)(ws + space.sinks);
   g.scale = w->scale;
   sink_chunks(a, &g.sink_tiles, &g.chunks, &g.chunk);
   if ((int64_t)(a.tiles + g.sink_tiles * g.chunks) * w->kv_heads * w->batch > 0x3fffffffll) return PX_ERR_UNSUPPORTED;
-  const auto go = w->dtype == PX_F16 ? (w->d <= 64 ? window_bwd<true, 1> : window_bwd<true, 2>) : (w->d <= 64 ? window_bwd<false, 1> : window_bwd<false, 2>);
-  return go(*w, own_q, own_k, a, g, rows_out(dout), rows_out(o), rows_out(dq), rows_out(dk), rows_out(dv), dbias, st) ? PX_OK : PX_ERR_LAUNCH;
+  const BwdRows rows = {q, k, v, o, dout, dq, dk, dv};
+  return (w->dtype == PX_F16 ? window_bwd<true>(*w, rows, a, g, dbias, st) : window_bwd<false>(*w, rows, a, g, dbias, st)) ? PX_OK : PX_ERR_LAUNCH;
 }
