@@ -51,6 +51,19 @@ __device__ __forceinline__ void mma_streamed(uint32_t d_tmem, uint32_t a_tmem, u
     umma_bf16_ts(d_tmem, a_tmem + 8 * ks, umma_desc_mn_sw128(b + ks * 2048, kKT * 128, 1024), idesc, !first || ks > 0);
 }
 
+// The same with A in shared memory, a panel of 64.
+__device__ __forceinline__ void mma_streamed_ss(uint32_t d_tmem, uint32_t a, uint32_t b, uint32_t idesc, bool first) {
+#pragma unroll
+  for (int ks = 0; ks < 4; ++ks)
+    umma_bf16(d_tmem, umma_desc_sw128(a) + 2 * ks, umma_desc_mn_sw128(b + ks * 2048, 64 * 128, 1024), idesc, !first || ks > 0);
+}
+// 32 values (16 words) of row `row` into such a panel, columns 32 * half and up.
+__device__ __forceinline__ void panel_store(unsigned char* panel, int row, int half, const uint32_t (&w)[16]) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    *reinterpret_cast<uint4*>(panel + row * 128 + (((4 * half + e) ^ (row & 7)) << 4)) = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+}
+
 // Streamed key tiles of the queries [q0, q0 + 128): the first tiles as far as they hold sinks, then those of the window.
 template <int kKT>
 struct KeyTiles {
@@ -79,13 +92,30 @@ __device__ __forceinline__ uint32_t visible_bits(const WindowArgs& a, int i, int
   const int hi = i + a.right - k0;
   return (bits_between(i - a.left - k0, hi) | bits_between(0, min(a.sinks - 1 - k0, hi))) & keys;
 }
-// What a block of 32 queries from q0 and 32 keys from k0 is, as far as the window goes: out of sight, or seen by all of the queries.
+// What a block of 32 queries and 32 keys is, as far as the window goes: out of sight, or seen whole by all of the queries.
 __device__ __forceinline__ bool block_dead(const WindowArgs& a, int q0, int k0) {
   return k0 > q0 + 31 + a.right || (k0 + 31 < q0 - a.left && k0 >= a.sinks);
 }
 __device__ __forceinline__ bool block_whole(const WindowArgs& a, int q0, int k0) {
   return k0 + 31 <= q0 + a.right && (k0 >= q0 + 31 - a.left || k0 + 32 <= a.sinks);
 }
+// For the 32 queries of a warp: which runs of keys are plain, that is seen whole, and with one bias for all.  Formed once, so that the tiles in the
+// middle of a wide window cost four comparisons.
+struct PlainKeys {
+  int lo, hi, sink, low, high;
+  bool none;
+  float flat_low, flat_high;
+  __device__ __forceinline__ PlainKeys(const WindowArgs& a, int q0, const float* bias, int bias_floats) {
+    none = a.mask != nullptr;
+    lo = q0 + 31 - a.left, hi = min(q0 + a.right, a.n - 1), sink = a.sinks - 1;      // first and last key of a run
+    low = a.r < 0 ? 0x3fffffff : q0 - a.r, high = a.r < 0 ? 0x3fffffff : q0 + 31 + a.r;
+    flat_low = a.r < 0 ? 0.f : bias[0], flat_high = a.r < 0 ? 0.f : bias[bias_floats - 1];
+  }
+  __device__ __forceinline__ bool plain(int first, int last) const {
+    return !none && last <= hi && (first >= lo || last <= sink) && (last <= low || first >= high);
+  }
+  __device__ __forceinline__ float flat(int last) const { return last <= low ? flat_low : flat_high; }
+};
 
 // The learned bias of one head times log2(e), by offset j - i and continued beyond +-r far enough that every offset of a block of 32 x 32 that reaches
 // into (-r, r) has its place.

@@ -12,6 +12,8 @@
 // Keys that are sinks are seen by all later queries.  Their CTA takes the queries of the window, like any other; the
 // queries beyond are cut into chunks of about as many tiles, a CTA each, and window_sink_kernel adds the chunks up in their order.
 #pragma once
+#include <type_traits>
+
 #include "px_window.cuh"
 
 namespace px {
@@ -180,13 +182,13 @@ window_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     const float nlse = g.nlse[(size_t)bh * a.npad + i];
     float* const sums = bias + ext * (1 + warp);                   // by offset, as the bias lies
     float* const stage = bias + ext * 9 + 32 * warp;
+    const f32x2 scale = both2(a.c), ndelta2 = both2(ndelta);
+    const float flat_low = a.r < 0 ? 0.f : bias[0], flat_high = a.r < 0 ? 0.f : bias[ext - 1];
     bool ok = true;
     for (int t = 0; t < tiles.count; ++t) {
       const int k0 = tiles.key(t), kh = k0 + 32 * half;
-      const uint32_t keys = key_bits(a, batch, kh, lane);
+      const uint32_t keys = a.mask || kh + 32 > a.n ? key_bits(a, batch, kh, lane) : 0xffffffffu;
       const bool dead = keys == 0 || block_dead(a, qw, kh);
-      // masked keys of the tile: their rows of K become zeros, those of this half by its four warps
-      const bool hidden = keys != bits_between(0, a.n - 1 - kh);
       ok = mbar_wait(&bars.ready, t & 1, 32u);
       __syncwarp();
       tc_fence_after();
@@ -202,25 +204,25 @@ window_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       ok = L::ahead ? __all_sync(0xffffffffu, ok) != 0 : barrier_all(2 + quarter, 64, ok);
       if (!ok) break;
       if (lane == 0) mbar_arrive(&bars.taken);
-      const BlockBias bb(a, bias, qw, kh);
+      const bool is_low = kh + 31 - qw <= -a.r, near = a.r >= 0 && !is_low && kh - qw - 31 < a.r;
       if (!dead) {
-        const float shift = nlse + bb.flat;
-        if (bb.near) {
+        if (near) {
           const float* const y = bias_row(a, bias, i, kh);
 #pragma unroll
-          for (int c = 0; c < 32; c += 2) {
-            float y0 = y[c], y1 = y[c + 1];
-            add2(y0, y1, nlse, nlse);
-            fma2(s[c], s[c + 1], s[c], s[c + 1], a.c, a.c, y0, y1);
-          }
+          for (int c = 0; c < 32; ++c) s[c] = fmaf(s[c], a.c, y[c] + nlse);
         } else {
+          const float shift = nlse + (is_low ? flat_low : flat_high);
+          const f32x2 shift2 = pair2(shift, shift);
 #pragma unroll
-          for (int c = 0; c < 32; c += 2) fma2(s[c], s[c + 1], s[c], s[c + 1], a.c, a.c, shift, shift);
+          for (int c = 0; c < 32; c += 2) {
+            const float2 x = apart2(fma2(pair2(s[c], s[c + 1]), scale, shift2));
+            s[c] = x.x, s[c + 1] = x.y;
+          }
         }
 #pragma unroll
         for (int c = 0; c < 32; c += 2) {
-          add2(d[c], d[c + 1], ndelta, ndelta);
-          mul2(d[c], d[c + 1], fast_exp2(s[c]), fast_exp2(s[c + 1]));
+          const float2 x = apart2(mul2(add2(pair2(d[c], d[c + 1]), ndelta2), pair2(fast_exp2(s[c]), fast_exp2(s[c + 1]))));
+          d[c] = x.x, d[c + 1] = x.y;
         }
         if (keys != 0xffffffffu || !block_whole(a, qw, kh)) {
           const uint32_t seen = visible_bits(a, i, kh, keys);
@@ -240,7 +242,8 @@ window_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       }
       tc_fence_after();
       tmem_st16(t_lane + L::col_ds + 16 * half, w);
-      if (hidden) {
+      // masked keys of the tile: their rows of K become zeros, those of this half by its four warps
+      if (keys != 0xffffffffu && keys != bits_between(0, a.n - 1 - kh)) {
         mbar_wait(&bars.first_full[t % kStages], (t / kStages) & 1, 128u);      // complete: S(t) is; orders these writes behind the copy's
         if (!(keys >> lane & 1)) clear_row<kPanels, kWCols>(sm + L::k + (t % kStages) * L::tile, 32 * half + lane, quarter, 4);
         fence_async_shared();
@@ -250,7 +253,7 @@ window_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars.given);
       if (kBiasGrad && !dead) {
-        if (bb.near) {
+        if (near) {
           // Sums along the diagonals of a 32 x 32 block: the running sum moves one lane on with each column, and leaves by the last lane.
           float run = 0.f;
 #pragma unroll
@@ -266,11 +269,12 @@ window_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           if (lane < 31) at[31 - lane] += run;
           __syncwarp();
         } else {
-          float v0 = 0.f, v1 = 0.f;
+          f32x2 v = pair2(0.f, 0.f);
 #pragma unroll
-          for (int c = 0; c < 32; c += 2) add2(v0, v1, d[c], d[c + 1]);
-          if (bb.low) low += v0 + v1;
-          else high += v0 + v1;
+          for (int c = 0; c < 32; c += 2) v = add2(v, pair2(d[c], d[c + 1]));
+          const float2 x = apart2(v);
+          if (is_low) low += x.x + x.y;
+          else high += x.x + x.y;
         }
       }
     }
@@ -353,16 +357,17 @@ __global__ void __launch_bounds__(1024) window_dbias_kernel(const float* __restr
 
 // ---- dK, dV ----------------------------------------------------------------------------------------------------------
 // TMEM, heads up to 32: S^T (64) | dP^T (64) | P^T (32) | dS^T (32) | dV (32) | dK (32), two CTAs an SM; beyond 64 the same with dV and dK of 128 and one CTA.
-// The next S^T and dP^T are made while these P^T and dS^T are.  Heads of 33 to 64: S^T | dP^T | dV (64) | dK (64), P^T and dS^T in the places of S^T and dP^T.
+// Heads of 33 to 64: S^T | dP^T | dV (64) | dK (64), P^T and dS^T in shared memory.  The next S^T and dP^T are made while these P^T and dS^T are.
 template <int kD>
 struct WindowDkvLayout {
   static constexpr int panels = kD > 64 ? 2 : 1, tile = panels * kWCols * 128, stat = 2 * kWCols * 4;
-  static constexpr bool ahead = kD != 64;
+  static constexpr bool p_shared = kD == 64;
   static constexpr int cols = kD == 128 ? 512 : 256, ctas = kD == 128 ? 1 : 2;
-  static constexpr int col_p = ahead ? 2 * kWCols : 0, col_ds = ahead ? col_p + kWCols / 2 : kWCols;
-  static constexpr int col_v = ahead ? 3 * kWCols : 2 * kWCols, col_k = col_v + kD;
+  static constexpr int col_p = 2 * kWCols, col_ds = col_p + kWCols / 2;
+  static constexpr int col_v = p_shared ? 2 * kWCols : 3 * kWCols, col_k = col_v + kD;
   static_assert(col_k + kD <= cols, "tensor memory of a CTA");
-  static constexpr int k = 0, v = panels * kWRows * 128, q = 2 * v, dout = q + 2 * tile, stats = dout + 2 * tile, bars = stats + 2 * stat;
+  static constexpr int k = 0, v = panels * kWRows * 128, q = 2 * v, dout = q + 2 * tile, p = dout + 2 * tile;
+  static constexpr int ds = p + (p_shared ? kWRows * 128 : 0), stats = ds + (p_shared ? kWRows * 128 : 0), bars = stats + 2 * stat;
   static constexpr int bias = bars + 128;
   static constexpr int bytes(int r) { return bias + bias_floats(r) * 4; }
 };
@@ -476,43 +481,40 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       ok = mbar_wait_warp(&bars.own_full, 0, 1u) && issue(0);
     }
     for (int t = 0; t < tiles.count && ok; ++t) {
-      if (L::ahead) {
-        ok = mbar_wait_warp(&bars.taken, t & 1, 8u);
+      ok = mbar_wait_warp(&bars.taken, t & 1, 8u);
+      if (!ok) break;
+      if (t > 0 && t + 1 < tiles.count) {                     // the streamed tile of the step before is free
+        ok = mbar_wait_warp(&bars.done, (t - 1) & 1, 16u);
         if (!ok) break;
-        if (t > 0 && t + 1 < tiles.count) {                   // the streamed tile of the step before is free
-          ok = mbar_wait_warp(&bars.done, (t - 1) & 1, 16u);
-          if (!ok) break;
-          if (elect_lane()) load((t + 1) & 1);
-          __syncwarp();
-          coming.next(tiles);
-        }
-        if (t + 1 < tiles.count && !(ok = issue(t + 1))) break;
+        if (elect_lane()) load((t + 1) & 1);
+        __syncwarp();
+        coming.next(tiles);
       }
+      if (t + 1 < tiles.count && !(ok = issue(t + 1))) break;
       ok = mbar_wait_warp(&bars.given, t & 1, 8u);
       if (!ok) break;
       tc_fence_after();
       if (elect_lane()) {
         const int s = t & 1;
-        mma_streamed<kWCols>(tmem + L::col_v, tmem + L::col_p, do_at + s * L::tile, idesc_d, t == 0);
-        mma_streamed<kWCols>(tmem + L::col_k, tmem + L::col_ds, q_at + s * L::tile, idesc_d, t == 0);
+        if (L::p_shared) {
+          mma_streamed_ss(tmem + L::col_v, smem_u32(sm + L::p), do_at + s * L::tile, idesc_d, t == 0);
+          mma_streamed_ss(tmem + L::col_k, smem_u32(sm + L::ds), q_at + s * L::tile, idesc_d, t == 0);
+        } else {
+          mma_streamed<kWCols>(tmem + L::col_v, tmem + L::col_p, do_at + s * L::tile, idesc_d, t == 0);
+          mma_streamed<kWCols>(tmem + L::col_k, tmem + L::col_ds, q_at + s * L::tile, idesc_d, t == 0);
+        }
         umma_commit(&bars.done);
       }
       __syncwarp();
-      if (!L::ahead) {
-        ok = mbar_wait_warp(&bars.done, t & 1, 16u);          // the streamed tile and the places of S^T and dP^T are free
-        if (!ok) break;
-        if (t + 2 < tiles.count) {
-          if (elect_lane()) load(t & 1);
-          __syncwarp();
-          coming.next(tiles);
-        }
-        if (t + 1 < tiles.count) ok = issue(t + 1);
-      }
     }
   } else {
     // ------------------------------------------------------------------ one key row x 32 queries a thread
     const int quarter = warp & 3, half = warp >> 2, row = 32 * quarter + lane, j = k0 + row, kw = k0 + 32 * quarter;
     const uint32_t t_lane = tmem + ((uint32_t)(32 * quarter) << 16);
+    const f32x2 scale = both2(a.c);
+    // blocks of queries from qh on that see all of this warp's keys, and those whose bias is the first or the last entry for all
+    const int whole_from = any_masked ? 0x3fffffff : kw + 31 - a.right, whole_to = min(kw + 32 <= a.sinks ? a.n : kw - 31 + a.left, a.n - 32);
+    const int low_from = kw + 31 + a.r, high_to = kw - 31 - a.r;
     bool ok = true;
     int filled = -1;                               // the group's head whose bias is in shared memory
     const bool wide = a.r >= 0 && a.group > 1;     // the bias changes on the way: all eight warps keep together
@@ -533,97 +535,111 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       ok = mbar_wait(&bars.first_full[s], (t >> 1) & 1, 64u) && ok;
       __syncwarp();
       tc_fence_after();
-      float p[32], d[32];
-      if (!dead) {
-        tmem_ld32(t_lane + 32 * half, *reinterpret_cast<uint32_t(*)[32]>(&p[0]));
-        tmem_ld32(t_lane + kWCols + 32 * half, *reinterpret_cast<uint32_t(*)[32]>(&d[0]));
-        tmem_wait_ld();
+      uint32_t wp[16], wd[16], nothing = 0, seen = 0xffffffffu;
+      bool near = false;
+      float flat = 0.f;
+      const float* y = bias;
+      if (a.r >= 0) {
+        const bool high = qh <= high_to;
+        near = !high && qh < low_from;
+        flat = near ? 0.f : bias[high ? bias_floats(a.r) - 1 : 0];
+        if (near) y = bias_row(a, bias, qh, j);                 // of query qh + c: y[-c]
       }
-      tc_fence_before();
-      // where P^T and dS^T go to the places of S^T and dP^T, both halves have to have read these
-      if (L::ahead && !wide) ok = __all_sync(0xffffffffu, ok) != 0;
-      else ok = barrier_all(wide ? 1 : 2 + quarter, wide ? 256 : 64, ok);
-      if (!ok) break;
-      if (L::ahead && lane == 0) mbar_arrive(&bars.taken);
-      uint32_t wp[16], wd[16];
-      if (!dead) {
-        const float4* const nlse4 = reinterpret_cast<const float4*>(sm + L::stats + s * L::stat) + 8 * half;
-        const float4* const ndelta4 = nlse4 + kWCols / 4;
-        const BlockBias bb(a, bias, qh, kw);
-        if (bb.near) {
-          const float* const y = bias_row(a, bias, qh, j);      // of query qh + c: y[-c]
+      if (qh < whole_from || qh > whole_to)
+        // queries j - right .. j + left, all from j - right on for a sink, none for a masked key
+        seen = bits_between(j - a.right - qh, masked ? -1 : j < a.sinks ? 31 : j + a.left - qh);
+      if (a.mask) {
+        const float* const mine = reinterpret_cast<const float*>(sm + L::stats + s * L::stat) + 32 * half;
+        nothing = __ballot_sync(0xffffffffu, mine[lane] == -CUDART_INF_F);      // queries that see nothing
+        seen &= ~nothing;
+      }
+      const bool seen_all = __all_sync(0xffffffffu, seen == 0xffffffffu);
 #pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            float4 l4 = nlse4[c];
-            add2(l4.x, l4.y, y[-4 * c], y[-4 * c - 1]);
-            add2(l4.z, l4.w, y[-4 * c - 2], y[-4 * c - 3]);
-            fma2(p[4 * c], p[4 * c + 1], p[4 * c], p[4 * c + 1], a.c, a.c, l4.x, l4.y);
-            fma2(p[4 * c + 2], p[4 * c + 3], p[4 * c + 2], p[4 * c + 3], a.c, a.c, l4.z, l4.w);
+      for (int h = 0; h < 2; ++h) {                             // 16 columns at a time, for the registers' sake
+        float p[16], d[16];
+        if (!dead) {
+          tmem_ld16(t_lane + 32 * half + 16 * h, *reinterpret_cast<uint32_t(*)[16]>(&p[0]));
+          tmem_ld16(t_lane + kWCols + 32 * half + 16 * h, *reinterpret_cast<uint32_t(*)[16]>(&d[0]));
+          tmem_wait_ld();
+        }
+        if (h == 1) {
+          tc_fence_before();
+          ok = wide ? barrier_all(1, 256, ok) : __all_sync(0xffffffffu, ok) != 0;
+          if (!ok) break;
+          if (lane == 0) mbar_arrive(&bars.taken);
+        }
+        if (dead) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) wp[8 * h + e] = wd[8 * h + e] = 0u;
+          continue;
+        }
+        const ulonglong2* const nlse4 = reinterpret_cast<const ulonglong2*>(sm + L::stats + s * L::stat) + 8 * half + 4 * h;
+        const ulonglong2* const ndelta4 = nlse4 + kWCols / 4;
+        if (near) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const ulonglong2 l4 = nlse4[c];
+            const int b = 16 * h + 4 * c;
+            const float2 u = apart2(fma2(pair2(p[4 * c], p[4 * c + 1]), scale, add2(l4.x, pair2(y[-b], y[-b - 1]))));
+            const float2 v = apart2(fma2(pair2(p[4 * c + 2], p[4 * c + 3]), scale, add2(l4.y, pair2(y[-b - 2], y[-b - 3]))));
+            p[4 * c] = u.x, p[4 * c + 1] = u.y, p[4 * c + 2] = v.x, p[4 * c + 3] = v.y;
+          }
+        } else {
+          const f32x2 flat2 = pair2(flat, flat);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const ulonglong2 l4 = nlse4[c];
+            const float2 u = apart2(fma2(pair2(p[4 * c], p[4 * c + 1]), scale, add2(l4.x, flat2)));
+            const float2 v = apart2(fma2(pair2(p[4 * c + 2], p[4 * c + 3]), scale, add2(l4.y, flat2)));
+            p[4 * c] = u.x, p[4 * c + 1] = u.y, p[4 * c + 2] = v.x, p[4 * c + 3] = v.y;
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const ulonglong2 e4 = ndelta4[c];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) p[4 * c + x] = fast_exp2(p[4 * c + x]);
+          const float2 u = apart2(mul2(add2(pair2(d[4 * c], d[4 * c + 1]), e4.x), pair2(p[4 * c], p[4 * c + 1])));
+          const float2 v = apart2(mul2(add2(pair2(d[4 * c + 2], d[4 * c + 3]), e4.y), pair2(p[4 * c + 2], p[4 * c + 3])));
+          d[4 * c] = u.x, d[4 * c + 1] = u.y, d[4 * c + 2] = v.x, d[4 * c + 3] = v.y;
+        }
+        if (seen_all) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            wp[8 * h + e] = pack16x2<kF16>(p[2 * e], p[2 * e + 1]);
+            wd[8 * h + e] = pack16x2<kF16>(d[2 * e], d[2 * e + 1]);
           }
         } else {
 #pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            float4 l4 = nlse4[c];
-            add2(l4.x, l4.y, bb.flat, bb.flat);
-            add2(l4.z, l4.w, bb.flat, bb.flat);
-            fma2(p[4 * c], p[4 * c + 1], p[4 * c], p[4 * c + 1], a.c, a.c, l4.x, l4.y);
-            fma2(p[4 * c + 2], p[4 * c + 3], p[4 * c + 2], p[4 * c + 3], a.c, a.c, l4.z, l4.w);
-          }
-        }
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          const float4 e4 = ndelta4[c];
-          add2(d[4 * c], d[4 * c + 1], e4.x, e4.y);
-          add2(d[4 * c + 2], d[4 * c + 3], e4.z, e4.w);
-#pragma unroll
-          for (int x = 0; x < 4; ++x) p[4 * c + x] = fast_exp2(p[4 * c + x]);
-          mul2(d[4 * c], d[4 * c + 1], p[4 * c], p[4 * c + 1]);
-          mul2(d[4 * c + 2], d[4 * c + 3], p[4 * c + 2], p[4 * c + 3]);
-        }
-        if (any_masked || !block_whole(a, qh, kw)) {
-          // queries j - right .. j + left, all from j - right on for a sink, none for a masked key
-          const int from = j - a.right - qh, to = masked ? -1 : j < a.sinks ? 31 : j + a.left - qh;
-          const uint32_t seen = bits_between(from, to);
-#pragma unroll
-          for (int c = 0; c < 32; ++c) {
-            const bool see = seen >> c & 1u;
-            p[c] = see ? p[c] : 0.f;
-            d[c] = see ? d[c] : 0.f;
+          for (int e = 0; e < 8; ++e) {
+            const bool a0 = seen >> (16 * h + 2 * e) & 1u, a1 = seen >> (16 * h + 2 * e + 1) & 1u;
+            wp[8 * h + e] = pack16x2<kF16>(a0 ? p[2 * e] : 0.f, a1 ? p[2 * e + 1] : 0.f);
+            wd[8 * h + e] = pack16x2<kF16>(a0 ? d[2 * e] : 0.f, a1 ? d[2 * e + 1] : 0.f);
           }
         }
       }
-      if (a.mask) {
-        // queries that see nothing: whatever their rows of Q and dO hold becomes zeros; those of this half by its four warps
-        const float* const mine = reinterpret_cast<const float*>(sm + L::stats + s * L::stat) + 32 * half;
-        const uint32_t nothing = __ballot_sync(0xffffffffu, mine[lane] == -CUDART_INF_F);
-        if (nothing) {
-          if (!dead) {
-#pragma unroll
-            for (int c = 0; c < 32; ++c)
-              if (nothing >> c & 1u) p[c] = d[c] = 0.f;
-          }
-          if (nothing >> lane & 1u) {
-            clear_row<kPanels, kWCols>(sm + L::q + s * L::tile, 32 * half + lane, quarter, 4);
-            clear_row<kPanels, kWCols>(sm + L::dout + s * L::tile, 32 * half + lane, quarter, 4);
-          }
-          fence_async_shared();
+      if (!ok) break;
+      if (nothing) {                                // whatever their rows of Q and dO hold becomes zeros; those of this half by its four warps
+        if (nothing >> lane & 1u) {
+          clear_row<kPanels, kWCols>(sm + L::q + s * L::tile, 32 * half + lane, quarter, 4);
+          clear_row<kPanels, kWCols>(sm + L::dout + s * L::tile, 32 * half + lane, quarter, 4);
         }
       }
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        wp[e] = dead ? 0u : pack16x2<kF16>(p[2 * e], p[2 * e + 1]);
-        wd[e] = dead ? 0u : pack16x2<kF16>(d[2 * e], d[2 * e + 1]);
-      }
-      if (L::ahead && t > 0) {                      // the products before have read their P^T and dS^T
+      if (t > 0) {                                  // the products before have read their P^T and dS^T
         ok = mbar_wait(&bars.done, (t - 1) & 1, 64u);
-        if (!wide) ok = __all_sync(0xffffffffu, ok) != 0;
-        else ok = barrier_all(1, 256, ok);
+        ok = wide ? barrier_all(1, 256, ok) : __all_sync(0xffffffffu, ok) != 0;
         if (!ok) break;
       }
       tc_fence_after();
-      tmem_st16(t_lane + L::col_p + 16 * half, wp);
-      tmem_st16(t_lane + L::col_ds + 16 * half, wd);
-      tmem_wait_st();
+      if (L::p_shared) {
+        panel_store(sm + L::p, row, half, wp);
+        panel_store(sm + L::ds, row, half, wd);
+      } else {
+        tmem_st16(t_lane + L::col_p + 16 * half, wp);
+        tmem_st16(t_lane + L::col_ds + 16 * half, wd);
+        tmem_wait_st();
+      }
+      if (L::p_shared || nothing) fence_async_shared();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars.given);

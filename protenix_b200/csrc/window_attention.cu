@@ -18,6 +18,8 @@
 // continued beyond its ends, so that a thread's 64 values lie side by side.
 //
 // TMEM: S / P (64 columns) | O.  d <= 64: 128 columns, four CTAs an SM hide one another's chain of product, softmax, product.
+#include <type_traits>
+
 #include "px_window.cuh"
 
 namespace px {
@@ -34,11 +36,13 @@ static_assert(sizeof(WindowFwdBars) <= 128, "room for the barriers");
 // kD: the head size that the accumulator has room for, 32, 64 or 128.
 template <int kD>
 struct WindowFwdLayout {
-  static constexpr int panels = kD > 64 ? 2 : 1, keys = kD == 64 ? 128 : 64, ctas = kD == 32 ? 4 : 2;
-  static constexpr int cols = kD == 32 ? 128 : 256, col_p = keys, col_o = keys + keys / 2;      // S | P | O
+  static constexpr int panels = kD > 64 ? 2 : 1, keys = 64, ctas = kD == 32 ? 4 : kD == 64 ? 3 : 2;
+  // TMEM: S | P | O.  Heads of 33 to 64: S | O, and P in shared memory, so that 128 columns are enough.
+  static constexpr bool p_shared = kD == 64;
+  static constexpr int cols = kD == 128 ? 256 : 128, col_p = keys, col_o = p_shared ? keys : keys + keys / 2;
   static_assert(col_o + kD <= cols, "tensor memory of a CTA");
   static constexpr int q = 0, tile = panels * keys * 128;
-  static constexpr int k = panels * kWRows * 128, v = k + 2 * tile, bars = v + 2 * tile;
+  static constexpr int k = panels * kWRows * 128, v = k + 2 * tile, p = v + 2 * tile, bars = p + (p_shared ? kWRows * 128 : 0);
   static constexpr int bias = bars + 128;
   static constexpr int bytes(int r) { return bias + bias_floats(r) * 4; }
 };
@@ -129,7 +133,8 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       if (!ok) break;
       tc_fence_after();
       if (elect_lane()) {
-        mma_streamed<kKT>(tmem + L::col_o, tmem + L::col_p, v_at + (t & 1) * L::tile, idesc_o, t == 0);
+        if (L::p_shared) mma_streamed_ss(tmem + L::col_o, smem_u32(sm + L::p), v_at + (t & 1) * L::tile, idesc_o, t == 0);
+        else mma_streamed<kKT>(tmem + L::col_o, tmem + L::col_p, v_at + (t & 1) * L::tile, idesc_o, t == 0);
         umma_commit(&bars.pv_done);
       }
       __syncwarp();
@@ -138,21 +143,26 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     // ------------------------------------------------------------------ one query row a thread
     const int row = threadIdx.x, i = q0 + row, qw = q0 + 32 * warp;
     const uint32_t t_s = tmem + ((uint32_t)(32 * warp) << 16), t_p = t_s + L::col_p, t_o = t_s + L::col_o;
-    float m = -CUDART_INF_F, l0 = 0.f, l1 = 0.f;
-    bool ok = true;
-    for (int t = 0; t < tiles.count; ++t) {
-      const int k0 = tiles.key(t);
+    float m = -CUDART_INF_F;
+    f32x2 l = pair2(0.f, 0.f);
+    const f32x2 scale = both2(a.c);
+    const PlainKeys runs(a, qw, bias, bias_floats(a.r));
+    // One tile: S into registers, P out of them.  kPlain: all of it is seen, with one bias.
+    const auto work = [&](int t, int k0, auto plain) {
+      constexpr bool kPlain = decltype(plain)::value;
       uint32_t keys[kBlocks];
       bool dead[kBlocks], hidden = false;
 #pragma unroll
       for (int b = 0; b < kBlocks; ++b) {
+        dead[b] = false;
+        if (kPlain) continue;
         keys[b] = key_bits(a, batch, k0 + 32 * b, lane);
         dead[b] = keys[b] == 0 || block_dead(a, qw, k0 + 32 * b);
         hidden = hidden || keys[b] != bits_between(0, a.n - 1 - (k0 + 32 * b));
       }
-      ok = mbar_wait(&bars.s_full, t & 1, 32u);
+      bool ok = mbar_wait(&bars.s_full, t & 1, 32u);
       ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
+      if (!ok) return false;
       tc_fence_after();
       float s[kKT];
 #pragma unroll
@@ -162,33 +172,42 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars.s_free);
       // logits = s * mul + add, in base 2
-      float mul[kBlocks], add[kBlocks], mt = -CUDART_INF_F;
+      float mt = -CUDART_INF_F, add[kBlocks];
+      f32x2 mul[kBlocks];
+      if (kPlain) {
+        mt = max32(s);
 #pragma unroll
-      for (int b = 0; b < kBlocks; ++b) {
-        if (dead[b]) continue;
-        const int kb = k0 + 32 * b;
-        float* const x = s + 32 * b;
-        const BlockBias bb(a, bias, qw, kb);
-        mul[b] = a.c, add[b] = bb.flat;
-        if (bb.near) {
-          const float* const y = bias_row(a, bias, i, kb);
+        for (int b = 1; b < kBlocks; ++b) mt = fmaxf(mt, max32(s + 32 * b));
+        add[0] = runs.flat(k0 + kKT - 1);
+        mt = fmaf(mt, a.c, add[0]);
+      } else {
 #pragma unroll
-          for (int c = 0; c < 32; c += 2) fma2(x[c], x[c + 1], x[c], x[c + 1], a.c, a.c, y[c], y[c + 1]);
-          mul[b] = 1.f, add[b] = 0.f;
+        for (int b = 0; b < kBlocks; ++b) {
+          if (dead[b]) continue;
+          const int kb = k0 + 32 * b;
+          float* const x = s + 32 * b;
+          const BlockBias bb(a, bias, qw, kb);
+          mul[b] = scale, add[b] = bb.flat;
+          if (bb.near) {
+            const float* const y = bias_row(a, bias, i, kb);
+#pragma unroll
+            for (int c = 0; c < 32; ++c) x[c] = fmaf(x[c], a.c, y[c]);
+            mul[b] = pair2(1.f, 1.f), add[b] = 0.f;
+          }
+          if (keys[b] != 0xffffffffu || !block_whole(a, qw, kb)) {
+            const uint32_t seen = visible_bits(a, i, kb, keys[b]);
+#pragma unroll
+            for (int c = 0; c < 32; ++c) x[c] = (seen >> c & 1u) ? x[c] : -CUDART_INF_F;
+          }
+          mt = fmaxf(mt, fmaf(max32(x), bb.near ? 1.f : a.c, add[b]));
         }
-        if (keys[b] != 0xffffffffu || !block_whole(a, qw, kb)) {
-          const uint32_t seen = visible_bits(a, i, kb, keys[b]);
-#pragma unroll
-          for (int c = 0; c < 32; ++c) x[c] = (seen >> c & 1u) ? x[c] : -CUDART_INF_F;
-        }
-        mt = fmaxf(mt, fmaf(max32(x), mul[b], add[b]));
       }
       const bool up = mt > m + kWRescaleGap;
       const bool move = __any_sync(0xffffffffu, up) && t > 0;      // the first product overwrites O
       const float m_old = m;
       m = up ? mt : m;
       const float shift = m == -CUDART_INF_F ? 0.f : -m;
-      float r0 = 0.f, r1 = 0.f;
+      f32x2 sum = pair2(0.f, 0.f);
       uint32_t w[kKT / 2];
 #pragma unroll
       for (int b = 0; b < kBlocks; ++b) {
@@ -197,25 +216,25 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           for (int e = 0; e < 16; ++e) w[16 * b + e] = 0u;
           continue;
         }
-        const float sh = add[b] + shift;
+        const float sh = add[kPlain ? 0 : b] + shift;
+        const f32x2 sh2 = pair2(sh, sh), mul2 = kPlain ? scale : mul[b];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          float p0 = s[32 * b + 2 * e], p1 = s[32 * b + 2 * e + 1];
-          fma2(p0, p1, p0, p1, mul[b], mul[b], sh, sh);
-          p0 = fast_exp2(p0), p1 = fast_exp2(p1);
-          add2(r0, r1, p0, p1);
+          const float2 x = apart2(fma2(pair2(s[32 * b + 2 * e], s[32 * b + 2 * e + 1]), mul2, sh2));
+          const float p0 = fast_exp2(x.x), p1 = fast_exp2(x.y);
+          sum = add2(sum, pair2(p0, p1));
           w[16 * b + e] = pack16x2<kF16>(p0, p1);
         }
       }
       if (t > 0) {                                                  // P and O are at rest
         ok = mbar_wait(&bars.pv_done, (t - 1) & 1, 128u);
         ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
+        if (!ok) return false;
         tc_fence_after();
       }
       if (move) {
         const float alpha = up ? fast_exp2(m_old - m) : 1.f;
-        l0 *= alpha, l1 *= alpha;
+        l = mul2(l, pair2(alpha, alpha));
         for (int c = 0; c < a.d; c += 16) {
           uint32_t x[16];
           tmem_ld16(t_o + c, x);
@@ -225,32 +244,41 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           tmem_st16(t_o + c, x);
         }
       }
-      add2(l0, l1, r0, r1);
+      l = add2(l, sum);
 #pragma unroll
-      for (int b = 0; b < kBlocks; ++b) tmem_st16(t_p + 16 * b, *reinterpret_cast<const uint32_t(*)[16]>(&w[16 * b]));
+      for (int b = 0; b < kBlocks; ++b) {
+        if (L::p_shared) panel_store(sm + L::p, row, b, *reinterpret_cast<const uint32_t(*)[16]>(&w[16 * b]));
+        else tmem_st16(t_p + 16 * b, *reinterpret_cast<const uint32_t(*)[16]>(&w[16 * b]));
+      }
       if (hidden) {                                                 // masked keys: their rows of V
-        ok = mbar_wait_warp(&bars.v_full[t & 1], (t >> 1) & 1, 64u);
-        if (!ok) break;
+        if (!mbar_wait_warp(&bars.v_full[t & 1], (t >> 1) & 1, 64u)) return false;
         constexpr int kParts = 128 / kKT;
         const int r = row % kKT;
         uint32_t word = keys[0];
 #pragma unroll
         for (int b = 1; b < kBlocks; ++b) word = r >> 5 == b ? keys[b] : word;
         if (!(word >> (r & 31) & 1)) clear_row<kPanels, kKT>(sm + L::v + (t & 1) * L::tile, r, row / kKT, kParts);
-        fence_async_shared();
       }
+      if (L::p_shared || hidden) fence_async_shared();
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars.p_ready);
+      return true;
+    };
+    bool ok = true;
+    for (int t = 0; t < tiles.count && ok; ++t) {
+      const int k0 = tiles.key(t);
+      ok = runs.plain(k0, k0 + kKT - 1) ? work(t, k0, std::true_type()) : work(t, k0, std::false_type());
     }
     ok = ok && mbar_wait(&bars.pv_done, (tiles.count - 1) & 1, 128u);
     ok = __all_sync(0xffffffffu, ok);
     if (ok) {
       tc_fence_after();
-      const float l = l0 + l1;
+      const float2 both = apart2(l);
+      const float denominator = both.x + both.y;
       const bool empty = m == -CUDART_INF_F;
-      const float inv = empty ? 0.f : 1.f / l;
+      const float inv = empty ? 0.f : 1.f / denominator;
       uint16_t* const out = o.at(batch, head, i);
       for (int c = 0; c < a.d; c += 16) {
         uint32_t x[16];
@@ -262,7 +290,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         }
       }
       // Rows that see nothing, and those beyond the last, have weights of zero in the backward pass.
-      if (nlse) nlse[(size_t)bh * a.npad + i] = i < a.n && !empty ? -(m + log2f(l)) : -CUDART_INF_F;
+      if (nlse) nlse[(size_t)bh * a.npad + i] = i < a.n && !empty ? -(m + log2f(denominator)) : -CUDART_INF_F;
     }
   }
   tc_fence_before();
