@@ -28,12 +28,13 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
       ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
       : "memory");
 }
-// A tile of `rows` rows as panels of 64 elements (128 bytes, 128-byte swizzle), one behind the other.  Elements beyond d and rows beyond n
-// arrive as zeros.
+// A tile of `rows` rows (a multiple of 64, which is the box) as panels of 64 elements (128 bytes, 128-byte swizzle), one behind the other.  Elements
+// beyond d and rows beyond n arrive as zeros.
 template <int kPanels>
 __device__ __forceinline__ void load_rows(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int rows, int row0, int head, int batch) {
 #pragma unroll
-  for (int p = 0; p < kPanels; ++p) tma_load_4d(dst + p * rows * 128, map, bar, 64 * p, row0, head, batch);
+  for (int p = 0; p < kPanels; ++p)
+    for (int r = 0; r < rows; r += 64) tma_load_4d(dst + (p * rows + r) * 128, map, bar, 64 * p, row0 + r, head, batch);
 }
 
 // D[128][rows of B] = A B^T over d, both K-major panels of 64 (one lane).
@@ -128,8 +129,8 @@ __device__ __forceinline__ float bias_value(const WindowArgs& a, int head, int b
                                            : __half2float(__ldg((const __half*)a.bias + at));
   return v * kLog2e;
 }
-__device__ __forceinline__ void bias_fill(const WindowArgs& a, int head, float* to) {
-  for (int k = threadIdx.x; k < bias_floats(a.r); k += blockDim.x) to[k] = bias_value(a, head, min(max(k - kWBiasBeyond, 0), 2 * a.r));
+__device__ __forceinline__ void bias_fill(const WindowArgs& a, int head, float* to, int threads) {
+  for (int k = threadIdx.x; k < bias_floats(a.r); k += threads) to[k] = bias_value(a, head, min(max(k - kWBiasBeyond, 0), 2 * a.r));
 }
 // How the bias meets a block of 32 queries from q0 and 32 keys from k0: `near`, by offset; otherwise one number, `flat` (the offsets are all clipped
 // to the same side, or there is no bias).
@@ -180,6 +181,15 @@ __device__ __forceinline__ bool barrier_all(int id, int threads, bool ok) {
                : "r"((int)ok), "r"(id), "r"(threads)
                : "memory");
   return all != 0;
+}
+__device__ __forceinline__ void barrier_of(int id, int threads) { asm volatile("barrier.cta.sync %0, %1;\n" ::"r"(id), "r"(threads) : "memory"); }
+__device__ __forceinline__ bool barrier_any(int id, int threads, bool p) {
+  int any;
+  asm volatile("{\n .reg .pred p, q;\n setp.ne.b32 p, %1, 0;\n barrier.cta.red.or.pred q, %2, %3, p;\n selp.b32 %0, 1, 0, q;\n}\n"
+               : "=r"(any)
+               : "r"((int)p), "r"(id), "r"(threads)
+               : "memory");
+  return any != 0;
 }
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
 

@@ -10,7 +10,7 @@
 // products.  dS and P are rounded to the operands' type for the products they enter and stay fp32 in the bias's gradient.
 //
 // Keys that are sinks are seen by all later queries.  Their CTA takes the queries of the window, like any other; the
-// queries beyond are cut into chunks of about as many tiles, a CTA each, and window_sink_kernel adds the chunks up in their order.
+// queries beyond are cut into chunks of about as many tiles, a CTA each, and the last of these CTAs adds the chunks up in their order.
 #pragma once
 #include <type_traits>
 
@@ -25,8 +25,11 @@ struct WindowBwdArgs {
   float* ndelta;                 // -delta, the same shape
   float* dbias;                  // partial sums [batch * heads * tiles][2 r + 1] or NULL
   float* sinks;                  // partial sums [batch * kv_heads][sink_tiles][1 + chunks][2][128][dn] (dK, dV)
+  unsigned int* arrived;         // [batch * kv_heads][sink_tiles]: how many of the sums are there
+  void* dbias_out;               // [heads][2 r + 1], the type of the bias, or NULL
   float scale;
   int sink_tiles, chunks, chunk; // chunk: streamed tiles of one
+  int bias_blocks, batches;      // blocks of 32 buckets a head
 };
 
 struct WindowBwdBars {
@@ -85,12 +88,8 @@ window_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   if (!cta_ready(skip, warp == 8, bars.tmem_base, kCols)) return;
   const uint32_t tmem = bars.tmem_base;
   const int ext = bias_floats(a.r);
-  if (a.r >= 0) {
-    bias_fill(a, head, bias);
-    if (kBiasGrad)
-      for (int k = threadIdx.x; k < 8 * ext; k += kWBwdThreads) bias[ext + k] = 0.f;
-    __syncthreads();
-  }
+  if (blockIdx.x == 0 && warp == 8)      // for window_dkv_kernel, which runs behind this one
+    for (int k = lane; k < g.batches * a.kv_heads * g.sink_tiles; k += 32) g.arrived[k] = 0u;
 
   float low = 0.f, high = 0.f;                     // sums of dS over offsets that are clipped
   if (warp == 8) {
@@ -176,7 +175,12 @@ window_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       }
     }
     part[half * kWRows + row] = sum;
-    asm volatile("bar.sync 1, 256;\n" ::: "memory");
+    if (a.r >= 0) {
+      bias_fill(a, head, bias, 256);
+      if (kBiasGrad)
+        for (int k = threadIdx.x; k < 8 * ext; k += 256) bias[ext + k] = 0.f;
+    }
+    barrier_of(1, 256);
     const float ndelta = -(part[row] + part[kWRows + row]);
     if (half == 0) g.ndelta[(size_t)bh * a.npad + i] = ndelta;      // 0 beyond the last row
     const float nlse = g.nlse[(size_t)bh * a.npad + i];
@@ -333,25 +337,25 @@ window_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   }
 }
 
-// dbias[head][b] of the CTAs' sums, in their order: 32 buckets a block, 32 slices of the CTAs of a head.
-__global__ void __launch_bounds__(1024) window_dbias_kernel(const float* __restrict__ partial, void* __restrict__ dbias, int type, int batches, int heads,
-                                                            int tiles, int buckets) {
-  __shared__ float slice[32][33];
-  const int lane = threadIdx.x & 31, s = threadIdx.x >> 5, b = blockIdx.x * 32 + lane, head = blockIdx.y;
+// dbias[head][b] of the CTAs' sums, in their order: 32 buckets (block `of` of a head's), nine slices of the CTAs of the head, a warp each.
+__device__ __forceinline__ void sum_dbias(const WindowArgs& a, const WindowBwdArgs& g, int head, int of, float* slice) {
+  const int lane = threadIdx.x & 31, s = threadIdx.x >> 5, buckets = 2 * a.r + 1, b = of * 32 + lane;
+  constexpr int kSlices = kWBwdThreads / 32;
   float v = 0.f;
   if (b < buckets)
-    for (int k = s; k < batches * tiles; k += 32)
-      v += partial[((size_t)((k / tiles) * heads + head) * tiles + k % tiles) * buckets + b];
-  slice[s][lane] = v;
+#pragma unroll 4
+    for (int k = s; k < g.batches * a.tiles; k += kSlices)
+      v += g.dbias[((size_t)((k / a.tiles) * a.heads + head) * a.tiles + k % a.tiles) * buckets + b];
+  slice[s * 32 + lane] = v;
   __syncthreads();
   if (s == 0 && b < buckets) {
     float sum = 0.f;
 #pragma unroll
-    for (int e = 0; e < 32; ++e) sum += slice[e][lane];
+    for (int e = 0; e < kSlices; ++e) sum += slice[e * 32 + lane];
     const size_t at = (size_t)head * buckets + b;
-    if (type == PX_F32) ((float*)dbias)[at] = sum;
-    else if (type == PX_BF16) ((bf16*)dbias)[at] = __float2bfloat16_rn(sum);
-    else ((__half*)dbias)[at] = __float2half_rn(sum);
+    if (a.bias_type == PX_F32) ((float*)g.dbias_out)[at] = sum;
+    else if (a.bias_type == PX_BF16) ((bf16*)g.dbias_out)[at] = __float2bfloat16_rn(sum);
+    else ((__half*)g.dbias_out)[at] = __float2half_rn(sum);
   }
 }
 
@@ -371,6 +375,24 @@ struct WindowDkvLayout {
   static constexpr int bias = bars + 128;
   static constexpr int bytes(int r) { return bias + bias_floats(r) * 4; }
 };
+
+// The rows of dK and dV of one key tile, from the parts that its CTAs have left: a thread = 8 values.
+template <bool kF16>
+__device__ __forceinline__ void sum_sinks(const WindowArgs& a, const WindowBwdArgs& g, const RowsOut& dk, const RowsOut& dv, int bkv, int own) {
+  const int dn = (a.d + 15) & ~15, pieces = a.d / 8, rows = min(a.n - own * kWRows, kWRows);
+  for (int u = threadIdx.x; u < 2 * rows * pieces; u += kWBwdThreads) {
+    const int c = u % pieces * 8, row = u / pieces % rows, which = u / pieces / rows;
+    const RowsOut& out = which ? dv : dk;
+    if (!out.data) continue;
+    const float* from = g.sinks + ((size_t)bkv * g.sink_tiles + own) * (1 + g.chunks) * 2 * kWRows * dn + (size_t)which * kWRows * dn + (size_t)row * dn + c;
+    float v[8] = {};
+    for (int k = 0; k <= g.chunks; ++k, from += 2 * kWRows * dn) {
+      const float4 x = __ldcg(reinterpret_cast<const float4*>(from)), y = __ldcg(reinterpret_cast<const float4*>(from + 4));
+      v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w, v[4] += y.x, v[5] += y.y, v[6] += y.z, v[7] += y.w;
+    }
+    store8<kF16>(out.at(bkv / a.kv_heads, bkv % a.kv_heads, own * kWRows + row) + c, reinterpret_cast<const uint32_t*>(v), 1.f);
+  }
+}
 
 // The queries of one CTA: streamed tiles first .. first + count - 1 of `per` a head, over the heads of the group.
 struct QueryTiles {
@@ -399,8 +421,15 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   WindowBwdBars& bars = *reinterpret_cast<WindowBwdBars*>(sm + L::bars);
   float* const bias = reinterpret_cast<float*>(sm + L::bias);
   const int warp = warp_index(), lane = threadIdx.x & 31;
+  const int buckets = g.dbias_out ? a.heads * g.bias_blocks : 0;
+  if ((int)blockIdx.x < buckets) {
+    pdl_wait();
+    sum_dbias(a, g, blockIdx.x / g.bias_blocks, blockIdx.x % g.bias_blocks, reinterpret_cast<float*>(sm));
+    return;
+  }
+  const int block = blockIdx.x - buckets;
   // the chunks of the sinks first: they are the longest
-  const int extra = g.sink_tiles * g.chunks, blocks = a.tiles + extra, bkv = blockIdx.x / blocks, at = blockIdx.x % blocks;
+  const int extra = g.sink_tiles * g.chunks, blocks = a.tiles + extra, bkv = block / blocks, at = block % blocks;
   const int kv = bkv % a.kv_heads, batch = bkv / a.kv_heads;
   const int own = at < extra ? at / g.chunks : at - extra, k0 = own * kWRows;
   const int last = last_of_window(a.n, a.left, k0);
@@ -434,9 +463,6 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   if (warp == 8) tmem_alloc(&bars.tmem_base, kCols);
   if (!cta_ready(skip, warp == 8, bars.tmem_base, kCols)) return;
   const uint32_t tmem = bars.tmem_base;
-  const int own_key = min(k0 + (int)(threadIdx.x & 127), a.n - 1);
-  const bool masked = a.mask && __ldg(a.mask + (size_t)batch * a.n + own_key) == 0;
-  const bool any_masked = __syncthreads_or(masked) != 0;
 
   if (warp == 8) {
     // ------------------------------------------------------------------ copies and products
@@ -511,6 +537,8 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     // ------------------------------------------------------------------ one key row x 32 queries a thread
     const int quarter = warp & 3, half = warp >> 2, row = 32 * quarter + lane, j = k0 + row, kw = k0 + 32 * quarter;
     const uint32_t t_lane = tmem + ((uint32_t)(32 * quarter) << 16);
+    const bool masked = a.mask && __ldg(a.mask + (size_t)batch * a.n + min(j, a.n - 1)) == 0;
+    const bool any_masked = a.mask && barrier_any(1, 256, masked);
     const f32x2 scale = both2(a.c);
     // blocks of queries from qh on that see all of this warp's keys, and those whose bias is the first or the last entry for all
     const int whole_from = any_masked ? 0x3fffffff : kw + 31 - a.right, whole_to = min(kw + 32 <= a.sinks ? a.n : kw - 31 + a.left, a.n - 32);
@@ -523,10 +551,9 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       const int qh = (tiles.first + now.tile) * kWCols + 32 * half, s = t & 1;
       if (a.r >= 0 && now.member != filled) {
         // all are past the tile before (barrier below), but not all are through with it
-        asm volatile("bar.sync 1, 256;\n" ::: "memory");
-        for (int k = threadIdx.x; k < bias_floats(a.r); k += 256)
-          bias[k] = bias_value(a, kv * a.group + now.member, min(max(k - kWBiasBeyond, 0), 2 * a.r));
-        asm volatile("bar.sync 1, 256;\n" ::: "memory");
+        barrier_of(1, 256);
+        bias_fill(a, kv * a.group + now.member, bias, 256);
+        barrier_of(1, 256);
         filled = now.member;
       }
       const bool dead = qh >= a.n || block_dead(a, qh, kw);
@@ -651,7 +678,7 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     if (ok) {
       tc_fence_after();
       const int dn = (a.d + 15) & ~15;
-      // where the key is a sink with chunks, this is one of the sums that window_sink_kernel adds up: its own first, then the chunks
+      // where the key is a sink with chunks, this is one of the sums that the last of its CTAs adds up: its own first, then the chunks
       const bool summed = g.chunks > 0 && own < g.sink_tiles;
       float* const to = g.sinks + (((size_t)bkv * g.sink_tiles + own) * (1 + g.chunks) + (at < extra ? 1 + at % g.chunks : 0)) * 2 * kWRows * dn +
                         (size_t)row * dn;
@@ -683,31 +710,24 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       }
     }
   }
+  const bool summed = g.chunks > 0 && own < g.sink_tiles;
+  if (summed) __threadfence();      // this CTA's sums are seen before its arrival is
   tc_fence_before();
   cta_teardown_sync();
   if (warp == 8) {
     tc_fence_after();
     tmem_free(tmem, kCols);
   }
-}
-
-// Rows of dK and dV that the chunks of the sinks have parts of: thread = 8 values.
-template <bool kF16>
-__global__ void __launch_bounds__(256) window_sink_kernel(const WindowArgs a, const WindowBwdArgs g, const RowsOut dk, const RowsOut dv) {
-  const int dn = (a.d + 15) & ~15, pieces = a.d / 8, rows = min(a.n, g.sink_tiles * kWRows), per = (2 * rows * pieces + 255) / 256;
-  const int bkv = blockIdx.x / per, u = blockIdx.x % per * 256 + threadIdx.x;
-  if (u >= 2 * rows * pieces) return;
-  const int c = u % pieces * 8, j = u / pieces % rows, which = u / pieces / rows;
-  const RowsOut& out = which ? dv : dk;
-  if (!out.data) return;
-  const float* from = g.sinks + ((size_t)bkv * g.sink_tiles + j / kWRows) * (1 + g.chunks) * 2 * kWRows * dn + (size_t)which * kWRows * dn +
-                      (size_t)(j % kWRows) * dn + c;
-  float v[8] = {};
-  for (int k = 0; k <= g.chunks; ++k, from += 2 * kWRows * dn) {
-    const float4 x = *reinterpret_cast<const float4*>(from), y = *reinterpret_cast<const float4*>(from + 4);
-    v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w, v[4] += y.x, v[5] += y.y, v[6] += y.z, v[7] += y.w;
+  if (summed) {
+    // whoever arrives last adds the sums up, in their order
+    uint32_t& count = bars.tmem_base;      // no longer needed
+    if (threadIdx.x == 0) count = atomicAdd(g.arrived + (size_t)bkv * g.sink_tiles + own, 1u);
+    __syncthreads();
+    if (count == (uint32_t)g.chunks) {
+      __threadfence();
+      sum_sinks<kF16>(a, g, dk, dv, bkv, own);
+    }
   }
-  store8<kF16>(out.at(bkv / a.kv_heads, bkv % a.kv_heads, j) + c, reinterpret_cast<const uint32_t*>(v), 1.f);
 }
 
 }  // namespace px

@@ -297,9 +297,9 @@ Tensor window_attention(const Tensor& q, const Tensor& k, const Tensor& v, int64
     want.push_back(n);
     if (mask->dim() < 1 || !at::is_expandable_to(mask->sizes(), want)) fail("mask must be [..., N] over the batch axes of q, got " + shape_of(*mask));
     const Tensor truth = mask->scalar_type() == at::kBool ? mask->detach() : mask->detach().ne(0);
-    m = truth.expand(want).reshape({batch, n}).contiguous();
+    m = truth.dim() == 2 && truth.size(0) == batch ? truth.contiguous() : truth.expand(want).reshape({batch, n}).contiguous();
   }
-  const auto four = [&](const Tensor& t) { return t.reshape({batch, t.size(-3), n, d}); };
+  const auto four = [&](const Tensor& t) { return t.dim() == 4 ? t : t.reshape({batch, t.size(-3), n, d}); };
   const Tensor q4 = four(q), k4 = four(k), v4 = four(v);
   const auto wants = [](const Tensor& t) { return t.requires_grad(); };
   Tensor o;
@@ -309,5 +309,5 @@ Tensor window_attention(const Tensor& q, const Tensor& k, const Tensor& v, int64
     const Tensor b = has(bias) ? bias->contiguous() : Tensor();
     o = window_forward(rows_fitted(q4), rows_fitted(k4), rows_fitted(v4), b, m.has_value() ? *m : Tensor(), {left, right, sinks, scale}, nullptr);
   }
-  return o.reshape(q.sizes());
+  return q.dim() == 4 ? o : o.reshape(q.sizes());
 }

@@ -79,11 +79,6 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   if (warp == 4) tmem_alloc(&bars.tmem_base, kCols);
   if (!cta_ready(skip, warp == 4, bars.tmem_base, kCols)) return;
   const uint32_t tmem = bars.tmem_base;
-  if (a.r >= 0) {
-    bias_fill(a, head, bias);
-    __syncthreads();
-  }
-
   if (warp == 4) {
     // ------------------------------------------------------------------ copies and products
     const int kv = head / a.group;
@@ -143,6 +138,10 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     // ------------------------------------------------------------------ one query row a thread
     const int row = threadIdx.x, i = q0 + row, qw = q0 + 32 * warp;
     const uint32_t t_s = tmem + ((uint32_t)(32 * warp) << 16), t_p = t_s + L::col_p, t_o = t_s + L::col_o;
+    if (a.r >= 0) {
+      bias_fill(a, head, bias, 128);
+      barrier_of(1, 128);
+    }
     float m = -CUDART_INF_F;
     f32x2 l = pair2(0.f, 0.f);
     const f32x2 scale = both2(a.c);
@@ -316,15 +315,15 @@ static bool have_context() {
   return cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess;
 }
 
-// [batch][head][n][d] 16-bit values: boxes of 64 elements x `rows`.
-static bool rows_map(CUtensorMap* map, const px_rows& t, const px_window& w, int64_t heads, uint32_t rows) {
+// [batch][head][n][d] 16-bit values: boxes of 64 elements x 64 rows.
+static bool rows_map(CUtensorMap* map, const px_rows& t, const px_window& w, int64_t heads) {
   EncodeTiledFn enc = tensor_map_encoder();
   if (!enc) return false;
   // the stride of an axis of length one is not used, but checked
   const auto stride = [&](int64_t s, int64_t len) { return (cuuint64_t)(len > 1 ? s * 2 : (w.d * 2 + 15) / 16 * 16); };
   const cuuint64_t dims[4] = {(cuuint64_t)w.d, (cuuint64_t)w.n, (cuuint64_t)heads, (cuuint64_t)w.batch};
   const cuuint64_t strides[3] = {stride(t.row, w.n), stride(t.head, heads), stride(t.batch, w.batch)};
-  const cuuint32_t box[4] = {64, rows, 1, 1}, one[4] = {1, 1, 1, 1};
+  const cuuint32_t box[4] = {64, 64, 1, 1}, one[4] = {1, 1, 1, 1};
   return enc(map, w.dtype == PX_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(t.data), dims,
              strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -362,7 +361,7 @@ static bool launch_window_fwd(const px_window& w, const px_rows& q, const px_row
                               float* lse, cudaStream_t st) {
   typedef WindowFwdLayout<kD> L;
   CUtensorMap mq, mk, mv;
-  if (!rows_map(&mq, q, w, w.heads, kWRows) || !rows_map(&mk, k, w, w.kv_heads, L::keys) || !rows_map(&mv, v, w, w.kv_heads, L::keys)) return false;
+  if (!rows_map(&mq, q, w, w.heads) || !rows_map(&mk, k, w, w.kv_heads) || !rows_map(&mv, v, w, w.kv_heads)) return false;
   static SmemLimit limit;
   if (!limit.set(window_fwd_kernel<kF16, kD>, L::bytes(kWMaxR) + 1024)) return false;
   return launch_pdl(window_fwd_kernel<kF16, kD>, dim3((unsigned)((int64_t)a.tiles * w.heads * w.batch)), kWFwdThreads, (size_t)L::bytes(a.r) + 1024,
@@ -404,7 +403,7 @@ static void sink_chunks(const WindowArgs& a, int* tiles, int* chunks, int* chunk
 }
 static int64_t al256(int64_t n) { return (n + 255) / 256 * 256; }
 struct WindowSpace {
-  int64_t delta, dbias, sinks, total;      // where they begin; bytes
+  int64_t delta, dbias, sinks, arrived, total;      // where they begin; bytes
 };
 static WindowSpace window_space(const px_window& w, const WindowArgs& a, bool bias_grad) {
   int tiles, chunks, chunk;
@@ -413,16 +412,11 @@ static WindowSpace window_space(const px_window& w, const WindowArgs& a, bool bi
   s.delta = 0;
   s.dbias = al256(w.batch * w.heads * (int64_t)a.npad * 4);
   s.sinks = s.dbias + (bias_grad ? al256(w.batch * w.heads * a.tiles * (2 * (int64_t)a.r + 1) * 4) : 0);
-  s.total = s.sinks + w.batch * w.kv_heads * (int64_t)tiles * (1 + chunks) * 2 * kWRows * ((a.d + 15) & ~15) * 4;
+  s.arrived = s.sinks + al256(w.batch * w.kv_heads * (int64_t)tiles * (1 + chunks) * 2 * kWRows * ((a.d + 15) & ~15) * 4);
+  s.total = s.arrived + w.batch * w.kv_heads * (int64_t)tiles * 4;
   return s;
 }
 
-// q, dO, k, v as a kernel cuts them that owns 128 rows of queries (own_q) or keys and streams the others.
-static bool bwd_maps(CUtensorMap* m, const px_window& w, const px_rows& q, const px_rows& dout, const px_rows& k, const px_rows& v, bool own_q) {
-  const uint32_t rq = own_q ? kWRows : kWCols, rk = own_q ? kWCols : kWRows;
-  return rows_map(&m[0], q, w, w.heads, rq) && rows_map(&m[1], dout, w, w.heads, rq) && rows_map(&m[2], k, w, w.kv_heads, rk) &&
-         rows_map(&m[3], v, w, w.kv_heads, rk);
-}
 template <bool kF16, int kD, bool kBiasGrad>
 static bool launch_window_dq(const CUtensorMap* m, const WindowArgs& a, const WindowBwdArgs& g, const RowsOut& dout, const RowsOut& o,
                              const RowsOut& dq, int64_t blocks, cudaStream_t st) {
@@ -451,27 +445,17 @@ static bool window_bwd(const px_window& w, const BwdRows& x, const WindowArgs& a
   const int64_t blocks = (int64_t)a.tiles * w.heads * w.batch;
   const RowsOut dout = rows_out(x.dout), o = rows_out(x.o), dq = rows_out(x.dq), dk = rows_out(x.dk), dv = rows_out(x.dv);
   CUtensorMap m[4];
-  if (!bwd_maps(m, w, *x.q, *x.dout, *x.k, *x.v, true)) return false;
+  if (!rows_map(&m[0], *x.q, w, w.heads) || !rows_map(&m[1], *x.dout, w, w.heads) || !rows_map(&m[2], *x.k, w, w.kv_heads) ||
+      !rows_map(&m[3], *x.v, w, w.kv_heads))
+    return false;
   const auto go_q = w.d <= 64 ? (dbias ? launch_window_dq<kF16, 64, true> : launch_window_dq<kF16, 64, false>)
                               : (dbias ? launch_window_dq<kF16, 128, true> : launch_window_dq<kF16, 128, false>);
   if (!go_q(m, a, g, dout, o, dq, blocks, st)) return false;
-  if (dbias) {
-    const int buckets = 2 * a.r + 1;
-    window_dbias_kernel<<<dim3((unsigned)((buckets + 31) / 32), (unsigned)w.heads), 1024, 0, st>>>(g.dbias, dbias, a.bias_type, (int)w.batch, a.heads,
-                                                                                                a.tiles, buckets);
-    if (cudaGetLastError() != cudaSuccess) return false;
-  }
-  if (!dk.data && !dv.data) return true;
-  if (!bwd_maps(m, w, *x.q, *x.dout, *x.k, *x.v, false)) return false;
+  const int64_t own = dk.data || dv.data ? (int64_t)(a.tiles + g.sink_tiles * g.chunks) * w.kv_heads * w.batch : 0;
+  const int64_t buckets = dbias ? (int64_t)w.heads * g.bias_blocks : 0;      // these come first: short, and there is room beside them
+  if (own + buckets == 0) return true;
   const auto go_kv = w.d <= 32 ? launch_window_dkv<kF16, 32> : w.d <= 64 ? launch_window_dkv<kF16, 64> : launch_window_dkv<kF16, 128>;
-  if (!go_kv(m, a, g, dk, dv, (int64_t)(a.tiles + g.sink_tiles * g.chunks) * w.kv_heads * w.batch, st)) return false;
-  if (g.chunks > 0) {
-    const int rows = a.n < g.sink_tiles * kWRows ? a.n : g.sink_tiles * kWRows;
-    const int64_t per = (2 * (int64_t)rows * (a.d / 8) + 255) / 256;
-    window_sink_kernel<kF16><<<(unsigned)(per * w.batch * w.kv_heads), 256, 0, st>>>(a, g, dk, dv);
-    if (cudaGetLastError() != cudaSuccess) return false;
-  }
-  return true;
+  return go_kv(m, a, g, dk, dv, own + buckets, st);
 }
 
 }  // namespace px
@@ -507,6 +491,10 @@ extern "C" int32_t px_window_bwd(const px_window* w, const px_rows* q, const px_
   g.ndelta = (float*)(ws + space.delta);
   g.dbias = (float*)(ws + space.dbias);
   g.sinks = (float*)(ws + space.sinks);
+  g.arrived = (unsigned int*)(ws + space.arrived);
+  g.dbias_out = dbias;
+  g.bias_blocks = dbias ? (2 * a.r + 1 + 31) / 32 : 0;
+  g.batches = (int)w->batch;
   g.scale = w->scale;
   sink_chunks(a, &g.sink_tiles, &g.chunks, &g.chunk);
   if ((int64_t)(a.tiles + g.sink_tiles * g.chunks) * w->kv_heads * w->batch > 0x3fffffffll) return PX_ERR_UNSUPPORTED;
