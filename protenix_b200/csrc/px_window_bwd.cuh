@@ -34,7 +34,7 @@ struct WindowBwdArgs {
 
 struct WindowBwdBars {
   // streamed operands; S and dP, complete and in registers; P and dS; the products with them
-  uint64_t own_full, first_full[2], second_full[2], ready, taken, given, done;
+  uint64_t own_full, first_full[3], second_full[2], ready, taken, given, done;
   uint32_t tmem_base;
 };
 
@@ -43,11 +43,12 @@ struct WindowBwdBars {
 // kD: the head size that there is room for, 64 or 128.
 template <int kD>
 struct WindowDqLayout {
-  static constexpr int panels = kD / 64, stages = kD == 64 ? 2 : 1, tile = panels * kWCols * 128;
+  // K's tiles serve two products: three of them, or the next S would wait for one that was asked for only when the dS before was through
+  static constexpr int panels = kD / 64, k_stages = kD == 64 ? 3 : 1, v_stages = kD == 64 ? 2 : 1, tile = panels * kWCols * 128;
   static constexpr bool ahead = kD == 64;
   static constexpr int cols = 256, col_ds = ahead ? 2 * kWCols : 0, col_q = ahead ? 2 * kWCols + kWCols / 2 : 2 * kWCols;
   static_assert(col_q + kD <= cols, "tensor memory of a CTA");
-  static constexpr int q = 0, dout = panels * kWRows * 128, k = 2 * dout, v = k + stages * tile, bars = v + stages * tile;
+  static constexpr int q = 0, dout = panels * kWRows * 128, k = 2 * dout, v = k + k_stages * tile, bars = v + v_stages * tile;
   static constexpr int part = bars + 128, bias = part + 2 * kWRows * 4;
   static constexpr int bytes(int r, bool grad) { return bias + bias_floats(r) * 4 * (grad ? 9 : 1) + (grad ? 8 * 32 * 4 : 0); }
 };
@@ -60,7 +61,7 @@ window_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                  const RowsOut dq) {
   typedef WindowDqLayout<kD> L;
   constexpr uint32_t kCols = L::cols;
-  constexpr int kStages = L::stages, kPanels = L::panels;
+  constexpr int kK = L::k_stages, kV = L::v_stages, kPanels = L::panels;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* sm = smem_aligned(smem_raw);
   WindowBwdBars& bars = *reinterpret_cast<WindowBwdBars*>(sm + L::bars);
@@ -74,10 +75,8 @@ window_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   if (threadIdx.x == 0) {
     prefetch_maps(map_q, map_do, map_k, map_v);
     mbar_init(&bars.own_full, 1);
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(&bars.first_full[s], 1);
-      mbar_init(&bars.second_full[s], 1);
-    }
+    for (int s = 0; s < 3; ++s) mbar_init(&bars.first_full[s], 1);
+    for (int s = 0; s < 2; ++s) mbar_init(&bars.second_full[s], 1);
     mbar_init(&bars.ready, 1);
     mbar_init(&bars.taken, 8);
     mbar_init(&bars.given, 8);
@@ -98,18 +97,20 @@ window_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     const uint32_t q_at = smem_u32(sm), do_at = smem_u32(sm + L::dout), k_at = smem_u32(sm + L::k), v_at = smem_u32(sm + L::v);
     const uint32_t idesc_s = umma_idesc_16(128, kWCols, kF16, kF16), idesc_q = umma_idesc_16(128, (a.d + 15) & ~15, kF16, kF16, false, true);
     const int steps = (a.d + 15) / 16;
-    const auto load = [&](int t, uint64_t* full, const CUtensorMap* map, uint32_t at) {      // one lane
-      const int s = t % kStages;
-      mbar_expect_tx(&full[s], L::tile);
-      load_rows<kPanels>(at + s * L::tile, map, &full[s], kWCols, tiles.key(t), kv, batch);
+    const auto load_k = [&](int t) {      // one lane
+      mbar_expect_tx(&bars.first_full[t % kK], L::tile);
+      load_rows<kPanels>(k_at + t % kK * L::tile, &map_k, &bars.first_full[t % kK], kWCols, tiles.key(t), kv, batch);
+    };
+    const auto load_v = [&](int t) {
+      mbar_expect_tx(&bars.second_full[t % kV], L::tile);
+      load_rows<kPanels>(v_at + t % kV * L::tile, &map_v, &bars.second_full[t % kV], kWCols, tiles.key(t), kv, batch);
     };
     const auto issue = [&](int t) {
-      const int s = t % kStages, parity = (t / kStages) & 1;
-      if (!mbar_wait_warp(&bars.first_full[s], parity, 2u) || !mbar_wait_warp(&bars.second_full[s], parity, 4u)) return false;
+      if (!mbar_wait_warp(&bars.first_full[t % kK], (t / kK) & 1, 2u) || !mbar_wait_warp(&bars.second_full[t % kV], (t / kV) & 1, 4u)) return false;
       tc_fence_after();
       if (elect_lane()) {
-        mma_rows(tmem, q_at, k_at + s * L::tile, kWCols, steps, idesc_s);
-        mma_rows(tmem + kWCols, do_at, v_at + s * L::tile, kWCols, steps, idesc_s);
+        mma_rows(tmem, q_at, k_at + t % kK * L::tile, kWCols, steps, idesc_s);
+        mma_rows(tmem + kWCols, do_at, v_at + t % kV * L::tile, kWCols, steps, idesc_s);
         umma_commit(&bars.ready);
       }
       __syncwarp();
@@ -118,10 +119,12 @@ window_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     if (elect_lane()) {
       mbar_expect_tx(&bars.own_full, 2 * kPanels * kWRows * 128);
       load_rows<kPanels>(q_at, &map_q, &bars.own_full, kWRows, q0, head, batch);
+      load_k(0);
       load_rows<kPanels>(do_at, &map_do, &bars.own_full, kWRows, q0, head, batch);
-      for (int t = 0; t < kStages && t < tiles.count; ++t) {
-        load(t, bars.first_full, &map_k, k_at);
-        load(t, bars.second_full, &map_v, v_at);
+      load_v(0);
+      for (int t = 1; t < kK && t < tiles.count; ++t) {
+        load_k(t);
+        if (t < kV) load_v(t);
       }
     }
     __syncwarp();
@@ -129,29 +132,29 @@ window_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     for (int t = 0; t < tiles.count && ok; ++t) {
       ok = mbar_wait_warp(&bars.taken, t & 1, 8u);            // S(t) and dP(t) are complete and in registers: V's tile is free
       if (!ok) break;
-      if (t + kStages < tiles.count && elect_lane()) load(t + kStages, bars.second_full, &map_v, v_at);
+      if (t + kV < tiles.count && elect_lane()) load_v(t + kV);
       __syncwarp();
       if (L::ahead) {
-        if (t > 0 && t + 1 < tiles.count) {                   // K's tile of the step before is free
+        if (t + 1 < tiles.count && !(ok = issue(t + 1))) break;
+        if (t > 0 && t - 1 + kK < tiles.count) {              // K's tile of the step before is free
           ok = mbar_wait_warp(&bars.done, (t - 1) & 1, 16u);
           if (!ok) break;
-          if (elect_lane()) load(t + 1, bars.first_full, &map_k, k_at);
+          if (elect_lane()) load_k(t - 1 + kK);
           __syncwarp();
         }
-        if (t + 1 < tiles.count && !(ok = issue(t + 1))) break;
       }
       ok = mbar_wait_warp(&bars.given, t & 1, 8u);
       if (!ok) break;
       tc_fence_after();
       if (elect_lane()) {
-        mma_streamed<kWCols>(tmem + L::col_q, tmem + L::col_ds, k_at + (t % kStages) * L::tile, idesc_q, t == 0);
+        mma_streamed<kWCols>(tmem + L::col_q, tmem + L::col_ds, k_at + t % kK * L::tile, idesc_q, t == 0);
         umma_commit(&bars.done);
       }
       __syncwarp();
       if (!L::ahead) {
         ok = mbar_wait_warp(&bars.done, t & 1, 16u);          // K's tile and the place of S are free
         if (!ok) break;
-        if (t + 1 < tiles.count && elect_lane()) load(t + 1, bars.first_full, &map_k, k_at);
+        if (t + 1 < tiles.count && elect_lane()) load_k(t + 1);
         __syncwarp();
         if (t + 1 < tiles.count) ok = issue(t + 1);
       }
@@ -160,30 +163,37 @@ window_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     // ------------------------------------------------------------------ one query row x 32 keys a thread
     const int quarter = warp & 3, half = warp >> 2, row = 32 * quarter + lane, i = q0 + row, qw = q0 + 32 * quarter;
     const uint32_t t_lane = tmem + ((uint32_t)(32 * quarter) << 16);
-    // delta = dO . O, each thread over its half of the 16-byte pieces of the row
-    float sum = 0.f;
-    if (i < a.n) {
-      const uint16_t *x = dout.at(batch, head, i), *y = o.at(batch, head, i);
-      for (int c = 8 * half; c < a.d; c += 16) {
-        const uint4 u = __ldg(reinterpret_cast<const uint4*>(x + c)), v = __ldg(reinterpret_cast<const uint4*>(y + c));
-        const uint32_t us[4] = {u.x, u.y, u.z, u.w}, vs[4] = {v.x, v.y, v.z, v.w};
+    // All loads of the beginning at once: one after the other they took 4000 cycles, as much as two tiles.  delta = dO . O, each thread over
+    // its half of the 16-byte pieces of the row.
+    const float nlse = g.nlse[(size_t)bh * a.npad + i];
+    uint4 u[kD / 16], v[kD / 16];
+    const uint16_t *x = dout.at(batch, head, i), *y = o.at(batch, head, i);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 p = unpack16x2<kF16>(us[e]), q = unpack16x2<kF16>(vs[e]);
-          sum = fmaf(p.x, q.x, fmaf(p.y, q.y, sum));
-        }
-      }
+    for (int e = 0; e < kD / 16; ++e) {
+      const int c = 8 * half + 16 * e;
+      const bool there = i < a.n && c < a.d;
+      u[e] = there ? __ldg(reinterpret_cast<const uint4*>(x + c)) : make_uint4(0u, 0u, 0u, 0u);
+      v[e] = there ? __ldg(reinterpret_cast<const uint4*>(y + c)) : make_uint4(0u, 0u, 0u, 0u);
     }
-    part[half * kWRows + row] = sum;
     if (a.r >= 0) {
       bias_fill(a, head, bias, 256);
       if (kBiasGrad)
         for (int k = threadIdx.x; k < 8 * ext; k += 256) bias[ext + k] = 0.f;
     }
+    float sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < kD / 16; ++e) {
+      const uint32_t us[4] = {u[e].x, u[e].y, u[e].z, u[e].w}, vs[4] = {v[e].x, v[e].y, v[e].z, v[e].w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 p = unpack16x2<kF16>(us[k]), q = unpack16x2<kF16>(vs[k]);
+        sum = fmaf(p.x, q.x, fmaf(p.y, q.y, sum));
+      }
+    }
+    part[half * kWRows + row] = sum;
     barrier_of(1, 256);
     const float ndelta = -(part[row] + part[kWRows + row]);
     if (half == 0) g.ndelta[(size_t)bh * a.npad + i] = ndelta;      // 0 beyond the last row
-    const float nlse = g.nlse[(size_t)bh * a.npad + i];
     float* const sums = bias + ext * (1 + warp);                   // by offset, as the bias lies
     float* const stage = bias + ext * 9 + 32 * warp;
     const f32x2 scale = both2(a.c), ndelta2 = both2(ndelta);
@@ -248,8 +258,8 @@ window_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       tmem_st16(t_lane + L::col_ds + 16 * half, w);
       // masked keys of the tile: their rows of K become zeros, those of this half by its four warps
       if (keys != 0xffffffffu && keys != bits_between(0, a.n - 1 - kh)) {
-        mbar_wait(&bars.first_full[t % kStages], (t / kStages) & 1, 128u);      // complete: S(t) is; orders these writes behind the copy's
-        if (!(keys >> lane & 1)) clear_row<kPanels, kWCols>(sm + L::k + (t % kStages) * L::tile, 32 * half + lane, quarter, 4);
+        mbar_wait(&bars.first_full[t % kK], (t / kK) & 1, 128u);      // complete: S(t) is; orders these writes behind the copy's
+        if (!(keys >> lane & 1)) clear_row<kPanels, kWCols>(sm + L::k + t % kK * L::tile, 32 * half + lane, quarter, 4);
         fence_async_shared();
       }
       tmem_wait_st();
@@ -258,20 +268,26 @@ window_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       if (lane == 0) mbar_arrive(&bars.given);
       if (kBiasGrad && !dead) {
         if (near) {
-          // Sums along the diagonals of a 32 x 32 block: the running sum moves one lane on with each column, and leaves by the last lane.
-          float run = 0.f;
+          // Sums along the diagonals of a 32 x 32 block, 8 columns at a time (four chains beside one another: a single one waits for its shuffles):
+          // the running sum moves one lane on with each column, and leaves by the last lane.
+          float run[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int c = 0; c < 32; ++c) {
-            run = __shfl_up_sync(0xffffffffu, run, 1);
-            run = (lane == 0 ? 0.f : run) + d[c];
-            if (lane == 31) stage[c] = run;         // offset c - 31 of the block is complete
-          }
+          for (int c = 0; c < 8; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float up = __shfl_up_sync(0xffffffffu, run[e], 1);
+              run[e] = (lane == 0 ? 0.f : up) + d[8 * e + c];
+              if (lane == 31) stage[8 * e + c] = run[e];      // offset 8 e + c - 31 of the block, as far as these columns go
+            }
           __syncwarp();
           float* const at = sums + (kh - qw + a.r + kWBiasBeyond);
           at[lane - 31] += stage[lane];
           __syncwarp();
-          if (lane < 31) at[31 - lane] += run;
-          __syncwarp();
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if (lane < 31) at[8 * e + 7 - lane] += run[e];
+            __syncwarp();
+          }
         } else {
           f32x2 v = pair2(0.f, 0.f);
 #pragma unroll
@@ -310,29 +326,22 @@ window_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     tmem_free(tmem, kCols);
   }
   if (kBiasGrad) {
-    float* const out = g.dbias + (size_t)blockIdx.x * (2 * a.r + 1);
-    for (int b = threadIdx.x; b < 2 * a.r + 1; b += kWBwdThreads) {
-      float v = 0.f;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v += bias[ext * (1 + k) + b + kWBiasBeyond];
-      out[b] = v;
-    }
-    // the two ends: what lies beyond them, a warp each
+    // the two ends first, with what lies beyond them, a warp each
     if (warp < 2) {
-      __syncwarp();
-      float v = 0.f;
-      for (int k = 0; k < 8; ++k) {
-        const float* const s = bias + ext * (1 + k) + (warp == 0 ? 0 : 2 * a.r + 1 + kWBiasBeyond);
-        for (int e = lane; e < kWBiasBeyond; e += 32) v += s[e];
-        if (lane == k) v += part[8 * warp + k];
-      }
+      const float* const s = bias + ext + (warp == 0 ? 0 : 2 * a.r + 1 + kWBiasBeyond);
+      float v = lane < 8 ? part[8 * warp + lane] : 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v += s[ext * k + lane] + s[ext * k + 32 + lane];
       v = warp_sum(v);
       if (lane == 0) part[32 + warp] = v;
     }
     __syncthreads();
-    if (threadIdx.x == 0) {
-      out[0] += part[32];
-      out[2 * a.r] += part[33];
+    float* const out = g.dbias + (size_t)blockIdx.x * (2 * a.r + 1);
+    for (int b = threadIdx.x; b < 2 * a.r + 1; b += kWBwdThreads) {
+      float v = (b == 0 ? part[32] : 0.f) + (b == 2 * a.r ? part[33] : 0.f);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v += bias[ext * (1 + k) + b + kWBiasBeyond];
+      out[b] = v;
     }
   }
 }
@@ -364,14 +373,15 @@ __device__ __forceinline__ void sum_dbias(const WindowArgs& a, const WindowBwdAr
 // Heads of 33 to 64: S^T | dP^T | dV (64) | dK (64), P^T and dS^T in shared memory.  The next S^T and dP^T are made while these P^T and dS^T are.
 template <int kD>
 struct WindowDkvLayout {
-  static constexpr int panels = kD > 64 ? 2 : 1, tile = panels * kWCols * 128, stat = 2 * kWCols * 4;
+  // streamed tiles: three, or the next S^T would wait for one that was asked for only when the dS^T before was through; heads of 33 to 64 have room for two
+  static constexpr int panels = kD > 64 ? 2 : 1, stages = kD == 32 ? 3 : 2, tile = panels * kWCols * 128, stat = 2 * kWCols * 4;
   static constexpr bool p_shared = kD == 64;
   static constexpr int cols = kD == 128 ? 512 : 256, ctas = kD == 128 ? 1 : 2;
   static constexpr int col_p = 2 * kWCols, col_ds = col_p + kWCols / 2;
   static constexpr int col_v = p_shared ? 2 * kWCols : 3 * kWCols, col_k = col_v + kD;
   static_assert(col_k + kD <= cols, "tensor memory of a CTA");
-  static constexpr int k = 0, v = panels * kWRows * 128, q = 2 * v, dout = q + 2 * tile, p = dout + 2 * tile;
-  static constexpr int ds = p + (p_shared ? kWRows * 128 : 0), stats = ds + (p_shared ? kWRows * 128 : 0), bars = stats + 2 * stat;
+  static constexpr int k = 0, v = panels * kWRows * 128, q = 2 * v, dout = q + stages * tile, p = dout + stages * tile;
+  static constexpr int ds = p + (p_shared ? kWRows * 128 : 0), stats = ds + (p_shared ? kWRows * 128 : 0), bars = stats + stages * stat;
   static constexpr int bias = bars + 128;
   static constexpr int bytes(int r) { return bias + bias_floats(r) * 4; }
 };
@@ -386,6 +396,7 @@ __device__ __forceinline__ void sum_sinks(const WindowArgs& a, const WindowBwdAr
     if (!out.data) continue;
     const float* from = g.sinks + ((size_t)bkv * g.sink_tiles + own) * (1 + g.chunks) * 2 * kWRows * dn + (size_t)which * kWRows * dn + (size_t)row * dn + c;
     float v[8] = {};
+#pragma unroll 4
     for (int k = 0; k <= g.chunks; ++k, from += 2 * kWRows * dn) {
       const float4 x = __ldcg(reinterpret_cast<const float4*>(from)), y = __ldcg(reinterpret_cast<const float4*>(from + 4));
       v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w, v[4] += y.x, v[5] += y.y, v[6] += y.z, v[7] += y.w;
@@ -415,7 +426,7 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
                   const __grid_constant__ CUtensorMap map_v, const WindowArgs a, const WindowBwdArgs g, const RowsOut dk, const RowsOut dv) {
   typedef WindowDkvLayout<kD> L;
   constexpr uint32_t kCols = L::cols;
-  constexpr int kPanels = L::panels;
+  constexpr int kPanels = L::panels, kStages = L::stages;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* sm = smem_aligned(smem_raw);
   WindowBwdBars& bars = *reinterpret_cast<WindowBwdBars*>(sm + L::bars);
@@ -450,10 +461,8 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   if (threadIdx.x == 0) {
     prefetch_maps(map_q, map_do, map_k, map_v);
     mbar_init(&bars.own_full, 1);
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(&bars.first_full[s], 1);
-      mbar_init(&bars.second_full[s], 1);
-    }
+    for (int s = 0; s < 3; ++s) mbar_init(&bars.first_full[s], 1);
+    for (int s = 0; s < 2; ++s) mbar_init(&bars.second_full[s], 1);
     mbar_init(&bars.ready, 1);
     mbar_init(&bars.taken, 8);
     mbar_init(&bars.given, 8);
@@ -480,8 +489,8 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       bulk_load(sm + L::stats + s * L::stat + kWCols * 4, g.ndelta + row, kWCols * 4, &bars.first_full[s]);
     };
     const auto issue = [&](int t) {
-      const int s = t & 1;
-      if (!mbar_wait_warp(&bars.first_full[s], (t >> 1) & 1, 2u)) return false;
+      const int s = t % kStages;
+      if (!mbar_wait_warp(&bars.first_full[s], (t / kStages) & 1, 2u)) return false;
       tc_fence_after();
       if (elect_lane()) {
         mma_rows(tmem, k_at, q_at + s * L::tile, kWCols, steps, idesc_s);
@@ -499,7 +508,7 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         load_rows<kPanels>(v_at, &map_v, &bars.own_full, kWRows, k0, kv, batch);
       }
       __syncwarp();
-      for (int t = 0; t < 2 && t < tiles.count; ++t) {
+      for (int t = 0; t < kStages && t < tiles.count; ++t) {
         if (elect_lane()) load(t);
         __syncwarp();
         coming.next(tiles);
@@ -509,19 +518,20 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     for (int t = 0; t < tiles.count && ok; ++t) {
       ok = mbar_wait_warp(&bars.taken, t & 1, 8u);
       if (!ok) break;
-      if (t > 0 && t + 1 < tiles.count) {                     // the streamed tile of the step before is free
+      if (kStages > 2 && t + 1 < tiles.count && !(ok = issue(t + 1))) break;
+      if (t > 0 && t - 1 + kStages < tiles.count) {           // the streamed tile of the step before is free
         ok = mbar_wait_warp(&bars.done, (t - 1) & 1, 16u);
         if (!ok) break;
-        if (elect_lane()) load((t + 1) & 1);
+        if (elect_lane()) load((t - 1) % kStages);
         __syncwarp();
         coming.next(tiles);
       }
-      if (t + 1 < tiles.count && !(ok = issue(t + 1))) break;
+      if (kStages == 2 && t + 1 < tiles.count && !(ok = issue(t + 1))) break;
       ok = mbar_wait_warp(&bars.given, t & 1, 8u);
       if (!ok) break;
       tc_fence_after();
       if (elect_lane()) {
-        const int s = t & 1;
+        const int s = t % kStages;
         if (L::p_shared) {
           mma_streamed_ss(tmem + L::col_v, smem_u32(sm + L::p), do_at + s * L::tile, idesc_d, t == 0);
           mma_streamed_ss(tmem + L::col_k, smem_u32(sm + L::ds), q_at + s * L::tile, idesc_d, t == 0);
@@ -548,7 +558,7 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     const bool wide = a.r >= 0 && a.group > 1;     // the bias changes on the way: all eight warps keep together
     QueryItem now(tiles);
     for (int t = 0; t < tiles.count; ++t, now.next(tiles)) {
-      const int qh = (tiles.first + now.tile) * kWCols + 32 * half, s = t & 1;
+      const int qh = (tiles.first + now.tile) * kWCols + 32 * half, s = t % kStages;
       if (a.r >= 0 && now.member != filled) {
         // all are past the tile before (barrier below), but not all are through with it
         barrier_of(1, 256);
@@ -559,7 +569,7 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       const bool dead = qh >= a.n || block_dead(a, qh, kw);
       ok = mbar_wait(&bars.ready, t & 1, 32u);
       // the statistics came with the operands; this wait only makes the copy's writes visible here
-      ok = mbar_wait(&bars.first_full[s], (t >> 1) & 1, 64u) && ok;
+      ok = mbar_wait(&bars.first_full[s], (t / kStages) & 1, 64u) && ok;
       __syncwarp();
       tc_fence_after();
       uint32_t wp[16], wd[16], nothing = 0, seen = 0xffffffffu;
