@@ -37,26 +37,27 @@ __device__ __forceinline__ void load_rows(uint32_t dst, const CUtensorMap* map, 
     for (int r = 0; r < rows; r += 64) tma_load_4d(dst + (p * rows + r) * 128, map, bar, 64 * p, row0 + r, head, batch);
 }
 
-// D[128][rows of B] = A B^T over d, both K-major panels of 64 (one lane).
-__device__ __forceinline__ void mma_rows(uint32_t d_tmem, uint32_t a, uint32_t b, int b_rows, int steps, uint32_t idesc) {
-  for (int ks = 0; ks < steps; ++ks) {
-    const uint32_t panel = ks >> 2, at = 2 * (ks & 3);
-    umma_bf16(d_tmem, umma_desc_sw128(a + panel * (kWRows * 128)) + at, umma_desc_sw128(b + panel * b_rows * 128) + at, idesc, ks > 0);
-  }
-}
-// D[128][d] += A[128][kKT] B with A in tensor memory and B the streamed tile [kKT][d], read along its rows (one lane).
-template <int kKT>
-__device__ __forceinline__ void mma_streamed(uint32_t d_tmem, uint32_t a_tmem, uint32_t b, uint32_t idesc, bool first) {
+// The products, by one lane.  What their descriptors have in common is formed once a call.
+//
+// D[128][kRows] = A B^T over d (`steps` of 16), A [128] and B [kRows] rows, both K-major panels of 64.
+template <int kPanels, int kRows>
+__device__ __forceinline__ void mma_rows(uint32_t d_tmem, uint32_t a, uint32_t b, int steps, uint32_t idesc) {
+  const uint64_t da = umma_desc_sw128(a), db = umma_desc_sw128(b);
 #pragma unroll
-  for (int ks = 0; ks < kKT / 16; ++ks)
-    umma_bf16_ts(d_tmem, a_tmem + 8 * ks, umma_desc_mn_sw128(b + ks * 2048, kKT * 128, 1024), idesc, !first || ks > 0);
+  for (int ks = 0; ks < 4 * kPanels; ++ks)
+    if (ks < steps) umma_bf16(d_tmem, da + (ks >> 2) * (kWRows * 8) + 2 * (ks & 3), db + (ks >> 2) * (kRows * 8) + 2 * (ks & 3), idesc, ks > 0);
 }
-
+// D[128][d] += A[128][64] B with A in tensor memory and B a streamed tile [64][d], read along its rows.
+__device__ __forceinline__ void mma_streamed(uint32_t d_tmem, uint32_t a_tmem, uint32_t b, uint32_t idesc, bool first) {
+  const uint64_t db = umma_desc_mn_sw128(b, 64 * 128, 1024);
+#pragma unroll
+  for (int ks = 0; ks < 4; ++ks) umma_bf16_ts(d_tmem, a_tmem + 8 * ks, db + 128 * ks, idesc, !first || ks > 0);
+}
 // The same with A in shared memory, a panel of 64.
 __device__ __forceinline__ void mma_streamed_ss(uint32_t d_tmem, uint32_t a, uint32_t b, uint32_t idesc, bool first) {
+  const uint64_t da = umma_desc_sw128(a), db = umma_desc_mn_sw128(b, 64 * 128, 1024);
 #pragma unroll
-  for (int ks = 0; ks < 4; ++ks)
-    umma_bf16(d_tmem, umma_desc_sw128(a) + 2 * ks, umma_desc_mn_sw128(b + ks * 2048, 64 * 128, 1024), idesc, !first || ks > 0);
+  for (int ks = 0; ks < 4; ++ks) umma_bf16(d_tmem, da + 2 * ks, db + 128 * ks, idesc, !first || ks > 0);
 }
 // 32 values (16 words) of row `row` into such a panel, columns 32 * half and up.
 __device__ __forceinline__ void panel_store(unsigned char* panel, int row, int half, const uint32_t (&w)[16]) {

@@ -109,8 +109,8 @@ window_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       if (!mbar_wait_warp(&bars.first_full[t % kK], (t / kK) & 1, 2u) || !mbar_wait_warp(&bars.second_full[t % kV], (t / kV) & 1, 4u)) return false;
       tc_fence_after();
       if (elect_lane()) {
-        mma_rows(tmem, q_at, k_at + t % kK * L::tile, kWCols, steps, idesc_s);
-        mma_rows(tmem + kWCols, do_at, v_at + t % kV * L::tile, kWCols, steps, idesc_s);
+        mma_rows<kPanels, kWCols>(tmem, q_at, k_at + t % kK * L::tile, steps, idesc_s);
+        mma_rows<kPanels, kWCols>(tmem + kWCols, do_at, v_at + t % kV * L::tile, steps, idesc_s);
         umma_commit(&bars.ready);
       }
       __syncwarp();
@@ -147,7 +147,7 @@ window_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       if (!ok) break;
       tc_fence_after();
       if (elect_lane()) {
-        mma_streamed<kWCols>(tmem + L::col_q, tmem + L::col_ds, k_at + t % kK * L::tile, idesc_q, t == 0);
+        mma_streamed(tmem + L::col_q, tmem + L::col_ds, k_at + t % kK * L::tile, idesc_q, t == 0);
         umma_commit(&bars.done);
       }
       __syncwarp();
@@ -493,8 +493,8 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       if (!mbar_wait_warp(&bars.first_full[s], (t / kStages) & 1, 2u)) return false;
       tc_fence_after();
       if (elect_lane()) {
-        mma_rows(tmem, k_at, q_at + s * L::tile, kWCols, steps, idesc_s);
-        mma_rows(tmem + kWCols, v_at, do_at + s * L::tile, kWCols, steps, idesc_s);
+        mma_rows<kPanels, kWCols>(tmem, k_at, q_at + s * L::tile, steps, idesc_s);
+        mma_rows<kPanels, kWCols>(tmem + kWCols, v_at, do_at + s * L::tile, steps, idesc_s);
         umma_commit(&bars.ready);
       }
       __syncwarp();
@@ -536,8 +536,8 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           mma_streamed_ss(tmem + L::col_v, smem_u32(sm + L::p), do_at + s * L::tile, idesc_d, t == 0);
           mma_streamed_ss(tmem + L::col_k, smem_u32(sm + L::ds), q_at + s * L::tile, idesc_d, t == 0);
         } else {
-          mma_streamed<kWCols>(tmem + L::col_v, tmem + L::col_p, do_at + s * L::tile, idesc_d, t == 0);
-          mma_streamed<kWCols>(tmem + L::col_k, tmem + L::col_ds, q_at + s * L::tile, idesc_d, t == 0);
+          mma_streamed(tmem + L::col_v, tmem + L::col_p, do_at + s * L::tile, idesc_d, t == 0);
+          mma_streamed(tmem + L::col_k, tmem + L::col_ds, q_at + s * L::tile, idesc_d, t == 0);
         }
         umma_commit(&bars.done);
       }

@@ -96,7 +96,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       if (!mbar_wait_warp(&bars.k_full[t & 1], (t >> 1) & 1, 2u)) return false;
       tc_fence_after();
       if (elect_lane()) {
-        mma_rows(tmem, q_at, k_at + (t & 1) * L::tile, kKT, (a.d + 15) / 16, idesc_s);
+        mma_rows<kPanels, kKT>(tmem, q_at, k_at + (t & 1) * L::tile, (a.d + 15) / 16, idesc_s);
         umma_commit(&bars.s_full);
       }
       __syncwarp();
@@ -129,7 +129,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       tc_fence_after();
       if (elect_lane()) {
         if (L::p_shared) mma_streamed_ss(tmem + L::col_o, smem_u32(sm + L::p), v_at + (t & 1) * L::tile, idesc_o, t == 0);
-        else mma_streamed<kKT>(tmem + L::col_o, tmem + L::col_p, v_at + (t & 1) * L::tile, idesc_o, t == 0);
+        else mma_streamed(tmem + L::col_o, tmem + L::col_p, v_at + (t & 1) * L::tile, idesc_o, t == 0);
         umma_commit(&bars.pv_done);
       }
       __syncwarp();
