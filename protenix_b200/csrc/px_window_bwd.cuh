@@ -6,8 +6,9 @@
 // gradient.  window_dkv_kernel owns 128 keys and streams the queries that see them, those of all heads of the group one after the other.
 // The price is S and dP twice: seven products a tile pair in place of five.
 //
-// Eight compute warps, a thread = one row x 32 of the 64 columns (no reduction along a row is needed here), one warp for copies and
-// products.  dS and P are rounded to the operands' type for the products they enter and stay fp32 in the bias's gradient.
+// Eight compute warps, a thread = one row x 32 of the 64 columns (no reduction along a row is needed here).  Copies and products have one warp in the first
+// kernel and two in the second, whose four products a step take an issuing warp some 1000 cycles beside busy ones (177 -> 168 us for a causal window
+// of 1024 over 8192 tokens; in the first kernel two warps were slower, 142 us against 114).  dS and P are rounded to the operands' type for the products they enter and stay fp32 in the bias's gradient.
 //
 // Keys that are sinks are seen by all later queries.  Their CTA takes the queries of the window, like any other; the
 // queries beyond are cut into chunks of about as many tiles, a CTA each, and the last of these CTAs adds the chunks up in their order.
@@ -18,7 +19,8 @@
 
 namespace px {
 
-constexpr int kWBwdThreads = 288;
+constexpr int kWDqThreads = 288;      // eight warps of rows, one for copies and products
+constexpr int kWDkvThreads = 320;     // eight warps of rows, one for S^T and dP^T, one for the products with P^T and dS^T
 
 struct WindowBwdArgs {
   const float* nlse;             // [batch * heads][npad], base 2, negative; -inf for rows that see nothing and beyond the last
@@ -55,7 +57,7 @@ struct WindowDqLayout {
 static_assert(sizeof(WindowBwdBars) <= 128, "room for the barriers");
 
 template <bool kF16, int kD, bool kBiasGrad>
-__global__ void __launch_bounds__(kWBwdThreads, 2)
+__global__ void __launch_bounds__(kWDqThreads, 2)
 window_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do, const __grid_constant__ CUtensorMap map_k,
                  const __grid_constant__ CUtensorMap map_v, const WindowArgs a, const WindowBwdArgs g, const RowsOut dout, const RowsOut o,
                  const RowsOut dq) {
@@ -337,7 +339,7 @@ window_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     }
     __syncthreads();
     float* const out = g.dbias + (size_t)blockIdx.x * (2 * a.r + 1);
-    for (int b = threadIdx.x; b < 2 * a.r + 1; b += kWBwdThreads) {
+    for (int b = threadIdx.x; b < 2 * a.r + 1; b += kWDqThreads) {
       float v = (b == 0 ? part[32] : 0.f) + (b == 2 * a.r ? part[33] : 0.f);
 #pragma unroll
       for (int k = 0; k < 8; ++k) v += bias[ext * (1 + k) + b + kWBiasBeyond];
@@ -346,10 +348,10 @@ window_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   }
 }
 
-// dbias[head][b] of the CTAs' sums, in their order: 32 buckets (block `of` of a head's), nine slices of the CTAs of the head, a warp each.
+// dbias[head][b] of the CTAs' sums, in their order: 32 buckets (block `of` of a head's), a slice of the CTAs of the head for each warp.
 __device__ __forceinline__ void sum_dbias(const WindowArgs& a, const WindowBwdArgs& g, int head, int of, float* slice) {
   const int lane = threadIdx.x & 31, s = threadIdx.x >> 5, buckets = 2 * a.r + 1, b = of * 32 + lane;
-  constexpr int kSlices = kWBwdThreads / 32;
+  constexpr int kSlices = kWDkvThreads / 32;
   float v = 0.f;
   if (b < buckets)
 #pragma unroll 4
@@ -390,7 +392,7 @@ struct WindowDkvLayout {
 template <bool kF16>
 __device__ __forceinline__ void sum_sinks(const WindowArgs& a, const WindowBwdArgs& g, const RowsOut& dk, const RowsOut& dv, int bkv, int own) {
   const int dn = (a.d + 15) & ~15, pieces = a.d / 8, rows = min(a.n - own * kWRows, kWRows);
-  for (int u = threadIdx.x; u < 2 * rows * pieces; u += kWBwdThreads) {
+  for (int u = threadIdx.x; u < 2 * rows * pieces; u += kWDkvThreads) {
     const int c = u % pieces * 8, row = u / pieces % rows, which = u / pieces / rows;
     const RowsOut& out = which ? dv : dk;
     if (!out.data) continue;
@@ -421,7 +423,7 @@ __host__ __device__ __forceinline__ int last_of_window(int n, int left, int k0) 
 }
 
 template <bool kF16, int kD>
-__global__ void __launch_bounds__(kWBwdThreads, WindowDkvLayout<kD>::ctas)
+__global__ void __launch_bounds__(kWDkvThreads, WindowDkvLayout<kD>::ctas)
 window_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do, const __grid_constant__ CUtensorMap map_k,
                   const __grid_constant__ CUtensorMap map_v, const WindowArgs a, const WindowBwdArgs g, const RowsOut dk, const RowsOut dv) {
   typedef WindowDkvLayout<kD> L;
@@ -473,7 +475,7 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   if (!cta_ready(skip, warp == 8, bars.tmem_base, kCols)) return;
   const uint32_t tmem = bars.tmem_base;
 
-  if (warp == 8) {
+  if (warp >= 8) {
     // ------------------------------------------------------------------ copies and products
     const uint32_t k_at = smem_u32(sm), v_at = smem_u32(sm + L::v), q_at = smem_u32(sm + L::q), do_at = smem_u32(sm + L::dout);
     const uint32_t idesc_s = umma_idesc_16(128, kWCols, kF16, kF16), idesc_d = umma_idesc_16(128, (a.d + 15) & ~15, kF16, kF16, false, true);
@@ -501,47 +503,47 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       return true;
     };
     bool ok = true;
-    if (tiles.count > 0) {
-      if (elect_lane()) {
-        mbar_expect_tx(&bars.own_full, 2 * kPanels * kWRows * 128);
-        load_rows<kPanels>(k_at, &map_k, &bars.own_full, kWRows, k0, kv, batch);
-        load_rows<kPanels>(v_at, &map_v, &bars.own_full, kWRows, k0, kv, batch);
-      }
-      __syncwarp();
-      for (int t = 0; t < kStages && t < tiles.count; ++t) {
-        if (elect_lane()) load(t);
-        __syncwarp();
-        coming.next(tiles);
-      }
-      ok = mbar_wait_warp(&bars.own_full, 0, 1u) && issue(0);
-    }
-    for (int t = 0; t < tiles.count && ok; ++t) {
-      ok = mbar_wait_warp(&bars.taken, t & 1, 8u);
-      if (!ok) break;
-      if (kStages > 2 && t + 1 < tiles.count && !(ok = issue(t + 1))) break;
-      if (t > 0 && t - 1 + kStages < tiles.count) {           // the streamed tile of the step before is free
-        ok = mbar_wait_warp(&bars.done, (t - 1) & 1, 16u);
-        if (!ok) break;
-        if (elect_lane()) load((t - 1) % kStages);
-        __syncwarp();
-        coming.next(tiles);
-      }
-      if (kStages == 2 && t + 1 < tiles.count && !(ok = issue(t + 1))) break;
-      ok = mbar_wait_warp(&bars.given, t & 1, 8u);
-      if (!ok) break;
-      tc_fence_after();
-      if (elect_lane()) {
-        const int s = t % kStages;
-        if (L::p_shared) {
-          mma_streamed_ss(tmem + L::col_v, smem_u32(sm + L::p), do_at + s * L::tile, idesc_d, t == 0);
-          mma_streamed_ss(tmem + L::col_k, smem_u32(sm + L::ds), q_at + s * L::tile, idesc_d, t == 0);
-        } else {
-          mma_streamed(tmem + L::col_v, tmem + L::col_p, do_at + s * L::tile, idesc_d, t == 0);
-          mma_streamed(tmem + L::col_k, tmem + L::col_ds, q_at + s * L::tile, idesc_d, t == 0);
+    if (warp == 8) {
+      if (tiles.count > 0) {
+        if (elect_lane()) {
+          mbar_expect_tx(&bars.own_full, 2 * kPanels * kWRows * 128);
+          load_rows<kPanels>(k_at, &map_k, &bars.own_full, kWRows, k0, kv, batch);
+          load_rows<kPanels>(v_at, &map_v, &bars.own_full, kWRows, k0, kv, batch);
         }
-        umma_commit(&bars.done);
+        __syncwarp();
+        for (int t = 0; t < kStages && t < tiles.count; ++t) {
+          if (elect_lane()) load(t);
+          __syncwarp();
+          coming.next(tiles);
+        }
+        ok = mbar_wait_warp(&bars.own_full, 0, 1u) && issue(0);
       }
-      __syncwarp();
+      for (int t = 0; t + 1 < tiles.count && ok; ++t) ok = mbar_wait_warp(&bars.taken, t & 1, 8u) && issue(t + 1);
+    } else {
+      for (int t = 0; t < kStages; ++t) coming.next(tiles);
+      for (int t = 0; t < tiles.count && ok; ++t) {
+        ok = mbar_wait_warp(&bars.given, t & 1, 8u);
+        if (!ok) break;
+        tc_fence_after();
+        const int s = t % kStages;
+        if (elect_lane()) {
+          if (L::p_shared) {
+            mma_streamed_ss(tmem + L::col_v, smem_u32(sm + L::p), do_at + s * L::tile, idesc_d, t == 0);
+            mma_streamed_ss(tmem + L::col_k, smem_u32(sm + L::ds), q_at + s * L::tile, idesc_d, t == 0);
+          } else {
+            mma_streamed(tmem + L::col_v, tmem + L::col_p, do_at + s * L::tile, idesc_d, t == 0);
+            mma_streamed(tmem + L::col_k, tmem + L::col_ds, q_at + s * L::tile, idesc_d, t == 0);
+          }
+          umma_commit(&bars.done);
+        }
+        __syncwarp();
+        if (t + kStages < tiles.count) {                      // the streamed tile is free then
+          ok = mbar_wait_warp(&bars.done, t & 1, 16u);
+          if (ok && elect_lane()) load(s);
+          __syncwarp();
+          coming.next(tiles);
+        }
+      }
     }
   } else {
     // ------------------------------------------------------------------ one key row x 32 queries a thread
