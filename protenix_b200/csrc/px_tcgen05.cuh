@@ -277,6 +277,13 @@ static inline EncodeTiledFn tensor_map_encoder() {
   return fn;
 }
 
+// A thread that has not used the device yet, as the one that runs a backward pass, has no context for the driver to encode a map in: naming the
+// device that is current anyway gives it one.
+static inline bool have_context() {
+  int dev = 0;
+  return cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess;
+}
+
 // 3-D tiled map: dims/strides innermost first (strides in bytes for dims 1 and 2), zero fill outside.
 static inline bool make_map_3d(CUtensorMap* map, CUtensorMapDataType dt, const void* base, uint64_t d0, uint64_t d1,
                                uint64_t d2, uint64_t s1, uint64_t s2, uint32_t b0, uint32_t b1,

@@ -65,7 +65,7 @@ __device__ __forceinline__ void store4<__half>(__half* p, float4 v) {
 
 constexpr int kRpFwdThreads = 1024;      // one block an SM
 
-// codes: what relpos_bwd_kernel reads, [row of all batches][strip][32] (the last pair's beyond the row), or NULL.  slice: channels of W that are
+// codes: what the backward pass reads, one a pair, or NULL.  slice: channels of W that are
 // brought into shared memory at a time, all of them unless the tables are large.
 template <typename T>
 __global__ void __launch_bounds__(kRpFwdThreads) relpos_fwd_kernel(RelposArgs a, const float* __restrict__ w, T* __restrict__ z,
@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(kRpFwdThreads) relpos_fwd_kernel(RelposArgs a,
     const long long i = u / strips;                                      // counts the rows of all batches
     const int j0 = (int)(u - i * strips) * kRpPairs, count = (int)min((long long)kRpPairs, a.n - j0);
     const uint32_t code = relpos_code(a, i, i / a.n * a.n + j0 + min(lane, count - 1));
-    if (codes && blockIdx.y == 0) codes[u * kRpPairs + lane] = code;
+    if (codes && blockIdx.y == 0 && lane < count) codes[i * a.n + j0 + lane] = code;
     T* out = z + (i * a.n + j0) * a.c + c0 + 4 * lane;
     uint32_t have = 0xffffffffu;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -139,6 +139,25 @@ template <>
 __device__ __forceinline__ float load1<__half>(const __half* p) { return __half2float(*p); }
 
 constexpr int kRpBwdThreads = kRpChunk;      // a thread = one channel
+
+// The columns of W from a thread's sums by table row (row k: mine[k * kRpChunk]): a row of the first table counts for its position and its token column, one of
+// the second for its own and, unless the entities differ, the entity's.
+__device__ __forceinline__ void relpos_fold(const RelposArgs& a, const float* mine, float* out) {
+  const int t = a.columns(), tok = 2 * a.r + 2, ent = 4 * a.r + 4, rows1 = a.rows1();
+  const auto range = [&](int from, int to) {
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int k = from; k < to; k += 4)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += k + e < to ? mine[(k + e) * kRpChunk] : 0.f;
+    return (v[0] + v[1]) + (v[2] + v[3]);
+  };
+#pragma unroll 8
+  for (int k = 0; k < ent - 1; ++k) out[k * kRpChunk] = mine[k * kRpChunk];
+  out[a.r * kRpChunk] = mine[a.r * kRpChunk] + range(tok, rows1);      // pairs of one residue, whatever their tokens
+  out[(ent - 1) * kRpChunk] = range(0, tok);
+  out[ent * kRpChunk] = range(rows1, rows1 + 2 * a.s + 1);
+  for (int k = ent + 1; k < t; ++k) out[k * kRpChunk] = mine[(rows1 + k - ent - 1) * kRpChunk];
+}
 
 // Block b adds up the units [b * per, (b + 1) * per) of its channels; a unit is a row's strip of 32 pairs.  partial: [chunk][block][columns][kRpChunk].
 template <typename T>
@@ -211,14 +230,16 @@ __global__ void __launch_bounds__(kRpBwdThreads, 2) relpos_bwd_kernel(RelposArgs
       row2 = (int)(now >> 16);
     }
   };
-  const uint32_t* const my_codes = codes + begin * kRpPairs + lane;
-  uint32_t code = 0, next = steps > 0 ? __ldg(my_codes) : 0;
+  const auto code_at = [&](const Place& p) { return __ldg(codes + p.i * n + min(p.strip * kRpPairs + lane, n - 1)); };
+  Place then = here;
+  uint32_t code = 0, next = steps > 0 ? code_at(then) : 0;
   bool ok = true;
   for (int step = 0; step < steps; ++step) {
     const int part = step % kParts, count = pairs_of(here, part), b = step % kRpStages;
     if (part == 0) {
       code = next;
-      if (step + kParts < steps) next = __ldg(my_codes + (long long)(step / kParts + 1) * kRpPairs);
+      then.next(strips);
+      if (step + kParts < steps) next = code_at(then);
     }
     ok = mbar_wait_warp(&full[b], (step / kRpStages) & 1, 1u);
     // All are through with the stage that is filled next.  (Barriers of the four warps' own, asked by a fifth warp or by the first, let them drift apart and
@@ -283,22 +304,151 @@ __global__ void __launch_bounds__(kRpBwdThreads, 2) relpos_bwd_kernel(RelposArgs
   }
   flush(row1, run1);
   flush(row2 >= 0 ? rows1 + row2 : -1, run2);
-  // the columns of W: a table row counts for its position and its token column, a copy row for its own and, unless the entities differ, the entity's
-  const int t = a.columns(), tok = 2 * a.r + 2, ent = 4 * a.r + 4;
-  float* const out = partial + ((long long)blockIdx.y * gridDim.x + blockIdx.x) * t * kRpChunk + threadIdx.x;
-  const auto range = [&](int from, int to) {
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int k = from; k < to; k += 4)
+  relpos_fold(a, mine, partial + ((long long)blockIdx.y * gridDim.x + blockIdx.x) * a.columns() * kRpChunk + threadIdx.x);
+}
+
+// The same for 16-bit dz on the tensor cores: the sums by table row are dz^T times the pairs' two-hot rows, M = 128 channels, N = table rows, K = pairs.
+// dz enters as it lies (its channels are the contiguous index: an MN-major operand), the two-hot operand [table row][64 pairs] lives in shared memory and costs
+// a lane two stores a pair to set and two to clear (four warps of them: one took 1100 cycles a tile, where memory takes 700); the products with one are exact.  64 pairs are 288 cycles of the tensor pipe (N = 144), less than half of what
+// their 16 KB take to arrive.  The tensor core truncates when it adds, so an accumulator takes eight tiles (32 additions) before four warps add it, rounding to
+// nearest, to fp32 sums in shared memory, while the next tiles go to the other accumulator.
+// Warps 0..3 drain (a thread = one channel), 4 brings dz, 5 issues the products, 6..9 write the two-hot operands, 32 pairs of every other tile each.
+constexpr int kRpTile = 64, kRpRing = 4, kRpGroup = 8;      // pairs of a tile, tiles on their way, tiles of an accumulator
+constexpr int kRpTcThreads = 10 * 32, kRpTileBytes = kRpTile * kRpChunk * 2;
+constexpr int kRpTcRows = 208;                              // what shared memory holds of sums and operands
+struct RpTcBars {
+  uint64_t full[kRpRing], empty[kRpRing], hot_full[2], hot_empty[2], acc_full[2], acc_free[2];
+  uint32_t tmem_base;
+};
+
+template <bool kF16>
+__global__ void __launch_bounds__(kRpTcThreads, 1) relpos_bwd_tc_kernel(const __grid_constant__ CUtensorMap map, RelposArgs a,
+                                                                        const uint32_t* __restrict__ codes, float* __restrict__ partial, int n_cols,
+                                                                        int per) {
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char* sm = smem_aligned(smem_raw);
+  unsigned char* const hot = sm + kRpRing * kRpTileBytes;                                    // two operands [n_cols][64], 128-byte swizzle
+  float* const sums = reinterpret_cast<float*>(hot + 2 * n_cols * 128);                      // [n_cols][128]
+  RpTcBars& bars = *reinterpret_cast<RpTcBars*>(reinterpret_cast<unsigned char*>(sums) + n_cols * kRpChunk * 4);
+  const int warp = warp_index(), lane = threadIdx.x & 31, c0 = blockIdx.y * kRpChunk;
+  const long long all = (a.pairs + kRpTile - 1) / kRpTile, begin = (long long)blockIdx.x * per;
+  const int tiles = (int)(min(begin + per, all) - begin), groups = (tiles + kRpGroup - 1) / kRpGroup;
+  const bool skip = cta_begin();
+  if (threadIdx.x == 0) {
+    for (int k = 0; k < kRpRing; ++k) {
+      mbar_init(&bars.full[k], 1);
+      mbar_init(&bars.empty[k], 1);
+    }
+    for (int k = 0; k < 2; ++k) {
+      mbar_init(&bars.hot_full[k], 2);
+      mbar_init(&bars.hot_empty[k], 1);
+      mbar_init(&bars.acc_full[k], 1);
+      mbar_init(&bars.acc_free[k], 4);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+  }
+  for (int k = threadIdx.x; k < 2 * n_cols * 8; k += kRpTcThreads) reinterpret_cast<uint4*>(hot)[k] = make_uint4(0u, 0u, 0u, 0u);
+  if (warp == 5) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&bars.tmem_base)), "r"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+  }
+  if (!cta_ready(skip, warp == 5, bars.tmem_base, 512)) return;
+  const uint32_t tmem = bars.tmem_base;
+  if (warp == 4) {
+    bool ok = true;
+    for (int t = 0; t < tiles && ok; ++t) {
+      const int s = t % kRpRing;
+      if (t >= kRpRing) ok = mbar_wait_warp(&bars.empty[s], (t / kRpRing - 1) & 1, 1u);
+      if (ok && elect_lane()) {
+        const int p0 = (int)((begin + t) * kRpTile);
+        const uint32_t dst = smem_u32(sm + s * kRpTileBytes);
+        mbar_expect_tx(&bars.full[s], kRpTileBytes);
+        tma_load_3d(dst, &map, &bars.full[s], c0, p0, 0);
+        tma_load_3d(dst + kRpTile * 128, &map, &bars.full[s], c0 + 64, p0, 0);
+      }
+      __syncwarp();
+    }
+  } else if (warp >= 6) {
+    const int rows1 = a.rows1();
+    const int b = warp & 1, k = 32 * ((warp - 6) >> 1) + lane;      // the operand, and this lane's pair of each of its tiles
+    unsigned char* const operand = hot + b * n_cols * 128;
+    const auto code_at = [&](int t) {
+      const long long p = (begin + t) * kRpTile + k;
+      return t < tiles && p < a.pairs ? __ldg(codes + p) : 0xffffffffu;
+    };
+    const auto put = [&](uint32_t code, uint16_t v) {
+      if (code == 0xffffffffu) return;
+      const int first = code & 0xffffu, second = rows1 + (code >> 16);
+      *reinterpret_cast<uint16_t*>(operand + first * 128 + (((k >> 3) ^ (first & 7)) << 4) + 2 * (k & 7)) = v;
+      *reinterpret_cast<uint16_t*>(operand + second * 128 + (((k >> 3) ^ (second & 7)) << 4) + 2 * (k & 7)) = v;
+    };
+    constexpr uint16_t kOne = kF16 ? 0x3c00 : 0x3f80;
+    uint32_t was = 0xffffffffu, next = code_at(b);
+    bool ok = true;
+    for (int t = b; t < tiles && ok; t += 2) {
+      const uint32_t now = next;
+      next = code_at(t + 2);
+      if (t >= 2) ok = mbar_wait_warp(&bars.hot_empty[b], (t / 2 - 1) & 1, 2u);
+      if (now != was) {
+        put(was, 0);
+        put(now, kOne);
+        was = now;
+      }
+      asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars.hot_full[b]);
+    }
+  } else if (warp == 5) {
+    // the operands' first contents are zeros written by all threads
+    asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+    const uint32_t idesc = umma_idesc_16(128, n_cols, kF16, kF16, true, false);
+    bool ok = true;
+    for (int t = 0; t < tiles && ok; ++t) {
+      const int s = t % kRpRing, b = t & 1, g = t / kRpGroup, in_group = t % kRpGroup;
+      if (in_group == 0 && g >= 2) ok = mbar_wait_warp(&bars.acc_free[g & 1], (g / 2 - 1) & 1, 4u);
+      ok = ok && mbar_wait_warp(&bars.hot_full[b], (t / 2) & 1, 8u) && mbar_wait_warp(&bars.full[s], (t / kRpRing) & 1, 16u);
+      if (!ok) break;
+      tc_fence_after();
+      if (elect_lane()) {
+        const uint64_t da = umma_desc_mn_sw128(smem_u32(sm + s * kRpTileBytes), kRpTile * 128, 1024), db = umma_desc_sw128(smem_u32(hot + b * n_cols * 128));
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] += k + e < to ? mine[(k + e) * kRpChunk] : 0.f;
-    return (v[0] + v[1]) + (v[2] + v[3]);
-  };
-#pragma unroll 8
-  for (int k = 0; k < ent - 1; ++k) out[k * kRpChunk] = mine[k * kRpChunk];
-  out[a.r * kRpChunk] = mine[a.r * kRpChunk] + range(tok, rows1);      // pairs of one residue, whatever their tokens
-  out[(ent - 1) * kRpChunk] = range(0, tok);
-  out[ent * kRpChunk] = range(rows1, rows1 + 2 * a.s + 1);
-  for (int k = ent + 1; k < t; ++k) out[k * kRpChunk] = mine[(rows1 + k - ent - 1) * kRpChunk];
+        for (int ks = 0; ks < kRpTile / 16; ++ks) umma_bf16(tmem + 256 * (g & 1), da + 128 * ks, db + 2 * ks, idesc, in_group > 0 || ks > 0);
+        umma_commit(&bars.empty[s]);
+        umma_commit(&bars.hot_empty[b]);
+        if (in_group == kRpGroup - 1 || t == tiles - 1) umma_commit(&bars.acc_full[g & 1]);
+      }
+      __syncwarp();
+    }
+  } else {
+    float* const mine = sums + threadIdx.x;       // a thread's channel: row k at mine[k * kRpChunk]
+    const uint32_t t_lane = tmem + ((uint32_t)(32 * warp) << 16);
+    bool ok = true;
+    for (int g = 0; g < groups; ++g) {
+      ok = mbar_wait_warp(&bars.acc_full[g & 1], (g >> 1) & 1, 32u);
+      if (!ok) break;
+      tc_fence_after();
+      for (int k = 0; k < n_cols; k += 16) {
+        uint32_t x[16];
+        tmem_ld16(t_lane + 256 * (g & 1) + k, x);
+        float v[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] = g > 0 ? mine[(k + e) * kRpChunk] : 0.f;
+        tmem_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mine[(k + e) * kRpChunk] = v[e] + __uint_as_float(x[e]);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars.acc_free[g & 1]);
+    }
+    if (ok) relpos_fold(a, mine, partial + ((long long)blockIdx.y * gridDim.x + blockIdx.x) * a.columns() * kRpChunk + threadIdx.x);
+  }
+  tc_fence_before();
+  cta_teardown_sync();
+  if (warp == 5) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512) : "memory");
+  }
 }
 
 // dw[c][t] = the blocks' sums, in their order: eight slices of the blocks, each added up by one thread a channel, then the slices.
@@ -333,6 +483,11 @@ static bool relpos_fits(int64_t c, int32_t r, int32_t s) {
 static int64_t relpos_units(int64_t batch, int64_t n) { return batch * n * ((n + kRpPairs - 1) / kRpPairs); }
 static int64_t relpos_blocks(int64_t units) { return std::max<int64_t>(1, std::min<int64_t>(2 * sm_count(), units / 16)); }
 
+// 16-bit gradients with tables that fit.
+static bool relpos_on_tensor_cores(int64_t pairs, int n_cols, int32_t dtype) {
+  return dtype != PX_F32 && n_cols <= kRpTcRows && pairs < (int64_t)0x7fffff00;
+}
+
 }  // namespace px
 
 using namespace px;
@@ -344,7 +499,7 @@ extern "C" int64_t px_relpos_workspace_bytes(int64_t batch, int64_t n, int64_t c
 }
 
 extern "C" int64_t px_relpos_codes_bytes(int64_t batch, int64_t n) {
-  return relpos_sizes(batch, n, 8, 0, 0) && n > 0 ? relpos_units(batch, n) * kRpPairs * 4 : 0;
+  return relpos_sizes(batch, n, 8, 0, 0) ? batch * n * n * 4 : 0;
 }
 
 extern "C" int32_t px_relpos_fwd(const int64_t* asym_id, const int64_t* residue_index, const int64_t* entity_id, const int64_t* token_index,
@@ -384,20 +539,40 @@ extern "C" int32_t px_relpos_bwd(const uint32_t* codes, const void* dz, float* d
     return cudaMemsetAsync(dw, 0, (size_t)c * a.columns() * 4, st) == cudaSuccess ? PX_OK : PX_ERR_LAUNCH;
   if (!codes || !dz || !workspace || (((uintptr_t)dz | (uintptr_t)workspace) & 15)) return PX_ERR_BAD_ARG;
   if (workspace_bytes < px_relpos_workspace_bytes(batch, n, c, r_max, s_max)) return PX_ERR_WORKSPACE;
-  const int64_t units = relpos_units(batch, n), most = relpos_blocks(units), per = (units + most - 1) / most;
-  const int blocks = (int)((units + per - 1) / per);
   const unsigned chunks = (unsigned)((c + kRpChunk - 1) / kRpChunk);
   float* const partial = (float*)workspace;
-  const size_t fixed = (size_t)kRpStages * kRpStageBytes, smem = fixed + (size_t)(a.rows1() + a.rows2()) * kRpChunk * 4;
-  static SmemLimit limit[3];
-  const auto go = [&](auto* kernel, auto* in) {
-    if (!limit[dtype].set(kernel, fixed + (size_t)kRpMaxRows * kRpChunk * 4)) return false;
-    kernel<<<dim3((unsigned)blocks, chunks), kRpBwdThreads, smem, st>>>(a, in, codes, partial, (int)per);
-    return cudaGetLastError() == cudaSuccess;
-  };
-  const bool done = dtype == PX_F32    ? go(relpos_bwd_kernel<float>, (const float*)dz)
-                    : dtype == PX_BF16 ? go(relpos_bwd_kernel<bf16>, (const bf16*)dz)
-                                       : go(relpos_bwd_kernel<__half>, (const __half*)dz);
+  const int rows = a.rows1() + a.rows2(), n_cols = (rows + 15) / 16 * 16;
+  int blocks;
+  bool done;
+  if (relpos_on_tensor_cores(a.pairs, n_cols, dtype)) {
+    const int64_t tiles = (a.pairs + kRpTile - 1) / kRpTile, most = std::min<int64_t>(relpos_blocks(relpos_units(batch, n)), sm_count());
+    const int64_t per = (tiles + most - 1) / most;
+    blocks = (int)((tiles + per - 1) / per);
+    CUtensorMap map;
+    if (!have_context() ||
+        !make_map_3d(&map, dtype == PX_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, dz, (uint64_t)c, (uint64_t)a.pairs, 1,
+                     (uint64_t)c * 2, (uint64_t)a.pairs * c * 2, 64, kRpTile, CU_TENSOR_MAP_SWIZZLE_128B))
+      return PX_ERR_LAUNCH;
+    const auto bytes = [](int cols) { return (size_t)kRpRing * kRpTileBytes + (size_t)cols * (2 * 128 + kRpChunk * 4) + sizeof(RpTcBars) + 1024; };
+    static SmemLimit limit[2];
+    const auto kernel = dtype == PX_F16 ? relpos_bwd_tc_kernel<true> : relpos_bwd_tc_kernel<false>;
+    if (!limit[dtype == PX_F16].set(kernel, bytes(kRpTcRows))) return PX_ERR_LAUNCH;
+    kernel<<<dim3((unsigned)blocks, chunks), kRpTcThreads, bytes(n_cols), st>>>(map, a, codes, partial, n_cols, (int)per);
+    done = cudaGetLastError() == cudaSuccess;
+  } else {
+    const int64_t units = relpos_units(batch, n), most = relpos_blocks(units), per = (units + most - 1) / most;
+    blocks = (int)((units + per - 1) / per);
+    const size_t fixed = (size_t)kRpStages * kRpStageBytes, smem = fixed + (size_t)rows * kRpChunk * 4;
+    static SmemLimit limit[3];
+    const auto go = [&](auto* kernel, auto* in) {
+      if (!limit[dtype].set(kernel, fixed + (size_t)kRpMaxRows * kRpChunk * 4)) return false;
+      kernel<<<dim3((unsigned)blocks, chunks), kRpBwdThreads, smem, st>>>(a, in, codes, partial, (int)per);
+      return cudaGetLastError() == cudaSuccess;
+    };
+    done = dtype == PX_F32    ? go(relpos_bwd_kernel<float>, (const float*)dz)
+           : dtype == PX_BF16 ? go(relpos_bwd_kernel<bf16>, (const bf16*)dz)
+                              : go(relpos_bwd_kernel<__half>, (const __half*)dz);
+  }
   if (!done) return PX_ERR_LAUNCH;
   relpos_reduce_kernel<<<dim3((unsigned)a.columns(), chunks), 8 * kRpChunk, 0, st>>>(partial, dw, blocks, a.columns(), (int)c);
   return cudaGetLastError() == cudaSuccess ? PX_OK : PX_ERR_LAUNCH;

@@ -308,13 +308,6 @@ namespace px {
 
 PX_DEFINE_FAMILY_HOOKS(window)
 
-// A thread that has not used the device yet, as the one that runs a backward pass, has no context for the driver to encode a map in: naming the
-// device that is current anyway gives it one.
-static bool have_context() {
-  int dev = 0;
-  return cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess;
-}
-
 // [batch][head][n][d] 16-bit values: boxes of 64 elements x 64 rows.
 static bool rows_map(CUtensorMap* map, const px_rows& t, const px_window& w, int64_t heads) {
   EncodeTiledFn enc = tensor_map_encoder();
