@@ -68,13 +68,14 @@ struct DropoutArgs {
   long long* used;                     // receives the pair that the call used, or NULL
 };
 
-// Whether the elements at, at + 1, ... are kept.  `at` is a multiple of four unless VEC is 1.
-template <int VEC>
+// Whether the elements at, at + 1, ... are kept.  `at` is a multiple of four unless VEC is 1.  kFew: there are fewer than 2^34 of them, so that the counter's
+// second word is zero like the offset's are fixed, and two of the twenty products need not be made for each block of four.
+template <int VEC, bool kFew>
 __device__ __forceinline__ void kept(const DropoutArgs& a, const RoundKeys& keys, unsigned long long offset, long long at, bool (&keep)[VEC]) {
 #pragma unroll
   for (int q = 0; q < (VEC + 3) / 4; ++q) {
     const unsigned long long block = ((unsigned long long)at >> 2) + q;
-    uint32_t c[4] = {(uint32_t)block, (uint32_t)(block >> 32), (uint32_t)offset, (uint32_t)(offset >> 32)};
+    uint32_t c[4] = {(uint32_t)block, kFew ? 0u : (uint32_t)(block >> 32), (uint32_t)offset, (uint32_t)(offset >> 32)};
     philox4x32(c, keys);
     if constexpr (VEC == 1) {
       const int w = (int)(at & 3);
@@ -117,7 +118,7 @@ __device__ __forceinline__ Pack<T, VEC> dropped(const Pack<T, VEC>& x, const Pac
 }
 
 // One value per element: thread = 16 bytes, the last of them element by element.
-template <typename T, int VEC, bool kResidual>
+template <typename T, int VEC, bool kResidual, bool kFew>
 __global__ void __launch_bounds__(256) dropout_kernel(const T* residual, const T* x, T* out, DropoutArgs a) {
   typedef Pack<T, VEC> V;
   const unsigned long long seed = a.state ? (unsigned long long)a.state[0] : a.seed;
@@ -134,7 +135,7 @@ __global__ void __launch_bounds__(256) dropout_kernel(const T* residual, const T
       V rv = xv;
       if (kResidual) rv = *reinterpret_cast<const V*>(residual + i);
       bool keep[VEC];
-      kept<VEC>(a, keys, offset, i, keep);
+      kept<VEC, kFew>(a, keys, offset, i, keep);
       *reinterpret_cast<V*>(out + i) = dropped<T, VEC, kResidual>(xv, rv, keep, a.scale);
     } else {
       for (long long e = i; e < total; ++e) {
@@ -142,7 +143,7 @@ __global__ void __launch_bounds__(256) dropout_kernel(const T* residual, const T
         Pack<T, 1> r1 = x1;
         if (kResidual) r1.v[0] = residual[e];
         bool keep[1];
-        kept<1>(a, keys, offset, e, keep);
+        kept<1, false>(a, keys, offset, e, keep);
         out[e] = dropped<T, 1, kResidual>(x1, r1, keep, a.scale).v[0];
       }
     }
@@ -177,7 +178,7 @@ __global__ void __launch_bounds__(256) dropout_shared_kernel(const T* residual, 
       }
     }
     bool keep[VEC];
-    kept<VEC>(a, keys, offset, m, keep);
+    kept<VEC, false>(a, keys, offset, m, keep);
 #pragma unroll
     for (int s = 0; s < kSharedRows; ++s)
       if (s < count) *reinterpret_cast<V*>(out + at + s * a.inner) = dropped<T, VEC, kResidual>(xv[s], rv[s], keep, a.scale);
@@ -189,7 +190,8 @@ static cudaError_t launch_dropout_as(const void* residual, const void* x, void* 
   const int64_t most = (int64_t)sm_count() * 32;           // blocks
   if (a.shared == 1) {
     const int64_t blocks = std::min<int64_t>((a.inner / VEC + 1 + 255) / 256, most);
-    dropout_kernel<T, VEC, kResidual><<<(unsigned)blocks, 256, 0, st>>>((const T*)residual, (const T*)x, (T*)out, a);
+    const auto kernel = a.inner < (1ll << 34) ? dropout_kernel<T, VEC, kResidual, true> : dropout_kernel<T, VEC, kResidual, false>;
+    kernel<<<(unsigned)blocks, 256, 0, st>>>((const T*)residual, (const T*)x, (T*)out, a);
   } else {
     const int64_t units = a.outer * a.inner / VEC * ((a.shared + kSharedRows - 1) / kSharedRows);
     const int64_t blocks = std::min<int64_t>((units + 255) / 256, most);

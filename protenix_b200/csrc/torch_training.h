@@ -297,7 +297,7 @@ Tensor window_attention(const Tensor& q, const Tensor& k, const Tensor& v, int64
     want.push_back(n);
     if (mask->dim() < 1 || !at::is_expandable_to(mask->sizes(), want)) fail("mask must be [..., N] over the batch axes of q, got " + shape_of(*mask));
     const Tensor truth = mask->scalar_type() == at::kBool ? mask->detach() : mask->detach().ne(0);
-    m = truth.dim() == 2 && truth.size(0) == batch ? truth.contiguous() : truth.expand(want).reshape({batch, n}).contiguous();
+    m = truth.dim() == 2 && truth.size(0) == batch && truth.size(1) == n ? truth.contiguous() : truth.expand(want).reshape({batch, n}).contiguous();
   }
   const auto four = [&](const Tensor& t) { return t.dim() == 4 ? t : t.reshape({batch, t.size(-3), n, d}); };
   const Tensor q4 = four(q), k4 = four(k), v4 = four(v);

@@ -182,6 +182,22 @@ def test_layouts():
 
 
 @pytest.mark.gpu
+def test_shapes_of_a_mask():
+    """One row for all samples, one value for a sample, any type."""
+    q, k, v, grad, _ = _inputs(3, 2, 2, 140, 32, BF16)
+    at = torch.arange(140, device="cuda")
+    row = (at % 3 != 0)
+    want = px.window_attention(q, k, v, 20, mask=row[None].expand(3, 140).contiguous())
+    for m in (row, row[None], row.float(), row.to(torch.int32) * 7, row[None].expand(3, 140)):
+        assert torch.equal(px.window_attention(q, k, v, 20, mask=m), want)
+    some = torch.tensor([[True], [False], [True]], device="cuda")
+    got = px.window_attention(q, k, v, 20, mask=some)
+    plain = px.window_attention(q, k, v, 20)
+    assert torch.equal(got[0], plain[0]) and torch.equal(got[2], plain[2]) and not got[1].any()
+    assert torch.equal(px.window_attention(q, k, v, 20, mask=torch.ones(1, device="cuda")), plain)
+
+
+@pytest.mark.gpu
 def test_some_gradients_only():
     q, k, v, grad, bias = _inputs(1, 4, 2, 200, 32, BF16, 8)
     want = _run(q, k, v, grad, bias, None, 50, 0, 3)
