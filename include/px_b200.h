@@ -417,6 +417,7 @@ PX_API int32_t px_relpos_bwd(const uint32_t* codes, const void* dz, float* dw, v
  * Rows q, o [batch][heads][n][d], k, v [batch][kv_heads][n][d] with the strides of px_rows; query head h uses key head h / (heads /
  * kv_heads).  PX_BF16 or PX_F16; d a multiple of 8 up to 128; products of 16-bit operands, everything else fp32.  What masked keys and
  * queries that see nothing hold (NaN included) has no influence.  lse: px_window_lse_floats() floats that the backward pass reads, or NULL.
+ * o_rest (rows like o, same type, or NULL): what the rounding of o has taken off, which makes the gradients of narrow windows up to three times as exact.
  * px_window_bwd writes those of dq, dk, dv (types and shapes of q, k, v) and dbias (bias_dtype) that are not NULL; sums have a fixed
  * order.  Workspace aligned to 256 bytes.  Stands in for the local attention of protenix/model/modules/primitives.py
  * (n_queries / n_keys) where the window moves with the query, not with its block. */
@@ -434,11 +435,11 @@ typedef struct {
   int32_t dtype, bias_dtype;
 } px_window;
 PX_API int64_t px_window_lse_floats(int64_t batch, int64_t heads, int64_t n);
-PX_API int32_t px_window_fwd(const px_window* w, const px_rows* q, const px_rows* k, const px_rows* v, const px_rows* o, float* lse,
-                      void* stream);
+PX_API int32_t px_window_fwd(const px_window* w, const px_rows* q, const px_rows* k, const px_rows* v, const px_rows* o, const px_rows* o_rest,
+                      float* lse, void* stream);
 PX_API int64_t px_window_workspace_bytes(const px_window* w, int32_t bias_grad);
-PX_API int32_t px_window_bwd(const px_window* w, const px_rows* q, const px_rows* k, const px_rows* v, const px_rows* o, const px_rows* dout,
-                      const float* lse, const px_rows* dq, const px_rows* dk, const px_rows* dv, void* dbias, void* workspace,
+PX_API int32_t px_window_bwd(const px_window* w, const px_rows* q, const px_rows* k, const px_rows* v, const px_rows* o, const px_rows* o_rest,
+                      const px_rows* dout, const float* lse, const px_rows* dq, const px_rows* dk, const px_rows* dv, void* dbias, void* workspace,
                       int64_t workspace_bytes, void* stream);
 
 /* ---- Exchange between the GPUs of one box (row-sharded path) ------------------------------

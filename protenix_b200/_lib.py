@@ -86,9 +86,9 @@ SIGNATURES = {
     "px_relpos_fwd": (I32, [P, P, P, P, P, P, P, P, I64, I64, I64, I32, I32, I32, P]),
     "px_relpos_bwd": (I32, [P, P, P, P, I64, I64, I64, I64, I32, I32, I32, P]),
     "px_window_lse_floats": (I64, [I64, I64, I64]),
-    "px_window_fwd": (I32, [P, P, P, P, P, P, P]),
+    "px_window_fwd": (I32, [P, P, P, P, P, P, P, P]),
     "px_window_workspace_bytes": (I64, [P, I32]),
-    "px_window_bwd": (I32, [P, P, P, P, P, P, P, P, P, P, P, P, I64, P]),
+    "px_window_bwd": (I32, [P, P, P, P, P, P, P, P, P, P, P, P, P, I64, P]),
     "px_opm_outer": (I32, [P, P, P, I64, I64, I64, P]),
     "px_opm_out": (I32, [P, P, P, P, P, P, I32, I64, I64, I32, P]),
     "px_peer_alloc": (I32, [I64, P, P]),

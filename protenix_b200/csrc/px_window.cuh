@@ -204,6 +204,22 @@ __device__ __forceinline__ void store8(void* to, const uint32_t* v, float scale)
   *reinterpret_cast<uint4*>(to) = w;
 }
 
+// The same, and what the rounding has taken off each value as 16 bits more, at `rest` unless that is NULL.
+template <bool kF16>
+__device__ __forceinline__ void store8(void* to, void* rest, const uint32_t* v, float scale) {
+  uint4 w, r;
+  uint32_t *o = reinterpret_cast<uint32_t*>(&w), *q = reinterpret_cast<uint32_t*>(&r);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float a = __uint_as_float(v[2 * e]) * scale, b = __uint_as_float(v[2 * e + 1]) * scale;
+    o[e] = pack16x2<kF16>(a, b);
+    const float2 back = unpack16x2<kF16>(o[e]);
+    q[e] = pack16x2<kF16>(a - back.x, b - back.y);
+  }
+  *reinterpret_cast<uint4*>(to) = w;
+  if (rest) *reinterpret_cast<uint4*>(rest) = r;
+}
+
 __device__ __forceinline__ void tmem_alloc(uint32_t* base, uint32_t cols) {      // whole warp
   asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(base)), "r"(cols) : "memory");
   asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");

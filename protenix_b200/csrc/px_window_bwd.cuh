@@ -60,7 +60,7 @@ template <bool kF16, int kD, bool kBiasGrad>
 __global__ void __launch_bounds__(kWDqThreads, 2)
 window_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do, const __grid_constant__ CUtensorMap map_k,
                  const __grid_constant__ CUtensorMap map_v, const WindowArgs a, const WindowBwdArgs g, const RowsOut dout, const RowsOut o,
-                 const RowsOut dq) {
+                 const RowsOut rest, const RowsOut dq) {
   typedef WindowDqLayout<kD> L;
   constexpr uint32_t kCols = L::cols;
   constexpr int kK = L::k_stages, kV = L::v_stages, kPanels = L::panels;
@@ -165,17 +165,18 @@ window_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     // ------------------------------------------------------------------ one query row x 32 keys a thread
     const int quarter = warp & 3, half = warp >> 2, row = 32 * quarter + lane, i = q0 + row, qw = q0 + 32 * quarter;
     const uint32_t t_lane = tmem + ((uint32_t)(32 * quarter) << 16);
-    // All loads of the beginning at once: one after the other they took 4000 cycles, as much as two tiles.  delta = dO . O, each thread over
-    // its half of the 16-byte pieces of the row.
+    // All loads of the beginning at once: one after the other they took 4000 cycles, as much as two tiles.  delta = dO . O with what the
+    // rounding of O has taken off, each thread over its half of the 16-byte pieces of the row.
     const float nlse = g.nlse[(size_t)bh * a.npad + i];
-    uint4 u[kD / 16], v[kD / 16];
-    const uint16_t *x = dout.at(batch, head, i), *y = o.at(batch, head, i);
+    uint4 u[kD / 16], v[kD / 16], z[kD / 16];
+    const uint16_t *x = dout.at(batch, head, i), *y = o.at(batch, head, i), *more = rest.data ? rest.at(batch, head, i) : nullptr;
 #pragma unroll
     for (int e = 0; e < kD / 16; ++e) {
       const int c = 8 * half + 16 * e;
       const bool there = i < a.n && c < a.d;
       u[e] = there ? __ldg(reinterpret_cast<const uint4*>(x + c)) : make_uint4(0u, 0u, 0u, 0u);
       v[e] = there ? __ldg(reinterpret_cast<const uint4*>(y + c)) : make_uint4(0u, 0u, 0u, 0u);
+      z[e] = there && more ? __ldg(reinterpret_cast<const uint4*>(more + c)) : make_uint4(0u, 0u, 0u, 0u);
     }
     if (a.r >= 0) {
       bias_fill(a, head, bias, 256);
@@ -185,11 +186,11 @@ window_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     float sum = 0.f;
 #pragma unroll
     for (int e = 0; e < kD / 16; ++e) {
-      const uint32_t us[4] = {u[e].x, u[e].y, u[e].z, u[e].w}, vs[4] = {v[e].x, v[e].y, v[e].z, v[e].w};
+      const uint32_t us[4] = {u[e].x, u[e].y, u[e].z, u[e].w}, vs[4] = {v[e].x, v[e].y, v[e].z, v[e].w}, zs[4] = {z[e].x, z[e].y, z[e].z, z[e].w};
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const float2 p = unpack16x2<kF16>(us[k]), q = unpack16x2<kF16>(vs[k]);
-        sum = fmaf(p.x, q.x, fmaf(p.y, q.y, sum));
+        const float2 p = unpack16x2<kF16>(us[k]), q = unpack16x2<kF16>(vs[k]), r = unpack16x2<kF16>(zs[k]);
+        sum = fmaf(p.x, q.x + r.x, fmaf(p.y, q.y + r.y, sum));
       }
     }
     part[half * kWRows + row] = sum;

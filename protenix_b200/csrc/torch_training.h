@@ -208,13 +208,14 @@ px_window window_of(const Tensor& q, const Tensor& k, const Tensor& bias, const 
   w.dtype = dtype_code(q, "q");
   return w;
 }
-Tensor window_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& bias, const Tensor& mask, const WindowCall& c, Tensor* lse) {
+Tensor window_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& bias, const Tensor& mask, const WindowCall& c, Tensor* lse, Tensor* rest) {
   const Tensor o = rows_like(q);
   const px_window w = window_of(q, k, bias, mask, c);
   if (lse) *lse = at::empty({abi.px_window_lse_floats(w.batch, w.heads, w.n)}, q.options().dtype(at::kFloat));
-  const px_rows rq = rows_of(q), rk = rows_of(k), rv = rows_of(v), ro = rows_of(o);
+  if (rest) *rest = rows_like(q);
+  const px_rows rq = rows_of(q), rk = rows_of(k), rv = rows_of(v), ro = rows_of(o), rr = rest ? rows_of(*rest) : px_rows{};
   const cudaStream_t st = at::cuda::getCurrentCUDAStream();
-  launch("px_window_fwd", st, [&] { return abi.px_window_fwd(&w, &rq, &rk, &rv, &ro, lse ? (float*)lse->data_ptr() : nullptr, st); });
+  launch("px_window_fwd", st, [&] { return abi.px_window_fwd(&w, &rq, &rk, &rv, &ro, rest ? &rr : nullptr, lse ? (float*)lse->data_ptr() : nullptr, st); });
   return o;
 }
 
@@ -224,9 +225,9 @@ struct WindowFunction : torch::autograd::Function<WindowFunction> {
     c10::cuda::CUDAGuard guard(q_.device());
     const Tensor q = rows_fitted(q_), k = rows_fitted(k_), v = rows_fitted(v_);
     const Tensor bias = has(bias_) ? bias_->contiguous() : Tensor(), mask = has(mask_) ? *mask_ : Tensor();
-    Tensor lse;
-    const Tensor o = window_forward(q, k, v, bias, mask, {left, right, sinks, scale}, &lse);
-    ctx->save_for_backward({q, k, v, o, lse, bias, mask});
+    Tensor lse, rest;
+    const Tensor o = window_forward(q, k, v, bias, mask, {left, right, sinks, scale}, &lse, &rest);
+    ctx->save_for_backward({q, k, v, o, lse, bias, mask, rest});
     ctx->saved_data["window"] = c10::List<int64_t>({left, right, sinks});
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["f"] = (int64_t)q_.requires_grad() | (int64_t)k_.requires_grad() << 1 | (int64_t)v_.requires_grad() << 2 |
@@ -250,10 +251,10 @@ struct WindowFunction : torch::autograd::Function<WindowFunction> {
     const int64_t bytes = abi.px_window_workspace_bytes(&w, f >> 3 & 1);
     const Tensor ws = bytes_like(q, bytes);
     const auto opt = [](const Tensor& t) { return t.defined() ? rows_of(t) : px_rows{}; };
-    const px_rows rq = rows_of(q), rk = rows_of(k), rv = rows_of(v), ro = rows_of(o), rg = rows_of(dout), gq = opt(dq), gk = opt(dk), gv = opt(dv);
+    const px_rows rq = rows_of(q), rk = rows_of(k), rv = rows_of(v), ro = rows_of(o), rr = rows_of(saved[7]), rg = rows_of(dout), gq = opt(dq), gk = opt(dk), gv = opt(dv);
     const cudaStream_t st = at::cuda::getCurrentCUDAStream();
     launch("px_window_bwd", st, [&] {
-      return abi.px_window_bwd(&w, &rq, &rk, &rv, &ro, &rg, (const float*)lse.data_ptr(), dq.defined() ? &gq : nullptr,
+      return abi.px_window_bwd(&w, &rq, &rk, &rv, &ro, &rr, &rg, (const float*)lse.data_ptr(), dq.defined() ? &gq : nullptr,
                                dk.defined() ? &gk : nullptr, dv.defined() ? &gv : nullptr, dbias.defined() ? dbias.data_ptr() : nullptr,
                                ws.data_ptr(), bytes, st);
     });
@@ -307,7 +308,7 @@ Tensor window_attention(const Tensor& q, const Tensor& k, const Tensor& v, int64
     o = WindowFunction::apply(q4, k4, v4, bias, m, left, right, sinks, scale);
   } else {
     const Tensor b = has(bias) ? bias->contiguous() : Tensor();
-    o = window_forward(rows_fitted(q4), rows_fitted(k4), rows_fitted(v4), b, m.has_value() ? *m : Tensor(), {left, right, sinks, scale}, nullptr);
+    o = window_forward(rows_fitted(q4), rows_fitted(k4), rows_fitted(v4), b, m.has_value() ? *m : Tensor(), {left, right, sinks, scale}, nullptr, nullptr);
   }
   return q.dim() == 4 ? o : o.reshape(q.sizes());
 }

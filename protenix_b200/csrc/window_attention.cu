@@ -50,7 +50,7 @@ struct WindowFwdLayout {
 template <bool kF16, int kD>
 __global__ void __launch_bounds__(kWFwdThreads, WindowFwdLayout<kD>::ctas)
 window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                  const WindowArgs a, const RowsOut o, float* __restrict__ nlse) {
+                  const WindowArgs a, const RowsOut o, const RowsOut rest, float* __restrict__ nlse) {
   typedef WindowFwdLayout<kD> L;
   constexpr uint32_t kCols = L::cols;
   constexpr int kPanels = L::panels, kKT = L::keys, kBlocks = kKT / 32;
@@ -278,14 +278,14 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       const float denominator = both.x + both.y;
       const bool empty = m == -CUDART_INF_F;
       const float inv = empty ? 0.f : 1.f / denominator;
-      uint16_t* const out = o.at(batch, head, i);
+      uint16_t *const out = o.at(batch, head, i), *const more = rest.data ? rest.at(batch, head, i) : nullptr;
       for (int c = 0; c < a.d; c += 16) {
         uint32_t x[16];
         tmem_ld16(t_o + c, x);
         tmem_wait_ld();
         if (i < a.n) {
-          store8<kF16>(out + c, x, inv);
-          if (c + 8 < a.d) store8<kF16>(out + c + 8, x + 8, inv);
+          store8<kF16>(out + c, more ? more + c : nullptr, x, inv);
+          if (c + 8 < a.d) store8<kF16>(out + c + 8, more ? more + c + 8 : nullptr, x + 8, inv);
         }
       }
       // Rows that see nothing, and those beyond the last, have weights of zero in the backward pass.
@@ -351,14 +351,14 @@ static WindowArgs window_args(const px_window& w) {
 
 template <bool kF16, int kD>
 static bool launch_window_fwd(const px_window& w, const px_rows& q, const px_rows& k, const px_rows& v, const WindowArgs& a, const RowsOut& o,
-                              float* lse, cudaStream_t st) {
+                              const RowsOut& rest, float* lse, cudaStream_t st) {
   typedef WindowFwdLayout<kD> L;
   CUtensorMap mq, mk, mv;
   if (!rows_map(&mq, q, w, w.heads) || !rows_map(&mk, k, w, w.kv_heads) || !rows_map(&mv, v, w, w.kv_heads)) return false;
   static SmemLimit limit;
   if (!limit.set(window_fwd_kernel<kF16, kD>, L::bytes(kWMaxR) + 1024)) return false;
   return launch_pdl(window_fwd_kernel<kF16, kD>, dim3((unsigned)((int64_t)a.tiles * w.heads * w.batch)), kWFwdThreads, (size_t)L::bytes(a.r) + 1024,
-                    st, mq, mk, mv, a, o, lse);
+                    st, mq, mk, mv, a, o, rest, lse);
 }
 
 }  // namespace px
@@ -367,19 +367,20 @@ using namespace px;
 
 extern "C" int64_t px_window_lse_floats(int64_t batch, int64_t heads, int64_t n) { return batch * heads * ((n + kWRows - 1) / kWRows * kWRows); }
 
-extern "C" int32_t px_window_fwd(const px_window* w, const px_rows* q, const px_rows* k, const px_rows* v, const px_rows* o, float* lse,
-                                 void* stream) {
+extern "C" int32_t px_window_fwd(const px_window* w, const px_rows* q, const px_rows* k, const px_rows* v, const px_rows* o, const px_rows* o_rest,
+                                 float* lse, void* stream) {
   const int32_t status = window_check(w);
   if (status != PX_OK) return status;
   if (w->batch == 0 || w->n == 0) return PX_OK;
-  if (!rows_fit(q, *w, w->heads) || !rows_fit(k, *w, w->kv_heads) || !rows_fit(v, *w, w->kv_heads) || !rows_fit(o, *w, w->heads))
+  if (!rows_fit(q, *w, w->heads) || !rows_fit(k, *w, w->kv_heads) || !rows_fit(v, *w, w->kv_heads) || !rows_fit(o, *w, w->heads) ||
+      (o_rest && !rows_fit(o_rest, *w, w->heads)))
     return PX_ERR_BAD_ARG;
   if (!have_context()) return PX_ERR_LAUNCH;
   const auto go = w->dtype == PX_F16 ? (w->d <= 32 ? launch_window_fwd<true, 32> : w->d <= 64 ? launch_window_fwd<true, 64> : launch_window_fwd<true, 128>)
                                      : (w->d <= 32   ? launch_window_fwd<false, 32>
                                         : w->d <= 64 ? launch_window_fwd<false, 64>
                                                      : launch_window_fwd<false, 128>);
-  return go(*w, *q, *k, *v, window_args(*w), rows_out(o), lse, (cudaStream_t)stream) ? PX_OK : PX_ERR_LAUNCH;
+  return go(*w, *q, *k, *v, window_args(*w), rows_out(o), rows_out(o_rest), lse, (cudaStream_t)stream) ? PX_OK : PX_ERR_LAUNCH;
 }
 
 namespace px {
@@ -412,13 +413,13 @@ static WindowSpace window_space(const px_window& w, const WindowArgs& a, bool bi
 
 template <bool kF16, int kD, bool kBiasGrad>
 static bool launch_window_dq(const CUtensorMap* m, const WindowArgs& a, const WindowBwdArgs& g, const RowsOut& dout, const RowsOut& o,
-                             const RowsOut& dq, int64_t blocks, cudaStream_t st) {
+                             const RowsOut& rest, const RowsOut& dq, int64_t blocks, cudaStream_t st) {
   typedef WindowDqLayout<kD> L;
   static SmemLimit limit;
   const auto kernel = window_dq_kernel<kF16, kD, kBiasGrad>;
   if (!limit.set(kernel, L::bytes(kWMaxR, kBiasGrad) + 1024)) return false;
   return launch_pdl(kernel, dim3((unsigned)blocks), kWDqThreads, (size_t)L::bytes(a.r, kBiasGrad) + 1024, st, m[0], m[1], m[2], m[3], a, g, dout, o,
-                    dq);
+                    rest, dq);
 }
 template <bool kF16, int kD>
 static bool launch_window_dkv(const CUtensorMap* m, const WindowArgs& a, const WindowBwdArgs& g, const RowsOut& dk, const RowsOut& dv, int64_t blocks,
@@ -431,19 +432,19 @@ static bool launch_window_dkv(const CUtensorMap* m, const WindowArgs& a, const W
 }
 
 struct BwdRows {
-  const px_rows *q, *k, *v, *o, *dout, *dq, *dk, *dv;
+  const px_rows *q, *k, *v, *o, *o_rest, *dout, *dq, *dk, *dv;
 };
 template <bool kF16>
 static bool window_bwd(const px_window& w, const BwdRows& x, const WindowArgs& a, const WindowBwdArgs& g, void* dbias, cudaStream_t st) {
   const int64_t blocks = (int64_t)a.tiles * w.heads * w.batch;
-  const RowsOut dout = rows_out(x.dout), o = rows_out(x.o), dq = rows_out(x.dq), dk = rows_out(x.dk), dv = rows_out(x.dv);
+  const RowsOut dout = rows_out(x.dout), o = rows_out(x.o), rest = rows_out(x.o_rest), dq = rows_out(x.dq), dk = rows_out(x.dk), dv = rows_out(x.dv);
   CUtensorMap m[4];
   if (!rows_map(&m[0], *x.q, w, w.heads) || !rows_map(&m[1], *x.dout, w, w.heads) || !rows_map(&m[2], *x.k, w, w.kv_heads) ||
       !rows_map(&m[3], *x.v, w, w.kv_heads))
     return false;
   const auto go_q = w.d <= 64 ? (dbias ? launch_window_dq<kF16, 64, true> : launch_window_dq<kF16, 64, false>)
                               : (dbias ? launch_window_dq<kF16, 128, true> : launch_window_dq<kF16, 128, false>);
-  if (!go_q(m, a, g, dout, o, dq, blocks, st)) return false;
+  if (!go_q(m, a, g, dout, o, rest, dq, blocks, st)) return false;
   const int64_t own = dk.data || dv.data ? (int64_t)(a.tiles + g.sink_tiles * g.chunks) * w.kv_heads * w.batch : 0;
   const int64_t buckets = dbias ? (int64_t)w.heads * g.bias_blocks : 0;      // these come first: short, and there is room beside them
   if (own + buckets == 0) return true;
@@ -458,8 +459,8 @@ extern "C" int64_t px_window_workspace_bytes(const px_window* w, int32_t bias_gr
   return window_space(*w, window_args(*w), bias_grad && w->r_max >= 0).total;
 }
 
-extern "C" int32_t px_window_bwd(const px_window* w, const px_rows* q, const px_rows* k, const px_rows* v, const px_rows* o, const px_rows* dout,
-                                 const float* lse, const px_rows* dq, const px_rows* dk, const px_rows* dv, void* dbias, void* workspace,
+extern "C" int32_t px_window_bwd(const px_window* w, const px_rows* q, const px_rows* k, const px_rows* v, const px_rows* o, const px_rows* o_rest,
+                                 const px_rows* dout, const float* lse, const px_rows* dq, const px_rows* dk, const px_rows* dv, void* dbias, void* workspace,
                                  int64_t workspace_bytes, void* stream) {
   const int32_t status = window_check(w);
   if (status != PX_OK) return status;
@@ -470,7 +471,7 @@ extern "C" int32_t px_window_bwd(const px_window* w, const px_rows* q, const px_
     return cudaMemsetAsync(dbias, 0, bytes, st) == cudaSuccess ? PX_OK : PX_ERR_LAUNCH;
   }
   if (!rows_fit(q, *w, w->heads) || !rows_fit(k, *w, w->kv_heads) || !rows_fit(v, *w, w->kv_heads) || !rows_fit(o, *w, w->heads) ||
-      !rows_fit(dout, *w, w->heads) || (dq && !rows_fit(dq, *w, w->heads)) || (dk && !rows_fit(dk, *w, w->kv_heads)) ||
+      (o_rest && !rows_fit(o_rest, *w, w->heads)) || !rows_fit(dout, *w, w->heads) || (dq && !rows_fit(dq, *w, w->heads)) || (dk && !rows_fit(dk, *w, w->kv_heads)) ||
       (dv && !rows_fit(dv, *w, w->kv_heads)) || !lse || ((uintptr_t)lse & 15) || !workspace || ((uintptr_t)workspace & 255) ||
       (dbias && w->r_max < 0))
     return PX_ERR_BAD_ARG;
@@ -491,6 +492,6 @@ extern "C" int32_t px_window_bwd(const px_window* w, const px_rows* q, const px_
   g.scale = w->scale;
   sink_chunks(a, &g.sink_tiles, &g.chunks, &g.chunk);
   if ((int64_t)(a.tiles + g.sink_tiles * g.chunks) * w->kv_heads * w->batch > 0x3fffffffll) return PX_ERR_UNSUPPORTED;
-  const BwdRows rows = {q, k, v, o, dout, dq, dk, dv};
+  const BwdRows rows = {q, k, v, o, o_rest, dout, dq, dk, dv};
   return (w->dtype == PX_F16 ? window_bwd<true>(*w, rows, a, g, dbias, st) : window_bwd<false>(*w, rows, a, g, dbias, st)) ? PX_OK : PX_ERR_LAUNCH;
 }

@@ -332,7 +332,7 @@ def test_status_codes_of_the_c_interface():
 
     def fwd(q=Rows(at, 1280, 320, 32), **kw):
         w, x = Window(**{**good, **kw}), Rows(at, 1280, 320, 32)
-        return lib.px_window_fwd(ref(w), ref(q), ref(x), ref(x), ref(x), None, None)
+        return lib.px_window_fwd(ref(w), ref(q), ref(x), ref(x), ref(x), None, None, None)
 
     assert fwd(n=0) == 0 and fwd(batch=0) == 0
     for kw in ({"kv_heads": 3}, {"left": -1}, {"d": 0}, {"scale": 0.0}, {"scale": float("nan")}, {"r_max": 2}, {"heads": 0}):
@@ -345,5 +345,5 @@ def test_status_codes_of_the_c_interface():
     size = lib.px_window_workspace_bytes(ref(w), 0)
     assert size >= 4 * 128 * 4 and lib.px_window_workspace_bytes(ref(Window(**{**good, "d": 12})), 0) == 0
     work = at // 256 * 256 + 256      # never touched: only its alignment is looked at
-    bwd = lambda bytes_, lse=at, dbias=None: lib.px_window_bwd(ref(w), ref(x), ref(x), ref(x), ref(x), ref(x), lse, ref(x), ref(x), ref(x), dbias, work, bytes_, None)
+    bwd = lambda bytes_, lse=at, dbias=None: lib.px_window_bwd(ref(w), ref(x), ref(x), ref(x), ref(x), None, ref(x), lse, ref(x), ref(x), ref(x), dbias, work, bytes_, None)
     assert bwd(size - 1) == -4 and bwd(size, lse=None) == -1 and bwd(size, dbias=at) == -1
