@@ -92,7 +92,8 @@ window_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   if (blockIdx.x == 0 && warp == 8)      // for window_dkv_kernel, which runs behind this one
     for (int k = lane; k < g.batches * a.kv_heads * g.sink_tiles; k += 32) g.arrived[k] = 0u;
 
-  float low = 0.f, high = 0.f;                     // sums of dS over offsets that are clipped
+  // Sums of this thread's dS over offsets that are clipped and over the others, and of its P over the clipped ones.
+  float low = 0.f, high = 0.f, inner = 0.f, p_low = 0.f, p_high = 0.f;
   if (warp == 8) {
     // ------------------------------------------------------------------ copies and products
     const int kv = head / a.group;
@@ -238,13 +239,17 @@ window_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         }
 #pragma unroll
         for (int c = 0; c < 32; c += 2) {
-          const float2 x = apart2(mul2(add2(pair2(d[c], d[c + 1]), ndelta2), pair2(fast_exp2(s[c]), fast_exp2(s[c + 1]))));
+          s[c] = fast_exp2(s[c]), s[c + 1] = fast_exp2(s[c + 1]);
+          const float2 x = apart2(mul2(add2(pair2(d[c], d[c + 1]), ndelta2), pair2(s[c], s[c + 1])));
           d[c] = x.x, d[c + 1] = x.y;
         }
         if (keys != 0xffffffffu || !block_whole(a, qw, kh)) {
           const uint32_t seen = visible_bits(a, i, kh, keys);
 #pragma unroll
-          for (int c = 0; c < 32; ++c) d[c] = (seen >> c & 1u) ? d[c] : 0.f;
+          for (int c = 0; c < 32; ++c) {
+            d[c] = (seen >> c & 1u) ? d[c] : 0.f;
+            if (kBiasGrad) s[c] = (seen >> c & 1u) ? s[c] : 0.f;
+          }
         }
 #pragma unroll
         for (int e = 0; e < 16; ++e) w[e] = pack16x2<kF16>(d[2 * e], d[2 * e + 1]);
@@ -270,7 +275,12 @@ window_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars.given);
       if (kBiasGrad && !dead) {
+        f32x2 v = pair2(0.f, 0.f);
+#pragma unroll
+        for (int c = 0; c < 32; c += 2) v = add2(v, pair2(d[c], d[c + 1]));
+        const float2 x = apart2(v);
         if (near) {
+          inner += x.x + x.y;
           // Sums along the diagonals of a 32 x 32 block, 8 columns at a time (four chains beside one another: a single one waits for its shuffles):
           // the running sum moves one lane on with each column, and leaves by the last lane.
           float run[4] = {0.f, 0.f, 0.f, 0.f};
@@ -292,12 +302,12 @@ window_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             __syncwarp();
           }
         } else {
-          f32x2 v = pair2(0.f, 0.f);
+          f32x2 p = pair2(0.f, 0.f);
 #pragma unroll
-          for (int c = 0; c < 32; c += 2) v = add2(v, pair2(d[c], d[c + 1]));
-          const float2 x = apart2(v);
-          if (is_low) low += x.x + x.y;
-          else high += x.x + x.y;
+          for (int c = 0; c < 32; c += 2) p = add2(p, pair2(s[c], s[c + 1]));
+          const float2 y = apart2(p);
+          if (is_low) low += x.x + x.y, p_low += y.x + y.y;
+          else high += x.x + x.y, p_high += y.x + y.y;
         }
       }
     }
@@ -317,6 +327,13 @@ window_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       }
     }
     if (kBiasGrad) {
+      // dS adds up to zero along a row; what is left is the error of delta, which lies in every dS of the row as P times it.  In the sums over the clipped
+      // offsets, where many keys of a row come together, it is taken out (37 sinks, two other keys: dbias off by 4.2e-3 in bf16 without, 2.9e-3 with it; 2 to 6 % of the kernel).
+      part[half * kWRows + row] = low + high + inner;
+      ok = barrier_all(2 + quarter, 64, ok);
+      const float left_over = part[row] + part[kWRows + row];
+      low = fmaf(-left_over, p_low, low), high = fmaf(-left_over, p_high, high);
+      barrier_of(1, 256);                          // `part` has been read
       low = warp_sum(low);
       high = warp_sum(high);
       if (lane == 0) part[warp] = low, part[8 + warp] = high;
