@@ -8,14 +8,19 @@
 // Two table rows make a pair: bt differs from 2 r + 1 only where bp = r, and the entity's flag follows from bc, so there are
 // 4 r + 3 sums W_pos + W_tok and 2 s + 2 sums W_chain + W_ent (both tables 70 KB of shared memory for r = 32, s = 2 and 128 channels).
 //
-// Forward: memory-bound writer, a warp takes 32 neighbouring pairs of a row; a lane finds one pair's two rows (a code, kept for the
-// backward pass: 4 bytes beside the pair's 256 or 512), then the warp writes pair after pair, 4 channels a lane, and looks the rows up again only
-// where they change (most neighbours are far apart or in another chain: clipped alike).
+// Forward: a warp takes 32 neighbouring pairs of a row; a lane finds one pair's two rows (a code, kept for the backward pass: 4 bytes beside the
+// pair's 256 or 512), then the warp writes pair after pair, 4 channels a lane, and looks the rows up again only where they change (most neighbours are
+// far apart or in another chain: clipped alike).  Memory-bound writer: 1501 tokens x 128 channels in bf16, 104 us for 586 MB = 5.6 TB/s, 86 % of a
+// copy's rate.  Small calls pay for the tables of each CTA: 384 tokens 17.7 us (38 MB), 97 tokens 6 us.
 //
-// Backward: memory-bound reader.  A block (a thread = one channel) reads strips of 32 pairs of a row through a ring of bulk copies and holds
-// sums of its own for every table row in shared memory, so there are no atomics and a call gives the same bits every time.  Neighbours with
-// the same rows are added up in registers; neighbours whose rows all differ, as near the diagonal, go to their sums eight at a time; the rest one by one.
+// Backward: memory-bound reader, two forms.  This one, for fp32 and for tables that the other has no room for: a block (a thread = one channel) reads
+// strips of 32 pairs of a row through a ring of bulk copies and holds sums of its own for every table row in shared memory, so there are no atomics and
+// a call gives the same bits every time.  Neighbours with the same rows are added up in registers; neighbours whose rows all differ, as near the
+// diagonal, go to their sums eight at a time; the rest one by one.  Shared memory's read-add-write of these sums bounds it.
 // The blocks' sums, folded to the columns of W, are added up in their order by a second kernel.
+//
+// What is not finite: a dz of one pair that is infinite or NaN makes its channel NaN in the columns of its own rows here; the form on the tensor cores
+// spreads it over all columns of the channel (0 x inf).
 #include "px_tcgen05.cuh"
 
 namespace px {
@@ -309,8 +314,9 @@ __global__ void __launch_bounds__(kRpBwdThreads, 2) relpos_bwd_kernel(RelposArgs
 
 // The same for 16-bit dz on the tensor cores: the sums by table row are dz^T times the pairs' two-hot rows, M = 128 channels, N = table rows, K = pairs.
 // dz enters as it lies (its channels are the contiguous index: an MN-major operand), the two-hot operand [table row][64 pairs] lives in shared memory and costs
-// a lane two stores a pair to set and two to clear (four warps of them: one took 1100 cycles a tile, where memory takes 700); the products with one are exact.  64 pairs are 288 cycles of the tensor pipe (N = 144), less than half of what
-// their 16 KB take to arrive.  The tensor core truncates when it adds, so an accumulator takes eight tiles (32 additions) before four warps add it, rounding to
+// a lane two stores a pair to set and two to clear (four warps of them: one took 1100 cycles a tile, where memory takes 700); the products with one are exact.
+// 64 pairs are 288 cycles of the tensor pipe (N = 144), less than half of what their 16 KB take to arrive.  Memory bounds it: 1501 tokens x 128
+// channels, 110 us for 577 MB + 9 MB of codes = 5.3 TB/s, 81 % of a copy's rate.  The tensor core truncates when it adds, so an accumulator takes eight tiles (32 additions) before four warps add it, rounding to
 // nearest, to fp32 sums in shared memory, while the next tiles go to the other accumulator.
 // Warps 0..3 drain (a thread = one channel), 4 brings dz, 5 issues the products, 6..9 write the two-hot operands, 32 pairs of every other tile each.
 constexpr int kRpTile = 64, kRpRing = 4, kRpGroup = 8;      // pairs of a tile, tiles on their way, tiles of an accumulator
@@ -473,7 +479,7 @@ __global__ void __launch_bounds__(8 * kRpChunk) relpos_reduce_kernel(const float
 PX_DEFINE_FAMILY_HOOKS(relpos)
 
 static bool relpos_sizes(int64_t batch, int64_t n, int64_t c, int32_t r, int32_t s) {
-  return batch >= 0 && n >= 0 && c > 0 && r >= 0 && s >= 0 && n < (1 << 24) && batch < (1 << 24) && c < (1 << 16);
+  return batch >= 0 && n >= 0 && c > 0 && r >= 0 && s >= 0 && n < (1 << 17) && batch < (1 << 17) && c < (1 << 16);
 }
 static bool relpos_fits(int64_t c, int32_t r, int32_t s) {
   return c % 8 == 0 && r <= kRpMaxRows && s <= kRpMaxRows && 4 * r + 2 * s + 5 <= kRpMaxRows;
@@ -483,7 +489,9 @@ static bool relpos_fits(int64_t c, int32_t r, int32_t s) {
 static int64_t relpos_units(int64_t batch, int64_t n) { return batch * n * ((n + kRpPairs - 1) / kRpPairs); }
 static int64_t relpos_blocks(int64_t units) { return std::max<int64_t>(1, std::min<int64_t>(2 * sm_count(), units / 16)); }
 
-// 16-bit gradients with tables that fit.
+// 16-bit gradients with tables that fit, at every size: on the tensor cores / one by one (bf16, 128 channels, r = 32, s = 2), us: 33 tokens 7.6 / 23.3,
+// 97 8.3 / 25.9, 200 8.8 / 22.7, 384 12.1 / 21.1, 600 27.7 / 38.4, 1000 61.6 / 85.1, 1501 110 / 158.  fp32 would need three 16-bit parts of dz, and room
+// for them in shared memory beside the sums.
 static bool relpos_on_tensor_cores(int64_t pairs, int n_cols, int32_t dtype) {
   return dtype != PX_F32 && n_cols <= kRpTcRows && pairs < (int64_t)0x7fffff00;
 }

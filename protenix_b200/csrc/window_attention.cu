@@ -7,17 +7,22 @@
 // group of q's heads each.
 //
 // One CTA = 128 queries of a head, streamed over the 64-key tiles that they see.  Warps 0..3: one thread a query row.  Warp 4
-// loads Q once and K, V tiles by TMA (panels of 64 elements, 128-byte swizzle, a ring of two each) and issues S = Q K^T and,
-// once the rows have put P (16 bits) in S's place in tensor memory, O += P V with V read as it lies, along its rows.
+// loads Q once and K, V tiles by TMA (panels of 64 elements, 128-byte swizzle, a ring of two each) and issues S = Q K^T and, once the rows have left P
+// (16 bits), O += P V with V read as it lies, along its rows.  The next S is made while this one, by then in registers, becomes P.
 // Softmax is online in base 2 with a reference maximum that moves (and O with it) only when a tile exceeds it by more than 8: P is 2^8 at most.
-// Logits, statistics and O are fp32; P is rounded to the type of V, which the product needs (relative error of half a step, 2^-9 or 2^-12,
+// Logits, statistics and O are fp32; P is rounded to the type of V, which the product needs (relative error of half a step, 2^-8 or 2^-11 at most,
 // with either sign); the denominators sum the fp32 values.
 //
-// Tiles that every query sees whole, the larger part of a wide window, take no per-element test; elsewhere a row's visible keys are a 64-bit
-// word.  Where all offsets of a tile are clipped alike the bias is one number, elsewhere it is read from shared memory, where the head's row lies
-// continued beyond its ends, so that a thread's 64 values lie side by side.
+// Blocks of 32 queries x 32 keys out of sight cost nothing but zeros.  Tiles that a warp's rows see whole and with one bias for all, the larger part of a
+// wide window, take a loop of their own without tests; elsewhere a row's visible keys are a word of 32 bits, and where the offsets are not all clipped
+// alike the bias is read from shared memory, where the head's row lies continued beyond its ends, so that a thread's values lie side by side.
 //
-// TMEM: S / P (64 columns) | O.  d <= 64: 128 columns, four CTAs an SM hide one another's chain of product, softmax, product.
+// What bounds it: the chain of a tile in a row's thread (maximum, exponentials, rounding: some 330 instructions where nothing is tested, 2000 cycles beside
+// the other warps), not a unit: at 8192 tokens, 16 heads of 64, causal window of 1024, 88 us (370 TFLOP/s), the special-function unit is busy for a third of the time and
+// the tensor pipe for a fifth; at 16384 tokens, 8 heads of 128, window of 2048, 152 us = 850 TFLOP/s, the tensor pipe for half.  So as many CTAs an SM as tensor
+// memory, shared memory and registers allow: four (heads up to 32), three, two.  Short windows (atoms: four tiles a CTA) pay as much for a CTA's beginning and
+// end.  Built, measured and not kept: 128 keys a tile for heads of 64 (2 % slower), eight warps of rows with 32 keys each (10 to 40 %), copies issued by the row
+// warps (7 %), window and bias in one table with -inf (1 to 8 %).
 #include <type_traits>
 
 #include "px_window.cuh"
@@ -216,10 +221,10 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           continue;
         }
         const float sh = add[kPlain ? 0 : b] + shift;
-        const f32x2 sh2 = pair2(sh, sh), mul2 = kPlain ? scale : mul[b];
+        const f32x2 sh2 = pair2(sh, sh), by2 = kPlain ? scale : mul[b];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const float2 x = apart2(fma2(pair2(s[32 * b + 2 * e], s[32 * b + 2 * e + 1]), mul2, sh2));
+          const float2 x = apart2(fma2(pair2(s[32 * b + 2 * e], s[32 * b + 2 * e + 1]), by2, sh2));
           const float p0 = fast_exp2(x.x), p1 = fast_exp2(x.y);
           sum = add2(sum, pair2(p0, p1));
           w[16 * b + e] = pack16x2<kF16>(p0, p1);
@@ -327,6 +332,7 @@ static int32_t window_check(const px_window* w) {
       w->heads % w->kv_heads != 0 || !(w->scale > 0.f) || !(w->scale <= 3.0e38f))
     return PX_ERR_BAD_ARG;
   if ((w->dtype != PX_BF16 && w->dtype != PX_F16) || w->d % 8 != 0 || w->d > 128 || w->n > (1 << 24) || w->r_max > kWMaxR) return PX_ERR_UNSUPPORTED;
+  if (w->heads / w->kv_heads * (w->n / kWCols + 1) > 0x3fffffffll) return PX_ERR_UNSUPPORTED;
   if (w->batch * w->heads * ((w->n + kWRows - 1) / kWRows) > 0x3fffffffll || w->batch > 65535 || w->heads > 65535) return PX_ERR_UNSUPPORTED;
   if (w->r_max >= 0 && (!w->bias || (w->bias_dtype != PX_F32 && w->bias_dtype != PX_BF16 && w->bias_dtype != PX_F16))) return PX_ERR_BAD_ARG;
   return PX_OK;
@@ -392,6 +398,7 @@ static void sink_chunks(const WindowArgs& a, int* tiles, int* chunks, int* chunk
   *chunk = window > 64 ? window : 64;
   int most = 0;
   if (*tiles > 0) most = ((a.n - 1) / kWCols - last_of_window(a.n, a.left, 0)) * a.group;      // the first tile has the most
+  if (*tiles > 16 && *chunk < (most + 1) / 2) *chunk = (most + 1) / 2;      // CTAs enough, and each chunk takes memory for its sums
   *chunks = most > 0 ? (most + *chunk - 1) / *chunk : 0;
   if (*chunks == 0) *tiles = 0;
 }
