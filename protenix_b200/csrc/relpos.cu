@@ -6,12 +6,13 @@
 // and the gradient of W: sums of dz over the pairs of a bucket.  The one-hot matrix never exists.
 //
 // Two table rows make a pair: bt differs from 2 r + 1 only where bp = r, and the entity's flag follows from bc, so there are
-// 4 r + 3 sums W_pos + W_tok and 2 s + 2 sums W_chain + W_ent (both tables 70 KB of shared memory for r = 32, s = 2 and 128 channels).
+// 4 r + 3 sums W_pos + W_tok and 2 s + 2 sums W_chain + W_ent (both tables 35 KB of shared memory for r = 32, s = 2 and 64 channels).
 //
 // Forward: a warp takes 32 neighbouring pairs of a row; a lane finds one pair's two rows (a code, kept for the backward pass: 4 bytes beside the
-// pair's 256 or 512), then the warp writes pair after pair, 4 channels a lane, and looks the rows up again only where they change (most neighbours are
-// far apart or in another chain: clipped alike).  Memory-bound writer: 1501 tokens x 128 channels in bf16, 104 us for 586 MB = 5.6 TB/s, 86 % of a
-// copy's rate.  Small calls pay for the tables of each CTA: 384 tokens 17.7 us (38 MB), 97 tokens 6 us.
+// pair's 256 or 512), then the warp writes them, a few pairs side by side, 4 channels a lane, and looks the rows up again only where they change (most neighbours are
+// far apart or in another chain: clipped alike).  Memory-bound writer: 1501 tokens x 128 channels in bf16, 91 us for 577 MB = 6.3 TB/s, 97 % of a
+// copy's rate, and up to 104 with the 9 MB of codes between backward passes; 384 tokens in fp32 15.5 us for 76 MB = 4.9 TB/s.  The smallest wait for W, from which every block makes its tables:
+// 97 tokens 5 us for 4.8 MB.  So a block's tables are for 32 or 64 channels.
 //
 // Backward: memory-bound reader, two forms.  This one, for fp32 and for tables that the other has no room for: a block (a thread = one channel) reads
 // strips of 32 pairs of a row through a ring of bulk copies and holds sums of its own for every table row in shared memory, so there are no atomics and
@@ -25,7 +26,7 @@
 
 namespace px {
 
-constexpr int kRpChunk = 128;           // channels a block handles
+constexpr int kRpChunk = 128;           // channels a block of the backward pass handles
 constexpr int kRpMaxRows = 380;         // rows of both tables together: what shared memory holds beside the backward pass's ring
 constexpr int kRpPairs = 32;            // pairs of a warp's step, and of a backward stage of 16-bit values
 constexpr int kRpStages = 4;
@@ -70,67 +71,80 @@ __device__ __forceinline__ void store4<__half>(__half* p, float4 v) {
 
 constexpr int kRpFwdThreads = 1024;      // one block an SM
 
-// codes: what the backward pass reads, one a pair, or NULL.  slice: channels of W that are
+// kW: channels of a block, whose table is made for all of them.  codes: what the backward pass reads, one a pair, or NULL.  slice: channels of W that are
 // brought into shared memory at a time, all of them unless the tables are large.
-template <typename T>
+template <typename T, int kW>
 __global__ void __launch_bounds__(kRpFwdThreads) relpos_fwd_kernel(RelposArgs a, const float* __restrict__ w, T* __restrict__ z,
                                                                    uint32_t* __restrict__ codes, int slice) {
+  constexpr int kLanes = kW / 4, kSide = 32 / kLanes;                   // lanes of a pair, pairs side by side in a warp
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   __shared__ uint64_t full;
-  const int c0 = blockIdx.y * kRpChunk, channels = min(kRpChunk, a.c - c0), t = a.columns();
+  const int c0 = blockIdx.y * kW, channels = min(kW, a.c - c0), t = a.columns();
   const int rows1 = a.rows1(), rows = rows1 + a.rows2(), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int tok = 2 * a.r + 2, ent = 4 * a.r + 4, chain = ent + 1;      // first columns of the parts of W behind the first
-  float* const table = reinterpret_cast<float*>(smem_raw);              // [rows][kRpChunk]
-  float* const part = table + rows * kRpChunk;                          // [slice][t]
+  float* const table = reinterpret_cast<float*>(smem_raw);              // [rows][kW]
+  float* const part = table + rows * kW;                                // [slice][t]
   if (threadIdx.x == 0) {
     mbar_init(&full, 1);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    const int count = min(slice, channels);
+    mbar_expect_tx(&full, (uint32_t)(count * t * 4));
+    bulk_load(part, w + (long long)c0 * t, (uint32_t)(count * t * 4), &full);
   }
+  const int strips = (int)((a.n + kRpPairs - 1) / kRpPairs);
+  const long long units = a.pairs / a.n * strips, warps = (long long)gridDim.x * (kRpFwdThreads / 32);
+  long long u = (long long)warp * gridDim.x + blockIdx.x;               // the blocks have equal shares, however few units there are
+  const auto code_of = [&](long long unit) {                            // of this lane's pair
+    const long long i = unit / strips;                                  // counts the rows of all batches
+    const int j = (int)(unit - i * strips) * kRpPairs + lane;
+    return relpos_code(a, i, i / a.n * a.n + min((long long)j, a.n - 1));
+  };
+  uint32_t code = u < units ? code_of(u) : 0u;                          // asked for while W is on its way
   __syncthreads();
   bool ok = true;
   for (int s0 = 0, k = 0; s0 < channels; s0 += slice, ++k) {
     const int count = min(slice, channels - s0);
-    if (threadIdx.x == 0) {
+    if (s0 > 0 && threadIdx.x == 0) {
       mbar_expect_tx(&full, (uint32_t)(count * t * 4));
       bulk_load(part, w + (long long)(c0 + s0) * t, (uint32_t)(count * t * 4), &full);
     }
     ok = mbar_wait(&full, k & 1, 2u) && ok;
     // A lane = a channel: t is odd, so neither side of this transposition meets a bank twice.
-    for (int u = threadIdx.x; u < rows * kRpChunk; u += kRpFwdThreads) {
-      const int ch = u % kRpChunk, row = u / kRpChunk;
+    for (int v = threadIdx.x; v < rows * kW; v += kRpFwdThreads) {
+      const int ch = v % kW, row = v / kW;
       if (ch < count) {
         const float* const f = part + ch * t;
-        const float v = row < tok     ? f[row] + f[tok + 2 * a.r + 1]
+        const float x = row < tok     ? f[row] + f[tok + 2 * a.r + 1]
                         : row < rows1 ? f[a.r] + f[row]
                                       : f[chain + row - rows1] + (row - rows1 < 2 * a.s + 1 ? f[ent] : 0.f);
-        table[row * kRpChunk + s0 + ch] = v;
+        table[row * kW + s0 + ch] = x;
       }
     }
     ok = __syncthreads_and(ok) != 0;
   }
   if (!ok) return;
-  const int strips = (int)((a.n + kRpPairs - 1) / kRpPairs);
-  const long long units = a.pairs / a.n * strips, warps = (long long)gridDim.x * (kRpFwdThreads / 32);
-  const bool mine = 4 * lane < channels;
-  for (long long u = (long long)warp * gridDim.x + blockIdx.x; u < units; u += warps) {      // the blocks have equal shares, however few units there are
-    const long long i = u / strips;                                      // counts the rows of all batches
+  const int at = 4 * (lane % kLanes), side = lane / kLanes;
+  const bool mine = at < channels;
+  while (u < units) {
+    const long long i = u / strips;
     const int j0 = (int)(u - i * strips) * kRpPairs, count = (int)min((long long)kRpPairs, a.n - j0);
-    const uint32_t code = relpos_code(a, i, i / a.n * a.n + j0 + min(lane, count - 1));
     if (codes && blockIdx.y == 0 && lane < count) codes[i * a.n + j0 + lane] = code;
-    T* out = z + (i * a.n + j0) * a.c + c0 + 4 * lane;
+    T* out = z + (i * a.n + j0 + side) * a.c + c0 + at;
     uint32_t have = 0xffffffffu;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-    for (int k = 0; k < count; ++k) {
-      const uint32_t now = __shfl_sync(0xffffffffu, code, k);
+    for (int k = 0; k < count; k += kSide) {
+      const uint32_t now = __shfl_sync(0xffffffffu, code, k + side);
       if (now != have) {
         have = now;
-        const float4 p = *reinterpret_cast<const float4*>(table + (now & 0xffffu) * kRpChunk + 4 * lane);
-        const float4 q = *reinterpret_cast<const float4*>(table + (rows1 + (now >> 16)) * kRpChunk + 4 * lane);
+        const float4 p = *reinterpret_cast<const float4*>(table + (now & 0xffffu) * kW + at);
+        const float4 q = *reinterpret_cast<const float4*>(table + (rows1 + (now >> 16)) * kW + at);
         v = make_float4(p.x + q.x, p.y + q.y, p.z + q.z, p.w + q.w);
       }
-      if (mine) store4(out + (long long)k * a.c, v);
+      if (mine && k + side < count) store4(out + (long long)k * a.c, v);
     }
+    u += warps;
+    if (u < units) code = code_of(u);
   }
 }
 
@@ -484,10 +498,17 @@ static bool relpos_sizes(int64_t batch, int64_t n, int64_t c, int32_t r, int32_t
 static bool relpos_fits(int64_t c, int32_t r, int32_t s) {
   return c % 8 == 0 && r <= kRpMaxRows && s <= kRpMaxRows && 4 * r + 2 * s + 5 <= kRpMaxRows;
 }
-// Backward pass: units (strips of 32 pairs of a row), and blocks: two an SM, and no more than leave each some units, since each brings
-// sums of its own.
+// Backward pass: units (strips of 32 pairs of a row), and blocks: two an SM, and no more than leave each two units, since each brings sums of its own
+// (16 units and 2, both kernels, us: 33 tokens in fp32 32.2 / 10.8, 97 35.1 / 13.2, 200 31.9 / 18.3; bf16, 33 9.8 / 9.2, 97 11.1 / 10.5, 200 11.9 / 12.3).
 static int64_t relpos_units(int64_t batch, int64_t n) { return batch * n * ((n + kRpPairs - 1) / kRpPairs); }
-static int64_t relpos_blocks(int64_t units) { return std::max<int64_t>(1, std::min<int64_t>(2 * sm_count(), units / 16)); }
+static int64_t relpos_blocks(int64_t units) { return std::max<int64_t>(1, std::min<int64_t>(2 * sm_count(), units / 2)); }
+
+// Forward, channels of a block: 32 while each of its warps has one strip at most, for then the tables are what it waits for; otherwise 64.  With 32 / 64 / 128
+// channels (128 in all, r = 32, s = 2), us: 97 tokens in fp32 5.0 / 6.1 / 8.8; 150 5.9 / 6.5 / 8.9; 200 8.2 / 7.7 / 9.5; 384 15.1 / 15.8 / 17.6;
+// 1501 196 / 187 / 193; bf16, 200 7.3 / 6.6 / 9.1; 600 23.7 / 19.5 / 22.0; 1501 117 / 91 / 98.  (Two blocks an SM are slower at every size: 97 tokens 8.4.)
+static bool relpos_narrow(int64_t batch, int64_t n, int64_t c) {
+  return relpos_units(batch, n) <= kRpFwdThreads / 32 * std::max<int64_t>(sm_count() / ((c + 31) / 32), 1);
+}
 
 // 16-bit gradients with tables that fit, at every size: on the tensor cores / one by one (bf16, 128 channels, r = 32, s = 2), us: 33 tokens 7.6 / 23.3,
 // 97 8.3 / 25.9, 200 8.8 / 22.7, 384 12.1 / 21.1, 600 27.7 / 38.4, 1000 61.6 / 85.1, 1501 110 / 158.  fp32 would need three 16-bit parts of dz, and room
@@ -519,20 +540,23 @@ extern "C" int32_t px_relpos_fwd(const int64_t* asym_id, const int64_t* residue_
   if (!asym_id || !residue_index || !entity_id || !token_index || !sym_id || !w || !z || (((uintptr_t)z | (uintptr_t)w) & 15)) return PX_ERR_BAD_ARG;
   const RelposArgs a = {(const long long*)asym_id, (const long long*)residue_index, (const long long*)entity_id, (const long long*)token_index,
                         (const long long*)sym_id, n, batch * n * n, (int)c, r_max, s_max};
-  constexpr size_t kRoom = (size_t)226 << 10;
-  const size_t table = (size_t)(a.rows1() + a.rows2()) * kRpChunk * 4, row = (size_t)a.columns() * 4;
-  const int slice = (int)std::min<size_t>(kRpChunk, (kRoom - table) / row / 8 * 8);      // at least 8: see kRpMaxRows
-  // a few strips a block at least, one block an SM at most
-  const dim3 grid((unsigned)std::min<int64_t>((relpos_units(batch, n) + 3) / 4, sm_count()), (unsigned)((c + kRpChunk - 1) / kRpChunk));
-  static SmemLimit limit[3];
-  const auto go = [&](auto* kernel, auto* out) {
-    if (!limit[dtype].set(kernel, kRoom)) return false;
+  const auto go = [&](auto* kernel, auto* out, int width, SmemLimit& limit) {
+    constexpr size_t kRoom = (size_t)226 << 10;
+    const size_t table = (size_t)(a.rows1() + a.rows2()) * width * 4, row = (size_t)a.columns() * 4;
+    const int slice = (int)std::min<size_t>(width, (kRoom - table) / row / 8 * 8);      // at least 8: see kRpMaxRows
+    // a few strips a block at least, one block an SM at most
+    const int64_t parts = (c + width - 1) / width;
+    const dim3 grid((unsigned)std::min<int64_t>((relpos_units(batch, n) + 3) / 4, std::max<int64_t>(sm_count() / parts, 1)), (unsigned)parts);
+    if (!limit.set(kernel, kRoom)) return false;
     kernel<<<grid, kRpFwdThreads, table + slice * row, (cudaStream_t)stream>>>(a, w, out, codes, slice);
     return cudaGetLastError() == cudaSuccess;
   };
-  const bool done = dtype == PX_F32    ? go(relpos_fwd_kernel<float>, (float*)z)
-                    : dtype == PX_BF16 ? go(relpos_fwd_kernel<bf16>, (bf16*)z)
-                                       : go(relpos_fwd_kernel<__half>, (__half*)z);
+  static SmemLimit limits[2][3];
+  const auto as = [&](auto* out) {
+    typedef std::remove_pointer_t<decltype(out)> T;
+    return relpos_narrow(batch, n, c) ? go(relpos_fwd_kernel<T, 32>, out, 32, limits[0][dtype]) : go(relpos_fwd_kernel<T, 64>, out, 64, limits[1][dtype]);
+  };
+  const bool done = dtype == PX_F32 ? as((float*)z) : dtype == PX_BF16 ? as((bf16*)z) : as((__half*)z);
   return done ? PX_OK : PX_ERR_LAUNCH;
 }
 
