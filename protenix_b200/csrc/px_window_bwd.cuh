@@ -12,8 +12,8 @@
 // they enter and stay fp32 in the bias's gradient.
 //
 // What bounds them is, as forward, what the warps issue for a tile (exponentials, products, rounding, the bias's sums), with 16 warps an SM, as many as
-// tensor memory allows.  At 8192 tokens, 16 heads of 64 over 4 of keys, causal window of 1024: 125 us and 168 (three products and four of 16 GFLOP each:
-// 390 and 380 TFLOP/s).  Atoms, five samples of 3987 with 4 heads of 32, windows of 128, a bias by offset: 35 us and 29.
+// tensor memory allows.  At 8192 tokens, 16 heads of 64 over 4 of keys, causal window of 1024: 125 us and 156 (three products and four of 16 GFLOP each:
+// 390 and 410 TFLOP/s).  Atoms, five samples of 3987 with 4 heads of 32, windows of 128, a bias by offset: 35 us and 29.
 //
 // Keys that are sinks are seen by all later queries.  Their CTA takes the queries of the window, like any other; the
 // queries beyond are cut into chunks of about as many tiles, a CTA each, and the last of these CTAs adds the chunks up in their order.
@@ -578,19 +578,18 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     // blocks of queries from qh on that see all of this warp's keys, and those whose bias is the first or the last entry for all
     const int whole_from = any_masked ? 0x3fffffff : kw + 31 - a.right, whole_to = min(kw + 32 <= a.sinks ? a.n : kw - 31 + a.left, a.n - 32);
     const int low_from = kw + 31 + a.r, high_to = kw - 31 - a.r;
-    bool ok = true;
+    bool ok = true;                                // of the warp: one whose wait ran out goes on to the barriers alone
     int filled = -1;                               // the group's head whose bias is in shared memory
-    const bool wide = a.r >= 0 && a.group > 1;     // the bias changes on the way: all eight warps keep together
     QueryItem now(tiles);
     for (int t = 0; t < tiles.count; ++t, now.next(tiles)) {
       const int qh = (tiles.first + now.tile) * kWCols + 32 * half, s = t % kStages;
       if (a.r >= 0 && now.member != filled) {
-        // all are past the tile before (barrier below), but not all are through with it
-        barrier_of(1, 256);
+        barrier_of(1, 256);                        // all are through with the tile before
         bias_fill(a, kv * a.group + now.member, bias, 256);
         barrier_of(1, 256);
         filled = now.member;
       }
+      if (!ok) continue;
       const bool dead = qh >= a.n || block_dead(a, qh, kw);
       ok = mbar_wait(&bars.ready, t & 1, 32u);
       // the statistics came with the operands; this wait only makes the copy's writes visible here
@@ -626,7 +625,7 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         }
         if (h == 1) {
           tc_fence_before();
-          ok = wide ? barrier_all(1, 256, ok) : __all_sync(0xffffffffu, ok) != 0;
+          ok = __all_sync(0xffffffffu, ok) != 0;
           if (!ok) break;
           if (lane == 0) mbar_arrive(&bars.taken);
         }
@@ -680,7 +679,7 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           }
         }
       }
-      if (!ok) break;
+      if (!ok) continue;
       if (nothing) {                                // whatever their rows of Q and dO hold becomes zeros; those of this half by its four warps
         if (nothing >> lane & 1u) {
           clear_row<kPanels, kWCols>(sm + L::q + s * L::tile, 32 * half + lane, quarter, 4);
@@ -689,8 +688,8 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       }
       if (t > 0) {                                  // the products before have read their P^T and dS^T
         ok = mbar_wait(&bars.done, (t - 1) & 1, 64u);
-        ok = wide ? barrier_all(1, 256, ok) : __all_sync(0xffffffffu, ok) != 0;
-        if (!ok) break;
+        ok = __all_sync(0xffffffffu, ok) != 0;
+        if (!ok) continue;
       }
       tc_fence_after();
       if (L::p_shared) {
