@@ -1,10 +1,14 @@
 // Gradients of windowed attention (part of window_attention.cu).  With P recomputed from the forward pass's lse:
 //   dV = P^T dO;  dP = dO V^T;  delta_i = dO_i . O_i;  dS = P (dP - delta);  dQ = scale dS K;  dK = scale dS^T Q;
 //   dbias[head][b] = sum of dS over the pairs of bucket b.
-// Two kernels of one form, each with its own rows in shared memory and a loop over streamed tiles of 64, so that every sum has one owner and a
-// fixed order (no atomics): window_dq_kernel owns 128 queries and streams keys; it also sums delta (and leaves it for the other) and the bias's
-// gradient.  window_dkv_kernel owns 128 keys and streams the queries that see them, those of all heads of the group one after the other.
-// The price is S and dP twice: seven products a tile pair in place of five.
+// A small kernel for delta, then two of one form, each with its own rows in shared memory and a loop over streamed tiles of 64, so that every sum has one
+// owner and a fixed order (no atomics): window_dq_kernel owns 128 queries and streams keys; it also sums the bias's gradient. window_dkv_kernel owns 128 keys
+// and streams the queries that see them, those of all heads of the group one after the other.  The price is S and dP twice: seven products a tile
+// pair in place of five.
+//
+// The two are independent but for the sums of the bias, so the second lets its blocks in as soon as the last of the first's has begun: window_dq_kernel
+// signals its dependents once its wait for window_delta_kernel is over, and a block of window_dkv_kernel waits for that grid only at its end (or, where it adds
+// the bias's sums up, before it begins).  Neither fills a whole number of rounds over the SMs, and now they share the rest.
 //
 // Eight compute warps, a thread = one row x 32 of the 64 columns (no reduction along a row is needed here).  Copies and products have one warp in the first
 // kernel and two in the second, whose four products a step take an issuing warp some 1000 cycles beside busy ones (177 -> 168 us for a causal window
@@ -37,7 +41,44 @@ struct WindowBwdArgs {
   float scale;
   int sink_tiles, chunks, chunk; // chunk: streamed tiles of one
   int bias_blocks, batches;      // blocks of 32 buckets a head
+  bool own, early;               // dK or dV is wanted; window_dkv_kernel begins beside window_dq_kernel
 };
+
+// -delta = -dO . O, O with what its rounding has taken off: a group of lanes a row, a lane = 16 bytes; zeros beyond the last row.  Memory-bound.
+__host__ __device__ constexpr int delta_rows(int lanes) { return lanes == 4 ? 2 : 4; }                      // of a group
+__host__ __device__ constexpr int delta_block(int lanes) { return 256 / lanes * delta_rows(lanes); }     // of a block: 128 or 64, which divide npad
+template <bool kF16, int kLanes>
+__global__ void __launch_bounds__(256) window_delta_kernel(const WindowArgs a, const WindowBwdArgs g, const RowsOut dout, const RowsOut o, const RowsOut rest) {
+  pdl_wait();
+  if (blockIdx.x == 0)      // for window_dkv_kernel
+    for (int k = threadIdx.x; k < g.batches * a.kv_heads * g.sink_tiles; k += 256) g.arrived[k] = 0u;
+  constexpr int kRows = delta_rows(kLanes);
+  const int lane = threadIdx.x % kLanes, c = 8 * lane, blocks = a.npad / delta_block(kLanes), bh = blockIdx.x / blocks, head = bh % a.heads, batch = bh / a.heads;
+  const int first = (int)(blockIdx.x % blocks) * delta_block(kLanes) + threadIdx.x / kLanes;
+  uint4 u[kRows], v[kRows], z[kRows];
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    const int i = first + r * (256 / kLanes);
+    const bool there = i < a.n && c < a.d;
+    const uint4 none = make_uint4(0u, 0u, 0u, 0u);
+    u[r] = there ? __ldg(reinterpret_cast<const uint4*>(dout.at(batch, head, i) + c)) : none;
+    v[r] = there ? __ldg(reinterpret_cast<const uint4*>(o.at(batch, head, i) + c)) : none;
+    z[r] = there && rest.data ? __ldg(reinterpret_cast<const uint4*>(rest.at(batch, head, i) + c)) : none;
+  }
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    const uint32_t us[4] = {u[r].x, u[r].y, u[r].z, u[r].w}, vs[4] = {v[r].x, v[r].y, v[r].z, v[r].w}, zs[4] = {z[r].x, z[r].y, z[r].z, z[r].w};
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 p = unpack16x2<kF16>(us[k]), q = unpack16x2<kF16>(vs[k]), x = unpack16x2<kF16>(zs[k]);
+      sum = fmaf(p.x, q.x + x.x, fmaf(p.y, q.y + x.y, sum));
+    }
+#pragma unroll
+    for (int w = kLanes / 2; w > 0; w /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+    if (lane == 0) g.ndelta[(size_t)bh * a.npad + first + r * (256 / kLanes)] = -sum;
+  }
+}
 
 struct WindowBwdBars {
   // streamed operands; S and dP, complete and in registers; P and dS; the products with them
@@ -64,8 +105,7 @@ static_assert(sizeof(WindowBwdBars) <= 128, "room for the barriers");
 template <bool kF16, int kD, bool kBiasGrad>
 __global__ void __launch_bounds__(kWDqThreads, 2)
 window_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do, const __grid_constant__ CUtensorMap map_k,
-                 const __grid_constant__ CUtensorMap map_v, const WindowArgs a, const WindowBwdArgs g, const RowsOut dout, const RowsOut o,
-                 const RowsOut rest, const RowsOut dq) {
+                 const __grid_constant__ CUtensorMap map_v, const WindowArgs a, const WindowBwdArgs g, const RowsOut dq) {
   typedef WindowDqLayout<kD> L;
   constexpr uint32_t kCols = L::cols;
   constexpr int kK = L::k_stages, kV = L::v_stages, kPanels = L::panels;
@@ -92,10 +132,10 @@ window_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   }
   if (warp == 8) tmem_alloc(&bars.tmem_base, kCols);
   if (!cta_ready(skip, warp == 8, bars.tmem_base, kCols)) return;
+  // window_delta_kernel is complete: when all blocks have come this far, those of window_dkv_kernel may begin
+  if (g.early) asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
   const uint32_t tmem = bars.tmem_base;
   const int ext = bias_floats(a.r);
-  if (blockIdx.x == 0 && warp == 8)      // for window_dkv_kernel, which runs behind this one
-    for (int k = lane; k < g.batches * a.kv_heads * g.sink_tiles; k += 32) g.arrived[k] = 0u;
 
   // Sums of this thread's dS over offsets that are clipped and over the others, and of its P over the clipped ones.
   float low = 0.f, high = 0.f, inner = 0.f, p_low = 0.f, p_high = 0.f;
@@ -171,38 +211,13 @@ window_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     // ------------------------------------------------------------------ one query row x 32 keys a thread
     const int quarter = warp & 3, half = warp >> 2, row = 32 * quarter + lane, i = q0 + row, qw = q0 + 32 * quarter;
     const uint32_t t_lane = tmem + ((uint32_t)(32 * quarter) << 16);
-    // All loads of the beginning at once: one after the other they took 4000 cycles, as much as two tiles.  delta = dO . O with what the
-    // rounding of O has taken off, each thread over its half of the 16-byte pieces of the row.
-    const float nlse = g.nlse[(size_t)bh * a.npad + i];
-    uint4 u[kD / 16], v[kD / 16], z[kD / 16];
-    const uint16_t *x = dout.at(batch, head, i), *y = o.at(batch, head, i), *more = rest.data ? rest.at(batch, head, i) : nullptr;
-#pragma unroll
-    for (int e = 0; e < kD / 16; ++e) {
-      const int c = 8 * half + 16 * e;
-      const bool there = i < a.n && c < a.d;
-      u[e] = there ? __ldg(reinterpret_cast<const uint4*>(x + c)) : make_uint4(0u, 0u, 0u, 0u);
-      v[e] = there ? __ldg(reinterpret_cast<const uint4*>(y + c)) : make_uint4(0u, 0u, 0u, 0u);
-      z[e] = there && more ? __ldg(reinterpret_cast<const uint4*>(more + c)) : make_uint4(0u, 0u, 0u, 0u);
-    }
+    const float nlse = g.nlse[(size_t)bh * a.npad + i], ndelta = g.ndelta[(size_t)bh * a.npad + i];
     if (a.r >= 0) {
       bias_fill(a, head, bias, 256);
       if (kBiasGrad)
         for (int k = threadIdx.x; k < 8 * ext; k += 256) bias[ext + k] = 0.f;
     }
-    float sum = 0.f;
-#pragma unroll
-    for (int e = 0; e < kD / 16; ++e) {
-      const uint32_t us[4] = {u[e].x, u[e].y, u[e].z, u[e].w}, vs[4] = {v[e].x, v[e].y, v[e].z, v[e].w}, zs[4] = {z[e].x, z[e].y, z[e].z, z[e].w};
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float2 p = unpack16x2<kF16>(us[k]), q = unpack16x2<kF16>(vs[k]), r = unpack16x2<kF16>(zs[k]);
-        sum = fmaf(p.x, q.x + r.x, fmaf(p.y, q.y + r.y, sum));
-      }
-    }
-    part[half * kWRows + row] = sum;
-    barrier_of(1, 256);
-    const float ndelta = -(part[row] + part[kWRows + row]);
-    if (half == 0) g.ndelta[(size_t)bh * a.npad + i] = ndelta;      // 0 beyond the last row
+    if (a.r >= 0) barrier_of(1, 256);
     float* const sums = bias + ext * (1 + warp);                   // by offset, as the bias lies
     float* const stage = bias + ext * 9 + 32 * warp;
     const f32x2 scale = both2(a.c), ndelta2 = both2(ndelta);
@@ -457,20 +472,23 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   WindowBwdBars& bars = *reinterpret_cast<WindowBwdBars*>(sm + L::bars);
   float* const bias = reinterpret_cast<float*>(sm + L::bias);
   const int warp = warp_index(), lane = threadIdx.x & 31;
-  const int buckets = g.dbias_out ? a.heads * g.bias_blocks : 0;
-  if ((int)blockIdx.x < buckets) {
+  // the chunks of the sinks, which may be the longest, then the key tiles, then the sums of the bias, which need all of window_dq_kernel
+  const int extra = g.sink_tiles * g.chunks, kv_all = a.kv_heads * g.batches;
+  int block = blockIdx.x - (g.own ? (a.tiles + extra) * kv_all : 0);
+  if (block >= 0) {
     pdl_wait();
-    sum_dbias(a, g, blockIdx.x / g.bias_blocks, blockIdx.x % g.bias_blocks, reinterpret_cast<float*>(sm));
+    sum_dbias(a, g, block / g.bias_blocks, block % g.bias_blocks, reinterpret_cast<float*>(sm));
     return;
   }
-  const int block = blockIdx.x - buckets;
-  // the chunks of the sinks first: they are the longest
-  const int extra = g.sink_tiles * g.chunks, blocks = a.tiles + extra, bkv = block / blocks, at = block % blocks;
+  block = blockIdx.x;
+  const bool chunk = block < extra * kv_all;
+  if (!chunk) block -= extra * kv_all;
+  const int each = chunk ? extra : a.tiles, bkv = block / each, at = block % each;      // at: of the chunks, or the key tile
   const int kv = bkv % a.kv_heads, batch = bkv / a.kv_heads;
-  const int own = at < extra ? at / g.chunks : at - extra, k0 = own * kWRows;
+  const int own = chunk ? at / g.chunks : at, k0 = own * kWRows;
   const int last = last_of_window(a.n, a.left, k0);
   QueryTiles tiles;
-  if (at < extra) {
+  if (chunk) {
     tiles.first = last + 1;
     tiles.per = max((a.n - 1) / kWCols - last, 1);
     tiles.begin = at % g.chunks * g.chunk;
@@ -495,7 +513,15 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
   if (warp == 8) tmem_alloc(&bars.tmem_base, kCols);
-  if (!cta_ready(skip, warp == 8, bars.tmem_base, kCols)) return;
+  // as cta_ready, but beside window_dq_kernel: what this kernel reads was complete before that one's blocks signalled
+  tc_fence_before();
+  const bool stop = __syncthreads_or(skip) != 0;
+  tc_fence_after();
+  if (!g.early || stop) pdl_wait();
+  if (stop) {
+    if (warp == 8) tmem_free(bars.tmem_base, kCols);
+    return;
+  }
   const uint32_t tmem = bars.tmem_base;
 
   if (warp >= 8) {
@@ -714,7 +740,7 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       const int dn = (a.d + 15) & ~15;
       // where the key is a sink with chunks, this is one of the sums that the last of its CTAs adds up: its own first, then the chunks
       const bool summed = g.chunks > 0 && own < g.sink_tiles;
-      float* const to = g.sinks + (((size_t)bkv * g.sink_tiles + own) * (1 + g.chunks) + (at < extra ? 1 + at % g.chunks : 0)) * 2 * kWRows * dn +
+      float* const to = g.sinks + (((size_t)bkv * g.sink_tiles + own) * (1 + g.chunks) + (chunk ? 1 + at % g.chunks : 0)) * 2 * kWRows * dn +
                         (size_t)row * dn;
       for (int which = 0; which < 2; ++which) {      // dK, dV
         const RowsOut& out = which ? dv : dk;
@@ -762,6 +788,7 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       sum_sinks<kF16>(a, g, dk, dv, bkv, own);
     }
   }
+  if (g.early) pdl_wait();      // the grid ends behind window_dq_kernel's, as whatever comes next expects
 }
 
 }  // namespace px

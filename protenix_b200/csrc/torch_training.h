@@ -193,8 +193,9 @@ Tensor rows_fitted(const Tensor& t) {
 px_rows rows_of(const Tensor& t) { return {t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)}; }
 // A tensor of t's shape whose heads lie inside the rows where t's do, so that what follows (a projection of all heads) needs no copy.
 Tensor rows_like(const Tensor& t) {
-  const bool inside = t.size(1) > 1 && t.size(2) > 1 && t.stride(1) < t.stride(2);
-  return inside ? at::empty({t.size(0), t.size(2), t.size(1), t.size(3)}, t.options()).transpose(1, 2) : at::empty(t.sizes(), t.options());
+  const int64_t b = t.size(0), h = t.size(1), n = t.size(2), d = t.size(3);
+  const bool inside = h > 1 && n > 1 && t.stride(1) < t.stride(2);
+  return inside ? at::empty_strided({b, h, n, d}, {n * h * d, d, h * d, 1}, t.options()) : at::empty(t.sizes(), t.options());
 }
 px_window window_of(const Tensor& q, const Tensor& k, const Tensor& bias, const Tensor& mask, const WindowCall& c) {
   px_window w = {};

@@ -394,12 +394,13 @@ namespace px {
 // How the queries beyond the window that see sinks are cut: key tiles that hold sinks, chunks each, streamed tiles a chunk.
 static void sink_chunks(const WindowArgs& a, int* tiles, int* chunks, int* chunk) {
   *tiles = (a.sinks + kWRows - 1) / kWRows;
-  const int window = ((kWRows + a.left + a.right) / kWCols + 2) * a.group;      // about what the other CTAs have
-  *chunk = window > 64 ? window : 64;
   int most = 0;
   if (*tiles > 0) most = ((a.n - 1) / kWCols - last_of_window(a.n, a.left, 0)) * a.group;      // the first tile has the most
+  const int window = ((kWRows + a.left + a.right) / kWCols + 2) * a.group;      // about what the other CTAs have
+  *chunk = std::max(window, std::max(16, (most + 15) / 16));
   if (*tiles > 16 && *chunk < (most + 1) / 2) *chunk = (most + 1) / 2;      // CTAs enough, and each chunk takes memory for its sums
   *chunks = most > 0 ? (most + *chunk - 1) / *chunk : 0;
+  if (*chunks > 0) *chunk = (most + *chunks - 1) / *chunks;      // alike
   if (*chunks == 0) *tiles = 0;
 }
 static int64_t al256(int64_t n) { return (n + 255) / 256 * 256; }
@@ -418,15 +419,18 @@ static WindowSpace window_space(const px_window& w, const WindowArgs& a, bool bi
   return s;
 }
 
+template <bool kF16, int kLanes>
+static bool launch_window_delta(const WindowArgs& a, const WindowBwdArgs& g, const RowsOut& dout, const RowsOut& o, const RowsOut& rest, cudaStream_t st) {
+  const int64_t blocks = (int64_t)a.heads * g.batches * (a.npad / delta_block(kLanes));
+  return launch_pdl(window_delta_kernel<kF16, kLanes>, dim3((unsigned)blocks), 256, 0, st, a, g, dout, o, rest);
+}
 template <bool kF16, int kD, bool kBiasGrad>
-static bool launch_window_dq(const CUtensorMap* m, const WindowArgs& a, const WindowBwdArgs& g, const RowsOut& dout, const RowsOut& o,
-                             const RowsOut& rest, const RowsOut& dq, int64_t blocks, cudaStream_t st) {
+static bool launch_window_dq(const CUtensorMap* m, const WindowArgs& a, const WindowBwdArgs& g, const RowsOut& dq, int64_t blocks, cudaStream_t st) {
   typedef WindowDqLayout<kD> L;
   static SmemLimit limit;
   const auto kernel = window_dq_kernel<kF16, kD, kBiasGrad>;
   if (!limit.set(kernel, L::bytes(kWMaxR, kBiasGrad) + 1024)) return false;
-  return launch_pdl(kernel, dim3((unsigned)blocks), kWDqThreads, (size_t)L::bytes(a.r, kBiasGrad) + 1024, st, m[0], m[1], m[2], m[3], a, g, dout, o,
-                    rest, dq);
+  return launch_pdl(kernel, dim3((unsigned)blocks), kWDqThreads, (size_t)L::bytes(a.r, kBiasGrad) + 1024, st, m[0], m[1], m[2], m[3], a, g, dq);
 }
 template <bool kF16, int kD>
 static bool launch_window_dkv(const CUtensorMap* m, const WindowArgs& a, const WindowBwdArgs& g, const RowsOut& dk, const RowsOut& dv, int64_t blocks,
@@ -442,18 +446,24 @@ struct BwdRows {
   const px_rows *q, *k, *v, *o, *o_rest, *dout, *dq, *dk, *dv;
 };
 template <bool kF16>
-static bool window_bwd(const px_window& w, const BwdRows& x, const WindowArgs& a, const WindowBwdArgs& g, void* dbias, cudaStream_t st) {
+static bool window_bwd(const px_window& w, const BwdRows& x, const WindowArgs& a, WindowBwdArgs g, void* dbias, cudaStream_t st) {
   const int64_t blocks = (int64_t)a.tiles * w.heads * w.batch;
   const RowsOut dout = rows_out(x.dout), o = rows_out(x.o), rest = rows_out(x.o_rest), dq = rows_out(x.dq), dk = rows_out(x.dk), dv = rows_out(x.dv);
   CUtensorMap m[4];
   if (!rows_map(&m[0], *x.q, w, w.heads) || !rows_map(&m[1], *x.dout, w, w.heads) || !rows_map(&m[2], *x.k, w, w.kv_heads) ||
       !rows_map(&m[3], *x.v, w, w.kv_heads))
     return false;
+  g.own = dk.data || dv.data;
+  const bool queries = dq.data || dbias;
+  g.early = queries && g.own;
+  if (!queries && !g.own) return true;
+  const auto go_delta = w.d <= 32 ? launch_window_delta<kF16, 4> : w.d <= 64 ? launch_window_delta<kF16, 8> : launch_window_delta<kF16, 16>;
+  if (!go_delta(a, g, dout, o, rest, st)) return false;
   const auto go_q = w.d <= 64 ? (dbias ? launch_window_dq<kF16, 64, true> : launch_window_dq<kF16, 64, false>)
                               : (dbias ? launch_window_dq<kF16, 128, true> : launch_window_dq<kF16, 128, false>);
-  if (!go_q(m, a, g, dout, o, rest, dq, blocks, st)) return false;
-  const int64_t own = dk.data || dv.data ? (int64_t)(a.tiles + g.sink_tiles * g.chunks) * w.kv_heads * w.batch : 0;
-  const int64_t buckets = dbias ? (int64_t)w.heads * g.bias_blocks : 0;      // these come first: short, and there is room beside them
+  if (queries && !go_q(m, a, g, dq, blocks, st)) return false;
+  const int64_t own = g.own ? (int64_t)(a.tiles + g.sink_tiles * g.chunks) * w.kv_heads * w.batch : 0;
+  const int64_t buckets = dbias ? (int64_t)w.heads * g.bias_blocks : 0;
   if (own + buckets == 0) return true;
   const auto go_kv = w.d <= 32 ? launch_window_dkv<kF16, 32> : w.d <= 64 ? launch_window_dkv<kF16, 64> : launch_window_dkv<kF16, 128>;
   return go_kv(m, a, g, dk, dv, own + buckets, st);

@@ -232,6 +232,29 @@ def test_gradients_against_differences():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv_heads,d", [(16, 4, 64), (8, 8, 32), (4, 2, 128)])
+def test_what_follows_sees_all_gradients(heads, kv_heads, d):
+    """The kernels of the backward pass run beside one another; whatever is launched behind it, by this package or another, waits for all of them."""
+    q, k, v, grad, bias = _inputs(1, heads, kv_heads, 3000, d, BF16, 128)
+    want = _run(q, k, v, grad, bias, None, 300, 0, 4)
+    leaves = [t.detach().clone().requires_grad_() for t in (q, k, v, bias)]
+    results = []
+    for i in range(12):
+        o = px.window_attention(*leaves[:3], (300, 0), sinks=4, rel_bias=leaves[3])
+        dq, dk, dv, db = torch.autograd.grad(o, leaves, grad)
+        if i % 2:
+            results.append((dq + 0, dk + 0, dv + 0, db + 0, None))
+        else:
+            results.append((dq, dk, dv, db, ops.layer_norm(dq.reshape(-1, d), None, None)))
+        del dq, dk, dv, db
+    normed = ops.layer_norm(want["dq"].reshape(-1, d), None, None)
+    ops.device_error_flags()
+    for *grads, n in results:
+        assert all(torch.equal(g, want[x]) for g, x in zip(grads, NAMES))
+        assert n is None or torch.equal(n, normed)
+
+
+@pytest.mark.gpu
 def test_same_bits_on_other_streams_and_in_a_graph():
     q, k, v, grad, bias = _inputs(2, 8, 2, 900, 64, BF16, 32)
     m = _mask("end", 2, 900)
