@@ -10,14 +10,15 @@
 // signals its dependents once its wait for window_delta_kernel is over, and a block of window_dkv_kernel waits for that grid only at its end (or, where it adds
 // the bias's sums up, before it begins).  Neither fills a whole number of rounds over the SMs, and now they share the rest.
 //
-// Eight compute warps, a thread = one row x 32 of the 64 columns (no reduction along a row is needed here).  Copies and products have one warp in the first
-// kernel and two in the second, whose four products a step take an issuing warp some 1000 cycles beside busy ones (177 -> 168 us for a causal window
-// of 1024 over 8192 tokens; in the first kernel two warps were slower, 142 us against 114).  dS and P are rounded to the operands' type for the products
-// they enter and stay fp32 in the bias's gradient.
+// Compute warps: a thread = one row x 32 of the 64 columns (no reduction along a row is needed here), x 16 where the block is alone on its SM.  Copies and
+// products have one warp in the first kernel and two in the second, whose four products a step take an issuing warp some 1000 cycles beside busy ones
+// (177 -> 168 us for a causal window of 1024 over 8192 tokens; in the first kernel two warps were slower, 142 us against 114).  dS and P are rounded to the
+// operands' type for the products they enter and stay fp32 in the bias's gradient.
 //
 // What bounds them is, as forward, what the warps issue for a tile (exponentials, products, rounding, the bias's sums), with 16 warps an SM, as many as
-// tensor memory allows.  At 8192 tokens, 16 heads of 64 over 4 of keys, causal window of 1024: 125 us and 156 (three products and four of 16 GFLOP each:
-// 390 and 410 TFLOP/s).  Atoms, five samples of 3987 with 4 heads of 32, windows of 128, a bias by offset: 35 us and 29.
+// tensor memory allows.  At 8192 tokens, 16 heads of 64 over 4 of keys, causal window of 1024, from the first kernel's beginning to the last one's end: 252 us
+// (280 one behind the other) for seven products of 16 GFLOP; 8 heads of 128 over 2: 207 us.  2 x 1237 tokens, 16 heads of 24, window 200 + 200: 60 (80).
+// Atoms, five samples of 3987 with 4 heads of 32, windows of 128, a bias by offset: 55 (64).
 //
 // Keys that are sinks are seen by all later queries.  Their CTA takes the queries of the window, like any other; the
 // queries beyond are cut into chunks of about as many tiles, a CTA each, and the last of these CTAs adds the chunks up in their order.
@@ -29,7 +30,6 @@
 namespace px {
 
 constexpr int kWDqThreads = 288;      // eight warps of rows, one for copies and products
-constexpr int kWDkvThreads = 320;     // eight warps of rows, one for S^T and dP^T, one for the products with P^T and dS^T
 
 struct WindowBwdArgs {
   const float* nlse;             // [batch * heads][npad], base 2, negative; -inf for rows that see nothing and beyond the last
@@ -82,7 +82,7 @@ __global__ void __launch_bounds__(256) window_delta_kernel(const WindowArgs a, c
 
 struct WindowBwdBars {
   // streamed operands; S and dP, complete and in registers; P and dS; the products with them
-  uint64_t own_full, first_full[3], second_full[2], ready, taken, given, done;
+  uint64_t own_full, first_full[4], second_full[2], ready, taken, given, done;
   uint32_t tmem_base;
 };
 
@@ -122,7 +122,7 @@ window_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   if (threadIdx.x == 0) {
     prefetch_maps(map_q, map_do, map_k, map_v);
     mbar_init(&bars.own_full, 1);
-    for (int s = 0; s < 3; ++s) mbar_init(&bars.first_full[s], 1);
+    for (int s = 0; s < 4; ++s) mbar_init(&bars.first_full[s], 1);
     for (int s = 0; s < 2; ++s) mbar_init(&bars.second_full[s], 1);
     mbar_init(&bars.ready, 1);
     mbar_init(&bars.taken, 8);
@@ -387,9 +387,10 @@ window_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
 }
 
 // dbias[head][b] of the CTAs' sums, in their order: 32 buckets (block `of` of a head's), a slice of the CTAs of the head for each warp.
+template <int kThreads>
 __device__ __forceinline__ void sum_dbias(const WindowArgs& a, const WindowBwdArgs& g, int head, int of, float* slice) {
   const int lane = threadIdx.x & 31, s = threadIdx.x >> 5, buckets = 2 * a.r + 1, b = of * 32 + lane;
-  constexpr int kSlices = kWDkvThreads / 32;
+  constexpr int kSlices = kThreads / 32;
   float v = 0.f;
   if (b < buckets)
 #pragma unroll 4
@@ -413,10 +414,14 @@ __device__ __forceinline__ void sum_dbias(const WindowArgs& a, const WindowBwdAr
 // Heads of 33 to 64: S^T | dP^T | dV (64) | dK (64), P^T and dS^T in shared memory.  The next S^T and dP^T are made while these P^T and dS^T are.
 template <int kD>
 struct WindowDkvLayout {
-  // streamed tiles: three, or the next S^T would wait for one that was asked for only when the dS^T before was through; heads of 33 to 64 have room for two
-  static constexpr int panels = kD > 64 ? 2 : 1, stages = kD == 32 ? 3 : 2, tile = panels * kWCols * 128, stat = 2 * kWCols * 4;
+  // Streamed tiles: three or more, or the next S^T waits for one that was asked for only when the dS^T before was through (heads of 128: two 167 us, four 148);
+  // heads of 33 to 64 have room for two.
+  static constexpr int panels = kD > 64 ? 2 : 1, stages = kD == 64 ? 2 : kD == 32 ? 3 : 4, tile = panels * kWCols * 128, stat = 2 * kWCols * 4;
   static constexpr bool p_shared = kD == 64;
   static constexpr int cols = kD == 128 ? 512 : 256, ctas = kD == 128 ? 1 : 2;
+  // Warps of rows: 16 an SM whatever the head size, a thread = 32 of the 64 columns or, where the CTA is alone, 16.  Then one warp for S^T and dP^T, one for
+  // the products with P^T and dS^T.
+  static constexpr int warps = 16 / ctas, groups = warps / 4, rows = 32 * warps, threads = rows + 64;
   static constexpr int col_p = 2 * kWCols, col_ds = col_p + kWCols / 2;
   static constexpr int col_v = p_shared ? 2 * kWCols : 3 * kWCols, col_k = col_v + kD;
   static_assert(col_k + kD <= cols, "tensor memory of a CTA");
@@ -427,10 +432,10 @@ struct WindowDkvLayout {
 };
 
 // The rows of dK and dV of one key tile, from the parts that its CTAs have left: a thread = 8 values.
-template <bool kF16>
+template <bool kF16, int kThreads>
 __device__ __forceinline__ void sum_sinks(const WindowArgs& a, const WindowBwdArgs& g, const RowsOut& dk, const RowsOut& dv, int bkv, int own) {
   const int dn = (a.d + 15) & ~15, pieces = a.d / 8, rows = min(a.n - own * kWRows, kWRows);
-  for (int u = threadIdx.x; u < 2 * rows * pieces; u += kWDkvThreads) {
+  for (int u = threadIdx.x; u < 2 * rows * pieces; u += kThreads) {
     const int c = u % pieces * 8, row = u / pieces % rows, which = u / pieces / rows;
     const RowsOut& out = which ? dv : dk;
     if (!out.data) continue;
@@ -461,12 +466,12 @@ __host__ __device__ __forceinline__ int last_of_window(int n, int left, int k0) 
 }
 
 template <bool kF16, int kD>
-__global__ void __launch_bounds__(kWDkvThreads, WindowDkvLayout<kD>::ctas)
+__global__ void __launch_bounds__(WindowDkvLayout<kD>::threads, WindowDkvLayout<kD>::ctas)
 window_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do, const __grid_constant__ CUtensorMap map_k,
                   const __grid_constant__ CUtensorMap map_v, const WindowArgs a, const WindowBwdArgs g, const RowsOut dk, const RowsOut dv) {
   typedef WindowDkvLayout<kD> L;
   constexpr uint32_t kCols = L::cols;
-  constexpr int kPanels = L::panels, kStages = L::stages;
+  constexpr int kPanels = L::panels, kStages = L::stages, kFirst = L::warps;      // kFirst: the first control warp
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* sm = smem_aligned(smem_raw);
   WindowBwdBars& bars = *reinterpret_cast<WindowBwdBars*>(sm + L::bars);
@@ -477,7 +482,7 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   int block = blockIdx.x - (g.own ? (a.tiles + extra) * kv_all : 0);
   if (block >= 0) {
     pdl_wait();
-    sum_dbias(a, g, block / g.bias_blocks, block % g.bias_blocks, reinterpret_cast<float*>(sm));
+    sum_dbias<L::threads>(a, g, block / g.bias_blocks, block % g.bias_blocks, reinterpret_cast<float*>(sm));
     return;
   }
   block = blockIdx.x;
@@ -504,27 +509,27 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   if (threadIdx.x == 0) {
     prefetch_maps(map_q, map_do, map_k, map_v);
     mbar_init(&bars.own_full, 1);
-    for (int s = 0; s < 3; ++s) mbar_init(&bars.first_full[s], 1);
+    for (int s = 0; s < 4; ++s) mbar_init(&bars.first_full[s], 1);
     for (int s = 0; s < 2; ++s) mbar_init(&bars.second_full[s], 1);
     mbar_init(&bars.ready, 1);
-    mbar_init(&bars.taken, 8);
-    mbar_init(&bars.given, 8);
+    mbar_init(&bars.taken, L::warps);
+    mbar_init(&bars.given, L::warps);
     mbar_init(&bars.done, 1);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
-  if (warp == 8) tmem_alloc(&bars.tmem_base, kCols);
+  if (warp == kFirst) tmem_alloc(&bars.tmem_base, kCols);
   // as cta_ready, but beside window_dq_kernel: what this kernel reads was complete before that one's blocks signalled
   tc_fence_before();
   const bool stop = __syncthreads_or(skip) != 0;
   tc_fence_after();
   if (!g.early || stop) pdl_wait();
   if (stop) {
-    if (warp == 8) tmem_free(bars.tmem_base, kCols);
+    if (warp == kFirst) tmem_free(bars.tmem_base, kCols);
     return;
   }
   const uint32_t tmem = bars.tmem_base;
 
-  if (warp >= 8) {
+  if (warp >= kFirst) {
     // ------------------------------------------------------------------ copies and products
     const uint32_t k_at = smem_u32(sm), v_at = smem_u32(sm + L::v), q_at = smem_u32(sm + L::q), do_at = smem_u32(sm + L::dout);
     const uint32_t idesc_s = umma_idesc_16(128, kWCols, kF16, kF16), idesc_d = umma_idesc_16(128, (a.d + 15) & ~15, kF16, kF16, false, true);
@@ -552,7 +557,7 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       return true;
     };
     bool ok = true;
-    if (warp == 8) {
+    if (warp == kFirst) {
       if (tiles.count > 0) {
         if (elect_lane()) {
           mbar_expect_tx(&bars.own_full, 2 * kPanels * kWRows * 128);
@@ -595,11 +600,12 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       }
     }
   } else {
-    // ------------------------------------------------------------------ one key row x 32 queries a thread
-    const int quarter = warp & 3, half = warp >> 2, row = 32 * quarter + lane, j = k0 + row, kw = k0 + 32 * quarter;
+    // ------------------------------------------------------------------ one key row x 32 queries a thread, or 16 of the 32
+    constexpr int kHalves = L::groups == 2 ? 2 : 1;
+    const int quarter = warp & 3, group = warp >> 2, half = group / (L::groups / 2), row = 32 * quarter + lane, j = k0 + row, kw = k0 + 32 * quarter;
     const uint32_t t_lane = tmem + ((uint32_t)(32 * quarter) << 16);
     const bool masked = a.mask && __ldg(a.mask + (size_t)batch * a.n + min(j, a.n - 1)) == 0;
-    const bool any_masked = a.mask && barrier_any(1, 256, masked);
+    const bool any_masked = a.mask && barrier_any(1, L::rows, masked);
     const f32x2 scale = both2(a.c);
     // blocks of queries from qh on that see all of this warp's keys, and those whose bias is the first or the last entry for all
     const int whole_from = any_masked ? 0x3fffffff : kw + 31 - a.right, whole_to = min(kw + 32 <= a.sinks ? a.n : kw - 31 + a.left, a.n - 32);
@@ -610,9 +616,9 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     for (int t = 0; t < tiles.count; ++t, now.next(tiles)) {
       const int qh = (tiles.first + now.tile) * kWCols + 32 * half, s = t % kStages;
       if (a.r >= 0 && now.member != filled) {
-        barrier_of(1, 256);                        // all are through with the tile before
-        bias_fill(a, kv * a.group + now.member, bias, 256);
-        barrier_of(1, 256);
+        barrier_of(1, L::rows);                        // all are through with the tile before
+        bias_fill(a, kv * a.group + now.member, bias, L::rows);
+        barrier_of(1, L::rows);
         filled = now.member;
       }
       if (!ok) continue;
@@ -622,7 +628,7 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       ok = mbar_wait(&bars.first_full[s], (t / kStages) & 1, 64u) && ok;
       __syncwarp();
       tc_fence_after();
-      uint32_t wp[16], wd[16], nothing = 0, seen = 0xffffffffu;
+      uint32_t wp[8 * kHalves], wd[8 * kHalves], nothing = 0, seen = 0xffffffffu;
       bool near = false;
       float flat = 0.f;
       const float* y = bias;
@@ -642,14 +648,15 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       }
       const bool seen_all = __all_sync(0xffffffffu, seen == 0xffffffffu);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {                             // 16 columns at a time, for the registers' sake
+      for (int k = 0; k < kHalves; ++k) {                       // 16 columns at a time, for the registers' sake
+        const int h = kHalves == 2 ? k : group & 1;
         float p[16], d[16];
         if (!dead) {
           tmem_ld16(t_lane + 32 * half + 16 * h, *reinterpret_cast<uint32_t(*)[16]>(&p[0]));
           tmem_ld16(t_lane + kWCols + 32 * half + 16 * h, *reinterpret_cast<uint32_t(*)[16]>(&d[0]));
           tmem_wait_ld();
         }
-        if (h == 1) {
+        if (k == kHalves - 1) {
           tc_fence_before();
           ok = __all_sync(0xffffffffu, ok) != 0;
           if (!ok) break;
@@ -657,7 +664,7 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         }
         if (dead) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) wp[8 * h + e] = wd[8 * h + e] = 0u;
+          for (int e = 0; e < 8; ++e) wp[8 * k + e] = wd[8 * k + e] = 0u;
           continue;
         }
         const ulonglong2* const nlse4 = reinterpret_cast<const ulonglong2*>(sm + L::stats + s * L::stat) + 8 * half + 4 * h;
@@ -693,21 +700,21 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         if (seen_all) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            wp[8 * h + e] = pack16x2<kF16>(p[2 * e], p[2 * e + 1]);
-            wd[8 * h + e] = pack16x2<kF16>(d[2 * e], d[2 * e + 1]);
+            wp[8 * k + e] = pack16x2<kF16>(p[2 * e], p[2 * e + 1]);
+            wd[8 * k + e] = pack16x2<kF16>(d[2 * e], d[2 * e + 1]);
           }
         } else {
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             const bool a0 = seen >> (16 * h + 2 * e) & 1u, a1 = seen >> (16 * h + 2 * e + 1) & 1u;
-            wp[8 * h + e] = pack16x2<kF16>(a0 ? p[2 * e] : 0.f, a1 ? p[2 * e + 1] : 0.f);
-            wd[8 * h + e] = pack16x2<kF16>(a0 ? d[2 * e] : 0.f, a1 ? d[2 * e + 1] : 0.f);
+            wp[8 * k + e] = pack16x2<kF16>(a0 ? p[2 * e] : 0.f, a1 ? p[2 * e + 1] : 0.f);
+            wd[8 * k + e] = pack16x2<kF16>(a0 ? d[2 * e] : 0.f, a1 ? d[2 * e + 1] : 0.f);
           }
         }
       }
       if (!ok) continue;
-      if (nothing) {                                // whatever their rows of Q and dO hold becomes zeros; those of this half by its four warps
-        if (nothing >> lane & 1u) {
+      if (nothing) {                                // whatever their rows of Q and dO hold becomes zeros; those of this half by four of its warps
+        if ((nothing >> lane & 1u) && (kHalves == 2 || (group & 1) == 0)) {
           clear_row<kPanels, kWCols>(sm + L::q + s * L::tile, 32 * half + lane, quarter, 4);
           clear_row<kPanels, kWCols>(sm + L::dout + s * L::tile, 32 * half + lane, quarter, 4);
         }
@@ -718,12 +725,17 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         if (!ok) continue;
       }
       tc_fence_after();
-      if (L::p_shared) {
+      if constexpr (L::p_shared) {
         panel_store(sm + L::p, row, half, wp);
         panel_store(sm + L::ds, row, half, wd);
       } else {
-        tmem_st16(t_lane + L::col_p + 16 * half, wp);
-        tmem_st16(t_lane + L::col_ds + 16 * half, wd);
+        if constexpr (kHalves == 2) {
+          tmem_st16(t_lane + L::col_p + 16 * half, wp);
+          tmem_st16(t_lane + L::col_ds + 16 * half, wd);
+        } else {
+          tmem_st8(t_lane + L::col_p + 8 * group, wp);
+          tmem_st8(t_lane + L::col_ds + 8 * group, wd);
+        }
         tmem_wait_st();
       }
       if (L::p_shared || nothing) fence_async_shared();
@@ -746,7 +758,7 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         const RowsOut& out = which ? dv : dk;
         const float scale = which ? 1.f : g.scale;
         if (!out.data) continue;
-        for (int c = 16 * half; c < a.d; c += 32) {
+        for (int c = 16 * group; c < a.d; c += 16 * L::groups) {
           uint32_t x[16];
           if (tiles.count > 0) {
             tmem_ld16(t_lane + (which ? L::col_v : L::col_k) + c, x);
@@ -774,7 +786,7 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   if (summed) __threadfence();      // this CTA's sums are seen before its arrival is
   tc_fence_before();
   cta_teardown_sync();
-  if (warp == 8) {
+  if (warp == kFirst) {
     tc_fence_after();
     tmem_free(tmem, kCols);
   }
@@ -785,7 +797,7 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     __syncthreads();
     if (count == (uint32_t)g.chunks) {
       __threadfence();
-      sum_sinks<kF16>(a, g, dk, dv, bkv, own);
+      sum_sinks<kF16, L::threads>(a, g, dk, dv, bkv, own);
     }
   }
   if (g.early) pdl_wait();      // the grid ends behind window_dq_kernel's, as whatever comes next expects

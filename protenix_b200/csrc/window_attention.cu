@@ -439,7 +439,7 @@ static bool launch_window_dkv(const CUtensorMap* m, const WindowArgs& a, const W
   static SmemLimit limit;
   const auto kernel = window_dkv_kernel<kF16, kD>;
   if (!limit.set(kernel, L::bytes(kWMaxR) + 1024)) return false;
-  return launch_pdl(kernel, dim3((unsigned)blocks), kWDkvThreads, (size_t)L::bytes(a.r) + 1024, st, m[0], m[1], m[2], m[3], a, g, dk, dv);
+  return launch_pdl(kernel, dim3((unsigned)blocks), L::threads, (size_t)L::bytes(a.r) + 1024, st, m[0], m[1], m[2], m[3], a, g, dk, dv);
 }
 
 struct BwdRows {
