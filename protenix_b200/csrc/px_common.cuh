@@ -132,8 +132,9 @@ __device__ __forceinline__ float4 load4(const bf16* p) {
 // Programmatic dependent launch: a kernel launched with launch_pdl may start while the one before it drains, and waits here,
 // before it touches anything that earlier kernels wrote or read, until those are complete.  Its launch, barrier set-up,
 // tensor-memory allocation and fetch of the resident weights then overlap that end (a block at N = 128: 28 launches, 278 us
-// without, 225 us with).  Nothing signals its dependents early (griddepcontrol.launch_dependents at the top of every kernel
-// measured 235 us, and 1.5 % more at N = 1536: what starts early takes room from what runs).
+// without, 225 us with).  Nothing on that path signals its dependents early (griddepcontrol.launch_dependents at the top of every
+// kernel measured 235 us, and 1.5 % more at N = 1536: what starts early takes room from what runs); window_dq_kernel does, for the kernel behind
+// it, which needs nothing of it until its own end.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
 
 // Launch that may overlap the end of the kernel before it (see pdl_wait).
