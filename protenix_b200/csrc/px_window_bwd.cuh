@@ -348,7 +348,8 @@ window_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     }
     if (kBiasGrad) {
       // dS adds up to zero along a row; what is left is the error of delta, which lies in every dS of the row as P times it.  In the sums over the clipped
-      // offsets, where many keys of a row come together, it is taken out (37 sinks, two other keys: dbias off by 4.2e-3 in bf16 without, 2.9e-3 with it; 2 to 6 % of the kernel).
+      // offsets, where many keys of a row come together, it is taken out (37 sinks, two other keys: dbias off by 4.2e-3 in bf16 without,
+      // 2.9e-3 with it; 2 to 6 % of the kernel).
       part[half * kWRows + row] = low + high + inner;
       ok = barrier_all(2 + quarter, 64, ok);
       const float left_over = part[row] + part[kWRows + row];

@@ -9,10 +9,10 @@
 // 4 r + 3 sums W_pos + W_tok and 2 s + 2 sums W_chain + W_ent (both tables 35 KB of shared memory for r = 32, s = 2 and 64 channels).
 //
 // Forward: a warp takes 32 neighbouring pairs of a row; a lane finds one pair's two rows (a code, kept for the backward pass: 4 bytes beside the
-// pair's 256 or 512), then the warp writes them, a few pairs side by side, 4 channels a lane, and looks the rows up again only where they change (most neighbours are
-// far apart or in another chain: clipped alike).  Memory-bound writer: 1501 tokens x 128 channels in bf16, 91 us for 577 MB = 6.3 TB/s, 97 % of a
-// copy's rate, and up to 104 with the 9 MB of codes between backward passes; 384 tokens in fp32 15.5 us for 76 MB = 4.9 TB/s.  The smallest wait for W, from which every block makes its tables:
-// 97 tokens 5 us for 4.8 MB.  So a block's tables are for 32 or 64 channels.
+// pair's 256 or 512), then the warp writes them, a few pairs side by side, 4 channels a lane, and looks the rows up again only where they
+// change (most neighbours are far apart or in another chain: clipped alike).  Memory-bound writer: 1501 tokens x 128 channels in bf16, 91 us for
+// 577 MB = 6.3 TB/s, 97 % of a copy's rate, and up to 104 with the 9 MB of codes between backward passes; 384 tokens in fp32 16 us for 76 MB = 4.7 TB/s.
+// The smallest wait for W, from which every block makes its tables: 97 tokens 5 us for 4.8 MB.  So a block's tables are for 32 or 64 channels.
 //
 // Backward: memory-bound reader, two forms.  This one, for fp32 and for tables that the other has no room for: a block (a thread = one channel) reads
 // strips of 32 pairs of a row through a ring of bulk copies and holds sums of its own for every table row in shared memory, so there are no atomics and
@@ -330,8 +330,9 @@ __global__ void __launch_bounds__(kRpBwdThreads, 2) relpos_bwd_kernel(RelposArgs
 // dz enters as it lies (its channels are the contiguous index: an MN-major operand), the two-hot operand [table row][64 pairs] lives in shared memory and costs
 // a lane two stores a pair to set and two to clear (four warps of them: one took 1100 cycles a tile, where memory takes 700); the products with one are exact.
 // 64 pairs are 288 cycles of the tensor pipe (N = 144), less than half of what their 16 KB take to arrive.  Memory bounds it: 1501 tokens x 128
-// channels, 110 us for 577 MB + 9 MB of codes = 5.3 TB/s, 81 % of a copy's rate.  The tensor core truncates when it adds, so an accumulator takes eight tiles (32 additions) before four warps add it, rounding to
-// nearest, to fp32 sums in shared memory, while the next tiles go to the other accumulator.
+// channels, 110 us for 577 MB + 9 MB of codes = 5.3 TB/s, 81 % of a copy's rate (six tiles on their way, or codes asked for two tiles ahead: the same).
+// The tensor core truncates when it adds, so an accumulator takes eight tiles (32 additions) before four warps add it, rounding to nearest, to fp32
+// sums in shared memory, while the next tiles go to the other accumulator.
 // Warps 0..3 drain (a thread = one channel), 4 brings dz, 5 issues the products, 6..9 write the two-hot operands, 32 pairs of every other tile each.
 constexpr int kRpTile = 64, kRpRing = 4, kRpGroup = 8;      // pairs of a tile, tiles on their way, tiles of an accumulator
 constexpr int kRpTcThreads = 10 * 32, kRpTileBytes = kRpTile * kRpChunk * 2;
