@@ -419,7 +419,7 @@ PX_API int32_t px_relpos_bwd(const uint32_t* codes, const void* dz, float* dw, v
  * queries that see nothing hold (NaN included) has no influence.  lse: px_window_lse_floats() floats that the backward pass reads, or NULL.
  * o_rest (rows like o, same type, or NULL): what the rounding of o has taken off, which makes the gradients of narrow windows up to three times as exact.
  * px_window_bwd writes those of dq, dk, dv (types and shapes of q, k, v) and dbias (bias_dtype) that are not NULL; sums have a fixed
- * order.  Workspace aligned to 256 bytes.  Stands in for the local attention of protenix/model/modules/primitives.py
+ * order, and what fp16 cannot hold comes out infinite or NaN.  Workspace aligned to 256 bytes.  Stands in for the local attention of protenix/model/modules/primitives.py
  * (n_queries / n_keys) where the window moves with the query, not with its block. */
 typedef struct {
   void* data;

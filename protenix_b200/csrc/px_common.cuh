@@ -39,10 +39,20 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
 __device__ __forceinline__ float2 unpack_f16x2(uint32_t u) {
   return __half22float2(*reinterpret_cast<const __half2*>(&u));
 }
+// The same without the saturation: what fp16 cannot hold becomes infinite, for values whose overflow a caller has to see (gradients).
+__device__ __forceinline__ uint32_t pack_f16x2_inf(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
 // The two 16-bit operand formats of the tensor-core kernels: bf16 (kF16 = false) and fp16 (kF16 = true).
 template <bool kF16>
 __device__ __forceinline__ uint32_t pack16x2(float lo, float hi) {
   return kF16 ? pack_f16x2(lo, hi) : pack_bf16x2(lo, hi);
+}
+template <bool kF16>
+__device__ __forceinline__ uint32_t pack16x2_inf(float lo, float hi) {
+  return kF16 ? pack_f16x2_inf(lo, hi) : pack_bf16x2(lo, hi);
 }
 template <bool kF16>
 __device__ __forceinline__ float2 unpack16x2(uint32_t u);

@@ -194,17 +194,17 @@ __device__ __forceinline__ bool barrier_any(int id, int threads, bool p) {
 }
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
 
-// 8 values of a row as 16 bytes.
+// 8 values of a gradient's row as 16 bytes; beyond the range of the type they are infinite, by which a loss scaler knows them.
 template <bool kF16>
 __device__ __forceinline__ void store8(void* to, const uint32_t* v, float scale) {
   uint4 w;
   uint32_t* o = reinterpret_cast<uint32_t*>(&w);
 #pragma unroll
-  for (int e = 0; e < 4; ++e) o[e] = pack16x2<kF16>(__uint_as_float(v[2 * e]) * scale, __uint_as_float(v[2 * e + 1]) * scale);
+  for (int e = 0; e < 4; ++e) o[e] = pack16x2_inf<kF16>(__uint_as_float(v[2 * e]) * scale, __uint_as_float(v[2 * e + 1]) * scale);
   *reinterpret_cast<uint4*>(to) = w;
 }
 
-// The same, and what the rounding has taken off each value as 16 bits more, at `rest` unless that is NULL.
+// 8 values of an output's row, and what the rounding has taken off each value as 16 bits more, at `rest` unless that is NULL.
 template <bool kF16>
 __device__ __forceinline__ void store8(void* to, void* rest, const uint32_t* v, float scale) {
   uint4 w, r;

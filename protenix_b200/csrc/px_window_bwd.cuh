@@ -13,7 +13,8 @@
 // Compute warps: a thread = one row x 32 of the 64 columns (no reduction along a row is needed here), x 16 where the block is alone on its SM.  Copies and
 // products have one warp in the first kernel and two in the second, whose four products a step take an issuing warp some 1000 cycles beside busy ones
 // (177 -> 168 us for a causal window of 1024 over 8192 tokens; in the first kernel two warps were slower, 142 us against 114).  dS and P are rounded to the
-// operands' type for the products they enter and stay fp32 in the bias's gradient.
+// operands' type for the products they enter and stay fp32 in the bias's gradient.  A dS or a gradient that fp16 cannot hold becomes infinite and what it enters
+// infinite or NaN: clipped it would pass for a number, and a loss scaler would not learn that its scale is too large.
 //
 // What bounds them is, as forward, what the warps issue for a tile (exponentials, products, rounding, the bias's sums), with 16 warps an SM, as many as
 // tensor memory allows.  At 8192 tokens, 16 heads of 64 over 4 of keys, causal window of 1024, from the first kernel's beginning to the last one's end: 252 us
@@ -272,7 +273,7 @@ window_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           }
         }
 #pragma unroll
-        for (int e = 0; e < 16; ++e) w[e] = pack16x2<kF16>(d[2 * e], d[2 * e + 1]);
+        for (int e = 0; e < 16; ++e) w[e] = pack16x2_inf<kF16>(d[2 * e], d[2 * e + 1]);
       } else {
 #pragma unroll
         for (int e = 0; e < 16; ++e) w[e] = 0u;
@@ -702,14 +703,14 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             wp[8 * k + e] = pack16x2<kF16>(p[2 * e], p[2 * e + 1]);
-            wd[8 * k + e] = pack16x2<kF16>(d[2 * e], d[2 * e + 1]);
+            wd[8 * k + e] = pack16x2_inf<kF16>(d[2 * e], d[2 * e + 1]);
           }
         } else {
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             const bool a0 = seen >> (16 * h + 2 * e) & 1u, a1 = seen >> (16 * h + 2 * e + 1) & 1u;
             wp[8 * k + e] = pack16x2<kF16>(a0 ? p[2 * e] : 0.f, a1 ? p[2 * e + 1] : 0.f);
-            wd[8 * k + e] = pack16x2<kF16>(a0 ? d[2 * e] : 0.f, a1 ? d[2 * e + 1] : 0.f);
+            wd[8 * k + e] = pack16x2_inf<kF16>(a0 ? d[2 * e] : 0.f, a1 ? d[2 * e + 1] : 0.f);
           }
         }
       }

@@ -28,7 +28,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     ``rel_bias`` [H, 2 r + 1], fp32 or of q's type, r up to 256: learned, added to the logits by the clipped offset, entry
     clip(j - i, -r, r) + r.  ``scale``: positive, default D ** -0.5.
 
-    Logits, softmax and sums are fp32; the weights, and their gradients, are rounded to q's type where a product takes them.  Differentiable
+    Logits, softmax and sums are fp32; the weights, and their gradients, are rounded to q's type where a product takes them.  A gradient that
+    fp16 cannot hold, on the way to the result or as such, comes out infinite or NaN, so that a loss scaler finds it.  Differentiable
     once in q, k, v and rel_bias; the gradients are the same to the bit on each call.
     """
     left, right = (window, window) if isinstance(window, int) else window
