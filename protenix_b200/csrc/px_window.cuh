@@ -204,15 +204,18 @@ __device__ __forceinline__ void store8(void* to, const uint32_t* v, float scale)
   *reinterpret_cast<uint4*>(to) = w;
 }
 
-// 8 values of an output's row, and what the rounding has taken off each value as 16 bits more, at `rest` unless that is NULL.
+// A mean of fp16 values before it is rounded: infinite or NaN where one of them is, but never because the rounding of the weights has lifted it beyond 65504.
+__device__ __forceinline__ float mean_of_f16(float v) { return fabsf(v) < CUDART_INF_F ? fminf(fmaxf(v, -65504.f), 65504.f) : v; }
+// 8 values of an output's row as 16 bytes, and what the rounding has taken off each as 16 bits more, at `rest` unless that is NULL.
 template <bool kF16>
 __device__ __forceinline__ void store8(void* to, void* rest, const uint32_t* v, float scale) {
   uint4 w, r;
   uint32_t *o = reinterpret_cast<uint32_t*>(&w), *q = reinterpret_cast<uint32_t*>(&r);
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    const float a = __uint_as_float(v[2 * e]) * scale, b = __uint_as_float(v[2 * e + 1]) * scale;
-    o[e] = pack16x2<kF16>(a, b);
+    float a = __uint_as_float(v[2 * e]) * scale, b = __uint_as_float(v[2 * e + 1]) * scale;
+    if constexpr (kF16) a = mean_of_f16(a), b = mean_of_f16(b);
+    o[e] = pack16x2_inf<kF16>(a, b);
     const float2 back = unpack16x2<kF16>(o[e]);
     q[e] = pack16x2<kF16>(a - back.x, b - back.y);
   }
