@@ -282,7 +282,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       tc_fence_after();
       const float2 both = apart2(l);
       const float denominator = both.x + both.y;
-      const bool empty = m == -CUDART_INF_F;
+      const bool empty = denominator == 0.f;      // not by m, which a row of NaN leaves at -inf, too
       const float inv = empty ? 0.f : 1.f / denominator;
       uint16_t *const out = o.at(batch, head, i), *const more = rest.data ? rest.at(batch, head, i) : nullptr;
       for (int c = 0; c < a.d; c += 16) {

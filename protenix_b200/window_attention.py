@@ -23,7 +23,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
 
     Query i sees key j when j <= i + right and (j >= i - left or j < sinks), ``window`` = (left, right) or one number for both, and
     ``mask`` [..., N] (any type, nonzero = there) holds at j.  right = 0 is causal.  A query that sees nothing gives zeros and no gradient,
-    and what masked keys and such queries hold, NaN included, has no influence.  (A NaN elsewhere may reach all queries of its tile of 128.)
+    and what masked keys and such queries hold, NaN included, has no influence.  (A NaN or an infinity elsewhere may reach
+    all queries, and in the backward pass all keys, of its tile of 128.)
 
     ``rel_bias`` [H, 2 r + 1], fp32 or of q's type, r up to 256: learned, added to the logits by the clipped offset, entry
     clip(j - i, -r, r) + r.  ``scale``: positive, default D ** -0.5.
