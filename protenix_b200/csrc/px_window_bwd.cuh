@@ -433,6 +433,10 @@ struct WindowDkvLayout {
   static constexpr int bytes(int r) { return bias + bias_floats(r) * 4; }
 };
 
+// P in fp16 is rounded times this (P is 1 at most, 2^15 fits) and dV divided by it: weights are normal numbers down to 2^-29, where 2^-14 would be the last and all weights of a
+// wide window could be off alike (10.5 steps of 2^-24: 5 %; a loss scale does not reach P).
+constexpr float kWPUp = 32768.f;
+
 // The rows of dK and dV of one key tile, from the parts that its CTAs have left: a thread = 8 values.
 template <bool kF16, int kThreads>
 __device__ __forceinline__ void sum_sinks(const WindowArgs& a, const WindowBwdArgs& g, const RowsOut& dk, const RowsOut& dv, int bkv, int own) {
@@ -609,6 +613,7 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     const bool masked = a.mask && __ldg(a.mask + (size_t)batch * a.n + min(j, a.n - 1)) == 0;
     const bool any_masked = a.mask && barrier_any(1, L::rows, masked);
     const f32x2 scale = both2(a.c);
+    constexpr float up = kF16 ? kWPUp : 1.f;
     // blocks of queries from qh on that see all of this warp's keys, and those whose bias is the first or the last entry for all
     const int whole_from = any_masked ? 0x3fffffff : kw + 31 - a.right, whole_to = min(kw + 32 <= a.sinks ? a.n : kw - 31 + a.left, a.n - 32);
     const int low_from = kw + 31 + a.r, high_to = kw - 31 - a.r;
@@ -702,14 +707,14 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         if (seen_all) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            wp[8 * k + e] = pack16x2<kF16>(p[2 * e], p[2 * e + 1]);
+            wp[8 * k + e] = pack16x2<kF16>(up * p[2 * e], up * p[2 * e + 1]);
             wd[8 * k + e] = pack16x2_inf<kF16>(d[2 * e], d[2 * e + 1]);
           }
         } else {
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             const bool a0 = seen >> (16 * h + 2 * e) & 1u, a1 = seen >> (16 * h + 2 * e + 1) & 1u;
-            wp[8 * k + e] = pack16x2<kF16>(a0 ? p[2 * e] : 0.f, a1 ? p[2 * e + 1] : 0.f);
+            wp[8 * k + e] = pack16x2<kF16>(a0 ? up * p[2 * e] : 0.f, a1 ? up * p[2 * e + 1] : 0.f);
             wd[8 * k + e] = pack16x2_inf<kF16>(a0 ? d[2 * e] : 0.f, a1 ? d[2 * e + 1] : 0.f);
           }
         }
@@ -758,7 +763,7 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
                         (size_t)row * dn;
       for (int which = 0; which < 2; ++which) {      // dK, dV
         const RowsOut& out = which ? dv : dk;
-        const float scale = which ? 1.f : g.scale;
+        const float scale = which ? (kF16 ? 1.f / kWPUp : 1.f) : g.scale;
         if (!out.data) continue;
         for (int c = 16 * group; c < a.d; c += 16 * L::groups) {
           uint32_t x[16];
