@@ -9,7 +9,7 @@
 // One CTA = 128 queries of a head, streamed over the 64-key tiles that they see.  Warps 0..3: one thread a query row.  Warp 4
 // loads Q once and K, V tiles by TMA (panels of 64 elements, 128-byte swizzle, a ring of two each) and issues S = Q K^T and, once the rows have left P
 // (16 bits), O += P V with V read as it lies, along its rows.  The next S is made while this one, by then in registers, becomes P.
-// Softmax is online in base 2 with a reference maximum that moves (and O with it) only when a tile exceeds it by more than 8: P is 2^8 at most.
+// Softmax is online in base 2 with a reference maximum that moves (and O with it) only when a tile exceeds it by more than 8: P is 2^8 at most (2^15 in fp16, see kWUpF16).
 // Logits, statistics and O are fp32; P is rounded to the type of V, which the product needs (relative error of half a step, 2^-8 or 2^-11 at most,
 // with either sign); the denominators sum the fp32 values.
 //
@@ -31,6 +31,9 @@
 namespace px {
 
 constexpr float kWRescaleGap = 8.0f;
+// P in fp16 is 2^7 times as large as against the reference maximum, 2^15 at most: weights are normal numbers down to 2^-21 of the row's largest at least, where 2^-14
+// would be the last and those of many keys could be off alike (10.5 steps of 2^-24: 5 %).  The denominator has the same factor.
+constexpr float kWUpF16 = 7.0f;
 constexpr int kWFwdThreads = 160;
 
 struct WindowFwdBars {
@@ -148,6 +151,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       bias_fill(a, head, bias, 128);
       barrier_of(1, 128);
     }
+    constexpr float kUp = kF16 ? kWUpF16 : 0.f;      // in base 2
     float m = -CUDART_INF_F;
     f32x2 l = pair2(0.f, 0.f);
     const f32x2 scale = both2(a.c);
@@ -211,7 +215,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       const bool move = __any_sync(0xffffffffu, up) && t > 0;      // the first product overwrites O
       const float m_old = m;
       m = up ? mt : m;
-      const float shift = m == -CUDART_INF_F ? 0.f : -m;
+      const float shift = (m == -CUDART_INF_F ? 0.f : -m) + kUp;
       f32x2 sum = pair2(0.f, 0.f);
       uint32_t w[kKT / 2];
 #pragma unroll
@@ -295,7 +299,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         }
       }
       // Rows that see nothing, and those beyond the last, have weights of zero in the backward pass.
-      if (nlse) nlse[(size_t)bh * a.npad + i] = i < a.n && !empty ? -(m + log2f(denominator)) : -CUDART_INF_F;
+      if (nlse) nlse[(size_t)bh * a.npad + i] = i < a.n && !empty ? kUp - m - log2f(denominator) : -CUDART_INF_F;
     }
   }
   tc_fence_before();

@@ -23,10 +23,23 @@ def _one_large(n, d, at):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("at", [0, 150, 299])
+def test_output_of_small_weights(d, at):
+    """The large key's value is zero, so that o is what the others add up to.  Each term: the weight rounded (U), fp32 steps and an exponential of a logit of
+    14.3 (2^-20 (1 + 14.3) < 2^-16); then the result rounded (U)."""
+    n = 300
+    q, k, v = _one_large(n, d, at)
+    v[:, :, at] = 0
+    o = px.window_attention(q, k, v, n, scale=1.0)
+    want = reference(q, k, v, n, n, scale=1.0)["o"][0]
+    assert bool(((o.double() - want).abs() <= (2.01 * U + 2.0 ** -16) * want.abs()).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [32, 64, 128])
 @pytest.mark.parametrize("n,window,sinks,at", [(300, (300, 300), 0, 0), (300, (300, 300), 0, 150), (4300, (33, 0), 3, 1)])
 def test_gradient_of_values_with_small_weights(d, n, window, sinks, at):
-    """dV of the other keys, whose terms all have one sign.  Each term: the weight rounded (U), fp32 steps and an exponential of a logit of
-    14.3 (2^-20 (1 + 14.3) < 2^-16); then the result rounded (U)."""
+    """dV of the other keys, whose terms all have one sign: the same roundings."""
     q, k, grad = _one_large(n, d, at)
     v = torch.zeros_like(q).requires_grad_()
     if n > 300:
