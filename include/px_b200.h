@@ -431,7 +431,7 @@ typedef struct {
   int64_t r_max;       /* clipping distance of the bias, at most 256; negative: no bias */
   const void* bias;    /* [heads][2 r_max + 1] */
   const uint8_t* mask; /* [batch][n], or NULL */
-  float scale;         /* positive and finite */
+  float scale;         /* positive, and finite also times log2(e): at most 2.35e38 */
   int32_t dtype, bias_dtype;
 } px_window;
 PX_API int64_t px_window_lse_floats(int64_t batch, int64_t heads, int64_t n);

@@ -281,7 +281,7 @@ Tensor window_attention(const Tensor& q, const Tensor& k, const Tensor& v, int64
   if (n > (1 << 24)) fail("at most 2^24 rows");
   if (left < 0 || right < 0 || sinks < 0) fail("window and sinks must not be negative");
   const double scale = scale_.has_value() ? *scale_ : 1.0 / std::sqrt((double)d);
-  if (!(scale > 0.0) || !((float)scale > 0.f) || !((float)scale <= 3.0e38f)) fail("scale must be positive and finite");
+  if (!(scale > 0.0) || !((float)scale > 0.f) || !((float)scale <= 2.35e38f)) fail("scale must be positive and finite, also times log2(e)");
   int64_t batch = 1;
   for (int64_t i = 0; i < q.dim() - 3; ++i) batch *= q.size(i);
   if (batch > 65535 || h > 65535) fail("at most 65535 samples and heads");

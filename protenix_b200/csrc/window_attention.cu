@@ -332,9 +332,10 @@ static bool rows_map(CUtensorMap* map, const px_rows& t, const px_window& w, int
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+constexpr float kWMaxScale = 2.35e38f;      // the kernels multiply by scale * log2(e), which has to be finite
 static int32_t window_check(const px_window* w) {
   if (!w || w->batch < 0 || w->n < 0 || w->heads <= 0 || w->kv_heads <= 0 || w->d <= 0 || w->left < 0 || w->right < 0 || w->sinks < 0 ||
-      w->heads % w->kv_heads != 0 || !(w->scale > 0.f) || !(w->scale <= 3.0e38f))
+      w->heads % w->kv_heads != 0 || !(w->scale > 0.f) || !(w->scale <= kWMaxScale))
     return PX_ERR_BAD_ARG;
   if ((w->dtype != PX_BF16 && w->dtype != PX_F16) || w->d % 8 != 0 || w->d > 128 || w->n > (1 << 24) || w->r_max > kWMaxR) return PX_ERR_UNSUPPORTED;
   if (w->heads / w->kv_heads * (w->n / kWCols + 1) > 0x3fffffffll) return PX_ERR_UNSUPPORTED;
