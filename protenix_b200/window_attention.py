@@ -27,7 +27,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     all queries, and in the backward pass all keys, of its tile of 128.)
 
     ``rel_bias`` [H, 2 r + 1], fp32 or of q's type, r up to 256: learned, added to the logits by the clipped offset, entry
-    clip(j - i, -r, r) + r.  ``scale``: positive, default D ** -0.5.
+    clip(j - i, -r, r) + r; an entry of minus infinity, or one that is times log2(e) (fp32 below -2.35e38), hides its offset like a mask.  ``scale``: positive,
+    default D ** -0.5.
 
     Logits, softmax and sums are fp32; the weights, and their gradients, are rounded to q's type where a product takes them.  A gradient that
     fp16 cannot hold, on the way to the result or as such, comes out infinite or NaN, so that a loss scaler finds it.  Differentiable
