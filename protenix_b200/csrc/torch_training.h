@@ -73,7 +73,7 @@ Tensor dropout_apply(const OptTensor& residual, const Tensor& x, const Drop& d, 
 }
 
 Tensor counter_dropout_add(const OptTensor& residual, const Tensor& x, double p, int64_t seed, int64_t offset, const OptTensor& state,
-                           const c10::optional<int64_t>& shared_dim) {
+                           const c10::optional<int64_t>& shared_dim, bool training) {
   need_cuda(x, "x");
   dtype_code(x, "x");
   if (!(p >= 0.0 && p <= 1.0)) fail("the dropout probability must lie in [0, 1]");
@@ -91,6 +91,7 @@ Tensor counter_dropout_add(const OptTensor& residual, const Tensor& x, double p,
     dim = *shared_dim < 0 ? *shared_dim + x.dim() : *shared_dim;
     if (dim < 0 || dim >= x.dim()) fail("shared_dim " + std::to_string(*shared_dim) + " is out of range for x of shape " + shape_of(x));
   }
+  if (!training) return has(residual) ? *residual + x : x.clone();
   return dropout_apply(residual, x, Drop{p, seed, offset, dim}, has(state) ? *state : Tensor());
 }
 

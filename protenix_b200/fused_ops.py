@@ -38,15 +38,14 @@ def dropout_add(residual: Optional[torch.Tensor], x: torch.Tensor, p_drop: float
 
     Kept elements are scaled by 1 / (1 - p_drop); product and sum are fp32 and are rounded once.  A dropped element contributes
     nothing whatever x holds there.  p_drop = 1 drops everything.  fp32, bf16 and fp16 CUDA tensors of any shape.
+    ``training`` False: residual + x (a copy of x), after the same checks of the arguments.
     """
     if not x.is_cuda:
         raise RuntimeError("dropout_add: CUDA tensors only, this package has no CPU path")
-    if not training:
-        return x.clone() if residual is None else residual + x
     state = seed if isinstance(seed, torch.Tensor) else None
     if state is not None and offset != 0:
         raise RuntimeError("dropout_add: a seed tensor holds the offset, too")
     for name, v in (("seed", 0 if state is not None else seed), ("offset", offset)):
         if not isinstance(v, int) or not 0 <= v < 1 << 63:
             raise RuntimeError(f"dropout_add: {name} must be an integer in [0, 2^63), got {v!r}")
-    return native.load().counter_dropout_add(residual, x, p_drop, 0 if state is not None else seed, offset, state, shared_dim)
+    return native.load().counter_dropout_add(residual, x, p_drop, 0 if state is not None else seed, offset, state, shared_dim, training)
