@@ -127,6 +127,10 @@ void need_on(const Tensor& t, const at::Device& dev, const char* name) {
   need_cuda(t, name);
   if (t.device() != dev) fail(std::string(name) + " must be on the device of the other tensors");
 }
+// A tangent of forward-mode differentiation would be lost without a word: a dual tensor does not require a gradient, and the kernels see its value alone.
+void no_tangent(const Tensor& t, const char* name) {
+  if (t._fw_grad(0).defined()) fail(std::string(name) + " has a tangent: forward-mode differentiation is not supported");
+}
 int dtype_code(const Tensor& t, const char* name) {
   switch (t.scalar_type()) {
     case at::kFloat: return PX_F32;
@@ -955,6 +959,9 @@ struct LayerNormFunction : torch::autograd::Function<LayerNormFunction> {
 
 Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bias, int64_t width, double eps) {
   ln_check(x, width);
+  no_tangent(x, "input");
+  if (has(weight)) no_tangent(*weight, "weight");
+  if (has(bias)) no_tangent(*bias, "bias");
   auto wants = [](const OptTensor& t) { return has(t) && t->requires_grad(); };
   if (at::GradMode::is_enabled() && (x.requires_grad() || wants(weight) || wants(bias)))
     return LayerNormFunction::apply(x, weight, bias, eps);
@@ -996,6 +1003,8 @@ Tensor dropout_add(const Tensor& residual, const Tensor& x, double p) {
   dtype_code(x, "x");
   need_on(residual, x.device(), "residual");
   if (residual.sizes() != x.sizes() || residual.scalar_type() != x.scalar_type()) fail("residual must match x");
+  no_tangent(x, "x");
+  no_tangent(residual, "residual");
   auto shape = x.sizes().vec();
   shape[shape.size() - 3] = 1;
   Tensor mask;

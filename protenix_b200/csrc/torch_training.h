@@ -92,6 +92,8 @@ Tensor counter_dropout_add(const OptTensor& residual, const Tensor& x, double p,
     if (dim < 0 || dim >= x.dim()) fail("shared_dim " + std::to_string(*shared_dim) + " is out of range for x of shape " + shape_of(x));
   }
   if (!training) return has(residual) ? *residual + x : x.clone();
+  no_tangent(x, "x");
+  if (has(residual)) no_tangent(*residual, "residual");
   return dropout_apply(residual, x, Drop{p, seed, offset, dim}, has(state) ? *state : Tensor());
 }
 
@@ -152,6 +154,7 @@ Tensor relative_position_encoding(const Tensor& weight, const std::vector<Tensor
   static const char* const names[] = {"asym_id", "residue_index", "entity_id", "token_index", "sym_id"};
   need_cuda(weight, "weight");
   dtype_code(weight, "weight");
+  no_tangent(weight, "weight");
   if (r < 0 || s < 0 || r > (1 << 20) || s > (1 << 20)) fail("r_max and s_max must not be negative");
   if (weight.dim() != 2 || weight.size(1) != 4 * r + 2 * s + 7)
     fail("weight must be [c, " + std::to_string(4 * r + 2 * s + 7) + "] for these r_max and s_max, got " + shape_of(weight));
@@ -292,6 +295,10 @@ Tensor window_attention(const Tensor& q, const Tensor& k, const Tensor& v, int64
       fail("rel_bias must be [H, 2 r + 1] with r at most 256, got " + shape_of(*bias));
     if (bias->scalar_type() != at::kFloat && bias->scalar_type() != q.scalar_type()) fail("rel_bias must be float32 or of the type of q");
   }
+  no_tangent(q, "q");
+  no_tangent(k, "k");
+  no_tangent(v, "v");
+  if (has(bias)) no_tangent(*bias, "rel_bias");
   c10::cuda::CUDAGuard guard(q.device());
   OptTensor m;
   if (has(mask)) {
