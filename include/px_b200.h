@@ -137,9 +137,10 @@ PX_API int32_t px_trimul_contract(const px_f16* a, const px_f16* b, px_f16* x, i
 /* Device-side waits are bounded: a kernel whose wait runs out records a flag, stops issuing work, frees what it
  * holds and returns; kernels launched while a flag is set return without working.  The call synchronises the
  * device, then returns and clears the record: bit f of *flags (PX_FAMILY_*) is set when a wait of kernel family f
- * gave up -- the outputs written since the last call are then not valid.  px_device_error_detail also fills
- * detail[PX_N_FAMILIES] with the wait codes of each family (which pipeline role gave up).  No counterpart in the
- * reference (torch reports asynchronous failures through the CUDA error state). */
+ * gave up -- the outputs written since the last call are then not valid.  px_device_error_words also fills
+ * detail[f], f < count, with the wait codes of family f (which pipeline role gave up); words beyond the last family are left
+ * as they are.  px_device_error_detail (for callers of version 100, whose arrays have PX_DETAIL_WORDS words) fills those of the first sixteen
+ * families only.  No counterpart in the reference (torch reports asynchronous failures through the CUDA error state). */
 #define PX_FAMILY_CONTRACT 0
 #define PX_FAMILY_FLASH 1
 #define PX_FAMILY_TRANSITION 2
@@ -158,9 +159,11 @@ PX_API int32_t px_trimul_contract(const px_f16* a, const px_f16* b, px_f16* x, i
 #define PX_FAMILY_MSA_ROWS 15
 #define PX_FAMILY_RELPOS 16
 #define PX_FAMILY_WINDOW 17
-#define PX_N_FAMILIES 18
+#define PX_N_FAMILIES 18 /* grows: give px_device_error_words the size of the array that it fills */
+#define PX_DETAIL_WORDS 16
 PX_API int32_t px_device_error_flags(uint32_t* flags);
 PX_API int32_t px_device_error_detail(uint32_t* flags, uint32_t* detail);
+PX_API int32_t px_device_error_words(uint32_t* flags, uint32_t* detail, int32_t count);
 /* Limit of every bounded wait on the current device, in SM clock cycles (default 2^28, about 0.14 s); cycles <= 0
  * restores the default.  No counterpart in the reference. */
 PX_API int32_t px_set_wait_limit_cycles(int64_t cycles);

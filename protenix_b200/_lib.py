@@ -31,6 +31,7 @@ SIGNATURES = {
     "px_trimul_contract": (I32, [P, P, P, I64, I64, I64, P]),
     "px_device_error_flags": (I32, [P]),
     "px_device_error_detail": (I32, [P, P]),
+    "px_device_error_words": (I32, [P, P, I32]),
     "px_set_wait_limit_cycles": (I32, [I64]),
     "px_selftest_wait_timeout": (I32, [P, P]),
     "px_standardise_rows": (I32, [P, P, I64, F, P]),

@@ -28,22 +28,26 @@ const LimitFn kLimitFns[PX_N_FAMILIES] = {px::contract_set_wait_limit, px::flash
 }  // namespace
 
 // Synchronises the device and returns (and clears) what the bounded waits recorded: bit f of *flags is set when a wait
-// of kernel family f ran out; detail[f] (optional, PX_N_FAMILIES words) holds that family's wait codes, which name
-// the pipeline role that gave up (0x80000000: the word could not be read).
-extern "C" int32_t px_device_error_detail(uint32_t* flags, uint32_t* detail) {
-  if (!flags) return PX_ERR_BAD_ARG;
+// of kernel family f ran out; detail[f], f < count, holds that family's wait codes, which name the pipeline role that gave up
+// (0x80000000: the word could not be read).
+extern "C" int32_t px_device_error_words(uint32_t* flags, uint32_t* detail, int32_t count) {
+  if (!flags || count < 0 || (count > 0 && !detail)) return PX_ERR_BAD_ARG;
   if (cudaDeviceSynchronize() != cudaSuccess) return PX_ERR_LAUNCH;
   uint32_t word = 0;
   for (int f = 0; f < PX_N_FAMILIES; ++f) {
     const uint32_t v = kFlagFns[f]();
     if (v) word |= 1u << f;
-    if (detail) detail[f] = v;
+    if (f < count) detail[f] = v;
   }
   *flags = word;
   return PX_OK;
 }
 
-extern "C" int32_t px_device_error_flags(uint32_t* flags) { return px_device_error_detail(flags, nullptr); }
+extern "C" int32_t px_device_error_detail(uint32_t* flags, uint32_t* detail) {
+  return px_device_error_words(flags, detail, detail ? PX_DETAIL_WORDS : 0);
+}
+
+extern "C" int32_t px_device_error_flags(uint32_t* flags) { return px_device_error_words(flags, nullptr, 0); }
 
 // Replaces the limit (clock cycles) of every bounded wait on the current device; cycles <= 0 restores the default.
 extern "C" int32_t px_set_wait_limit_cycles(int64_t cycles) {
@@ -53,7 +57,7 @@ extern "C" int32_t px_set_wait_limit_cycles(int64_t cycles) {
   return PX_OK;
 }
 
-extern "C" int32_t px_version(void) { return 100; }
+extern "C" int32_t px_version(void) { return 101; }
 
 extern "C" const char* px_status_string(int32_t status) {
   switch (status) {

@@ -158,7 +158,7 @@ def device_error_flags(device=None, raise_on_error: bool = True) -> int:
     flags = ctypes.c_uint32(0)
     detail = (ctypes.c_uint32 * len(KERNEL_FAMILIES))()
     with torch.cuda.device(device if device is not None else torch.cuda.current_device()):
-        _lib.check(_lib.load().px_device_error_detail(ctypes.byref(flags), detail), "px_device_error_detail")
+        _lib.check(_lib.load().px_device_error_words(ctypes.byref(flags), detail, len(detail)), "px_device_error_words")
     if flags.value and raise_on_error:
         what = ", ".join(f"{KERNEL_FAMILIES[f]} (wait codes 0x{detail[f]:x})" for f in range(len(KERNEL_FAMILIES))
                          if flags.value >> f & 1)
