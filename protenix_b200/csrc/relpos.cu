@@ -70,12 +70,13 @@ __device__ __forceinline__ void store4<__half>(__half* p, float4 v) {
 }
 
 constexpr int kRpFwdThreads = 1024;      // one block an SM
+constexpr int kRpFwdBytes = 226 << 10;   // shared memory of one: the tables and, beside them, its channels of W
+static_assert((kRpMaxRows + kRpMaxRows + 2) * 64 * 4 <= kRpFwdBytes, "room for 64 channels");      // W has two columns more than the tables have rows
 
-// kW: channels of a block, whose table is made for all of them.  codes: what the backward pass reads, one a pair, or NULL.  slice: channels of W that are
-// brought into shared memory at a time, all of them unless the tables are large.
+// kW: channels of a block, whose table is made for all of them.  codes: what the backward pass reads, one a pair, or NULL.
 template <typename T, int kW>
 __global__ void __launch_bounds__(kRpFwdThreads) relpos_fwd_kernel(RelposArgs a, const float* __restrict__ w, T* __restrict__ z,
-                                                                   uint32_t* __restrict__ codes, int slice) {
+                                                                   uint32_t* __restrict__ codes) {
   constexpr int kLanes = kW / 4, kSide = 32 / kLanes;                   // lanes of a pair, pairs side by side in a warp
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   __shared__ uint64_t full;
@@ -83,13 +84,12 @@ __global__ void __launch_bounds__(kRpFwdThreads) relpos_fwd_kernel(RelposArgs a,
   const int rows1 = a.rows1(), rows = rows1 + a.rows2(), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int tok = 2 * a.r + 2, ent = 4 * a.r + 4, chain = ent + 1;      // first columns of the parts of W behind the first
   float* const table = reinterpret_cast<float*>(smem_raw);              // [rows][kW]
-  float* const part = table + rows * kW;                                // [slice][t]
+  float* const part = table + rows * kW;                                // [kW][t]
   if (threadIdx.x == 0) {
     mbar_init(&full, 1);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
-    const int count = min(slice, channels);
-    mbar_expect_tx(&full, (uint32_t)(count * t * 4));
-    bulk_load(part, w + (long long)c0 * t, (uint32_t)(count * t * 4), &full);
+    mbar_expect_tx(&full, (uint32_t)(channels * t * 4));
+    bulk_load(part, w + (long long)c0 * t, (uint32_t)(channels * t * 4), &full);
   }
   const int strips = (int)((a.n + kRpPairs - 1) / kRpPairs);
   const long long units = a.pairs / a.n * strips, warps = (long long)gridDim.x * (kRpFwdThreads / 32);
@@ -101,28 +101,19 @@ __global__ void __launch_bounds__(kRpFwdThreads) relpos_fwd_kernel(RelposArgs a,
   };
   uint32_t code = u < units ? code_of(u) : 0u;                          // asked for while W is on its way
   __syncthreads();
-  bool ok = true;
-  for (int s0 = 0, k = 0; s0 < channels; s0 += slice, ++k) {
-    const int count = min(slice, channels - s0);
-    if (s0 > 0 && threadIdx.x == 0) {
-      mbar_expect_tx(&full, (uint32_t)(count * t * 4));
-      bulk_load(part, w + (long long)(c0 + s0) * t, (uint32_t)(count * t * 4), &full);
+  const bool ok = mbar_wait(&full, 0, 2u);
+  // A lane = a channel: t is odd, so neither side of this transposition meets a bank twice.
+  for (int v = threadIdx.x; v < rows * kW; v += kRpFwdThreads) {
+    const int ch = v % kW, row = v / kW;
+    if (ch < channels) {
+      const float* const f = part + ch * t;
+      const float x = row < tok     ? f[row] + f[tok + 2 * a.r + 1]
+                      : row < rows1 ? f[a.r] + f[row]
+                                    : f[chain + row - rows1] + (row - rows1 < 2 * a.s + 1 ? f[ent] : 0.f);
+      table[row * kW + ch] = x;
     }
-    ok = mbar_wait(&full, k & 1, 2u) && ok;
-    // A lane = a channel: t is odd, so neither side of this transposition meets a bank twice.
-    for (int v = threadIdx.x; v < rows * kW; v += kRpFwdThreads) {
-      const int ch = v % kW, row = v / kW;
-      if (ch < count) {
-        const float* const f = part + ch * t;
-        const float x = row < tok     ? f[row] + f[tok + 2 * a.r + 1]
-                        : row < rows1 ? f[a.r] + f[row]
-                                      : f[chain + row - rows1] + (row - rows1 < 2 * a.s + 1 ? f[ent] : 0.f);
-        table[row * kW + s0 + ch] = x;
-      }
-    }
-    ok = __syncthreads_and(ok) != 0;
   }
-  if (!ok) return;
+  if (!__syncthreads_and(ok)) return;
   const int at = 4 * (lane % kLanes), side = lane / kLanes;
   const bool mine = at < channels;
   while (u < units) {
@@ -542,14 +533,12 @@ extern "C" int32_t px_relpos_fwd(const int64_t* asym_id, const int64_t* residue_
   const RelposArgs a = {(const long long*)asym_id, (const long long*)residue_index, (const long long*)entity_id, (const long long*)token_index,
                         (const long long*)sym_id, n, batch * n * n, (int)c, r_max, s_max};
   const auto go = [&](auto* kernel, auto* out, int width, SmemLimit& limit) {
-    constexpr size_t kRoom = (size_t)226 << 10;
-    const size_t table = (size_t)(a.rows1() + a.rows2()) * width * 4, row = (size_t)a.columns() * 4;
-    const int slice = (int)std::min<size_t>(width, (kRoom - table) / row / 8 * 8);      // at least 8: see kRpMaxRows
+    const size_t smem = (size_t)(a.rows1() + a.rows2() + a.columns()) * width * 4;
     // a few strips a block at least, one block an SM at most
     const int64_t parts = (c + width - 1) / width;
     const dim3 grid((unsigned)std::min<int64_t>((relpos_units(batch, n) + 3) / 4, std::max<int64_t>(sm_count() / parts, 1)), (unsigned)parts);
-    if (!limit.set(kernel, kRoom)) return false;
-    kernel<<<grid, kRpFwdThreads, table + slice * row, (cudaStream_t)stream>>>(a, w, out, codes, slice);
+    if (!limit.set(kernel, kRpFwdBytes)) return false;
+    kernel<<<grid, kRpFwdThreads, smem, (cudaStream_t)stream>>>(a, w, out, codes);
     return cudaGetLastError() == cudaSuccess;
   };
   static SmemLimit limits[2][3];
