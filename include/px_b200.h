@@ -404,7 +404,8 @@ PX_API int32_t px_dropout_add(const void* residual, const void* x, void* out, in
  * z[b][i][j][:] = W onehot(buckets of (i, j)), features [batch][n], W fp32 [c][4 r_max + 2 s_max + 7] (columns: residue
  * offsets, token offsets, same entity, copy offsets, as the reference concatenates them), z PX_F32, PX_BF16 or PX_F16 [batch][n][n][c].
  * The forward pass leaves the buckets of each pair in `codes` (px_relpos_codes_bytes; NULL: not wanted) for the backward pass.
- * The gradient dw (fp32, like W) is a sum over the pairs of each bucket in a fixed order.  c a multiple of 8,
+ * The gradient dw (fp32, like W) is a sum over the pairs of each bucket in a fixed order.  A dz that is infinite or NaN stays so in its channel: in the
+ * columns of its pair for PX_F32, in all columns for the 16-bit types (unless 4 r_max + 2 s_max + 5 is above 208).  c a multiple of 8,
  * 4 r_max + 2 s_max + 5 <= 380; w, z, dz aligned to 16 bytes.  Replace RelativePositionEncoding (protenix/model/modules/embedders.py) and its autograd. */
 PX_API int64_t px_relpos_codes_bytes(int64_t batch, int64_t n);
 PX_API int64_t px_relpos_workspace_bytes(int64_t batch, int64_t n, int64_t c, int32_t r_max, int32_t s_max);

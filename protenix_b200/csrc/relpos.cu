@@ -20,8 +20,8 @@
 // diagonal, go to their sums eight at a time; the rest one by one.  Shared memory's read-add-write of these sums bounds it.
 // The blocks' sums, folded to the columns of W, are added up in their order by a second kernel.
 //
-// What is not finite: a dz of one pair that is infinite or NaN makes its channel NaN in the columns of its own rows here; the form on the tensor cores
-// spreads it over all columns of the channel (0 x inf).
+// What is not finite: a dz of one pair that is infinite or NaN stays so in its channel, in the columns of its own pair here; the form on the tensor cores
+// makes all columns of the channel NaN (0 x inf).
 #include "px_tcgen05.cuh"
 
 namespace px {

@@ -26,7 +26,8 @@ def relative_position_encoding(weight: torch.Tensor, asym_id: torch.Tensor, resi
 
     ``weight``: [c, 4 r_max + 2 s_max + 7], columns in the reference's order: residue offsets -r_max .. r_max and "another chain",
     token offsets likewise, "same entity", copy offsets -s_max .. s_max and "another entity".  c is a multiple of 8.  Sums are
-    fp32 whatever the types; the gradient of ``weight`` is the same to the bit on each call.
+    fp32 whatever the types; the gradient of ``weight`` is the same to the bit on each call.  A gradient of z that is infinite or NaN makes its channel of
+    ``weight``'s gradient so: the columns of its pair for an fp32 z, all of them for a 16-bit one.
     """
     return native.load().relative_position_encoding(weight, [asym_id, residue_index, entity_id, token_index, sym_id], r_max, s_max, dtype)
 
