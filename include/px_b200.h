@@ -428,7 +428,7 @@ PX_API int32_t px_relpos_bwd(const uint32_t* codes, const void* dz, float* dw, v
  * (n_queries / n_keys) where the window moves with the query, not with its block. */
 typedef struct {
   void* data;
-  int64_t batch, head, row; /* strides in elements, multiples of 8; ignored for an axis of length one */
+  int64_t batch, head, row; /* strides in elements, multiples of 8 and d at least; ignored for an axis of length one */
 } px_rows;
 typedef struct {
   int64_t batch, heads, kv_heads, n, d;

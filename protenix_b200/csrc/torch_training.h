@@ -186,10 +186,10 @@ struct WindowCall {
   double scale;
 };
 
-// [B, H, N, D] as the kernels address it: rows of neighbouring elements, 16-byte aligned, positive strides that are multiples of 16 bytes.
+// [B, H, N, D] as the kernels address it: rows of neighbouring elements, 16-byte aligned, that do not overlap, strides that are multiples of 16 bytes.
 Tensor rows_fitted(const Tensor& t) {
   bool fits = t.size(3) <= 1 || t.stride(3) == 1;
-  for (int i = 0; i < 3; ++i) fits = fits && (t.size(i) <= 1 || (t.stride(i) > 0 && t.stride(i) % 8 == 0));
+  for (int i = 0; i < 3; ++i) fits = fits && (t.size(i) <= 1 || (t.stride(i) >= t.size(3) && t.stride(i) % 8 == 0));
   if (fits && ((uintptr_t)t.data_ptr() & 15) == 0) return t;
   const Tensor c = t.contiguous();
   return ((uintptr_t)c.data_ptr() & 15) == 0 ? c : c.clone();

@@ -343,9 +343,10 @@ static int32_t window_check(const px_window* w) {
   if (w->r_max >= 0 && (!w->bias || (w->bias_dtype != PX_F32 && w->bias_dtype != PX_BF16 && w->bias_dtype != PX_F16))) return PX_ERR_BAD_ARG;
   return PX_OK;
 }
-// Rows that the kernels can address: 16-byte aligned, strides of the axes longer than one multiples of 8 elements, positive and below 2^40 bytes.
+// Rows that the kernels can address: 16-byte aligned, strides of the axes longer than one multiples of 8 elements, a row at least (a tensor map
+// asks for it) and below 2^40 bytes.
 static bool rows_fit(const px_rows* t, const px_window& w, int64_t heads) {
-  const auto fits = [](int64_t s, int64_t len) { return len <= 1 || (s > 0 && s % 8 == 0 && s < (1ll << 38)); };
+  const auto fits = [&](int64_t s, int64_t len) { return len <= 1 || (s >= w.d && s % 8 == 0 && s < (1ll << 38)); };
   return t && t->data && ((uintptr_t)t->data & 15) == 0 && fits(t->row, w.n) && fits(t->head, heads) && fits(t->batch, w.batch);
 }
 static RowsOut rows_out(const px_rows* t) {

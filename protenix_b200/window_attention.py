@@ -19,7 +19,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
 
     ``q`` [..., H, N, D], ``k`` and ``v`` [..., H_kv, N, D] (H_kv divides H: query head h reads head h // (H / H_kv)), bf16 or fp16, D a multiple
     of 8 up to 128.  Views are taken as they are (heads inside the rows of one projection, say); what the kernels cannot
-    address (broadcast axes, rows that do not begin on 16 bytes) is copied.  The output lies in memory like q: heads inside the rows where q's are.
+    address (broadcast axes, rows that overlap or do not begin on 16 bytes) is copied.  The output lies in memory like q: heads inside the rows where q's are.
 
     Query i sees key j when j <= i + right and (j >= i - left or j < sinks), ``window`` = (left, right) or one number for both, and
     ``mask`` [..., N] (any type, nonzero = there) holds at j.  right = 0 is causal.  A query that sees nothing gives zeros and no gradient,
