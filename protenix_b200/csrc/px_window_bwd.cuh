@@ -16,8 +16,8 @@
 // operands' type for the products they enter and stay fp32 in the bias's gradient.  A dS or a gradient that fp16 cannot hold becomes infinite and what it enters
 // infinite or NaN: clipped it would pass for a number, and a loss scaler would not learn that its scale is too large.
 //
-// What bounds them is, as forward, what the warps issue for a tile (exponentials, products, rounding, the bias's sums), with 16 warps an SM, as many as
-// tensor memory allows.  At 8192 tokens, 16 heads of 64 over 4 of keys, causal window of 1024, from the first kernel's beginning to the last one's end: 252 us
+// What bounds them is, as forward, what the warps issue for a tile (exponentials, products, rounding, the bias's sums), and the latency of each
+// warp's chain: issue slots 32 to 54 %, tensor pipe 26 to 48 %, with 16 row warps an SM, whose S, dP, P, dS and sums fill tensor memory.  At 8192 tokens, 16 heads of 64 over 4 of keys, causal window of 1024, from the first kernel's beginning to the last one's end: 252 us
 // (280 one behind the other) for seven products of 16 GFLOP; 8 heads of 128 over 2: 207 us.  2 x 1237 tokens, 16 heads of 24, window 200 + 200: 60 (80).
 // Atoms, five samples of 3987 with 4 heads of 32, windows of 128, a bias by offset: 55 (64).
 //

@@ -19,8 +19,9 @@
 //
 // What bounds it: the chain of a tile in a row's thread (maximum, exponentials, rounding: some 330 instructions where nothing is tested, 2000 cycles beside
 // the other warps), not a unit: at 8192 tokens, 16 heads of 64, causal window of 1024, 88 us (370 TFLOP/s), the special-function unit is
-// busy for two fifths of the time and the tensor pipe for a fifth; at 16384 tokens, 8 heads of 128, window of 2048, 152 us = 850 TFLOP/s, both for half.
-// So as many CTAs an SM as tensor memory, shared memory and registers allow: four (heads up to 32), three, two.  Short windows (atoms: four tiles a CTA) pay as much for a CTA's beginning and
+// busy for two fifths of the time and the tensor pipe for a fifth; at 16384 tokens, 8 heads of 128, window of 2048, both for half: 141 us in a loop over the same
+// inputs (920 TFLOP/s), 165 to 170 where the inputs change from pass to pass (770 TFLOP/s).
+// So as many CTAs an SM as tensor memory, shared memory and registers allow: four (heads up to 32), three, two, with four row warps each.  Short windows (atoms: four tiles a CTA) pay as much for a CTA's beginning and
 // end.  Built, measured and not kept: 128 keys a tile for heads of 64 (2 % slower), eight warps of rows with 32 keys each (10 to 40 %), copies issued by the row
 // warps (7 %), window and bias in one table with -inf (1 to 8 %), the maximum looked for only where a tile's sum is large (heads of 128 1.5 % faster, of 64 4 % slower).
 // A second allocation of tensor memory for P (heads of 64) would be asked for while holding the first, which could wait for good beside other kernels.
