@@ -420,7 +420,8 @@ PX_API int32_t px_relpos_bwd(const uint32_t* codes, const void* dz, float* dw, v
  * j <= i + right, j >= i - left or j < sinks, and mask[j] is not zero.  A query that sees nothing gives 0 and takes part in no gradient.
  * Rows q, o [batch][heads][n][d], k, v [batch][kv_heads][n][d] with the strides of px_rows; query head h uses key head h / (heads /
  * kv_heads).  PX_BF16 or PX_F16; d a multiple of 8 up to 128; products of 16-bit operands, everything else fp32.  What masked keys and
- * queries that see nothing hold (NaN included) has no influence.  lse: px_window_lse_floats() floats that the backward pass reads, or NULL.
+ * queries that see nothing hold (NaN included) has no influence; a NaN or an infinity elsewhere may reach all rows of its tile of 128.  A bias that is -inf
+ * times log2(e) hides its offset.  lse: px_window_lse_floats() floats that the backward pass reads, or NULL.
  * o_rest (rows like o, same type, or NULL): what the rounding of o has taken off.  Without it dbias of narrow windows with sinks is
  * off by about twice as much (64 draws each of windows of 1 to 2 with 37 to 64 sinks in bf16: 2.2e-3, 2.4e-3, 1.5e-3 in place of 1.2e-3, 1.2e-3, 0.8e-3), dq and dk by 5 to 8 % more.
  * px_window_bwd writes those of dq, dk, dv (types and shapes of q, k, v) and dbias (bias_dtype) that are not NULL; sums have a fixed
