@@ -159,7 +159,8 @@ PX_API int32_t px_trimul_contract(const px_f16* a, const px_f16* b, px_f16* x, i
 #define PX_FAMILY_MSA_ROWS 15
 #define PX_FAMILY_RELPOS 16
 #define PX_FAMILY_WINDOW 17
-#define PX_N_FAMILIES 18 /* grows: give px_device_error_words the size of the array that it fills */
+#define PX_FAMILY_LOSS 18
+#define PX_N_FAMILIES 19 /* grows: give px_device_error_words the size of the array that it fills */
 #define PX_DETAIL_WORDS 16
 PX_API int32_t px_device_error_flags(uint32_t* flags);
 PX_API int32_t px_device_error_detail(uint32_t* flags, uint32_t* detail);
@@ -447,6 +448,33 @@ PX_API int64_t px_window_workspace_bytes(const px_window* w, int32_t bias_grad);
 PX_API int32_t px_window_bwd(const px_window* w, const px_rows* q, const px_rows* k, const px_rows* v, const px_rows* o, const px_rows* o_rest,
                       const px_rows* dout, const float* lse, const px_rows* dq, const px_rows* dk, const px_rows* dv, void* dbias, void* workspace,
                       int64_t workspace_bytes, void* stream);
+
+/* ---- Softmax cross entropy of a linear head, without its logits (training path) ----------------
+ * l = x w^T + bias for rows x [rows][c] and classes w [classes][c] (PX_BF16 or PX_F16, row strides in elements), bias fp32 or NULL;
+ * loss_i = lse_i - (1 - smoothing) l_i,target - smoothing / classes sum_v l_iv.  Rows whose target is `ignore` have loss 0 and take no part in
+ * any gradient, whatever they hold; a target outside the classes makes its row's loss, and the gradients that it enters, NaN.
+ * px_head_loss_fwd writes norm [rows][2] (reference and sum of the exponentials, for the backward pass), the rows' losses [rows] (NULL: not wanted) and their sum or mean over the rows that count
+ * (total, with 1 / count or 1 in `inverse` for the backward pass; NULL: not wanted; the mean of nothing is NaN).
+ * px_head_loss_bwd writes those of dx [rows][c], dw [classes][c] (type of x, contiguous) and dbias [classes] (fp32) that are not NULL, from the gradient of
+ * the total (each = 0: one number) or of the rows' losses (each = 1, `inverse` not read).  It forms the logits again, for so many classes at a time
+ * that 16 bits a logit stay within 512 MiB (256 classes at least).  Sums are fp32, across rows fp64, and have a fixed order.  c a multiple of 8, pointers aligned
+ * to 16 bytes, workspaces to 256.  No counterpart in the reference, whose heads (protenix/model/modules/head.py) leave the loss to torch. */
+typedef struct {
+  const void* x;
+  const void* w;
+  const float* bias;
+  const int64_t* target;
+  int64_t rows, c, classes, x_stride, w_stride;
+  int64_t ignore;
+  float smoothing;
+  int32_t dtype;
+} px_head;
+PX_API int64_t px_head_loss_workspace_bytes(int64_t rows, int64_t classes);
+PX_API int32_t px_head_loss_fwd(const px_head* head, float* norm, float* losses, float* total, float* inverse, int32_t mean, void* workspace,
+                         int64_t workspace_bytes, void* stream);
+PX_API int64_t px_head_loss_bwd_workspace_bytes(const px_head* head, int32_t dx, int32_t dw, int32_t dbias);
+PX_API int32_t px_head_loss_bwd(const px_head* head, const float* norm, const float* grad, int32_t each, const float* inverse, void* dx, void* dw,
+                         float* dbias, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* ---- Exchange between the GPUs of one box (row-sharded path) ------------------------------
  * No counterpart in the reference (which runs the Pairformer on one GPU).  A peer buffer is a

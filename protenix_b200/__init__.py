@@ -1,6 +1,7 @@
 """B200-native (sm_100a) Pairformer pair-representation forward path behind the module API of
 bytedance/Protenix.  One code path: hand-written CUDA kernels reached through a C ABI
 (``include/px_b200.h``); nothing falls back to the CPU or to another back-end."""
+from .cross_entropy import linear_cross_entropy
 from .embedders import RelativePositionEncoding, relative_position_encoding
 from .layer_norm import FusedLayerNorm, LayerNorm
 from .msa import OuterProductMean
@@ -21,6 +22,6 @@ __all__ = [
     "TriangleAttentionStartingNode", "TriangleMultiplicationIncoming", "TriangleMultiplicationOutgoing",
     "TriangleMultiplicativeUpdate", "dropout_add_rowwise", "RecyclingTrunk", "OuterProductMean",
     "weights_changed", "dropout_add", "RelativePositionEncoding", "relative_position_encoding",
-    "window_attention",
+    "window_attention", "linear_cross_entropy",
 ]
 __version__ = "0.1.0"

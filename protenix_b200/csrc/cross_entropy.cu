@@ -1,0 +1,751 @@
+// Softmax cross entropy of a linear head, and its gradient, without the logits:
+//   l_iv = x_i . w_v + b_v,   lse_i = log sum_v exp l_iv,   loss_i = lse_i - (1 - e) l_it - e / V sum_v l_iv
+//   dl_iv = g_i (exp(l_iv - lse_i) - (1 - e) [v = t_i] - e / V),   dx = dl W,   dW = dl^T x,   db = sum_i dl_i
+//
+// Forward, one product whose epilogue keeps of a tile [128 rows][kN classes] each row's maximum, sum of exponentials and (smoothed
+// labels) sum of logits, and the logit of the row's class where it lies in the tile; a second kernel joins the tiles of a row.
+// Backward, for a piece of the classes at a time: the same product again, whose epilogue writes dl in 16 bits, then dx += dl W and
+// dW = dl^T x from it.  What a piece leaves in memory is 16 bits a pair of row and class, kPieceBytes at most, whatever the number of classes.
+// Four products of 2 N V C where three are the least (the logits are formed twice).
+//
+// dl is formed without the scale of the loss, in [-2, 2] (fp16: times 2^14, so that probabilities down to 2^-28 stay normal numbers); the scale is
+// applied in fp32 where dx and dW are rounded.  Logits, exponentials and all sums are fp32, or fp64 across rows.
+//
+// Rows that are ignored take no part whatever they hold: their dl is zero by selection, and where one holds an infinity or a NaN (which a zero
+// weight would not silence) dW takes a copy of x in which those rows are zero; the copy is made only then.
+#include <math_constants.h>
+
+#include "px_gemm.cuh"
+
+namespace px {
+
+constexpr int64_t kPieceBytes = 512ll << 20;
+constexpr int kScanBlocks = 592;
+constexpr float kDlScaleF16 = 16384.f;
+
+// What the small kernels of a backward pass leave for the products.
+struct LossScale {
+  float out;            // what dx and dW are multiplied by
+  float each;           // what the gradient of a row's loss is multiplied by, so that the largest is one
+  uint32_t dirty;       // an ignored row holds what is not finite
+};
+
+// What exponentials are taken relative to, in powers of two, for a maximum that may be that of nothing.
+__device__ __forceinline__ float reference(float m) { return m == -CUDART_INF_F ? 0.f : m; }
+
+// A row's part in the loss: its class, or a class that no column has.
+__device__ __forceinline__ bool row_counts(int64_t target, int64_t ignore) { return target != ignore; }
+
+// ---- forward ---------------------------------------------------------------------------------------------------------
+struct EpiStats {
+  const int64_t* target;
+  const float* bias;        // or NULL
+  float2* part;             // [tiles_n][rows]: maximum times log2(e), sum of exponentials relative to it
+  float* part_sum;          // [tiles_n][rows]: sum of logits, or NULL
+  float* hit;               // [rows]: logit of the row's class
+  uint32_t* arrivals;
+  int rows, classes;
+  static constexpr bool kMeets = true;
+  __device__ __forceinline__ void begin() const { *arrivals = 0; }
+
+  template <class S>
+  __device__ __forceinline__ void tile(const GemmEpiTile& e, bool ok) const {
+    constexpr int kCols = S::kN / 2;                        // of this warp
+    const int row = e.m0 + e.lane, base = e.n0 + e.half * kCols;
+    const bool there = row < rows;
+    const int64_t t = there ? target[row] - base : -1;
+    const int mine = t >= 0 && t < kCols ? (int)t : -1;     // the column that is the row's class
+    float m = -CUDART_INF_F, s = 0.f, sum = 0.f;
+#pragma unroll 1
+    for (int c = 0; c < kCols; c += 32) {
+      const int left = classes - (base + c);
+      if (left <= 0) break;
+      uint32_t r[32];
+      tmem_ld32(e.acc + e.half * kCols + c, r);
+      tmem_wait_ld();
+      float v[32];
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+      if (bias) {
+        if (left >= 32) {
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            const float4 b = __ldg(reinterpret_cast<const float4*>(bias + base + c + j));
+            v[j] += b.x, v[j + 1] += b.y, v[j + 2] += b.z, v[j + 3] += b.w;
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (j < left) v[j] += __ldg(bias + base + c + j);
+        }
+      }
+      if (left < 32) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (j >= left) v[j] = -CUDART_INF_F;
+      }
+      if (part_sum) {
+        float a[4] = {};
+#pragma unroll
+        for (int j = 0; j < 32; ++j) a[j & 3] += j < left ? v[j] : 0.f;
+        sum += (a[0] + a[1]) + (a[2] + a[3]);
+      }
+      if (mine >= c && mine < c + 32) {
+        float h = 0.f;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) h = mine - c == j ? v[j] : h;
+        hit[row] = h;
+      }
+      float top[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+      for (int j = 4; j < 32; ++j) top[j & 3] = fmaxf(top[j & 3], v[j]);
+      const float next = fmaxf(m, kLog2e * fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
+      const float ref = reference(next);
+      float a[4] = {s * fast_exp2(m - ref), 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < 32; ++j) a[j & 3] += fast_exp2(fmaf(v[j], kLog2e, -ref));
+      s = (a[0] + a[1]) + (a[2] + a[3]);
+      m = next;
+    }
+    // the two halves of the columns
+    float* const x = reinterpret_cast<float*>(e.extra) + 32 * e.quarter + e.lane;
+    if (e.half) x[0] = m, x[128] = s, x[256] = sum;
+    gemm_epi_sync();
+    if (!e.half) {
+      const float m1 = x[0], next = fmaxf(m, m1), ref = reference(next);
+      s = s * fast_exp2(m - ref) + x[128] * fast_exp2(m1 - ref);
+      if (there) {
+        const int64_t at = (int64_t)e.at.nt * rows + row;
+        part[at] = make_float2(next, s);
+        if (part_sum) part_sum[at] = sum + x[256];
+      }
+    }
+    gemm_epi_sync();
+  }
+};
+
+// Joins the tiles of each row: lse, loss, and (total) their mean or sum over the rows that count.  32 rows a block, the parts of a row over its
+// warps; the last block to arrive adds up what the blocks have left, in their order.
+constexpr int kJoinWarps = 16;
+struct JoinArgs {
+  const float2* part;
+  const float* part_sum;
+  const float* hit;
+  const int64_t* target;
+  float2* norm;             // [rows]: what exp(l - lse) is formed from, exp2(l log2(e) - x) / y
+  float* losses;            // [rows], or NULL
+  float* total;             // or NULL
+  float* inverse;           // receives 1 / count
+  double2* sums;            // [blocks]
+  uint32_t* arrivals;
+  int64_t ignore;
+  int rows, classes, parts, mean;
+  float smooth;
+};
+__global__ void __launch_bounds__(32 * kJoinWarps) loss_join_kernel(const JoinArgs a) {
+  __shared__ float xm[kJoinWarps][32], xs[kJoinWarps][32], xl[kJoinWarps][32];
+  __shared__ double tl[32 * kJoinWarps], tc[32 * kJoinWarps];
+  __shared__ bool last;
+  pdl_wait();
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, row = blockIdx.x * 32 + lane;
+  float m = -CUDART_INF_F, s = 0.f, sum = 0.f;
+  if (row < a.rows) {
+    for (int p = w; p < a.parts; p += kJoinWarps) {
+      const int64_t at = (int64_t)p * a.rows + row;
+      const float2 x = a.part[at];
+      const float next = fmaxf(m, x.x), ref = reference(next);
+      s = s * fast_exp2(m - ref) + x.y * fast_exp2(x.x - ref);
+      m = next;
+      if (a.part_sum) sum += a.part_sum[at];
+    }
+  }
+  xm[w][lane] = m, xs[w][lane] = s, xl[w][lane] = sum;
+  __syncthreads();
+  double l = 0.0, c = 0.0;
+  if (w == 0 && row < a.rows) {
+#pragma unroll 1
+    for (int i = 1; i < kJoinWarps; ++i) m = fmaxf(m, xm[i][lane]);
+    const float ref = reference(m);
+    s = sum = 0.f;
+#pragma unroll 1
+    for (int i = 0; i < kJoinWarps; ++i) s += xs[i][lane] * fast_exp2(xm[i][lane] - ref), sum += xl[i][lane];
+    const int64_t t = a.target[row];
+    const bool counts = row_counts(t, a.ignore);
+    float loss = 0.f;
+    if (counts) {
+      // all logits relative to the same reference: nothing of its size is left in the difference
+      loss = CUDART_NAN_F;
+      if (t >= 0 && t < a.classes) loss = log2f(s) - (1.f - a.smooth) * fmaf(a.hit[row], kLog2e, -ref);
+      if (a.part_sum) loss -= a.smooth * fmaf(sum / (float)a.classes, kLog2e, -ref);
+      loss = loss < 0.f ? 0.f : loss * 0.6931471805599453f;
+      l = loss, c = 1.0;
+    }
+    a.norm[row] = make_float2(ref, s);
+    if (a.losses) a.losses[row] = loss;
+  }
+  if (!a.total) return;
+  if (w == 0) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o), c += __shfl_xor_sync(0xffffffffu, c, o);
+    if (lane == 0) {
+      a.sums[blockIdx.x] = make_double2(l, c);
+      __threadfence();
+      last = atomicAdd(a.arrivals, 1u) == gridDim.x - 1;
+    }
+  }
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  l = c = 0.0;
+  for (int i = threadIdx.x; i < (int)gridDim.x; i += 32 * kJoinWarps) {
+    const double2 v = __ldcg(a.sums + i);
+    l += v.x, c += v.y;
+  }
+  tl[threadIdx.x] = l, tc[threadIdx.x] = c;
+  __syncthreads();
+  for (int o = 16 * kJoinWarps; o > 0; o >>= 1) {
+    if ((int)threadIdx.x < o) tl[threadIdx.x] += tl[threadIdx.x + o], tc[threadIdx.x] += tc[threadIdx.x + o];
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) {
+    *a.total = (float)(a.mean ? tl[0] / tc[0] : tl[0]);      // the mean of nothing is NaN
+    *a.inverse = a.mean ? (float)(1.0 / fmax(tc[0], 1.0)) : 1.f;
+  }
+}
+
+// ---- backward: what the products need to know first ------------------------------------------------------------------
+struct ScanArgs {
+  const void* x;
+  int64_t x_stride;
+  const int64_t* target;
+  const float* grad;        // of the loss: one number, or (each) one a row
+  uint2* found;             // [kScanBlocks]: not finite in an ignored row; bits of the largest finite |grad|
+  int64_t ignore, rows;
+  int c, each;
+};
+__device__ __forceinline__ bool finite16x2(uint32_t u, bool f16) {
+  const uint32_t e = f16 ? 0x7c007c00u : 0x7f807f80u, lo = e & 0xffffu, hi = e & 0xffff0000u;
+  return (u & lo) != lo && (u & hi) != hi;
+}
+// A warp a row; rows that count cost their target.
+__global__ void __launch_bounds__(256) loss_scan_kernel(const ScanArgs a, bool f16) {
+  __shared__ uint32_t bad[8], big[8];
+  pdl_wait();
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  uint32_t dirty = 0, top = 0;
+  for (int64_t r0 = ((int64_t)blockIdx.x * 8 + w) * 32; r0 < a.rows; r0 += (int64_t)gridDim.x * 256) {
+    const int64_t row = r0 + lane;
+    const bool ignored = row < a.rows && !row_counts(a.target[row], a.ignore);
+    if (a.each && row < a.rows && !ignored) {
+      const float g = fabsf(a.grad[row]);
+      if (g < CUDART_INF_F) top = max(top, __float_as_uint(g));
+    }
+    for (uint32_t left = __ballot_sync(0xffffffffu, ignored); left; left &= left - 1) {
+      const uint4* p = reinterpret_cast<const uint4*>((const uint16_t*)a.x + (r0 + __ffs(left) - 1) * a.x_stride);
+      for (int i = lane; i < a.c / 8; i += 32) {
+        const uint4 v = __ldg(p + i);
+        if (!(finite16x2(v.x, f16) && finite16x2(v.y, f16) && finite16x2(v.z, f16) && finite16x2(v.w, f16))) dirty = 1;
+      }
+    }
+  }
+  dirty = __any_sync(0xffffffffu, dirty);
+  top = __reduce_max_sync(0xffffffffu, top);
+  if (lane == 0) bad[w] = dirty, big[w] = top;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < 8; ++i) dirty |= bad[i], top = max(top, big[i]);
+    a.found[blockIdx.x] = make_uint2(dirty, top);
+  }
+}
+// Joins that, forms the scales, and copies x without the ignored rows where one of them is not finite.
+__global__ void __launch_bounds__(256) loss_prepare_kernel(const ScanArgs a, const float* __restrict__ inverse, uint16_t* __restrict__ clean, LossScale* __restrict__ scale,
+                                                           int blocks, float dl_scale) {
+  pdl_wait();
+  uint32_t dirty = 0, top = 0;
+  for (int i = threadIdx.x; i < blocks; i += 256) {
+    const uint2 f = a.found[i];
+    dirty |= f.x, top = max(top, f.y);
+  }
+  __shared__ uint32_t big;
+  if (threadIdx.x == 0) big = 0;
+  dirty = __syncthreads_or((int)dirty) != 0;
+  if (a.each) {
+    top = __reduce_max_sync(0xffffffffu, top);
+    if ((threadIdx.x & 31) == 0) atomicMax(&big, top);
+    __syncthreads();
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    const float largest = __uint_as_float(big);
+    // divided by a power of two, so that nothing is rounded; the smallest powers have no reciprocal that is finite
+    const float power = fmaxf(__uint_as_float(__float_as_uint(largest) & 0x7f800000u), 1.17549435e-38f);
+    LossScale s;
+    s.out = a.each ? power / dl_scale : a.grad[0] * *inverse / dl_scale;
+    s.each = a.each ? 1.f / power : 1.f;
+    s.dirty = dirty;
+    *scale = s;
+  }
+  if (!dirty) return;
+  const int per = a.c / 8;
+  const int64_t all = a.rows * per;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+    const int64_t row = i / per;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (row_counts(a.target[row], a.ignore)) v = __ldg(reinterpret_cast<const uint4*>((const uint16_t*)a.x + row * a.x_stride) + (i - row * per));
+    reinterpret_cast<uint4*>(clean)[i] = v;
+  }
+}
+
+// v[0] of lane j = the sum of v[j] over the lanes: at each step half of the columns go to the other half of the lanes.
+template <int kHalf = 16>
+__device__ __forceinline__ void column_sums(float (&v)[32], int lane) {
+  const bool up = (lane & kHalf) != 0;
+#pragma unroll
+  for (int j = 0; j < kHalf; ++j) {
+    const float give = up ? v[j] : v[j + kHalf], keep = up ? v[j + kHalf] : v[j];
+    v[j] = keep + __shfl_xor_sync(0xffffffffu, give, kHalf);
+  }
+  if constexpr (kHalf > 1) column_sums<kHalf / 2>(v, lane);
+}
+
+// ---- backward: dl ----------------------------------------------------------------------------------------------------
+struct EpiLogitGrad {
+  CUtensorMap out;          // dl [rows][classes of the piece], boxes of 32 x 64
+  const int64_t* target;
+  const float* bias;        // of the piece, or NULL
+  const float2* norm;
+  const float* grad;        // of each row's loss, or NULL
+  const LossScale* scale;
+  float* part_bias;         // [32-row groups][classes of the piece]: sums of dl, or NULL
+  int64_t ignore;
+  int rows, classes, first, all_classes;      // first: the piece's first class
+  float smooth;
+  int f16;
+  static constexpr bool kMeets = false;
+  __device__ __forceinline__ void begin() const {}
+
+  template <class S>
+  __device__ __forceinline__ void tile(const GemmEpiTile& e, bool) const {
+    constexpr int kCols = S::kN == 64 ? 64 : S::kN / 2;     // blocks of 64: of a narrow tile, half of the warps have none
+    const int row = e.m0 + e.lane, base = e.n0 + e.half * kCols;
+    if (e.m0 >= rows || (S::kN == 64 && e.half)) return;
+    const int64_t t = row < rows ? target[row] : ignore;
+    const bool counts = row < rows && row_counts(t, ignore);
+    const int64_t in_piece = t - first - base;
+    const int mine = counts && t >= 0 && t < all_classes && in_piece >= 0 && in_piece < kCols ? (int)in_piece : -1;
+    // dl = factor (p - smooth / V) - (mine) factor (1 - smooth), p = exp2(l log2(e) + ref) / sum
+    float factor = 0.f, ref = 0.f, over = 0.f;
+    if (counts) {
+      factor = grad ? grad[row] * scale->each : 1.f;
+      if (t < 0 || t >= all_classes) factor = CUDART_NAN_F;
+      if (f16) factor *= kDlScaleF16;
+      const float2 n = norm[row];
+      ref = -n.x, over = factor / n.y;
+    }
+    const float less = factor * smooth / (float)all_classes, hit = factor * (1.f - smooth);
+#pragma unroll 1
+    for (int c = 0; c < kCols; c += 64) {
+      if (base + c >= classes) break;
+      if (e.lane == 0) tma_store_wait_read<0>();
+      __syncwarp();
+#pragma unroll 1
+      for (int h = 0; h < 64; h += 32) {
+        const int left = classes - (base + c + h);
+        uint32_t r[32];
+        tmem_ld32(e.acc + e.half * kCols + c + h, r);
+        tmem_wait_ld();
+        float v[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+        if (bias) {
+          if (left >= 32) {
+#pragma unroll
+            for (int j = 0; j < 32; j += 4) {
+              const float4 b = __ldg(reinterpret_cast<const float4*>(bias + base + c + h + j));
+              v[j] += b.x, v[j + 1] += b.y, v[j + 2] += b.z, v[j + 3] += b.w;
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (j < left) v[j] += __ldg(bias + base + c + h + j);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = fmaf(over, fast_exp2(fmaf(v[j], kLog2e, ref)), -less);
+        if (mine >= c + h && mine < c + h + 32) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (mine - (c + h) == j) v[j] -= hit;
+        }
+        if (!counts) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = 0.f;
+        }
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          uint4 o;
+          if (f16) {
+            o.x = pack_f16x2_inf(v[8 * p], v[8 * p + 1]), o.y = pack_f16x2_inf(v[8 * p + 2], v[8 * p + 3]);
+            o.z = pack_f16x2_inf(v[8 * p + 4], v[8 * p + 5]), o.w = pack_f16x2_inf(v[8 * p + 6], v[8 * p + 7]);
+          } else {
+            o.x = pack_bf16x2(v[8 * p], v[8 * p + 1]), o.y = pack_bf16x2(v[8 * p + 2], v[8 * p + 3]);
+            o.z = pack_bf16x2(v[8 * p + 4], v[8 * p + 5]), o.w = pack_bf16x2(v[8 * p + 6], v[8 * p + 7]);
+          }
+          *reinterpret_cast<uint4*>(e.stg + e.lane * 128 + (((h / 8 + p) ^ (e.lane & 7)) << 4)) = o;
+        }
+        if (part_bias) {
+          column_sums(v, e.lane);
+          if (e.lane < left) part_bias[(int64_t)(e.m0 / 32) * classes + base + c + h + e.lane] = v[0];
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+      __syncwarp();
+      if (e.lane == 0) {
+        tma_store_3d(&out, smem_u32(e.stg), base + c, e.m0, 0);
+        tma_store_commit();
+      }
+    }
+  }
+};
+
+// db of a piece: a warp's lanes along the classes, the groups of rows over the warps, in a fixed order.
+__global__ void __launch_bounds__(512) loss_bias_kernel(const float* __restrict__ part, float* __restrict__ db, const LossScale* __restrict__ scale, int classes, int groups) {
+  __shared__ float x[16][32];
+  pdl_wait();
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, v = blockIdx.x * 32 + lane;
+  double s = 0.0;
+  if (v < classes)
+    for (int g = w; g < groups; g += 16) s += part[(int64_t)g * classes + v];
+  x[w][lane] = (float)s;
+  __syncthreads();
+  if (w == 0 && v < classes) {
+    float all = 0.f;
+    for (int i = 0; i < 16; ++i) all += x[i][lane];
+    db[v] = all * scale->out;
+  }
+}
+
+// ---- backward: dx and dW ---------------------------------------------------------------------------------------------
+// kF32: sums of one split, stored (or added to what the pieces before have left); otherwise the result in 16 bits.
+template <bool kF32>
+struct EpiGrad {
+  CUtensorMap out;          // boxes of 32 rows of 128 bytes
+  const LossScale* scale;
+  const int64_t* target;    // of the rows, those that are ignored get zeros; or NULL
+  int64_t ignore;
+  int rows, cols, add, f16;
+  static constexpr bool kMeets = false;
+  __device__ __forceinline__ void begin() const {}
+
+  template <class S>
+  __device__ __forceinline__ void tile(const GemmEpiTile& e, bool) const {
+    constexpr int kCols = S::kN / 2, kBlock = kF32 ? 32 : 64;
+    if (e.m0 >= rows) return;
+    const int base = e.n0 + e.half * kCols, row = e.m0 + e.lane;
+    const float by = kF32 ? 1.f : scale->out;
+    const bool zero = !kF32 && target && row < rows && !row_counts(target[row], ignore);
+#pragma unroll 1
+    for (int c = 0; c < kCols; c += kBlock) {
+      if (base + c >= cols) break;
+      if (e.lane == 0) tma_store_wait_read<0>();
+      __syncwarp();
+#pragma unroll
+      for (int h = 0; h < kBlock; h += 32) {
+        uint32_t r[32];
+        tmem_ld32(e.acc + e.half * kCols + c + h, r);
+        tmem_wait_ld();
+        if constexpr (kF32) {
+#pragma unroll
+          for (int p = 0; p < 8; ++p)
+            *reinterpret_cast<uint4*>(e.stg + e.lane * 128 + ((p ^ (e.lane & 7)) << 4)) = make_uint4(r[4 * p], r[4 * p + 1], r[4 * p + 2], r[4 * p + 3]);
+        } else {
+#pragma unroll
+          for (int p = 0; p < 4; ++p) {
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = zero ? 0.f : by * __uint_as_float(r[8 * p + j]);
+            uint4 o;
+            if (f16)
+              o = make_uint4(pack_f16x2_inf(v[0], v[1]), pack_f16x2_inf(v[2], v[3]), pack_f16x2_inf(v[4], v[5]), pack_f16x2_inf(v[6], v[7]));
+            else
+              o = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+            *reinterpret_cast<uint4*>(e.stg + e.lane * 128 + (((h / 8 + p) ^ (e.lane & 7)) << 4)) = o;
+          }
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+      __syncwarp();
+      if (e.lane == 0) {
+        if (kF32 && add)
+          asm volatile("cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.bulk_group [%0, {%2, %3, %4}], [%1];\n"
+                       ::"l"(reinterpret_cast<uint64_t>(&out)), "r"(smem_u32(e.stg)), "r"(base + c), "r"(e.m0), "r"(e.at.split)
+                       : "memory");
+        else
+          tma_store_3d(&out, smem_u32(e.stg), base + c, e.m0, e.at.split);
+        tma_store_commit();
+      }
+    }
+  }
+};
+
+// The splits' sums in their order, scaled and rounded.
+__global__ void __launch_bounds__(256) loss_gather_kernel(const float* __restrict__ slots, uint16_t* __restrict__ out, const LossScale* __restrict__ scale,
+                                                          const int64_t* __restrict__ target, int64_t ignore, int64_t rows, int c, int splits, bool f16) {
+  pdl_wait();
+  const int64_t all = rows * c / 4;
+  const float by = scale->out;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = 0; k < splits; ++k) {
+      const float4 v = *reinterpret_cast<const float4*>(slots + (int64_t)k * rows * c + 4 * i);
+      s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+    }
+    s.x *= by, s.y *= by, s.z *= by, s.w *= by;
+    if (target && !row_counts(target[4 * i / c], ignore)) s = make_float4(0.f, 0.f, 0.f, 0.f);
+    reinterpret_cast<uint2*>(out)[i] = f16 ? make_uint2(pack_f16x2_inf(s.x, s.y), pack_f16x2_inf(s.z, s.w)) : make_uint2(pack_bf16x2(s.x, s.y), pack_bf16x2(s.z, s.w));
+  }
+}
+
+PX_DEFINE_FAMILY_HOOKS(loss)
+
+// ---- host ------------------------------------------------------------------------------------------------------------
+static int64_t up(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
+
+// Shapes of the products: logits (both operands along k), dx (W across), dW (both across).
+typedef GemmShape<1, 64, 1, false, false, 6> Logits64;
+typedef GemmShape<1, 256, 1, false, false, 4> Logits256;
+typedef GemmShape<2, 256, 1, false, false, 5> LogitsPair;
+typedef GemmShape<1, 128, 1, false, true, 5> Dx128;
+typedef GemmShape<1, 256, 1, false, true, 4> Dx256;
+typedef GemmShape<2, 256, 1, false, true, 5> DxPair;
+typedef GemmShape<1, 128, 1, true, true, 5> Dw128;
+typedef GemmShape<1, 256, 1, true, true, 4> Dw256;
+typedef GemmShape<2, 256, 1, true, true, 5> DwPair;
+
+// A product's tiles, and the parts that a long axis is cut into where its tiles are fewer than the SMs.
+struct HeadCut {
+  int ctas, kn;
+  GemmTiles t;
+};
+static HeadCut cut(int64_t m, int64_t n, int64_t k, bool split, int narrow) {
+  HeadCut c;
+  const int64_t sms = sm_count();
+  c.kn = n <= narrow ? narrow : 256;
+  c.ctas = c.kn == 256 && m > 128 && up(m, 256) / 256 * (up(n, 256) / 256) >= sms ? 2 : 1;
+  c.t = {};
+  c.t.tiles_m = (int)(up(m, 128 * c.ctas) / (128 * c.ctas)), c.t.tiles_n = (int)(up(n, c.kn) / c.kn);
+  c.t.batch = 1, c.t.splits = 1, c.t.group = 8;
+  c.t.nk = c.t.nk_split = (int)(up(k, kGemmK) / kGemmK);
+  const int64_t tiles = (int64_t)c.t.tiles_m * c.t.tiles_n;
+  if (split && tiles * 2 <= sms) {
+    int64_t s = std::min<int64_t>(sms / tiles, c.t.nk / 4);      // at least four steps each
+    if (s > 1) {
+      c.t.nk_split = (int)((c.t.nk + s - 1) / s);
+      c.t.splits = (c.t.nk + c.t.nk_split - 1) / c.t.nk_split;
+    }
+  }
+  return c;
+}
+
+struct HeadPlan {
+  int64_t piece, pieces, ld;               // classes of a piece, row stride of dl
+  HeadCut logits, dx, dw;
+  bool dx_slots;
+  int64_t scale, found, clean, dl, dx_at, dw_at, db_at, bytes;
+};
+static HeadPlan head_plan(const px_head& h, bool want_dx, bool want_dw, bool want_db) {
+  HeadPlan p;
+  int64_t most = std::max<int64_t>(256, kPieceBytes / (2 * h.rows) / 256 * 256);
+  p.pieces = (h.classes + most - 1) / most;
+  p.piece = p.pieces == 1 ? h.classes : up((h.classes + p.pieces - 1) / p.pieces, 256);
+  p.pieces = (h.classes + p.piece - 1) / p.piece;
+  p.ld = up(p.piece, 8);
+  p.logits = cut(h.rows, p.piece, h.c, false, 64);
+  p.dx = cut(h.rows, h.c, p.piece, true, 128);
+  p.dw = cut(p.piece, h.c, h.rows, true, 128);
+  p.dx_slots = p.dx.t.splits > 1 || p.pieces > 1;
+  int64_t at = 0;
+  const auto take = [&](int64_t bytes) {
+    const int64_t here = at;
+    at += up(bytes, 1024);
+    return here;
+  };
+  p.scale = take(sizeof(LossScale));
+  p.found = take(kScanBlocks * sizeof(uint2));
+  p.clean = take(want_dw ? h.rows * h.c * 2 : 0);
+  p.dl = take(h.rows * p.ld * 2);
+  p.dx_at = take(want_dx && p.dx_slots ? p.dx.t.splits * h.rows * h.c * 4 : 0);
+  p.dw_at = take(want_dw && p.dw.t.splits > 1 ? p.dw.t.splits * p.piece * h.c * 4 : 0);
+  p.db_at = take(want_db ? up(h.rows, 32) / 32 * p.piece * 4 : 0);
+  p.bytes = at;
+  return p;
+}
+
+static int32_t check_head(const px_head* h) {
+  if (!h || h->rows < 0 || h->c <= 0 || h->classes <= 0) return PX_ERR_BAD_ARG;
+  if (h->rows == 0) return PX_OK;
+  if (!h->x || !h->w || !h->target || h->x_stride < h->c || h->w_stride < h->c || h->x_stride % 8 || h->w_stride % 8) return PX_ERR_BAD_ARG;
+  if (((uintptr_t)h->x | (uintptr_t)h->w | (uintptr_t)h->bias) & 15) return PX_ERR_BAD_ARG;
+  if (!(h->smoothing >= 0.f && h->smoothing <= 1.f)) return PX_ERR_BAD_ARG;
+  if ((h->dtype != PX_BF16 && h->dtype != PX_F16) || h->c % 8 || h->c > (1 << 20) || h->classes > (1 << 24) || h->rows > (1 << 26)) return PX_ERR_UNSUPPORTED;
+  if (up(h->rows, 128) / 128 * (up(h->classes, 64) / 64) > (1ll << 30)) return PX_ERR_UNSUPPORTED;
+  return PX_OK;
+}
+// boxes of 32 rows of 128 bytes of a result
+static bool out_map(CUtensorMap* map, CUtensorMapDataType type, int size, const void* base, int64_t cols, int64_t rows, int64_t ld, int64_t slots) {
+  return make_map_3d(map, type, base, (uint64_t)cols, (uint64_t)rows, (uint64_t)slots, (uint64_t)ld * size, (uint64_t)rows * ld * size, 128 / size, 32,
+                     CU_TENSOR_MAP_SWIZZLE_128B);
+}
+static CUtensorMapDataType type16(bool f16) { return f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16; }
+
+// rows of x against `classes` rows of w from class `first` on
+template <class Epi>
+static int32_t launch_logits(const px_head& h, int64_t first, int64_t classes, const HeadCut& c, const Epi& epi, cudaStream_t st) {
+  const bool f16 = h.dtype == PX_F16;
+  GemmOperands ops = {};
+  if (!gemm_map(&ops.a, f16, h.x, h.c, h.rows, 1, h.x_stride, h.rows * h.x_stride, kGemmM) ||
+      !gemm_map(&ops.b, f16, (const uint16_t*)h.w + first * h.w_stride, h.c, classes, 1, h.w_stride, classes * h.w_stride, c.kn / c.ctas))
+    return PX_ERR_LAUNCH;
+  GemmTiles t = c.t;
+  t.tiles_n = (int)(up(classes, c.kn) / c.kn);
+  if (c.kn == 64) return ops.idesc = Logits64::idesc(f16), gemm_launch<Logits64>(ops, epi, t, st);
+  if (c.ctas == 1) return ops.idesc = Logits256::idesc(f16), gemm_launch<Logits256>(ops, epi, t, st);
+  return ops.idesc = LogitsPair::idesc(f16), gemm_launch<LogitsPair>(ops, epi, t, st);
+}
+template <class N, class W, class P, class Epi>
+static int32_t launch_grad(GemmOperands& ops, bool f16, const HeadCut& c, const Epi& epi, const GemmTiles& t, cudaStream_t st) {
+  if (c.kn == 128) return ops.idesc = N::idesc(f16), gemm_launch<N>(ops, epi, t, st);
+  if (c.ctas == 1) return ops.idesc = W::idesc(f16), gemm_launch<W>(ops, epi, t, st);
+  return ops.idesc = P::idesc(f16), gemm_launch<P>(ops, epi, t, st);
+}
+static int32_t gather(const float* slots, void* out, const LossScale* scale, const int64_t* target, int64_t ignore, int64_t rows, int64_t c, int splits, bool f16, cudaStream_t st) {
+  const int64_t blocks = std::min<int64_t>((rows * c / 4 + 255) / 256, 8 * sm_count());
+  return launch_pdl(loss_gather_kernel, dim3((unsigned)blocks), 256, 0, st, slots, (uint16_t*)out, scale, target, ignore, rows, (int)c, splits, f16) ? PX_OK : PX_ERR_LAUNCH;
+}
+
+}  // namespace px
+
+using namespace px;
+
+extern "C" int64_t px_head_loss_workspace_bytes(int64_t rows, int64_t classes) {
+  if (rows <= 0 || classes <= 0) return 0;
+  const int64_t tiles = up(classes, classes <= 64 ? 64 : 256) / (classes <= 64 ? 64 : 256);
+  return 1024 + up(rows * 4, 1024) + up((rows + 31) / 32 * 16, 1024) + up(tiles * rows * 8, 1024) + up(tiles * rows * 4, 1024);
+}
+
+extern "C" int32_t px_head_loss_fwd(const px_head* head, float* norm, float* losses, float* total, float* inverse, int32_t mean, void* workspace,
+                                    int64_t workspace_bytes, void* stream) {
+  if (const int32_t status = check_head(head)) return status;
+  const px_head& h = *head;
+  if (!losses && !total) return PX_ERR_BAD_ARG;
+  if (h.rows == 0) return PX_ERR_BAD_ARG;
+  if (!norm || (total && !inverse) || !workspace || ((uintptr_t)workspace & 255) || ((uintptr_t)norm & 15)) return PX_ERR_BAD_ARG;
+  if (workspace_bytes < px_head_loss_workspace_bytes(h.rows, h.classes)) return PX_ERR_WORKSPACE;
+  if (!have_context()) return PX_ERR_LAUNCH;
+  const cudaStream_t st = (cudaStream_t)stream;
+  const HeadCut c = cut(h.rows, h.classes, h.c, false, 64);
+  char* at = (char*)workspace;
+  uint32_t* arrivals = (uint32_t*)at;
+  at += 1024;
+  float* hit = (float*)at;
+  at += up(h.rows * 4, 1024);
+  double2* sums = (double2*)at;
+  at += up((h.rows + 31) / 32 * 16, 1024);
+  float2* part = (float2*)at;
+  at += up(c.t.tiles_n * h.rows * 8, 1024);
+  EpiStats epi = {h.target, h.bias, part, h.smoothing > 0.f ? (float*)at : nullptr, hit, arrivals, (int)h.rows, (int)h.classes};
+  if (const int32_t status = launch_logits(h, 0, h.classes, c, epi, st)) return status;
+  JoinArgs j = {part, epi.part_sum, hit, h.target, (float2*)norm, losses, total, inverse, sums, arrivals, h.ignore, (int)h.rows, (int)h.classes, c.t.tiles_n, mean, h.smoothing};
+  return launch_pdl(loss_join_kernel, dim3((unsigned)((h.rows + 31) / 32)), 32 * kJoinWarps, 0, st, j) ? PX_OK : PX_ERR_LAUNCH;
+}
+
+extern "C" int64_t px_head_loss_bwd_workspace_bytes(const px_head* head, int32_t dx, int32_t dw, int32_t dbias) {
+  if (!head || head->rows <= 0 || head->c <= 0 || head->classes <= 0) return 0;
+  return head_plan(*head, dx, dw, dbias).bytes;
+}
+
+extern "C" int32_t px_head_loss_bwd(const px_head* head, const float* norm, const float* grad, int32_t each, const float* inverse, void* dx, void* dw,
+                                    float* dbias, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (const int32_t status = check_head(head)) return status;
+  const px_head& h = *head;
+  if (h.rows == 0 || !norm || !grad || (!each && !inverse) || !workspace || ((uintptr_t)workspace & 255)) return PX_ERR_BAD_ARG;
+  if (((uintptr_t)dx | (uintptr_t)dw | (uintptr_t)norm) & 15) return PX_ERR_BAD_ARG;
+  const HeadPlan p = head_plan(h, dx, dw, dbias);
+  if (workspace_bytes < p.bytes) return PX_ERR_WORKSPACE;
+  if (!have_context()) return PX_ERR_LAUNCH;
+  if (!dx && !dw && !dbias) return PX_OK;
+  const cudaStream_t st = (cudaStream_t)stream;
+  const bool f16 = h.dtype == PX_F16;
+  char* const ws = (char*)workspace;
+  LossScale* scale = (LossScale*)(ws + p.scale);
+  uint16_t* dl = (uint16_t*)(ws + p.dl);
+  uint16_t* clean = (uint16_t*)(ws + p.clean);
+  float* part_bias = (float*)(ws + p.db_at);
+  const ScanArgs scan = {h.x, h.x_stride, h.target, grad, (uint2*)(ws + p.found), h.ignore, h.rows, dw ? (int)h.c : 0, each};
+  const int scan_blocks = (int)std::min<int64_t>((h.rows + 255) / 256, kScanBlocks);
+  if (!launch_pdl(loss_scan_kernel, dim3(scan_blocks), 256, 0, st, scan, f16)) return PX_ERR_LAUNCH;
+  const int copy_blocks = dw ? (int)std::min<int64_t>((h.rows * h.c / 8 + 255) / 256, 2 * sm_count()) : 1;
+  if (!launch_pdl(loss_prepare_kernel, dim3(copy_blocks), 256, 0, st, scan, inverse, clean, scale, scan_blocks, f16 ? kDlScaleF16 : 1.f)) return PX_ERR_LAUNCH;
+
+  for (int64_t i = 0; i < p.pieces; ++i) {
+    const int64_t first = i * p.piece, vc = std::min(p.piece, h.classes - first);
+    EpiLogitGrad el = {};
+    if (!out_map(&el.out, type16(f16), 2, dl, vc, h.rows, p.ld, 1)) return PX_ERR_LAUNCH;
+    el.target = h.target, el.bias = h.bias ? h.bias + first : nullptr, el.norm = (const float2*)norm, el.grad = each ? grad : nullptr, el.scale = scale;
+    el.part_bias = dbias ? part_bias : nullptr, el.ignore = h.ignore, el.rows = (int)h.rows, el.classes = (int)vc, el.first = (int)first;
+    el.all_classes = (int)h.classes, el.smooth = h.smoothing, el.f16 = f16;
+    if (const int32_t status = launch_logits(h, first, vc, p.logits, el, st)) return status;
+    if (dbias && !launch_pdl(loss_bias_kernel, dim3((unsigned)((vc + 31) / 32)), 512, 0, st, (const float*)part_bias, dbias + first, (const LossScale*)scale, (int)vc,
+                             (int)((h.rows + 31) / 32)))
+      return PX_ERR_LAUNCH;
+    if (dx) {
+      GemmOperands ops = {};
+      if (!gemm_map(&ops.a, f16, dl, vc, h.rows, 1, p.ld, h.rows * p.ld, kGemmM) ||
+          !gemm_map(&ops.b, f16, (const uint16_t*)h.w + first * h.w_stride, h.c, vc, 1, h.w_stride, vc * h.w_stride, kGemmK))
+        return PX_ERR_LAUNCH;
+      GemmTiles t = p.dx.t;
+      t.nk = (int)(up(vc, kGemmK) / kGemmK);
+      if (t.splits == 1) t.nk_split = t.nk;
+      // a last piece may be too short for all splits: the ones that it has leave the others' sums as they are
+      t.splits = (t.nk + t.nk_split - 1) / t.nk_split;
+      int32_t status;
+      if (p.dx_slots) {
+        EpiGrad<true> ep = {};
+        if (!out_map(&ep.out, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, ws + p.dx_at, h.c, h.rows, h.c, p.dx.t.splits)) return PX_ERR_LAUNCH;
+        ep.rows = (int)h.rows, ep.cols = (int)h.c, ep.add = i > 0;
+        status = launch_grad<Dx128, Dx256, DxPair>(ops, f16, p.dx, ep, t, st);
+      } else {
+        EpiGrad<false> ep = {};
+        if (!out_map(&ep.out, type16(f16), 2, dx, h.c, h.rows, h.c, 1)) return PX_ERR_LAUNCH;
+        ep.scale = scale, ep.target = h.target, ep.ignore = h.ignore, ep.rows = (int)h.rows, ep.cols = (int)h.c, ep.f16 = f16;
+        status = launch_grad<Dx128, Dx256, DxPair>(ops, f16, p.dx, ep, t, st);
+      }
+      if (status) return status;
+    }
+    if (dw) {
+      uint16_t* to = (uint16_t*)dw + first * h.c;
+      GemmOperands ops = {};
+      if (!gemm_map(&ops.a, f16, dl, vc, h.rows, 1, p.ld, h.rows * p.ld, kGemmK) || !gemm_map(&ops.b, f16, h.x, h.c, h.rows, 1, h.x_stride, h.rows * h.x_stride, kGemmK) ||
+          !gemm_map(&ops.b_other, f16, clean, h.c, h.rows, 1, h.c, h.rows * h.c, kGemmK))
+        return PX_ERR_LAUNCH;
+      ops.other = &scale->dirty;
+      GemmTiles t = p.dw.t;
+      t.tiles_m = (int)(up(vc, 128 * p.dw.ctas) / (128 * p.dw.ctas));
+      int32_t status;
+      if (t.splits > 1) {
+        EpiGrad<true> ep = {};
+        if (!out_map(&ep.out, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, ws + p.dw_at, h.c, vc, h.c, t.splits)) return PX_ERR_LAUNCH;
+        ep.rows = (int)vc, ep.cols = (int)h.c;
+        status = launch_grad<Dw128, Dw256, DwPair>(ops, f16, p.dw, ep, t, st);
+        if (!status) status = gather((const float*)(ws + p.dw_at), to, scale, nullptr, 0, vc, h.c, t.splits, f16, st);
+      } else {
+        EpiGrad<false> ep = {};
+        if (!out_map(&ep.out, type16(f16), 2, to, h.c, vc, h.c, 1)) return PX_ERR_LAUNCH;
+        ep.scale = scale, ep.rows = (int)vc, ep.cols = (int)h.c, ep.f16 = f16;
+        status = launch_grad<Dw128, Dw256, DwPair>(ops, f16, p.dw, ep, t, st);
+      }
+      if (status) return status;
+    }
+  }
+  if (dx && p.dx_slots) return gather((const float*)(ws + p.dx_at), dx, scale, h.target, h.ignore, h.rows, h.c, p.dx.t.splits, f16, st);
+  return PX_OK;
+}

@@ -1,4 +1,5 @@
-// The host path of the training operators: dropout-add from a counter-based generator, relative position encoding, windowed attention.
+// The host path of the training operators: dropout-add from a counter-based generator, relative position encoding, windowed attention,
+// cross entropy of a linear head.
 // Part of torch_ext.cpp (inside its unnamed namespace).  Each is an autograd function whose two directions are launches of the
 // C ABI.  Gradients are computed in kernels, so the ones that are not linear in what they differentiate have no second derivative: a
 // backward pass that is asked to build a graph is refused.
@@ -320,4 +321,130 @@ Tensor window_attention(const Tensor& q, const Tensor& k, const Tensor& v, int64
     o = window_forward(rows_fitted(q4), rows_fitted(k4), rows_fitted(v4), b, m.has_value() ? *m : Tensor(), {left, right, sinks, scale}, nullptr, nullptr);
   }
   return q.dim() == 4 ? o : o.reshape(q.sizes());
+}
+
+// ---- cross entropy of a linear head ----------------------------------------------------------------------------------
+struct HeadCall {
+  int64_t ignore;
+  double smoothing;
+  int64_t reduction;      // 0: a loss for each row, 1: mean, 2: sum
+};
+
+// [rows, C] as the kernels address it: rows of neighbouring elements that do not overlap, 16-byte aligned.
+Tensor matrix_fitted(const Tensor& t) {
+  const bool fits = (t.size(1) <= 1 || t.stride(1) == 1) && (t.size(0) <= 1 || (t.stride(0) >= t.size(1) && t.stride(0) % 8 == 0));
+  return fits && ((uintptr_t)t.data_ptr() & 15) == 0 ? t : aligned(t);
+}
+int64_t row_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+px_head head_of(const Tensor& x, const Tensor& w, const Tensor& bias, const Tensor& target, const HeadCall& c) {
+  px_head h = {};
+  h.x = x.data_ptr(), h.w = w.data_ptr(), h.target = (const int64_t*)target.data_ptr();
+  h.bias = bias.defined() ? (const float*)bias.data_ptr() : nullptr;
+  h.rows = x.size(0), h.c = x.size(1), h.classes = w.size(0);
+  h.x_stride = row_stride(x), h.w_stride = row_stride(w);
+  h.ignore = c.ignore, h.smoothing = (float)c.smoothing, h.dtype = dtype_code(x, "x");
+  return h;
+}
+// The loss; norm and inverse receive what the backward pass reads.
+Tensor head_loss_forward(const Tensor& x, const Tensor& w, const Tensor& bias, const Tensor& target, const HeadCall& c, Tensor& norm, Tensor& inverse) {
+  const px_head h = head_of(x, w, bias, target, c);
+  const auto f32 = x.options().dtype(at::kFloat);
+  const Tensor loss = c.reduction ? at::empty({}, f32) : at::empty({h.rows}, f32);
+  norm = at::empty({h.rows, 2}, f32);
+  if (c.reduction) inverse = at::empty({}, f32);
+  const int64_t bytes = abi.px_head_loss_workspace_bytes(h.rows, h.classes);
+  const Tensor ws = bytes_like(x, bytes);
+  const cudaStream_t st = at::cuda::getCurrentCUDAStream();
+  launch("px_head_loss_fwd", st, [&] {
+    return abi.px_head_loss_fwd(&h, (float*)norm.data_ptr(), c.reduction ? nullptr : (float*)loss.data_ptr(), c.reduction ? (float*)loss.data_ptr() : nullptr,
+                                c.reduction ? (float*)inverse.data_ptr() : nullptr, c.reduction == 1, ws.data_ptr(), bytes, st);
+  });
+  return loss;
+}
+
+struct HeadLossFunction : torch::autograd::Function<HeadLossFunction> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x_, const Tensor& w_, const OptTensor& bias_, const Tensor& target,
+                        int64_t ignore, double smoothing, int64_t reduction) {
+    c10::cuda::CUDAGuard guard(x_.device());
+    const Tensor x = matrix_fitted(x_), w = matrix_fitted(w_), bias = has(bias_) ? aligned(bias_->to(at::kFloat)) : Tensor();
+    Tensor norm, inverse;
+    const Tensor loss = head_loss_forward(x, w, bias, target, {ignore, smoothing, reduction}, norm, inverse);
+    ctx->save_for_backward({x, w, bias, target, norm, inverse});
+    ctx->saved_data["ignore"] = ignore;
+    ctx->saved_data["smoothing"] = smoothing;
+    ctx->saved_data["reduction"] = reduction;
+    ctx->saved_data["bias"] = (int64_t)(has(bias_) ? bias_->scalar_type() : at::kFloat);
+    ctx->saved_data["f"] = (int64_t)x_.requires_grad() | (int64_t)w_.requires_grad() << 1 | (int64_t)(has(bias_) && bias_->requires_grad()) << 2;
+    return loss;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    first_derivative_only("linear_cross_entropy");
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &w = saved[1], &bias = saved[2], &target = saved[3], &norm = saved[4], &inverse = saved[5];
+    c10::cuda::CUDAGuard guard(x.device());
+    const int64_t f = ctx->saved_data["f"].toInt(), reduction = ctx->saved_data["reduction"].toInt();
+    const px_head h = head_of(x, w, bias, target, {ctx->saved_data["ignore"].toInt(), ctx->saved_data["smoothing"].toDouble(), reduction});
+    const Tensor g = grads[0].to(at::kFloat).contiguous();
+    Tensor dx, dw, db;
+    if (f & 1) dx = at::empty({h.rows, h.c}, x.options());
+    if (f & 2) dw = at::empty({h.classes, h.c}, w.options());
+    if (f & 4) db = at::empty({h.classes}, x.options().dtype(at::kFloat));
+    const int64_t bytes = abi.px_head_loss_bwd_workspace_bytes(&h, f & 1, f >> 1 & 1, f >> 2 & 1);
+    const Tensor ws = bytes_like(x, bytes);
+    const cudaStream_t st = at::cuda::getCurrentCUDAStream();
+    launch("px_head_loss_bwd", st, [&] {
+      return abi.px_head_loss_bwd(&h, (const float*)norm.data_ptr(), (const float*)g.data_ptr(), reduction == 0, reduction ? (const float*)inverse.data_ptr() : nullptr,
+                                  dx.defined() ? dx.data_ptr() : nullptr, dw.defined() ? dw.data_ptr() : nullptr, db.defined() ? (float*)db.data_ptr() : nullptr,
+                                  ws.data_ptr(), bytes, st);
+    });
+    if (db.defined()) db = db.to((at::ScalarType)ctx->saved_data["bias"].toInt());
+    return {dx, dw, db, Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Tensor linear_cross_entropy(const Tensor& x, const Tensor& weight, const Tensor& target, const OptTensor& bias, int64_t ignore, double smoothing,
+                            const std::string& reduction) {
+  need_cuda(x, "x");
+  if (x.scalar_type() != at::kBFloat16 && x.scalar_type() != at::kHalf) fail("x and weight must be bfloat16 or float16");
+  need_on(weight, x.device(), "weight");
+  need_on(target, x.device(), "target");
+  if (weight.scalar_type() != x.scalar_type()) fail("weight must have the type of x");
+  if (x.dim() < 1 || weight.dim() != 2 || weight.size(1) != x.size(-1)) fail("x must be [..., C] and weight [V, C], got " + shape_of(x) + " and " + shape_of(weight));
+  const int64_t c = x.size(-1), classes = weight.size(0);
+  if (classes < 1 || classes > (1 << 24) || c < 8 || c % 8 != 0 || c > (1 << 20))
+    fail("the kernels handle 1 to 2^24 classes and a multiple of 8 channels up to 2^20, got a weight of " + shape_of(weight));
+  if (!at::isIntegralType(target.scalar_type(), false)) fail("target must be an integer tensor");
+  if (!target.sizes().equals(x.sizes().slice(0, x.dim() - 1))) fail("target must be [...] for x [..., C], got " + shape_of(target) + " and " + shape_of(x));
+  if (!(smoothing >= 0.0 && smoothing <= 1.0)) fail("label_smoothing must lie in [0, 1]");
+  const int64_t how = reduction == "none" ? 0 : reduction == "mean" ? 1 : reduction == "sum" ? 2 : -1;
+  if (how < 0) fail("reduction must be 'none', 'mean' or 'sum', got '" + reduction + "'");
+  if (has(bias)) {
+    need_on(*bias, x.device(), "bias");
+    if (bias->dim() != 1 || bias->size(0) != classes) fail("bias must be [V], got " + shape_of(*bias));
+    if (bias->scalar_type() != at::kFloat && bias->scalar_type() != x.scalar_type()) fail("bias must be float32 or of the type of x");
+  }
+  const int64_t rows = target.numel();
+  if (rows > (1 << 26) || (rows + 127) / 128 * ((classes + 63) / 64) > (1ll << 30)) fail("at most 2^26 rows, and 2^43 logits");
+  no_tangent(x, "x");
+  no_tangent(weight, "weight");
+  if (has(bias)) no_tangent(*bias, "bias");
+  c10::cuda::CUDAGuard guard(x.device());
+  const auto wants = [](const Tensor& t) { return t.requires_grad(); };
+  const bool train = at::GradMode::is_enabled() && (wants(x) || wants(weight) || (has(bias) && wants(*bias)));
+  if (rows == 0) {      // nothing to launch: what the formula gives, with gradients of zero
+    Tensor rest = weight.slice(0, 0, 0).to(at::kFloat).sum();
+    if (has(bias)) rest = rest + bias->slice(0, 0, 0).to(at::kFloat).sum();
+    const Tensor each = x.to(at::kFloat).sum(-1) + rest;
+    return how == 0 ? each : how == 1 ? each.sum() / 0.0 : each.sum();
+  }
+  const Tensor x2 = x.reshape({rows, c});
+  const Tensor t = target.detach().to(at::kLong).reshape({rows}).contiguous();
+  Tensor loss;
+  if (train) {
+    loss = HeadLossFunction::apply(x2, weight, bias, t, ignore, smoothing, how);
+  } else {
+    Tensor norm, inverse;
+    loss = head_loss_forward(matrix_fitted(x2), matrix_fitted(weight), has(bias) ? aligned(bias->to(at::kFloat)) : Tensor(), t, {ignore, smoothing, how}, norm, inverse);
+  }
+  return how == 0 ? loss.reshape(target.sizes()) : loss;
 }
