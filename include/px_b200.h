@@ -449,6 +449,23 @@ PX_API int32_t px_window_bwd(const px_window* w, const px_rows* q, const px_rows
                       const px_rows* dout, const float* lse, const px_rows* dq, const px_rows* dk, const px_rows* dv, void* dbias, void* workspace,
                       int64_t workspace_bytes, void* stream);
 
+/* ---- Rotary positions of several axes ------------------------------------------------------------
+ * Pair j of a head of q [batch][heads][n][d] and k [batch][kv_heads][n][d] turns by positions[batch][row][axis of j] * base^-e: channels (j, j + pairs), or
+ * (2 j, 2 j + 1) if interleaved, pairs = the sum of `sections` (the number of pairs of each axis, in their order, on the host), at most d / 2 and 256; the
+ * channels behind them stay as they are.  e = j / pairs, or (per_axis) the pair's place in its section over the section's length.  inverse: by the negated angles
+ * (the gradient).  Angles are exact modulo a turn for every int64 position; products are fp32, rounded once.  PX_F32, PX_BF16 or PX_F16; strides in elements, of
+ * outputs as of inputs (inputs may repeat rows by strides of zero); 16-byte accesses where strides, pointers and `pairs` allow them.  k NULL with kv_heads 0: q alone.
+ * No counterpart in the reference, whose attention takes positions as a bias of pairs. */
+typedef struct {
+  const int64_t* positions;
+  int64_t position_batch, position_row, position_axis; /* strides in elements */
+  int64_t batch, heads, kv_heads, n, d;
+  const int32_t* sections;
+  double base; /* 1 to 1e30 */
+  int32_t axes, interleaved, per_axis, dtype;
+} px_rotary;
+PX_API int32_t px_rotary_turn(const px_rotary* r, const px_rows* q, const px_rows* q_out, const px_rows* k, const px_rows* k_out, int32_t inverse, void* stream);
+
 /* ---- Softmax cross entropy of a linear head, without its logits (training path) ----------------
  * l = x w^T + bias for rows x [rows][c] and classes w [classes][c] (PX_BF16 or PX_F16, row strides in elements), bias fp32 or NULL;
  * loss_i = lse_i - (1 - smoothing) l_i,target - smoothing / classes sum_v l_iv.  Rows whose target is `ignore` have loss 0 and take no part in

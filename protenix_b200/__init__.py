@@ -8,6 +8,7 @@ from .msa import OuterProductMean
 from .pairformer import PairformerBlock, PairformerStack
 from .primitives import Linear, LinearNoBias, Transition
 from .recycling import RecyclingTrunk
+from .rotary import rotary_embedding
 from .transformer import AttentionPairBias
 from .triangular import (OpenfoldLinear, TriangleAttention, TriangleAttentionEndingNode,
                          TriangleAttentionStartingNode, TriangleMultiplicationIncoming,
@@ -22,6 +23,6 @@ __all__ = [
     "TriangleAttentionStartingNode", "TriangleMultiplicationIncoming", "TriangleMultiplicationOutgoing",
     "TriangleMultiplicativeUpdate", "dropout_add_rowwise", "RecyclingTrunk", "OuterProductMean",
     "weights_changed", "dropout_add", "RelativePositionEncoding", "relative_position_encoding",
-    "window_attention", "linear_cross_entropy",
+    "window_attention", "linear_cross_entropy", "rotary_embedding",
 ]
 __version__ = "0.1.0"

@@ -1,5 +1,5 @@
 // The host path of the training operators: dropout-add from a counter-based generator, relative position encoding, windowed attention,
-// cross entropy of a linear head.
+// cross entropy of a linear head, rotary positions.
 // Part of torch_ext.cpp (inside its unnamed namespace).  Each is an autograd function whose two directions are launches of the
 // C ABI.  Gradients are computed in kernels, so the ones that are not linear in what they differentiate have no second derivative: a
 // backward pass that is asked to build a graph is refused.
@@ -447,4 +447,113 @@ Tensor linear_cross_entropy(const Tensor& x, const Tensor& weight, const Tensor&
     loss = head_loss_forward(matrix_fitted(x2), matrix_fitted(weight), has(bias) ? aligned(bias->to(at::kFloat)) : Tensor(), t, {ignore, smoothing, how}, norm, inverse);
   }
   return how == 0 ? loss.reshape(target.sizes()) : loss;
+}
+
+// ---- rotary positions ------------------------------------------------------------------------------------------------
+struct RotaryCall {
+  std::vector<int64_t> sections;
+  double base;
+  bool interleaved, per_axis, inverse;
+};
+typedef std::pair<Tensor, Tensor> TwoTensors;
+
+Tensor channels_fitted(const Tensor& t) { return t.size(3) <= 1 || t.stride(3) == 1 ? t : t.contiguous(); }
+// q and k [B, H, N, D] turned (k undefined: q alone); positions [B, N, A], int64, any strides.
+TwoTensors rotary_launch(const Tensor& q_, const Tensor& k_, const Tensor& positions, const RotaryCall& c) {
+  c10::cuda::CUDAGuard guard(q_.device());
+  const Tensor q = channels_fitted(q_), k = k_.defined() ? channels_fitted(k_) : k_;
+  const Tensor qo = rows_like(q), ko = k.defined() ? rows_like(k) : k;
+  const std::vector<int32_t> sections(c.sections.begin(), c.sections.end());
+  px_rotary r = {};
+  r.positions = (const int64_t*)positions.data_ptr();
+  r.position_batch = positions.stride(0), r.position_row = positions.stride(1), r.position_axis = positions.stride(2);
+  r.batch = q.size(0), r.heads = q.size(1), r.kv_heads = k.defined() ? k.size(1) : 0, r.n = q.size(2), r.d = q.size(3);
+  r.sections = sections.data(), r.axes = (int32_t)sections.size(), r.base = c.base;
+  r.interleaved = c.interleaved, r.per_axis = c.per_axis, r.dtype = dtype_code(q, "q");
+  const px_rows iq = rows_of(q), oq = rows_of(qo), ik = k.defined() ? rows_of(k) : px_rows{}, ok = k.defined() ? rows_of(ko) : px_rows{};
+  const cudaStream_t st = at::cuda::getCurrentCUDAStream();
+  launch("px_rotary_turn", st, [&] { return abi.px_rotary_turn(&r, &iq, &oq, k.defined() ? &ik : nullptr, k.defined() ? &ok : nullptr, c.inverse, st); });
+  return {qo, ko};
+}
+
+TwoTensors rotary_apply(const Tensor& q, const Tensor& k, const Tensor& positions, const RotaryCall& c);
+
+struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const OptTensor& k, const Tensor& positions,
+                                                std::vector<int64_t> sections, double base, bool interleaved, bool per_axis, bool inverse) {
+    ctx->set_materialize_grads(false);
+    const auto out = rotary_launch(q, has(k) ? *k : Tensor(), positions, {sections, base, interleaved, per_axis, inverse});
+    ctx->save_for_backward({positions});
+    ctx->saved_data["sections"] = c10::List<int64_t>(c10::ArrayRef<int64_t>(sections));
+    ctx->saved_data["base"] = base;
+    ctx->saved_data["how"] = (int64_t)interleaved | (int64_t)per_axis << 1 | (int64_t)inverse << 2;
+    ctx->saved_data["f"] = (int64_t)q.requires_grad() | (int64_t)(has(k) && k->requires_grad()) << 1;
+    if (out.second.defined()) return {out.first, out.second};
+    return {out.first};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const int64_t f = ctx->saved_data["f"].toInt(), how = ctx->saved_data["how"].toInt();
+    const Tensor positions = ctx->get_saved_variables()[0];
+    const RotaryCall c = {ctx->saved_data["sections"].toIntVector(), ctx->saved_data["base"].toDouble(), (how & 1) != 0, (how & 2) != 0, (how & 4) == 0};
+    const Tensor gq = f & 1 ? grads[0] : Tensor(), gk = f & 2 && grads.size() > 1 ? grads[1] : Tensor();
+    Tensor dq, dk;      // the operator again, by the negated angles: differentiable like it
+    if (gq.defined() && gk.defined())
+      std::tie(dq, dk) = rotary_apply(gq, gk, positions, c);
+    else if (gq.defined())
+      dq = rotary_apply(gq, Tensor(), positions, c).first;
+    else if (gk.defined())
+      dk = rotary_apply(gk, Tensor(), positions, c).first;
+    return {dq, dk, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+TwoTensors rotary_apply(const Tensor& q, const Tensor& k, const Tensor& positions, const RotaryCall& c) {
+  if (at::GradMode::is_enabled() && (q.requires_grad() || (k.defined() && k.requires_grad()))) {
+    const auto out = RotaryFunction::apply(q, k.defined() ? OptTensor(k) : OptTensor(), positions, c.sections, c.base, c.interleaved, c.per_axis, c.inverse);
+    return {out[0], k.defined() ? out[1] : Tensor()};
+  }
+  return rotary_launch(q, k, positions, c);
+}
+
+py::object rotary_embedding(const Tensor& q, const OptTensor& k, const Tensor& positions, const std::vector<int64_t>& sections, double base,
+                            bool interleaved, bool per_axis) {
+  need_cuda(q, "q");
+  dtype_code(q, "q");
+  if (q.dim() < 3) fail("q must be [..., H, N, D], got " + shape_of(q));
+  const int64_t n = q.size(-2), d = q.size(-1), axes = (int64_t)sections.size();
+  const auto batch_axes = q.sizes().slice(0, q.dim() - 3);
+  if (q.size(-3) < 1 || d < 2 || d > 65536) fail("q must have at least one head and 2 to 65536 channels, got " + shape_of(q));
+  if (has(k)) {
+    need_on(*k, q.device(), "k");
+    if (k->scalar_type() != q.scalar_type()) fail("k must have the type of q");
+    if (k->dim() != q.dim() || k->size(-1) != d || k->size(-2) != n || k->size(-3) < 1 || !k->sizes().slice(0, k->dim() - 3).equals(batch_axes))
+      fail("k must be [..., H_kv, N, D] with the batch axes, N and D of q; got " + shape_of(q) + " and " + shape_of(*k));
+  }
+  need_on(positions, q.device(), "positions");
+  if (!at::isIntegralType(positions.scalar_type(), false)) fail("positions must be an integer tensor");
+  int64_t pairs = 0;
+  for (int64_t s : sections) {
+    if (s < 0 || s > d / 2) fail("sections must be numbers of pairs, from 0 to D / 2");
+    pairs += s;
+  }
+  if (axes < 1 || axes > 255 || pairs < 1 || pairs > 256 || 2 * pairs > d) fail("sections must hold 1 to D / 2 pairs, 256 at most, on up to 255 axes");
+  if (!(base >= 1.0 && base <= 1e30)) fail("base must lie in [1, 1e30]");
+  auto want = batch_axes.vec();
+  want.push_back(n);
+  want.push_back(axes);
+  if (positions.dim() < 2 || positions.size(-1) != axes || !at::is_expandable_to(positions.sizes(), want))
+    fail("positions must be [..., N, A] over the batch axes of q, one axis for each section, got " + shape_of(positions));
+  no_tangent(q, "q");
+  if (has(k)) no_tangent(*k, "k");
+  int64_t batch = 1;
+  for (int64_t b : batch_axes) batch *= b;
+  const int64_t heads = q.size(-3) + (has(k) ? k->size(-3) : 0);
+  if (batch > 65535 || heads > 65536 || n > (1 << 30)) fail("at most 65535 samples, 65536 heads and 2^30 rows");
+  c10::cuda::CUDAGuard guard(q.device());
+  const Tensor p = positions.detach().to(at::kLong).expand(want).reshape({batch, n, axes});
+  const auto four = [&](const Tensor& t) { return t.dim() == 4 ? t : t.reshape({batch, t.size(-3), n, d}); };
+  const auto out = rotary_apply(four(q), has(k) ? four(*k) : Tensor(), p, {sections, base, interleaved, per_axis, false});
+  const auto back = [&](const Tensor& t, const Tensor& like) { return like.dim() == 4 ? t : t.reshape(like.sizes()); };
+  const py::object first = py::cast(back(out.first, q));
+  return has(k) ? py::object(py::make_tuple(first, back(out.second, *k))) : first;
 }
