@@ -160,7 +160,8 @@ PX_API int32_t px_trimul_contract(const px_f16* a, const px_f16* b, px_f16* x, i
 #define PX_FAMILY_RELPOS 16
 #define PX_FAMILY_WINDOW 17
 #define PX_FAMILY_LOSS 18
-#define PX_N_FAMILIES 19 /* grows: give px_device_error_words the size of the array that it fills */
+#define PX_FAMILY_UPDATE 19
+#define PX_N_FAMILIES 20 /* grows: give px_device_error_words the size of the array that it fills */
 #define PX_DETAIL_WORDS 16
 PX_API int32_t px_device_error_flags(uint32_t* flags);
 PX_API int32_t px_device_error_detail(uint32_t* flags, uint32_t* detail);
@@ -492,6 +493,16 @@ PX_API int32_t px_head_loss_fwd(const px_head* head, float* norm, float* losses,
 PX_API int64_t px_head_loss_bwd_workspace_bytes(const px_head* head, int32_t dx, int32_t dw, int32_t dbias);
 PX_API int32_t px_head_loss_bwd(const px_head* head, const float* norm, const float* grad, int32_t each, const float* inverse, void* dx, void* dw,
                          float* dbias, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---- Orthogonalised matrices (Newton-Schulz) ------------------------------------------------------
+ * out = P_steps(... P_1(g / (|g| + eps))) for each of `batch` matrices [m][n], |g| the root of the sum of squares,
+ * P_i(X) = a X + b (X X^T) X + c (X X^T)^2 X with (a, b, c) = coefficients[3 i ..] (on the host).  g and out of one type (PX_F32, PX_BF16, PX_F16), contiguous, out may be g;
+ * 1 to 1000 steps, m and n up to 2^20.  Products take operands of 22 bits (two fp16 planes) and add in fp32, whatever the type; iterates and polynomials may grow to
+ * 60 (an overflow comes out infinite or NaN).  A matrix that is not finite gives NaN and leaves the others alone.  Workspace aligned to 256 bytes.  No
+ * counterpart in the reference. */
+PX_API int64_t px_orthogonalize_workspace_bytes(int64_t batch, int64_t m, int64_t n);
+PX_API int32_t px_orthogonalize(const void* g, void* out, int64_t batch, int64_t m, int64_t n, const float* coefficients, int32_t steps, double eps, int32_t dtype,
+                         void* workspace, int64_t workspace_bytes, void* stream);
 
 /* ---- Exchange between the GPUs of one box (row-sharded path) ------------------------------
  * No counterpart in the reference (which runs the Pairformer on one GPU).  A peer buffer is a

@@ -511,15 +511,15 @@ PX_DEFINE_FAMILY_HOOKS(loss)
 static int64_t up(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
 
 // Shapes of the products: logits (both operands along k), dx (W across), dW (both across).
-typedef GemmShape<1, 64, 1, false, false, 6> Logits64;
-typedef GemmShape<1, 256, 1, false, false, 4> Logits256;
-typedef GemmShape<2, 256, 1, false, false, 5> LogitsPair;
-typedef GemmShape<1, 128, 1, false, true, 5> Dx128;
-typedef GemmShape<1, 256, 1, false, true, 4> Dx256;
-typedef GemmShape<2, 256, 1, false, true, 5> DxPair;
-typedef GemmShape<1, 128, 1, true, true, 5> Dw128;
-typedef GemmShape<1, 256, 1, true, true, 4> Dw256;
-typedef GemmShape<2, 256, 1, true, true, 5> DwPair;
+typedef GemmShape<1, 64, false, false, 6> Logits64;
+typedef GemmShape<1, 256, false, false, 4> Logits256;
+typedef GemmShape<2, 256, false, false, 5> LogitsPair;
+typedef GemmShape<1, 128, false, true, 5> Dx128;
+typedef GemmShape<1, 256, false, true, 4> Dx256;
+typedef GemmShape<2, 256, false, true, 5> DxPair;
+typedef GemmShape<1, 128, true, true, 5> Dw128;
+typedef GemmShape<1, 256, true, true, 4> Dw256;
+typedef GemmShape<2, 256, true, true, 5> DwPair;
 
 // A product's tiles, and the parts that a long axis is cut into where its tiles are fewer than the SMs.
 struct HeadCut {

@@ -1,0 +1,595 @@
+// Newton-Schulz orthogonalisation of matrices: X = G / (|G| + eps), |.| the root of the sum of squares, then for each step
+//   A = X X^T,   X <- (a I + b A + c A^2) X
+// (for tall matrices from the other side: A = X^T X, X <- X (a I + b A + c A^2), the same result without a transposition).  An odd polynomial of the
+// singular values: the steps drive them towards one and leave the singular vectors.
+//
+// Three products a step on the tensor cores (px_gemm.cuh).  Iterates of 16 bits are not enough: the polynomial multiplies small singular values by up
+// to 3.4 a step, and the rounding noise of an iterate with them.  For 384 x 1536 in a simulation the result is off by 1.2e-2 (noise), 0.11 (falling
+// spectrum) and 0.34 (rank 8) with bf16 iterates, 1.5e-3 to 4e-2 with fp16 ones, 7e-6 to 6e-5 with fp32 throughout.  So every
+// operand is two fp16 planes, v = hi + 2^-11 lo (22 bits), and three of the four products are formed: 3e-7 to 8e-6.
+// Values are stored times 2^10 (planes keep their bits down to 2^-34 of an element; iterates and polynomials may grow to 60).
+//
+// A and the polynomial are symmetric: only tiles on and above the diagonal are formed, the epilogue stores each a second time transposed, which
+// saves half of two of the three products.
+#include "px_gemm.cuh"
+
+namespace px {
+
+constexpr float kPlaneScale = 1024.f;
+
+// ---- norm and first iterate ------------------------------------------------------------------------------------------
+constexpr int kNormBlocks = 64;
+template <typename T>
+__global__ void __launch_bounds__(256) ortho_norm_kernel(const T* __restrict__ g, double* __restrict__ sums, int64_t elements) {
+  __shared__ double part[8];
+  pdl_wait();
+  const T* p = g + blockIdx.y * elements;
+  double s0 = 0.0, s1 = 0.0;
+  int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t step = (int64_t)gridDim.x * 256;
+  for (; i + step < elements; i += 2 * step) {
+    const double a = (double)(float)p[i], b = (double)(float)p[i + step];
+    s0 += a * a, s1 += b * b;
+  }
+  if (i < elements) {
+    const double a = (double)(float)p[i];
+    s0 += a * a;
+  }
+  s0 += s1;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s0 += __shfl_xor_sync(0xffffffffu, s0, o);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s0;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 8; ++w) s0 += part[w];
+    sums[blockIdx.y * gridDim.x + blockIdx.x] = s0;
+  }
+}
+// v = hi + 2^-11 lo
+__device__ __forceinline__ void split_planes(float v, __half& hi, __half& lo) {
+  hi = __float2half_rn(v);
+  lo = __float2half_rn((v - __half2float(hi)) * 2048.f);
+}
+__device__ __forceinline__ void split_planes2(float x, float y, uint32_t& hi, uint32_t& lo) {
+  hi = pack_f16x2_inf(x, y);
+  const float2 h = unpack_f16x2(hi);
+  lo = pack_f16x2_inf((x - h.x) * 2048.f, (y - h.y) * 2048.f);
+}
+// The planes of G 2^10 / (|G| + eps), eight columns a thread; columns behind n are zero.
+template <typename T>
+__global__ void __launch_bounds__(256) ortho_split_kernel(const T* __restrict__ g, const double* __restrict__ sums, uint4* __restrict__ planes, int64_t m, int64_t n,
+                                                          int64_t ld, int parts, double eps) {
+  __shared__ double by;
+  pdl_wait();
+  const int64_t z = blockIdx.y;
+  if (threadIdx.x == 0) {
+    double s = 0.0;
+    for (int i = 0; i < parts; ++i) s += sums[z * parts + i];
+    by = (double)kPlaneScale / (sqrt(s) + eps);
+  }
+  __syncthreads();
+  const double scale = by;
+  const int64_t per = ld / 8, all = m * per;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+    const int64_t row = i / per, col = (i - row * per) * 8;
+    const T* p = g + (z * m + row) * n + col;
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = col + j < n ? (float)((double)(float)p[j] * scale) : 0.f;
+    uint4 hi, lo;
+    split_planes2(v[0], v[1], hi.x, lo.x), split_planes2(v[2], v[3], hi.y, lo.y);
+    split_planes2(v[4], v[5], hi.z, lo.z), split_planes2(v[6], v[7], hi.w, lo.w);
+    planes[2 * z * all + i] = hi;
+    planes[(2 * z + 1) * all + i] = lo;
+  }
+}
+// The other way, for results whose rows TMA cannot store.
+template <typename T>
+__global__ void __launch_bounds__(256) ortho_join_kernel(const __half* __restrict__ planes, T* __restrict__ out, int64_t m, int64_t n, int64_t ld) {
+  pdl_wait();
+  const int64_t z = blockIdx.y, all = m * n;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+    const int64_t row = i / n, at = (2 * z * m + row) * ld + (i - row * n);
+    out[z * all + i] = (T)((__half2float(planes[at]) + __half2float(planes[at + m * ld]) * (1.f / 2048.f)) * (1.f / kPlaneScale));
+  }
+}
+
+// ---- the product -----------------------------------------------------------------------------------------------------
+// D = A B^T of operands in two planes: D1 = hi hi, D2 = hi lo + lo hi, D = D1 + 2^-11 D2.  The tensor core truncates where it adds, which shortens a sum
+// of positive terms by 3e-8 a step of 16 k (384 x 1536 in fp32: 1.6e-5 off with one accumulator for all of K, plain fp32 products 3e-6 to 7e-6).  So D1
+// has a fresh accumulator for each `chunk` stages of 64 k, which the epilogue's warps add to their registers, rounding to nearest, while the next one
+// fills.  Of chunk = 1, 2, 4, 8 the results of eight 1024 x 1024 matrices are off by 1.6, 2.8, 5.1, 9.7e-6 in 614, 593, 581, 562 us, 4096 x 4096 takes 4540, 4110,
+// 3870, 3670: 1 where the result is fp32, 2 for fp16 and 8 for bf16, whose own rounding is 2e-4 and 1.7e-3.  D2, 2^-11 as large, is added up in tensor memory.  Tiles of 128 x 128, or 256 x 256 for a pair of CTAs in two units of 128 columns (64 of
+// each CTA's rows of B): tensor memory holds two accumulators of a unit and D2 of the tile.
+template <int kCtas_, bool kAMn_, bool kBMn_>
+struct PlaneShape {
+  static constexpr int kCtas = kCtas_, kUnits = kCtas, kSide = 128 * kCtas, kStages = 3;
+  static constexpr bool kAMn = kAMn_, kBMn = kBMn_;
+  static constexpr int kPlaneBytes = kGemmM * kGemmK * 2, kStageBytes = 4 * kPlaneBytes;      // A hi, A lo, B hi, B lo: 128 rows each
+  static constexpr int kStg = kStages * kStageBytes, kBars = kStg + kGemmEpiWarps * kGemmStgBytes;
+  static constexpr size_t kSmem = kBars + 256 + 1024;
+  static constexpr uint32_t kIdesc = umma_idesc_f16(kGemmM * kCtas, 128, kAMn, kBMn);
+  static_assert(kSmem <= 232448, "shared memory budget");
+};
+struct PlaneBarriers {
+  uint64_t full[3], empty[3], part_full[2], part_empty[2], rest_full, rest_empty;
+  uint32_t tmem_base, peer_stop;
+};
+
+// What becomes of the product: planes of a factor times it (and the polynomial's other terms), symmetric ones stored twice; or the result.
+struct OrthoEnd {
+  CUtensorMap out;              // planes: boxes of 32 x 32 (z = 2 matrix + plane); result: of 32 rows of 32 columns
+  const __half* gram;           // planes of A, for the polynomial; or NULL
+  float factor, a, b;           // v = factor D + b A + a I
+  int rows, cols, ld;           // ld: of gram
+  int type, symmetric, result;  // type: of the result, whichever product this is
+
+  __device__ __forceinline__ void store(unsigned char* stg, int lane, int x, int y, int z) const {
+    asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+    __syncwarp();
+    if (lane == 0) {
+      tma_store_3d(&out, smem_u32(stg), x, y, 2 * z);
+      tma_store_3d(&out, smem_u32(stg) + 2048, x, y, 2 * z + 1);
+      tma_store_commit();
+    }
+  }
+  // v: 32 columns from col on of row m0 + lane
+  __device__ __forceinline__ void block(float* v, int m0, int col, int z, bool twice, unsigned char* stg, int lane) const {
+    const int row = m0 + lane;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] *= factor;
+    if (gram) {
+      const __half* p = gram + ((int64_t)2 * z * rows + row) * ld + col;
+      if (row < rows) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (col + 8 * k < ld) {
+            const uint4 h = *reinterpret_cast<const uint4*>(p + 8 * k), l = *reinterpret_cast<const uint4*>(p + (int64_t)rows * ld + 8 * k);
+            const uint32_t hs[4] = {h.x, h.y, h.z, h.w}, ls[4] = {l.x, l.y, l.z, l.w};
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              const float2 x = unpack_f16x2(hs[w]), y = unpack_f16x2(ls[w]);
+              v[8 * k + 2 * w] = fmaf(b, fmaf(y.x, 1.f / 2048.f, x.x), v[8 * k + 2 * w]);
+              v[8 * k + 2 * w + 1] = fmaf(b, fmaf(y.y, 1.f / 2048.f, x.y), v[8 * k + 2 * w + 1]);
+            }
+          }
+        }
+      }
+      const int diagonal = row - col;
+      if (diagonal >= 0 && diagonal < 32) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (j == diagonal) v[j] += a * kPlaneScale;
+      }
+    }
+    if (lane == 0) tma_store_wait_read<0>();
+    __syncwarp();
+    if (result) {
+      if (type == PX_F32) {
+#pragma unroll
+        for (int p = 0; p < 8; ++p)
+          *reinterpret_cast<float4*>(stg + lane * 128 + ((p ^ (lane & 7)) << 4)) = make_float4(v[4 * p], v[4 * p + 1], v[4 * p + 2], v[4 * p + 3]);
+      } else {
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          uint32_t o[4];
+#pragma unroll
+          for (int w = 0; w < 4; ++w) o[w] = type == PX_F16 ? pack_f16x2_inf(v[8 * p + 2 * w], v[8 * p + 2 * w + 1]) : pack_bf16x2(v[8 * p + 2 * w], v[8 * p + 2 * w + 1]);
+          *reinterpret_cast<uint4*>(stg + lane * 64 + ((p ^ (lane >> 1 & 3)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+      __syncwarp();
+      if (lane == 0) {
+        tma_store_3d(&out, smem_u32(stg), col, m0, z);
+        tma_store_commit();
+      }
+      return;
+    }
+    uint32_t hi[16], lo[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) split_planes2(v[2 * j], v[2 * j + 1], hi[j], lo[j]);
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      const int at = lane * 64 + ((p ^ (lane >> 1 & 3)) << 4);
+      *reinterpret_cast<uint4*>(stg + at) = make_uint4(hi[4 * p], hi[4 * p + 1], hi[4 * p + 2], hi[4 * p + 3]);
+      *reinterpret_cast<uint4*>(stg + 2048 + at) = make_uint4(lo[4 * p], lo[4 * p + 1], lo[4 * p + 2], lo[4 * p + 3]);
+    }
+    store(stg, lane, col, m0, z);
+    if (twice) {
+      if (lane == 0) tma_store_wait_read<0>();
+      __syncwarp();
+      // lane = column of the transposed block
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        const int at = j * 64 + (((lane >> 3) ^ (j >> 1 & 3)) << 4) + 2 * (lane & 7);
+        *reinterpret_cast<uint16_t*>(stg + at) = (uint16_t)(hi[j / 2] >> (16 * (j & 1)));
+        *reinterpret_cast<uint16_t*>(stg + 2048 + at) = (uint16_t)(lo[j / 2] >> (16 * (j & 1)));
+      }
+      store(stg, lane, m0, col, z);
+    }
+  }
+};
+
+template <class S>
+__global__ void __launch_bounds__(kGemmThreads, 1)
+plane_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ OrthoEnd end, const GemmTiles tiles, int chunk) {
+  constexpr bool kPair = S::kCtas == 2;
+  constexpr int kStages = S::kStages, kUnits = S::kUnits;
+  constexpr uint32_t kCols = 512;      // two accumulators of 128 columns, D2 of 128 or 256
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char* ring = smem_aligned(smem_raw);
+  PlaneBarriers& bars = *reinterpret_cast<PlaneBarriers*>(ring + S::kBars);
+  const int warp = warp_index(), lane = threadIdx.x & 31;
+  const uint32_t rank = kPair ? cluster_rank() : 0;
+  const int first_tile = blockIdx.x / S::kCtas, tile_step = gridDim.x / S::kCtas;
+
+  const bool skip = cta_begin();
+  if (threadIdx.x == 32) prefetch_maps(map_a, map_b, end.out);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&bars.full[s], 1);
+      mbar_init(&bars.empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&bars.part_full[b], 1);
+      mbar_init(&bars.part_empty[b], kGemmEpiWarps * S::kCtas);
+    }
+    mbar_init(&bars.rest_full, 1);
+    mbar_init(&bars.rest_empty, kGemmEpiWarps * S::kCtas);
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+  }
+  if (warp == 0) {
+    if constexpr (kPair) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&bars.tmem_base)), "r"(kCols) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&bars.tmem_base)), "r"(kCols) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+    }
+  }
+  bool stop;
+  tc_fence_before();
+  if constexpr (kPair) {
+    // both CTAs work or neither does
+    stop = __syncthreads_or(skip) != 0;
+    if (threadIdx.x == 0)
+      asm volatile("st.shared::cluster.u32 [%0], %1;\n" ::"r"(map_to_rank(smem_u32(&bars.peer_stop), rank ^ 1)), "r"((uint32_t)stop) : "memory");
+    tc_cluster_sync();
+    stop = stop || *reinterpret_cast<volatile uint32_t*>(&bars.peer_stop) != 0;
+  } else {
+    stop = __syncthreads_or(skip) != 0;
+  }
+  tc_fence_after();
+  pdl_wait();
+  const uint32_t tmem_base = bars.tmem_base;
+
+  if (stop) {
+    // nothing
+  } else if (warp == 0) {
+    uint32_t it = 0;
+    bool ok = true;
+    for (int tile = first_tile; tile < tiles.total && ok; tile += tile_step) {
+      const GemmTile t = gemm_tile(tiles, tile);
+      const int m0 = t.mt * S::kSide + (int)rank * 128, n0 = t.nt * S::kSide + (int)rank * 128;
+      for (int kt = 0; kt < t.nk && ok; ++kt, ++it) {
+        const int s = it % kStages;
+        ok = mbar_wait_warp(&bars.empty[s], ((it / kStages) & 1) ^ 1, 1u);
+        if (!ok) break;
+        if (elect_lane()) {
+          const uint32_t sa = smem_u32(ring + s * S::kStageBytes);
+          if (rank == 0) mbar_expect_tx(&bars.full[s], S::kCtas * S::kStageBytes);
+          const uint32_t bar = kPair ? map_to_rank(smem_u32(&bars.full[s]), 0) : 0;
+          auto load = [&](uint32_t dst, const CUtensorMap* map, bool across, int from, int z) {
+            for (int j = 0; j < (across ? 2 : 1); ++j) {
+              const int x = across ? from + 64 * j : kt * kGemmK, y = across ? kt * kGemmK : from;
+              if constexpr (kPair)
+                tma_load_3d_pair(dst + 8192 * j, map, bar, x, y, z);
+              else
+                tma_load_3d(dst + 8192 * j, map, &bars.full[s], x, y, z);
+            }
+          };
+#pragma unroll
+          for (int p = 0; p < 2; ++p) {
+            load(sa + p * S::kPlaneBytes, &map_a, S::kAMn, m0, 2 * t.z + p);
+            load(sa + (2 + p) * S::kPlaneBytes, &map_b, S::kBMn, n0, 2 * t.z + p);
+          }
+        }
+        __syncwarp();
+      }
+    }
+  } else if (warp == 1) {
+    if (rank == 0) {
+      uint32_t it = 0, unit = 0, count = 0;
+      bool ok = true;
+      for (int tile = first_tile; tile < tiles.total && ok; tile += tile_step, ++count) {
+        const GemmTile t = gemm_tile(tiles, tile);
+        ok = mbar_wait_warp(&bars.rest_empty, (count & 1) ^ 1, 2u);
+        for (int kt = 0; kt < t.nk && ok; ++kt, ++it) {
+          const int s = it % kStages;
+          ok = mbar_wait_warp(&bars.full[s], (it / kStages) & 1, 4u);
+          const bool begins = (kt & (chunk - 1)) == 0, ends = ((kt + 1) & (chunk - 1)) == 0 || kt == t.nk - 1;
+          for (int h = 0; h < kUnits && ok; ++h) {
+            const uint32_t at = unit + h, buf = at & 1;
+            if (begins) ok = mbar_wait_warp(&bars.part_empty[buf], ((at >> 1) & 1) ^ 1, 8u);
+            if (!ok) break;
+            tc_fence_after();
+            if (elect_lane()) {
+              const uint32_t sa = smem_u32(ring + s * S::kStageBytes), sb = sa + 2 * S::kPlaneBytes + h * 8192;
+              const uint64_t da = S::kAMn ? umma_desc_mn_sw128(sa, 8192, 1024) : umma_desc_sw128(sa);
+              const uint64_t db = S::kBMn ? umma_desc_mn_sw128(sb, 8192, 1024) : umma_desc_sw128(sb);
+              constexpr uint64_t kLo = S::kPlaneBytes >> 4;
+              auto mma = [&](uint32_t d, uint64_t a, uint64_t b, uint32_t more) {
+                if constexpr (kPair)
+                  umma_pair(d, a, b, S::kIdesc, more);
+                else
+                  umma_bf16(d, a, b, S::kIdesc, more);
+              };
+              const uint32_t d1 = tmem_base + 128 * buf, d2 = tmem_base + 256 + 128 * h;
+#pragma unroll
+              for (int ks = 0; ks < kGemmK / 16; ++ks) mma(d1, da + (S::kAMn ? 128 : 2) * ks, db + (S::kBMn ? 128 : 2) * ks, !begins || ks > 0);
+              if (!ends) {
+              } else if constexpr (kPair)
+                umma_commit_pair(&bars.part_full[buf]);
+              else
+                umma_commit(&bars.part_full[buf]);
+#pragma unroll
+              for (int ks = 0; ks < kGemmK / 16; ++ks) {
+                const uint64_t a = da + (S::kAMn ? 128 : 2) * ks, b = db + (S::kBMn ? 128 : 2) * ks;
+                mma(d2, a, b + kLo, (kt | ks) ? 1u : 0u);
+                mma(d2, a + kLo, b, 1u);
+              }
+              if (h == kUnits - 1) {
+                if constexpr (kPair)
+                  umma_commit_pair(&bars.empty[s]);
+                else
+                  umma_commit(&bars.empty[s]);
+                if (kt == t.nk - 1) {
+                  if constexpr (kPair)
+                    umma_commit_pair(&bars.rest_full);
+                  else
+                    umma_commit(&bars.rest_full);
+                }
+              }
+            }
+            __syncwarp();
+          }
+          if (ends) unit += kUnits;
+        }
+      }
+    }
+  } else {
+    const int q = warp & 3, half = (warp - 2) >> 2;
+    unsigned char* const stg = ring + S::kStg + (warp - 2) * kGemmStgBytes;
+    const uint32_t lanes = tmem_base + ((uint32_t)(32 * q) << 16) + 64 * half;
+    auto arrive = [&](uint64_t* bar) {
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (kPair)
+          mbar_arrive_cluster(map_to_rank(smem_u32(bar), 0));
+        else
+          mbar_arrive(bar);
+      }
+    };
+    uint32_t unit = 0, count = 0;
+    bool ok = true;
+    for (int tile = first_tile; tile < tiles.total && ok; tile += tile_step, ++count) {
+      const GemmTile t = gemm_tile(tiles, tile);
+      float sum[kUnits][64];
+#pragma unroll
+      for (int h = 0; h < kUnits; ++h)
+#pragma unroll
+        for (int j = 0; j < 64; ++j) sum[h][j] = 0.f;
+      for (int kt = 0; kt < t.nk && ok; kt += chunk) {
+#pragma unroll
+        for (int h = 0; h < kUnits; ++h, ++unit) {
+          const uint32_t buf = unit & 1;
+          ok = ok && mbar_wait_warp(&bars.part_full[buf], (unit >> 1) & 1, 16u);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int c = 0; c < 64; c += 32) {
+            uint32_t r[32];
+            tmem_ld32(lanes + 128 * buf + c, r);
+            tmem_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) add2(sum[h][c + j], sum[h][c + j + 1], __uint_as_float(r[j]), __uint_as_float(r[j + 1]));
+          }
+          arrive(&bars.part_empty[buf]);
+        }
+      }
+      ok = ok && mbar_wait_warp(&bars.rest_full, count & 1, 32u);
+      if (!ok) break;
+      tc_fence_after();
+#pragma unroll
+      for (int h = 0; h < kUnits; ++h) {
+#pragma unroll
+        for (int c = 0; c < 64; c += 32) {
+          uint32_t r[32];
+          tmem_ld32(lanes + 256 + 128 * h + c, r);
+          tmem_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) sum[h][c + j] = fmaf(__uint_as_float(r[j]), 1.f / 2048.f, sum[h][c + j]);
+        }
+      }
+      arrive(&bars.rest_empty);
+      const int m0 = t.mt * S::kSide + (int)rank * 128 + 32 * q, n0 = t.nt * S::kSide + 64 * kUnits * half;
+      if (m0 < end.rows) {
+#pragma unroll
+        for (int h = 0; h < kUnits; ++h) {
+#pragma unroll
+          for (int c = 0; c < 64; c += 32) {
+            const int col = n0 + 64 * h + c;
+            if (col < end.cols) end.block(&sum[h][c], m0, col, t.z, end.symmetric && t.mt != t.nt, stg, lane);
+          }
+        }
+      }
+    }
+    if (lane == 0) tma_store_wait_read<0>();
+  }
+
+  // teardown: everybody meets, then the allocating warp frees the tensor memory
+  __syncwarp();
+  tc_fence_before();
+  cta_teardown_sync();
+  if constexpr (kPair) tc_cluster_sync();          // nobody leaves while its pair may still signal or read it
+  if (warp == 0) {
+    tc_fence_after();
+    if constexpr (kPair)
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem_base), "r"(kCols) : "memory");
+    else
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem_base), "r"(kCols) : "memory");
+  }
+  if constexpr (kPair) tc_cluster_sync();
+}
+
+PX_DEFINE_FAMILY_HOOKS(update)
+
+// ---- host ------------------------------------------------------------------------------------------------------------
+static int64_t ortho_up(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
+
+// planes [batch][2][rows][ld], of which `inner` columns count
+struct Planes {
+  __half* at;
+  int64_t rows, inner, ld;
+};
+static bool operand_map(CUtensorMap* map, const Planes& p, int64_t batch, bool across) {
+  return gemm_map(map, true, p.at, p.inner, p.rows, 2 * batch, p.ld, p.rows * p.ld, across ? kGemmK : kGemmM);
+}
+static bool planes_out(CUtensorMap* map, const Planes& p, int64_t batch) {
+  return make_map_3d(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, p.at, (uint64_t)p.inner, (uint64_t)p.rows, (uint64_t)(2 * batch), (uint64_t)p.ld * 2, (uint64_t)p.rows * p.ld * 2, 32,
+                     32, CU_TENSOR_MAP_SWIZZLE_64B);
+}
+template <class S>
+static int32_t launch_planes(const CUtensorMap& ma, const CUtensorMap& mb, const OrthoEnd& end, GemmTiles t, int64_t m, int64_t n, cudaStream_t st) {
+  const int chunk = end.type == PX_F32 ? 1 : end.type == PX_F16 ? 2 : 8;
+  t.tiles_m = (int)(ortho_up(m, S::kSide) / S::kSide), t.tiles_n = (int)(ortho_up(n, S::kSide) / S::kSide);
+  const int64_t total = t.batch * (t.symmetric ? (int64_t)t.tiles_m * (t.tiles_m + 1) / 2 : (int64_t)t.tiles_m * t.tiles_n);
+  if (total > 0x7fffffff) return PX_ERR_UNSUPPORTED;
+  t.total = (int)total;
+  static SmemLimit limit;
+  if (!limit.set(plane_product_kernel<S>, S::kSmem)) return PX_ERR_LAUNCH;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = S::kCtas, at[1].val.clusterDim.y = 1, at[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(even_grid(total, sm_count() / S::kCtas) * S::kCtas));
+  cfg.blockDim = dim3(kGemmThreads);
+  cfg.dynamicSmemBytes = S::kSmem;
+  cfg.stream = st;
+  cfg.attrs = at;
+  cfg.numAttrs = S::kCtas > 1 ? 2 : 1;
+  if (cudaLaunchKernelEx(&cfg, plane_product_kernel<S>, ma, mb, end, t, chunk) == cudaSuccess) return PX_OK;
+  cudaGetLastError();
+  return PX_ERR_LAUNCH;
+}
+template <bool kAMn, bool kBMn>
+static int32_t ortho_product(const Planes& a, const Planes& b, int64_t batch, int64_t m, int64_t n, int64_t k, const OrthoEnd& end, cudaStream_t st) {
+  CUtensorMap ma, mb;
+  if (!operand_map(&ma, a, batch, kAMn) || !operand_map(&mb, b, batch, kBMn)) return PX_ERR_LAUNCH;
+  GemmTiles t = {};
+  t.batch = (int)batch, t.splits = 1, t.group = 8, t.symmetric = end.symmetric;
+  t.nk = t.nk_split = (int)(ortho_up(k, kGemmK) / kGemmK);
+  const int64_t tm = ortho_up(m, 256) / 256, tn = ortho_up(n, 256) / 256;
+  if (batch * (end.symmetric ? tm * (tm + 1) / 2 : tm * tn) >= sm_count()) return launch_planes<PlaneShape<2, kAMn, kBMn>>(ma, mb, end, t, m, n, st);
+  return launch_planes<PlaneShape<1, kAMn, kBMn>>(ma, mb, end, t, m, n, st);
+}
+
+struct OrthoPlan {
+  int64_t ld, s, lds, sums, x[2], gram, poly, bytes;
+};
+static OrthoPlan ortho_plan(int64_t batch, int64_t m, int64_t n) {
+  OrthoPlan p;
+  p.s = std::min(m, n);
+  p.ld = ortho_up(n, 8), p.lds = ortho_up(p.s, 8);
+  int64_t at = 0;
+  const auto take = [&](int64_t bytes) {
+    const int64_t here = at;
+    at += ortho_up(bytes, 1024);
+    return here;
+  };
+  p.sums = take(batch * kNormBlocks * 8);
+  for (int64_t& x : p.x) x = take(batch * 2 * m * p.ld * 2);
+  p.gram = take(batch * 2 * p.s * p.lds * 2);
+  p.poly = take(batch * 2 * p.s * p.lds * 2);
+  p.bytes = at;
+  return p;
+}
+template <typename T>
+static bool ortho_first(const void* g, double* sums, uint4* planes, int64_t batch, int64_t m, int64_t n, int64_t ld, double eps, cudaStream_t st) {
+  const int parts = (int)std::min<int64_t>(kNormBlocks, (m * n + 4095) / 4096);
+  if (!launch_pdl(ortho_norm_kernel<T>, dim3(parts, (unsigned)batch), 256, 0, st, (const T*)g, sums, m * n)) return false;
+  const int64_t blocks = std::min<int64_t>((m * ld / 8 + 255) / 256, std::max<int64_t>(1, 8 * sm_count() / batch));
+  return launch_pdl(ortho_split_kernel<T>, dim3((unsigned)blocks, (unsigned)batch), 256, 0, st, (const T*)g, (const double*)sums, planes, m, n, ld, parts, eps);
+}
+template <typename T>
+static bool ortho_last(const __half* planes, void* out, int64_t batch, int64_t m, int64_t n, int64_t ld, cudaStream_t st) {
+  const int64_t blocks = std::min<int64_t>((m * n + 255) / 256, std::max<int64_t>(1, 8 * sm_count() / batch));
+  return launch_pdl(ortho_join_kernel<T>, dim3((unsigned)blocks, (unsigned)batch), 256, 0, st, planes, (T*)out, m, n, ld);
+}
+
+}  // namespace px
+
+using namespace px;
+
+extern "C" int64_t px_orthogonalize_workspace_bytes(int64_t batch, int64_t m, int64_t n) {
+  return batch <= 0 || m <= 0 || n <= 0 ? 0 : ortho_plan(batch, m, n).bytes;
+}
+
+extern "C" int32_t px_orthogonalize(const void* g, void* out, int64_t batch, int64_t m, int64_t n, const float* coefficients, int32_t steps, double eps, int32_t dtype,
+                                    void* workspace, int64_t workspace_bytes, void* stream) {
+  if (batch < 0 || m < 0 || n < 0 || steps < 1 || !coefficients || !(eps >= 0.0)) return PX_ERR_BAD_ARG;
+  if (dtype != PX_F32 && dtype != PX_BF16 && dtype != PX_F16) return PX_ERR_UNSUPPORTED;
+  if (batch > 65535 || m > (1 << 20) || n > (1 << 20) || steps > 1000) return PX_ERR_UNSUPPORTED;
+  if (batch == 0 || m == 0 || n == 0) return PX_OK;
+  if (!g || !out || !workspace || ((uintptr_t)workspace & 255) || (((uintptr_t)g | (uintptr_t)out) & (dtype == PX_F32 ? 3 : 1))) return PX_ERR_BAD_ARG;
+  const OrthoPlan p = ortho_plan(batch, m, n);
+  if (workspace_bytes < p.bytes) return PX_ERR_WORKSPACE;
+  if (!have_context()) return PX_ERR_LAUNCH;
+  const cudaStream_t st = (cudaStream_t)stream;
+  char* const ws = (char*)workspace;
+  const bool wide = m <= n;
+  double* sums = (double*)(ws + p.sums);
+  Planes x = {(__half*)(ws + p.x[0]), m, n, p.ld}, next = {(__half*)(ws + p.x[1]), m, n, p.ld};
+  const Planes gram = {(__half*)(ws + p.gram), p.s, p.s, p.lds}, poly = {(__half*)(ws + p.poly), p.s, p.s, p.lds};
+  const bool ok = dtype == PX_F32    ? ortho_first<float>(g, sums, (uint4*)x.at, batch, m, n, p.ld, eps, st)
+                  : dtype == PX_BF16 ? ortho_first<bf16>(g, sums, (uint4*)x.at, batch, m, n, p.ld, eps, st)
+                                     : ortho_first<__half>(g, sums, (uint4*)x.at, batch, m, n, p.ld, eps, st);
+  if (!ok) return PX_ERR_LAUNCH;
+  const int size = dtype == PX_F32 ? 4 : 2;
+  const bool direct = n * size % 16 == 0 && ((uintptr_t)out & 15) == 0;      // what TMA can store
+  for (int i = 0; i < steps; ++i) {
+    const float a = coefficients[3 * i], b = coefficients[3 * i + 1], c = coefficients[3 * i + 2];
+    OrthoEnd e = {};
+    if (!planes_out(&e.out, gram, batch)) return PX_ERR_LAUNCH;
+    e.factor = 1.f / kPlaneScale, e.rows = e.cols = (int)p.s, e.ld = (int)p.lds, e.symmetric = 1, e.type = dtype;
+    int32_t status = wide ? ortho_product<false, false>(x, x, batch, p.s, p.s, n, e, st) : ortho_product<true, true>(x, x, batch, p.s, p.s, m, e, st);
+    if (status) return status;
+    if (!planes_out(&e.out, poly, batch)) return PX_ERR_LAUNCH;
+    e.gram = gram.at, e.factor = c / kPlaneScale, e.a = a, e.b = b;
+    status = ortho_product<false, false>(gram, gram, batch, p.s, p.s, p.s, e, st);
+    if (status) return status;
+    e = {};
+    e.factor = 1.f / kPlaneScale, e.rows = (int)m, e.cols = (int)n, e.type = dtype;
+    if (i == steps - 1 && direct) {
+      e.result = 1, e.factor = 1.f / (kPlaneScale * kPlaneScale);
+      const CUtensorMapDataType type = dtype == PX_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : dtype == PX_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+      if (!make_map_3d(&e.out, type, out, (uint64_t)n, (uint64_t)m, (uint64_t)batch, (uint64_t)n * size, (uint64_t)m * n * size, 32, 32,
+                       dtype == PX_F32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B))
+        return PX_ERR_LAUNCH;
+    } else if (!planes_out(&e.out, next, batch)) {
+      return PX_ERR_LAUNCH;
+    }
+    status = wide ? ortho_product<false, true>(poly, x, batch, m, n, m, e, st) : ortho_product<false, false>(x, poly, batch, m, n, n, e, st);
+    if (status) return status;
+    std::swap(x.at, next.at);
+  }
+  if (direct) return PX_OK;
+  const bool done = dtype == PX_F32    ? ortho_last<float>(x.at, out, batch, m, n, p.ld, st)
+                    : dtype == PX_BF16 ? ortho_last<bf16>(x.at, out, batch, m, n, p.ld, st)
+                                       : ortho_last<__half>(x.at, out, batch, m, n, p.ld, st);
+  return done ? PX_OK : PX_ERR_LAUNCH;
+}

@@ -1,18 +1,13 @@
 // A persistent product D(m, n) = sum_k A(m, k) B(n, k) of 16-bit operands on the tensor cores, whose epilogue is a parameter: the
-// passes of the cross entropy (cross_entropy.cu) and of the orthogonalised update (orthogonalize.cu) are this kernel with others.
+// passes of the cross entropy (cross_entropy.cu).
 //
 // Operands lie along k ([m][k], K-major) or across it ([k][m], MN-major); TMA fills tiles of 128 m (n) by 64 k in 128-byte
 // swizzle either way, and zeroes what lies outside, so no size needs to be a multiple of anything but the row strides (16 bytes).
 // One CTA works on 128 x kN, or a pair of them (cta_group::2) on 256 x kN, each with its own 128 rows of A and half of B: the pair asks L2 for
 // 64 bytes a cycle where a CTA alone with kN = 256 asks for 96.
 //
-// kPlanes = 2: an operand is the sum of two fp16 planes, v = hi + 2^-11 lo, each rounded to nearest, so that it carries 22 bits.  Three of
-// the four partial products are formed; hi hi goes to one accumulator and the other two to a second one, because the tensor core
-// truncates where it adds: the small terms would lose their bits, and the large sum would be cut three times as often.  The epilogue puts
-// D1 + 2^-11 D2 together.
-//
 // Roles: warp 0 copies, warp 1 issues products, eight warps are the epilogue (a quarter of the lanes and half of the columns each).
-// Accumulators are double-buffered where tensor memory has room (not for two planes of 256 columns).
+// Accumulators are double-buffered.
 #pragma once
 #include "px_pair.cuh"
 #include "px_rowpipe.cuh"
@@ -23,15 +18,14 @@ constexpr int kGemmM = 128, kGemmK = 64;          // rows of a CTA's tile, k of 
 constexpr int kGemmEpiWarps = 8, kGemmThreads = 64 + 32 * kGemmEpiWarps;
 constexpr int kGemmStgBytes = 4096;               // staged block of a warp: 32 rows of 128 bytes
 
-template <int kCtas_, int kN_, int kPlanes_, bool kAMn_, bool kBMn_, int kStages_>
+template <int kCtas_, int kN_, bool kAMn_, bool kBMn_, int kStages_>
 struct GemmShape {
-  static constexpr int kCtas = kCtas_, kN = kN_, kPlanes = kPlanes_, kStages = kStages_;
+  static constexpr int kCtas = kCtas_, kN = kN_, kStages = kStages_;
   static constexpr bool kAMn = kAMn_, kBMn = kBMn_;
   static constexpr int kBRows = kN / kCtas;       // rows of B that a CTA loads
   static constexpr int kABytes = kGemmM * kGemmK * 2, kBBytes = kBRows * kGemmK * 2;
-  static constexpr int kStageBytes = kPlanes * (kABytes + kBBytes);
-  static constexpr int kAccCols = kPlanes * kN, kAccs = 2 * kAccCols <= 512 ? 2 : 1;
-  static constexpr uint32_t kCols = kAccs * kAccCols <= 128 ? 128 : kAccs * kAccCols <= 256 ? 256 : 512;
+  static constexpr int kStageBytes = kABytes + kBBytes;
+  static constexpr uint32_t kCols = 2 * kN;
   static constexpr int kStg = kStages * kStageBytes, kExtra = kStg + kGemmEpiWarps * kGemmStgBytes, kExtraBytes = 1536;
   static constexpr int kBars = kExtra + kExtraBytes;
   static constexpr size_t kSmem = kBars + 256 + 1024;
@@ -41,7 +35,7 @@ struct GemmShape {
 };
 
 // The tiles of a product: `batch` products of tiles_m x tiles_n tiles, each over `nk` steps of 64 k in `splits` parts.  symmetric: only
-// tiles (i, j) with i <= j (square tiles).  Tiles run through `group` rows of tiles column by column, so that what is worked on at once reads few operands.
+// tiles (i, j) with i <= j (square ones).  Tiles run through `group` rows of tiles column by column, so that what is worked on at once reads few operands.
 struct GemmTiles {
   int tiles_m, tiles_n, batch, splits, nk, nk_split, group, symmetric, total;
 };
@@ -97,7 +91,7 @@ template <class S, class Epi>
 __global__ void __launch_bounds__(kGemmThreads, 1)
 gemm_kernel(const __grid_constant__ GemmOperands ops, const __grid_constant__ Epi epi, const GemmTiles tiles) {
   constexpr bool kPair = S::kCtas == 2;
-  constexpr int kStages = S::kStages, kAccs = S::kAccs;
+  constexpr int kStages = S::kStages;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* ring = smem_aligned(smem_raw);
   GemmBarriers& bars = *reinterpret_cast<GemmBarriers*>(ring + S::kBars);
@@ -160,7 +154,7 @@ gemm_kernel(const __grid_constant__ GemmOperands ops, const __grid_constant__ Ep
         ok = mbar_wait_warp(&bars.empty[s], ph ^ 1, 1u);
         if (!ok) break;
         if (elect_lane()) {
-          const uint32_t sa = smem_u32(ring + s * S::kStageBytes), sb = sa + S::kPlanes * S::kABytes;
+          const uint32_t sa = smem_u32(ring + s * S::kStageBytes), sb = sa + S::kABytes;
           const int k = (t.k0 + kt) * kGemmK;
           if (rank == 0) mbar_expect_tx(&bars.full[s], S::kCtas * S::kStageBytes);
           const uint32_t bar = kPair ? map_to_rank(smem_u32(&bars.full[s]), 0) : 0;
@@ -170,21 +164,17 @@ gemm_kernel(const __grid_constant__ GemmOperands ops, const __grid_constant__ Ep
             else
               tma_load_3d(dst, map, &bars.full[s], x, y, z);
           };
+          if constexpr (S::kAMn) {
 #pragma unroll
-          for (int p = 0; p < S::kPlanes; ++p) {
-            const int z = t.z * S::kPlanes + p;
-            if constexpr (S::kAMn) {
+            for (int j = 0; j < kGemmM / 64; ++j) load(sa + j * 8192, &ops.a, m0 + 64 * j, k, t.z);
+          } else {
+            load(sa, &ops.a, k, m0, t.z);
+          }
+          if constexpr (S::kBMn) {
 #pragma unroll
-              for (int j = 0; j < kGemmM / 64; ++j) load(sa + p * S::kABytes + j * 8192, &ops.a, m0 + 64 * j, k, z);
-            } else {
-              load(sa + p * S::kABytes, &ops.a, k, m0, z);
-            }
-            if constexpr (S::kBMn) {
-#pragma unroll
-              for (int j = 0; j < S::kBRows / 64; ++j) load(sb + p * S::kBBytes + j * 8192, map_b, n0 + 64 * j, k, z);
-            } else {
-              load(sb + p * S::kBBytes, map_b, k, n0, z);
-            }
+            for (int j = 0; j < S::kBRows / 64; ++j) load(sb + j * 8192, map_b, n0 + 64 * j, k, t.z);
+          } else {
+            load(sb, map_b, k, n0, t.z);
           }
         }
         __syncwarp();
@@ -196,11 +186,11 @@ gemm_kernel(const __grid_constant__ GemmOperands ops, const __grid_constant__ Ep
       bool ok = true;
       for (int tile = first_tile; tile < tiles.total && ok; tile += tile_step, ++count) {
         const GemmTile t = gemm_tile(tiles, tile);
-        const uint32_t ab = count % kAccs, aph = (count / kAccs) & 1;
+        const uint32_t ab = count & 1, aph = (count >> 1) & 1;
         ok = mbar_wait_warp(&bars.acc_empty[ab], aph ^ 1, 2u);
         if (!ok) break;
         tc_fence_after();
-        const uint32_t d1 = tmem_base + ab * S::kAccCols, d2 = d1 + S::kN;
+        const uint32_t d = tmem_base + ab * S::kN;
         for (int kt = 0; kt < t.nk; ++kt, ++it) {
           const int s = it % kStages;
           const uint32_t ph = (it / kStages) & 1;
@@ -208,24 +198,17 @@ gemm_kernel(const __grid_constant__ GemmOperands ops, const __grid_constant__ Ep
           if (!ok) break;
           tc_fence_after();
           if (elect_lane()) {
-            const uint32_t sa = smem_u32(ring + s * S::kStageBytes), sb = sa + S::kPlanes * S::kABytes;
+            const uint32_t sa = smem_u32(ring + s * S::kStageBytes), sb = sa + S::kABytes;
             const uint64_t da = S::kAMn ? umma_desc_mn_sw128(sa, 8192, 1024) : umma_desc_sw128(sa);
             const uint64_t db = S::kBMn ? umma_desc_mn_sw128(sb, 8192, 1024) : umma_desc_sw128(sb);
-            auto mma = [&](uint32_t d, uint64_t a, uint64_t b, uint32_t acc) {
-              if constexpr (kPair)
-                umma_pair(d, a, b, ops.idesc, acc);
-              else
-                umma_bf16(d, a, b, ops.idesc, acc);
-            };
 #pragma unroll
             for (int ks = 0; ks < kGemmK / 16; ++ks) {     // 16 k: two 16-byte pieces of a row, or sixteen rows of 128 bytes
               const uint64_t a = da + (S::kAMn ? 128 : 2) * ks, b = db + (S::kBMn ? 128 : 2) * ks;
               const uint32_t more = (kt | ks) ? 1u : 0u;
-              mma(d1, a, b, more);
-              if constexpr (S::kPlanes == 2) {
-                mma(d2, a, b + (S::kBBytes >> 4), more);
-                mma(d2, a + (S::kABytes >> 4), b, 1u);
-              }
+              if constexpr (kPair)
+                umma_pair(d, a, b, ops.idesc, more);
+              else
+                umma_bf16(d, a, b, ops.idesc, more);
             }
             if constexpr (kPair)
               umma_commit_pair(&bars.empty[s]);
@@ -250,13 +233,13 @@ gemm_kernel(const __grid_constant__ GemmOperands ops, const __grid_constant__ Ep
     for (int tile = first_tile; tile < tiles.total; tile += tile_step, ++count) {
       GemmEpiTile e;
       e.at = gemm_tile(tiles, tile);
-      const uint32_t ab = count % kAccs, aph = (count / kAccs) & 1;
+      const uint32_t ab = count & 1, aph = (count >> 1) & 1;
       ok = ok && mbar_wait_warp(&bars.acc_full[ab], aph, 8u);
       if (!Epi::kMeets && !ok) break;                      // an epilogue whose warps meet goes through all tiles
       tc_fence_after();
       e.m0 = (e.at.mt * S::kCtas + (int)rank) * kGemmM + 32 * q;
       e.n0 = e.at.nt * S::kN;
-      e.acc = tmem_base + ((uint32_t)(32 * q) << 16) + ab * S::kAccCols;
+      e.acc = tmem_base + ((uint32_t)(32 * q) << 16) + ab * S::kN;
       e.quarter = q, e.half = half, e.lane = lane;
       e.stg = ring + S::kStg + (warp - 2) * kGemmStgBytes;
       e.extra = ring + S::kExtra;
@@ -287,9 +270,6 @@ gemm_kernel(const __grid_constant__ GemmOperands ops, const __grid_constant__ Ep
   }
   if constexpr (kPair) tc_cluster_sync();
 }
-
-// The value of column j of the accumulators, from registers that hold both (kPlanes = 2) or the one.
-__device__ __forceinline__ float gemm_sum(uint32_t d1, uint32_t d2) { return fmaf(__uint_as_float(d2), 1.f / 2048.f, __uint_as_float(d1)); }
 
 // The map of an operand: `rows` rows of `inner` elements, `stride` elements apart, `batch` of them `plane` elements apart.  K-major operands
 // come in boxes of box_rows rows (their tile), MN-major ones in boxes of 64 k.

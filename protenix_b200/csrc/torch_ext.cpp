@@ -63,7 +63,8 @@ constexpr int64_t kCz = 128, kCs = 384, kHeadsSingle = 16, kHeads = 4, kHeadDim 
   X(px_msa_rows_weights_bytes) X(px_msa_rows_prepare) X(px_msa_transition_weights_bytes) X(px_msa_transition_prepare) X(px_msa_transition) \
   X(px_dropout_add) X(px_relpos_codes_bytes) X(px_relpos_workspace_bytes) X(px_relpos_fwd) X(px_relpos_bwd) X(px_window_lse_floats) \
   X(px_window_fwd) X(px_window_workspace_bytes) X(px_window_bwd) X(px_head_loss_workspace_bytes) X(px_head_loss_fwd) \
-  X(px_head_loss_bwd_workspace_bytes) X(px_head_loss_bwd) X(px_rotary_turn)
+  X(px_head_loss_bwd_workspace_bytes) X(px_head_loss_bwd) X(px_rotary_turn) \
+  X(px_orthogonalize_workspace_bytes) X(px_orthogonalize)
 struct Abi {
 #define X(f) decltype(&::f) f = nullptr;
   PX_FUNCTIONS(X)
@@ -1029,6 +1030,7 @@ PYBIND11_MODULE(_C, m) {
   m.def("window_attention", &window_attention);
   m.def("linear_cross_entropy", &linear_cross_entropy);
   m.def("rotary_embedding", &rotary_embedding);
+  m.def("orthogonalize", &orthogonalize);
   m.def("counter_dropout_add", &counter_dropout_add);
   m.def("relative_position_encoding", &relative_position_encoding);
   py::class_<Params, std::shared_ptr<Params>>(m, "Params")

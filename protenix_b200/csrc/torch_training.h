@@ -1,5 +1,5 @@
 // The host path of the training operators: dropout-add from a counter-based generator, relative position encoding, windowed attention,
-// cross entropy of a linear head, rotary positions.
+// cross entropy of a linear head, rotary positions, orthogonalised matrices.
 // Part of torch_ext.cpp (inside its unnamed namespace).  Each is an autograd function whose two directions are launches of the
 // C ABI.  Gradients are computed in kernels, so the ones that are not linear in what they differentiate have no second derivative: a
 // backward pass that is asked to build a graph is refused.
@@ -556,4 +556,31 @@ py::object rotary_embedding(const Tensor& q, const OptTensor& k, const Tensor& p
   const auto back = [&](const Tensor& t, const Tensor& like) { return like.dim() == 4 ? t : t.reshape(like.sizes()); };
   const py::object first = py::cast(back(out.first, q));
   return has(k) ? py::object(py::make_tuple(first, back(out.second, *k))) : first;
+}
+
+// ---- orthogonalised matrices -----------------------------------------------------------------------------------------
+Tensor orthogonalize(const Tensor& g_, const std::vector<double>& coefficients, double eps) {
+  need_cuda(g_, "g");
+  const int type = dtype_code(g_, "g");
+  if (g_.dim() < 2) fail("g must be [..., M, N], got " + shape_of(g_));
+  const int64_t m = g_.size(-2), n = g_.size(-1), batch = m && n ? g_.numel() / (m * n) : 0;
+  const int64_t steps = (int64_t)coefficients.size() / 3;
+  if (coefficients.size() % 3 != 0 || steps < 1 || steps > 1000) fail("coefficients must be 1 to 1000 triples (a, b, c)");
+  for (double c : coefficients)
+    if (!std::isfinite((float)c)) fail("coefficients must be finite");
+  if (!(eps >= 0.0) || !std::isfinite(eps)) fail("eps must not be negative");
+  if (batch > 65535 || m > (1 << 20) || n > (1 << 20)) fail("at most 65535 matrices of 2^20 rows and columns, got " + shape_of(g_));
+  no_tangent(g_, "g");
+  if (at::GradMode::is_enabled() && g_.requires_grad()) fail("orthogonalize is not differentiable: call it on a detached tensor or under no_grad");
+  c10::cuda::CUDAGuard guard(g_.device());
+  const Tensor g = g_.contiguous(), out = at::empty(g.sizes(), g.options());
+  if (batch == 0) return out;
+  const std::vector<float> c(coefficients.begin(), coefficients.end());
+  const int64_t bytes = abi.px_orthogonalize_workspace_bytes(batch, m, n);
+  const Tensor ws = bytes_like(g, bytes);
+  const cudaStream_t st = at::cuda::getCurrentCUDAStream();
+  launch("px_orthogonalize", st, [&] {
+    return abi.px_orthogonalize(g.data_ptr(), out.data_ptr(), batch, m, n, c.data(), (int32_t)steps, eps, type, ws.data_ptr(), bytes, st);
+  });
+  return out;
 }
