@@ -5,7 +5,7 @@ from .cross_entropy import linear_cross_entropy
 from .embedders import RelativePositionEncoding, relative_position_encoding
 from .layer_norm import FusedLayerNorm, LayerNorm
 from .msa import OuterProductMean
-from .orthogonalize import orthogonalize
+from .orthogonalize import Muon, orthogonalize
 from .pairformer import PairformerBlock, PairformerStack
 from .primitives import Linear, LinearNoBias, Transition
 from .recycling import RecyclingTrunk
@@ -24,6 +24,6 @@ __all__ = [
     "TriangleAttentionStartingNode", "TriangleMultiplicationIncoming", "TriangleMultiplicationOutgoing",
     "TriangleMultiplicativeUpdate", "dropout_add_rowwise", "RecyclingTrunk", "OuterProductMean",
     "weights_changed", "dropout_add", "RelativePositionEncoding", "relative_position_encoding",
-    "window_attention", "linear_cross_entropy", "rotary_embedding", "orthogonalize",
+    "window_attention", "linear_cross_entropy", "rotary_embedding", "orthogonalize", "Muon",
 ]
 __version__ = "0.1.0"

@@ -3,7 +3,7 @@
 //
 // Memory bound: every element is read and written once, the angles are few.  Angles: a turn is 2^64, a pair's speed a 64-bit fraction of it, and
 // position * speed modulo 2^64 is exact for any position, where fp32 angles are off by 0.06 at position 10^6; its top 32 bits go to
-// sincospif.  A thread forms the sines of kVec pairs (16 bytes of each half) and uses them for kHeads heads of q and k; threads beside one another take
+// sincospif.  A thread forms the sines of kVec pairs (16 bytes of each half) and uses them for all heads of its group; threads beside one another take
 // neighbouring pairs, then neighbouring heads, so that heads inside the rows of a projection are read as whole lines.
 #include <math.h>
 
@@ -23,7 +23,7 @@ struct RotaryArgs {
   const int64_t* positions;
   int64_t pb, pr, pa;
   int64_t n;
-  int heads, all_heads, head_groups;   // groups: threads that share a token's pairs
+  int heads, all_heads, head_groups;   // group g: heads g, g + head_groups, ..
   int pairs, chunks, d;                // chunks of kVec pairs, then of 2 kVec channels that stay as they are
   int tokens;                          // of a block
   int interleaved, inverse;
@@ -74,24 +74,8 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const __grid_con
       at1 = at0 + kVec;
     }
     const bool second = at1 < a.d;     // the channels that stay may end with the first vector
-    Vec x[kHeads], y[kHeads];
-    T* to[kHeads];
-#pragma unroll
-    for (int h = 0; h < kHeads; ++h) {
-      const int head = group + h * a.head_groups;
-      to[h] = nullptr;
-      if (head < a.all_heads) {
-        const bool is_k = head >= a.heads;
-        const RotaryTensor& t = is_k ? a.k : a.q;
-        const int64_t hh = is_k ? head - a.heads : head;
-        const T* p = (const T*)t.from + b * t.fb + hh * t.fh + row * t.fr;
-        x[h] = *reinterpret_cast<const Vec*>(p + at0);
-        if (second) y[h] = *reinterpret_cast<const Vec*>(p + at1);
-        to[h] = (T*)t.to + b * t.tb + hh * t.th + row * t.tr;
-      }
-    }
+    float c[kVec], s[kVec];
     if (turn) {
-      float c[kVec], s[kVec];
       const int64_t* p = a.positions + b * a.pb + row * a.pr;
 #pragma unroll
       for (int j = 0; j < kVec; ++j) {
@@ -100,50 +84,74 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const __grid_con
         sincospif((float)(int32_t)(turns >> 32) * 4.656612873077393e-10f, &s[j], &c[j]);      // 2^-31: half turns
         if (a.inverse) s[j] = -s[j];
       }
+    }
+#pragma unroll 1
+    for (int head0 = group; head0 < a.all_heads; head0 += kHeads * a.head_groups) {
+      Vec x[kHeads], y[kHeads];
+      T* to[kHeads];
 #pragma unroll
       for (int h = 0; h < kHeads; ++h) {
+        const int head = head0 + h * a.head_groups;
+        to[h] = nullptr;
+        if (head < a.all_heads) {
+          const bool is_k = head >= a.heads;
+          const RotaryTensor& t = is_k ? a.k : a.q;
+          const int64_t hh = is_k ? head - a.heads : head;
+          const T* p = (const T*)t.from + b * t.fb + hh * t.fh + row * t.fr;
+          x[h] = *reinterpret_cast<const Vec*>(p + at0);
+          if (second) y[h] = *reinterpret_cast<const Vec*>(p + at1);
+          to[h] = (T*)t.to + b * t.tb + hh * t.th + row * t.tr;
+        }
+      }
+      if (turn) {
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) {
-          if (a.interleaved && kVec > 1) {
-            // pair j: channels 2 j and 2 j + 1 of the two vectors as one
-            Vec& w = 2 * j < kVec ? x[h] : y[h];
-            const int e = 2 * j < kVec ? 2 * j : 2 * j - kVec;
-            const float u = rotary_float(w.v[e]), v = rotary_float(w.v[(e + 1) % kVec]);
-            w.v[e] = rotary_round<T>(rotary_sum(u, c[j], -v, s[j]));
-            w.v[(e + 1) % kVec] = rotary_round<T>(rotary_sum(v, c[j], u, s[j]));
-          } else {
-            const float u = rotary_float(x[h].v[j]), v = rotary_float(y[h].v[j]);
-            x[h].v[j] = rotary_round<T>(rotary_sum(u, c[j], -v, s[j]));
-            y[h].v[j] = rotary_round<T>(rotary_sum(v, c[j], u, s[j]));
+        for (int h = 0; h < kHeads; ++h) {
+#pragma unroll
+          for (int j = 0; j < kVec; ++j) {
+            if (a.interleaved && kVec > 1) {
+              // pair j: channels 2 j and 2 j + 1 of the two vectors as one
+              Vec& w = 2 * j < kVec ? x[h] : y[h];
+              const int e = 2 * j < kVec ? 2 * j : 2 * j - kVec;
+              const float u = rotary_float(w.v[e]), v = rotary_float(w.v[(e + 1) % kVec]);
+              w.v[e] = rotary_round<T>(rotary_sum(u, c[j], -v, s[j]));
+              w.v[(e + 1) % kVec] = rotary_round<T>(rotary_sum(v, c[j], u, s[j]));
+            } else {
+              const float u = rotary_float(x[h].v[j]), v = rotary_float(y[h].v[j]);
+              x[h].v[j] = rotary_round<T>(rotary_sum(u, c[j], -v, s[j]));
+              y[h].v[j] = rotary_round<T>(rotary_sum(v, c[j], u, s[j]));
+            }
           }
         }
       }
-    }
 #pragma unroll
-    for (int h = 0; h < kHeads; ++h) {
-      if (to[h]) {
-        *reinterpret_cast<Vec*>(to[h] + at0) = x[h];
-        if (second) *reinterpret_cast<Vec*>(to[h] + at1) = y[h];
+      for (int h = 0; h < kHeads; ++h) {
+        if (to[h]) {
+          *reinterpret_cast<Vec*>(to[h] + at0) = x[h];
+          if (second) *reinterpret_cast<Vec*>(to[h] + at1) = y[h];
+        }
       }
     }
   }
 }
 
 template <typename T, int kVec, int kHeads>
-static bool launch_rotary(RotaryArgs& a, int64_t batch, cudaStream_t st) {
-  a.head_groups = (a.all_heads + kHeads - 1) / kHeads;
-  a.chunks = a.pairs / kVec + (a.d - 2 * a.pairs + 2 * kVec - 1) / (2 * kVec);
-  const int per = a.chunks * a.head_groups;
+static bool launch_rotary(RotaryArgs& a, int64_t batch, int groups, cudaStream_t st) {
+  a.head_groups = groups;
+  const int per = a.chunks * groups;
   a.tokens = (int)std::min<int64_t>(a.n, std::max(1, kRotaryThreads / per));
   const int64_t blocks = (a.n + a.tokens - 1) / a.tokens;
   return launch_pdl(rotary_kernel<T, kVec, kHeads>, dim3((unsigned)blocks, (unsigned)batch), kRotaryThreads, 0, st, a);
 }
 
-// Threads that take four heads each form a quarter of the sines, and have four times as many loads on their way.
+// The fewer groups the heads of a token are dealt to, the fewer threads form the same sines; as few as leave two rounds of threads on all SMs.  Four
+// heads at a time are on their way then; where there are not that many threads, one.
 template <typename T, int kVec>
 static bool launch_rotary(RotaryArgs& a, int64_t batch, cudaStream_t st) {
-  const int64_t threads = batch * a.n * a.all_heads * std::max(1, a.d / (2 * kVec));
-  return threads / 4 >= (int64_t)sm_count() * 1024 ? launch_rotary<T, kVec, 4>(a, batch, st) : launch_rotary<T, kVec, 1>(a, batch, st);
+  a.chunks = a.pairs / kVec + (a.d - 2 * a.pairs + 2 * kVec - 1) / (2 * kVec);
+  const int64_t threads = batch * a.n * a.chunks, want = (int64_t)sm_count() * 2048;
+  const int64_t groups = (want + threads - 1) / threads, most = (a.all_heads + 3) / 4;
+  if (groups <= most) return launch_rotary<T, kVec, 4>(a, batch, (int)groups, st);
+  return launch_rotary<T, kVec, 1>(a, batch, (int)std::min<int64_t>(groups, a.all_heads), st);
 }
 template <typename T>
 static bool launch_rotary(RotaryArgs& a, int vec, int64_t batch, cudaStream_t st) {
@@ -200,13 +208,14 @@ extern "C" int32_t px_rotary_turn(const px_rotary* r, const px_rows* q, const px
   a.heads = (int)r->heads, a.all_heads = (int)(r->heads + r->kv_heads);
   a.pairs = (int)pairs, a.d = (int)r->d;
   a.interleaved = r->interleaved != 0, a.inverse = inverse != 0;
+  // one power an axis, or one in all; their products are off by 2^-63 a factor
+  const long double turn = 0.159154943091895335768883763372514362034459645740L * 18446744073709551616.0L;      // 2^64 / 2 pi
+  long double speed = turn, step = powl((long double)r->base, -1.0L / pairs);
   int j = 0;
-  for (int i = 0; i < r->axes; ++i)
-    for (int e = 0; e < r->sections[i]; ++e, ++j) {
-      const long double exponent = r->per_axis ? (long double)e / r->sections[i] : (long double)j / pairs;
-      a.speed[j] = (uint64_t)llrintl(powl((long double)r->base, -exponent) * 0.159154943091895335768883763372514362034459645740L * 18446744073709551616.0L);
-      a.axis[j] = (uint8_t)i;
-    }
+  for (int i = 0; i < r->axes; ++i) {
+    if (r->per_axis && r->sections[i]) speed = turn, step = powl((long double)r->base, -1.0L / r->sections[i]);
+    for (int e = 0; e < r->sections[i]; ++e, ++j, speed *= step) a.speed[j] = (uint64_t)llrintl(speed), a.axis[j] = (uint8_t)i;
+  }
   const cudaStream_t st = (cudaStream_t)stream;
   const bool ok = r->dtype == PX_F32    ? launch_rotary<float>(a, vec, r->batch, st)
                   : r->dtype == PX_BF16 ? launch_rotary<bf16>(a, vec, r->batch, st)

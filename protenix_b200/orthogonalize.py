@@ -33,3 +33,53 @@ def orthogonalize(g: torch.Tensor, steps: int = 5, coefficients: Coefficients = 
     if any(len(c) != 3 for c in triples):
         raise RuntimeError("orthogonalize: coefficients are triples (a, b, c)")
     return native.load().orthogonalize(g, [float(x) for c in triples for x in c], eps)
+
+
+class Muon(torch.optim.Optimizer):
+    """Momentum whose matrices are orthogonalised before they are applied.
+
+    For each parameter p [..., M, N] with gradient g: buf <- momentum buf + g, u = g + momentum buf (``nesterov``) or buf,
+    p <- (1 - lr weight_decay) p - lr sqrt(max(1, M / N)) orthogonalize(u).  Parameters of one shape and type are orthogonalised in one call.  For weights
+    with two axes or more; biases, norms and tables of embeddings want another optimiser beside it.  fp32, bf16 and fp16 CUDA parameters.
+    """
+
+    def __init__(self, params: Iterable[torch.Tensor], lr: float = 0.02, momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0,
+                 steps: int = 5, coefficients: Coefficients = DEFAULT, eps: float = 1e-7) -> None:
+        if not lr >= 0.0 or not 0.0 <= momentum < 1.0 or not weight_decay >= 0.0:
+            raise ValueError("Muon: lr and weight_decay must not be negative, momentum must lie in [0, 1)")
+        super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=steps, coefficients=coefficients, eps=eps))
+
+    def add_param_group(self, group) -> None:
+        super().add_param_group(group)
+        for p in self.param_groups[-1]["params"]:
+            if p.dim() < 2:
+                self.param_groups.pop()
+                raise ValueError(f"Muon: parameters have two axes or more, got one of shape {tuple(p.shape)}")
+
+    @torch.no_grad()
+    def step(self, closure=None) -> Optional[torch.Tensor]:
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            sets = {}
+            for p in group["params"]:
+                if p.grad is not None:
+                    if p.grad.is_sparse:
+                        raise RuntimeError("Muon: sparse gradients are not supported")
+                    sets.setdefault((p.shape, p.dtype, p.device), []).append(p)
+            for (shape, dtype, device), params in sets.items():
+                grads = [p.grad for p in params]
+                for p in params:
+                    if "momentum_buffer" not in self.state[p]:
+                        self.state[p]["momentum_buffer"] = torch.zeros_like(p)
+                held = [self.state[p]["momentum_buffer"] for p in params]
+                torch._foreach_mul_(held, group["momentum"])
+                torch._foreach_add_(held, grads)
+                update = torch._foreach_add(grads, held, alpha=group["momentum"]) if group["nesterov"] else held
+                turned = orthogonalize(torch.stack(update), group["steps"], group["coefficients"], group["eps"])
+                if group["weight_decay"]:
+                    torch._foreach_mul_(params, 1.0 - group["lr"] * group["weight_decay"])
+                torch._foreach_add_(params, list(turned.unbind(0)), alpha=-group["lr"] * max(1.0, shape[-2] / shape[-1]) ** 0.5)
+        return loss
