@@ -5,13 +5,20 @@
 // position * speed modulo 2^64 is exact for any position, where fp32 angles are off by 0.06 at position 10^6; its top 32 bits go to
 // sincospif.  A thread forms the sines of kVec pairs (16 bytes of each half) and uses them for all heads of its group; threads beside one another take
 // neighbouring pairs, then neighbouring heads, so that heads inside the rows of a projection are read as whole lines.
+//
+// 2 x 16384 tokens, 16 + 4 heads of 128, bf16, 336 MB: 60 us (5.6 TB/s; at once on their way 1, 2, 4 heads a thread 66, 60, 59); 5 x 31896, 8 heads of 32, fp32: 56
+// (5.9 TB/s; 59, 56, 59).  With four heads, each vector converted by elements, 116 registers: 101 us.
 #include <math.h>
+#include <string.h>
+
+#include <type_traits>
 
 #include "px_common.cuh"
 
 namespace px {
 
 constexpr int kRotaryPairs = 256, kRotaryThreads = 256;
+constexpr int kHeadsAtOnce = 2, kWantThreads = 2048;      // a thread's heads on their way; threads that an SM shall have
 
 struct RotaryTensor {
   const void* from;
@@ -23,36 +30,93 @@ struct RotaryArgs {
   const int64_t* positions;
   int64_t pb, pr, pa;
   int64_t n;
-  int heads, all_heads, head_groups;   // group g: heads g, g + head_groups, ..
+  int heads, kv_heads, head_groups;   // group g: heads g, g + head_groups, ..
   int pairs, chunks, d;                // chunks of kVec pairs, then of 2 kVec channels that stay as they are
   int tokens;                          // of a block
-  int interleaved, inverse;
+  int inverse;
   uint64_t speed[kRotaryPairs];        // turns a position, times 2^64
   uint8_t axis[kRotaryPairs];
 };
-
-template <typename T>
-__device__ __forceinline__ float rotary_float(T v) { return (float)v; }
-template <typename T>
-__device__ __forceinline__ T rotary_round(float v);
-template <>
-__device__ __forceinline__ float rotary_round<float>(float v) { return v; }
-template <>
-__device__ __forceinline__ bf16 rotary_round<bf16>(float v) { return __float2bfloat16_rn(v); }
-template <>
-__device__ __forceinline__ __half rotary_round<__half>(float v) { return __float2half_rn(v); }
-
-// a b + c d, in the same order in every form of the kernel
-__device__ __forceinline__ float rotary_sum(float a, float b, float c, float d) { return fmaf(a, b, __fmul_rn(c, d)); }
 
 template <typename T, int kVec>
 struct alignas(sizeof(T) * kVec) RotaryVec {
   T v[kVec];
 };
+// Two values at a time where there are two: one conversion for both.
+template <typename T, int kVec>
+__device__ __forceinline__ void rotary_read(const RotaryVec<T, kVec>& x, float* f) {
+  if constexpr (sizeof(T) == 2 && kVec > 1) {
+#pragma unroll
+    for (int j = 0; j < kVec; j += 2) {
+      uint32_t u;
+      memcpy(&u, &x.v[j], 4);
+      const float2 p = unpack16x2<std::is_same<T, __half>::value>(u);
+      f[j] = p.x, f[j + 1] = p.y;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) f[j] = (float)x.v[j];
+  }
+}
+template <typename T, int kVec>
+__device__ __forceinline__ void rotary_write(RotaryVec<T, kVec>& x, const float* f) {
+  if constexpr (sizeof(T) == 2 && kVec > 1) {
+#pragma unroll
+    for (int j = 0; j < kVec; j += 2) {
+      const uint32_t u = pack16x2_inf<std::is_same<T, __half>::value>(f[j], f[j + 1]);
+      memcpy(&x.v[j], &u, 4);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) x.v[j] = (T)f[j];
+  }
+}
+// a b + c d, in the same order in every form of the kernel
+__device__ __forceinline__ float rotary_sum(float a, float b, float c, float d) { return fmaf(a, b, __fmul_rn(c, d)); }
 
-template <typename T, int kVec, int kHeads>
-__global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const __grid_constant__ RotaryArgs a) {
+// The heads first, first + step, .. of one tensor, at channels at0 and at1; kHeads of them are on their way at once.
+template <typename T, int kVec, int kHeads, bool kNeighbours>
+__device__ __forceinline__ void rotary_heads(const RotaryTensor& t, int64_t b, int64_t row, int first, int heads, int step, int at0, int at1, bool second, bool turn,
+                                             const float (&c)[kVec], const float (&s)[kVec]) {
   typedef RotaryVec<T, kVec> Vec;
+  const T* from = (const T*)t.from + b * t.fb + row * t.fr;
+  T* to = (T*)t.to + b * t.tb + row * t.tr;
+#pragma unroll 1
+  for (int h0 = first; h0 < heads; h0 += kHeads * step) {
+    Vec x[kHeads], y[kHeads];
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i) {
+      const int64_t h = h0 + i * step;
+      if (h < heads) {
+        x[i] = *reinterpret_cast<const Vec*>(from + h * t.fh + at0);
+        if (second) y[i] = *reinterpret_cast<const Vec*>(from + h * t.fh + at1);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i) {
+      const int64_t h = h0 + i * step;
+      if (h >= heads) break;
+      if (turn) {
+        float f[2 * kVec], g[2 * kVec];
+        rotary_read<T, kVec>(x[i], f);
+        rotary_read<T, kVec>(y[i], f + kVec);
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) {
+          const int u = kNeighbours ? 2 * j : j, v = kNeighbours ? 2 * j + 1 : j + kVec;
+          g[u] = rotary_sum(f[u], c[j], -f[v], s[j]);
+          g[v] = rotary_sum(f[v], c[j], f[u], s[j]);
+        }
+        rotary_write<T, kVec>(x[i], g);
+        rotary_write<T, kVec>(y[i], g + kVec);
+      }
+      *reinterpret_cast<Vec*>(to + h * t.th + at0) = x[i];
+      if (second) *reinterpret_cast<Vec*>(to + h * t.th + at1) = y[i];
+    }
+  }
+}
+
+template <typename T, int kVec, int kHeads, bool kNeighbours>
+__global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const __grid_constant__ RotaryArgs a) {
   __shared__ uint64_t speed[kRotaryPairs];
   __shared__ uint8_t axis[kRotaryPairs];
   for (int i = threadIdx.x; i < a.pairs; i += kRotaryThreads) speed[i] = a.speed[i], axis[i] = a.axis[i];
@@ -67,14 +131,14 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const __grid_con
     const bool turn = chunk < turning;
     int at0, at1;                      // the two vectors of a head: the halves of the pairs, or neighbours
     if (turn) {
-      at0 = a.interleaved ? 2 * kVec * chunk : kVec * chunk;
-      at1 = a.interleaved ? at0 + kVec : at0 + a.pairs;
+      at0 = kNeighbours ? 2 * kVec * chunk : kVec * chunk;
+      at1 = kNeighbours ? at0 + kVec : at0 + a.pairs;
     } else {
       at0 = 2 * a.pairs + 2 * kVec * (chunk - turning);
       at1 = at0 + kVec;
     }
     const bool second = at1 < a.d;     // the channels that stay may end with the first vector
-    float c[kVec], s[kVec];
+    float c[kVec] = {}, s[kVec] = {};
     if (turn) {
       const int64_t* p = a.positions + b * a.pb + row * a.pr;
 #pragma unroll
@@ -85,83 +149,42 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const __grid_con
         if (a.inverse) s[j] = -s[j];
       }
     }
-#pragma unroll 1
-    for (int head0 = group; head0 < a.all_heads; head0 += kHeads * a.head_groups) {
-      Vec x[kHeads], y[kHeads];
-      T* to[kHeads];
-#pragma unroll
-      for (int h = 0; h < kHeads; ++h) {
-        const int head = head0 + h * a.head_groups;
-        to[h] = nullptr;
-        if (head < a.all_heads) {
-          const bool is_k = head >= a.heads;
-          const RotaryTensor& t = is_k ? a.k : a.q;
-          const int64_t hh = is_k ? head - a.heads : head;
-          const T* p = (const T*)t.from + b * t.fb + hh * t.fh + row * t.fr;
-          x[h] = *reinterpret_cast<const Vec*>(p + at0);
-          if (second) y[h] = *reinterpret_cast<const Vec*>(p + at1);
-          to[h] = (T*)t.to + b * t.tb + hh * t.th + row * t.tr;
-        }
-      }
-      if (turn) {
-#pragma unroll
-        for (int h = 0; h < kHeads; ++h) {
-#pragma unroll
-          for (int j = 0; j < kVec; ++j) {
-            if (a.interleaved && kVec > 1) {
-              // pair j: channels 2 j and 2 j + 1 of the two vectors as one
-              Vec& w = 2 * j < kVec ? x[h] : y[h];
-              const int e = 2 * j < kVec ? 2 * j : 2 * j - kVec;
-              const float u = rotary_float(w.v[e]), v = rotary_float(w.v[(e + 1) % kVec]);
-              w.v[e] = rotary_round<T>(rotary_sum(u, c[j], -v, s[j]));
-              w.v[(e + 1) % kVec] = rotary_round<T>(rotary_sum(v, c[j], u, s[j]));
-            } else {
-              const float u = rotary_float(x[h].v[j]), v = rotary_float(y[h].v[j]);
-              x[h].v[j] = rotary_round<T>(rotary_sum(u, c[j], -v, s[j]));
-              y[h].v[j] = rotary_round<T>(rotary_sum(v, c[j], u, s[j]));
-            }
-          }
-        }
-      }
-#pragma unroll
-      for (int h = 0; h < kHeads; ++h) {
-        if (to[h]) {
-          *reinterpret_cast<Vec*>(to[h] + at0) = x[h];
-          if (second) *reinterpret_cast<Vec*>(to[h] + at1) = y[h];
-        }
-      }
-    }
+    rotary_heads<T, kVec, kHeads, kNeighbours>(a.q, b, row, group, a.heads, a.head_groups, at0, at1, second, turn, c, s);
+    rotary_heads<T, kVec, kHeads, kNeighbours>(a.k, b, row, group, a.kv_heads, a.head_groups, at0, at1, second, turn, c, s);
   }
 }
 
-template <typename T, int kVec, int kHeads>
+template <typename T, int kVec, int kHeads, bool kNeighbours>
 static bool launch_rotary(RotaryArgs& a, int64_t batch, int groups, cudaStream_t st) {
   a.head_groups = groups;
   const int per = a.chunks * groups;
   a.tokens = (int)std::min<int64_t>(a.n, std::max(1, kRotaryThreads / per));
   const int64_t blocks = (a.n + a.tokens - 1) / a.tokens;
-  return launch_pdl(rotary_kernel<T, kVec, kHeads>, dim3((unsigned)blocks, (unsigned)batch), kRotaryThreads, 0, st, a);
+  return launch_pdl(rotary_kernel<T, kVec, kHeads, kNeighbours>, dim3((unsigned)blocks, (unsigned)batch), kRotaryThreads, 0, st, a);
 }
 
-// The fewer groups the heads of a token are dealt to, the fewer threads form the same sines; as few as leave two rounds of threads on all SMs.  Four
-// heads at a time are on their way then; where there are not that many threads, one.
-template <typename T, int kVec>
+// The fewer groups the heads of a token are dealt to, the fewer threads form the same sines; as few as leave every SM kWantThreads.
+template <typename T, int kVec, bool kNeighbours>
 static bool launch_rotary(RotaryArgs& a, int64_t batch, cudaStream_t st) {
   a.chunks = a.pairs / kVec + (a.d - 2 * a.pairs + 2 * kVec - 1) / (2 * kVec);
-  const int64_t threads = batch * a.n * a.chunks, want = (int64_t)sm_count() * 2048;
-  const int64_t groups = (want + threads - 1) / threads, most = (a.all_heads + 3) / 4;
-  if (groups <= most) return launch_rotary<T, kVec, 4>(a, batch, (int)groups, st);
-  return launch_rotary<T, kVec, 1>(a, batch, (int)std::min<int64_t>(groups, a.all_heads), st);
+  const int64_t threads = batch * a.n * a.chunks, want = (int64_t)sm_count() * kWantThreads, groups = (want + threads - 1) / threads;
+  const int heads = std::max(a.heads, a.kv_heads);
+  if (groups * kHeadsAtOnce <= heads) return launch_rotary<T, kVec, kHeadsAtOnce, kNeighbours>(a, batch, (int)groups, st);
+  return launch_rotary<T, kVec, 1, kNeighbours>(a, batch, (int)std::min<int64_t>(groups, heads), st);
 }
-template <typename T>
+template <typename T, bool kNeighbours>
 static bool launch_rotary(RotaryArgs& a, int vec, int64_t batch, cudaStream_t st) {
   switch (vec) {
     case 8:
-      if constexpr (sizeof(T) == 2) return launch_rotary<T, 8>(a, batch, st);
-    case 4: return launch_rotary<T, 4>(a, batch, st);
-    case 2: return launch_rotary<T, 2>(a, batch, st);
-    default: return launch_rotary<T, 1>(a, batch, st);
+      if constexpr (sizeof(T) == 2) return launch_rotary<T, 8, kNeighbours>(a, batch, st);
+    case 4: return launch_rotary<T, 4, kNeighbours>(a, batch, st);
+    case 2: return launch_rotary<T, 2, kNeighbours>(a, batch, st);
+    default: return launch_rotary<T, 1, kNeighbours>(a, batch, st);
   }
+}
+template <typename T>
+static bool launch_rotary(RotaryArgs& a, int vec, bool neighbours, int64_t batch, cudaStream_t st) {
+  return neighbours ? launch_rotary<T, true>(a, vec, batch, st) : launch_rotary<T, false>(a, vec, batch, st);
 }
 
 }  // namespace px
@@ -205,9 +228,9 @@ extern "C" int32_t px_rotary_turn(const px_rotary* r, const px_rows* q, const px
   a.positions = r->positions;
   a.pb = r->position_batch, a.pr = r->position_row, a.pa = r->position_axis;
   a.n = r->n;
-  a.heads = (int)r->heads, a.all_heads = (int)(r->heads + r->kv_heads);
+  a.heads = (int)r->heads, a.kv_heads = (int)r->kv_heads;
   a.pairs = (int)pairs, a.d = (int)r->d;
-  a.interleaved = r->interleaved != 0, a.inverse = inverse != 0;
+  a.inverse = inverse != 0;
   // one power an axis, or one in all; their products are off by 2^-63 a factor
   const long double turn = 0.159154943091895335768883763372514362034459645740L * 18446744073709551616.0L;      // 2^64 / 2 pi
   long double speed = turn, step = powl((long double)r->base, -1.0L / pairs);
@@ -217,8 +240,8 @@ extern "C" int32_t px_rotary_turn(const px_rotary* r, const px_rows* q, const px
     for (int e = 0; e < r->sections[i]; ++e, ++j, speed *= step) a.speed[j] = (uint64_t)llrintl(speed), a.axis[j] = (uint8_t)i;
   }
   const cudaStream_t st = (cudaStream_t)stream;
-  const bool ok = r->dtype == PX_F32    ? launch_rotary<float>(a, vec, r->batch, st)
-                  : r->dtype == PX_BF16 ? launch_rotary<bf16>(a, vec, r->batch, st)
-                                        : launch_rotary<__half>(a, vec, r->batch, st);
+  const bool ok = r->dtype == PX_F32    ? launch_rotary<float>(a, vec, r->interleaved != 0, r->batch, st)
+                  : r->dtype == PX_BF16 ? launch_rotary<bf16>(a, vec, r->interleaved != 0, r->batch, st)
+                                        : launch_rotary<__half>(a, vec, r->interleaved != 0, r->batch, st);
   return ok ? PX_OK : PX_ERR_LAUNCH;
 }
