@@ -468,31 +468,31 @@ typedef struct {
 PX_API int32_t px_rotary_turn(const px_rotary* r, const px_rows* q, const px_rows* q_out, const px_rows* k, const px_rows* k_out, int32_t inverse, void* stream);
 
 /* ---- Softmax cross entropy of a linear head, without its logits (training path) ----------------
- * l = x w^T + bias for rows x [rows][c] and classes w [classes][c] (PX_BF16 or PX_F16, row strides in elements), bias fp32 or NULL;
+ * l = x w^T + bias for rows x [rows][c] and classes w [classes][c] (PX_BF16 or PX_F16, row strides in elements), bias or NULL;
  * loss_i = lse_i - (1 - smoothing) l_i,target - smoothing / classes sum_v l_iv.  Rows whose target is `ignore` have loss 0 and take no part in
  * any gradient, whatever they hold; a target outside the classes makes its row's loss, and the gradients that it enters, NaN.
  * px_head_loss_fwd writes norm [rows][2] (reference and sum of the exponentials, for the backward pass), the rows' losses [rows] (NULL: not wanted) and their sum or mean over the rows that count
  * (total, with 1 / count or 1 in `inverse` for the backward pass; NULL: not wanted; the mean of nothing is NaN).
- * px_head_loss_bwd writes those of dx [rows][c], dw [classes][c] (type of x, contiguous) and dbias [classes] (fp32) that are not NULL, from the gradient of
+ * px_head_loss_bwd writes those of dx [rows][c], dw [classes][c] (type of x, contiguous) and dbias [classes] (type of the bias) that are not NULL, from the gradient of
  * the total (each = 0: one number) or of the rows' losses (each = 1, `inverse` not read).  It forms the logits again, for so many classes at a time
  * that 16 bits a logit stay within 512 MiB (256 classes at least).  Sums are fp32, across rows fp64, and have a fixed order.  c a multiple of 8, pointers aligned
  * to 16 bytes, workspaces to 256.  No counterpart in the reference, whose heads (protenix/model/modules/head.py) leave the loss to torch. */
 typedef struct {
   const void* x;
   const void* w;
-  const float* bias;
+  const void* bias;
   const int64_t* target;
   int64_t rows, c, classes, x_stride, w_stride;
   int64_t ignore;
   float smoothing;
-  int32_t dtype;
+  int32_t dtype, bias_dtype; /* of the bias: PX_F32, or dtype */
 } px_head;
 PX_API int64_t px_head_loss_workspace_bytes(int64_t rows, int64_t classes);
 PX_API int32_t px_head_loss_fwd(const px_head* head, float* norm, float* losses, float* total, float* inverse, int32_t mean, void* workspace,
                          int64_t workspace_bytes, void* stream);
 PX_API int64_t px_head_loss_bwd_workspace_bytes(const px_head* head, int32_t dx, int32_t dw, int32_t dbias);
 PX_API int32_t px_head_loss_bwd(const px_head* head, const float* norm, const float* grad, int32_t each, const float* inverse, void* dx, void* dw,
-                         float* dbias, void* workspace, int64_t workspace_bytes, void* stream);
+                         void* dbias, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* ---- Orthogonalised matrices (Newton-Schulz) ------------------------------------------------------
  * out = P_steps(... P_1(g / (|g| + eps))) for each of `batch` matrices [m][n], |g| the root of the sum of squares,

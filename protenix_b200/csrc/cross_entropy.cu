@@ -13,33 +13,17 @@
 //
 // Rows that are ignored take no part whatever they hold: their dl is zero by selection, and where one holds an infinity or a NaN (which a zero
 // weight would not silence) dW takes a copy of x in which those rows are zero; the copy is made only then.
-#include <math_constants.h>
-
-#include "px_gemm.cuh"
+#include "px_head_small.cuh"
 
 namespace px {
 
 constexpr int64_t kPieceBytes = 512ll << 20;
 constexpr int kScanBlocks = 592;
-constexpr float kDlScaleF16 = 16384.f;
-
-// What the small kernels of a backward pass leave for the products.
-struct LossScale {
-  float out;            // what dx and dW are multiplied by
-  float each;           // what the gradient of a row's loss is multiplied by, so that the largest is one
-  uint32_t dirty;       // an ignored row holds what is not finite
-};
-
-// What exponentials are taken relative to, in powers of two, for a maximum that may be that of nothing.
-__device__ __forceinline__ float reference(float m) { return m == -CUDART_INF_F ? 0.f : m; }
-
-// A row's part in the loss: its class, or a class that no column has.
-__device__ __forceinline__ bool row_counts(int64_t target, int64_t ignore) { return target != ignore; }
 
 // ---- forward ---------------------------------------------------------------------------------------------------------
 struct EpiStats {
   const int64_t* target;
-  const float* bias;        // or NULL
+  HeadBias bias;
   float2* part;             // [tiles_n][rows]: maximum times log2(e), sum of exponentials relative to it
   float* part_sum;          // [tiles_n][rows]: sum of logits, or NULL
   float* hit;               // [rows]: logit of the row's class
@@ -66,19 +50,7 @@ struct EpiStats {
       float v[32];
 #pragma unroll
       for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
-      if (bias) {
-        if (left >= 32) {
-#pragma unroll
-          for (int j = 0; j < 32; j += 4) {
-            const float4 b = __ldg(reinterpret_cast<const float4*>(bias + base + c + j));
-            v[j] += b.x, v[j + 1] += b.y, v[j + 2] += b.z, v[j + 3] += b.w;
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (j < left) v[j] += __ldg(bias + base + c + j);
-        }
-      }
+      add_bias(v, bias, base + c, left);
       if (left < 32) {
 #pragma unroll
         for (int j = 0; j < 32; ++j)
@@ -173,11 +145,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) loss_join_kernel(const JoinAr
     const bool counts = row_counts(t, a.ignore);
     float loss = 0.f;
     if (counts) {
-      // all logits relative to the same reference: nothing of its size is left in the difference
-      loss = CUDART_NAN_F;
-      if (t >= 0 && t < a.classes) loss = log2f(s) - (1.f - a.smooth) * fmaf(a.hit[row], kLog2e, -ref);
-      if (a.part_sum) loss -= a.smooth * fmaf(sum / (float)a.classes, kLog2e, -ref);
-      loss = loss < 0.f ? 0.f : loss * 0.6931471805599453f;
+      loss = row_loss(s, ref, a.hit[row], t >= 0 && t < a.classes, a.smooth, sum, a.classes);
       l = loss, c = 1.0;
     }
     a.norm[row] = make_float2(ref, s);
@@ -295,23 +263,11 @@ __global__ void __launch_bounds__(256) loss_prepare_kernel(const ScanArgs a, con
   }
 }
 
-// v[0] of lane j = the sum of v[j] over the lanes: at each step half of the columns go to the other half of the lanes.
-template <int kHalf = 16>
-__device__ __forceinline__ void column_sums(float (&v)[32], int lane) {
-  const bool up = (lane & kHalf) != 0;
-#pragma unroll
-  for (int j = 0; j < kHalf; ++j) {
-    const float give = up ? v[j] : v[j + kHalf], keep = up ? v[j + kHalf] : v[j];
-    v[j] = keep + __shfl_xor_sync(0xffffffffu, give, kHalf);
-  }
-  if constexpr (kHalf > 1) column_sums<kHalf / 2>(v, lane);
-}
-
 // ---- backward: dl ----------------------------------------------------------------------------------------------------
 struct EpiLogitGrad {
   CUtensorMap out;          // dl [rows][classes of the piece], boxes of 32 x 64
   const int64_t* target;
-  const float* bias;        // of the piece, or NULL
+  HeadBias bias;            // of the piece
   const float2* norm;
   const float* grad;        // of each row's loss, or NULL
   const LossScale* scale;
@@ -356,19 +312,7 @@ struct EpiLogitGrad {
         float v[32];
 #pragma unroll
         for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
-        if (bias) {
-          if (left >= 32) {
-#pragma unroll
-            for (int j = 0; j < 32; j += 4) {
-              const float4 b = __ldg(reinterpret_cast<const float4*>(bias + base + c + h + j));
-              v[j] += b.x, v[j + 1] += b.y, v[j + 2] += b.z, v[j + 3] += b.w;
-            }
-          } else {
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (j < left) v[j] += __ldg(bias + base + c + h + j);
-          }
-        }
+        add_bias(v, bias, base + c + h, left);
 #pragma unroll
         for (int j = 0; j < 32; ++j) v[j] = fmaf(over, fast_exp2(fmaf(v[j], kLog2e, ref)), -less);
         if (mine >= c + h && mine < c + h + 32) {
@@ -408,7 +352,8 @@ struct EpiLogitGrad {
 };
 
 // db of a piece: a warp's lanes along the classes, the groups of rows over the warps, in a fixed order.
-__global__ void __launch_bounds__(512) loss_bias_kernel(const float* __restrict__ part, float* __restrict__ db, const LossScale* __restrict__ scale, int classes, int groups) {
+__global__ void __launch_bounds__(512) loss_bias_kernel(const float* __restrict__ part, void* __restrict__ db, int type, const LossScale* __restrict__ scale,
+                                                        int classes, int groups) {
   __shared__ float x[16][32];
   pdl_wait();
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, v = blockIdx.x * 32 + lane;
@@ -420,7 +365,7 @@ __global__ void __launch_bounds__(512) loss_bias_kernel(const float* __restrict_
   if (w == 0 && v < classes) {
     float all = 0.f;
     for (int i = 0; i < 16; ++i) all += x[i][lane];
-    db[v] = all * scale->out;
+    bias_store(db, type, v, all * scale->out);
   }
 }
 
@@ -586,6 +531,7 @@ static int32_t check_head(const px_head* h) {
   if (!h->x || !h->w || !h->target || h->x_stride < h->c || h->w_stride < h->c || h->x_stride % 8 || h->w_stride % 8) return PX_ERR_BAD_ARG;
   if (((uintptr_t)h->x | (uintptr_t)h->w | (uintptr_t)h->bias) & 15) return PX_ERR_BAD_ARG;
   if (!(h->smoothing >= 0.f && h->smoothing <= 1.f)) return PX_ERR_BAD_ARG;
+  if (h->bias_dtype != PX_F32 && h->bias_dtype != h->dtype) return PX_ERR_UNSUPPORTED;
   if ((h->dtype != PX_BF16 && h->dtype != PX_F16) || h->c % 8 || h->c > (1 << 20) || h->classes > (1 << 24) || h->rows > (1 << 26)) return PX_ERR_UNSUPPORTED;
   if (up(h->rows, 128) / 128 * (up(h->classes, 64) / 64) > (1ll << 30)) return PX_ERR_UNSUPPORTED;
   return PX_OK;
@@ -622,6 +568,45 @@ static int32_t gather(const float* slots, void* out, const LossScale* scale, con
   return launch_pdl(loss_gather_kernel, dim3((unsigned)blocks), 256, 0, st, slots, (uint16_t*)out, scale, target, ignore, rows, (int)c, splits, f16) ? PX_OK : PX_ERR_LAUNCH;
 }
 
+// ---- heads that fit an SM --------------------------------------------------------------------------------------------
+static bool small_head(int64_t c, int64_t classes) { return c <= kSmallC && classes <= kSmallV; }
+static int64_t small_vp(int64_t classes) { return classes <= 64 ? 64 : 128; }
+
+static bool small_args(SmallArgs* a, const px_head& h) {
+  const bool f16 = h.dtype == PX_F16;
+  const int vp = (int)small_vp(h.classes);
+  *a = {};
+  if (!gemm_map(&a->x, f16, h.x, h.c, h.rows, 1, h.x_stride, h.rows * h.x_stride, 128) || !gemm_map(&a->w, f16, h.w, h.c, h.classes, 1, h.w_stride, h.classes * h.w_stride, vp))
+    return false;
+  a->dx = a->x;
+  a->target = h.target, a->bias = {h.bias, h.bias_dtype}, a->ignore = h.ignore, a->rows = (int)h.rows, a->classes = (int)h.classes;
+  a->panels = (int)(up(h.c, 64) / 64), a->tiles = (int)(up(h.rows, 128) / 128), a->f16 = f16, a->smooth = h.smoothing;
+  a->idesc_logits = umma_idesc_16(128, vp, f16, f16);
+  a->idesc_dx = umma_idesc_16(128, 64 * a->panels, f16, f16, false, true);
+  a->idesc_dw = umma_idesc_16(128, vp, f16, f16, true, true);
+  return true;
+}
+static int small_ctas(int64_t rows) { return even_grid(up(rows, 128) / 128, sm_count()); }
+template <bool kBackward, int kVp>
+static bool launch_small(const SmallArgs& a, cudaStream_t st) {
+  typedef SmallShape<kBackward, kVp> S;
+  static SmemLimit limit;
+  return limit.set(small_head_kernel<kBackward, kVp>, S::kSmem) && launch_pdl(small_head_kernel<kBackward, kVp>, dim3(small_ctas(a.rows)), kSmallThreads, S::kSmem, st, a);
+}
+template <bool kBackward>
+static bool launch_small(const SmallArgs& a, cudaStream_t st) {
+  return a.classes <= 64 ? launch_small<kBackward, 64>(a, st) : launch_small<kBackward, 128>(a, st);
+}
+struct SmallPlan {
+  int64_t scale, found, w, b, bytes;
+};
+static SmallPlan small_plan(const px_head& h) {
+  const int64_t ctas = small_ctas(h.rows), vp = small_vp(h.classes);
+  SmallPlan p;
+  p.scale = 0, p.found = 1024, p.w = p.found + up(kScanBlocks * 8, 1024), p.b = p.w + ctas * 128 * vp * 4, p.bytes = p.b + ctas * 4 * vp * 4;
+  return p;
+}
+
 }  // namespace px
 
 using namespace px;
@@ -642,6 +627,13 @@ extern "C" int32_t px_head_loss_fwd(const px_head* head, float* norm, float* los
   if (workspace_bytes < px_head_loss_workspace_bytes(h.rows, h.classes)) return PX_ERR_WORKSPACE;
   if (!have_context()) return PX_ERR_LAUNCH;
   const cudaStream_t st = (cudaStream_t)stream;
+  if (small_head(h.c, h.classes)) {
+    SmallArgs a;
+    if (!small_args(&a, h)) return PX_ERR_LAUNCH;
+    a.norm = (float2*)norm, a.losses = losses, a.sums = total ? (double2*)workspace : nullptr;
+    if (!launch_small<false>(a, st)) return PX_ERR_LAUNCH;
+    return !total || launch_pdl(small_total_kernel, dim3(1), 32, 0, st, (const double2*)workspace, small_ctas(h.rows), total, inverse, (int)mean) ? PX_OK : PX_ERR_LAUNCH;
+  }
   const HeadCut c = cut(h.rows, h.classes, h.c, false, 64);
   char* at = (char*)workspace;
   uint32_t* arrivals = (uint32_t*)at;
@@ -652,7 +644,7 @@ extern "C" int32_t px_head_loss_fwd(const px_head* head, float* norm, float* los
   at += up((h.rows + 31) / 32 * 16, 1024);
   float2* part = (float2*)at;
   at += up(c.t.tiles_n * h.rows * 8, 1024);
-  EpiStats epi = {h.target, h.bias, part, h.smoothing > 0.f ? (float*)at : nullptr, hit, arrivals, (int)h.rows, (int)h.classes};
+  EpiStats epi = {h.target, {h.bias, h.bias_dtype}, part, h.smoothing > 0.f ? (float*)at : nullptr, hit, arrivals, (int)h.rows, (int)h.classes};
   if (const int32_t status = launch_logits(h, 0, h.classes, c, epi, st)) return status;
   JoinArgs j = {part, epi.part_sum, hit, h.target, (float2*)norm, losses, total, inverse, sums, arrivals, h.ignore, (int)h.rows, (int)h.classes, c.t.tiles_n, mean, h.smoothing};
   return launch_pdl(loss_join_kernel, dim3((unsigned)((h.rows + 31) / 32)), 32 * kJoinWarps, 0, st, j) ? PX_OK : PX_ERR_LAUNCH;
@@ -660,41 +652,64 @@ extern "C" int32_t px_head_loss_fwd(const px_head* head, float* norm, float* los
 
 extern "C" int64_t px_head_loss_bwd_workspace_bytes(const px_head* head, int32_t dx, int32_t dw, int32_t dbias) {
   if (!head || head->rows <= 0 || head->c <= 0 || head->classes <= 0) return 0;
-  return head_plan(*head, dx, dw, dbias).bytes;
+  return small_head(head->c, head->classes) ? small_plan(*head).bytes : head_plan(*head, dx, dw, dbias).bytes;
 }
 
 extern "C" int32_t px_head_loss_bwd(const px_head* head, const float* norm, const float* grad, int32_t each, const float* inverse, void* dx, void* dw,
-                                    float* dbias, void* workspace, int64_t workspace_bytes, void* stream) {
+                                    void* dbias, void* workspace, int64_t workspace_bytes, void* stream) {
   if (const int32_t status = check_head(head)) return status;
   const px_head& h = *head;
   if (h.rows == 0 || !norm || !grad || (!each && !inverse) || !workspace || ((uintptr_t)workspace & 255)) return PX_ERR_BAD_ARG;
   if (((uintptr_t)dx | (uintptr_t)dw | (uintptr_t)norm) & 15) return PX_ERR_BAD_ARG;
-  const HeadPlan p = head_plan(h, dx, dw, dbias);
-  if (workspace_bytes < p.bytes) return PX_ERR_WORKSPACE;
+  if (workspace_bytes < px_head_loss_bwd_workspace_bytes(head, dx != nullptr, dw != nullptr, dbias != nullptr)) return PX_ERR_WORKSPACE;
   if (!have_context()) return PX_ERR_LAUNCH;
   if (!dx && !dw && !dbias) return PX_OK;
   const cudaStream_t st = (cudaStream_t)stream;
   const bool f16 = h.dtype == PX_F16;
+  const float dl_scale = f16 ? kDlScaleF16 : 1.f;
+  const int64_t bias_size = h.bias_dtype == PX_F32 ? 4 : 2;
+  const int scan_blocks = (int)std::min<int64_t>((h.rows + 255) / 256, kScanBlocks);
   char* const ws = (char*)workspace;
+  if (small_head(h.c, h.classes)) {
+    const SmallPlan p = small_plan(h);
+    SmallArgs a;
+    if (!small_args(&a, h) || (dx && !out_map(&a.dx, type16(f16), 2, dx, h.c, h.rows, h.c, 1))) return PX_ERR_LAUNCH;
+    a.norm = (float2*)const_cast<float*>(norm), a.grad = grad, a.inverse = inverse, a.want_dx = dx != nullptr;
+    a.part_w = dw ? (float*)(ws + p.w) : nullptr, a.part_b = dbias ? (float*)(ws + p.b) : nullptr;
+    if (each) {
+      const ScanArgs scan = {h.x, h.x_stride, h.target, grad, (uint2*)(ws + p.found), h.ignore, h.rows, 0, each};
+      a.scale = (const LossScale*)(ws + p.scale);
+      if (!launch_pdl(loss_scan_kernel, dim3(scan_blocks), 256, 0, st, scan, f16) ||
+          !launch_pdl(loss_prepare_kernel, dim3(1), 256, 0, st, scan, inverse, nullptr, (LossScale*)(ws + p.scale), scan_blocks, dl_scale))
+        return PX_ERR_LAUNCH;
+    }
+    if (!launch_small<true>(a, st)) return PX_ERR_LAUNCH;
+    if (!dw && !dbias) return PX_OK;
+    const int vp = (int)small_vp(h.classes), groups = vp / 32;
+    return launch_pdl(small_join_kernel, dim3((unsigned)(groups * (h.c / 8 + 1))), 256, 0, st, (const float*)a.part_w, (const float*)a.part_b, (uint16_t*)dw, dbias,
+                      small_ctas(h.rows), vp, (int)h.c, (int)h.classes, (int)f16, (int)h.bias_dtype)
+               ? PX_OK
+               : PX_ERR_LAUNCH;
+  }
+  const HeadPlan p = head_plan(h, dx, dw, dbias);
   LossScale* scale = (LossScale*)(ws + p.scale);
   uint16_t* dl = (uint16_t*)(ws + p.dl);
   uint16_t* clean = (uint16_t*)(ws + p.clean);
   float* part_bias = (float*)(ws + p.db_at);
   const ScanArgs scan = {h.x, h.x_stride, h.target, grad, (uint2*)(ws + p.found), h.ignore, h.rows, dw ? (int)h.c : 0, each};
-  const int scan_blocks = (int)std::min<int64_t>((h.rows + 255) / 256, kScanBlocks);
   if (!launch_pdl(loss_scan_kernel, dim3(scan_blocks), 256, 0, st, scan, f16)) return PX_ERR_LAUNCH;
   const int copy_blocks = dw ? (int)std::min<int64_t>((h.rows * h.c / 8 + 255) / 256, 2 * sm_count()) : 1;
-  if (!launch_pdl(loss_prepare_kernel, dim3(copy_blocks), 256, 0, st, scan, inverse, clean, scale, scan_blocks, f16 ? kDlScaleF16 : 1.f)) return PX_ERR_LAUNCH;
+  if (!launch_pdl(loss_prepare_kernel, dim3(copy_blocks), 256, 0, st, scan, inverse, clean, scale, scan_blocks, dl_scale)) return PX_ERR_LAUNCH;
 
   for (int64_t i = 0; i < p.pieces; ++i) {
     const int64_t first = i * p.piece, vc = std::min(p.piece, h.classes - first);
     EpiLogitGrad el = {};
     if (!out_map(&el.out, type16(f16), 2, dl, vc, h.rows, p.ld, 1)) return PX_ERR_LAUNCH;
-    el.target = h.target, el.bias = h.bias ? h.bias + first : nullptr, el.norm = (const float2*)norm, el.grad = each ? grad : nullptr, el.scale = scale;
+    el.target = h.target, el.bias = {h.bias ? (const char*)h.bias + first * bias_size : nullptr, h.bias_dtype}, el.norm = (const float2*)norm, el.grad = each ? grad : nullptr, el.scale = scale;
     el.part_bias = dbias ? part_bias : nullptr, el.ignore = h.ignore, el.rows = (int)h.rows, el.classes = (int)vc, el.first = (int)first;
     el.all_classes = (int)h.classes, el.smooth = h.smoothing, el.f16 = f16;
     if (const int32_t status = launch_logits(h, first, vc, p.logits, el, st)) return status;
-    if (dbias && !launch_pdl(loss_bias_kernel, dim3((unsigned)((vc + 31) / 32)), 512, 0, st, (const float*)part_bias, dbias + first, (const LossScale*)scale, (int)vc,
+    if (dbias && !launch_pdl(loss_bias_kernel, dim3((unsigned)((vc + 31) / 32)), 512, 0, st, (const float*)part_bias, (void*)((char*)dbias + first * bias_size), (int)h.bias_dtype, (const LossScale*)scale, (int)vc,
                              (int)((h.rows + 31) / 32)))
       return PX_ERR_LAUNCH;
     if (dx) {

@@ -1,0 +1,90 @@
+// What the kernels of the cross entropy share (cross_entropy.cu, px_head_small.cuh).
+#pragma once
+#include <math_constants.h>
+
+#include "px_gemm.cuh"
+
+namespace px {
+
+constexpr float kDlScaleF16 = 16384.f;
+
+// What the small kernels of a backward pass leave for the products.
+struct LossScale {
+  float out;            // what dx and dW are multiplied by
+  float each;           // what the gradient of a row's loss is multiplied by, so that the largest is one
+  uint32_t dirty;       // an ignored row holds what is not finite
+};
+
+// What exponentials are taken relative to, in powers of two, for a maximum that may be that of nothing.
+__device__ __forceinline__ float reference(float m) { return m == -CUDART_INF_F ? 0.f : m; }
+
+// A row's part in the loss: its class, or a class that no column has.
+__device__ __forceinline__ bool row_counts(int64_t target, int64_t ignore) { return target != ignore; }
+
+// The loss of a row from its sum of exponentials, all logits relative to the same reference (in powers of two): nothing of its size is left in the
+// difference.  valid: the row's class is one; hit: its logit; all: the sum of the logits (smooth > 0).
+__device__ __forceinline__ float row_loss(float sum, float ref, float hit, bool valid, float smooth, float all, int classes) {
+  float loss = CUDART_NAN_F;
+  if (valid) loss = log2f(sum) - (1.f - smooth) * fmaf(hit, kLog2e, -ref);
+  if (smooth > 0.f) loss -= smooth * fmaf(all / (float)classes, kLog2e, -ref);
+  return loss < 0.f ? 0.f : loss * 0.6931471805599453f;
+}
+
+// A bias in fp32 or 16 bits, 16-byte aligned.
+struct HeadBias {
+  const void* at;      // or NULL
+  int type;
+};
+__device__ __forceinline__ float bias_value(const HeadBias& b, int i) {
+  return b.type == PX_F32 ? __ldg((const float*)b.at + i) : b.type == PX_F16 ? __half2float(__ldg((const __half*)b.at + i)) : __bfloat162float(__ldg((const bf16*)b.at + i));
+}
+// v += the bias of 32 classes from `first` (a multiple of 32) on, of which `left` are there.
+__device__ __forceinline__ void add_bias(float (&v)[32], const HeadBias& b, int first, int left) {
+  if (!b.at) return;
+  if (left < 32) {
+    // the classes of the last tile one by one: lane j has the j-th
+    const int lane = threadIdx.x & 31;
+    const float mine = lane < left ? bias_value(b, first + lane) : 0.f;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] += __shfl_sync(0xffffffffu, mine, j);
+  } else if (b.type == PX_F32) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 4) {
+      const float4 x = __ldg(reinterpret_cast<const float4*>((const float*)b.at + first + j));
+      v[j] += x.x, v[j + 1] += x.y, v[j + 2] += x.z, v[j + 3] += x.w;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; j += 8) {
+      const uint4 u = __ldg(reinterpret_cast<const uint4*>((const uint16_t*)b.at + first + j));
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 x = b.type == PX_F16 ? unpack_f16x2(w[k]) : unpack_bf16x2(w[k]);
+        v[j + 2 * k] += x.x, v[j + 2 * k + 1] += x.y;
+      }
+    }
+  }
+}
+__device__ __forceinline__ void bias_store(void* to, int type, int i, float v) {
+  if (type == PX_F32)
+    ((float*)to)[i] = v;
+  else if (type == PX_F16)
+    ((__half*)to)[i] = __float2half_rn(v);
+  else
+    ((bf16*)to)[i] = __float2bfloat16_rn(v);
+}
+
+// v[0] of lane j = the sum of v[j] over the lanes: at each step half of the columns go to the other half of the lanes.
+template <int kHalf = 16>
+__device__ __forceinline__ void column_sums(float (&v)[32], int lane) {
+  const bool up = (lane & kHalf) != 0;
+#pragma unroll
+  for (int j = 0; j < kHalf; ++j) {
+    const float give = up ? v[j] : v[j + kHalf], keep = up ? v[j + kHalf] : v[j];
+    v[j] = keep + __shfl_xor_sync(0xffffffffu, give, kHalf);
+  }
+  if constexpr (kHalf > 1) column_sums<kHalf / 2>(v, lane);
+}
+
+}  // namespace px

@@ -339,7 +339,7 @@ int64_t row_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.siz
 px_head head_of(const Tensor& x, const Tensor& w, const Tensor& bias, const Tensor& target, const HeadCall& c) {
   px_head h = {};
   h.x = x.data_ptr(), h.w = w.data_ptr(), h.target = (const int64_t*)target.data_ptr();
-  h.bias = bias.defined() ? (const float*)bias.data_ptr() : nullptr;
+  h.bias = bias.defined() ? bias.data_ptr() : nullptr, h.bias_dtype = bias.defined() ? dtype_code(bias, "bias") : PX_F32;
   h.rows = x.size(0), h.c = x.size(1), h.classes = w.size(0);
   h.x_stride = row_stride(x), h.w_stride = row_stride(w);
   h.ignore = c.ignore, h.smoothing = (float)c.smoothing, h.dtype = dtype_code(x, "x");
@@ -366,14 +366,13 @@ struct HeadLossFunction : torch::autograd::Function<HeadLossFunction> {
   static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x_, const Tensor& w_, const OptTensor& bias_, const Tensor& target,
                         int64_t ignore, double smoothing, int64_t reduction) {
     c10::cuda::CUDAGuard guard(x_.device());
-    const Tensor x = matrix_fitted(x_), w = matrix_fitted(w_), bias = has(bias_) ? aligned(bias_->to(at::kFloat)) : Tensor();
+    const Tensor x = matrix_fitted(x_), w = matrix_fitted(w_), bias = has(bias_) ? aligned(*bias_) : Tensor();
     Tensor norm, inverse;
     const Tensor loss = head_loss_forward(x, w, bias, target, {ignore, smoothing, reduction}, norm, inverse);
     ctx->save_for_backward({x, w, bias, target, norm, inverse});
     ctx->saved_data["ignore"] = ignore;
     ctx->saved_data["smoothing"] = smoothing;
     ctx->saved_data["reduction"] = reduction;
-    ctx->saved_data["bias"] = (int64_t)(has(bias_) ? bias_->scalar_type() : at::kFloat);
     ctx->saved_data["f"] = (int64_t)x_.requires_grad() | (int64_t)w_.requires_grad() << 1 | (int64_t)(has(bias_) && bias_->requires_grad()) << 2;
     return loss;
   }
@@ -388,16 +387,15 @@ struct HeadLossFunction : torch::autograd::Function<HeadLossFunction> {
     Tensor dx, dw, db;
     if (f & 1) dx = at::empty({h.rows, h.c}, x.options());
     if (f & 2) dw = at::empty({h.classes, h.c}, w.options());
-    if (f & 4) db = at::empty({h.classes}, x.options().dtype(at::kFloat));
+    if (f & 4) db = at::empty({h.classes}, bias.options());
     const int64_t bytes = abi.px_head_loss_bwd_workspace_bytes(&h, f & 1, f >> 1 & 1, f >> 2 & 1);
     const Tensor ws = bytes_like(x, bytes);
     const cudaStream_t st = at::cuda::getCurrentCUDAStream();
     launch("px_head_loss_bwd", st, [&] {
       return abi.px_head_loss_bwd(&h, (const float*)norm.data_ptr(), (const float*)g.data_ptr(), reduction == 0, reduction ? (const float*)inverse.data_ptr() : nullptr,
-                                  dx.defined() ? dx.data_ptr() : nullptr, dw.defined() ? dw.data_ptr() : nullptr, db.defined() ? (float*)db.data_ptr() : nullptr,
+                                  dx.defined() ? dx.data_ptr() : nullptr, dw.defined() ? dw.data_ptr() : nullptr, db.defined() ? db.data_ptr() : nullptr,
                                   ws.data_ptr(), bytes, st);
     });
-    if (db.defined()) db = db.to((at::ScalarType)ctx->saved_data["bias"].toInt());
     return {dx, dw, db, Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
@@ -444,7 +442,7 @@ Tensor linear_cross_entropy(const Tensor& x, const Tensor& weight, const Tensor&
     loss = HeadLossFunction::apply(x2, weight, bias, t, ignore, smoothing, how);
   } else {
     Tensor norm, inverse;
-    loss = head_loss_forward(matrix_fitted(x2), matrix_fitted(weight), has(bias) ? aligned(bias->to(at::kFloat)) : Tensor(), t, {ignore, smoothing, how}, norm, inverse);
+    loss = head_loss_forward(matrix_fitted(x2), matrix_fitted(weight), has(bias) ? aligned(*bias) : Tensor(), t, {ignore, smoothing, how}, norm, inverse);
   }
   return how == 0 ? loss.reshape(target.sizes()) : loss;
 }

@@ -9,7 +9,7 @@ from protenix_b200 import _lib
 class Head(ctypes.Structure):
     _fields_ = [("x", ctypes.c_void_p), ("w", ctypes.c_void_p), ("bias", ctypes.c_void_p), ("target", ctypes.c_void_p), ("rows", ctypes.c_int64),
                 ("c", ctypes.c_int64), ("classes", ctypes.c_int64), ("x_stride", ctypes.c_int64), ("w_stride", ctypes.c_int64), ("ignore", ctypes.c_int64),
-                ("smoothing", ctypes.c_float), ("dtype", ctypes.c_int32)]
+                ("smoothing", ctypes.c_float), ("dtype", ctypes.c_int32), ("bias_dtype", ctypes.c_int32)]
 
 
 BUFFER = ctypes.create_string_buffer(4096)
@@ -17,7 +17,7 @@ AT = (ctypes.addressof(BUFFER) + 1023) // 1024 * 1024
 
 
 def _head(**changed):
-    h = dict(x=AT, w=AT, bias=None, target=AT, rows=10, c=64, classes=20, x_stride=64, w_stride=64, ignore=-100, smoothing=0.0, dtype=_lib.PX_BF16)
+    h = dict(x=AT, w=AT, bias=None, target=AT, rows=10, c=64, classes=20, x_stride=64, w_stride=64, ignore=-100, smoothing=0.0, dtype=_lib.PX_BF16, bias_dtype=_lib.PX_F32)
     h.update(changed)
     return Head(**h)
 
@@ -25,7 +25,7 @@ def _head(**changed):
 @pytest.mark.parametrize("changed,status", [
     (dict(rows=-1), -1), (dict(c=0), -1), (dict(classes=0), -1), (dict(x=None), -1), (dict(w=None), -1), (dict(target=None), -1), (dict(x_stride=56), -1),
     (dict(w_stride=68), -1), (dict(x=AT + 2), -1), (dict(w=AT + 8), -1), (dict(bias=AT + 4), -1), (dict(smoothing=1.5), -1), (dict(smoothing=float("nan")), -1),
-    (dict(dtype=_lib.PX_F32), -2), (dict(c=60), -2), (dict(classes=(1 << 24) + 1), -2), (dict(rows=(1 << 26) + 1), -2), (dict(rows=1 << 26, classes=1 << 24), -2)])
+    (dict(dtype=_lib.PX_F32), -2), (dict(bias_dtype=_lib.PX_F16), -2), (dict(c=60), -2), (dict(classes=(1 << 24) + 1), -2), (dict(rows=(1 << 26) + 1), -2), (dict(rows=1 << 26, classes=1 << 24), -2)])
 def test_heads(changed, status):
     lib, h = _lib.load(), _head(**changed)
     assert lib.px_head_loss_fwd(ctypes.byref(h), AT, AT, AT, AT, 1, AT, 1 << 40, None) == status
