@@ -63,10 +63,7 @@ struct EpiStats {
         sum += (a[0] + a[1]) + (a[2] + a[3]);
       }
       if (mine >= c && mine < c + 32) {
-        float h = 0.f;
-#pragma unroll
-        for (int j = 0; j < 32; ++j) h = mine - c == j ? v[j] : h;
-        hit[row] = h;
+        hit[row] = pick(v, mine - c);
       }
       float top[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
@@ -297,7 +294,7 @@ struct EpiLogitGrad {
       const float2 n = norm[row];
       ref = -n.x, over = factor / n.y;
     }
-    const float less = factor * smooth / (float)all_classes, hit = factor * (1.f - smooth);
+    const float less = factor * smooth / (float)all_classes, less_hit = -less - factor * (1.f - smooth);
 #pragma unroll 1
     for (int c = 0; c < kCols; c += 64) {
       if (base + c >= classes) break;
@@ -313,12 +310,13 @@ struct EpiLogitGrad {
 #pragma unroll
         for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
         add_bias(v, bias, base + c + h, left);
+        const int own = mine - (c + h);
+        if (__any_sync(0xffffffffu, own >= 0 && own < 32)) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = fmaf(over, fast_exp2(fmaf(v[j], kLog2e, ref)), -less);
-        if (mine >= c + h && mine < c + h + 32) {
+          for (int j = 0; j < 32; ++j) v[j] = fmaf(over, fast_exp2(fmaf(v[j], kLog2e, ref)), own == j ? less_hit : -less);
+        } else {
 #pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (mine - (c + h) == j) v[j] -= hit;
+          for (int j = 0; j < 32; ++j) v[j] = fmaf(over, fast_exp2(fmaf(v[j], kLog2e, ref)), -less);
         }
         if (!counts) {
 #pragma unroll

@@ -30,6 +30,14 @@ __device__ __forceinline__ float row_loss(float sum, float ref, float hit, bool 
   return loss < 0.f ? 0.f : loss * 0.6931471805599453f;
 }
 
+// v[at], 0 <= at < 32, by selection: written as a choice of elements the compiler makes it an indexed load and keeps v in local memory.
+__device__ __forceinline__ float pick(const float (&v)[32], int at) {
+  uint32_t u = 0;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) u |= __float_as_uint(v[j]) & (at == j ? 0xffffffffu : 0u);
+  return __uint_as_float(u);
+}
+
 // A bias in fp32 or 16 bits, 16-byte aligned.
 struct HeadBias {
   const void* at;      // or NULL

@@ -196,8 +196,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_head_kernel(const __gr
 #pragma unroll
             for (int j = 0; j < 32; ++j) all += c + j < a.classes ? v[j] : 0.f;
           }
-#pragma unroll
-          for (int j = 0; j < 32; ++j) hit = mine == c + j ? v[j] : hit;
+          if (mine >= c && mine < c + 32) hit = pick(v, mine - c);
           float top[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
           for (int j = 4; j < 32; ++j) top[j & 3] = fmaxf(top[j & 3], v[j]);
@@ -229,7 +228,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_head_kernel(const __gr
           const float2 n = a.norm[row];
           ref = -n.x, over = factor / n.y;
         }
-        const float less = factor * a.smooth / (float)a.classes, hit = factor * (1.f - a.smooth);
+        const float less = factor * a.smooth / (float)a.classes, less_hit = -less - factor * (1.f - a.smooth);
         ok = mbar_wait_warp(&bars.dl_empty[bl], ((i >> 1) & 1) ^ 1, 128u);
         if (!ok) break;
         unsigned char* const dl = sm + S::kDl + bl * S::kDlBytes;
@@ -246,16 +245,15 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_head_kernel(const __gr
           }
           float v[32];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = fmaf(over, fast_exp2(fmaf(__uint_as_float(r[j]) + bias[c + j], kLog2e, ref)), -less);
+          for (int j = 0; j < 32; ++j) v[j] = fmaf(over, fast_exp2(fmaf(__uint_as_float(r[j]) + bias[c + j], kLog2e, ref)), mine == c + j ? less_hit : -less);
           if (c + 32 > a.classes) {
 #pragma unroll
             for (int j = 0; j < 32; ++j)
               if (c + j >= a.classes) v[j] = 0.f;
           }
+          if (!counts) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            if (mine == c + j) v[j] -= hit;
-            if (!counts) v[j] = 0.f;
+            for (int j = 0; j < 32; ++j) v[j] = 0.f;
           }
 #pragma unroll
           for (int p = 0; p < 4; ++p) {
