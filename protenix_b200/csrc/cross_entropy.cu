@@ -18,7 +18,7 @@
 namespace px {
 
 constexpr int64_t kPieceBytes = 512ll << 20;
-constexpr int kScanBlocks = 592;
+constexpr int kScanBlocks = 592, kScanRows = 4;       // rows of a warp
 
 // ---- forward ---------------------------------------------------------------------------------------------------------
 struct EpiStats {
@@ -32,30 +32,33 @@ struct EpiStats {
   static constexpr bool kMeets = true;
   __device__ __forceinline__ void begin() const { *arrivals = 0; }
 
+  struct Row {
+    int mine;                 // the column that is the row's class, or -1
+    bool plain;               // all classes are there, without a bias
+  };
   template <class S>
-  __device__ __forceinline__ void tile(const GemmEpiTile& e, bool ok) const {
-    constexpr int kCols = S::kN / 2;                        // of this warp
-    const int row = e.m0 + e.lane, base = e.n0 + e.half * kCols;
+  __device__ __forceinline__ Row before(const GemmEpiTile& e) const {
+    const int row = e.m0 + e.lane;
+    const int64_t t = row < rows ? target[row] - e.n0 : -1;
+    return {t >= 0 && t < S::kPartCols ? (int)t : -1, warp_bias<S>(e, bias, classes)};
+  }
+  template <class S>
+  __device__ __forceinline__ void tile(const GemmEpiTile& e, const Row& at) const {
+    constexpr int kCols = S::kPartCols;
+    const int row = e.m0 + e.lane, base = e.n0, mine = at.mine;
     const bool there = row < rows;
-    const int64_t t = there ? target[row] - base : -1;
-    const int mine = t >= 0 && t < kCols ? (int)t : -1;     // the column that is the row's class
     float m = -CUDART_INF_F, s = 0.f, sum = 0.f;
 #pragma unroll 1
     for (int c = 0; c < kCols; c += 32) {
       const int left = classes - (base + c);
       if (left <= 0) break;
       uint32_t r[32];
-      tmem_ld32(e.acc + e.half * kCols + c, r);
+      tmem_ld32(e.acc + c, r);
       tmem_wait_ld();
       float v[32];
 #pragma unroll
       for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
-      add_bias(v, bias, base + c, left);
-      if (left < 32) {
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-          if (j >= left) v[j] = -CUDART_INF_F;
-      }
+      if (!at.plain) add_bias(v, e.own + c);
       if (part_sum) {
         float a[4] = {};
 #pragma unroll
@@ -76,20 +79,25 @@ struct EpiStats {
       s = (a[0] + a[1]) + (a[2] + a[3]);
       m = next;
     }
-    // the two halves of the columns
-    float* const x = reinterpret_cast<float*>(e.extra) + 32 * e.quarter + e.lane;
-    if (e.half) x[0] = m, x[128] = s, x[256] = sum;
-    gemm_epi_sync();
-    if (!e.half) {
-      const float m1 = x[0], next = fmaxf(m, m1), ref = reference(next);
-      s = s * fast_exp2(m - ref) + x[128] * fast_exp2(m1 - ref);
+    // the parts of the columns
+    float* const x = e.shared + 32 * e.quarter + e.lane;
+    if (e.part) x[384 * (e.part - 1)] = m, x[384 * (e.part - 1) + 128] = s, x[384 * (e.part - 1) + 256] = sum;
+    gemm_epi_sync<S>();
+    if (!e.part) {
+      float next = m;
+#pragma unroll
+      for (int p = 0; p < S::kParts - 1; ++p) next = fmaxf(next, x[384 * p]);
+      const float ref = reference(next);
+      s *= fast_exp2(m - ref);
+#pragma unroll
+      for (int p = 0; p < S::kParts - 1; ++p) s = fmaf(x[384 * p + 128], fast_exp2(x[384 * p] - ref), s), sum += x[384 * p + 256];
       if (there) {
         const int64_t at = (int64_t)e.at.nt * rows + row;
         part[at] = make_float2(next, s);
-        if (part_sum) part_sum[at] = sum + x[256];
+        if (part_sum) part_sum[at] = sum;
       }
     }
-    gemm_epi_sync();
+    gemm_epi_sync<S>();
   }
 };
 
@@ -119,13 +127,21 @@ __global__ void __launch_bounds__(32 * kJoinWarps) loss_join_kernel(const JoinAr
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, row = blockIdx.x * 32 + lane;
   float m = -CUDART_INF_F, s = 0.f, sum = 0.f;
   if (row < a.rows) {
-    for (int p = w; p < a.parts; p += kJoinWarps) {
-      const int64_t at = (int64_t)p * a.rows + row;
-      const float2 x = a.part[at];
-      const float next = fmaxf(m, x.x), ref = reference(next);
-      s = s * fast_exp2(m - ref) + x.y * fast_exp2(x.x - ref);
+    for (int p = w; p < a.parts; p += 4 * kJoinWarps) {      // four on their way at once
+      float2 x[4];
+      float t[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int64_t at = (int64_t)(p + j * kJoinWarps) * a.rows + row;
+        const bool there = p + j * kJoinWarps < a.parts;
+        x[j] = there ? a.part[at] : make_float2(-CUDART_INF_F, 0.f);
+        t[j] = there && a.part_sum ? a.part_sum[at] : 0.f;
+      }
+      const float next = fmaxf(m, fmaxf(fmaxf(x[0].x, x[1].x), fmaxf(x[2].x, x[3].x))), ref = reference(next);
+      s *= fast_exp2(m - ref);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s = fmaf(x[j].y, fast_exp2(x[j].x - ref), s), sum += t[j];
       m = next;
-      if (a.part_sum) sum += a.part_sum[at];
     }
   }
   xm[w][lane] = m, xs[w][lane] = s, xl[w][lane] = sum;
@@ -198,15 +214,16 @@ __global__ void __launch_bounds__(256) loss_scan_kernel(const ScanArgs a, bool f
   pdl_wait();
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   uint32_t dirty = 0, top = 0;
-  for (int64_t r0 = ((int64_t)blockIdx.x * 8 + w) * 32; r0 < a.rows; r0 += (int64_t)gridDim.x * 256) {
+  for (int64_t r0 = ((int64_t)blockIdx.x * 8 + w) * kScanRows; r0 < a.rows; r0 += (int64_t)gridDim.x * 8 * kScanRows) {
     const int64_t row = r0 + lane;
-    const bool ignored = row < a.rows && !row_counts(a.target[row], a.ignore);
-    if (a.each && row < a.rows && !ignored) {
+    const bool there = lane < kScanRows && row < a.rows, ignored = there && !row_counts(a.target[row], a.ignore);
+    if (a.each && there && !ignored) {
       const float g = fabsf(a.grad[row]);
       if (g < CUDART_INF_F) top = max(top, __float_as_uint(g));
     }
     for (uint32_t left = __ballot_sync(0xffffffffu, ignored); left; left &= left - 1) {
       const uint4* p = reinterpret_cast<const uint4*>((const uint16_t*)a.x + (r0 + __ffs(left) - 1) * a.x_stride);
+#pragma unroll 4
       for (int i = lane; i < a.c / 8; i += 32) {
         const uint4 v = __ldg(p + i);
         if (!(finite16x2(v.x, f16) && finite16x2(v.y, f16) && finite16x2(v.z, f16) && finite16x2(v.w, f16))) dirty = 1;
@@ -276,25 +293,39 @@ struct EpiLogitGrad {
   static constexpr bool kMeets = false;
   __device__ __forceinline__ void begin() const {}
 
-  template <class S>
-  __device__ __forceinline__ void tile(const GemmEpiTile& e, bool) const {
-    constexpr int kCols = S::kN == 64 ? 64 : S::kN / 2;     // blocks of 64: of a narrow tile, half of the warps have none
-    const int row = e.m0 + e.lane, base = e.n0 + e.half * kCols;
-    if (e.m0 >= rows || (S::kN == 64 && e.half)) return;
-    const int64_t t = row < rows ? target[row] : ignore;
-    const bool counts = row < rows && row_counts(t, ignore);
-    const int64_t in_piece = t - first - base;
-    const int mine = counts && t >= 0 && t < all_classes && in_piece >= 0 && in_piece < kCols ? (int)in_piece : -1;
+  struct Row {
     // dl = factor (p - smooth / V) - (mine) factor (1 - smooth), p = exp2(l log2(e) + ref) / sum
-    float factor = 0.f, ref = 0.f, over = 0.f;
-    if (counts) {
-      factor = grad ? grad[row] * scale->each : 1.f;
-      if (t < 0 || t >= all_classes) factor = CUDART_NAN_F;
+    float over, ref, less, less_hit;
+    int mine;
+    bool counts, plain;
+  };
+  template <class S>
+  __device__ __forceinline__ Row before(const GemmEpiTile& e) const {
+    Row at = {};
+    const int row = e.m0 + e.lane;
+    const int64_t t = row < rows ? target[row] : ignore;
+    at.counts = row < rows && row_counts(t, ignore);
+    const int64_t in_part = t - first - e.n0;
+    const bool valid = t >= 0 && t < all_classes;
+    at.mine = at.counts && valid && in_part >= 0 && in_part < S::kPartCols ? (int)in_part : -1;
+    if (at.counts) {
+      float factor = grad ? grad[row] * scale->each : 1.f;
+      if (!valid) factor = CUDART_NAN_F;
       if (f16) factor *= kDlScaleF16;
       const float2 n = norm[row];
-      ref = -n.x, over = factor / n.y;
+      at.ref = -n.x, at.over = factor / n.y;
+      at.less = factor * smooth / (float)all_classes, at.less_hit = -at.less - factor * (1.f - smooth);
     }
-    const float less = factor * smooth / (float)all_classes, less_hit = -less - factor * (1.f - smooth);
+    at.plain = warp_bias<S>(e, bias, classes);
+    return at;
+  }
+  template <class S>
+  __device__ __forceinline__ void tile(const GemmEpiTile& e, const Row& at) const {
+    constexpr int kCols = S::kPartCols;
+    if (e.m0 >= rows) return;
+    const int base = e.n0, mine = at.mine;
+    const float over = at.over, ref = at.ref, less = at.less, less_hit = at.less_hit;
+    const bool counts = at.counts;
 #pragma unroll 1
     for (int c = 0; c < kCols; c += 64) {
       if (base + c >= classes) break;
@@ -304,12 +335,12 @@ struct EpiLogitGrad {
       for (int h = 0; h < 64; h += 32) {
         const int left = classes - (base + c + h);
         uint32_t r[32];
-        tmem_ld32(e.acc + e.half * kCols + c + h, r);
+        tmem_ld32(e.acc + c + h, r);
         tmem_wait_ld();
         float v[32];
 #pragma unroll
         for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
-        add_bias(v, bias, base + c + h, left);
+        if (!at.plain) add_bias(v, e.own + c + h);
         const int own = mine - (c + h);
         if (__any_sync(0xffffffffu, own >= 0 && own < 32)) {
 #pragma unroll
@@ -379,13 +410,22 @@ struct EpiGrad {
   static constexpr bool kMeets = false;
   __device__ __forceinline__ void begin() const {}
 
+  struct Row {
+    float by;
+    bool zero;
+  };
   template <class S>
-  __device__ __forceinline__ void tile(const GemmEpiTile& e, bool) const {
-    constexpr int kCols = S::kN / 2, kBlock = kF32 ? 32 : 64;
+  __device__ __forceinline__ Row before(const GemmEpiTile& e) const {
+    const int row = e.m0 + e.lane;
+    return {kF32 ? 1.f : scale->out, !kF32 && target && row < rows && !row_counts(target[row], ignore)};
+  }
+  template <class S>
+  __device__ __forceinline__ void tile(const GemmEpiTile& e, const Row& at) const {
+    constexpr int kCols = S::kPartCols, kBlock = kF32 ? 32 : 64;
     if (e.m0 >= rows) return;
-    const int base = e.n0 + e.half * kCols, row = e.m0 + e.lane;
-    const float by = kF32 ? 1.f : scale->out;
-    const bool zero = !kF32 && target && row < rows && !row_counts(target[row], ignore);
+    const int base = e.n0;
+    const float by = at.by;
+    const bool zero = at.zero;
 #pragma unroll 1
     for (int c = 0; c < kCols; c += kBlock) {
       if (base + c >= cols) break;
@@ -394,7 +434,7 @@ struct EpiGrad {
 #pragma unroll
       for (int h = 0; h < kBlock; h += 32) {
         uint32_t r[32];
-        tmem_ld32(e.acc + e.half * kCols + c + h, r);
+        tmem_ld32(e.acc + c + h, r);
         tmem_wait_ld();
         if constexpr (kF32) {
 #pragma unroll
@@ -454,9 +494,9 @@ PX_DEFINE_FAMILY_HOOKS(loss)
 static int64_t up(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
 
 // Shapes of the products: logits (both operands along k), dx (W across), dW (both across).
-typedef GemmShape<1, 64, false, false, 6> Logits64;
-typedef GemmShape<1, 256, false, false, 4> Logits256;
-typedef GemmShape<2, 256, false, false, 5> LogitsPair;
+typedef GemmShape<1, 64, false, false, 6, 4, true> Logits64;
+typedef GemmShape<1, 256, false, false, 3, 16, true> Logits256;
+typedef GemmShape<2, 256, false, false, 4, 16, true> LogitsPair;
 typedef GemmShape<1, 128, false, true, 5> Dx128;
 typedef GemmShape<1, 256, false, true, 4> Dx256;
 typedef GemmShape<2, 256, false, true, 5> DxPair;
@@ -589,7 +629,7 @@ template <bool kBackward, int kVp>
 static bool launch_small(const SmallArgs& a, cudaStream_t st) {
   typedef SmallShape<kBackward, kVp> S;
   static SmemLimit limit;
-  return limit.set(small_head_kernel<kBackward, kVp>, S::kSmem) && launch_pdl(small_head_kernel<kBackward, kVp>, dim3(small_ctas(a.rows)), kSmallThreads, S::kSmem, st, a);
+  return limit.set(small_head_kernel<kBackward, kVp>, S::kSmem) && launch_pdl(small_head_kernel<kBackward, kVp>, dim3(small_ctas(a.rows)), S::kThreads, S::kSmem, st, a);
 }
 template <bool kBackward>
 static bool launch_small(const SmallArgs& a, cudaStream_t st) {
@@ -601,7 +641,7 @@ struct SmallPlan {
 static SmallPlan small_plan(const px_head& h) {
   const int64_t ctas = small_ctas(h.rows), vp = small_vp(h.classes);
   SmallPlan p;
-  p.scale = 0, p.found = 1024, p.w = p.found + up(kScanBlocks * 8, 1024), p.b = p.w + ctas * 128 * vp * 4, p.bytes = p.b + ctas * 4 * vp * 4;
+  p.scale = 0, p.found = 1024, p.w = p.found + up(kScanBlocks * 8, 1024), p.b = p.w + ctas * 128 * vp * 4, p.bytes = p.b + ctas * 8 * vp * 4;
   return p;
 }
 
@@ -666,7 +706,7 @@ extern "C" int32_t px_head_loss_bwd(const px_head* head, const float* norm, cons
   const bool f16 = h.dtype == PX_F16;
   const float dl_scale = f16 ? kDlScaleF16 : 1.f;
   const int64_t bias_size = h.bias_dtype == PX_F32 ? 4 : 2;
-  const int scan_blocks = (int)std::min<int64_t>((h.rows + 255) / 256, kScanBlocks);
+  const int scan_blocks = (int)std::min<int64_t>((h.rows + 8 * kScanRows - 1) / (8 * kScanRows), kScanBlocks);
   char* const ws = (char*)workspace;
   if (small_head(h.c, h.classes)) {
     const SmallPlan p = small_plan(h);
@@ -684,7 +724,7 @@ extern "C" int32_t px_head_loss_bwd(const px_head* head, const float* norm, cons
     if (!launch_small<true>(a, st)) return PX_ERR_LAUNCH;
     if (!dw && !dbias) return PX_OK;
     const int vp = (int)small_vp(h.classes), groups = vp / 32;
-    return launch_pdl(small_join_kernel, dim3((unsigned)(groups * (h.c / 8 + 1))), 256, 0, st, (const float*)a.part_w, (const float*)a.part_b, (uint16_t*)dw, dbias,
+    return launch_pdl(small_join_kernel, dim3((unsigned)(groups * (h.c + 1))), 256, 0, st, (const float*)a.part_w, (const float*)a.part_b, (uint16_t*)dw, dbias,
                       small_ctas(h.rows), vp, (int)h.c, (int)h.classes, (int)f16, (int)h.bias_dtype)
                ? PX_OK
                : PX_ERR_LAUNCH;

@@ -16,6 +16,7 @@
 namespace px {
 
 constexpr float kPlaneScale = 1024.f;
+constexpr int kOrthoEpiWarps = 8, kOrthoThreads = 64 + 32 * kOrthoEpiWarps;
 
 // ---- norm and first iterate ------------------------------------------------------------------------------------------
 constexpr int kNormBlocks = 64;
@@ -106,7 +107,7 @@ struct PlaneShape {
   static constexpr int kCtas = kCtas_, kUnits = kCtas, kSide = 128 * kCtas, kStages = 3;
   static constexpr bool kAMn = kAMn_, kBMn = kBMn_;
   static constexpr int kPlaneBytes = kGemmM * kGemmK * 2, kStageBytes = 4 * kPlaneBytes;      // A hi, A lo, B hi, B lo: 128 rows each
-  static constexpr int kStg = kStages * kStageBytes, kBars = kStg + kGemmEpiWarps * kGemmStgBytes;
+  static constexpr int kStg = kStages * kStageBytes, kBars = kStg + kOrthoEpiWarps * kGemmStgBytes;
   static constexpr size_t kSmem = kBars + 256 + 1024;
   static constexpr uint32_t kIdesc = umma_idesc_f16(kGemmM * kCtas, 128, kAMn, kBMn);
   static_assert(kSmem <= 232448, "shared memory budget");
@@ -212,7 +213,7 @@ struct OrthoEnd {
 };
 
 template <class S>
-__global__ void __launch_bounds__(kGemmThreads, 1)
+__global__ void __launch_bounds__(kOrthoThreads, 1)
 plane_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ OrthoEnd end, const GemmTiles tiles, int chunk) {
   constexpr bool kPair = S::kCtas == 2;
   constexpr int kStages = S::kStages, kUnits = S::kUnits;
@@ -233,10 +234,10 @@ plane_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&bars.part_full[b], 1);
-      mbar_init(&bars.part_empty[b], kGemmEpiWarps * S::kCtas);
+      mbar_init(&bars.part_empty[b], kOrthoEpiWarps * S::kCtas);
     }
     mbar_init(&bars.rest_full, 1);
-    mbar_init(&bars.rest_empty, kGemmEpiWarps * S::kCtas);
+    mbar_init(&bars.rest_empty, kOrthoEpiWarps * S::kCtas);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
   if (warp == 0) {
@@ -477,7 +478,7 @@ static int32_t launch_planes(const CUtensorMap& ma, const CUtensorMap& mb, const
   at[1].val.clusterDim.x = S::kCtas, at[1].val.clusterDim.y = 1, at[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(even_grid(total, sm_count() / S::kCtas) * S::kCtas));
-  cfg.blockDim = dim3(kGemmThreads);
+  cfg.blockDim = dim3(kOrthoThreads);
   cfg.dynamicSmemBytes = S::kSmem;
   cfg.stream = st;
   cfg.attrs = at;

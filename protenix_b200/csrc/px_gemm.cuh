@@ -6,7 +6,7 @@
 // One CTA works on 128 x kN, or a pair of them (cta_group::2) on 256 x kN, each with its own 128 rows of A and half of B: the pair asks L2 for
 // 64 bytes a cycle where a CTA alone with kN = 256 asks for 96.
 //
-// Roles: warp 0 copies, warp 1 issues products, eight warps are the epilogue (a quarter of the lanes and half of the columns each).
+// Roles: warp 0 copies, warp 1 issues products, kEpiWarps (4, 8 or 16) are the epilogue (a quarter of the lanes and 1, 1/2 or 1/4 of the columns each).
 // Accumulators are double-buffered.
 #pragma once
 #include "px_pair.cuh"
@@ -15,22 +15,22 @@
 namespace px {
 
 constexpr int kGemmM = 128, kGemmK = 64;          // rows of a CTA's tile, k of a stage
-constexpr int kGemmEpiWarps = 8, kGemmThreads = 64 + 32 * kGemmEpiWarps;
 constexpr int kGemmStgBytes = 4096;               // staged block of a warp: 32 rows of 128 bytes
 
-template <int kCtas_, int kN_, bool kAMn_, bool kBMn_, int kStages_>
+template <int kCtas_, int kN_, bool kAMn_, bool kBMn_, int kStages_, int kEpiWarps_ = 8, bool kEpiMemory = false>
 struct GemmShape {
-  static constexpr int kCtas = kCtas_, kN = kN_, kStages = kStages_;
+  static constexpr int kCtas = kCtas_, kN = kN_, kStages = kStages_, kEpiWarps = kEpiWarps_, kThreads = 64 + 32 * kEpiWarps;
+  static constexpr int kParts = kEpiWarps / 4, kPartCols = kN / kParts;      // columns of an epilogue warp
   static constexpr bool kAMn = kAMn_, kBMn = kBMn_;
   static constexpr int kBRows = kN / kCtas;       // rows of B that a CTA loads
   static constexpr int kABytes = kGemmM * kGemmK * 2, kBBytes = kBRows * kGemmK * 2;
   static constexpr int kStageBytes = kABytes + kBBytes;
   static constexpr uint32_t kCols = 2 * kN;
-  static constexpr int kStg = kStages * kStageBytes, kExtra = kStg + kGemmEpiWarps * kGemmStgBytes, kExtraBytes = 1536;
+  static constexpr int kStg = kStages * kStageBytes, kExtra = kStg + kEpiWarps * kGemmStgBytes, kExtraBytes = kEpiMemory ? 1536 * (kParts - 1) + 4 * kEpiWarps * kPartCols : 0;
   static constexpr int kBars = kExtra + kExtraBytes;
   static constexpr size_t kSmem = kBars + 256 + 1024;
   static_assert(kSmem <= 232448, "shared memory budget");
-  static_assert(kBRows % 64 == 0 && kN <= 256, "tile");
+  static_assert(kBRows % 64 == 0 && kN <= 256 && kPartCols >= 64, "tile");
   static constexpr uint32_t idesc(bool f16) { return umma_idesc_16(kGemmM * kCtas, kN, f16, f16, kAMn, kBMn); }
 };
 
@@ -79,16 +79,18 @@ struct GemmBarriers {
 // What an epilogue gets for a tile: its place, the accumulator's address with this warp's lanes in it, and what it may use in shared memory.
 struct GemmEpiTile {
   GemmTile at;
-  int m0, n0;                        // first row of this warp's 32, first column of the tile
-  uint32_t acc;                      // tensor memory, lanes of this warp, first column
-  int quarter, half, lane;
+  int m0, n0;                        // first of this warp's 32 rows, first of its columns
+  uint32_t acc;                      // tensor memory, lanes and first column of this warp
+  int quarter, part, lane;
   unsigned char* stg;                // kGemmStgBytes of this warp's own
-  unsigned char* extra;              // kExtraBytes shared by the epilogue's warps
+  float* own;                        // kEpiMemory: a number for each column of this warp, its own
+  float* shared;                     // 384 numbers for each part but the first, shared by the epilogue's warps
 };
-__device__ __forceinline__ void gemm_epi_sync() { asm volatile("bar.sync 1, %0;\n" ::"n"(32 * kGemmEpiWarps) : "memory"); }
+template <class S>
+__device__ __forceinline__ void gemm_epi_sync() { asm volatile("bar.sync 1, %0;\n" ::"n"(32 * S::kEpiWarps) : "memory"); }
 
 template <class S, class Epi>
-__global__ void __launch_bounds__(kGemmThreads, 1)
+__global__ void __launch_bounds__(S::kThreads, 1)
 gemm_kernel(const __grid_constant__ GemmOperands ops, const __grid_constant__ Epi epi, const GemmTiles tiles) {
   constexpr bool kPair = S::kCtas == 2;
   constexpr int kStages = S::kStages;
@@ -108,7 +110,7 @@ gemm_kernel(const __grid_constant__ GemmOperands ops, const __grid_constant__ Ep
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&bars.acc_full[b], 1);
-      mbar_init(&bars.acc_empty[b], kGemmEpiWarps * S::kCtas);
+      mbar_init(&bars.acc_empty[b], S::kEpiWarps * S::kCtas);
     }
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
@@ -227,23 +229,25 @@ gemm_kernel(const __grid_constant__ GemmOperands ops, const __grid_constant__ Ep
       }
     }
   } else {
-    const int q = warp & 3, half = (warp - 2) >> 2;        // the quarter of the lanes that this warp may access goes by its index
+    const int q = warp & 3;                                // the quarter of the lanes that this warp may access goes by its index
     uint32_t count = 0;
     bool ok = true;
+    GemmEpiTile e;
+    e.quarter = q, e.part = (warp - 2) >> 2, e.lane = lane;
+    e.stg = ring + S::kStg + (warp - 2) * kGemmStgBytes;
+    e.own = reinterpret_cast<float*>(ring + S::kExtra) + (warp - 2) * S::kPartCols;
+    e.shared = reinterpret_cast<float*>(ring + S::kExtra) + S::kEpiWarps * S::kPartCols;
     for (int tile = first_tile; tile < tiles.total; tile += tile_step, ++count) {
-      GemmEpiTile e;
       e.at = gemm_tile(tiles, tile);
       const uint32_t ab = count & 1, aph = (count >> 1) & 1;
+      e.m0 = (e.at.mt * S::kCtas + (int)rank) * kGemmM + 32 * q;
+      e.n0 = e.at.nt * S::kN + e.part * S::kPartCols;
+      e.acc = tmem_base + ((uint32_t)(32 * q) << 16) + ab * S::kN + e.part * S::kPartCols;
+      const typename Epi::Row row = epi.template before<S>(e);      // what it fetches is on its way while the product is
       ok = ok && mbar_wait_warp(&bars.acc_full[ab], aph, 8u);
       if (!Epi::kMeets && !ok) break;                      // an epilogue whose warps meet goes through all tiles
       tc_fence_after();
-      e.m0 = (e.at.mt * S::kCtas + (int)rank) * kGemmM + 32 * q;
-      e.n0 = e.at.nt * S::kN;
-      e.acc = tmem_base + ((uint32_t)(32 * q) << 16) + ab * S::kN;
-      e.quarter = q, e.half = half, e.lane = lane;
-      e.stg = ring + S::kStg + (warp - 2) * kGemmStgBytes;
-      e.extra = ring + S::kExtra;
-      epi.template tile<S>(e, ok);
+      epi.template tile<S>(e, row);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
@@ -293,7 +297,7 @@ static int32_t gemm_launch(const GemmOperands& ops, const Epi& epi, GemmTiles t,
   at[1].val.clusterDim.x = S::kCtas, at[1].val.clusterDim.y = 1, at[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(even_grid(total, sm_count() / S::kCtas) * S::kCtas));
-  cfg.blockDim = dim3(kGemmThreads);
+  cfg.blockDim = dim3(S::kThreads);
   cfg.dynamicSmemBytes = S::kSmem;
   cfg.stream = st;
   cfg.attrs = at;

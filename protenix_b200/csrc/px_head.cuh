@@ -46,32 +46,25 @@ struct HeadBias {
 __device__ __forceinline__ float bias_value(const HeadBias& b, int i) {
   return b.type == PX_F32 ? __ldg((const float*)b.at + i) : b.type == PX_F16 ? __half2float(__ldg((const __half*)b.at + i)) : __bfloat162float(__ldg((const bf16*)b.at + i));
 }
-// v += the bias of 32 classes from `first` (a multiple of 32) on, of which `left` are there.
-__device__ __forceinline__ void add_bias(float (&v)[32], const HeadBias& b, int first, int left) {
-  if (!b.at) return;
-  if (left < 32) {
-    // the classes of the last tile one by one: lane j has the j-th
-    const int lane = threadIdx.x & 31;
-    const float mine = lane < left ? bias_value(b, first + lane) : 0.f;
+// Leaves the bias of an epilogue warp's classes in its shared memory, minus infinity for classes that are not there (no exponential); true where
+// there is nothing to add.
+template <class S>
+__device__ __forceinline__ bool warp_bias(const GemmEpiTile& e, const HeadBias& b, int classes) {
+  if (!b.at && e.n0 + S::kPartCols <= classes) return true;
+  __syncwarp();
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] += __shfl_sync(0xffffffffu, mine, j);
-  } else if (b.type == PX_F32) {
+  for (int j = 0; j < S::kPartCols; j += 32) {
+    const int v = e.n0 + j + e.lane;
+    e.own[j + e.lane] = v >= classes ? -CUDART_INF_F : b.at ? bias_value(b, v) : 0.f;
+  }
+  __syncwarp();
+  return false;
+}
+__device__ __forceinline__ void add_bias(float (&v)[32], const float* b) {
 #pragma unroll
-    for (int j = 0; j < 32; j += 4) {
-      const float4 x = __ldg(reinterpret_cast<const float4*>((const float*)b.at + first + j));
-      v[j] += x.x, v[j + 1] += x.y, v[j + 2] += x.z, v[j + 3] += x.w;
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 32; j += 8) {
-      const uint4 u = __ldg(reinterpret_cast<const uint4*>((const uint16_t*)b.at + first + j));
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float2 x = b.type == PX_F16 ? unpack_f16x2(w[k]) : unpack_bf16x2(w[k]);
-        v[j + 2 * k] += x.x, v[j + 2 * k + 1] += x.y;
-      }
-    }
+  for (int j = 0; j < 32; j += 4) {
+    const float4 x = *reinterpret_cast<const float4*>(b + j);
+    v[j] += x.x, v[j + 1] += x.y, v[j + 2] += x.z, v[j + 3] += x.w;
   }
 }
 __device__ __forceinline__ void bias_store(void* to, int type, int i, float v) {

@@ -8,14 +8,14 @@
 //
 // Rows that are ignored: dl zero by selection, and their x is zeroed in shared memory before the product for dW reads it.
 //
-// Roles: warp 0 copies rows in, warp 1 issues products, warps 2 to 5 are rows of the softmax; warps 6 to 9 are forward a second set of those (the sets
-// take the tiles in turn), backward they round dx and store it.  The logits of tile i + 1 are issued before the gradients of tile i.
+// Roles: warp 0 copies rows in, warp 1 issues products, sets of four warps are the rows of the softmax and take the tiles in turn (four sets
+// forward, two backward); backward four more warps round dx and store it.  The logits of tile i + 1 are issued before the gradients of tile i.
 #pragma once
 #include "px_head.cuh"
 
 namespace px {
 
-constexpr int kSmallC = 128, kSmallV = 128, kSmallThreads = 320;
+constexpr int kSmallC = 128, kSmallV = 128;
 constexpr int kSmallPanel = 128 * 128;                    // [128 rows][64 channels or classes] in 16 bits
 
 struct SmallArgs {
@@ -29,7 +29,7 @@ struct SmallArgs {
   const float* inverse;
   const LossScale* scale;                                 // backward, with a gradient for each row; otherwise NULL
   float* part_w;                                          // backward: [CTAs][128][kVp], or NULL
-  float* part_b;                                          // backward: [4 CTAs][kVp], or NULL
+  float* part_b;                                          // backward: [8 CTAs][kVp], or NULL
   int64_t ignore;
   int rows, classes, panels, tiles, f16, want_dx;
   float smooth;
@@ -38,26 +38,27 @@ struct SmallArgs {
 
 template <bool kBackward, int kVp>
 struct SmallShape {
-  static constexpr int kStages = kBackward ? 3 : 5;
+  static constexpr int kStages = kBackward ? 3 : 5, kSets = kBackward ? 2 : 4;
+  static constexpr int kThreads = 64 + 128 * kSets + (kBackward ? 128 : 0);
   static constexpr int kXBytes = 2 * kSmallPanel, kWBytes = 2 * kVp * 128, kDlBytes = kVp / 64 * kSmallPanel;
   static constexpr int kW = kStages * kXBytes, kDl = kW + kWBytes, kStg = kDl + (kBackward ? 2 * kDlBytes : 0);
   static constexpr int kBias = kStg + (kBackward ? 4 * 2 * 4096 : 0), kBars = kBias + kVp * 4;
   static constexpr size_t kSmem = kBars + 256 + 1024;
   static_assert(kSmem <= 232448, "shared memory budget");
-  // tensor memory: logits (two of 64 classes, or of 128 forward), dx twice, dW^T
-  static constexpr int kLogits = kBackward && kVp == 128 ? 1 : 2;
-  static constexpr uint32_t kDx = kLogits * kVp, kDw = kDx + 256, kCols = kBackward ? 512 : 256;
+  // tensor memory: logits (one for each set, which then sees every phase of its barrier), dx (twice, where there is room), dW^T
+  static constexpr int kDxs = kVp == 128 ? 1 : 2;
+  static constexpr uint32_t kDx = kSets * kVp, kDw = kDx + 128 * kDxs, kCols = kBackward ? 512 : kSets * kVp;
   static_assert(!kBackward || kDw + kVp <= 512, "tensor memory");
 };
 struct SmallBarriers {
-  uint64_t w_full, x_full[5], x_empty[5], logit_full[2], logit_empty[2], dl_full[2], dl_empty[2], dx_full[2], dx_empty[2], done;
+  uint64_t w_full, x_full[5], x_empty[5], logit_full[4], logit_empty[4], dl_full[2], dl_empty[2], dx_full[2], dx_empty[2], done;
   uint32_t tmem_base;
 };
 
 template <bool kBackward, int kVp>
-__global__ void __launch_bounds__(kSmallThreads, 1) small_head_kernel(const __grid_constant__ SmallArgs a) {
+__global__ void __launch_bounds__(SmallShape<kBackward, kVp>::kThreads, 1) small_head_kernel(const __grid_constant__ SmallArgs a) {
   typedef SmallShape<kBackward, kVp> S;
-  constexpr int kLogits = S::kLogits;
+  constexpr int kLogits = S::kSets, kDxs = S::kDxs;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* sm = smem_aligned(smem_raw);
   SmallBarriers& bars = *reinterpret_cast<SmallBarriers*>(sm + S::kBars);
@@ -72,9 +73,11 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_head_kernel(const __gr
       mbar_init(&bars.x_full[s], 1);
       mbar_init(&bars.x_empty[s], 1);
     }
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < kLogits; ++b) {
       mbar_init(&bars.logit_full[b], 1);
       mbar_init(&bars.logit_empty[b], 4);
+    }
+    for (int b = 0; b < 2; ++b) {
       mbar_init(&bars.dl_full[b], 4);
       mbar_init(&bars.dl_empty[b], 1);
       mbar_init(&bars.dx_full[b], 1);
@@ -134,8 +137,8 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_head_kernel(const __gr
     for (int i = 0; i < mine && ok; ++i) {
       if (i + 1 < mine) logits(i + 1);
       if constexpr (kBackward) {
-        const int s = i % S::kStages, b = i & 1;
-        ok = ok && mbar_wait_warp(&bars.dl_full[b], (i >> 1) & 1, 16u) && mbar_wait_warp(&bars.dx_empty[b], ((i >> 1) & 1) ^ 1, 32u);
+        const int s = i % S::kStages, b = i & 1, d = i % kDxs;
+        ok = ok && mbar_wait_warp(&bars.dl_full[b], (i >> 1) & 1, 16u) && mbar_wait_warp(&bars.dx_empty[d], ((i / kDxs) & 1) ^ 1, 32u);
         if (!ok) break;
         tc_fence_after();
         if (elect_lane()) {
@@ -143,8 +146,8 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_head_kernel(const __gr
           const uint64_t al = umma_desc_sw128(dl), wl = umma_desc_mn_sw128(smem_u32(sm + S::kW), kVp * 128, 1024);
 #pragma unroll
           for (int ks = 0; ks < kVp / 16; ++ks)
-            umma_bf16(tmem + S::kDx + 128 * b, al + (ks >> 2) * (kSmallPanel >> 4) + 2 * (ks & 3), wl + 128 * ks, a.idesc_dx, ks > 0);
-          umma_commit(&bars.dx_full[b]);
+            umma_bf16(tmem + S::kDx + 128 * d, al + (ks >> 2) * (kSmallPanel >> 4) + 2 * (ks & 3), wl + 128 * ks, a.idesc_dx, ks > 0);
+          umma_commit(&bars.dx_full[d]);
           const uint64_t xt = umma_desc_mn_sw128(smem_u32(sm + s * S::kXBytes), kSmallPanel, 1024), bl = umma_desc_mn_sw128(dl, kSmallPanel, 1024);
 #pragma unroll
           for (int ks = 0; ks < 8; ++ks) umma_bf16(tmem + S::kDw, xt + 128 * ks, bl + 128 * ks, a.idesc_dw, (i | ks) ? 1u : 0u);
@@ -155,9 +158,10 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_head_kernel(const __gr
         __syncwarp();
       }
     }
-  } else if (!kBackward || warp < 6) {
+  } else if (warp < 2 + 4 * S::kSets) {
     // rows of the softmax
-    const int q = warp & 3, set = kBackward ? 0 : (warp - 2) >> 2, sets = kBackward ? 1 : 2;
+    const int q = warp & 3, set = (warp - 2) >> 2;
+    constexpr int sets = S::kSets;
     const uint32_t lanes = tmem + ((uint32_t)(32 * q) << 16);
     double total = 0.0;
     int counted = 0;
@@ -169,9 +173,21 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_head_kernel(const __gr
     }
     int i = set;
     bool ok = true;
+    int64_t next_t = a.ignore;
+    float2 next_n = {};
+    auto fetch = [&](int tile) {                            // a tile ahead
+      const int row = 128 * tile + 32 * q + lane;
+      if (tile < a.tiles && row < a.rows) {
+        next_t = a.target[row];
+        if (kBackward) next_n = a.norm[row];
+      }
+    };
+    fetch(blockIdx.x + set * gridDim.x);
     for (int tile = blockIdx.x + set * gridDim.x; tile < a.tiles && ok; tile += sets * gridDim.x, i += sets) {
       const int b = i % kLogits, s = i % S::kStages, row = 128 * tile + 32 * q + lane;
-      const int64_t t = row < a.rows ? a.target[row] : a.ignore;
+      const int64_t t = next_t;
+      const float2 n = next_n;
+      fetch(tile + sets * gridDim.x);
       const bool counts = row < a.rows && row_counts(t, a.ignore), valid = t >= 0 && t < a.classes;
       const int mine = counts && valid ? (int)t : -1;
       ok = mbar_wait_warp(&bars.logit_full[b], (i / kLogits) & 1, 64u);
@@ -191,7 +207,8 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_head_kernel(const __gr
           }
           float v[32];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]) + bias[c + j];
+          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+          add_bias(v, bias + c);
           if (a.smooth > 0.f) {
 #pragma unroll
             for (int j = 0; j < 32; ++j) all += c + j < a.classes ? v[j] : 0.f;
@@ -225,7 +242,6 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_head_kernel(const __gr
           factor = a.scale ? a.grad[row] * each : 1.f;
           if (!valid) factor = CUDART_NAN_F;
           if (a.f16) factor *= kDlScaleF16;
-          const float2 n = a.norm[row];
           ref = -n.x, over = factor / n.y;
         }
         const float less = factor * a.smooth / (float)a.classes, less_hit = -less - factor * (1.f - a.smooth);
@@ -245,7 +261,10 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_head_kernel(const __gr
           }
           float v[32];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = fmaf(over, fast_exp2(fmaf(__uint_as_float(r[j]) + bias[c + j], kLog2e, ref)), mine == c + j ? less_hit : -less);
+          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+          add_bias(v, bias + c);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = fmaf(over, fast_exp2(fmaf(v[j], kLog2e, ref)), mine == c + j ? less_hit : -less);
           if (c + 32 > a.classes) {
 #pragma unroll
             for (int j = 0; j < 32; ++j)
@@ -283,20 +302,20 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_head_kernel(const __gr
         double n = counted;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o), n += __shfl_xor_sync(0xffffffffu, n, o);
-        asm volatile("bar.sync 1, 256;\n" ::: "memory");
+        asm volatile("bar.sync 1, 512;\n" ::: "memory");
         if (lane == 0) x[warp - 2] = make_double2(total, n);
-        asm volatile("bar.sync 1, 256;\n" ::: "memory");
+        asm volatile("bar.sync 1, 512;\n" ::: "memory");
         if (warp == 2 && lane == 0) {
-          for (int w = 1; w < 8; ++w) total += x[w].x, n += x[w].y;
+          for (int w = 1; w < 16; ++w) total += x[w].x, n += x[w].y;
           a.sums[blockIdx.x] = make_double2(total, n);
         }
       }
     } else {
       if (a.part_b) {
 #pragma unroll
-        for (int c = 0; c < kVp / 32; ++c) a.part_b[((int64_t)blockIdx.x * 4 + q) * kVp + 32 * c + lane] = db[c] * out;
+        for (int c = 0; c < kVp / 32; ++c) a.part_b[((int64_t)blockIdx.x * 8 + (warp - 2)) * kVp + 32 * c + lane] = db[c] * out;
       }
-      if (a.part_w) {
+      if (a.part_w && set == 0) {
         const bool any = (int)blockIdx.x < a.tiles;
         if (any) ok = ok && mbar_wait_warp(&bars.done, 0, 256u);
         tc_fence_after();
@@ -320,9 +339,9 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_head_kernel(const __gr
     const float out = a.scale ? a.scale->out : a.grad[0] * *a.inverse * (a.f16 ? 1.f / kDlScaleF16 : 1.f);
     int i = 0;
     for (int tile = blockIdx.x; tile < a.tiles; tile += gridDim.x, ++i) {
-      const int b = i & 1, row = 128 * tile + 32 * q + lane;
+      const int d = i % kDxs, row = 128 * tile + 32 * q + lane;
       const bool zero = row < a.rows && !row_counts(a.target[row], a.ignore);
-      if (!mbar_wait_warp(&bars.dx_full[b], (i >> 1) & 1, 512u)) break;
+      if (!mbar_wait_warp(&bars.dx_full[d], (i / kDxs) & 1, 512u)) break;
       tc_fence_after();
       for (int p = 0; p < a.panels; ++p) {
         unsigned char* const stg = sm + S::kStg + (2 * q + p) * 4096;
@@ -333,7 +352,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_head_kernel(const __gr
 #pragma unroll
         for (int h = 0; h < 64; h += 32) {
           uint32_t r[32];
-          tmem_ld32(lanes + 128 * b + 64 * p + h, r);
+          tmem_ld32(lanes + 128 * d + 64 * p + h, r);
           tmem_wait_ld();
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
@@ -349,7 +368,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_head_kernel(const __gr
         if (p == a.panels - 1) {
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&bars.dx_empty[b]);
+          if (lane == 0) mbar_arrive(&bars.dx_empty[d]);
         }
         if (a.want_dx) {
           asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
@@ -385,34 +404,33 @@ __global__ void __launch_bounds__(32) small_total_kernel(const double2* __restri
     *inverse = mean ? (float)(1.0 / fmax(c, 1.0)) : 1.f;
   }
 }
-// dW and db from what the CTAs of a backward pass have left.  A block: 32 classes of eight channels (one of the last blocks: of the bias).
+// dW and db from what the CTAs of a backward pass have left: a block for 32 classes of a channel (or, the last ones, of the bias), its warps along the
+// CTAs, in a fixed order.
 __global__ void __launch_bounds__(256) small_join_kernel(const float* __restrict__ part_w, const float* __restrict__ part_b, uint16_t* __restrict__ dw, void* __restrict__ db,
                                                          int ctas, int vp, int c, int classes, int f16, int db_type) {
+  __shared__ float x[8][32];
   pdl_wait();
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, groups = vp / 32, v = (blockIdx.x % groups) * 32 + lane, first = (blockIdx.x / groups) * 8;
-  if (first < c) {
-    if (!part_w) return;
-    const int ch = first + w;
-    if (v >= classes) return;
-    float s[4] = {};
-    const float* p = part_w + (int64_t)ch * vp + v;
-    for (int k = 0; k < ctas; k += 4) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, groups = vp / 32, v = (blockIdx.x % groups) * 32 + lane, ch = blockIdx.x / groups;
+  const float* const p = ch < c ? part_w + (int64_t)ch * vp + v : part_b + v;
+  const int64_t step = ch < c ? 128 * vp : vp;
+  const int n = ch < c ? ctas : 8 * ctas;
+  if (!(ch < c ? part_w : part_b)) return;
+  float s[4] = {};
+  for (int k = w; k < n; k += 32) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (k + j < ctas) s[j] += p[(int64_t)(k + j) * 128 * vp];
-    }
-    const float sum = (s[0] + s[1]) + (s[2] + s[3]);
-    dw[(int64_t)v * c + ch] = f16 ? __half_as_ushort(__float2half_rn(sum)) : __bfloat16_as_ushort(__float2bfloat16_rn(sum));
-  } else if (part_b) {
-    __shared__ float x[8][32];
-    float s = 0.f;
-    for (int k = w; k < 4 * ctas; k += 8) s += part_b[(int64_t)k * vp + v];
-    x[w][lane] = s;
-    __syncthreads();
-    if (w == 0 && v < classes) {
-      for (int k = 1; k < 8; ++k) s += x[k][lane];
-      bias_store(db, db_type, v, s);
-    }
+    for (int j = 0; j < 4; ++j)
+      if (k + 8 * j < n) s[j] += p[(k + 8 * j) * step];
+  }
+  x[w][lane] = (s[0] + s[1]) + (s[2] + s[3]);
+  __syncthreads();
+  if (w == 0 && v < classes) {
+    float all = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) all += x[k][lane];
+    if (ch == c)
+      bias_store(db, db_type, v, all);
+    else
+      dw[(int64_t)v * c + ch] = f16 ? __half_as_ushort(__float2half_rn(all)) : __bfloat16_as_ushort(__float2bfloat16_rn(all));
   }
 }
 
