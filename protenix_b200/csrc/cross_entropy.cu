@@ -29,7 +29,7 @@ struct EpiStats {
   float* hit;               // [rows]: logit of the row's class
   uint32_t* arrivals;
   int rows, classes;
-  static constexpr bool kMeets = true;
+  static constexpr bool kMeets = true, kStores = false;
   __device__ __forceinline__ void begin() const { *arrivals = 0; }
 
   struct Row {
@@ -42,12 +42,13 @@ struct EpiStats {
     const int64_t t = row < rows ? target[row] - e.n0 : -1;
     return {t >= 0 && t < S::kPartCols ? (int)t : -1, warp_bias<S>(e, bias, classes)};
   }
-  template <class S>
-  __device__ __forceinline__ void tile(const GemmEpiTile& e, const Row& at) const {
+  template <class S, class F>
+  __device__ __forceinline__ void tile(const GemmEpiTile& e, const Row& at, F release) const {
     constexpr int kCols = S::kPartCols;
     const int row = e.m0 + e.lane, base = e.n0, mine = at.mine;
     const bool there = row < rows;
     float m = -CUDART_INF_F, s = 0.f, sum = 0.f;
+    if (base >= classes) release();
 #pragma unroll 1
     for (int c = 0; c < kCols; c += 32) {
       const int left = classes - (base + c);
@@ -55,6 +56,7 @@ struct EpiStats {
       uint32_t r[32];
       tmem_ld32(e.acc + c, r);
       tmem_wait_ld();
+      if (c + 32 == kCols || left <= 32) release();
       float v[32];
 #pragma unroll
       for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
@@ -82,7 +84,7 @@ struct EpiStats {
     // the parts of the columns
     float* const x = e.shared + 32 * e.quarter + e.lane;
     if (e.part) x[384 * (e.part - 1)] = m, x[384 * (e.part - 1) + 128] = s, x[384 * (e.part - 1) + 256] = sum;
-    gemm_epi_sync<S>();
+    gemm_epi_sync<S>(e.set);
     if (!e.part) {
       float next = m;
 #pragma unroll
@@ -97,7 +99,7 @@ struct EpiStats {
         if (part_sum) part_sum[at] = sum;
       }
     }
-    gemm_epi_sync<S>();
+    gemm_epi_sync<S>(e.set);
   }
 };
 
@@ -279,7 +281,7 @@ __global__ void __launch_bounds__(256) loss_prepare_kernel(const ScanArgs a, con
 
 // ---- backward: dl ----------------------------------------------------------------------------------------------------
 struct EpiLogitGrad {
-  CUtensorMap out;          // dl [rows][classes of the piece], boxes of 32 x 64
+  CUtensorMap out;          // dl [rows][classes of the piece], boxes of 32 x 32
   const int64_t* target;
   HeadBias bias;            // of the piece
   const float2* norm;
@@ -290,7 +292,7 @@ struct EpiLogitGrad {
   int rows, classes, first, all_classes;      // first: the piece's first class
   float smooth;
   int f16;
-  static constexpr bool kMeets = false;
+  static constexpr bool kMeets = false, kStores = true;
   __device__ __forceinline__ void begin() const {}
 
   struct Row {
@@ -319,62 +321,55 @@ struct EpiLogitGrad {
     at.plain = warp_bias<S>(e, bias, classes);
     return at;
   }
-  template <class S>
-  __device__ __forceinline__ void tile(const GemmEpiTile& e, const Row& at) const {
+  template <class S, class F>
+  __device__ __forceinline__ void tile(const GemmEpiTile& e, const Row& at, F release) const {
     constexpr int kCols = S::kPartCols;
-    if (e.m0 >= rows) return;
     const int base = e.n0, mine = at.mine;
+    if (e.m0 >= rows || base >= classes) return release();
     const float over = at.over, ref = at.ref, less = at.less, less_hit = at.less_hit;
     const bool counts = at.counts;
 #pragma unroll 1
-    for (int c = 0; c < kCols; c += 64) {
-      if (base + c >= classes) break;
+    for (int c = 0; c < kCols; c += 32) {
+      const int left = classes - (base + c);
+      if (left <= 0) break;
+      uint32_t r[32];
+      tmem_ld32(e.acc + c, r);
+      tmem_wait_ld();
+      if (c + 32 == kCols || left <= 32) release();
+      float v[32];
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+      if (!at.plain) add_bias(v, e.own + c);
+      const int own = mine - c;
+      if (__any_sync(0xffffffffu, own >= 0 && own < 32)) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = fmaf(over, fast_exp2(fmaf(v[j], kLog2e, ref)), own == j ? less_hit : -less);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = fmaf(over, fast_exp2(fmaf(v[j], kLog2e, ref)), -less);
+      }
+      if (!counts) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = 0.f;
+      }
       if (e.lane == 0) tma_store_wait_read<0>();
       __syncwarp();
-#pragma unroll 1
-      for (int h = 0; h < 64; h += 32) {
-        const int left = classes - (base + c + h);
-        uint32_t r[32];
-        tmem_ld32(e.acc + c + h, r);
-        tmem_wait_ld();
-        float v[32];
 #pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
-        if (!at.plain) add_bias(v, e.own + c + h);
-        const int own = mine - (c + h);
-        if (__any_sync(0xffffffffu, own >= 0 && own < 32)) {
+      for (int p = 0; p < 4; ++p) {
+        uint32_t o[4];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = fmaf(over, fast_exp2(fmaf(v[j], kLog2e, ref)), own == j ? less_hit : -less);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = fmaf(over, fast_exp2(fmaf(v[j], kLog2e, ref)), -less);
-        }
-        if (!counts) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = 0.f;
-        }
-#pragma unroll
-        for (int p = 0; p < 4; ++p) {
-          uint4 o;
-          if (f16) {
-            o.x = pack_f16x2_inf(v[8 * p], v[8 * p + 1]), o.y = pack_f16x2_inf(v[8 * p + 2], v[8 * p + 3]);
-            o.z = pack_f16x2_inf(v[8 * p + 4], v[8 * p + 5]), o.w = pack_f16x2_inf(v[8 * p + 6], v[8 * p + 7]);
-          } else {
-            o.x = pack_bf16x2(v[8 * p], v[8 * p + 1]), o.y = pack_bf16x2(v[8 * p + 2], v[8 * p + 3]);
-            o.z = pack_bf16x2(v[8 * p + 4], v[8 * p + 5]), o.w = pack_bf16x2(v[8 * p + 6], v[8 * p + 7]);
-          }
-          *reinterpret_cast<uint4*>(e.stg + e.lane * 128 + (((h / 8 + p) ^ (e.lane & 7)) << 4)) = o;
-        }
-        if (part_bias) {
-          column_sums(v, e.lane);
-          if (e.lane < left) part_bias[(int64_t)(e.m0 / 32) * classes + base + c + h + e.lane] = v[0];
-        }
+        for (int w = 0; w < 4; ++w) o[w] = f16 ? pack_f16x2_inf(v[8 * p + 2 * w], v[8 * p + 2 * w + 1]) : pack_bf16x2(v[8 * p + 2 * w], v[8 * p + 2 * w + 1]);
+        *reinterpret_cast<uint4*>(e.stg + e.lane * 64 + ((p ^ (e.lane >> 1 & 3)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
       }
       asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
       __syncwarp();
       if (e.lane == 0) {
         tma_store_3d(&out, smem_u32(e.stg), base + c, e.m0, 0);
         tma_store_commit();
+      }
+      if (part_bias) {
+        column_sums(v, e.lane);
+        if (e.lane < left) part_bias[(int64_t)(e.m0 / 32) * classes + base + c + e.lane] = v[0];
       }
     }
   }
@@ -419,11 +414,11 @@ struct EpiGrad {
     const int row = e.m0 + e.lane;
     return {kF32 ? 1.f : scale->out, !kF32 && target && row < rows && !row_counts(target[row], ignore)};
   }
-  template <class S>
-  __device__ __forceinline__ void tile(const GemmEpiTile& e, const Row& at) const {
+  template <class S, class F>
+  __device__ __forceinline__ void tile(const GemmEpiTile& e, const Row& at, F release) const {
     constexpr int kCols = S::kPartCols, kBlock = kF32 ? 32 : 64;
-    if (e.m0 >= rows) return;
     const int base = e.n0;
+    if (e.m0 >= rows || base >= cols) return release();
     const float by = at.by;
     const bool zero = at.zero;
 #pragma unroll 1
@@ -436,6 +431,7 @@ struct EpiGrad {
         uint32_t r[32];
         tmem_ld32(e.acc + c + h, r);
         tmem_wait_ld();
+        if (h + 32 == kBlock && (c + kBlock == kCols || base + c + kBlock >= cols)) release();
         if constexpr (kF32) {
 #pragma unroll
           for (int p = 0; p < 8; ++p)
@@ -494,9 +490,13 @@ PX_DEFINE_FAMILY_HOOKS(loss)
 static int64_t up(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
 
 // Shapes of the products: logits (both operands along k), dx (W across), dW (both across).
-typedef GemmShape<1, 64, false, false, 6, 4, true> Logits64;
-typedef GemmShape<1, 256, false, false, 3, 16, true> Logits256;
-typedef GemmShape<2, 256, false, false, 4, 16, true> LogitsPair;
+// The logits' epilogues: without anything to store (forward) or with blocks of 2 KB (backward).
+template <bool kStore>
+struct Logits {
+  typedef GemmShape<1, 64, false, false, 6, 2, 4, kStore ? 2048 : 0, true> Narrow;
+  typedef GemmShape<1, 256, false, false, kStore ? 3 : 4, 2, 8, kStore ? 2048 : 0, true> Single;
+  typedef GemmShape<2, 256, false, false, kStore ? 5 : 6, 2, 8, kStore ? 2048 : 0, true> Pair;
+};
 typedef GemmShape<1, 128, false, true, 5> Dx128;
 typedef GemmShape<1, 256, false, true, 4> Dx256;
 typedef GemmShape<2, 256, false, true, 5> DxPair;
@@ -579,6 +579,10 @@ static bool out_map(CUtensorMap* map, CUtensorMapDataType type, int size, const 
   return make_map_3d(map, type, base, (uint64_t)cols, (uint64_t)rows, (uint64_t)slots, (uint64_t)ld * size, (uint64_t)rows * ld * size, 128 / size, 32,
                      CU_TENSOR_MAP_SWIZZLE_128B);
 }
+// boxes of 32 x 32 of a result in 16 bits
+static bool dl_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, int64_t cols, int64_t rows, int64_t ld) {
+  return make_map_3d(map, type, base, (uint64_t)cols, (uint64_t)rows, 1, (uint64_t)ld * 2, (uint64_t)rows * ld * 2, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B);
+}
 static CUtensorMapDataType type16(bool f16) { return f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16; }
 
 // rows of x against `classes` rows of w from class `first` on
@@ -591,9 +595,10 @@ static int32_t launch_logits(const px_head& h, int64_t first, int64_t classes, c
     return PX_ERR_LAUNCH;
   GemmTiles t = c.t;
   t.tiles_n = (int)(up(classes, c.kn) / c.kn);
-  if (c.kn == 64) return ops.idesc = Logits64::idesc(f16), gemm_launch<Logits64>(ops, epi, t, st);
-  if (c.ctas == 1) return ops.idesc = Logits256::idesc(f16), gemm_launch<Logits256>(ops, epi, t, st);
-  return ops.idesc = LogitsPair::idesc(f16), gemm_launch<LogitsPair>(ops, epi, t, st);
+  typedef Logits<Epi::kStores> L;
+  if (c.kn == 64) return ops.idesc = L::Narrow::idesc(f16), gemm_launch<typename L::Narrow>(ops, epi, t, st);
+  if (c.ctas == 1) return ops.idesc = L::Single::idesc(f16), gemm_launch<typename L::Single>(ops, epi, t, st);
+  return ops.idesc = L::Pair::idesc(f16), gemm_launch<typename L::Pair>(ops, epi, t, st);
 }
 template <class N, class W, class P, class Epi>
 static int32_t launch_grad(GemmOperands& ops, bool f16, const HeadCut& c, const Epi& epi, const GemmTiles& t, cudaStream_t st) {
@@ -742,7 +747,7 @@ extern "C" int32_t px_head_loss_bwd(const px_head* head, const float* norm, cons
   for (int64_t i = 0; i < p.pieces; ++i) {
     const int64_t first = i * p.piece, vc = std::min(p.piece, h.classes - first);
     EpiLogitGrad el = {};
-    if (!out_map(&el.out, type16(f16), 2, dl, vc, h.rows, p.ld, 1)) return PX_ERR_LAUNCH;
+    if (!dl_map(&el.out, type16(f16), dl, vc, h.rows, p.ld)) return PX_ERR_LAUNCH;
     el.target = h.target, el.bias = {h.bias ? (const char*)h.bias + first * bias_size : nullptr, h.bias_dtype}, el.norm = (const float2*)norm, el.grad = each ? grad : nullptr, el.scale = scale;
     el.part_bias = dbias ? part_bias : nullptr, el.ignore = h.ignore, el.rows = (int)h.rows, el.classes = (int)vc, el.first = (int)first;
     el.all_classes = (int)h.classes, el.smooth = h.smoothing, el.f16 = f16;

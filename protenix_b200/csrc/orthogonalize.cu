@@ -17,6 +17,7 @@ namespace px {
 
 constexpr float kPlaneScale = 1024.f;
 constexpr int kOrthoEpiWarps = 8, kOrthoThreads = 64 + 32 * kOrthoEpiWarps;
+constexpr int kOrthoStgBytes = 4096;      // staged block of a warp
 
 // ---- norm and first iterate ------------------------------------------------------------------------------------------
 constexpr int kNormBlocks = 64;
@@ -107,7 +108,7 @@ struct PlaneShape {
   static constexpr int kCtas = kCtas_, kUnits = kCtas, kSide = 128 * kCtas, kStages = 3;
   static constexpr bool kAMn = kAMn_, kBMn = kBMn_;
   static constexpr int kPlaneBytes = kGemmM * kGemmK * 2, kStageBytes = 4 * kPlaneBytes;      // A hi, A lo, B hi, B lo: 128 rows each
-  static constexpr int kStg = kStages * kStageBytes, kBars = kStg + kOrthoEpiWarps * kGemmStgBytes;
+  static constexpr int kStg = kStages * kStageBytes, kBars = kStg + kOrthoEpiWarps * kOrthoStgBytes;
   static constexpr size_t kSmem = kBars + 256 + 1024;
   static constexpr uint32_t kIdesc = umma_idesc_f16(kGemmM * kCtas, 128, kAMn, kBMn);
   static_assert(kSmem <= 232448, "shared memory budget");
@@ -361,7 +362,7 @@ plane_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     }
   } else {
     const int q = warp & 3, half = (warp - 2) >> 2;
-    unsigned char* const stg = ring + S::kStg + (warp - 2) * kGemmStgBytes;
+    unsigned char* const stg = ring + S::kStg + (warp - 2) * kOrthoStgBytes;
     const uint32_t lanes = tmem_base + ((uint32_t)(32 * q) << 16) + 64 * half;
     auto arrive = [&](uint64_t* bar) {
       tc_fence_before();

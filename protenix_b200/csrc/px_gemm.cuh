@@ -6,7 +6,8 @@
 // One CTA works on 128 x kN, or a pair of them (cta_group::2) on 256 x kN, each with its own 128 rows of A and half of B: the pair asks L2 for
 // 64 bytes a cycle where a CTA alone with kN = 256 asks for 96.
 //
-// Roles: warp 0 copies, warp 1 issues products, kEpiWarps (4, 8 or 16) are the epilogue (a quarter of the lanes and 1, 1/2 or 1/4 of the columns each).
+// Roles: warp 0 copies, warp 1 issues products, kSets sets of kSetWarps (4 or 8) are the epilogue: a warp has a quarter of the lanes and all or half of
+// the columns; two sets take the tiles in turn, each with an accumulator of its own.
 // Accumulators are double-buffered.
 #pragma once
 #include "px_pair.cuh"
@@ -15,18 +16,17 @@
 namespace px {
 
 constexpr int kGemmM = 128, kGemmK = 64;          // rows of a CTA's tile, k of a stage
-constexpr int kGemmStgBytes = 4096;               // staged block of a warp: 32 rows of 128 bytes
 
-template <int kCtas_, int kN_, bool kAMn_, bool kBMn_, int kStages_, int kEpiWarps_ = 8, bool kEpiMemory = false>
+template <int kCtas_, int kN_, bool kAMn_, bool kBMn_, int kStages_, int kSets_ = 1, int kSetWarps_ = 8, int kStgBytes_ = 4096, bool kEpiMemory = false>
 struct GemmShape {
-  static constexpr int kCtas = kCtas_, kN = kN_, kStages = kStages_, kEpiWarps = kEpiWarps_, kThreads = 64 + 32 * kEpiWarps;
-  static constexpr int kParts = kEpiWarps / 4, kPartCols = kN / kParts;      // columns of an epilogue warp
+  static constexpr int kCtas = kCtas_, kN = kN_, kStages = kStages_, kSets = kSets_, kSetWarps = kSetWarps_, kEpiWarps = kSets * kSetWarps, kThreads = 64 + 32 * kEpiWarps;
+  static constexpr int kParts = kSetWarps / 4, kPartCols = kN / kParts, kStgBytes = kStgBytes_;      // columns of an epilogue warp
   static constexpr bool kAMn = kAMn_, kBMn = kBMn_;
   static constexpr int kBRows = kN / kCtas;       // rows of B that a CTA loads
   static constexpr int kABytes = kGemmM * kGemmK * 2, kBBytes = kBRows * kGemmK * 2;
   static constexpr int kStageBytes = kABytes + kBBytes;
   static constexpr uint32_t kCols = 2 * kN;
-  static constexpr int kStg = kStages * kStageBytes, kExtra = kStg + kEpiWarps * kGemmStgBytes, kExtraBytes = kEpiMemory ? 1536 * (kParts - 1) + 4 * kEpiWarps * kPartCols : 0;
+  static constexpr int kStg = kStages * kStageBytes, kExtra = kStg + kEpiWarps * kStgBytes, kExtraBytes = kEpiMemory ? 1536 * (kParts - 1) * kSets + 4 * kEpiWarps * kPartCols : 0;
   static constexpr int kBars = kExtra + kExtraBytes;
   static constexpr size_t kSmem = kBars + 256 + 1024;
   static_assert(kSmem <= 232448, "shared memory budget");
@@ -81,13 +81,13 @@ struct GemmEpiTile {
   GemmTile at;
   int m0, n0;                        // first of this warp's 32 rows, first of its columns
   uint32_t acc;                      // tensor memory, lanes and first column of this warp
-  int quarter, part, lane;
-  unsigned char* stg;                // kGemmStgBytes of this warp's own
+  int quarter, part, lane, set;
+  unsigned char* stg;                // kStgBytes of this warp's own, for blocks of 32 rows that leave by TMA
   float* own;                        // kEpiMemory: a number for each column of this warp, its own
-  float* shared;                     // 384 numbers for each part but the first, shared by the epilogue's warps
+  float* shared;                     // 384 numbers for each part but the first, shared by the warps of a set
 };
 template <class S>
-__device__ __forceinline__ void gemm_epi_sync() { asm volatile("bar.sync 1, %0;\n" ::"n"(32 * S::kEpiWarps) : "memory"); }
+__device__ __forceinline__ void gemm_epi_sync(int set) { asm volatile("bar.sync %0, %1;\n" ::"r"(1 + set), "n"(32 * S::kSetWarps) : "memory"); }
 
 template <class S, class Epi>
 __global__ void __launch_bounds__(S::kThreads, 1)
@@ -110,7 +110,7 @@ gemm_kernel(const __grid_constant__ GemmOperands ops, const __grid_constant__ Ep
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&bars.acc_full[b], 1);
-      mbar_init(&bars.acc_empty[b], S::kEpiWarps * S::kCtas);
+      mbar_init(&bars.acc_empty[b], S::kSetWarps * S::kCtas);
     }
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
@@ -230,14 +230,14 @@ gemm_kernel(const __grid_constant__ GemmOperands ops, const __grid_constant__ Ep
     }
   } else {
     const int q = warp & 3;                                // the quarter of the lanes that this warp may access goes by its index
-    uint32_t count = 0;
     bool ok = true;
     GemmEpiTile e;
-    e.quarter = q, e.part = (warp - 2) >> 2, e.lane = lane;
-    e.stg = ring + S::kStg + (warp - 2) * kGemmStgBytes;
+    e.quarter = q, e.set = (warp - 2) / S::kSetWarps, e.part = (warp - 2) % S::kSetWarps >> 2, e.lane = lane;
+    uint32_t count = e.set;
+    e.stg = ring + S::kStg + (warp - 2) * S::kStgBytes;
     e.own = reinterpret_cast<float*>(ring + S::kExtra) + (warp - 2) * S::kPartCols;
-    e.shared = reinterpret_cast<float*>(ring + S::kExtra) + S::kEpiWarps * S::kPartCols;
-    for (int tile = first_tile; tile < tiles.total; tile += tile_step, ++count) {
+    e.shared = reinterpret_cast<float*>(ring + S::kExtra) + S::kEpiWarps * S::kPartCols + 384 * (S::kParts - 1) * e.set;
+    for (int tile = first_tile + e.set * tile_step; tile < tiles.total; tile += S::kSets * tile_step, count += S::kSets) {
       e.at = gemm_tile(tiles, tile);
       const uint32_t ab = count & 1, aph = (count >> 1) & 1;
       e.m0 = (e.at.mt * S::kCtas + (int)rank) * kGemmM + 32 * q;
@@ -247,15 +247,17 @@ gemm_kernel(const __grid_constant__ GemmOperands ops, const __grid_constant__ Ep
       ok = ok && mbar_wait_warp(&bars.acc_full[ab], aph, 8u);
       if (!Epi::kMeets && !ok) break;                      // an epilogue whose warps meet goes through all tiles
       tc_fence_after();
-      epi.template tile<S>(e, row);
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        if constexpr (kPair)
-          mbar_arrive_cluster(map_to_rank(smem_u32(&bars.acc_empty[ab]), 0));
-        else
-          mbar_arrive(&bars.acc_empty[ab]);
-      }
+      // called once by a whole warp, when it has read the last of the accumulator
+      epi.template tile<S>(e, row, [&] {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if constexpr (kPair)
+            mbar_arrive_cluster(map_to_rank(smem_u32(&bars.acc_empty[ab]), 0));
+          else
+            mbar_arrive(&bars.acc_empty[ab]);
+        }
+      });
     }
     if (lane == 0) tma_store_wait_read<0>();
   }
