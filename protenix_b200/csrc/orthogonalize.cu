@@ -11,6 +11,8 @@
 //
 // A and the polynomial are symmetric: only tiles on and above the diagonal are formed, the epilogue stores each a second time transposed, which
 // saves half of two of the three products.
+#include <algorithm>
+
 #include "px_gemm.cuh"
 
 namespace px {
@@ -446,6 +448,12 @@ plane_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
   if constexpr (kPair) tc_cluster_sync();
 }
 
+}  // namespace px
+
+#include "px_ortho_small.cuh"
+
+namespace px {
+
 PX_DEFINE_FAMILY_HOOKS(update)
 
 // ---- host ------------------------------------------------------------------------------------------------------------
@@ -552,6 +560,17 @@ extern "C" int32_t px_orthogonalize(const void* g, void* out, int64_t batch, int
   if (workspace_bytes < p.bytes) return PX_ERR_WORKSPACE;
   if (!have_context()) return PX_ERR_LAUNCH;
   const cudaStream_t st = (cudaStream_t)stream;
+  int slices = 1;
+  if (const int ctas = small_ortho_ctas(batch, p.s, std::max(m, n), steps, &slices)) {
+    SmallOrtho a = {};
+    a.g = g, a.out = out, a.stride = m * n, a.ld = (int)n, a.side = (int)p.s, a.length = (int)std::max(m, n);
+    a.steps = steps, a.ctas = ctas, a.eps = eps;
+    std::copy(coefficients, coefficients + 3 * steps, a.abc);
+    const bool ok = dtype == PX_F32    ? launch_small_ortho<float>(a, batch, slices, m > n, st)
+                    : dtype == PX_BF16 ? launch_small_ortho<bf16>(a, batch, slices, m > n, st)
+                                       : launch_small_ortho<__half>(a, batch, slices, m > n, st);
+    return ok ? PX_OK : PX_ERR_LAUNCH;
+  }
   char* const ws = (char*)workspace;
   const bool wide = m <= n;
   double* sums = (double*)(ws + p.sums);
