@@ -49,15 +49,13 @@ __global__ void __launch_bounds__(256) ortho_norm_kernel(const T* __restrict__ g
     sums[blockIdx.y * gridDim.x + blockIdx.x] = s0;
   }
 }
-// v = hi + 2^-11 lo
-__device__ __forceinline__ void split_planes(float v, __half& hi, __half& lo) {
-  hi = __float2half_rn(v);
-  lo = __float2half_rn((v - __half2float(hi)) * 2048.f);
-}
+// v = hi + 2^-11 lo, two values at a time
 __device__ __forceinline__ void split_planes2(float x, float y, uint32_t& hi, uint32_t& lo) {
   hi = pack_f16x2_inf(x, y);
   const float2 h = unpack_f16x2(hi);
-  lo = pack_f16x2_inf((x - h.x) * 2048.f, (y - h.y) * 2048.f);
+  // 2048 v - 2048 hi, both exact
+  const float2 r = apart2(fma2(pair2(h.x, h.y), pair2(-2048.f, -2048.f), mul2(pair2(x, y), pair2(2048.f, 2048.f))));
+  lo = pack_f16x2_inf(r.x, r.y);
 }
 // The planes of G 2^10 / (|G| + eps), eight columns a thread; columns behind n are zero.
 template <typename T>
@@ -566,9 +564,9 @@ extern "C" int32_t px_orthogonalize(const void* g, void* out, int64_t batch, int
     a.g = g, a.out = out, a.stride = m * n, a.ld = (int)n, a.side = (int)p.s, a.length = (int)std::max(m, n);
     a.steps = steps, a.ctas = ctas, a.eps = eps;
     std::copy(coefficients, coefficients + 3 * steps, a.abc);
-    const bool ok = dtype == PX_F32    ? launch_small_ortho<float>(a, batch, slices, m > n, st)
-                    : dtype == PX_BF16 ? launch_small_ortho<bf16>(a, batch, slices, m > n, st)
-                                       : launch_small_ortho<__half>(a, batch, slices, m > n, st);
+    const int size = dtype == PX_F32 ? 4 : 2;
+    a.type = dtype, a.wide_access = n * size % 16 == 0 && (((uintptr_t)g | (uintptr_t)out) & 15) == 0;
+    const bool ok = launch_small_ortho(a, batch, slices, m > n, st);
     return ok ? PX_OK : PX_ERR_LAUNCH;
   }
   char* const ws = (char*)workspace;

@@ -14,7 +14,7 @@
 
 namespace px {
 
-constexpr int kSmallSteps = 32, kSmallOrthoThreads = 256;
+constexpr int kSmallSteps = 32, kSmallOrthoThreads = 256;      // and a warp that issues the products
 constexpr int kSmallPlane = 2 * 128 * 128;                 // [128][128] fp16, two panels of 64 columns
 
 struct SmallOrtho {
@@ -23,7 +23,8 @@ struct SmallOrtho {
   int64_t stride;               // of a matrix
   int ld;                       // its columns
   int side, length;             // short and long side
-  int steps, ctas;
+  int steps, ctas, type;
+  int wide_access;              // rows of the matrix are aligned to 16 bytes
   double eps;
   float abc[3 * kSmallSteps];
 };
@@ -35,7 +36,7 @@ struct SmallOrthoShape {
   static_assert(kSmem <= 232448, "shared memory budget");
 };
 struct SmallOrthoBarriers {
-  uint64_t done;
+  uint64_t lead, done;          // the leading products; all of them
   uint32_t tmem_base, stop[8];
   double part[8], sums[8];      // of this CTA's warps; of the cluster's CTAs
 };
@@ -43,11 +44,81 @@ struct SmallOrthoBarriers {
 __device__ __forceinline__ int plane_offset(int row, int piece) {      // of the 16 bytes with columns 8 piece ..
   return (piece >> 3) * (kSmallPlane / 2) + row * 128 + (((piece & 7) ^ (row & 7)) << 4);
 }
-template <typename T>
-__device__ __forceinline__ float small_value(const void* g, int64_t at) { return (float)((const T*)g)[at]; }
+// A slice as 128 rows of 128 floats, the way in and out, and A's parts.  Pieces of 16 bytes are exchanged by row, so that neither eight rows of a piece nor
+// a piece of every eighth row meet in a bank.
+__device__ __forceinline__ int float_offset(int row, int col) { return row * 512 + (((col >> 2) ^ ((row ^ (row >> 3)) & 31)) << 4) + 4 * (col & 3); }
+__device__ __forceinline__ float small_value(const void* g, int64_t at, int type) {
+  return type == PX_F32 ? ((const float*)g)[at] : type == PX_F16 ? __half2float(((const __half*)g)[at]) : __bfloat162float(((const bf16*)g)[at]);
+}
+// 16 bytes of a matrix as 4 or 8 values
+__device__ __forceinline__ int small_values(const uint4& u, int type, float (&v)[8]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (type == PX_F32) {
+      v[j] = __uint_as_float(w[j]);
+    } else {
+      const float2 x = type == PX_F16 ? unpack_f16x2(w[j]) : unpack_bf16x2(w[j]);
+      v[2 * j] = x.x, v[2 * j + 1] = x.y;
+    }
+  }
+  return type == PX_F32 ? 4 : 8;
+}
 
-template <typename T, int kSlices, bool kTall>
-__global__ void __launch_bounds__(kSmallOrthoThreads, 1) small_ortho_kernel(const __grid_constant__ SmallOrtho p) {
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.aligned;\n" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;\n" ::: "memory"); }
+
+// A from its parts in the kCtas CTAs of a cluster: every row goes to the CTA that adds it up (row / kShare), which writes the planes of the sum to all of
+// them.  `sum`: this thread's row, columns 64 half ..; the parts lie where A will be, part k from row k kShare on.
+template <int kCtas>
+__device__ __forceinline__ void exchange_gram(unsigned char* gram, int rank, int row, int half, const float (&sum)[64]) {
+  constexpr int kShare = 128 / kCtas, kGroups = 8 / kCtas;      // rows of a CTA; eight columns each of a thread
+  cluster_wait();                                               // nobody multiplies by what lies there any more
+  {
+    const int to = row / kShare, r = rank * kShare + row % kShare;
+    const uint32_t there = map_to_rank(smem_u32(gram), to);
+#pragma unroll
+    for (int k = 0; k < 16; ++k)
+      asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};\n" ::"r"(there + float_offset(r, 64 * half + 4 * k)), "f"(sum[4 * k]), "f"(sum[4 * k + 1]),
+                   "f"(sum[4 * k + 2]), "f"(sum[4 * k + 3])
+                   : "memory");
+  }
+  tc_cluster_sync();
+  uint4 hi[kGroups], lo[kGroups];
+#pragma unroll
+  for (int i = 0; i < kGroups; ++i) {
+    const int at = threadIdx.x + kSmallOrthoThreads * i, r = at >> 4, piece = at & 15;
+    float v[8] = {};
+#pragma unroll
+    for (int k = 0; k < kCtas; ++k) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float4 x = *reinterpret_cast<const float4*>(gram + float_offset(k * kShare + r, 8 * piece + 4 * j));
+        v[4 * j] += x.x, v[4 * j + 1] += x.y, v[4 * j + 2] += x.z, v[4 * j + 3] += x.w;
+      }
+    }
+    constexpr float f = 1.f / kPlaneScale;
+    split_planes2(f * v[0], f * v[1], hi[i].x, lo[i].x), split_planes2(f * v[2], f * v[3], hi[i].y, lo[i].y);
+    split_planes2(f * v[4], f * v[5], hi[i].z, lo[i].z), split_planes2(f * v[6], f * v[7], hi[i].w, lo[i].w);
+  }
+  tc_cluster_sync();                                            // all parts are read
+#pragma unroll
+  for (int i = 0; i < kGroups; ++i) {
+    const int at = threadIdx.x + kSmallOrthoThreads * i, r = rank * kShare + (at >> 4), piece = at & 15;
+    const uint32_t to = smem_u32(gram + plane_offset(r, piece));
+#pragma unroll
+    for (int k = 0; k < kCtas; ++k) {
+      const uint32_t there = map_to_rank(to, k);
+      asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(there), "r"(hi[i].x), "r"(hi[i].y), "r"(hi[i].z), "r"(hi[i].w) : "memory");
+      asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(there + kSmallPlane), "r"(lo[i].x), "r"(lo[i].y), "r"(lo[i].z), "r"(lo[i].w) : "memory");
+    }
+  }
+  asm volatile("fence.proxy.async;\n" ::: "memory");
+  tc_cluster_sync();
+}
+
+template <int kSlices, bool kTall>
+__global__ void __launch_bounds__(kSmallOrthoThreads + 32, 1) small_ortho_kernel(const __grid_constant__ SmallOrtho p) {
   typedef SmallOrthoShape<kSlices> S;
   constexpr float kScale = kPlaneScale;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
@@ -59,6 +130,7 @@ __global__ void __launch_bounds__(kSmallOrthoThreads, 1) small_ortho_kernel(cons
 
   bool skip = cta_begin();
   if (threadIdx.x == 0) {
+    mbar_init(&bars.lead, 1);
     mbar_init(&bars.done, 1);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
@@ -80,27 +152,138 @@ __global__ void __launch_bounds__(kSmallOrthoThreads, 1) small_ortho_kernel(cons
   pdl_wait();
   const uint32_t tmem = bars.tmem_base;
 
-  if (!skip) {
-    // ---- the first iterate -------------------------------------------------------------------------------------------
-    const void* const g = (const T*)p.g + matrix * p.stride;
-    const int first = rank * kSlices * 128;                // of this CTA's columns along the long side
-    // eight values along the long side: row r of the slices, columns c0 ..
-    auto read = [&](int i, float (&v)[8]) {
-      const int r = kTall ? i & 127 : i / (16 * kSlices), c0 = first + 8 * (kTall ? i >> 7 : i % (16 * kSlices));
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int c = c0 + j;
-        v[j] = r < p.side && c < p.length ? small_value<T>(g, kTall ? (int64_t)c * p.ld + r : (int64_t)r * p.ld + c) : 0.f;
+  constexpr uint32_t idesc_kk = umma_idesc_f16(128, 128), idesc_kn = umma_idesc_f16(128, 128, false, true);
+  constexpr uint64_t kLo = kSmallPlane >> 4, kPanel = kSmallPlane >> 5;
+  unsigned char* const gram = sm + S::kA;
+  // Before a product all threads meet: its operands are in shared memory, and the accumulators have been read.
+  auto meet = [&] {
+    tc_fence_before();
+    asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+    __syncthreads();
+  };
+
+  if (skip) {
+    // nothing
+  } else if (warp == 8) {
+    // ---- products: accumulators of the leading ones at columns 0, 128 and 384, of the rest at 256 ------------------------
+    const uint64_t gram_at = umma_desc_sw128(smem_u32(gram));
+    auto issue = [&](auto leading, auto rest) {
+      meet();
+      tc_fence_after();
+      if (elect_lane()) {
+        leading();
+        umma_commit(&bars.lead);
+        rest();
+        umma_commit(&bars.done);
       }
+      __syncwarp();
     };
-    double s = 0.0;
-#pragma unroll 4
-    for (int i = threadIdx.x; i < 2048 * kSlices; i += kSmallOrthoThreads) {
-      float v[8];
-      read(i, v);
+    // operand u along k, w along k (K-major) or across it
+    auto one = [&](uint64_t u, uint64_t w, bool across, uint32_t idesc) {
+      issue(
+          [&] {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) s = fma((double)v[j], (double)v[j], s);
+            for (int ks = 0; ks < 8; ++ks)
+              umma_bf16(tmem + 128 * (ks >> 2), u + (ks >> 2) * kPanel + 2 * (ks & 3), w + (across ? 128 * ks : (ks >> 2) * kPanel + 2 * (ks & 3)), idesc, (ks & 3) ? 1u : 0u);
+          },
+          [&] {
+#pragma unroll
+            for (int ks = 0; ks < 8; ++ks) {
+              const uint64_t x = u + (ks >> 2) * kPanel + 2 * (ks & 3), y = w + (across ? 128 * ks : (ks >> 2) * kPanel + 2 * (ks & 3));
+              umma_bf16(tmem + 256, x, y + kLo, idesc, ks ? 1u : 0u);
+              umma_bf16(tmem + 256, x + kLo, y, idesc, 1u);
+            }
+          });
+    };
+    auto slice_at = [&](int n) { return umma_desc_sw128(smem_u32(sm + S::kX + (n >> 1) * 2 * kSmallPlane)) + (n & 1) * kPanel; };      // panels of 64 k
+    // the barriers of the other warps' way in
+    __syncthreads();
+    if (p.ctas > 1) tc_cluster_sync();
+    else __syncthreads();
+    for (int n = 0; n < kSlices; ++n) __syncthreads();
+    if (p.ctas > 1) cluster_arrive();
+    for (int step = 0; step < p.steps; ++step) {
+      issue(
+          [&] {
+#pragma unroll
+            for (int n = 0; n < 2 * kSlices; ++n) {
+              const uint64_t x = slice_at(n);
+#pragma unroll
+              for (int ks = 0; ks < 4; ++ks) umma_bf16(tmem + (n == 2 ? 384 : 128 * (n & 1)), x + 2 * ks, x + 2 * ks, idesc_kk, (ks > 0 || n == 3) ? 1u : 0u);
+            }
+          },
+          [&] {
+#pragma unroll
+            for (int n = 0; n < 2 * kSlices; ++n) {
+              const uint64_t x = slice_at(n);
+#pragma unroll
+              for (int ks = 0; ks < 4; ++ks) {
+                umma_bf16(tmem + 256, x + 2 * ks, x + kLo + 2 * ks, idesc_kk, (n | ks) ? 1u : 0u);
+                umma_bf16(tmem + 256, x + kLo + 2 * ks, x + 2 * ks, idesc_kk, 1u);
+              }
+            }
+          });
+      if (p.ctas > 1) {
+        cluster_wait();
+        for (int k = 0; k < (p.ctas == 2 ? 1 : 3); ++k) tc_cluster_sync();
+      }
+      one(gram_at, gram_at, false, idesc_kk);
+      for (int n = 0; n < kSlices; ++n) one(gram_at, umma_desc_mn_sw128(smem_u32(sm + S::kX + n * 2 * kSmallPlane), kSmallPlane / 2, 1024), true, idesc_kn);
+      if (p.ctas > 1 && step < p.steps - 1) cluster_arrive();
     }
+    __syncthreads();
+  } else {
+    // ---- the first iterate -------------------------------------------------------------------------------------------
+    const int size = p.type == PX_F32 ? 4 : 2;
+    const char* const g = (const char*)p.g + matrix * p.stride * size;
+    const int first = rank * kSlices * 128;                // of this CTA's columns along the long side
+    // lines along the rows of the matrix, `unit` elements at a time: a line is a row of the slices, or (tall) a column of them
+    const int unit = p.wide_access ? 16 / size : 1, across = (kTall ? 128 : 128 * kSlices) / unit, lines = kTall ? 128 * kSlices : 128;
+    const int end = kTall ? p.side : min(p.length - first, 128 * kSlices), last_line = kTall ? min(p.length - first, lines) : p.side;
+    const int64_t from = kTall ? (int64_t)first * p.ld : first;
+    double s4[4] = {};
+    for (int i0 = threadIdx.x; i0 < across * lines; i0 += 8 * kSmallOrthoThreads) {
+      uint4 u[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int i = i0 + k * kSmallOrthoThreads, line = i / across, at = (i - line * across) * unit;
+        u[k] = make_uint4(0, 0, 0, 0);
+        if (line < last_line && at < end) {
+          const int64_t e = from + (int64_t)line * p.ld + at;
+          if (unit > 1) u[k] = __ldg(reinterpret_cast<const uint4*>(g + e * size));      // rows are whole pieces of 16 bytes
+          else u[k].x = __float_as_uint(small_value(g, e, p.type));
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int i = i0 + k * kSmallOrthoThreads, line = i / across, at = (i - line * across) * unit;
+        float v[8];
+        if (unit > 1) small_values(u[k], p.type, v);
+        else v[0] = __uint_as_float(u[k].x);
+        auto place = [&](int j) {
+          const int r = kTall ? at + j : line, c = kTall ? line : at + j;
+          return sm + S::kX + (c >> 7) * 2 * kSmallPlane + float_offset(r, c & 127);
+        };
+#pragma unroll
+        for (int j = 0; j < 8; j += 4) {
+          if (j >= unit) break;
+          if (unit == 1) {
+            s4[0] = fma((double)v[0], (double)v[0], s4[0]);
+            *reinterpret_cast<float*>(place(0)) = v[0];
+            break;
+          }
+#pragma unroll
+          for (int w = 0; w < 4; ++w) s4[w] = fma((double)v[j + w], (double)v[j + w], s4[w]);
+          if (kTall) {
+#pragma unroll
+            for (int w = 0; w < 4; ++w) *reinterpret_cast<float*>(place(j + w)) = v[j + w];
+          } else {
+            *reinterpret_cast<float4*>(place(j)) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+          }
+        }
+      }
+    }
+    double s = (s4[0] + s4[1]) + (s4[2] + s4[3]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     if (lane == 0) bars.part[warp] = s;
@@ -117,210 +300,189 @@ __global__ void __launch_bounds__(kSmallOrthoThreads, 1) small_ortho_kernel(cons
     s = 0.0;
     for (int r = 0; r < p.ctas; ++r) s += bars.sums[r];
     const double by = (double)kScale / (sqrt(s) + p.eps);
-#pragma unroll 2
-    for (int i = threadIdx.x; i < 2048 * kSlices; i += kSmallOrthoThreads) {
-      float v[8];
-      read(i, v);
-      uint32_t hi[4], lo[4];
+    const bool plain = by > 1e-30 && by < 1e30;            // fp32 holds the factor, and a value times it
+    const float by32 = (float)by;
+    auto times = [&](float v) { return plain ? v * by32 : (float)((double)v * by); };
+    // the planes take the place of the floats: a slice's are all read before the first is written
+#pragma unroll 1
+    for (int n = 0; n < kSlices; ++n) {
+      unsigned char* const slice = sm + S::kX + n * 2 * kSmallPlane;
+      uint4 hi[8], lo[8];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) split_planes2((float)((double)v[2 * j] * by), (float)((double)v[2 * j + 1] * by), hi[j], lo[j]);
-      const int r = kTall ? i & 127 : i / (16 * kSlices), piece = kTall ? i >> 7 : i % (16 * kSlices);
-      unsigned char* const x = sm + S::kX + (piece >> 4) * 2 * kSmallPlane + plane_offset(r, piece & 15);
-      *reinterpret_cast<uint4*>(x) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-      *reinterpret_cast<uint4*>(x + kSmallPlane) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      for (int i = 0; i < 8; ++i) {
+        const int at = threadIdx.x + kSmallOrthoThreads * i, r = at >> 4, c = 8 * (at & 15);
+        const float4 u = *reinterpret_cast<const float4*>(slice + float_offset(r, c)), v = *reinterpret_cast<const float4*>(slice + float_offset(r, c + 4));
+        split_planes2(times(u.x), times(u.y), hi[i].x, lo[i].x), split_planes2(times(u.z), times(u.w), hi[i].y, lo[i].y);
+        split_planes2(times(v.x), times(v.y), hi[i].z, lo[i].z), split_planes2(times(v.z), times(v.w), hi[i].w, lo[i].w);
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int at = threadIdx.x + kSmallOrthoThreads * i, x = plane_offset(at >> 4, at & 15);
+        *reinterpret_cast<uint4*>(slice + x) = hi[i];
+        *reinterpret_cast<uint4*>(slice + kSmallPlane + x) = lo[i];
+      }
     }
 
     // ---- the steps ---------------------------------------------------------------------------------------------------
-    constexpr uint32_t idesc_kk = umma_idesc_f16(128, 128), idesc_kn = umma_idesc_f16(128, 128, false, true);
-    constexpr uint64_t kLo = kSmallPlane >> 4, kPanel = kSmallPlane >> 5;
     uint32_t parity = 0;
-    // Accumulators: leading ones at columns 0, 128 and 384, the rest at 256.
-    auto product = [&](auto issue) {
-      tc_fence_before();
-      asm volatile("fence.proxy.async;\n" ::: "memory");
-      __syncthreads();
-      if (warp == 0) {
-        tc_fence_after();
-        asm volatile("fence.proxy.async;\n" ::: "memory");
-        if (elect_lane()) {
-          issue();
-          umma_commit(&bars.done);
+    float sum[64];                // of this thread's row, columns 64 half ..
+    const uint32_t lanes = tmem + ((uint32_t)(32 * q) << 16) + 64 * half;
+    const int row = 32 * q + lane;
+    // Where a wait gives up the work goes on, on values that the flag has declared void: the barriers of the cluster want everybody.
+    auto product = [&](bool third) {
+      meet();
+      // the leading accumulators are added up while the other products run
+      mbar_wait(&bars.lead, parity, 1u);
+      __syncwarp();
+      tc_fence_after();
+#pragma unroll
+      for (int c = 0; c < 64; c += 32) {
+        uint32_t a[32], b[32];
+        tmem_ld32(lanes + c, a);
+        tmem_ld32(lanes + 128 + c, b);
+        tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 32; ++j) sum[c + j] = __uint_as_float(a[j]) + __uint_as_float(b[j]);
+        if (third) {
+          tmem_ld32(lanes + 384 + c, a);
+          tmem_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) sum[c + j] += __uint_as_float(a[j]);
         }
-        __syncwarp();
       }
-      // where the wait gives up the work goes on, on values that the flag has declared void: the barriers of the cluster want everybody
-      mbar_wait(&bars.done, parity, 1u);
+      mbar_wait(&bars.done, parity, 2u);
       __syncwarp();
       parity ^= 1;
       tc_fence_after();
-    };
-    const uint32_t lanes = tmem + ((uint32_t)(32 * q) << 16) + 64 * half;
-    const int row = 32 * q + lane;
-    // 32 columns of the sums of all accumulators, from column 64 half + c on
-    auto sums = [&](int c, bool third, float (&v)[32]) {
-      uint32_t a[32];
-      tmem_ld32(lanes + 256 + c, a);
-      tmem_wait_ld();
 #pragma unroll
-      for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(a[j]) * (1.f / 2048.f);
-      for (int k = 0; k < (third ? 3 : 2); ++k) {
-        tmem_ld32(lanes + (k == 2 ? 384 : 128 * k) + c, a);
+      for (int c = 0; c < 64; c += 32) {
+        uint32_t a[32];
+        tmem_ld32(lanes + 256 + c, a);
         tmem_wait_ld();
 #pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] += __uint_as_float(a[j]);
+        for (int j = 0; j < 32; ++j) sum[c + j] = fmaf(__uint_as_float(a[j]), 1.f / 2048.f, sum[c + j]);
       }
     };
-    // planes of 32 values of this thread's row, from column 64 half + c on
-    auto put = [&](unsigned char* to, int c, const float (&v)[32]) {
+    // planes of `by` times the sums
+    auto put = [&](unsigned char* to, float by) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+      for (int k = 0; k < 8; ++k) {
         uint32_t hi[4], lo[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) split_planes2(v[8 * k + 2 * j], v[8 * k + 2 * j + 1], hi[j], lo[j]);
-        unsigned char* const x = to + plane_offset(row, 8 * half + c / 8 + k);
+        for (int j = 0; j < 4; ++j) split_planes2(by * sum[8 * k + 2 * j], by * sum[8 * k + 2 * j + 1], hi[j], lo[j]);
+        unsigned char* const x = to + plane_offset(row, 8 * half + k);
         *reinterpret_cast<uint4*>(x) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
         *reinterpret_cast<uint4*>(x + kSmallPlane) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
       }
     };
-    unsigned char* const gram = sm + S::kA;
+    auto put_floats = [&](unsigned char* to, float by) {
+#pragma unroll
+      for (int k = 0; k < 16; ++k)
+        *reinterpret_cast<float4*>(to + float_offset(row, 64 * half + 4 * k)) = make_float4(by * sum[4 * k], by * sum[4 * k + 1], by * sum[4 * k + 2], by * sum[4 * k + 3]);
+    };
+    if (p.ctas > 1) cluster_arrive();
     for (int step = 0; step < p.steps; ++step) {
       // A
-      product([&] {
-#pragma unroll
-        for (int n = 0; n < 2 * kSlices; ++n) {            // panels of 64 k
-          const uint64_t x = umma_desc_sw128(smem_u32(sm + S::kX + (n >> 1) * 2 * kSmallPlane)) + (n & 1) * kPanel;
-          const uint32_t lead = tmem + (n == 2 ? 384 : 128 * (n & 1));
-#pragma unroll
-          for (int ks = 0; ks < 4; ++ks) {
-            umma_bf16(lead, x + 2 * ks, x + 2 * ks, idesc_kk, (ks > 0 || n == 3) ? 1u : 0u);
-            umma_bf16(tmem + 256, x + 2 * ks, x + kLo + 2 * ks, idesc_kk, (n | ks) ? 1u : 0u);
-            umma_bf16(tmem + 256, x + kLo + 2 * ks, x + 2 * ks, idesc_kk, 1u);
-          }
-        }
-      });
+      product(kSlices == 2);
       if (p.ctas == 1) {
-#pragma unroll 1
-        for (int c = 0; c < 64; c += 32) {
-          float v[32];
-          sums(c, kSlices == 2, v);
-#pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] *= 1.f / kScale;
-          put(gram, c, v);
-        }
+        put(gram, 1.f / kScale);
       } else {
-        // this CTA's part in fp32, where A will be: 16-byte pieces exchanged by row
-#pragma unroll 1
-        for (int c = 0; c < 64; c += 32) {
-          float v[32];
-          sums(c, kSlices == 2, v);
+        if (p.ctas == 2) {
+          // each sends its whole part to the other, and both add up
+          cluster_wait();                                  // the other does not multiply by what lies there any more
+          const uint32_t there = map_to_rank(smem_u32(gram), rank ^ 1);
 #pragma unroll
-          for (int k = 0; k < 8; ++k)
-            *reinterpret_cast<float4*>(gram + row * 512 + (((16 * half + c / 4 + k) ^ (row & 31)) << 4)) = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
-        }
-        tc_cluster_sync();
-        const int share = 128 / p.ctas, groups = share * 16 / kSmallOrthoThreads;      // 4, 2 or 1 of eight columns a thread
-        uint4 hi[4], lo[4];
+          for (int k = 0; k < 16; ++k)
+            asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};\n" ::"r"(there + float_offset(row, 64 * half + 4 * k)), "f"(sum[4 * k]), "f"(sum[4 * k + 1]),
+                         "f"(sum[4 * k + 2]), "f"(sum[4 * k + 3])
+                         : "memory");
+          tc_cluster_sync();
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (i < groups) {
-            const int at = threadIdx.x + kSmallOrthoThreads * i, r = rank * share + (at >> 4), piece = at & 15;
-            float v[8] = {};
-            for (int k = 0; k < p.ctas; ++k) {
-#pragma unroll
-              for (int j = 0; j < 2; ++j) {
-                float4 x;
-                asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];\n"
-                             : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w)
-                             : "r"(map_to_rank(smem_u32(gram + r * 512 + (((2 * piece + j) ^ (r & 31)) << 4)), k))
-                             : "memory");
-                v[4 * j] += x.x, v[4 * j + 1] += x.y, v[4 * j + 2] += x.z, v[4 * j + 3] += x.w;
-              }
-            }
-            constexpr float f = 1.f / kScale;
-            split_planes2(f * v[0], f * v[1], hi[i].x, lo[i].x), split_planes2(f * v[2], f * v[3], hi[i].y, lo[i].y);
-            split_planes2(f * v[4], f * v[5], hi[i].z, lo[i].z), split_planes2(f * v[6], f * v[7], hi[i].w, lo[i].w);
+          for (int k = 0; k < 16; ++k) {
+            const float4 x = *reinterpret_cast<const float4*>(gram + float_offset(row, 64 * half + 4 * k));
+            sum[4 * k] += x.x, sum[4 * k + 1] += x.y, sum[4 * k + 2] += x.z, sum[4 * k + 3] += x.w;
           }
-        }
-        tc_cluster_sync();                                 // all parts are read
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (i < groups) {
-            const int at = threadIdx.x + kSmallOrthoThreads * i, r = rank * share + (at >> 4), piece = at & 15;
-            const uint32_t to = smem_u32(gram + plane_offset(r, piece));
-            for (int k = 0; k < p.ctas; ++k) {
-              const uint32_t there = map_to_rank(to, k);
-              asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(there), "r"(hi[i].x), "r"(hi[i].y), "r"(hi[i].z), "r"(hi[i].w) : "memory");
-              asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(there + kSmallPlane), "r"(lo[i].x), "r"(lo[i].y), "r"(lo[i].z), "r"(lo[i].w) : "memory");
-            }
-          }
-        }
-        asm volatile("fence.proxy.async;\n" ::: "memory");
-        tc_cluster_sync();
+          asm volatile("bar.sync 1, %0;\n" ::"n"(kSmallOrthoThreads) : "memory");
+          put(gram, 1.f / kScale);
+        } else if (p.ctas == 4) exchange_gram<4>(gram, rank, row, half, sum);
+        else exchange_gram<8>(gram, rank, row, half, sum);
       }
 
       // the polynomial, in the place of A
       const float a = p.abc[3 * step], b = p.abc[3 * step + 1], c2 = p.abc[3 * step + 2] / kScale;
-      product([&] {
-        const uint64_t x = umma_desc_sw128(smem_u32(gram));
+      product(false);
 #pragma unroll
-        for (int ks = 0; ks < 8; ++ks) {
-          const uint64_t y = x + (ks >> 2) * kPanel + 2 * (ks & 3);
-          umma_bf16(tmem + 128 * (ks >> 2), y, y, idesc_kk, (ks & 3) ? 1u : 0u);
-          umma_bf16(tmem + 256, y, y + kLo, idesc_kk, ks ? 1u : 0u);
-          umma_bf16(tmem + 256, y + kLo, y, idesc_kk, 1u);
+      for (int k = 0; k < 8; ++k) {
+        const unsigned char* const x = gram + plane_offset(row, 8 * half + k);
+        const uint4 h = *reinterpret_cast<const uint4*>(x), l = *reinterpret_cast<const uint4*>(x + kSmallPlane);
+        const uint32_t hs[4] = {h.x, h.y, h.z, h.w}, ls[4] = {l.x, l.y, l.z, l.w};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const float2 xh = unpack_f16x2(hs[w]), xl = unpack_f16x2(ls[w]);
+          const int j = 8 * k + 2 * w;
+          sum[j] = fmaf(c2, sum[j], b * fmaf(xl.x, 1.f / 2048.f, xh.x));
+          sum[j + 1] = fmaf(c2, sum[j + 1], b * fmaf(xl.y, 1.f / 2048.f, xh.y));
         }
-      });
-#pragma unroll 1
-      for (int c = 0; c < 64; c += 32) {
-        float v[32];
-        sums(c, false, v);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const unsigned char* const x = gram + plane_offset(row, 8 * half + c / 8 + k);
-          const uint4 h = *reinterpret_cast<const uint4*>(x), l = *reinterpret_cast<const uint4*>(x + kSmallPlane);
-          const uint32_t hs[4] = {h.x, h.y, h.z, h.w}, ls[4] = {l.x, l.y, l.z, l.w};
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const float2 xh = unpack_f16x2(hs[w]), xl = unpack_f16x2(ls[w]);
-            const int j = 8 * k + 2 * w, col = 64 * half + c + j;
-            v[j] = fmaf(c2, v[j], b * fmaf(xl.x, 1.f / 2048.f, xh.x)) + (row == col ? a * kScale : 0.f);
-            v[j + 1] = fmaf(c2, v[j + 1], b * fmaf(xl.y, 1.f / 2048.f, xh.y)) + (row == col + 1 ? a * kScale : 0.f);
-          }
-        }
-        put(gram, c, v);
       }
+      // the diagonal crosses half of the warps, in 32 of their columns
+      if (q == 2 * half) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) sum[j] += lane == j ? a * kScale : 0.f;
+      } else if (q == 2 * half + 1) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) sum[32 + j] += lane == j ? a * kScale : 0.f;
+      }
+      put(gram, 1.f);
 
       // X, a slice at a time
       const bool last = step == p.steps - 1;
 #pragma unroll 1
       for (int n = 0; n < kSlices; ++n) {
         unsigned char* const slice = sm + S::kX + n * 2 * kSmallPlane;
-        product([&] {
-          const uint64_t y = umma_desc_sw128(smem_u32(gram)), x = umma_desc_mn_sw128(smem_u32(slice), kSmallPlane / 2, 1024);
+        product(false);
+        if (last) put_floats(slice, 1.f / (kScale * kScale));
+        else put(slice, 1.f / kScale);
+      }
+      if (p.ctas > 1 && !last) cluster_arrive();           // this CTA has multiplied by the polynomial; waited for before its place is written
+    }
+
+    // ---- the result, along the rows of the matrix ----------------------------------------------------------------------
+    __syncthreads();
+    char* const out = (char*)p.out + matrix * p.stride * size;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < across * lines; i += kSmallOrthoThreads) {
+      const int line = i / across, at = (i - line * across) * unit;
+      if (line >= last_line || at >= end) continue;
+      float v[8];
+      auto place = [&](int j) {
+        const int r = kTall ? at + j : line, c = kTall ? line : at + j;
+        return sm + S::kX + (c >> 7) * 2 * kSmallPlane + float_offset(r, c & 127);
+      };
 #pragma unroll
-          for (int ks = 0; ks < 8; ++ks) {
-            const uint64_t u = y + (ks >> 2) * kPanel + 2 * (ks & 3), w = x + 128 * ks;
-            umma_bf16(tmem + 128 * (ks >> 2), u, w, idesc_kn, (ks & 3) ? 1u : 0u);
-            umma_bf16(tmem + 256, u, w + kLo, idesc_kn, ks ? 1u : 0u);
-            umma_bf16(tmem + 256, u + kLo, w, idesc_kn, 1u);
-          }
-        });
-#pragma unroll 1
-        for (int c = 0; c < 64; c += 32) {
-          float v[32];
-          sums(c, false, v);
-          if (!last) {
+      for (int j = 0; j < 8; j += 4) {
+        if (j >= unit) break;
+        if (unit == 1) {
+          v[0] = *reinterpret_cast<const float*>(place(0));
+        } else if (kTall) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] *= 1.f / kScale;
-            put(slice, c, v);
-          } else if (row < p.side) {
-            T* const out = (T*)p.out + matrix * p.stride;
-            const int col0 = first + 128 * n + 64 * half + c;
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (col0 + j < p.length) out[kTall ? (int64_t)(col0 + j) * p.ld + row : (int64_t)row * p.ld + col0 + j] = (T)(v[j] * (1.f / (kScale * kScale)));
-          }
+          for (int w = 0; w < 4; ++w) v[j + w] = *reinterpret_cast<const float*>(place(j + w));
+        } else {
+          const float4 x = *reinterpret_cast<const float4*>(place(j));
+          v[j] = x.x, v[j + 1] = x.y, v[j + 2] = x.z, v[j + 3] = x.w;
         }
+      }
+      char* const to = out + (from + (int64_t)line * p.ld + at) * size;
+      if (unit == 1) {
+        if (p.type == PX_F32) *(float*)to = v[0];
+        else if (p.type == PX_F16) *(__half*)to = __float2half_rn(v[0]);
+        else *(bf16*)to = __float2bfloat16_rn(v[0]);
+      } else if (p.type == PX_F32) {
+        *reinterpret_cast<float4*>(to) = make_float4(v[0], v[1], v[2], v[3]);
+      } else if (p.type == PX_F16) {
+        *reinterpret_cast<uint4*>(to) = make_uint4(pack_f16x2_inf(v[0], v[1]), pack_f16x2_inf(v[2], v[3]), pack_f16x2_inf(v[4], v[5]), pack_f16x2_inf(v[6], v[7]));
+      } else {
+        *reinterpret_cast<uint4*>(to) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
       }
     }
   }
@@ -335,11 +497,11 @@ __global__ void __launch_bounds__(kSmallOrthoThreads, 1) small_ortho_kernel(cons
   }
 }
 
-template <typename T, int kSlices, bool kTall>
+template <int kSlices, bool kTall>
 static bool launch_small_ortho(const SmallOrtho& p, int64_t batch, cudaStream_t st) {
   typedef SmallOrthoShape<kSlices> S;
   static SmemLimit limit;
-  if (!limit.set(small_ortho_kernel<T, kSlices, kTall>, S::kSmem)) return false;
+  if (!limit.set(small_ortho_kernel<kSlices, kTall>, S::kSmem)) return false;
   cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
@@ -347,12 +509,12 @@ static bool launch_small_ortho(const SmallOrtho& p, int64_t batch, cudaStream_t 
   at[1].val.clusterDim.x = p.ctas, at[1].val.clusterDim.y = 1, at[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(batch * p.ctas));
-  cfg.blockDim = dim3(kSmallOrthoThreads);
+  cfg.blockDim = dim3(kSmallOrthoThreads + 32);
   cfg.dynamicSmemBytes = S::kSmem;
   cfg.stream = st;
   cfg.attrs = at;
   cfg.numAttrs = p.ctas > 1 ? 2 : 1;
-  if (cudaLaunchKernelEx(&cfg, small_ortho_kernel<T, kSlices, kTall>, p) == cudaSuccess) return true;
+  if (cudaLaunchKernelEx(&cfg, small_ortho_kernel<kSlices, kTall>, p) == cudaSuccess) return true;
   cudaGetLastError();
   return false;
 }
@@ -365,10 +527,9 @@ static inline int small_ortho_ctas(int64_t batch, int64_t side, int64_t length, 
   *slices = one && (one == two || batch * one <= sm_count()) ? 1 : 2;
   return *slices == 1 ? one : two;
 }
-template <typename T>
 static bool launch_small_ortho(const SmallOrtho& p, int64_t batch, int slices, bool tall, cudaStream_t st) {
-  if (slices == 1) return tall ? launch_small_ortho<T, 1, true>(p, batch, st) : launch_small_ortho<T, 1, false>(p, batch, st);
-  return tall ? launch_small_ortho<T, 2, true>(p, batch, st) : launch_small_ortho<T, 2, false>(p, batch, st);
+  if (slices == 1) return tall ? launch_small_ortho<1, true>(p, batch, st) : launch_small_ortho<1, false>(p, batch, st);
+  return tall ? launch_small_ortho<2, true>(p, batch, st) : launch_small_ortho<2, false>(p, batch, st);
 }
 
 }  // namespace px
