@@ -22,22 +22,20 @@ constexpr int kOrthoEpiWarps = 8, kOrthoThreads = 64 + 32 * kOrthoEpiWarps;
 constexpr int kOrthoStgBytes = 4096;      // staged block of a warp
 
 // ---- norm and first iterate ------------------------------------------------------------------------------------------
-constexpr int kNormBlocks = 64;
+constexpr int kNormBlocks = 1024;      // of a matrix, at most
 template <typename T>
 __global__ void __launch_bounds__(256) ortho_norm_kernel(const T* __restrict__ g, double* __restrict__ sums, int64_t elements) {
   __shared__ double part[8];
   pdl_wait();
   const T* p = g + blockIdx.y * elements;
   double s0 = 0.0, s1 = 0.0;
-  int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int64_t step = (int64_t)gridDim.x * 256;
-  for (; i + step < elements; i += 2 * step) {
-    const double a = (double)(float)p[i], b = (double)(float)p[i + step];
-    s0 += a * a, s1 += b * b;
-  }
-  if (i < elements) {
-    const double a = (double)(float)p[i];
-    s0 += a * a;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < elements; i += 8 * step) {
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = i + j * step < elements ? (float)p[i + j * step] : 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) s0 = fma((double)v[j], (double)v[j], s0), s1 = fma((double)v[j + 1], (double)v[j + 1], s1);
   }
   s0 += s1;
 #pragma unroll
@@ -64,20 +62,24 @@ __global__ void __launch_bounds__(256) ortho_split_kernel(const T* __restrict__ 
   __shared__ double by;
   pdl_wait();
   const int64_t z = blockIdx.y;
-  if (threadIdx.x == 0) {
+  if (threadIdx.x < 32) {
     double s = 0.0;
-    for (int i = 0; i < parts; ++i) s += sums[z * parts + i];
-    by = (double)kPlaneScale / (sqrt(s) + eps);
+    for (int i = threadIdx.x; i < parts; i += 32) s += sums[z * parts + i];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (threadIdx.x == 0) by = (double)kPlaneScale / (sqrt(s) + eps);
   }
   __syncthreads();
   const double scale = by;
+  const bool plain = scale > 1e-30 && scale < 1e30;        // fp32 holds the factor, and a value times it
+  const float scale32 = (float)scale;
   const int64_t per = ld / 8, all = m * per;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
     const int64_t row = i / per, col = (i - row * per) * 8;
     const T* p = g + (z * m + row) * n + col;
     float v[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = col + j < n ? (float)((double)(float)p[j] * scale) : 0.f;
+    for (int j = 0; j < 8; ++j) v[j] = col + j < n ? (plain ? (float)p[j] * scale32 : (float)((double)(float)p[j] * scale)) : 0.f;
     uint4 hi, lo;
     split_planes2(v[0], v[1], hi.x, lo.x), split_planes2(v[2], v[3], hi.y, lo.y);
     split_planes2(v[4], v[5], hi.z, lo.z), split_planes2(v[6], v[7], hi.w, lo.w);
@@ -126,13 +128,26 @@ struct OrthoEnd {
   int rows, cols, ld;           // ld: of gram
   int type, symmetric, result;  // type: of the result, whichever product this is
 
+  // A plane of a block, which has a buffer of 2 KB; the one before may still be on its way out of the other.
   __device__ __forceinline__ void store(unsigned char* stg, int lane, int x, int y, int z) const {
     asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
     __syncwarp();
     if (lane == 0) {
-      tma_store_3d(&out, smem_u32(stg), x, y, 2 * z);
-      tma_store_3d(&out, smem_u32(stg) + 2048, x, y, 2 * z + 1);
+      tma_store_3d(&out, smem_u32(stg), x, y, z);
       tma_store_commit();
+    }
+  }
+  __device__ __forceinline__ void room(int lane) const {
+    if (lane == 0) tma_store_wait_read<1>();
+    __syncwarp();
+  }
+  // The planes of A at 32 columns from col on of a row.
+  __device__ __forceinline__ void fetch(uint4 (&h)[4], uint4 (&l)[4], int row, int col, int z) const {
+    const __half* p = gram + ((int64_t)2 * z * rows + row) * ld + col;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      h[k] = l[k] = make_uint4(0, 0, 0, 0);
+      if (row < rows && col + 8 * k < ld) h[k] = *reinterpret_cast<const uint4*>(p + 8 * k), l[k] = *reinterpret_cast<const uint4*>(p + (int64_t)rows * ld + 8 * k);
     }
   }
   // v: 32 columns from col on of row m0 + lane
@@ -141,32 +156,26 @@ struct OrthoEnd {
 #pragma unroll
     for (int j = 0; j < 32; ++j) v[j] *= factor;
     if (gram) {
-      const __half* p = gram + ((int64_t)2 * z * rows + row) * ld + col;
-      if (row < rows) {
+      uint4 h[4], l[4];
+      fetch(h, l, row, col, z);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          if (col + 8 * k < ld) {
-            const uint4 h = *reinterpret_cast<const uint4*>(p + 8 * k), l = *reinterpret_cast<const uint4*>(p + (int64_t)rows * ld + 8 * k);
-            const uint32_t hs[4] = {h.x, h.y, h.z, h.w}, ls[4] = {l.x, l.y, l.z, l.w};
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t hs[4] = {h[k].x, h[k].y, h[k].z, h[k].w}, ls[4] = {l[k].x, l[k].y, l[k].z, l[k].w};
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-              const float2 x = unpack_f16x2(hs[w]), y = unpack_f16x2(ls[w]);
-              v[8 * k + 2 * w] = fmaf(b, fmaf(y.x, 1.f / 2048.f, x.x), v[8 * k + 2 * w]);
-              v[8 * k + 2 * w + 1] = fmaf(b, fmaf(y.y, 1.f / 2048.f, x.y), v[8 * k + 2 * w + 1]);
-            }
-          }
+        for (int w = 0; w < 4; ++w) {
+          const float2 x = unpack_f16x2(hs[w]), y = unpack_f16x2(ls[w]);
+          v[8 * k + 2 * w] = fmaf(b, fmaf(y.x, 1.f / 2048.f, x.x), v[8 * k + 2 * w]);
+          v[8 * k + 2 * w + 1] = fmaf(b, fmaf(y.y, 1.f / 2048.f, x.y), v[8 * k + 2 * w + 1]);
         }
       }
-      const int diagonal = row - col;
-      if (diagonal >= 0 && diagonal < 32) {
+      if (m0 == col) {                       // blocks of 32 x 32: the diagonal is that of the block, or not in it
 #pragma unroll
-        for (int j = 0; j < 32; ++j)
-          if (j == diagonal) v[j] += a * kPlaneScale;
+        for (int j = 0; j < 32; ++j) v[j] += lane == j ? a * kPlaneScale : 0.f;
       }
     }
-    if (lane == 0) tma_store_wait_read<0>();
-    __syncwarp();
     if (result) {
+      if (lane == 0) tma_store_wait_read<0>();
+      __syncwarp();
       if (type == PX_F32) {
 #pragma unroll
         for (int p = 0; p < 8; ++p)
@@ -188,27 +197,27 @@ struct OrthoEnd {
       }
       return;
     }
-    uint32_t hi[16], lo[16];
+    uint32_t w[2][16];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) split_planes2(v[2 * j], v[2 * j + 1], hi[j], lo[j]);
+    for (int j = 0; j < 16; ++j) split_planes2(v[2 * j], v[2 * j + 1], w[0][j], w[1][j]);
 #pragma unroll
-    for (int p = 0; p < 4; ++p) {
-      const int at = lane * 64 + ((p ^ (lane >> 1 & 3)) << 4);
-      *reinterpret_cast<uint4*>(stg + at) = make_uint4(hi[4 * p], hi[4 * p + 1], hi[4 * p + 2], hi[4 * p + 3]);
-      *reinterpret_cast<uint4*>(stg + 2048 + at) = make_uint4(lo[4 * p], lo[4 * p + 1], lo[4 * p + 2], lo[4 * p + 3]);
+    for (int p = 0; p < 2; ++p) {
+      room(lane);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        *reinterpret_cast<uint4*>(stg + 2048 * p + lane * 64 + ((k ^ (lane >> 1 & 3)) << 4)) = make_uint4(w[p][4 * k], w[p][4 * k + 1], w[p][4 * k + 2], w[p][4 * k + 3]);
+      store(stg + 2048 * p, lane, col, m0, 2 * z + p);
     }
-    store(stg, lane, col, m0, z);
     if (twice) {
-      if (lane == 0) tma_store_wait_read<0>();
-      __syncwarp();
-      // lane = column of the transposed block
 #pragma unroll
-      for (int j = 0; j < 32; ++j) {
-        const int at = j * 64 + (((lane >> 3) ^ (j >> 1 & 3)) << 4) + 2 * (lane & 7);
-        *reinterpret_cast<uint16_t*>(stg + at) = (uint16_t)(hi[j / 2] >> (16 * (j & 1)));
-        *reinterpret_cast<uint16_t*>(stg + 2048 + at) = (uint16_t)(lo[j / 2] >> (16 * (j & 1)));
+      for (int p = 0; p < 2; ++p) {
+        room(lane);
+        // lane = column of the transposed block
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          *reinterpret_cast<uint16_t*>(stg + 2048 * p + j * 64 + (((lane >> 3) ^ (j >> 1 & 3)) << 4) + 2 * (lane & 7)) = (uint16_t)(w[p][j / 2] >> (16 * (j & 1)));
+        store(stg + 2048 * p, lane, m0, col, 2 * z + p);
       }
-      store(stg, lane, m0, col, z);
     }
   }
 };
@@ -274,13 +283,14 @@ plane_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     for (int tile = first_tile; tile < tiles.total && ok; tile += tile_step) {
       const GemmTile t = gemm_tile(tiles, tile);
       const int m0 = t.mt * S::kSide + (int)rank * 128, n0 = t.nt * S::kSide + (int)rank * 128;
+      const bool same = end.symmetric && t.mt == t.nt;      // rows against themselves: one operand is fetched
       for (int kt = 0; kt < t.nk && ok; ++kt, ++it) {
         const int s = it % kStages;
         ok = mbar_wait_warp(&bars.empty[s], ((it / kStages) & 1) ^ 1, 1u);
         if (!ok) break;
         if (elect_lane()) {
           const uint32_t sa = smem_u32(ring + s * S::kStageBytes);
-          if (rank == 0) mbar_expect_tx(&bars.full[s], S::kCtas * S::kStageBytes);
+          if (rank == 0) mbar_expect_tx(&bars.full[s], S::kCtas * (same ? S::kStageBytes / 2 : S::kStageBytes));
           const uint32_t bar = kPair ? map_to_rank(smem_u32(&bars.full[s]), 0) : 0;
           auto load = [&](uint32_t dst, const CUtensorMap* map, bool across, int from, int z) {
             for (int j = 0; j < (across ? 2 : 1); ++j) {
@@ -294,7 +304,7 @@ plane_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
 #pragma unroll
           for (int p = 0; p < 2; ++p) {
             load(sa + p * S::kPlaneBytes, &map_a, S::kAMn, m0, 2 * t.z + p);
-            load(sa + (2 + p) * S::kPlaneBytes, &map_b, S::kBMn, n0, 2 * t.z + p);
+            if (!same) load(sa + (2 + p) * S::kPlaneBytes, &map_b, S::kBMn, n0, 2 * t.z + p);
           }
         }
         __syncwarp();
@@ -317,7 +327,7 @@ plane_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
             if (!ok) break;
             tc_fence_after();
             if (elect_lane()) {
-              const uint32_t sa = smem_u32(ring + s * S::kStageBytes), sb = sa + 2 * S::kPlaneBytes + h * 8192;
+              const uint32_t sa = smem_u32(ring + s * S::kStageBytes), sb = sa + (end.symmetric && t.mt == t.nt ? 0 : 2 * S::kPlaneBytes) + h * 8192;
               const uint64_t da = S::kAMn ? umma_desc_mn_sw128(sa, 8192, 1024) : umma_desc_sw128(sa);
               const uint64_t db = S::kBMn ? umma_desc_mn_sw128(sb, 8192, 1024) : umma_desc_sw128(sb);
               constexpr uint64_t kLo = S::kPlaneBytes >> 4;
@@ -501,8 +511,12 @@ static int32_t ortho_product(const Planes& a, const Planes& b, int64_t batch, in
   GemmTiles t = {};
   t.batch = (int)batch, t.splits = 1, t.group = 8, t.symmetric = end.symmetric;
   t.nk = t.nk_split = (int)(ortho_up(k, kGemmK) / kGemmK);
-  const int64_t tm = ortho_up(m, 256) / 256, tn = ortho_up(n, 256) / 256;
-  if (batch * (end.symmetric ? tm * (tm + 1) / 2 : tm * tn) >= sm_count()) return launch_planes<PlaneShape<2, kAMn, kBMn>>(ma, mb, end, t, m, n, st);
+  // Cycles of both forms: the products of a stage take 768 a unit of 128 x 128, its 64 KB 1490 (44 bytes a cycle); a tile's epilogue some 6000 and 9000.
+  const auto cycles = [&](int64_t side, int64_t room, int64_t epilogue) {
+    const int64_t tm = ortho_up(m, side) / side, tn = ortho_up(n, side) / side, tiles = batch * (end.symmetric ? tm * (tm + 1) / 2 : tm * tn);
+    return (tiles + room - 1) / room * (t.nk * 1500 + epilogue);
+  };
+  if (cycles(256, sm_count() / 2, 9000) < cycles(128, sm_count(), 6000)) return launch_planes<PlaneShape<2, kAMn, kBMn>>(ma, mb, end, t, m, n, st);
   return launch_planes<PlaneShape<1, kAMn, kBMn>>(ma, mb, end, t, m, n, st);
 }
 
@@ -528,7 +542,8 @@ static OrthoPlan ortho_plan(int64_t batch, int64_t m, int64_t n) {
 }
 template <typename T>
 static bool ortho_first(const void* g, double* sums, uint4* planes, int64_t batch, int64_t m, int64_t n, int64_t ld, double eps, cudaStream_t st) {
-  const int parts = (int)std::min<int64_t>(kNormBlocks, (m * n + 4095) / 4096);
+  const int64_t blocks_each = std::max<int64_t>(8, 8 * sm_count() / batch);
+  const int parts = (int)std::min<int64_t>(std::min<int64_t>(kNormBlocks, blocks_each), (m * n + 2047) / 2048);
   if (!launch_pdl(ortho_norm_kernel<T>, dim3(parts, (unsigned)batch), 256, 0, st, (const T*)g, sums, m * n)) return false;
   const int64_t blocks = std::min<int64_t>((m * ld / 8 + 255) / 256, std::max<int64_t>(1, 8 * sm_count() / batch));
   return launch_pdl(ortho_split_kernel<T>, dim3((unsigned)blocks, (unsigned)batch), 256, 0, st, (const T*)g, (const double*)sums, planes, m, n, ld, parts, eps);
