@@ -21,6 +21,11 @@ constexpr float kPlaneScale = 1024.f;
 constexpr int kOrthoEpiWarps = 8, kOrthoThreads = 64 + 32 * kOrthoEpiWarps;
 constexpr int kOrthoStgBytes = 4096;      // staged block of a warp
 
+// An accumulator is cut after each 16 k, which takes half a step off a sum of positive terms on average, 5.8e-8 of it (2.3e-7 measured for a sum of squares of 128
+// and the product behind it), and the polynomial multiplies a common factor by up to 30 where singular values lie close together: what the
+// cuts of a growing sum over k, in accumulators of `chunk` times 64, take off on average is put back.  64 x 700 in fp32 is off by 4.5e-6 without, plain fp32 products give 1.8e-6.
+__host__ __device__ constexpr float uncut(int64_t k, int chunk) { return 1.f + 2.9e-8f * (float)(((k + 15) / 16 < 4 * chunk ? (k + 15) / 16 : 4 * chunk) + 1); }
+
 // ---- norm and first iterate ------------------------------------------------------------------------------------------
 constexpr int kNormBlocks = 1024;      // of a matrix, at most
 template <typename T>
@@ -467,21 +472,21 @@ PX_DEFINE_FAMILY_HOOKS(update)
 // ---- host ------------------------------------------------------------------------------------------------------------
 static int64_t ortho_up(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
 
-// planes [batch][2][rows][ld], of which `inner` columns count
+// planes [batch][2][rows][ld], of which `inner` columns count, with the maps of their copies: as an operand along k or across it, and on their way out
 struct Planes {
   __half* at;
-  int64_t rows, inner, ld;
+  CUtensorMap along, across, out;
+  bool set(__half* to, int64_t rows, int64_t inner, int64_t ld, int64_t batch) {
+    at = to;
+    return gemm_map(&along, true, at, inner, rows, 2 * batch, ld, rows * ld, kGemmM) && gemm_map(&across, true, at, inner, rows, 2 * batch, ld, rows * ld, kGemmK) &&
+           make_map_3d(&out, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, at, (uint64_t)inner, (uint64_t)rows, (uint64_t)(2 * batch), (uint64_t)ld * 2, (uint64_t)rows * ld * 2, 32, 32,
+                       CU_TENSOR_MAP_SWIZZLE_64B);
+  }
 };
-static bool operand_map(CUtensorMap* map, const Planes& p, int64_t batch, bool across) {
-  return gemm_map(map, true, p.at, p.inner, p.rows, 2 * batch, p.ld, p.rows * p.ld, across ? kGemmK : kGemmM);
-}
-static bool planes_out(CUtensorMap* map, const Planes& p, int64_t batch) {
-  return make_map_3d(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, p.at, (uint64_t)p.inner, (uint64_t)p.rows, (uint64_t)(2 * batch), (uint64_t)p.ld * 2, (uint64_t)p.rows * p.ld * 2, 32,
-                     32, CU_TENSOR_MAP_SWIZZLE_64B);
-}
 template <class S>
-static int32_t launch_planes(const CUtensorMap& ma, const CUtensorMap& mb, const OrthoEnd& end, GemmTiles t, int64_t m, int64_t n, cudaStream_t st) {
+static int32_t launch_planes(const CUtensorMap& ma, const CUtensorMap& mb, OrthoEnd end, GemmTiles t, int64_t m, int64_t n, int64_t k, cudaStream_t st) {
   const int chunk = end.type == PX_F32 ? 1 : end.type == PX_F16 ? 2 : 8;
+  end.factor *= uncut(k, chunk);
   t.tiles_m = (int)(ortho_up(m, S::kSide) / S::kSide), t.tiles_n = (int)(ortho_up(n, S::kSide) / S::kSide);
   const int64_t total = t.batch * (t.symmetric ? (int64_t)t.tiles_m * (t.tiles_m + 1) / 2 : (int64_t)t.tiles_m * t.tiles_n);
   if (total > 0x7fffffff) return PX_ERR_UNSUPPORTED;
@@ -506,8 +511,7 @@ static int32_t launch_planes(const CUtensorMap& ma, const CUtensorMap& mb, const
 }
 template <bool kAMn, bool kBMn>
 static int32_t ortho_product(const Planes& a, const Planes& b, int64_t batch, int64_t m, int64_t n, int64_t k, const OrthoEnd& end, cudaStream_t st) {
-  CUtensorMap ma, mb;
-  if (!operand_map(&ma, a, batch, kAMn) || !operand_map(&mb, b, batch, kBMn)) return PX_ERR_LAUNCH;
+  const CUtensorMap &ma = kAMn ? a.across : a.along, &mb = kBMn ? b.across : b.along;
   GemmTiles t = {};
   t.batch = (int)batch, t.splits = 1, t.group = 8, t.symmetric = end.symmetric;
   t.nk = t.nk_split = (int)(ortho_up(k, kGemmK) / kGemmK);
@@ -516,8 +520,8 @@ static int32_t ortho_product(const Planes& a, const Planes& b, int64_t batch, in
     const int64_t tm = ortho_up(m, side) / side, tn = ortho_up(n, side) / side, tiles = batch * (end.symmetric ? tm * (tm + 1) / 2 : tm * tn);
     return (tiles + room - 1) / room * (t.nk * 1500 + epilogue);
   };
-  if (cycles(256, sm_count() / 2, 9000) < cycles(128, sm_count(), 6000)) return launch_planes<PlaneShape<2, kAMn, kBMn>>(ma, mb, end, t, m, n, st);
-  return launch_planes<PlaneShape<1, kAMn, kBMn>>(ma, mb, end, t, m, n, st);
+  if (cycles(256, sm_count() / 2, 9000) < cycles(128, sm_count(), 6000)) return launch_planes<PlaneShape<2, kAMn, kBMn>>(ma, mb, end, t, m, n, k, st);
+  return launch_planes<PlaneShape<1, kAMn, kBMn>>(ma, mb, end, t, m, n, k, st);
 }
 
 struct OrthoPlan {
@@ -587,43 +591,40 @@ extern "C" int32_t px_orthogonalize(const void* g, void* out, int64_t batch, int
   char* const ws = (char*)workspace;
   const bool wide = m <= n;
   double* sums = (double*)(ws + p.sums);
-  Planes x = {(__half*)(ws + p.x[0]), m, n, p.ld}, next = {(__half*)(ws + p.x[1]), m, n, p.ld};
-  const Planes gram = {(__half*)(ws + p.gram), p.s, p.s, p.lds}, poly = {(__half*)(ws + p.poly), p.s, p.s, p.lds};
-  const bool ok = dtype == PX_F32    ? ortho_first<float>(g, sums, (uint4*)x.at, batch, m, n, p.ld, eps, st)
-                  : dtype == PX_BF16 ? ortho_first<bf16>(g, sums, (uint4*)x.at, batch, m, n, p.ld, eps, st)
-                                     : ortho_first<__half>(g, sums, (uint4*)x.at, batch, m, n, p.ld, eps, st);
+  Planes planes[2], gram, poly;
+  if (!planes[0].set((__half*)(ws + p.x[0]), m, n, p.ld, batch) || !planes[1].set((__half*)(ws + p.x[1]), m, n, p.ld, batch) ||
+      !gram.set((__half*)(ws + p.gram), p.s, p.s, p.lds, batch) || !poly.set((__half*)(ws + p.poly), p.s, p.s, p.lds, batch))
+    return PX_ERR_LAUNCH;
+  const bool ok = dtype == PX_F32    ? ortho_first<float>(g, sums, (uint4*)planes[0].at, batch, m, n, p.ld, eps, st)
+                  : dtype == PX_BF16 ? ortho_first<bf16>(g, sums, (uint4*)planes[0].at, batch, m, n, p.ld, eps, st)
+                                     : ortho_first<__half>(g, sums, (uint4*)planes[0].at, batch, m, n, p.ld, eps, st);
   if (!ok) return PX_ERR_LAUNCH;
   const int size = dtype == PX_F32 ? 4 : 2;
   const bool direct = n * size % 16 == 0 && ((uintptr_t)out & 15) == 0;      // what TMA can store
   for (int i = 0; i < steps; ++i) {
-    const float a = coefficients[3 * i], b = coefficients[3 * i + 1], c = coefficients[3 * i + 2];
+    const Planes &x = planes[i & 1], &next = planes[1 - (i & 1)];
     OrthoEnd e = {};
-    if (!planes_out(&e.out, gram, batch)) return PX_ERR_LAUNCH;
-    e.factor = 1.f / kPlaneScale, e.rows = e.cols = (int)p.s, e.ld = (int)p.lds, e.symmetric = 1, e.type = dtype;
+    e.out = gram.out, e.factor = 1.f / kPlaneScale, e.rows = e.cols = (int)p.s, e.ld = (int)p.lds, e.symmetric = 1, e.type = dtype;
     int32_t status = wide ? ortho_product<false, false>(x, x, batch, p.s, p.s, n, e, st) : ortho_product<true, true>(x, x, batch, p.s, p.s, m, e, st);
     if (status) return status;
-    if (!planes_out(&e.out, poly, batch)) return PX_ERR_LAUNCH;
-    e.gram = gram.at, e.factor = c / kPlaneScale, e.a = a, e.b = b;
+    e.out = poly.out, e.gram = gram.at, e.a = coefficients[3 * i], e.b = coefficients[3 * i + 1], e.factor = coefficients[3 * i + 2] / kPlaneScale;
     status = ortho_product<false, false>(gram, gram, batch, p.s, p.s, p.s, e, st);
     if (status) return status;
     e = {};
-    e.factor = 1.f / kPlaneScale, e.rows = (int)m, e.cols = (int)n, e.type = dtype;
+    e.out = next.out, e.factor = 1.f / kPlaneScale, e.rows = (int)m, e.cols = (int)n, e.type = dtype;
     if (i == steps - 1 && direct) {
       e.result = 1, e.factor = 1.f / (kPlaneScale * kPlaneScale);
       const CUtensorMapDataType type = dtype == PX_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : dtype == PX_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
       if (!make_map_3d(&e.out, type, out, (uint64_t)n, (uint64_t)m, (uint64_t)batch, (uint64_t)n * size, (uint64_t)m * n * size, 32, 32,
                        dtype == PX_F32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B))
         return PX_ERR_LAUNCH;
-    } else if (!planes_out(&e.out, next, batch)) {
-      return PX_ERR_LAUNCH;
     }
     status = wide ? ortho_product<false, true>(poly, x, batch, m, n, m, e, st) : ortho_product<false, false>(x, poly, batch, m, n, n, e, st);
     if (status) return status;
-    std::swap(x.at, next.at);
   }
   if (direct) return PX_OK;
-  const bool done = dtype == PX_F32    ? ortho_last<float>(x.at, out, batch, m, n, p.ld, st)
-                    : dtype == PX_BF16 ? ortho_last<bf16>(x.at, out, batch, m, n, p.ld, st)
-                                       : ortho_last<__half>(x.at, out, batch, m, n, p.ld, st);
+  const bool done = dtype == PX_F32    ? ortho_last<float>(planes[steps & 1].at, out, batch, m, n, p.ld, st)
+                    : dtype == PX_BF16 ? ortho_last<bf16>(planes[steps & 1].at, out, batch, m, n, p.ld, st)
+                                       : ortho_last<__half>(planes[steps & 1].at, out, batch, m, n, p.ld, st);
   return done ? PX_OK : PX_ERR_LAUNCH;
 }

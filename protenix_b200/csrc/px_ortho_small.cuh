@@ -6,8 +6,9 @@
 // 2 us a product with its epilogue, instead of a launch of 7 us each.
 //
 // A's parts of the CTAs are exchanged through distributed shared memory: each CTA adds up 128 / k rows from all k parts, in the order of their ranks, and
-// writes the planes of the sum to all of them.  Accumulators are as in plane_product_kernel: a fresh one for each 64 k (two slices: the last of four goes on
-// with the second), joined in registers, and one for the products with a low plane.
+// writes the planes of the sum to all of them.  Accumulators are as in plane_product_kernel: a fresh one for each 64 k, joined in
+// registers (two slices: the second's take the place of the first's, which the other warps read while the low planes are multiplied), and one for the products
+// with a low plane.
 #pragma once
 #include "px_pair.cuh"
 #include "px_rowpipe.cuh"
@@ -36,7 +37,8 @@ struct SmallOrthoShape {
   static_assert(kSmem <= 232448, "shared memory budget");
 };
 struct SmallOrthoBarriers {
-  uint64_t lead, done;          // the leading products; all of them
+  uint64_t lead, done;          // the leading products (of the first slice); all of them
+  uint64_t drained;             // the first have been read
   uint32_t tmem_base, stop[8];
   double part[8], sums[8];      // of this CTA's warps; of the cluster's CTAs
 };
@@ -69,9 +71,9 @@ __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;\n" ::: "memory"); }
 
 // A from its parts in the kCtas CTAs of a cluster: every row goes to the CTA that adds it up (row / kShare), which writes the planes of the sum to all of
-// them.  `sum`: this thread's row, columns 64 half ..; the parts lie where A will be, part k from row k kShare on.
+// them.  `sum`: this thread's row, columns 64 half ..; f: what A is multiplied by; the parts lie where A will be, part k from row k kShare on.
 template <int kCtas>
-__device__ __forceinline__ void exchange_gram(unsigned char* gram, int rank, int row, int half, const float (&sum)[64]) {
+__device__ __forceinline__ void exchange_gram(unsigned char* gram, int rank, int row, int half, const float (&sum)[64], float f) {
   constexpr int kShare = 128 / kCtas, kGroups = 8 / kCtas;      // rows of a CTA; eight columns each of a thread
   cluster_wait();                                               // nobody multiplies by what lies there any more
   {
@@ -97,7 +99,6 @@ __device__ __forceinline__ void exchange_gram(unsigned char* gram, int rank, int
         v[4 * j] += x.x, v[4 * j + 1] += x.y, v[4 * j + 2] += x.z, v[4 * j + 3] += x.w;
       }
     }
-    constexpr float f = 1.f / kPlaneScale;
     split_planes2(f * v[0], f * v[1], hi[i].x, lo[i].x), split_planes2(f * v[2], f * v[3], hi[i].y, lo[i].y);
     split_planes2(f * v[4], f * v[5], hi[i].z, lo[i].z), split_planes2(f * v[6], f * v[7], hi[i].w, lo[i].w);
   }
@@ -121,6 +122,7 @@ template <int kSlices, bool kTall>
 __global__ void __launch_bounds__(kSmallOrthoThreads + 32, 1) small_ortho_kernel(const __grid_constant__ SmallOrtho p) {
   typedef SmallOrthoShape<kSlices> S;
   constexpr float kScale = kPlaneScale;
+  const float uncut_gram = uncut(p.length, 1), uncut_side = uncut(p.side, 1);
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* sm = smem_aligned(smem_raw);
   SmallOrthoBarriers& bars = *reinterpret_cast<SmallOrthoBarriers*>(sm + S::kBars);
@@ -132,6 +134,7 @@ __global__ void __launch_bounds__(kSmallOrthoThreads + 32, 1) small_ortho_kernel
   if (threadIdx.x == 0) {
     mbar_init(&bars.lead, 1);
     mbar_init(&bars.done, 1);
+    mbar_init(&bars.drained, 8);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
   if (warp == 0) {
@@ -165,7 +168,7 @@ __global__ void __launch_bounds__(kSmallOrthoThreads + 32, 1) small_ortho_kernel
   if (skip) {
     // nothing
   } else if (warp == 8) {
-    // ---- products: accumulators of the leading ones at columns 0, 128 and 384, of the rest at 256 ------------------------
+    // ---- products: accumulators of the leading ones at columns 0 and 128, of the rest at 256 ------------------------
     const uint64_t gram_at = umma_desc_sw128(smem_u32(gram));
     auto issue = [&](auto leading, auto rest) {
       meet();
@@ -203,26 +206,40 @@ __global__ void __launch_bounds__(kSmallOrthoThreads + 32, 1) small_ortho_kernel
     for (int n = 0; n < kSlices; ++n) __syncthreads();
     if (p.ctas > 1) cluster_arrive();
     for (int step = 0; step < p.steps; ++step) {
-      issue(
-          [&] {
+      auto lead = [&](int slice) {
 #pragma unroll
-            for (int n = 0; n < 2 * kSlices; ++n) {
-              const uint64_t x = slice_at(n);
+        for (int n = 0; n < 2; ++n) {
+          const uint64_t x = slice_at(2 * slice + n);
 #pragma unroll
-              for (int ks = 0; ks < 4; ++ks) umma_bf16(tmem + (n == 2 ? 384 : 128 * (n & 1)), x + 2 * ks, x + 2 * ks, idesc_kk, (ks > 0 || n == 3) ? 1u : 0u);
-            }
-          },
-          [&] {
+          for (int ks = 0; ks < 4; ++ks) umma_bf16(tmem + 128 * n, x + 2 * ks, x + 2 * ks, idesc_kk, ks ? 1u : 0u);
+        }
+      };
+      meet();
+      tc_fence_after();
+      if (elect_lane()) {
+        lead(0);
+        umma_commit(&bars.lead);
 #pragma unroll
-            for (int n = 0; n < 2 * kSlices; ++n) {
-              const uint64_t x = slice_at(n);
+        for (int n = 0; n < 2 * kSlices; ++n) {
+          const uint64_t x = slice_at(n);
 #pragma unroll
-              for (int ks = 0; ks < 4; ++ks) {
-                umma_bf16(tmem + 256, x + 2 * ks, x + kLo + 2 * ks, idesc_kk, (n | ks) ? 1u : 0u);
-                umma_bf16(tmem + 256, x + kLo + 2 * ks, x + 2 * ks, idesc_kk, 1u);
-              }
-            }
-          });
+          for (int ks = 0; ks < 4; ++ks) {
+            umma_bf16(tmem + 256, x + 2 * ks, x + kLo + 2 * ks, idesc_kk, (n | ks) ? 1u : 0u);
+            umma_bf16(tmem + 256, x + kLo + 2 * ks, x + 2 * ks, idesc_kk, 1u);
+          }
+        }
+        if (kSlices == 1) umma_commit(&bars.done);
+      }
+      __syncwarp();
+      if (kSlices == 2) {
+        mbar_wait_warp(&bars.drained, step & 1, 4u);
+        tc_fence_after();
+        if (elect_lane()) {
+          lead(1);
+          umma_commit(&bars.done);
+        }
+        __syncwarp();
+      }
       if (p.ctas > 1) {
         cluster_wait();
         for (int k = 0; k < (p.ctas == 2 ? 1 : 3); ++k) tc_cluster_sync();
@@ -330,12 +347,7 @@ __global__ void __launch_bounds__(kSmallOrthoThreads + 32, 1) small_ortho_kernel
     const uint32_t lanes = tmem + ((uint32_t)(32 * q) << 16) + 64 * half;
     const int row = 32 * q + lane;
     // Where a wait gives up the work goes on, on values that the flag has declared void: the barriers of the cluster want everybody.
-    auto product = [&](bool third) {
-      meet();
-      // the leading accumulators are added up while the other products run
-      mbar_wait(&bars.lead, parity, 1u);
-      __syncwarp();
-      tc_fence_after();
+    auto leading = [&](bool first) {
 #pragma unroll
       for (int c = 0; c < 64; c += 32) {
         uint32_t a[32], b[32];
@@ -343,18 +355,29 @@ __global__ void __launch_bounds__(kSmallOrthoThreads + 32, 1) small_ortho_kernel
         tmem_ld32(lanes + 128 + c, b);
         tmem_wait_ld();
 #pragma unroll
-        for (int j = 0; j < 32; ++j) sum[c + j] = __uint_as_float(a[j]) + __uint_as_float(b[j]);
-        if (third) {
-          tmem_ld32(lanes + 384 + c, a);
-          tmem_wait_ld();
-#pragma unroll
-          for (int j = 0; j < 32; ++j) sum[c + j] += __uint_as_float(a[j]);
+        for (int j = 0; j < 32; ++j) {
+          const float s = __uint_as_float(a[j]) + __uint_as_float(b[j]);
+          sum[c + j] = first ? s : sum[c + j] + s;
         }
+      }
+    };
+    auto product = [&](bool two) {
+      meet();
+      // the leading accumulators are added up while the other products run
+      mbar_wait(&bars.lead, parity, 1u);
+      __syncwarp();
+      tc_fence_after();
+      leading(true);
+      if (two) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.drained);
       }
       mbar_wait(&bars.done, parity, 2u);
       __syncwarp();
       parity ^= 1;
       tc_fence_after();
+      if (two) leading(false);
 #pragma unroll
       for (int c = 0; c < 64; c += 32) {
         uint32_t a[32];
@@ -386,7 +409,7 @@ __global__ void __launch_bounds__(kSmallOrthoThreads + 32, 1) small_ortho_kernel
       // A
       product(kSlices == 2);
       if (p.ctas == 1) {
-        put(gram, 1.f / kScale);
+        put(gram, uncut_gram / kScale);
       } else {
         if (p.ctas == 2) {
           // each sends its whole part to the other, and both add up
@@ -404,13 +427,13 @@ __global__ void __launch_bounds__(kSmallOrthoThreads + 32, 1) small_ortho_kernel
             sum[4 * k] += x.x, sum[4 * k + 1] += x.y, sum[4 * k + 2] += x.z, sum[4 * k + 3] += x.w;
           }
           asm volatile("bar.sync 1, %0;\n" ::"n"(kSmallOrthoThreads) : "memory");
-          put(gram, 1.f / kScale);
-        } else if (p.ctas == 4) exchange_gram<4>(gram, rank, row, half, sum);
-        else exchange_gram<8>(gram, rank, row, half, sum);
+          put(gram, uncut_gram / kScale);
+        } else if (p.ctas == 4) exchange_gram<4>(gram, rank, row, half, sum, uncut_gram / kScale);
+        else exchange_gram<8>(gram, rank, row, half, sum, uncut_gram / kScale);
       }
 
       // the polynomial, in the place of A
-      const float a = p.abc[3 * step], b = p.abc[3 * step + 1], c2 = p.abc[3 * step + 2] / kScale;
+      const float a = p.abc[3 * step], b = p.abc[3 * step + 1], c2 = p.abc[3 * step + 2] * (uncut_side / kScale);
       product(false);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
@@ -441,8 +464,8 @@ __global__ void __launch_bounds__(kSmallOrthoThreads + 32, 1) small_ortho_kernel
       for (int n = 0; n < kSlices; ++n) {
         unsigned char* const slice = sm + S::kX + n * 2 * kSmallPlane;
         product(false);
-        if (last) put_floats(slice, 1.f / (kScale * kScale));
-        else put(slice, 1.f / kScale);
+        if (last) put_floats(slice, uncut_side / (kScale * kScale));
+        else put(slice, uncut_side / kScale);
       }
       if (p.ctas > 1 && !last) cluster_arrive();           // this CTA has multiplied by the polynomial; waited for before its place is written
     }

@@ -452,11 +452,12 @@ struct RotaryCall {
   std::vector<int64_t> sections;
   double base;
   bool interleaved, per_axis, inverse;
+  int64_t batch, row, axis;      // strides of the positions
 };
 typedef std::pair<Tensor, Tensor> TwoTensors;
 
 Tensor channels_fitted(const Tensor& t) { return t.size(3) <= 1 || t.stride(3) == 1 ? t : t.contiguous(); }
-// q and k [B, H, N, D] turned (k undefined: q alone); positions [B, N, A], int64, any strides.
+// q and k [B, H, N, D] turned (k undefined: q alone); positions int64, by the strides of the call.
 TwoTensors rotary_launch(const Tensor& q_, const Tensor& k_, const Tensor& positions, const RotaryCall& c) {
   c10::cuda::CUDAGuard guard(q_.device());
   const Tensor q = channels_fitted(q_), k = k_.defined() ? channels_fitted(k_) : k_;
@@ -464,7 +465,7 @@ TwoTensors rotary_launch(const Tensor& q_, const Tensor& k_, const Tensor& posit
   const std::vector<int32_t> sections(c.sections.begin(), c.sections.end());
   px_rotary r = {};
   r.positions = (const int64_t*)positions.data_ptr();
-  r.position_batch = positions.stride(0), r.position_row = positions.stride(1), r.position_axis = positions.stride(2);
+  r.position_batch = c.batch, r.position_row = c.row, r.position_axis = c.axis;
   r.batch = q.size(0), r.heads = q.size(1), r.kv_heads = k.defined() ? k.size(1) : 0, r.n = q.size(2), r.d = q.size(3);
   r.sections = sections.data(), r.axes = (int32_t)sections.size(), r.base = c.base;
   r.interleaved = c.interleaved, r.per_axis = c.per_axis, r.dtype = dtype_code(q, "q");
@@ -478,11 +479,13 @@ TwoTensors rotary_apply(const Tensor& q, const Tensor& k, const Tensor& position
 
 struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const OptTensor& k, const Tensor& positions,
-                                                std::vector<int64_t> sections, double base, bool interleaved, bool per_axis, bool inverse) {
+                                                std::vector<int64_t> sections, double base, bool interleaved, bool per_axis, bool inverse,
+                                                std::vector<int64_t> strides) {
     ctx->set_materialize_grads(false);
-    const auto out = rotary_launch(q, has(k) ? *k : Tensor(), positions, {sections, base, interleaved, per_axis, inverse});
+    const auto out = rotary_launch(q, has(k) ? *k : Tensor(), positions, {sections, base, interleaved, per_axis, inverse, strides[0], strides[1], strides[2]});
     ctx->save_for_backward({positions});
     ctx->saved_data["sections"] = c10::List<int64_t>(c10::ArrayRef<int64_t>(sections));
+    ctx->saved_data["strides"] = c10::List<int64_t>(c10::ArrayRef<int64_t>(strides));
     ctx->saved_data["base"] = base;
     ctx->saved_data["how"] = (int64_t)interleaved | (int64_t)per_axis << 1 | (int64_t)inverse << 2;
     ctx->saved_data["f"] = (int64_t)q.requires_grad() | (int64_t)(has(k) && k->requires_grad()) << 1;
@@ -492,7 +495,8 @@ struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     const int64_t f = ctx->saved_data["f"].toInt(), how = ctx->saved_data["how"].toInt();
     const Tensor positions = ctx->get_saved_variables()[0];
-    const RotaryCall c = {ctx->saved_data["sections"].toIntVector(), ctx->saved_data["base"].toDouble(), (how & 1) != 0, (how & 2) != 0, (how & 4) == 0};
+    const auto st = ctx->saved_data["strides"].toIntVector();
+    const RotaryCall c = {ctx->saved_data["sections"].toIntVector(), ctx->saved_data["base"].toDouble(), (how & 1) != 0, (how & 2) != 0, (how & 4) == 0, st[0], st[1], st[2]};
     const Tensor gq = f & 1 ? grads[0] : Tensor(), gk = f & 2 && grads.size() > 1 ? grads[1] : Tensor();
     Tensor dq, dk;      // the operator again, by the negated angles: differentiable like it
     if (gq.defined() && gk.defined())
@@ -501,13 +505,14 @@ struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
       dq = rotary_apply(gq, Tensor(), positions, c).first;
     else if (gk.defined())
       dk = rotary_apply(gk, Tensor(), positions, c).first;
-    return {dq, dk, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    return {dq, dk, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
 
 TwoTensors rotary_apply(const Tensor& q, const Tensor& k, const Tensor& positions, const RotaryCall& c) {
   if (at::GradMode::is_enabled() && (q.requires_grad() || (k.defined() && k.requires_grad()))) {
-    const auto out = RotaryFunction::apply(q, k.defined() ? OptTensor(k) : OptTensor(), positions, c.sections, c.base, c.interleaved, c.per_axis, c.inverse);
+    const auto out = RotaryFunction::apply(q, k.defined() ? OptTensor(k) : OptTensor(), positions, c.sections, c.base, c.interleaved, c.per_axis, c.inverse,
+                                           std::vector<int64_t>{c.batch, c.row, c.axis});
     return {out[0], k.defined() ? out[1] : Tensor()};
   }
   return rotary_launch(q, k, positions, c);
@@ -548,9 +553,17 @@ py::object rotary_embedding(const Tensor& q, const OptTensor& k, const Tensor& p
   const int64_t heads = q.size(-3) + (has(k) ? k->size(-3) : 0);
   if (batch > 65535 || heads > 65536 || n > (1 << 30)) fail("at most 65535 samples, 65536 heads and 2^30 rows");
   c10::cuda::CUDAGuard guard(q.device());
-  const Tensor p = positions.detach().to(at::kLong).expand(want).reshape({batch, n, axes});
+  Tensor p = positions.scalar_type() == at::kLong ? positions : positions.to(at::kLong);
+  RotaryCall call = {sections, base, interleaved, per_axis, false, 0, p.stride(-2), p.stride(-1)};
+  if (p.size(-2) != n) call.row = 0;      // one place for all rows
+  if (p.dim() == 3 && q.dim() == 4 && p.size(0) == batch) {
+    call.batch = p.stride(0);
+  } else if (p.numel() != p.size(-2) * axes) {      // samples of their own, over several axes or broadcast along some
+    p = p.expand(want).reshape({batch, n, axes});
+    call.batch = p.stride(0), call.row = p.stride(1), call.axis = p.stride(2);
+  }
   const auto four = [&](const Tensor& t) { return t.dim() == 4 ? t : t.reshape({batch, t.size(-3), n, d}); };
-  const auto out = rotary_apply(four(q), has(k) ? four(*k) : Tensor(), p, {sections, base, interleaved, per_axis, false});
+  const auto out = rotary_apply(four(q), has(k) ? four(*k) : Tensor(), p, call);
   const auto back = [&](const Tensor& t, const Tensor& like) { return like.dim() == 4 ? t : t.reshape(like.sizes()); };
   const py::object first = py::cast(back(out.first, q));
   return has(k) ? py::object(py::make_tuple(first, back(out.second, *k))) : first;

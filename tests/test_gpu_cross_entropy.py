@@ -60,7 +60,8 @@ def _grad_close(name, got, want, dtype, c):
     assert bool(((got.detach().double() - want[name]).abs() <= bound * (1 + 1e-9) + 1e-30).all()), name
 
 
-SIZES = [(1, 8, 2), (5, 8, 3), (128, 64, 64), (129, 72, 65), (384, 384, 32), (300, 128, 257), (31, 1024, 1000), (257, 264, 256), (1000, 136, 4999), (4096, 256, 8192)]
+SIZES = [(1, 8, 2), (5, 8, 3), (128, 64, 64), (129, 72, 65), (384, 384, 32), (300, 128, 257), (31, 1024, 1000), (257, 264, 256), (1000, 136, 4999), (4096, 256, 8192),
+         (1000, 128, 128), (257, 128, 127), (300, 64, 128), (130, 120, 129), (40000, 128, 64), (41001, 96, 100), (20000, 264, 70)]
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP16])
@@ -231,6 +232,55 @@ def test_a_gradient_that_is_not_finite_stays_in_its_row():
     ox, _ = torch.autograd.grad(px.linear_cross_entropy(x, w, t, reduction="none"), (x, w), torch.ones(150, device="cuda"))
     keep = torch.arange(150, device="cuda") != 7
     assert torch.equal(dx[keep], ox[keep]) and not bool(torch.isfinite(dx[7]).any()) and not bool(torch.isfinite(dw).any())
+
+
+@pytest.mark.parametrize("rows,c,v", [(150, 64, 90), (150, 136, 300)])
+@pytest.mark.parametrize("size", [math.inf, math.nan, 0.0])
+def test_a_scale_that_is_not_finite(rows, c, v, size):
+    """Rows that are ignored have gradients of zero all the same."""
+    x, w, _, t = _inputs(rows, c, v, BF16)
+    dx, dw = torch.autograd.grad(px.linear_cross_entropy(x, w, t) * size, (x, w))
+    assert not bool(dx[t == -100].any())
+    assert not bool(dx.any() or dw.any()) if size == 0.0 else not bool(torch.isfinite(dx[t != -100]).any())
+
+
+@pytest.mark.parametrize("c,v", [(128, 16), (1024, 200)])
+def test_offsets_beyond_32_bits(c, v):
+    """Rows that begin beyond 2^31 elements of x, and beyond 2^32 bytes of its gradient."""
+    rows = 2 ** 31 // c + 300
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.zeros(rows, c, dtype=BF16, device="cuda")
+    at = torch.cat([torch.arange(200), torch.arange(rows - 200, rows)]).cuda()
+    x[at] = torch.randn(400, c, generator=g, device="cuda").to(BF16)
+    x.requires_grad_()
+    w = (torch.randn(v, c, generator=g, device="cuda") / math.sqrt(c)).to(BF16).requires_grad_()
+    t = torch.full((rows,), -100, device="cuda")
+    t[at] = torch.randint(0, v, (400,), generator=g, device="cuda")
+    each = px.linear_cross_entropy(x, w, t, reduction="none")
+    dx, dw = torch.autograd.grad(each.sum(), (x, w))
+    want = _formula(x.detach()[at], w, None, t[at], 0.0, torch.ones(400, device="cuda"))
+    _loss_close(each.detach()[at], want, c)
+    want_dx = {k: want[k] for k in ("dx", "dx_abs", "dx_most")}
+    _grad_close("dx", dx[at], want_dx, BF16, c)
+    _grad_close("dw", dw, want, BF16, c)
+    assert int(torch.count_nonzero(dx)) == int(torch.count_nonzero(dx[at]))
+
+
+def test_two_streams_at_once():
+    sets = [_inputs(700, 128, v, BF16, BF16, seed=v) for v in (64, 3000)]
+    call = lambda s: [(loss := px.linear_cross_entropy(s[0], s[1], s[3], bias=s[2])).detach(), *torch.autograd.grad(loss, s[:3])]  # noqa: E731
+    want = [call(s) for s in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i, (s, st) in enumerate(zip(sets, streams)):
+            with torch.cuda.stream(st):
+                got[i].append(call(s))
+    torch.cuda.synchronize()
+    for w, many in zip(want, got):
+        for g in many:
+            assert all(torch.equal(a, b) for a, b in zip(w, g))
 
 
 def test_layouts():

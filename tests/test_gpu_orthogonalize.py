@@ -37,7 +37,8 @@ def _close(got, want, noise=4e-6):
     assert bool((off <= (u + noise) * size + 2.0 ** -25 * math.sqrt(want.shape[-1] * want.shape[-2])).all()), float((off / size).max())
 
 
-SIZES = [(1, 1, 1), (3, 1, 5), (2, 7, 3), (5, 16, 16), (2, 33, 130), (2, 130, 33), (7, 128, 128), (3, 129, 127), (4, 512, 128), (4, 128, 512), (2, 384, 1536), (1, 1000, 257), (1, 301, 299)]
+SIZES = [(1, 1, 1), (3, 1, 5), (2, 7, 3), (5, 16, 16), (2, 33, 130), (2, 130, 33), (7, 128, 128), (3, 129, 127), (4, 512, 128), (4, 128, 512), (2, 384, 1536), (1, 1000, 257), (1, 301, 299),
+         (2, 100, 500), (1, 128, 1000), (1, 1001, 90), (1, 90, 2000), (1, 2048, 64), (60, 128, 500), (60, 510, 100), (100, 256, 128), (40, 1000, 33), (150, 100, 100)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -50,7 +51,11 @@ def test_against_64_bits(batch, m, n, dtype):
     assert got.dtype == dtype and got.shape == g.shape and torch.equal(g, keep)
     _close(got, _iterated(g))
     assert torch.equal(got, px.orthogonalize(g))
-    assert torch.equal(got[batch - 1], px.orthogonalize(g[batch - 1]))      # a matrix does not depend on what lies beside it
+    # a matrix does not depend on what lies beside it; on how many there are it does in its last bits (the work is split otherwise)
+    others = torch.randn_like(g)
+    others[batch - 1] = g[batch - 1]
+    assert torch.equal(got[batch - 1], px.orthogonalize(others)[batch - 1])
+    _close(px.orthogonalize(g[batch - 1])[None], _iterated(g[batch - 1:]))
 
 
 @pytest.mark.parametrize("m,n", [(2048, 2048), (3000, 700), (1100, 4100)])
@@ -119,6 +124,28 @@ def test_layouts_and_empty():
     assert torch.equal(px.orthogonalize(half), px.orthogonalize(g.half()))
     for shape in ((0, 4, 5), (2, 0, 5), (2, 4, 0)):
         assert px.orthogonalize(torch.zeros(shape, device="cuda")).shape == shape
+
+
+def test_two_streams_at_once():
+    sets = [torch.randn(s, device="cuda") for s in ((40, 128, 512), (3, 300, 400), (20, 100, 90))]
+    want = [px.orthogonalize(g) for g in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    got = [[], [], []]
+    for _ in range(10):
+        for i, (g, st) in enumerate(zip(sets, streams)):
+            with torch.cuda.stream(st):
+                got[i].append(px.orthogonalize(g))
+    torch.cuda.synchronize()
+    ops.device_error_flags()
+    for w, many in zip(want, got):
+        assert all(torch.equal(w, g) for g in many)
+
+
+def test_many_steps():
+    """More than the one launch of small matrices holds."""
+    g = torch.randn(2, 30, 50, device="cuda")
+    _close(px.orthogonalize(g, steps=40, coefficients=(1.5, -0.5, 0.0)), _iterated(g, 40, (1.5, -0.5, 0.0)), 2e-5)
 
 
 def test_streams_and_capture():

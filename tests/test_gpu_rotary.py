@@ -98,6 +98,16 @@ def test_layouts(dtype):
     assert got[0].transpose(1, 2).is_contiguous()      # like q: heads inside the rows
     one = q[:1].expand(3, h, n, d)
     assert torch.equal(px.rotary_embedding(one, None, at, sections=(10, 6)), want[0][:1].expand(3, h, n, d))
+    here = torch.full((1, 2), 7, device="cuda")      # one place for all rows
+    assert torch.equal(px.rotary_embedding(q, None, here, sections=(10, 6)), px.rotary_embedding(q, None, here.expand(n, 2).contiguous(), sections=(10, 6)))
+    each = torch.randint(0, 50, (3, n, 2), device="cuda")
+    want3 = px.rotary_embedding(q, k, each, sections=(10, 6))
+    for i in range(3):
+        assert torch.equal(px.rotary_embedding(q[i:i + 1], None, each[i], sections=(10, 6)), want3[0][i:i + 1])
+    six = px.rotary_embedding(q[None].expand(2, 3, h, n, d), None, each.expand(2, 3, n, 2), sections=(10, 6))
+    assert torch.equal(six, want3[0].expand(2, 3, h, n, d))
+    mixed = px.rotary_embedding(q[None].expand(2, 3, h, n, d), None, each[:1, :, :].unsqueeze(1).expand(1, 1, n, 2), sections=(10, 6))
+    assert torch.equal(mixed[1], px.rotary_embedding(q, None, each[0], sections=(10, 6)))
     five = px.rotary_embedding(q[None], k[None], at.expand(1, 3, n, 2), sections=(10, 6))
     assert five[0].shape == (1, 3, h, n, d) and torch.equal(five[0][0], want[0]) and torch.equal(five[1][0], want[1])
     three = px.rotary_embedding(q[0], k[0], at, sections=(10, 6))
