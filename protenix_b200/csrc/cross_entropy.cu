@@ -29,6 +29,7 @@ struct EpiStats {
   float* hit;               // [rows]: logit of the row's class
   uint32_t* arrivals;
   int rows, classes;
+  float uncut;
   static constexpr bool kMeets = true, kStores = false;
   __device__ __forceinline__ void begin() const { *arrivals = 0; }
 
@@ -58,8 +59,7 @@ struct EpiStats {
       tmem_wait_ld();
       if (c + 32 == kCols || left <= 32) release();
       float v[32];
-#pragma unroll
-      for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+      logits_of(r, uncut, v);
       if (!at.plain) add_bias(v, e.own + c);
       if (part_sum) {
         float a[4] = {};
@@ -290,7 +290,7 @@ struct EpiLogitGrad {
   float* part_bias;         // [32-row groups][classes of the piece]: sums of dl, or NULL
   int64_t ignore;
   int rows, classes, first, all_classes;      // first: the piece's first class
-  float smooth;
+  float smooth, uncut;
   int f16;
   static constexpr bool kMeets = false, kStores = true;
   __device__ __forceinline__ void begin() const {}
@@ -337,8 +337,7 @@ struct EpiLogitGrad {
       tmem_wait_ld();
       if (c + 32 == kCols || left <= 32) release();
       float v[32];
-#pragma unroll
-      for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+      logits_of(r, uncut, v);
       if (!at.plain) add_bias(v, e.own + c);
       const int own = mine - c;
       if (__any_sync(0xffffffffu, own >= 0 && own < 32)) {
@@ -623,7 +622,7 @@ static bool small_args(SmallArgs* a, const px_head& h) {
     return false;
   a->dx = a->x;
   a->target = h.target, a->bias = {h.bias, h.bias_dtype}, a->ignore = h.ignore, a->rows = (int)h.rows, a->classes = (int)h.classes;
-  a->panels = (int)(up(h.c, 64) / 64), a->tiles = (int)(up(h.rows, 128) / 128), a->f16 = f16, a->smooth = h.smoothing;
+  a->panels = (int)(up(h.c, 64) / 64), a->tiles = (int)(up(h.rows, 128) / 128), a->f16 = f16, a->smooth = h.smoothing, a->uncut = uncut_logits(h.c);
   a->idesc_logits = umma_idesc_16(128, vp, f16, f16);
   a->idesc_dx = umma_idesc_16(128, 64 * a->panels, f16, f16, false, true);
   a->idesc_dw = umma_idesc_16(128, vp, f16, f16, true, true);
@@ -687,7 +686,7 @@ extern "C" int32_t px_head_loss_fwd(const px_head* head, float* norm, float* los
   at += up((h.rows + 31) / 32 * 16, 1024);
   float2* part = (float2*)at;
   at += up(c.t.tiles_n * h.rows * 8, 1024);
-  EpiStats epi = {h.target, {h.bias, h.bias_dtype}, part, h.smoothing > 0.f ? (float*)at : nullptr, hit, arrivals, (int)h.rows, (int)h.classes};
+  EpiStats epi = {h.target, {h.bias, h.bias_dtype}, part, h.smoothing > 0.f ? (float*)at : nullptr, hit, arrivals, (int)h.rows, (int)h.classes, uncut_logits(h.c)};
   if (const int32_t status = launch_logits(h, 0, h.classes, c, epi, st)) return status;
   JoinArgs j = {part, epi.part_sum, hit, h.target, (float2*)norm, losses, total, inverse, sums, arrivals, h.ignore, (int)h.rows, (int)h.classes, c.t.tiles_n, mean, h.smoothing};
   return launch_pdl(loss_join_kernel, dim3((unsigned)((h.rows + 31) / 32)), 32 * kJoinWarps, 0, st, j) ? PX_OK : PX_ERR_LAUNCH;
@@ -750,7 +749,7 @@ extern "C" int32_t px_head_loss_bwd(const px_head* head, const float* norm, cons
     if (!dl_map(&el.out, type16(f16), dl, vc, h.rows, p.ld)) return PX_ERR_LAUNCH;
     el.target = h.target, el.bias = {h.bias ? (const char*)h.bias + first * bias_size : nullptr, h.bias_dtype}, el.norm = (const float2*)norm, el.grad = each ? grad : nullptr, el.scale = scale;
     el.part_bias = dbias ? part_bias : nullptr, el.ignore = h.ignore, el.rows = (int)h.rows, el.classes = (int)vc, el.first = (int)first;
-    el.all_classes = (int)h.classes, el.smooth = h.smoothing, el.f16 = f16;
+    el.all_classes = (int)h.classes, el.smooth = h.smoothing, el.uncut = uncut_logits(h.c), el.f16 = f16;
     if (const int32_t status = launch_logits(h, first, vc, p.logits, el, st)) return status;
     if (dbias && !launch_pdl(loss_bias_kernel, dim3((unsigned)((vc + 31) / 32)), 512, 0, st, (const float*)part_bias, (void*)((char*)dbias + first * bias_size), (int)h.bias_dtype, (const LossScale*)scale, (int)vc,
                              (int)((h.rows + 31) / 32)))

@@ -32,7 +32,7 @@ struct SmallArgs {
   float* part_b;                                          // backward: [8 CTAs][kVp], or NULL
   int64_t ignore;
   int rows, classes, panels, tiles, f16, want_dx;
-  float smooth;
+  float smooth, uncut;
   uint32_t idesc_logits, idesc_dx, idesc_dw;
 };
 
@@ -206,8 +206,7 @@ __global__ void __launch_bounds__(SmallShape<kBackward, kVp>::kThreads, 1) small
             if (lane == 0) mbar_arrive(&bars.logit_empty[b]);
           }
           float v[32];
-#pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+          logits_of(r, a.uncut, v);
           add_bias(v, bias + c);
           if (a.smooth > 0.f) {
 #pragma unroll
@@ -260,8 +259,7 @@ __global__ void __launch_bounds__(SmallShape<kBackward, kVp>::kThreads, 1) small
             if (lane == 0) mbar_arrive(&bars.logit_empty[b]);
           }
           float v[32];
-#pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+          logits_of(r, a.uncut, v);
           add_bias(v, bias + c);
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] = fmaf(over, fast_exp2(fmaf(v[j], kLog2e, ref)), mine == c + j ? less_hit : -less);
