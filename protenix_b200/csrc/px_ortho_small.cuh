@@ -541,14 +541,27 @@ static bool launch_small_ortho(const SmallOrtho& p, int64_t batch, cudaStream_t 
   cudaGetLastError();
   return false;
 }
-// CTAs of a matrix: one slice each where the matrices then have room at once, otherwise two; 0: not this kernel.
+// CTAs of a matrix, 0: not this kernel.  us of five steps, bf16, with one slice a CTA | two: one CTA 37 to 42 | 59 to 61, two 60 to 64 | 83 to 86, four 67 to 74 | 94,
+// eight 72 to 79 | 92 to 100, as often as the clusters take turns (148, 74, 32 or 14 fit); by products of their own launches, 33 to 40 matrices of 128 x 512 (four CTAs
+// in two turns: 134) 131 to 140, 16 of 128 x 1024 (eight in two turns: 144) 149, 37 (four with two slices, in two turns: 176) 167.
 static inline int small_ortho_ctas(int64_t batch, int64_t side, int64_t length, int steps, int* slices) {
   if (side > 128 || steps > kSmallSteps) return 0;
-  const auto fit = [](int64_t n) { return n <= 1 ? 1 : n <= 2 ? 2 : n <= 4 ? 4 : n <= 8 ? 8 : 0; };
-  const int one = fit((length + 127) / 128), two = fit((length + 255) / 256);
-  if (!two) return 0;
-  *slices = one && (one == two || batch * one <= sm_count()) ? 1 : 2;
-  return *slices == 1 ? one : two;
+  static constexpr int kFit[4] = {148, 74, 32, 14}, kUs[4][2] = {{40, 60}, {62, 84}, {72, 95}, {78, 98}};
+  const int64_t sms = sm_count();
+  // launches of 6 us, and 0.7 us for each 64 k of the rounds of tiles
+  const auto rounds = [&](int64_t tiles) { return (batch * tiles + sms - 1) / sms; };
+  const int64_t along = (length + 127) / 128, sk = (side + 63) / 64;
+  double best = 90.0 + 3.5 * (double)(rounds(1) * ((length + 63) / 64 + sk) + rounds(along) * sk);
+  int ctas = 0;
+  for (int i = 0; i < 4; ++i) {
+    for (int n = 1; n <= 2; ++n) {
+      if (along > (n << i) || (i && along <= (n << (i - 1)))) continue;      // too few, or more than are needed
+      const int64_t fit = std::max<int64_t>(1, kFit[i] * sms / 148);
+      const double us = (double)((batch + fit - 1) / fit * kUs[i][n - 1]);
+      if (us < best) best = us, ctas = 1 << i, *slices = n;
+    }
+  }
+  return ctas;
 }
 static bool launch_small_ortho(const SmallOrtho& p, int64_t batch, int slices, bool tall, cudaStream_t st) {
   if (slices == 1) return tall ? launch_small_ortho<1, true>(p, batch, st) : launch_small_ortho<1, false>(p, batch, st);
