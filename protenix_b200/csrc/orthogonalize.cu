@@ -105,23 +105,25 @@ __global__ void __launch_bounds__(256) ortho_join_kernel(const __half* __restric
 
 // ---- the product -----------------------------------------------------------------------------------------------------
 // D = A B^T of operands in two planes: D1 = hi hi, D2 = hi lo + lo hi, D = D1 + 2^-11 D2.  The tensor core truncates where it adds, which shortens a sum
-// of positive terms by 3e-8 a step of 16 k (384 x 1536 in fp32: 1.6e-5 off with one accumulator for all of K, plain fp32 products 3e-6 to 7e-6).  So D1
-// has a fresh accumulator for each `chunk` stages of 64 k, which the epilogue's warps add to their registers, rounding to nearest, while the next one
-// fills.  Of chunk = 1, 2, 4, 8 the results of eight 1024 x 1024 matrices are off by 1.6, 2.8, 5.1, 9.7e-6 in 614, 593, 581, 562 us, 4096 x 4096 takes 4540, 4110,
-// 3870, 3670: 1 where the result is fp32, 2 for fp16 and 8 for bf16, whose own rounding is 2e-4 and 1.7e-3.  D2, 2^-11 as large, is added up in tensor memory.  Tiles of 128 x 128, or 256 x 256 for a pair of CTAs in two units of 128 columns (64 of
-// each CTA's rows of B): tensor memory holds two accumulators of a unit and D2 of the tile.
+// of positive terms by some 5e-8 a step of 16 k (384 x 1536 in fp32: 1.6e-5 off with one accumulator for all of K, plain fp32 products 3e-6 to 7e-6).  So D1
+// gets a fresh accumulator for each `chunk` stages of 64 k, which the epilogue's warps add to their registers, rounding to nearest, while the stage's products
+// with a low plane run; D2, 2^-11 as large, is added up in tensor memory.  Of chunk = 1, 2, 4, 8 the results of eight 1024 x 1024 matrices are off by 0.9, 1.4, 2.5,
+// 4.7e-6 (plain fp32 products 3.1e-6) and take 708, 634, 582, 552 us: 1 where the result is fp32, 2 for fp16 and 8 for bf16, whose own rounding is 2e-4 and 1.7e-3.
+//
+// Tiles of 128 x 128, or 256 x 256 for a pair of CTAs.  What bounds them is shared memory: a product of 128 x 128 x 16 reads 8 KB in 64 cycles, as much as there is,
+// and 64 KB a stage come in besides (0.71 us a stage, 768 cycles of it products); those of 256 columns, which only a pair has, read 12 KB in 128.
 template <int kCtas_, bool kAMn_, bool kBMn_>
 struct PlaneShape {
-  static constexpr int kCtas = kCtas_, kUnits = kCtas, kSide = 128 * kCtas, kStages = 3;
+  static constexpr int kCtas = kCtas_, kSide = 128 * kCtas, kStages = 3, kCols = 64 * kCtas;      // kCols: of an epilogue warp
   static constexpr bool kAMn = kAMn_, kBMn = kBMn_;
   static constexpr int kPlaneBytes = kGemmM * kGemmK * 2, kStageBytes = 4 * kPlaneBytes;      // A hi, A lo, B hi, B lo: 128 rows each
   static constexpr int kStg = kStages * kStageBytes, kBars = kStg + kOrthoEpiWarps * kOrthoStgBytes;
   static constexpr size_t kSmem = kBars + 256 + 1024;
-  static constexpr uint32_t kIdesc = umma_idesc_f16(kGemmM * kCtas, 128, kAMn, kBMn);
+  static constexpr uint32_t kIdesc = umma_idesc_f16(kSide, kSide, kAMn, kBMn);
   static_assert(kSmem <= 232448, "shared memory budget");
 };
 struct PlaneBarriers {
-  uint64_t full[3], empty[3], part_full[2], part_empty[2], rest_full, rest_empty;
+  uint64_t full[3], empty[3], part_full, part_empty, rest_full, rest_empty;
   uint32_t tmem_base, peer_stop;
 };
 
@@ -231,8 +233,8 @@ template <class S>
 __global__ void __launch_bounds__(kOrthoThreads, 1)
 plane_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ OrthoEnd end, const GemmTiles tiles, int chunk) {
   constexpr bool kPair = S::kCtas == 2;
-  constexpr int kStages = S::kStages, kUnits = S::kUnits;
-  constexpr uint32_t kCols = 512;      // two accumulators of 128 columns, D2 of 128 or 256
+  constexpr int kStages = S::kStages;
+  constexpr uint32_t kTmem = 2 * S::kSide;      // D1, D2
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* ring = smem_aligned(smem_raw);
   PlaneBarriers& bars = *reinterpret_cast<PlaneBarriers*>(ring + S::kBars);
@@ -247,20 +249,18 @@ plane_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
       mbar_init(&bars.full[s], 1);
       mbar_init(&bars.empty[s], 1);
     }
-    for (int b = 0; b < 2; ++b) {
-      mbar_init(&bars.part_full[b], 1);
-      mbar_init(&bars.part_empty[b], kOrthoEpiWarps * S::kCtas);
-    }
+    mbar_init(&bars.part_full, 1);
+    mbar_init(&bars.part_empty, kOrthoEpiWarps * S::kCtas);
     mbar_init(&bars.rest_full, 1);
     mbar_init(&bars.rest_empty, kOrthoEpiWarps * S::kCtas);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
   if (warp == 0) {
     if constexpr (kPair) {
-      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&bars.tmem_base)), "r"(kCols) : "memory");
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&bars.tmem_base)), "r"(kTmem) : "memory");
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
     } else {
-      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&bars.tmem_base)), "r"(kCols) : "memory");
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&bars.tmem_base)), "r"(kTmem) : "memory");
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
     }
   }
@@ -317,68 +317,55 @@ plane_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     }
   } else if (warp == 1) {
     if (rank == 0) {
-      uint32_t it = 0, unit = 0, count = 0;
+      uint32_t it = 0, part = 0, count = 0;
       bool ok = true;
       for (int tile = first_tile; tile < tiles.total && ok; tile += tile_step, ++count) {
         const GemmTile t = gemm_tile(tiles, tile);
         ok = mbar_wait_warp(&bars.rest_empty, (count & 1) ^ 1, 2u);
         for (int kt = 0; kt < t.nk && ok; ++kt, ++it) {
           const int s = it % kStages;
-          ok = mbar_wait_warp(&bars.full[s], (it / kStages) & 1, 4u);
           const bool begins = (kt & (chunk - 1)) == 0, ends = ((kt + 1) & (chunk - 1)) == 0 || kt == t.nk - 1;
-          for (int h = 0; h < kUnits && ok; ++h) {
-            const uint32_t at = unit + h, buf = at & 1;
-            if (begins) ok = mbar_wait_warp(&bars.part_empty[buf], ((at >> 1) & 1) ^ 1, 8u);
-            if (!ok) break;
-            tc_fence_after();
-            if (elect_lane()) {
-              const uint32_t sa = smem_u32(ring + s * S::kStageBytes), sb = sa + (end.symmetric && t.mt == t.nt ? 0 : 2 * S::kPlaneBytes) + h * 8192;
-              const uint64_t da = S::kAMn ? umma_desc_mn_sw128(sa, 8192, 1024) : umma_desc_sw128(sa);
-              const uint64_t db = S::kBMn ? umma_desc_mn_sw128(sb, 8192, 1024) : umma_desc_sw128(sb);
-              constexpr uint64_t kLo = S::kPlaneBytes >> 4;
-              auto mma = [&](uint32_t d, uint64_t a, uint64_t b, uint32_t more) {
-                if constexpr (kPair)
-                  umma_pair(d, a, b, S::kIdesc, more);
-                else
-                  umma_bf16(d, a, b, S::kIdesc, more);
-              };
-              const uint32_t d1 = tmem_base + 128 * buf, d2 = tmem_base + 256 + 128 * h;
-#pragma unroll
-              for (int ks = 0; ks < kGemmK / 16; ++ks) mma(d1, da + (S::kAMn ? 128 : 2) * ks, db + (S::kBMn ? 128 : 2) * ks, !begins || ks > 0);
-              if (!ends) {
-              } else if constexpr (kPair)
-                umma_commit_pair(&bars.part_full[buf]);
+          ok = mbar_wait_warp(&bars.full[s], (it / kStages) & 1, 4u) && (!begins || mbar_wait_warp(&bars.part_empty, (part & 1) ^ 1, 8u));
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_lane()) {
+            const uint32_t sa = smem_u32(ring + s * S::kStageBytes), sb = sa + (end.symmetric && t.mt == t.nt ? 0 : 2 * S::kPlaneBytes);
+            const uint64_t da = S::kAMn ? umma_desc_mn_sw128(sa, 8192, 1024) : umma_desc_sw128(sa);
+            const uint64_t db = S::kBMn ? umma_desc_mn_sw128(sb, 8192, 1024) : umma_desc_sw128(sb);
+            constexpr uint64_t kLo = S::kPlaneBytes >> 4;
+            auto mma = [&](uint32_t d, uint64_t a, uint64_t b, uint32_t more) {
+              if constexpr (kPair)
+                umma_pair(d, a, b, S::kIdesc, more);
               else
-                umma_commit(&bars.part_full[buf]);
+                umma_bf16(d, a, b, S::kIdesc, more);
+            };
+            auto commit = [&](uint64_t* bar) {
+              if constexpr (kPair)
+                umma_commit_pair(bar);
+              else
+                umma_commit(bar);
+            };
 #pragma unroll
-              for (int ks = 0; ks < kGemmK / 16; ++ks) {
-                const uint64_t a = da + (S::kAMn ? 128 : 2) * ks, b = db + (S::kBMn ? 128 : 2) * ks;
-                mma(d2, a, b + kLo, (kt | ks) ? 1u : 0u);
-                mma(d2, a + kLo, b, 1u);
-              }
-              if (h == kUnits - 1) {
-                if constexpr (kPair)
-                  umma_commit_pair(&bars.empty[s]);
-                else
-                  umma_commit(&bars.empty[s]);
-                if (kt == t.nk - 1) {
-                  if constexpr (kPair)
-                    umma_commit_pair(&bars.rest_full);
-                  else
-                    umma_commit(&bars.rest_full);
-                }
-              }
+            for (int ks = 0; ks < kGemmK / 16; ++ks) mma(tmem_base, da + (S::kAMn ? 128 : 2) * ks, db + (S::kBMn ? 128 : 2) * ks, !begins || ks > 0);
+            if (ends) commit(&bars.part_full);
+#pragma unroll
+            for (int ks = 0; ks < kGemmK / 16; ++ks) {
+              const uint64_t a = da + (S::kAMn ? 128 : 2) * ks, b = db + (S::kBMn ? 128 : 2) * ks;
+              mma(tmem_base + S::kSide, a, b + kLo, (kt | ks) ? 1u : 0u);
+              mma(tmem_base + S::kSide, a + kLo, b, 1u);
             }
-            __syncwarp();
+            commit(&bars.empty[s]);
+            if (kt == t.nk - 1) commit(&bars.rest_full);
           }
-          if (ends) unit += kUnits;
+          __syncwarp();
+          if (ends) ++part;
         }
       }
     }
   } else {
     const int q = warp & 3, half = (warp - 2) >> 2;
     unsigned char* const stg = ring + S::kStg + (warp - 2) * kOrthoStgBytes;
-    const uint32_t lanes = tmem_base + ((uint32_t)(32 * q) << 16) + 64 * half;
+    const uint32_t lanes = tmem_base + ((uint32_t)(32 * q) << 16) + S::kCols * half;
     auto arrive = [&](uint64_t* bar) {
       tc_fence_before();
       __syncwarp();
@@ -389,58 +376,44 @@ plane_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
           mbar_arrive(bar);
       }
     };
-    uint32_t unit = 0, count = 0;
+    uint32_t part = 0, count = 0;
     bool ok = true;
     for (int tile = first_tile; tile < tiles.total && ok; tile += tile_step, ++count) {
       const GemmTile t = gemm_tile(tiles, tile);
-      float sum[kUnits][64];
+      float sum[S::kCols];
 #pragma unroll
-      for (int h = 0; h < kUnits; ++h)
+      for (int j = 0; j < S::kCols; ++j) sum[j] = 0.f;
+      for (int kt = 0; kt < t.nk && ok; kt += chunk, ++part) {
+        ok = mbar_wait_warp(&bars.part_full, part & 1, 16u);
+        if (!ok) break;
+        tc_fence_after();
 #pragma unroll
-        for (int j = 0; j < 64; ++j) sum[h][j] = 0.f;
-      for (int kt = 0; kt < t.nk && ok; kt += chunk) {
+        for (int c = 0; c < S::kCols; c += 32) {
+          uint32_t r[32];
+          tmem_ld32(lanes + c, r);
+          tmem_wait_ld();
 #pragma unroll
-        for (int h = 0; h < kUnits; ++h, ++unit) {
-          const uint32_t buf = unit & 1;
-          ok = ok && mbar_wait_warp(&bars.part_full[buf], (unit >> 1) & 1, 16u);
-          if (!ok) break;
-          tc_fence_after();
-#pragma unroll
-          for (int c = 0; c < 64; c += 32) {
-            uint32_t r[32];
-            tmem_ld32(lanes + 128 * buf + c, r);
-            tmem_wait_ld();
-#pragma unroll
-            for (int j = 0; j < 32; j += 2) add2(sum[h][c + j], sum[h][c + j + 1], __uint_as_float(r[j]), __uint_as_float(r[j + 1]));
-          }
-          arrive(&bars.part_empty[buf]);
+          for (int j = 0; j < 32; j += 2) add2(sum[c + j], sum[c + j + 1], __uint_as_float(r[j]), __uint_as_float(r[j + 1]));
         }
+        arrive(&bars.part_empty);
       }
       ok = ok && mbar_wait_warp(&bars.rest_full, count & 1, 32u);
       if (!ok) break;
       tc_fence_after();
 #pragma unroll
-      for (int h = 0; h < kUnits; ++h) {
+      for (int c = 0; c < S::kCols; c += 32) {
+        uint32_t r[32];
+        tmem_ld32(lanes + S::kSide + c, r);
+        tmem_wait_ld();
 #pragma unroll
-        for (int c = 0; c < 64; c += 32) {
-          uint32_t r[32];
-          tmem_ld32(lanes + 256 + 128 * h + c, r);
-          tmem_wait_ld();
-#pragma unroll
-          for (int j = 0; j < 32; ++j) sum[h][c + j] = fmaf(__uint_as_float(r[j]), 1.f / 2048.f, sum[h][c + j]);
-        }
+        for (int j = 0; j < 32; ++j) sum[c + j] = fmaf(__uint_as_float(r[j]), 1.f / 2048.f, sum[c + j]);
       }
       arrive(&bars.rest_empty);
-      const int m0 = t.mt * S::kSide + (int)rank * 128 + 32 * q, n0 = t.nt * S::kSide + 64 * kUnits * half;
+      const int m0 = t.mt * S::kSide + (int)rank * 128 + 32 * q, n0 = t.nt * S::kSide + S::kCols * half;
       if (m0 < end.rows) {
 #pragma unroll
-        for (int h = 0; h < kUnits; ++h) {
-#pragma unroll
-          for (int c = 0; c < 64; c += 32) {
-            const int col = n0 + 64 * h + c;
-            if (col < end.cols) end.block(&sum[h][c], m0, col, t.z, end.symmetric && t.mt != t.nt, stg, lane);
-          }
-        }
+        for (int c = 0; c < S::kCols; c += 32)
+          if (n0 + c < end.cols) end.block(&sum[c], m0, n0 + c, t.z, end.symmetric && t.mt != t.nt, stg, lane);
       }
     }
     if (lane == 0) tma_store_wait_read<0>();
@@ -454,9 +427,9 @@ plane_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
   if (warp == 0) {
     tc_fence_after();
     if constexpr (kPair)
-      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem_base), "r"(kCols) : "memory");
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem_base), "r"(kTmem) : "memory");
     else
-      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem_base), "r"(kCols) : "memory");
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem_base), "r"(kTmem) : "memory");
   }
   if constexpr (kPair) tc_cluster_sync();
 }
@@ -515,12 +488,13 @@ static int32_t ortho_product(const Planes& a, const Planes& b, int64_t batch, in
   GemmTiles t = {};
   t.batch = (int)batch, t.splits = 1, t.group = 8, t.symmetric = end.symmetric;
   t.nk = t.nk_split = (int)(ortho_up(k, kGemmK) / kGemmK);
-  // Cycles of both forms: the products of a stage take 768 a unit of 128 x 128, its 64 KB 1490 (44 bytes a cycle); a tile's epilogue some 6000 and 9000.
-  const auto cycles = [&](int64_t side, int64_t room, int64_t epilogue) {
+  // Cycles of both forms: a stage of 64 k takes some 1500 of either, more of a pair whose accumulator is read after each (fp32 results); a tile's epilogue 6000
+  // and 9000.
+  const auto cycles = [&](int64_t side, int64_t room, int64_t stage, int64_t epilogue) {
     const int64_t tm = ortho_up(m, side) / side, tn = ortho_up(n, side) / side, tiles = batch * (end.symmetric ? tm * (tm + 1) / 2 : tm * tn);
-    return (tiles + room - 1) / room * (t.nk * 1500 + epilogue);
+    return (tiles + room - 1) / room * (t.nk * stage + epilogue);
   };
-  if (cycles(256, sm_count() / 2, 9000) < cycles(128, sm_count(), 6000)) return launch_planes<PlaneShape<2, kAMn, kBMn>>(ma, mb, end, t, m, n, k, st);
+  if (cycles(256, sm_count() / 2, end.type == PX_F32 ? 2200 : 1500, 9000) < cycles(128, sm_count(), 1500, 6000)) return launch_planes<PlaneShape<2, kAMn, kBMn>>(ma, mb, end, t, m, n, k, st);
   return launch_planes<PlaneShape<1, kAMn, kBMn>>(ma, mb, end, t, m, n, k, st);
 }
 
