@@ -503,29 +503,34 @@ typedef GemmShape<1, 128, true, true, 5> Dw128;
 typedef GemmShape<1, 256, true, true, 4> Dw256;
 typedef GemmShape<2, 256, true, true, 5> DwPair;
 
-// A product's tiles, and the parts that a long axis is cut into where its tiles are fewer than the SMs.
+// A product's tiles, and the parts that a long axis is cut into where its tiles are fewer than the SMs (at least four steps each).
 struct HeadCut {
   int ctas, kn;
   GemmTiles t;
 };
-static HeadCut cut(int64_t m, int64_t n, int64_t k, bool split, int narrow) {
-  HeadCut c;
-  const int64_t sms = sm_count();
-  c.kn = n <= narrow ? narrow : 256;
-  c.ctas = c.kn == 256 && m > 128 && up(m, 256) / 256 * (up(n, 256) / 256) >= sms ? 2 : 1;
-  c.t = {};
-  c.t.tiles_m = (int)(up(m, 128 * c.ctas) / (128 * c.ctas)), c.t.tiles_n = (int)(up(n, c.kn) / c.kn);
+static HeadCut cut_for(int ctas, int kn, int64_t m, int64_t n, int64_t k, bool split) {
+  HeadCut c = {ctas, kn, {}};
+  const int64_t room = sm_count() / ctas;
+  c.t.tiles_m = (int)(up(m, 128 * ctas) / (128 * ctas)), c.t.tiles_n = (int)(up(n, kn) / kn);
   c.t.batch = 1, c.t.splits = 1, c.t.group = 8;
   c.t.nk = c.t.nk_split = (int)(up(k, kGemmK) / kGemmK);
-  const int64_t tiles = (int64_t)c.t.tiles_m * c.t.tiles_n;
-  if (split && tiles * 2 <= sms) {
-    int64_t s = std::min<int64_t>(sms / tiles, c.t.nk / 4);      // at least four steps each
-    if (s > 1) {
-      c.t.nk_split = (int)((c.t.nk + s - 1) / s);
-      c.t.splits = (c.t.nk + c.t.nk_split - 1) / c.t.nk_split;
-    }
+  const int64_t tiles = (int64_t)c.t.tiles_m * c.t.tiles_n, s = std::min<int64_t>(room / tiles, c.t.nk / 4);
+  if (split && s > 1) {
+    c.t.nk_split = (int)((c.t.nk + s - 1) / s);
+    c.t.splits = (c.t.nk + c.t.nk_split - 1) / c.t.nk_split;
   }
   return c;
+}
+// A pair of CTAs asks L2 for a third less and goes through a step in some 600 cycles, where one alone takes 750 (both measured with all SMs at work): dx of 8192
+// rows, 32768 classes and 1024 channels, two rounds of either, 414 us alone.
+static HeadCut cut(int64_t m, int64_t n, int64_t k, bool split, int narrow) {
+  if (n <= narrow || m <= 128) return cut_for(1, n <= narrow ? narrow : 256, m, n, k, split);
+  const HeadCut one = cut_for(1, 256, m, n, k, split), two = cut_for(2, 256, m, n, k, split);
+  const auto cycles = [](const HeadCut& c, int64_t step) {
+    const int64_t tiles = (int64_t)c.t.tiles_m * c.t.tiles_n * c.t.splits, room = sm_count() / c.ctas;
+    return (tiles + room - 1) / room * (c.t.nk_split * step + 2000);
+  };
+  return cycles(two, 600) < cycles(one, 750) ? two : one;
 }
 
 struct HeadPlan {
