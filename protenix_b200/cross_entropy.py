@@ -24,8 +24,8 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     class counts 1 - e, and each class e / V more.  ``reduction``: "mean" (over the rows that count; of none NaN, with gradients of zero), "sum" or "none".
 
     Logits, exponentials and sums are fp32, sums over rows fp64.  The gradient of the logits is rounded to x's type where the products for x and
-    weight take it (fp16: times 2^14, so that small probabilities survive), before the scale of the loss is applied; that of bias is not.  Differentiable once in x,
-    weight and bias; the gradients have their types and are the same to the bit on each call.
+    weight take it, before the scale of the loss is applied (of losses by row, relative to the largest of their gradients); in fp16 what is below 2^-38 of that vanishes.
+    That of bias is not rounded before its sum.  Differentiable once in x, weight and bias; the gradients have their types and are the same to the bit on each call.
     """
     if not x.is_cuda:
         raise RuntimeError("linear_cross_entropy: CUDA tensors only, this package has no CPU path")

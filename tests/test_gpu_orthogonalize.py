@@ -126,6 +126,14 @@ def test_layouts_and_empty():
         assert px.orthogonalize(torch.zeros(shape, device="cuda")).shape == shape
 
 
+@pytest.mark.parametrize("batch,m,n", [(34000, 64, 1000), (17000, 130, 1000)])
+def test_offsets_beyond_32_bits(batch, m, n):
+    g = torch.randn(batch, m, n, device="cuda", dtype=torch.bfloat16)
+    got = px.orthogonalize(g)
+    at = torch.tensor([0, batch // 2, batch - 1], device="cuda")
+    _close(got[at], _iterated(g[at]))
+
+
 def test_two_streams_at_once():
     sets = [torch.randn(s, device="cuda") for s in ((40, 128, 512), (3, 300, 400), (20, 100, 90))]
     want = [px.orthogonalize(g) for g in sets]

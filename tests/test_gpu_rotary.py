@@ -160,6 +160,17 @@ def test_gradients():
     assert torch.autograd.grad(only[0].sum(), q)[0].shape == q.shape
 
 
+def test_offsets_beyond_32_bits():
+    """Rows that begin beyond 2^31 elements of q, and beyond 2^32 bytes."""
+    n, h, d = 2 ** 31 // (16 * 128) + 700, 16, 128
+    q = torch.zeros(1, n, h, d, dtype=torch.bfloat16, device="cuda").transpose(1, 2)
+    rows = torch.tensor([0, 1, n // 2, n - 600, n - 1], device="cuda")
+    q[:, :, rows] = torch.randn(1, h, 5, d, device="cuda").to(torch.bfloat16)
+    got = px.rotary_embedding(q, None, torch.arange(n, device="cuda")[:, None])
+    _close(got[:, :, rows], q[:, :, rows], rows[None, :, None], (64,), far=n * 2.0 ** -52)
+    assert int(torch.count_nonzero(got)) == int(torch.count_nonzero(got[:, :, rows]))
+
+
 def test_streams_and_capture():
     q, k = torch.randn(2, 4, 70, 64, device="cuda").half(), torch.randn(2, 2, 70, 64, device="cuda").half()
     at = torch.randint(0, 500, (2, 70, 1), device="cuda")
