@@ -9,6 +9,10 @@
 // Roles: warp 0 copies, warp 1 issues products, kSets sets of kSetWarps (4 or 8) are the epilogue: a warp has a quarter of the lanes and all or half of
 // the columns; two sets take the tiles in turn, each with an accumulator of its own.
 // Accumulators are double-buffered.
+//
+// 8192 rows, 2048 channels, 65536 classes, bf16, pairs: the sums of the forward pass at 1600 to 1650 TFLOP/s (a library product 1655), 1024 channels 1580, 512 1380 (tensor
+// pipe 78 % busy), 256 770: below some 700 channels the exponentials' threads take longer than the products (a tile of 256 x 256 costs them some 4 us).  One
+// set of eight epilogue warps 824, 580 and 504 us for 1024, 512 and 256 channels, one of sixteen 774, 575 and 452, two of eight 758, 475 and 357.
 #pragma once
 #include "px_pair.cuh"
 #include "px_rowpipe.cuh"
@@ -75,6 +79,8 @@ struct GemmBarriers {
   uint64_t full[8], empty[8], acc_full[2], acc_empty[2];
   uint32_t tmem_base, peer_stop;
 };
+
+static_assert(sizeof(GemmBarriers) <= 256, "barriers");
 
 // What an epilogue gets for a tile: its place, the accumulator's address with this warp's lanes in it, and what it may use in shared memory.
 struct GemmEpiTile {

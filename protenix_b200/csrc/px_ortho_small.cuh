@@ -42,6 +42,7 @@ struct SmallOrthoBarriers {
   uint32_t tmem_base, stop[8];
   double part[8], sums[8];      // of this CTA's warps; of the cluster's CTAs
 };
+static_assert(sizeof(SmallOrthoBarriers) <= 512, "barriers");
 
 __device__ __forceinline__ int plane_offset(int row, int piece) {      // of the 16 bytes with columns 8 piece ..
   return (piece >> 3) * (kSmallPlane / 2) + row * 128 + (((piece & 7) ^ (row & 7)) << 4);
