@@ -5,7 +5,8 @@
 // Forward, one product whose epilogue keeps of a tile [128 rows][kN classes] each row's maximum, sum of exponentials and (smoothed
 // labels) sum of logits, and the logit of the row's class where it lies in the tile; a second kernel joins the tiles of a row.
 // Backward, for a piece of the classes at a time: the same product again, whose epilogue writes dl in 16 bits, then dx += dl W and
-// dW = dl^T x from it.  What a piece leaves in memory is 16 bits a pair of row and class, kPieceBytes at most, whatever the number of classes.
+// dW = dl^T x from it.  What a piece leaves in memory is 16 bits a pair of row and class: kPieceBytes whatever the number of classes, or 512 bytes a row where
+// that is more (a piece has 256 classes at least).
 // Four products of 2 N V C where three are the least (the logits are formed twice).
 //
 // dl is formed without the scale of the loss, in [-2, 2] (fp16: times 2^14, so that probabilities down to 2^-28 stay normal numbers); the scale is

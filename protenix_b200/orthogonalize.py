@@ -29,7 +29,8 @@ def orthogonalize(g: torch.Tensor, steps: int = 5, coefficients: Coefficients = 
     """
     if not g.is_cuda:
         raise RuntimeError("orthogonalize: CUDA tensors only, this package has no CPU path")
-    triples = [tuple(c) for c in coefficients] if not isinstance(coefficients[0], (int, float)) else [tuple(coefficients)] * int(steps)
+    single = len(coefficients) > 0 and isinstance(coefficients[0], (int, float))
+    triples = [tuple(coefficients)] * int(steps) if single else [tuple(c) for c in coefficients]
     if any(len(c) != 3 for c in triples):
         raise RuntimeError("orthogonalize: coefficients are triples (a, b, c)")
     return native.load().orthogonalize(g, [float(x) for c in triples for x in c], eps)
@@ -81,5 +82,5 @@ class Muon(torch.optim.Optimizer):
                 turned = orthogonalize(torch.stack(update), group["steps"], group["coefficients"], group["eps"])
                 if group["weight_decay"]:
                     torch._foreach_mul_(params, 1.0 - group["lr"] * group["weight_decay"])
-                torch._foreach_add_(params, list(turned.unbind(0)), alpha=-group["lr"] * max(1.0, shape[-2] / shape[-1]) ** 0.5)
+                torch._foreach_add_(params, list(turned.unbind(0)), alpha=-group["lr"] * max(1.0, shape[-2] / max(shape[-1], 1)) ** 0.5)
         return loss

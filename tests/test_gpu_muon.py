@@ -47,6 +47,14 @@ def test_steps(nesterov, dtype):
     assert torch.equal(other.state[params[0]]["momentum_buffer"], opt.state[params[0]]["momentum_buffer"])
 
 
+def test_a_parameter_without_elements():
+    for shape in ((3, 0), (0, 3), (2, 0, 0)):
+        p = torch.nn.Parameter(torch.zeros(shape, device="cuda"))
+        p.grad = torch.zeros_like(p)
+        px.Muon([p]).step()
+        assert p.shape == shape
+
+
 def test_refusals():
     with pytest.raises(ValueError, match="two axes"):
         px.Muon([torch.nn.Parameter(torch.randn(5, device="cuda"))])

@@ -176,7 +176,7 @@ def test_streams_and_capture():
 
 def test_refusals():
     g = torch.randn(4, 8, device="cuda")
-    for x, kw in ((g.cpu(), {}), (g.double(), {}), (g[0], {}), (g, {"steps": 0}), (g, {"coefficients": [(1.0,)]}), (g, {"coefficients": [(1.0, 2.0)]}), (g, {"eps": -1.0}),
+    for x, kw in ((g.cpu(), {}), (g.double(), {}), (g[0], {}), (g, {"steps": 0}), (g, {"coefficients": [(1.0,)]}), (g, {"coefficients": [(1.0, 2.0)]}), (g, {"coefficients": []}), (g, {"eps": -1.0}),
                   (g, {"eps": math.nan}), (g, {"coefficients": (math.inf, 0.0, 0.0)}), (g, {"steps": 1001}), (g.clone().requires_grad_(), {})):
         with pytest.raises(RuntimeError):
             px.orthogonalize(x, **kw)
