@@ -471,7 +471,7 @@ PX_API int32_t px_rotary_turn(const px_rotary* r, const px_rows* q, const px_row
  * l = x w^T + bias for rows x [rows][c] and classes w [classes][c] (PX_BF16 or PX_F16, row strides in elements), bias or NULL;
  * loss_i = lse_i - (1 - smoothing) l_i,target - smoothing / classes sum_v l_iv.  Rows whose target is `ignore` have loss 0 and take no part in
  * any gradient, whatever they hold; a target outside the classes makes its row's loss, and the gradients that it enters, NaN.
- * px_head_loss_fwd writes norm [rows][2] (reference and sum of the exponentials, for the backward pass), the rows' losses [rows] (NULL: not wanted) and their sum or mean over the rows that count
+ * px_head_loss_fwd writes norm [rows + 1][2] (for the backward pass: reference and sum of the exponentials, last what it found in ignored rows), the rows' losses [rows] (NULL: not wanted) and their sum or mean over the rows that count
  * (total, with 1 / count or 1 in `inverse` for the backward pass; NULL: not wanted; the mean of nothing is NaN).
  * px_head_loss_bwd writes those of dx [rows][c], dw [classes][c] (type of x, contiguous) and dbias [classes] (type of the bias) that are not NULL, from the gradient of
  * the total (each = 0: one number) or of the rows' losses (each = 1, `inverse` not read).  It forms the logits again, for so many classes at a time

@@ -13,13 +13,16 @@
 // applied in fp32 where dx and dW are rounded.  Logits, exponentials and all sums are fp32, or fp64 across rows.
 //
 // Rows that are ignored take no part whatever they hold: their dl is zero by selection, and where one holds an infinity or a NaN (which a zero
-// weight would not silence) dW takes a copy of x in which those rows are zero; the copy is made only then.
+// weight would not silence) dW takes a copy of x in which those rows are zero; the copy is made only then.  A row of x that is not finite has no
+// finite logit, so the forward pass sees it in the row's sum; by a pass over the ignored rows and one for the verdict, two more launches, training on
+// 384 rows took 104 us and on 3001 12 us more.
 #include "px_head_small.cuh"
 
 namespace px {
 
 constexpr int64_t kPieceBytes = 512ll << 20;
-constexpr int kScanBlocks = 592, kScanRows = 4;       // rows of a warp
+constexpr int kScanBlocks = 592;
+constexpr int kBiasGroups = 256;       // of 32 rows, whose sums the epilogue of dW adds up
 
 // ---- forward ---------------------------------------------------------------------------------------------------------
 struct EpiStats {
@@ -29,10 +32,11 @@ struct EpiStats {
   float* part_sum;          // [tiles_n][rows]: sum of logits, or NULL
   float* hit;               // [rows]: logit of the row's class
   uint32_t* arrivals;
+  uint32_t* dirty;
   int rows, classes;
   float uncut;
   static constexpr bool kMeets = true, kStores = false;
-  __device__ __forceinline__ void begin() const { *arrivals = 0; }
+  __device__ __forceinline__ void begin() const { *arrivals = 0, *dirty = 0; }
 
   struct Row {
     int mine;                 // the column that is the row's class, or -1
@@ -118,6 +122,7 @@ struct JoinArgs {
   float* inverse;           // receives 1 / count
   double2* sums;            // [blocks]
   uint32_t* arrivals;
+  uint32_t* dirty;          // becomes one where an ignored row of x may not be finite
   int64_t ignore;
   int rows, classes, parts, mean;
   float smooth;
@@ -163,6 +168,8 @@ __global__ void __launch_bounds__(32 * kJoinWarps) loss_join_kernel(const JoinAr
     if (counts) {
       loss = row_loss(s, ref, a.hit[row], t >= 0 && t < a.classes, a.smooth, sum, a.classes);
       l = loss, c = 1.0;
+    } else if (!(s > 0.f && s < CUDART_INF_F)) {
+      *a.dirty = 1;
     }
     a.norm[row] = make_float2(ref, s);
     if (a.losses) a.losses[row] = loss;
@@ -197,86 +204,37 @@ __global__ void __launch_bounds__(32 * kJoinWarps) loss_join_kernel(const JoinAr
   }
 }
 
-// ---- backward: what the products need to know first ------------------------------------------------------------------
-struct ScanArgs {
-  const void* x;
-  int64_t x_stride;
-  const int64_t* target;
-  const float* grad;        // of the loss: one number, or (each) one a row
-  uint2* found;             // [kScanBlocks]: not finite in an ignored row; bits of the largest finite |grad|
-  int64_t ignore, rows;
-  int c, each;
-};
-__device__ __forceinline__ bool finite16x2(uint32_t u, bool f16) {
-  const uint32_t e = f16 ? 0x7c007c00u : 0x7f807f80u, lo = e & 0xffffu, hi = e & 0xffff0000u;
-  return (u & lo) != lo && (u & hi) != hi;
-}
-// A warp a row; rows that count cost their target.
-__global__ void __launch_bounds__(256) loss_scan_kernel(const ScanArgs a, bool f16) {
-  __shared__ uint32_t bad[8], big[8];
-  pdl_wait();
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  uint32_t dirty = 0, top = 0;
-  for (int64_t r0 = ((int64_t)blockIdx.x * 8 + w) * kScanRows; r0 < a.rows; r0 += (int64_t)gridDim.x * 8 * kScanRows) {
-    const int64_t row = r0 + lane;
-    const bool there = lane < kScanRows && row < a.rows, ignored = there && !row_counts(a.target[row], a.ignore);
-    if (a.each && there && !ignored) {
-      const float g = fabsf(a.grad[row]);
-      if (g < CUDART_INF_F) top = max(top, __float_as_uint(g));
-    }
-    for (uint32_t left = __ballot_sync(0xffffffffu, ignored); left; left &= left - 1) {
-      const uint4* p = reinterpret_cast<const uint4*>((const uint16_t*)a.x + (r0 + __ffs(left) - 1) * a.x_stride);
-#pragma unroll 4
-      for (int i = lane; i < a.c / 8; i += 32) {
-        const uint4 v = __ldg(p + i);
-        if (!(finite16x2(v.x, f16) && finite16x2(v.y, f16) && finite16x2(v.z, f16) && finite16x2(v.w, f16))) dirty = 1;
-      }
-    }
-  }
-  dirty = __any_sync(0xffffffffu, dirty);
-  top = __reduce_max_sync(0xffffffffu, top);
-  if (lane == 0) bad[w] = dirty, big[w] = top;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int i = 1; i < 8; ++i) dirty |= bad[i], top = max(top, big[i]);
-    a.found[blockIdx.x] = make_uint2(dirty, top);
-  }
-}
-// Joins that, forms the scales, and copies x without the ignored rows where one of them is not finite.
-__global__ void __launch_bounds__(256) loss_prepare_kernel(const ScanArgs a, const float* __restrict__ inverse, uint16_t* __restrict__ clean, LossScale* __restrict__ scale,
-                                                           int blocks, float dl_scale) {
-  pdl_wait();
-  uint32_t dirty = 0, top = 0;
-  for (int i = threadIdx.x; i < blocks; i += 256) {
-    const uint2 f = a.found[i];
-    dirty |= f.x, top = max(top, f.y);
-  }
+// ---- backward, with a gradient for each row --------------------------------------------------------------------------
+// Bits of the largest finite |gradient| of the rows that count, by block.
+__global__ void __launch_bounds__(256) loss_scan_kernel(const int64_t* __restrict__ target, const float* __restrict__ grad, uint32_t* __restrict__ found, int64_t ignore, int64_t rows) {
   __shared__ uint32_t big;
   if (threadIdx.x == 0) big = 0;
-  dirty = __syncthreads_or((int)dirty) != 0;
-  if (a.each) {
-    top = __reduce_max_sync(0xffffffffu, top);
-    if ((threadIdx.x & 31) == 0) atomicMax(&big, top);
-    __syncthreads();
+  __syncthreads();
+  pdl_wait();
+  uint32_t top = 0;
+  for (int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x; row < rows; row += (int64_t)gridDim.x * 256) {
+    const float g = fabsf(grad[row]);
+    if (row_counts(target[row], ignore) && g < CUDART_INF_F) top = max(top, __float_as_uint(g));
   }
-  if (blockIdx.x == 0 && threadIdx.x == 0) {
-    const float largest = __uint_as_float(big);
-    // divided by a power of two, so that nothing is rounded; the smallest powers have no reciprocal that is finite
-    const float power = fmaxf(__uint_as_float(__float_as_uint(largest) & 0x7f800000u), 1.17549435e-38f);
-    LossScale s;
-    s.out = a.each ? power / dl_scale : a.grad[0] * *inverse / dl_scale;
-    s.each = a.each ? 1.f / power : 1.f;
-    s.dirty = dirty;
-    *scale = s;
-  }
-  if (!dirty) return;
-  const int per = a.c / 8;
-  const int64_t all = a.rows * per;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
-    const int64_t row = i / per;
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (row_counts(a.target[row], a.ignore)) v = __ldg(reinterpret_cast<const uint4*>((const uint16_t*)a.x + row * a.x_stride) + (i - row * per));
-    reinterpret_cast<uint4*>(clean)[i] = v;
+  top = __reduce_max_sync(0xffffffffu, top);
+  if ((threadIdx.x & 31) == 0) atomicMax(&big, top);
+  __syncthreads();
+  if (threadIdx.x == 0) found[blockIdx.x] = big;
+}
+__global__ void __launch_bounds__(256) loss_scale_kernel(const uint32_t* __restrict__ found, LossScale* __restrict__ scale, int blocks, float by) {
+  __shared__ uint32_t big;
+  if (threadIdx.x == 0) big = 0;
+  __syncthreads();
+  pdl_wait();
+  uint32_t top = 0;
+  for (int i = threadIdx.x; i < blocks; i += 256) top = max(top, found[i]);
+  top = __reduce_max_sync(0xffffffffu, top);
+  if ((threadIdx.x & 31) == 0) atomicMax(&big, top);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    // a power of two, so that nothing is rounded; the smallest have no reciprocal that is finite
+    const float power = fmaxf(__uint_as_float(big & 0x7f800000u), 1.17549435e-38f);
+    *scale = {power * by, 1.f / power};
   }
 }
 
@@ -286,8 +244,13 @@ struct EpiLogitGrad {
   const int64_t* target;
   HeadBias bias;            // of the piece
   const float2* norm;
-  const float* grad;        // of each row's loss, or NULL
+  const float* grad;        // of each row's loss, with their scale, or NULL
   const LossScale* scale;
+  const uint16_t* x;        // where a row of it may not be finite: receives the ignored rows as zeros in `clean`
+  uint16_t* clean;          // or NULL
+  const uint32_t* dirty;
+  int64_t x_stride;
+  int c;
   float* part_bias;         // [32-row groups][classes of the piece]: sums of dl, or NULL
   int64_t ignore;
   int rows, classes, first, all_classes;      // first: the piece's first class
@@ -302,8 +265,20 @@ struct EpiLogitGrad {
     int mine;
     bool counts, plain;
   };
+  __device__ __forceinline__ void copy(int row0, int lane) const {
+    const int per = c / 8;
+#pragma unroll 1
+    for (int row = row0; row < min(row0 + 32, rows); ++row) {
+      const bool there = row_counts(target[row], ignore);
+      const uint4* const from = reinterpret_cast<const uint4*>(x + row * x_stride);
+      uint4* const to = reinterpret_cast<uint4*>(clean) + (int64_t)row * per;
+#pragma unroll 1
+      for (int i = lane; i < per; i += 32) to[i] = there ? __ldg(from + i) : make_uint4(0, 0, 0, 0);
+    }
+  }
   template <class S>
   __device__ __forceinline__ Row before(const GemmEpiTile& e) const {
+    if (clean && e.at.nt == 0 && e.part == 0 && *dirty) copy(e.m0, e.lane);      // the warps of the first classes see each row once
     Row at = {};
     const int row = e.m0 + e.lane;
     const int64_t t = row < rows ? target[row] : ignore;
@@ -376,8 +351,7 @@ struct EpiLogitGrad {
 };
 
 // db of a piece: a warp's lanes along the classes, the groups of rows over the warps, in a fixed order.
-__global__ void __launch_bounds__(512) loss_bias_kernel(const float* __restrict__ part, void* __restrict__ db, int type, const LossScale* __restrict__ scale,
-                                                        int classes, int groups) {
+__global__ void __launch_bounds__(512) loss_bias_kernel(const float* __restrict__ part, void* __restrict__ db, int type, const LossOut out, int classes, int groups) {
   __shared__ float x[16][32];
   pdl_wait();
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, v = blockIdx.x * 32 + lane;
@@ -389,7 +363,7 @@ __global__ void __launch_bounds__(512) loss_bias_kernel(const float* __restrict_
   if (w == 0 && v < classes) {
     float all = 0.f;
     for (int i = 0; i < 16; ++i) all += x[i][lane];
-    bias_store(db, type, v, all * scale->out);
+    bias_store(db, type, v, all * out());
   }
 }
 
@@ -397,11 +371,14 @@ __global__ void __launch_bounds__(512) loss_bias_kernel(const float* __restrict_
 // kF32: sums of one split, stored (or added to what the pieces before have left); otherwise the result in 16 bits.
 template <bool kF32>
 struct EpiGrad {
-  CUtensorMap out;          // boxes of 32 rows of 128 bytes
-  const LossScale* scale;
+  CUtensorMap map;          // boxes of 32 rows of 128 bytes
+  LossOut out;
   const int64_t* target;    // of the rows, those that are ignored get zeros; or NULL
   int64_t ignore;
   int rows, cols, add, f16;
+  const float* part_bias;   // dW: sums of dl over 32 rows each, which become db here, or NULL
+  void* db;
+  int groups, db_type;
   static constexpr bool kMeets = false;
   __device__ __forceinline__ void begin() const {}
 
@@ -412,7 +389,16 @@ struct EpiGrad {
   template <class S>
   __device__ __forceinline__ Row before(const GemmEpiTile& e) const {
     const int row = e.m0 + e.lane;
-    return {kF32 ? 1.f : scale->out, !kF32 && target && row < rows && !row_counts(target[row], ignore)};
+    const float by = out();
+    if (part_bias && e.at.nt == 0 && e.at.split == 0 && e.part == 0 && row < rows) {
+      double s[4] = {};
+      for (int g = 0; g < groups; g += 4) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[j] += g + j < groups ? part_bias[(int64_t)(g + j) * rows + row] : 0.f;
+      }
+      bias_store(db, db_type, row, (float)((s[0] + s[1]) + (s[2] + s[3])) * by);
+    }
+    return {by, !kF32 && target && row < rows && !row_counts(target[row], ignore)};
   }
   template <class S, class F>
   __device__ __forceinline__ void tile(const GemmEpiTile& e, const Row& at, F release) const {
@@ -456,10 +442,10 @@ struct EpiGrad {
       if (e.lane == 0) {
         if (kF32 && add)
           asm volatile("cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.bulk_group [%0, {%2, %3, %4}], [%1];\n"
-                       ::"l"(reinterpret_cast<uint64_t>(&out)), "r"(smem_u32(e.stg)), "r"(base + c), "r"(e.m0), "r"(e.at.split)
+                       ::"l"(reinterpret_cast<uint64_t>(&map)), "r"(smem_u32(e.stg)), "r"(base + c), "r"(e.m0), "r"(e.at.split)
                        : "memory");
         else
-          tma_store_3d(&out, smem_u32(e.stg), base + c, e.m0, e.at.split);
+          tma_store_3d(&map, smem_u32(e.stg), base + c, e.m0, e.at.split);
         tma_store_commit();
       }
     }
@@ -467,11 +453,11 @@ struct EpiGrad {
 };
 
 // The splits' sums in their order, scaled and rounded.
-__global__ void __launch_bounds__(256) loss_gather_kernel(const float* __restrict__ slots, uint16_t* __restrict__ out, const LossScale* __restrict__ scale,
+__global__ void __launch_bounds__(256) loss_gather_kernel(const float* __restrict__ slots, uint16_t* __restrict__ to, const LossOut out,
                                                           const int64_t* __restrict__ target, int64_t ignore, int64_t rows, int c, int splits, bool f16) {
   pdl_wait();
   const int64_t all = rows * c / 4;
-  const float by = scale->out;
+  const float by = out();
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int k = 0; k < splits; ++k) {
@@ -480,7 +466,7 @@ __global__ void __launch_bounds__(256) loss_gather_kernel(const float* __restric
     }
     s.x *= by, s.y *= by, s.z *= by, s.w *= by;
     if (target && !row_counts(target[4 * i / c], ignore)) s = make_float4(0.f, 0.f, 0.f, 0.f);
-    reinterpret_cast<uint2*>(out)[i] = f16 ? make_uint2(pack_f16x2_inf(s.x, s.y), pack_f16x2_inf(s.z, s.w)) : make_uint2(pack_bf16x2(s.x, s.y), pack_bf16x2(s.z, s.w));
+    reinterpret_cast<uint2*>(to)[i] = f16 ? make_uint2(pack_f16x2_inf(s.x, s.y), pack_f16x2_inf(s.z, s.w)) : make_uint2(pack_bf16x2(s.x, s.y), pack_bf16x2(s.z, s.w));
   }
 }
 
@@ -558,7 +544,7 @@ static HeadPlan head_plan(const px_head& h, bool want_dx, bool want_dw, bool wan
     return here;
   };
   p.scale = take(sizeof(LossScale));
-  p.found = take(kScanBlocks * sizeof(uint2));
+  p.found = take(kScanBlocks * 4);
   p.clean = take(want_dw ? h.rows * h.c * 2 : 0);
   p.dl = take(h.rows * p.ld * 2);
   p.dx_at = take(want_dx && p.dx_slots ? p.dx.t.splits * h.rows * h.c * 4 : 0);
@@ -611,9 +597,9 @@ static int32_t launch_grad(GemmOperands& ops, bool f16, const HeadCut& c, const 
   if (c.ctas == 1) return ops.idesc = W::idesc(f16), gemm_launch<W>(ops, epi, t, st);
   return ops.idesc = P::idesc(f16), gemm_launch<P>(ops, epi, t, st);
 }
-static int32_t gather(const float* slots, void* out, const LossScale* scale, const int64_t* target, int64_t ignore, int64_t rows, int64_t c, int splits, bool f16, cudaStream_t st) {
+static int32_t gather(const float* slots, void* to, const LossOut& out, const int64_t* target, int64_t ignore, int64_t rows, int64_t c, int splits, bool f16, cudaStream_t st) {
   const int64_t blocks = std::min<int64_t>((rows * c / 4 + 255) / 256, 8 * sm_count());
-  return launch_pdl(loss_gather_kernel, dim3((unsigned)blocks), 256, 0, st, slots, (uint16_t*)out, scale, target, ignore, rows, (int)c, splits, f16) ? PX_OK : PX_ERR_LAUNCH;
+  return launch_pdl(loss_gather_kernel, dim3((unsigned)blocks), 256, 0, st, slots, (uint16_t*)to, out, target, ignore, rows, (int)c, splits, f16) ? PX_OK : PX_ERR_LAUNCH;
 }
 
 // ---- heads that fit an SM --------------------------------------------------------------------------------------------
@@ -651,7 +637,7 @@ struct SmallPlan {
 static SmallPlan small_plan(const px_head& h) {
   const int64_t ctas = small_ctas(h.rows), vp = small_vp(h.classes);
   SmallPlan p;
-  p.scale = 0, p.found = 1024, p.w = p.found + up(kScanBlocks * 8, 1024), p.b = p.w + ctas * 128 * vp * 4, p.bytes = p.b + ctas * 8 * vp * 4;
+  p.scale = 0, p.found = 1024, p.w = p.found + up(kScanBlocks * 4, 1024), p.b = p.w + ctas * 128 * vp * 4, p.bytes = p.b + ctas * 8 * vp * 4;
   return p;
 }
 
@@ -692,9 +678,10 @@ extern "C" int32_t px_head_loss_fwd(const px_head* head, float* norm, float* los
   at += up((h.rows + 31) / 32 * 16, 1024);
   float2* part = (float2*)at;
   at += up(c.t.tiles_n * h.rows * 8, 1024);
-  EpiStats epi = {h.target, {h.bias, h.bias_dtype}, part, h.smoothing > 0.f ? (float*)at : nullptr, hit, arrivals, (int)h.rows, (int)h.classes, uncut_logits(h.c)};
+  uint32_t* const dirty = (uint32_t*)(norm + 2 * h.rows);
+  EpiStats epi = {h.target, {h.bias, h.bias_dtype}, part, h.smoothing > 0.f ? (float*)at : nullptr, hit, arrivals, dirty, (int)h.rows, (int)h.classes, uncut_logits(h.c)};
   if (const int32_t status = launch_logits(h, 0, h.classes, c, epi, st)) return status;
-  JoinArgs j = {part, epi.part_sum, hit, h.target, (float2*)norm, losses, total, inverse, sums, arrivals, h.ignore, (int)h.rows, (int)h.classes, c.t.tiles_n, mean, h.smoothing};
+  JoinArgs j = {part, epi.part_sum, hit, h.target, (float2*)norm, losses, total, inverse, sums, arrivals, dirty, h.ignore, (int)h.rows, (int)h.classes, c.t.tiles_n, mean, h.smoothing};
   return launch_pdl(loss_join_kernel, dim3((unsigned)((h.rows + 31) / 32)), 32 * kJoinWarps, 0, st, j) ? PX_OK : PX_ERR_LAUNCH;
 }
 
@@ -714,23 +701,26 @@ extern "C" int32_t px_head_loss_bwd(const px_head* head, const float* norm, cons
   if (!dx && !dw && !dbias) return PX_OK;
   const cudaStream_t st = (cudaStream_t)stream;
   const bool f16 = h.dtype == PX_F16;
-  const float dl_scale = f16 ? kDlScaleF16 : 1.f;
   const int64_t bias_size = h.bias_dtype == PX_F32 ? 4 : 2;
-  const int scan_blocks = (int)std::min<int64_t>((h.rows + 8 * kScanRows - 1) / (8 * kScanRows), kScanBlocks);
   char* const ws = (char*)workspace;
+  LossOut out = {nullptr, grad, inverse, f16 ? 1.f / kDlScaleF16 : 1.f};
+  const auto scales = [&](int64_t scale_at, int64_t found_at) {
+    if (!each) return true;
+    LossScale* const scale = (LossScale*)(ws + scale_at);
+    uint32_t* const found = (uint32_t*)(ws + found_at);
+    const int blocks = (int)std::min<int64_t>((h.rows + 255) / 256, kScanBlocks);
+    out.scale = scale;
+    return launch_pdl(loss_scan_kernel, dim3(blocks), 256, 0, st, h.target, grad, found, h.ignore, h.rows) &&
+           launch_pdl(loss_scale_kernel, dim3(1), 256, 0, st, (const uint32_t*)found, scale, blocks, out.by);
+  };
   if (small_head(h.c, h.classes)) {
     const SmallPlan p = small_plan(h);
     SmallArgs a;
     if (!small_args(&a, h) || (dx && !out_map(&a.dx, type16(f16), 2, dx, h.c, h.rows, h.c, 1))) return PX_ERR_LAUNCH;
-    a.norm = (float2*)const_cast<float*>(norm), a.grad = grad, a.inverse = inverse, a.want_dx = dx != nullptr;
+    a.norm = (float2*)const_cast<float*>(norm), a.want_dx = dx != nullptr;
     a.part_w = dw ? (float*)(ws + p.w) : nullptr, a.part_b = dbias ? (float*)(ws + p.b) : nullptr;
-    if (each) {
-      const ScanArgs scan = {h.x, h.x_stride, h.target, grad, (uint2*)(ws + p.found), h.ignore, h.rows, 0, each};
-      a.scale = (const LossScale*)(ws + p.scale);
-      if (!launch_pdl(loss_scan_kernel, dim3(scan_blocks), 256, 0, st, scan, f16) ||
-          !launch_pdl(loss_prepare_kernel, dim3(1), 256, 0, st, scan, inverse, nullptr, (LossScale*)(ws + p.scale), scan_blocks, dl_scale))
-        return PX_ERR_LAUNCH;
-    }
+    if (!scales(p.scale, p.found)) return PX_ERR_LAUNCH;
+    a.out = out;
     if (!launch_small<true>(a, st)) return PX_ERR_LAUNCH;
     if (!dw && !dbias) return PX_OK;
     const int vp = (int)small_vp(h.classes), groups = vp / 32;
@@ -740,26 +730,25 @@ extern "C" int32_t px_head_loss_bwd(const px_head* head, const float* norm, cons
                : PX_ERR_LAUNCH;
   }
   const HeadPlan p = head_plan(h, dx, dw, dbias);
-  LossScale* scale = (LossScale*)(ws + p.scale);
   uint16_t* dl = (uint16_t*)(ws + p.dl);
   uint16_t* clean = (uint16_t*)(ws + p.clean);
   float* part_bias = (float*)(ws + p.db_at);
-  const ScanArgs scan = {h.x, h.x_stride, h.target, grad, (uint2*)(ws + p.found), h.ignore, h.rows, dw ? (int)h.c : 0, each};
-  if (!launch_pdl(loss_scan_kernel, dim3(scan_blocks), 256, 0, st, scan, f16)) return PX_ERR_LAUNCH;
-  const int copy_blocks = dw ? (int)std::min<int64_t>((h.rows * h.c / 8 + 255) / 256, 2 * sm_count()) : 1;
-  if (!launch_pdl(loss_prepare_kernel, dim3(copy_blocks), 256, 0, st, scan, inverse, clean, scale, scan_blocks, dl_scale)) return PX_ERR_LAUNCH;
+  const uint32_t* const dirty = (const uint32_t*)(norm + 2 * h.rows);
+  const int bias_groups = (int)((h.rows + 31) / 32);
+  if (!scales(p.scale, p.found)) return PX_ERR_LAUNCH;
 
   for (int64_t i = 0; i < p.pieces; ++i) {
     const int64_t first = i * p.piece, vc = std::min(p.piece, h.classes - first);
     EpiLogitGrad el = {};
     if (!dl_map(&el.out, type16(f16), dl, vc, h.rows, p.ld)) return PX_ERR_LAUNCH;
-    el.target = h.target, el.bias = {h.bias ? (const char*)h.bias + first * bias_size : nullptr, h.bias_dtype}, el.norm = (const float2*)norm, el.grad = each ? grad : nullptr, el.scale = scale;
+    el.target = h.target, el.bias = {h.bias ? (const char*)h.bias + first * bias_size : nullptr, h.bias_dtype}, el.norm = (const float2*)norm, el.grad = each ? grad : nullptr, el.scale = out.scale;
+    if (dw && i == 0) el.x = (const uint16_t*)h.x, el.x_stride = h.x_stride, el.c = (int)h.c, el.clean = clean, el.dirty = dirty;
     el.part_bias = dbias ? part_bias : nullptr, el.ignore = h.ignore, el.rows = (int)h.rows, el.classes = (int)vc, el.first = (int)first;
     el.all_classes = (int)h.classes, el.smooth = h.smoothing, el.uncut = uncut_logits(h.c), el.f16 = f16;
     if (const int32_t status = launch_logits(h, first, vc, p.logits, el, st)) return status;
-    if (dbias && !launch_pdl(loss_bias_kernel, dim3((unsigned)((vc + 31) / 32)), 512, 0, st, (const float*)part_bias, (void*)((char*)dbias + first * bias_size), (int)h.bias_dtype, (const LossScale*)scale, (int)vc,
-                             (int)((h.rows + 31) / 32)))
-      return PX_ERR_LAUNCH;
+    void* const db = dbias ? (char*)dbias + first * bias_size : nullptr;
+    const bool bias_apart = dbias && (!dw || bias_groups > kBiasGroups);
+    if (bias_apart && !launch_pdl(loss_bias_kernel, dim3((unsigned)((vc + 31) / 32)), 512, 0, st, (const float*)part_bias, db, (int)h.bias_dtype, out, (int)vc, bias_groups)) return PX_ERR_LAUNCH;
     if (dx) {
       GemmOperands ops = {};
       if (!gemm_map(&ops.a, f16, dl, vc, h.rows, 1, p.ld, h.rows * p.ld, kGemmM) ||
@@ -773,13 +762,13 @@ extern "C" int32_t px_head_loss_bwd(const px_head* head, const float* norm, cons
       int32_t status;
       if (p.dx_slots) {
         EpiGrad<true> ep = {};
-        if (!out_map(&ep.out, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, ws + p.dx_at, h.c, h.rows, h.c, p.dx.t.splits)) return PX_ERR_LAUNCH;
-        ep.rows = (int)h.rows, ep.cols = (int)h.c, ep.add = i > 0;
+        if (!out_map(&ep.map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, ws + p.dx_at, h.c, h.rows, h.c, p.dx.t.splits)) return PX_ERR_LAUNCH;
+        ep.out = out, ep.rows = (int)h.rows, ep.cols = (int)h.c, ep.add = i > 0;
         status = launch_grad<Dx128, Dx256, DxPair>(ops, f16, p.dx, ep, t, st);
       } else {
         EpiGrad<false> ep = {};
-        if (!out_map(&ep.out, type16(f16), 2, dx, h.c, h.rows, h.c, 1)) return PX_ERR_LAUNCH;
-        ep.scale = scale, ep.target = h.target, ep.ignore = h.ignore, ep.rows = (int)h.rows, ep.cols = (int)h.c, ep.f16 = f16;
+        if (!out_map(&ep.map, type16(f16), 2, dx, h.c, h.rows, h.c, 1)) return PX_ERR_LAUNCH;
+        ep.out = out, ep.target = h.target, ep.ignore = h.ignore, ep.rows = (int)h.rows, ep.cols = (int)h.c, ep.f16 = f16;
         status = launch_grad<Dx128, Dx256, DxPair>(ops, f16, p.dx, ep, t, st);
       }
       if (status) return status;
@@ -790,25 +779,30 @@ extern "C" int32_t px_head_loss_bwd(const px_head* head, const float* norm, cons
       if (!gemm_map(&ops.a, f16, dl, vc, h.rows, 1, p.ld, h.rows * p.ld, kGemmK) || !gemm_map(&ops.b, f16, h.x, h.c, h.rows, 1, h.x_stride, h.rows * h.x_stride, kGemmK) ||
           !gemm_map(&ops.b_other, f16, clean, h.c, h.rows, 1, h.c, h.rows * h.c, kGemmK))
         return PX_ERR_LAUNCH;
-      ops.other = &scale->dirty;
+      ops.other = dirty;
       GemmTiles t = p.dw.t;
       t.tiles_m = (int)(up(vc, 128 * p.dw.ctas) / (128 * p.dw.ctas));
+      const auto bias_here = [&](auto& ep) {
+        if (dbias && !bias_apart) ep.part_bias = part_bias, ep.db = db, ep.groups = bias_groups, ep.db_type = (int)h.bias_dtype;
+      };
       int32_t status;
       if (t.splits > 1) {
         EpiGrad<true> ep = {};
-        if (!out_map(&ep.out, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, ws + p.dw_at, h.c, vc, h.c, t.splits)) return PX_ERR_LAUNCH;
-        ep.rows = (int)vc, ep.cols = (int)h.c;
+        bias_here(ep);
+        if (!out_map(&ep.map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, ws + p.dw_at, h.c, vc, h.c, t.splits)) return PX_ERR_LAUNCH;
+        ep.out = out, ep.rows = (int)vc, ep.cols = (int)h.c;
         status = launch_grad<Dw128, Dw256, DwPair>(ops, f16, p.dw, ep, t, st);
-        if (!status) status = gather((const float*)(ws + p.dw_at), to, scale, nullptr, 0, vc, h.c, t.splits, f16, st);
+        if (!status) status = gather((const float*)(ws + p.dw_at), to, out, nullptr, 0, vc, h.c, t.splits, f16, st);
       } else {
         EpiGrad<false> ep = {};
-        if (!out_map(&ep.out, type16(f16), 2, to, h.c, vc, h.c, 1)) return PX_ERR_LAUNCH;
-        ep.scale = scale, ep.rows = (int)vc, ep.cols = (int)h.c, ep.f16 = f16;
+        bias_here(ep);
+        if (!out_map(&ep.map, type16(f16), 2, to, h.c, vc, h.c, 1)) return PX_ERR_LAUNCH;
+        ep.out = out, ep.rows = (int)vc, ep.cols = (int)h.c, ep.f16 = f16;
         status = launch_grad<Dw128, Dw256, DwPair>(ops, f16, p.dw, ep, t, st);
       }
       if (status) return status;
     }
   }
-  if (dx && p.dx_slots) return gather((const float*)(ws + p.dx_at), dx, scale, h.target, h.ignore, h.rows, h.c, p.dx.t.splits, f16, st);
+  if (dx && p.dx_slots) return gather((const float*)(ws + p.dx_at), dx, out, h.target, h.ignore, h.rows, h.c, p.dx.t.splits, f16, st);
   return PX_OK;
 }

@@ -8,11 +8,18 @@ namespace px {
 
 constexpr float kDlScaleF16 = 16384.f;
 
-// What the small kernels of a backward pass leave for the products.
+// With a gradient for each row: the largest is made one where dl is rounded.
 struct LossScale {
   float out;            // what dx and dW are multiplied by
-  float each;           // what the gradient of a row's loss is multiplied by, so that the largest is one
-  uint32_t dirty;       // an ignored row holds what is not finite
+  float each;           // what the gradient of a row's loss is multiplied by
+};
+// What dx, dW and db are multiplied by where they leave.
+struct LossOut {
+  const LossScale* scale;      // of gradients by row, or NULL
+  const float* grad;           // of the mean or sum, with `inverse`
+  const float* inverse;
+  float by;                    // one over what dl is multiplied by
+  __device__ __forceinline__ float operator()() const { return scale ? scale->out : *grad * *inverse * by; }
 };
 
 // What exponentials are taken relative to, in powers of two, for a maximum that may be that of nothing.

@@ -29,9 +29,7 @@ struct SmallArgs {
   float2* norm;
   float* losses;                                          // forward: of the rows, or NULL
   double2* sums;                                          // forward: [CTAs] sum and number of the losses
-  const float* grad;                                      // backward
-  const float* inverse;
-  const LossScale* scale;                                 // backward, with a gradient for each row; otherwise NULL
+  LossOut out;                                            // backward
   float* part_w;                                          // backward: [CTAs][128][kVp], or NULL
   float* part_b;                                          // backward: [8 CTAs][kVp], or NULL
   int64_t ignore;
@@ -173,8 +171,8 @@ __global__ void __launch_bounds__(SmallShape<kBackward, kVp>::kThreads, 1) small
     float db[kVp / 32] = {};
     float out = 0.f, each = 1.f;
     if constexpr (kBackward) {
-      out = a.scale ? a.scale->out : a.grad[0] * *a.inverse * (a.f16 ? 1.f / kDlScaleF16 : 1.f);
-      each = a.scale ? a.scale->each : 1.f;
+      out = a.out();
+      each = a.out.scale ? a.out.scale->each : 1.f;
     }
     int i = set;
     bool ok = true;
@@ -243,7 +241,7 @@ __global__ void __launch_bounds__(SmallShape<kBackward, kVp>::kThreads, 1) small
         const int bl = i & 1;
         float factor = 0.f, ref = 0.f, over = 0.f;
         if (counts) {
-          factor = a.scale ? a.grad[row] * each : 1.f;
+          factor = a.out.scale ? a.out.grad[row] * each : 1.f;
           if (!valid) factor = CUDART_NAN_F;
           if (a.f16) factor *= kDlScaleF16;
           ref = -n.x, over = factor / n.y;
@@ -339,7 +337,7 @@ __global__ void __launch_bounds__(SmallShape<kBackward, kVp>::kThreads, 1) small
     // dx
     const int q = warp & 3;
     const uint32_t lanes = tmem + ((uint32_t)(32 * q) << 16) + S::kDx;
-    const float out = a.scale ? a.scale->out : a.grad[0] * *a.inverse * (a.f16 ? 1.f / kDlScaleF16 : 1.f);
+    const float out = a.out();
     int i = 0;
     for (int tile = blockIdx.x; tile < a.tiles; tile += gridDim.x, ++i) {
       const int d = i % kDxs, row = 128 * tile + 32 * q + lane;

@@ -350,7 +350,7 @@ Tensor head_loss_forward(const Tensor& x, const Tensor& w, const Tensor& bias, c
   const px_head h = head_of(x, w, bias, target, c);
   const auto f32 = x.options().dtype(at::kFloat);
   const Tensor loss = c.reduction ? at::empty({}, f32) : at::empty({h.rows}, f32);
-  norm = at::empty({h.rows, 2}, f32);
+  norm = at::empty({h.rows + 1, 2}, f32);
   if (c.reduction) inverse = at::empty({}, f32);
   const int64_t bytes = abi.px_head_loss_workspace_bytes(h.rows, h.classes);
   const Tensor ws = bytes_like(x, bytes);

@@ -131,6 +131,23 @@ def test_ignored_rows_have_no_influence(rows, c, v, hold):
         assert bool(torch.isfinite(z).all()) and torch.equal(a, z)
 
 
+@pytest.mark.parametrize("rows,c,v", [(70, 128, 130), (300, 264, 300), (9000, 136, 700)])
+@pytest.mark.parametrize("sign", [0.0, 1.0, -1.0])
+def test_one_element_of_an_ignored_row(rows, c, v, sign):
+    """Infinite logits of one sign, or NaN, in a single ignored row; its neighbours and the rows of other tiles keep their part."""
+    x, w, b, t = _inputs(rows, c, v, BF16, torch.float32, ignored=0.3, seed=4)
+    t[rows - 2] = -100
+    with torch.no_grad():
+        w[:, 5] = sign
+    outs = []
+    for hold in (0.0, math.inf):
+        x.data[rows - 2, 5] = hold
+        loss = px.linear_cross_entropy(x, w, t, b, label_smoothing=0.1)
+        outs.append((loss.detach(), *torch.autograd.grad(loss, (x, w, b))))
+    for y, z in zip(*outs):
+        assert bool(y.isfinite().all()) and torch.equal(y, z)
+
+
 @pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
 def test_all_rows_ignored(reduction):
     x, w, b, t = _inputs(140, 64, 70, FP16, FP16)
