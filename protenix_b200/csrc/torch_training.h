@@ -435,8 +435,9 @@ Tensor linear_cross_entropy(const Tensor& x, const Tensor& weight, const Tensor&
     const Tensor each = x.to(at::kFloat).sum(-1) + rest;
     return how == 0 ? each : how == 1 ? each.sum() / 0.0 : each.sum();
   }
-  const Tensor x2 = x.reshape({rows, c});
-  const Tensor t = target.detach().to(at::kLong).reshape({rows}).contiguous();
+  const Tensor x2 = x.dim() == 2 ? x : x.reshape({rows, c});      // a view would be a node of the graph
+  Tensor t = target.to(at::kLong);
+  t = (t.dim() == 1 ? t : t.reshape({rows})).contiguous();
   Tensor loss;
   if (train) {
     loss = HeadLossFunction::apply(x2, weight, bias, t, ignore, smoothing, how);
@@ -444,7 +445,7 @@ Tensor linear_cross_entropy(const Tensor& x, const Tensor& weight, const Tensor&
     Tensor norm, inverse;
     loss = head_loss_forward(matrix_fitted(x2), matrix_fitted(weight), has(bias) ? aligned(*bias) : Tensor(), t, {ignore, smoothing, how}, norm, inverse);
   }
-  return how == 0 ? loss.reshape(target.sizes()) : loss;
+  return how == 0 && target.dim() != 1 ? loss.reshape(target.sizes()) : loss;
 }
 
 // ---- rotary positions ------------------------------------------------------------------------------------------------
