@@ -490,21 +490,24 @@ typedef GemmShape<1, 128, true, true, 5> Dw128;
 typedef GemmShape<1, 256, true, true, 4> Dw256;
 typedef GemmShape<2, 256, true, true, 5> DwPair;
 
-// A product's tiles, and the parts that a long axis is cut into where its tiles are fewer than the SMs (at least four steps each).
+// A product's tiles, and the parts that a long axis is cut into (at least four steps each) where that shortens the rounds of its tiles: fewer tiles than SMs, or
+// a last round with few.
 struct HeadCut {
   int ctas, kn;
   GemmTiles t;
+  int64_t cycles;
 };
 static HeadCut cut_for(int ctas, int kn, int64_t m, int64_t n, int64_t k, bool split) {
-  HeadCut c = {ctas, kn, {}};
+  HeadCut c = {ctas, kn, {}, 0};
   const int64_t room = sm_count() / ctas;
   c.t.tiles_m = (int)(up(m, 128 * ctas) / (128 * ctas)), c.t.tiles_n = (int)(up(n, kn) / kn);
   c.t.batch = 1, c.t.splits = 1, c.t.group = 8;
   c.t.nk = c.t.nk_split = (int)(up(k, kGemmK) / kGemmK);
-  const int64_t tiles = (int64_t)c.t.tiles_m * c.t.tiles_n, s = std::min<int64_t>(room / tiles, c.t.nk / 4);
-  if (split && s > 1) {
-    c.t.nk_split = (int)((c.t.nk + s - 1) / s);
-    c.t.splits = (c.t.nk + c.t.nk_split - 1) / c.t.nk_split;
+  const int64_t tiles = (int64_t)c.t.tiles_m * c.t.tiles_n, step = ctas == 2 ? 600 : 750;
+  for (int64_t s = 1; s <= (split ? std::min<int64_t>(std::max<int64_t>(room / tiles, 4), c.t.nk / 4) : 1) || s == 1; ++s) {
+    const int64_t nk = (c.t.nk + s - 1) / s, parts = (c.t.nk + nk - 1) / nk;
+    const int64_t cycles = (tiles * parts + room - 1) / room * (nk * step + 2000) + (parts > 1 ? 4000 + m * n * parts / 400 : 0);
+    if (s == 1 || cycles < c.cycles) c.cycles = cycles, c.t.nk_split = (int)nk, c.t.splits = (int)parts;
   }
   return c;
 }
@@ -513,11 +516,7 @@ static HeadCut cut_for(int ctas, int kn, int64_t m, int64_t n, int64_t k, bool s
 static HeadCut cut(int64_t m, int64_t n, int64_t k, bool split, int narrow) {
   if (n <= narrow || m <= 128) return cut_for(1, n <= narrow ? narrow : 256, m, n, k, split);
   const HeadCut one = cut_for(1, 256, m, n, k, split), two = cut_for(2, 256, m, n, k, split);
-  const auto cycles = [](const HeadCut& c, int64_t step) {
-    const int64_t tiles = (int64_t)c.t.tiles_m * c.t.tiles_n * c.t.splits, room = sm_count() / c.ctas;
-    return (tiles + room - 1) / room * (c.t.nk_split * step + 2000);
-  };
-  return cycles(two, 600) < cycles(one, 750) ? two : one;
+  return two.cycles < one.cycles ? two : one;
 }
 
 struct HeadPlan {

@@ -32,19 +32,33 @@ __host__ __device__ constexpr float uncut(int64_t k, int chunk) { return 1.f + 2
 
 // ---- norm and first iterate ------------------------------------------------------------------------------------------
 constexpr int kNormBlocks = 1024;      // of a matrix, at most
-template <typename T>
+// kVec elements at a time: 16 bytes where matrices begin at a multiple of that (24 x 384 x 1536, bf16: by elements 14 us).
+template <typename T, int kVec>
 __global__ void __launch_bounds__(256) ortho_norm_kernel(const T* __restrict__ g, double* __restrict__ sums, int64_t elements) {
   __shared__ double part[8];
+  struct alignas(sizeof(T) * kVec) Vec {
+    T v[kVec];
+  };
   pdl_wait();
-  const T* p = g + blockIdx.y * elements;
+  const Vec* p = reinterpret_cast<const Vec*>(g + blockIdx.y * elements);
   double s0 = 0.0, s1 = 0.0;
-  const int64_t step = (int64_t)gridDim.x * 256;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < elements; i += 8 * step) {
-    float v[8];
+  const int64_t step = (int64_t)gridDim.x * 256, all = elements / kVec;
+  constexpr int kAtOnce = kVec == 1 ? 8 : 4;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += kAtOnce * step) {
+    Vec v[kAtOnce];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = i + j * step < elements ? (float)p[i + j * step] : 0.f;
+    for (int j = 0; j < kAtOnce; ++j)
+      if (i + j * step < all) v[j] = p[i + j * step];
 #pragma unroll
-    for (int j = 0; j < 8; j += 2) s0 = fma((double)v[j], (double)v[j], s0), s1 = fma((double)v[j + 1], (double)v[j + 1], s1);
+    for (int j = 0; j < kAtOnce; ++j) {
+      if (i + j * step >= all) break;
+#pragma unroll
+      for (int k = 0; k < kVec; ++k) {
+        const double x = (double)(float)v[j].v[k];
+        double& s = ((j * kVec + k) & 1) ? s1 : s0;
+        s = fma(x, x, s);
+      }
+    }
   }
   s0 += s1;
 #pragma unroll
@@ -528,7 +542,9 @@ template <typename T>
 static bool ortho_first(const void* g, double* sums, uint4* planes, int64_t batch, int64_t m, int64_t n, int64_t ld, double eps, cudaStream_t st) {
   const int64_t blocks_each = std::max<int64_t>(8, 8 * sm_count() / batch);
   const int parts = (int)std::min<int64_t>(std::min<int64_t>(kNormBlocks, blocks_each), (m * n + 2047) / 2048);
-  if (!launch_pdl(ortho_norm_kernel<T>, dim3(parts, (unsigned)batch), 256, 0, st, (const T*)g, sums, m * n)) return false;
+  constexpr int kVec = 16 / sizeof(T);
+  const bool wide = m * n % kVec == 0 && ((uintptr_t)g & 15) == 0;
+  if (!launch_pdl(wide ? ortho_norm_kernel<T, kVec> : ortho_norm_kernel<T, 1>, dim3(parts, (unsigned)batch), 256, 0, st, (const T*)g, sums, m * n)) return false;
   const int64_t blocks = std::min<int64_t>((m * ld / 8 + 255) / 256, std::max<int64_t>(1, 8 * sm_count() / batch));
   return launch_pdl(ortho_split_kernel<T>, dim3((unsigned)blocks, (unsigned)batch), 256, 0, st, (const T*)g, (const double*)sums, planes, m, n, ld, parts, eps);
 }
