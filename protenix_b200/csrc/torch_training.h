@@ -373,7 +373,6 @@ struct HeadLossFunction : torch::autograd::Function<HeadLossFunction> {
     ctx->saved_data["ignore"] = ignore;
     ctx->saved_data["smoothing"] = smoothing;
     ctx->saved_data["reduction"] = reduction;
-    ctx->saved_data["f"] = (int64_t)x_.requires_grad() | (int64_t)w_.requires_grad() << 1 | (int64_t)(has(bias_) && bias_->requires_grad()) << 2;
     return loss;
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
@@ -381,14 +380,16 @@ struct HeadLossFunction : torch::autograd::Function<HeadLossFunction> {
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &w = saved[1], &bias = saved[2], &target = saved[3], &norm = saved[4], &inverse = saved[5];
     c10::cuda::CUDAGuard guard(x.device());
-    const int64_t f = ctx->saved_data["f"].toInt(), reduction = ctx->saved_data["reduction"].toInt();
+    const int64_t reduction = ctx->saved_data["reduction"].toInt();
+    // of the tensors in their order; without a bias the third is the target, which never does
+    const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1), want_b = ctx->needs_input_grad(2);
     const px_head h = head_of(x, w, bias, target, {ctx->saved_data["ignore"].toInt(), ctx->saved_data["smoothing"].toDouble(), reduction});
     const Tensor g = grads[0].to(at::kFloat).contiguous();
     Tensor dx, dw, db;
-    if (f & 1) dx = at::empty({h.rows, h.c}, x.options());
-    if (f & 2) dw = at::empty({h.classes, h.c}, w.options());
-    if (f & 4) db = at::empty({h.classes}, bias.options());
-    const int64_t bytes = abi.px_head_loss_bwd_workspace_bytes(&h, f & 1, f >> 1 & 1, f >> 2 & 1);
+    if (want_x) dx = at::empty({h.rows, h.c}, x.options());
+    if (want_w) dw = at::empty({h.classes, h.c}, w.options());
+    if (want_b) db = at::empty({h.classes}, bias.options());
+    const int64_t bytes = abi.px_head_loss_bwd_workspace_bytes(&h, want_x, want_w, want_b);
     const Tensor ws = bytes_like(x, bytes);
     const cudaStream_t st = at::cuda::getCurrentCUDAStream();
     launch("px_head_loss_bwd", st, [&] {
@@ -489,16 +490,15 @@ struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
     ctx->saved_data["strides"] = c10::List<int64_t>(c10::ArrayRef<int64_t>(strides));
     ctx->saved_data["base"] = base;
     ctx->saved_data["how"] = (int64_t)interleaved | (int64_t)per_axis << 1 | (int64_t)inverse << 2;
-    ctx->saved_data["f"] = (int64_t)q.requires_grad() | (int64_t)(has(k) && k->requires_grad()) << 1;
     if (out.second.defined()) return {out.first, out.second};
     return {out.first};
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
-    const int64_t f = ctx->saved_data["f"].toInt(), how = ctx->saved_data["how"].toInt();
+    const int64_t how = ctx->saved_data["how"].toInt();
     const Tensor positions = ctx->get_saved_variables()[0];
     const auto st = ctx->saved_data["strides"].toIntVector();
     const RotaryCall c = {ctx->saved_data["sections"].toIntVector(), ctx->saved_data["base"].toDouble(), (how & 1) != 0, (how & 2) != 0, (how & 4) == 0, st[0], st[1], st[2]};
-    const Tensor gq = f & 1 ? grads[0] : Tensor(), gk = f & 2 && grads.size() > 1 ? grads[1] : Tensor();
+    const Tensor gq = ctx->needs_input_grad(0) ? grads[0] : Tensor(), gk = grads.size() > 1 && ctx->needs_input_grad(1) ? grads[1] : Tensor();
     Tensor dq, dk;      // the operator again, by the negated angles: differentiable like it
     if (gq.defined() && gk.defined())
       std::tie(dq, dk) = rotary_apply(gq, gk, positions, c);

@@ -115,6 +115,23 @@ def test_more_classes_than_a_piece(dtype):
     _grad_close("dw", grads[1], want, dtype, 64)
 
 
+@pytest.mark.parametrize("rows,v", [(2048, 19990), (19990, 2048)])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_a_last_round_of_few_tiles(rows, v, dtype):
+    """79 tiles of 256 x 256 for dW, or for dx: two rounds, or parts of them."""
+    x, w, b, t = _inputs(rows, 248, v, dtype, torch.float32, seed=6)
+    loss = px.linear_cross_entropy(x, w, t, b, reduction="sum")
+    grads = torch.autograd.grad(loss, (x, w, b))
+    want = _formula(x, w, b, t, weight=torch.ones(rows, device="cuda"))
+    for name, got in zip(("dx", "dw"), grads):
+        _grad_close(name, got, want, dtype, 248)
+    bound = 2.0 ** -23 * ((248 / 16 + 24) * 40 + 64) * want["db_most"]
+    assert bool(((grads[2].double() - want["db"]).abs() <= bound + 1e-30).all())
+    assert not bool(grads[0][t == -100].any())
+    again = torch.autograd.grad(px.linear_cross_entropy(x, w, t, b, reduction="sum"), (x, w, b))
+    assert all(torch.equal(y, z) for y, z in zip(grads, again))
+
+
 @pytest.mark.parametrize("rows,c,v", [(200, 64, 50), (200, 136, 700)])
 @pytest.mark.parametrize("hold", [math.nan, math.inf, -math.inf])
 def test_ignored_rows_have_no_influence(rows, c, v, hold):
@@ -332,6 +349,21 @@ def test_gradients_of_some_inputs():
         loss.backward()
         for y, f in zip(leaves, full):
             assert torch.equal(y.grad, f) if y.requires_grad else y.grad is None
+
+
+@pytest.mark.parametrize("v", [90, 300])
+@pytest.mark.parametrize("bias", [None, torch.float32])
+def test_some_of_the_gradients(v, bias):
+    """All inputs are leaves, and a call asks for some of their gradients."""
+    x, w, b, t = _inputs(150, 136, v, BF16, bias)
+    leaves = [y for y in (x, w, b) if y is not None]
+    loss = px.linear_cross_entropy(x, w, t, bias=b)
+    full = torch.autograd.grad(loss, leaves, retain_graph=True)
+    for which in range(1, 1 << len(leaves)):
+        some = [i for i in range(len(leaves)) if which >> i & 1]
+        for i, g in zip(some, torch.autograd.grad(loss, [leaves[i] for i in some], retain_graph=True)):
+            # db alone is added up by a kernel of its own, in another order
+            assert torch.equal(g, full[i]) if i < 2 else torch.allclose(g, full[i], rtol=0, atol=2.0 ** -20 * float(full[i].abs().max()))
 
 
 @pytest.mark.parametrize("v,smooth", [(24, 0.0), (700, 0.1)])

@@ -160,6 +160,14 @@ def test_gradients():
     assert torch.autograd.grad(only[0].sum(), q)[0].shape == q.shape
 
 
+def test_one_of_two_gradients():
+    q, k = (torch.randn(2, 3, 50, 32, device="cuda", requires_grad=True) for _ in range(2))
+    out = px.rotary_embedding(q, k, torch.arange(50, device="cuda")[:, None])
+    full = torch.autograd.grad(out, (q, k), out, retain_graph=True)
+    assert torch.equal(torch.autograd.grad(out, q, out, retain_graph=True)[0], full[0])
+    assert torch.equal(torch.autograd.grad(out, k, out, retain_graph=True)[0], full[1])
+
+
 def test_offsets_beyond_32_bits():
     """Rows that begin beyond 2^31 elements of q, and beyond 2^32 bytes."""
     n, h, d = 2 ** 31 // (16 * 128) + 700, 16, 128
