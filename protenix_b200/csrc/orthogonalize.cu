@@ -110,6 +110,29 @@ __global__ void __launch_bounds__(256) ortho_split_kernel(const T* __restrict__ 
     planes[(2 * z + 1) * all + i] = lo;
   }
 }
+// The planes of A from the sums over parts of the long side, fp32 [matrix][part][s][ld]; eight columns a thread.
+__global__ void __launch_bounds__(256) ortho_gram_kernel(const float* __restrict__ parts, uint4* __restrict__ planes, int s, int ld, int splits) {
+  pdl_wait();
+  const int64_t z = blockIdx.y, all = (int64_t)s * ld / 8;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+    const float* const p = parts + z * splits * s * ld + 8 * i;
+    float v[8] = {};
+#pragma unroll 4
+    for (int k = 0; k < splits; ++k) {
+      const float4 a = *reinterpret_cast<const float4*>(p + (int64_t)k * s * ld), b = *reinterpret_cast<const float4*>(p + (int64_t)k * s * ld + 4);
+      v[0] += a.x, v[1] += a.y, v[2] += a.z, v[3] += a.w, v[4] += b.x, v[5] += b.y, v[6] += b.z, v[7] += b.w;
+    }
+    const int col = (int)(8 * i % ld);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (col + j >= s) v[j] = 0.f;                        // nothing was stored there
+    uint4 hi, lo;
+    split_planes2(v[0], v[1], hi.x, lo.x), split_planes2(v[2], v[3], hi.y, lo.y);
+    split_planes2(v[4], v[5], hi.z, lo.z), split_planes2(v[6], v[7], hi.w, lo.w);
+    planes[2 * z * all + i] = hi;
+    planes[(2 * z + 1) * all + i] = lo;
+  }
+}
 // The other way, for results whose rows TMA cannot store.
 template <typename T>
 __global__ void __launch_bounds__(256) ortho_join_kernel(const __half* __restrict__ planes, T* __restrict__ out, int64_t m, int64_t n, int64_t ld) {
@@ -319,7 +342,7 @@ plane_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
           const uint32_t bar = kPair ? map_to_rank(smem_u32(&bars.full[s]), 0) : 0;
           auto load = [&](uint32_t dst, const CUtensorMap* map, bool across, int from, int z) {
             for (int j = 0; j < (across ? 2 : 1); ++j) {
-              const int x = across ? from + 64 * j : kt * kGemmK, y = across ? kt * kGemmK : from;
+              const int x = across ? from + 64 * j : (t.k0 + kt) * kGemmK, y = across ? (t.k0 + kt) * kGemmK : from;
               if constexpr (kPair)
                 tma_load_3d_pair(dst + 8192 * j, map, bar, x, y, z);
               else
@@ -433,7 +456,7 @@ plane_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
       if (m0 < end.rows) {
 #pragma unroll
         for (int c = 0; c < S::kCols; c += 32)
-          if (n0 + c < end.cols) end.block(&sum[c], m0, n0 + c, t.z, end.symmetric && t.mt != t.nt, stg, lane);
+          if (n0 + c < end.cols) end.block(&sum[c], m0, n0 + c, t.z * tiles.splits + t.split, end.symmetric && t.mt != t.nt, stg, lane);
       }
     }
     if (lane == 0) tma_store_wait_read<0>();
@@ -477,11 +500,11 @@ struct Planes {
   }
 };
 template <class S>
-static int32_t launch_planes(const CUtensorMap& ma, const CUtensorMap& mb, OrthoEnd end, GemmTiles t, int64_t m, int64_t n, int64_t k, cudaStream_t st) {
-  const int chunk = end.type == PX_F32 ? 1 : end.type == PX_F16 ? 2 : 8;
+static int32_t launch_planes(const CUtensorMap& ma, const CUtensorMap& mb, OrthoEnd end, GemmTiles t, int64_t m, int64_t n, int64_t k, int dtype, cudaStream_t st) {
+  const int chunk = dtype == PX_F32 ? 1 : dtype == PX_F16 ? 2 : 8;
   end.factor *= uncut(k, chunk);
   t.tiles_m = (int)(ortho_up(m, S::kSide) / S::kSide), t.tiles_n = (int)(ortho_up(n, S::kSide) / S::kSide);
-  const int64_t total = t.batch * (t.symmetric ? (int64_t)t.tiles_m * (t.tiles_m + 1) / 2 : (int64_t)t.tiles_m * t.tiles_n);
+  const int64_t total = (int64_t)t.batch * t.splits * (t.symmetric ? (int64_t)t.tiles_m * (t.tiles_m + 1) / 2 : (int64_t)t.tiles_m * t.tiles_n);
   if (total > 0x7fffffff) return PX_ERR_UNSUPPORTED;
   t.total = (int)total;
   static SmemLimit limit;
@@ -503,7 +526,7 @@ static int32_t launch_planes(const CUtensorMap& ma, const CUtensorMap& mb, Ortho
   return PX_ERR_LAUNCH;
 }
 template <bool kAMn, bool kBMn>
-static int32_t ortho_product(const Planes& a, const Planes& b, int64_t batch, int64_t m, int64_t n, int64_t k, const OrthoEnd& end, cudaStream_t st) {
+static int32_t ortho_product(const Planes& a, const Planes& b, int64_t batch, int64_t m, int64_t n, int64_t k, const OrthoEnd& end, int dtype, cudaStream_t st) {
   const CUtensorMap &ma = kAMn ? a.across : a.along, &mb = kBMn ? b.across : b.along;
   GemmTiles t = {};
   t.batch = (int)batch, t.splits = 1, t.group = 8, t.symmetric = end.symmetric;
@@ -514,12 +537,22 @@ static int32_t ortho_product(const Planes& a, const Planes& b, int64_t batch, in
     const int64_t tm = ortho_up(m, side) / side, tn = ortho_up(n, side) / side, tiles = batch * (end.symmetric ? tm * (tm + 1) / 2 : tm * tn);
     return (tiles + room - 1) / room * (t.nk * stage + epilogue);
   };
-  if (cycles(256, sm_count() / 2, end.type == PX_F32 ? 2200 : 1500, 9000) < cycles(128, sm_count(), 1500, 6000)) return launch_planes<PlaneShape<2, kAMn, kBMn>>(ma, mb, end, t, m, n, k, st);
-  return launch_planes<PlaneShape<1, kAMn, kBMn>>(ma, mb, end, t, m, n, k, st);
+  if (cycles(256, sm_count() / 2, dtype == PX_F32 ? 2200 : 1500, 9000) < cycles(128, sm_count(), 1500, 6000)) return launch_planes<PlaneShape<2, kAMn, kBMn>>(ma, mb, end, t, m, n, k, dtype, st);
+  return launch_planes<PlaneShape<1, kAMn, kBMn>>(ma, mb, end, t, m, n, k, dtype, st);
+}
+
+// Parts that the long side is cut into where A has few tiles: as many as the SMs take at once, of two stages at least, if they and the kernel that adds them up
+// (some 10000 cycles) are the faster.  Parts of all of A: it is not worth it to store two ways what is added up afterwards.
+static int gram_splits(int64_t batch, int64_t s, int64_t length) {
+  const int64_t side = (s + 127) / 128, tiles = batch * side * side, nk = (length + kGemmK - 1) / kGemmK, most = std::min<int64_t>(sm_count() / tiles, nk / 2);
+  if (most < 2) return 1;
+  const int64_t part = (nk + most - 1) / most, splits = (nk + part - 1) / part;
+  return part * 1500 + 10000 + splits * batch * s * s / 400 < nk * 1500 ? (int)splits : 1;
 }
 
 struct OrthoPlan {
-  int64_t ld, s, lds, sums, x[2], gram, poly, bytes;
+  int64_t ld, s, lds, sums, x[2], gram, poly, parts, bytes;
+  int splits;
 };
 static OrthoPlan ortho_plan(int64_t batch, int64_t m, int64_t n) {
   OrthoPlan p;
@@ -535,6 +568,8 @@ static OrthoPlan ortho_plan(int64_t batch, int64_t m, int64_t n) {
   for (int64_t& x : p.x) x = take(batch * 2 * m * p.ld * 2);
   p.gram = take(batch * 2 * p.s * p.lds * 2);
   p.poly = take(batch * 2 * p.s * p.lds * 2);
+  p.splits = gram_splits(batch, p.s, std::max(m, n));
+  p.parts = take(p.splits > 1 ? p.splits * batch * p.s * p.lds * 4 : 0);
   p.bytes = at;
   return p;
 }
@@ -601,10 +636,27 @@ extern "C" int32_t px_orthogonalize(const void* g, void* out, int64_t batch, int
     const Planes &x = planes[i & 1], &next = planes[1 - (i & 1)];
     OrthoEnd e = {};
     e.out = gram.out, e.factor = 1.f / kPlaneScale, e.rows = e.cols = (int)p.s, e.ld = (int)p.lds, e.symmetric = 1, e.type = dtype;
-    int32_t status = wide ? ortho_product<false, false>(x, x, batch, p.s, p.s, n, e, st) : ortho_product<true, true>(x, x, batch, p.s, p.s, m, e, st);
+    int32_t status;
+    if (p.splits > 1) {
+      OrthoEnd part = e;
+      part.symmetric = 0, part.result = 1, part.type = PX_F32;
+      if (!make_map_3d(&part.out, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, ws + p.parts, (uint64_t)p.s, (uint64_t)p.s, (uint64_t)(batch * p.splits), (uint64_t)p.lds * 4,
+                       (uint64_t)p.s * p.lds * 4, 32, 32, CU_TENSOR_MAP_SWIZZLE_128B))
+        return PX_ERR_LAUNCH;
+      GemmTiles t = {};
+      t.batch = (int)batch, t.splits = p.splits, t.group = 8, t.nk = (int)(ortho_up(std::max(m, n), kGemmK) / kGemmK);
+      t.nk_split = (t.nk + p.splits - 1) / p.splits;
+      status = wide ? launch_planes<PlaneShape<1, false, false>>(x.along, x.along, part, t, p.s, p.s, (int64_t)t.nk_split * kGemmK, dtype, st)
+                    : launch_planes<PlaneShape<1, true, true>>(x.across, x.across, part, t, p.s, p.s, (int64_t)t.nk_split * kGemmK, dtype, st);
+      const int64_t blocks = std::min<int64_t>((p.s * p.lds / 8 + 255) / 256, std::max<int64_t>(1, 8 * sm_count() / batch));
+      if (!status && !launch_pdl(ortho_gram_kernel, dim3((unsigned)blocks, (unsigned)batch), 256, 0, st, (const float*)(ws + p.parts), (uint4*)gram.at, (int)p.s, (int)p.lds, p.splits))
+        status = PX_ERR_LAUNCH;
+    } else {
+      status = wide ? ortho_product<false, false>(x, x, batch, p.s, p.s, n, e, dtype, st) : ortho_product<true, true>(x, x, batch, p.s, p.s, m, e, dtype, st);
+    }
     if (status) return status;
     e.out = poly.out, e.gram = gram.at, e.a = coefficients[3 * i], e.b = coefficients[3 * i + 1], e.factor = coefficients[3 * i + 2] / kPlaneScale;
-    status = ortho_product<false, false>(gram, gram, batch, p.s, p.s, p.s, e, st);
+    status = ortho_product<false, false>(gram, gram, batch, p.s, p.s, p.s, e, dtype, st);
     if (status) return status;
     e = {};
     e.out = next.out, e.factor = 1.f / kPlaneScale, e.rows = (int)m, e.cols = (int)n, e.type = dtype;
@@ -615,7 +667,7 @@ extern "C" int32_t px_orthogonalize(const void* g, void* out, int64_t batch, int
                        dtype == PX_F32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B))
         return PX_ERR_LAUNCH;
     }
-    status = wide ? ortho_product<false, true>(poly, x, batch, m, n, m, e, st) : ortho_product<false, false>(x, poly, batch, m, n, n, e, st);
+    status = wide ? ortho_product<false, true>(poly, x, batch, m, n, m, e, dtype, st) : ortho_product<false, false>(x, poly, batch, m, n, n, e, dtype, st);
     if (status) return status;
   }
   if (direct) return PX_OK;

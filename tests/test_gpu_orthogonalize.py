@@ -58,6 +58,19 @@ def test_against_64_bits(batch, m, n, dtype):
     _close(px.orthogonalize(g[batch - 1])[None], _iterated(g[batch - 1:]))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("batch,m,n", [(1, 256, 4096), (1, 4100, 200), (3, 1500, 140), (2, 129, 1025), (1, 77, 9000), (1, 9001, 131), (5, 300, 1500)])
+def test_long_sides(batch, m, n, dtype):
+    """The sum over the long side in parts."""
+    g = torch.randn(batch, m, n, device="cuda", generator=torch.Generator(device="cuda").manual_seed(m + n)).to(dtype)
+    got = px.orthogonalize(g)
+    ops.device_error_flags()
+    _close(got, _iterated(g))
+    assert torch.equal(got, px.orthogonalize(g))
+    g[0, 3, 5] = math.nan
+    assert bool(px.orthogonalize(g)[0].isnan().all())
+
+
 @pytest.mark.parametrize("m,n", [(2048, 2048), (3000, 700), (1100, 4100)])
 def test_large(m, n):
     """Tiles of pairs of CTAs, and whole rounds of them."""
