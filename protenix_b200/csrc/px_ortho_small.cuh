@@ -73,24 +73,27 @@ __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.w
 
 // A from its parts in the kCtas CTAs of a cluster: every row goes to the CTA that adds it up (row / kShare), which writes the planes of the sum to all of
 // them.  `sum`: this thread's row, columns 64 half ..; f: what A is multiplied by; the parts lie where A will be, part k from row k kShare on.
-template <int kCtas>
-__device__ __forceinline__ void exchange_gram(unsigned char* gram, int rank, int row, int half, const float (&sum)[64], float f) {
+// Rows and columns from `side` on (kAll: there are none) are left as they are: no sum takes them in, and no result that counts comes of them.
+template <int kCtas, bool kAll>
+__device__ __forceinline__ void exchange_gram(unsigned char* gram, int rank, int row, int half, const float (&sum)[64], float f, int side) {
   constexpr int kShare = 128 / kCtas, kGroups = 8 / kCtas;      // rows of a CTA; eight columns each of a thread
   cluster_wait();                                               // nobody multiplies by what lies there any more
-  {
+  if (kAll || row < side) {
     const int to = row / kShare, r = rank * kShare + row % kShare;
     const uint32_t there = map_to_rank(smem_u32(gram), to);
 #pragma unroll
     for (int k = 0; k < 16; ++k)
-      asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};\n" ::"r"(there + float_offset(r, 64 * half + 4 * k)), "f"(sum[4 * k]), "f"(sum[4 * k + 1]),
+      if (kAll || 64 * half + 4 * k < side) asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};\n" ::"r"(there + float_offset(r, 64 * half + 4 * k)), "f"(sum[4 * k]), "f"(sum[4 * k + 1]),
                    "f"(sum[4 * k + 2]), "f"(sum[4 * k + 3])
                    : "memory");
   }
+  __syncwarp();
   tc_cluster_sync();
   uint4 hi[kGroups], lo[kGroups];
 #pragma unroll
   for (int i = 0; i < kGroups; ++i) {
     const int at = threadIdx.x + kSmallOrthoThreads * i, r = at >> 4, piece = at & 15;
+    if (!kAll && (rank * kShare + r >= side || 8 * piece >= side)) continue;
     float v[8] = {};
 #pragma unroll
     for (int k = 0; k < kCtas; ++k) {
@@ -103,10 +106,12 @@ __device__ __forceinline__ void exchange_gram(unsigned char* gram, int rank, int
     split_planes2(f * v[0], f * v[1], hi[i].x, lo[i].x), split_planes2(f * v[2], f * v[3], hi[i].y, lo[i].y);
     split_planes2(f * v[4], f * v[5], hi[i].z, lo[i].z), split_planes2(f * v[6], f * v[7], hi[i].w, lo[i].w);
   }
+  __syncwarp();
   tc_cluster_sync();                                            // all parts are read
 #pragma unroll
   for (int i = 0; i < kGroups; ++i) {
     const int at = threadIdx.x + kSmallOrthoThreads * i, r = rank * kShare + (at >> 4), piece = at & 15;
+    if (!kAll && (r >= side || 8 * piece >= side)) continue;
     const uint32_t to = smem_u32(gram + plane_offset(r, piece));
 #pragma unroll
     for (int k = 0; k < kCtas; ++k) {
@@ -116,10 +121,11 @@ __device__ __forceinline__ void exchange_gram(unsigned char* gram, int rank, int
     }
   }
   asm volatile("fence.proxy.async;\n" ::: "memory");
+  __syncwarp();
   tc_cluster_sync();
 }
 
-template <int kSlices, bool kTall>
+template <int kSlices, bool kTall, bool kShort>
 __global__ void __launch_bounds__(kSmallOrthoThreads + 32, 1) small_ortho_kernel(const __grid_constant__ SmallOrtho p) {
   typedef SmallOrthoShape<kSlices> S;
   constexpr float kScale = kPlaneScale;
@@ -157,6 +163,9 @@ __global__ void __launch_bounds__(kSmallOrthoThreads + 32, 1) small_ortho_kernel
   const uint32_t tmem = bars.tmem_base;
 
   constexpr uint32_t idesc_kk = umma_idesc_f16(128, 128), idesc_kn = umma_idesc_f16(128, 128, false, true);
+  // Steps of 16 k that hold anything, of sums over the short side and of A's (kShort: the side is 112 or less): 48 x 16 x 16 take 29 us with them alone, 35 with
+  // all, 4 x 20 x 500 52 and 73.  Counts that the compiler does not know cost 128 x 128 2 of 37 us.
+  const int side_steps = kShort ? (p.side + 15) / 16 : 8, gram_steps = kShort && kSlices == 1 && p.ctas == 1 ? (p.length + 15) / 16 : 8 * kSlices;
   constexpr uint64_t kLo = kSmallPlane >> 4, kPanel = kSmallPlane >> 5;
   unsigned char* const gram = sm + S::kA;
   // Before a product all threads meet: its operands are in shared memory, and the accumulators have been read.
@@ -188,11 +197,12 @@ __global__ void __launch_bounds__(kSmallOrthoThreads + 32, 1) small_ortho_kernel
           [&] {
 #pragma unroll
             for (int ks = 0; ks < 8; ++ks)
-              umma_bf16(tmem + 128 * (ks >> 2), u + (ks >> 2) * kPanel + 2 * (ks & 3), w + (across ? 128 * ks : (ks >> 2) * kPanel + 2 * (ks & 3)), idesc, (ks & 3) ? 1u : 0u);
+              if (ks < side_steps) umma_bf16(tmem + 128 * (ks >> 2), u + (ks >> 2) * kPanel + 2 * (ks & 3), w + (across ? 128 * ks : (ks >> 2) * kPanel + 2 * (ks & 3)), idesc, (ks & 3) ? 1u : 0u);
           },
           [&] {
 #pragma unroll
             for (int ks = 0; ks < 8; ++ks) {
+              if (ks >= side_steps) break;
               const uint64_t x = u + (ks >> 2) * kPanel + 2 * (ks & 3), y = w + (across ? 128 * ks : (ks >> 2) * kPanel + 2 * (ks & 3));
               umma_bf16(tmem + 256, x, y + kLo, idesc, ks ? 1u : 0u);
               umma_bf16(tmem + 256, x + kLo, y, idesc, 1u);
@@ -212,7 +222,8 @@ __global__ void __launch_bounds__(kSmallOrthoThreads + 32, 1) small_ortho_kernel
         for (int n = 0; n < 2; ++n) {
           const uint64_t x = slice_at(2 * slice + n);
 #pragma unroll
-          for (int ks = 0; ks < 4; ++ks) umma_bf16(tmem + 128 * n, x + 2 * ks, x + 2 * ks, idesc_kk, ks ? 1u : 0u);
+          for (int ks = 0; ks < 4; ++ks)
+            if (8 * slice + 4 * n + ks < gram_steps) umma_bf16(tmem + 128 * n, x + 2 * ks, x + 2 * ks, idesc_kk, ks ? 1u : 0u);
         }
       };
       meet();
@@ -225,6 +236,7 @@ __global__ void __launch_bounds__(kSmallOrthoThreads + 32, 1) small_ortho_kernel
           const uint64_t x = slice_at(n);
 #pragma unroll
           for (int ks = 0; ks < 4; ++ks) {
+            if (4 * n + ks >= gram_steps) break;
             umma_bf16(tmem + 256, x + 2 * ks, x + kLo + 2 * ks, idesc_kk, (n | ks) ? 1u : 0u);
             umma_bf16(tmem + 256, x + kLo + 2 * ks, x + 2 * ks, idesc_kk, 1u);
           }
@@ -348,7 +360,7 @@ __global__ void __launch_bounds__(kSmallOrthoThreads + 32, 1) small_ortho_kernel
     const uint32_t lanes = tmem + ((uint32_t)(32 * q) << 16) + 64 * half;
     const int row = 32 * q + lane;
     // Where a wait gives up the work goes on, on values that the flag has declared void: the barriers of the cluster want everybody.
-    auto leading = [&](bool first) {
+    auto leading = [&](bool first, bool both) {
 #pragma unroll
       for (int c = 0; c < 64; c += 32) {
         uint32_t a[32], b[32];
@@ -357,18 +369,18 @@ __global__ void __launch_bounds__(kSmallOrthoThreads + 32, 1) small_ortho_kernel
         tmem_wait_ld();
 #pragma unroll
         for (int j = 0; j < 32; ++j) {
-          const float s = __uint_as_float(a[j]) + __uint_as_float(b[j]);
+          const float s = both ? __uint_as_float(a[j]) + __uint_as_float(b[j]) : __uint_as_float(a[j]);      // or nothing was added up there
           sum[c + j] = first ? s : sum[c + j] + s;
         }
       }
     };
-    auto product = [&](bool two) {
+    auto product = [&](bool two, int steps) {
       meet();
       // the leading accumulators are added up while the other products run
       mbar_wait(&bars.lead, parity, 1u);
       __syncwarp();
       tc_fence_after();
-      leading(true);
+      leading(true, steps > 4);
       if (two) {
         tc_fence_before();
         __syncwarp();
@@ -378,7 +390,7 @@ __global__ void __launch_bounds__(kSmallOrthoThreads + 32, 1) small_ortho_kernel
       __syncwarp();
       parity ^= 1;
       tc_fence_after();
-      if (two) leading(false);
+      if (two) leading(false, true);
 #pragma unroll
       for (int c = 0; c < 64; c += 32) {
         uint32_t a[32];
@@ -408,34 +420,42 @@ __global__ void __launch_bounds__(kSmallOrthoThreads + 32, 1) small_ortho_kernel
     if (p.ctas > 1) cluster_arrive();
     for (int step = 0; step < p.steps; ++step) {
       // A
-      product(kSlices == 2);
+      product(kSlices == 2, gram_steps);
       if (p.ctas == 1) {
         put(gram, uncut_gram / kScale);
       } else {
+        const int live = 16 * side_steps;
         if (p.ctas == 2) {
           // each sends its whole part to the other, and both add up
-          cluster_wait();                                  // the other does not multiply by what lies there any more
+          cluster_wait();                                // the other does not multiply by what lies there any more
           const uint32_t there = map_to_rank(smem_u32(gram), rank ^ 1);
 #pragma unroll
           for (int k = 0; k < 16; ++k)
-            asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};\n" ::"r"(there + float_offset(row, 64 * half + 4 * k)), "f"(sum[4 * k]), "f"(sum[4 * k + 1]),
-                         "f"(sum[4 * k + 2]), "f"(sum[4 * k + 3])
-                         : "memory");
+            if (!kShort || (row < live && 64 * half + 4 * k < live))
+              asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};\n" ::"r"(there + float_offset(row, 64 * half + 4 * k)), "f"(sum[4 * k]), "f"(sum[4 * k + 1]),
+                           "f"(sum[4 * k + 2]), "f"(sum[4 * k + 3])
+                           : "memory");
+          __syncwarp();
           tc_cluster_sync();
 #pragma unroll
           for (int k = 0; k < 16; ++k) {
+            if (kShort && (row >= live || 64 * half + 4 * k >= live)) break;
             const float4 x = *reinterpret_cast<const float4*>(gram + float_offset(row, 64 * half + 4 * k));
             sum[4 * k] += x.x, sum[4 * k + 1] += x.y, sum[4 * k + 2] += x.z, sum[4 * k + 3] += x.w;
           }
+          __syncwarp();
           asm volatile("bar.sync 1, %0;\n" ::"n"(kSmallOrthoThreads) : "memory");
           put(gram, uncut_gram / kScale);
-        } else if (p.ctas == 4) exchange_gram<4>(gram, rank, row, half, sum, uncut_gram / kScale);
-        else exchange_gram<8>(gram, rank, row, half, sum, uncut_gram / kScale);
+        } else if (p.ctas == 4) {
+          exchange_gram<4, !kShort>(gram, rank, row, half, sum, uncut_gram / kScale, live);
+        } else {
+          exchange_gram<8, !kShort>(gram, rank, row, half, sum, uncut_gram / kScale, live);
+        }
       }
 
       // the polynomial, in the place of A
       const float a = p.abc[3 * step], b = p.abc[3 * step + 1], c2 = p.abc[3 * step + 2] * (uncut_side / kScale);
-      product(false);
+      product(false, side_steps);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const unsigned char* const x = gram + plane_offset(row, 8 * half + k);
@@ -464,7 +484,7 @@ __global__ void __launch_bounds__(kSmallOrthoThreads + 32, 1) small_ortho_kernel
 #pragma unroll 1
       for (int n = 0; n < kSlices; ++n) {
         unsigned char* const slice = sm + S::kX + n * 2 * kSmallPlane;
-        product(false);
+        product(false, side_steps);
         if (last) put_floats(slice, uncut_side / (kScale * kScale));
         else put(slice, uncut_side / kScale);
       }
@@ -521,11 +541,11 @@ __global__ void __launch_bounds__(kSmallOrthoThreads + 32, 1) small_ortho_kernel
   }
 }
 
-template <int kSlices, bool kTall>
+template <int kSlices, bool kTall, bool kShort>
 static bool launch_small_ortho(const SmallOrtho& p, int64_t batch, cudaStream_t st) {
   typedef SmallOrthoShape<kSlices> S;
   static SmemLimit limit;
-  if (!limit.set(small_ortho_kernel<kSlices, kTall>, S::kSmem)) return false;
+  if (!limit.set(small_ortho_kernel<kSlices, kTall, kShort>, S::kSmem)) return false;
   cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
@@ -538,7 +558,7 @@ static bool launch_small_ortho(const SmallOrtho& p, int64_t batch, cudaStream_t 
   cfg.stream = st;
   cfg.attrs = at;
   cfg.numAttrs = p.ctas > 1 ? 2 : 1;
-  if (cudaLaunchKernelEx(&cfg, small_ortho_kernel<kSlices, kTall>, p) == cudaSuccess) return true;
+  if (cudaLaunchKernelEx(&cfg, small_ortho_kernel<kSlices, kTall, kShort>, p) == cudaSuccess) return true;
   cudaGetLastError();
   return false;
 }
@@ -564,9 +584,13 @@ static inline int small_ortho_ctas(int64_t batch, int64_t side, int64_t length, 
   }
   return ctas;
 }
+template <bool kShort>
 static bool launch_small_ortho(const SmallOrtho& p, int64_t batch, int slices, bool tall, cudaStream_t st) {
-  if (slices == 1) return tall ? launch_small_ortho<1, true>(p, batch, st) : launch_small_ortho<1, false>(p, batch, st);
-  return tall ? launch_small_ortho<2, true>(p, batch, st) : launch_small_ortho<2, false>(p, batch, st);
+  if (slices == 1) return tall ? launch_small_ortho<1, true, kShort>(p, batch, st) : launch_small_ortho<1, false, kShort>(p, batch, st);
+  return tall ? launch_small_ortho<2, true, kShort>(p, batch, st) : launch_small_ortho<2, false, kShort>(p, batch, st);
+}
+static bool launch_small_ortho(const SmallOrtho& p, int64_t batch, int slices, bool tall, cudaStream_t st) {
+  return p.side <= 112 ? launch_small_ortho<true>(p, batch, slices, tall, st) : launch_small_ortho<false>(p, batch, slices, tall, st);
 }
 
 }  // namespace px
