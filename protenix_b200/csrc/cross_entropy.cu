@@ -613,7 +613,7 @@ static bool small_args(SmallArgs* a, const px_head& h) {
     return false;
   a->dx = a->x;
   a->target = h.target, a->bias = {h.bias, h.bias_dtype}, a->ignore = h.ignore, a->rows = (int)h.rows, a->classes = (int)h.classes;
-  a->panels = (int)(up(h.c, 64) / 64), a->tiles = (int)(up(h.rows, 128) / 128), a->f16 = f16, a->smooth = h.smoothing, a->uncut = uncut_logits(h.c);
+  a->panels = (int)(up(h.c, 64) / 64), a->tiles = (int)(up(h.rows, 128) / 128), a->f16 = f16, a->smooth = h.smoothing, a->uncut = uncut_logits(h.c, h.dtype == PX_F16);
   a->idesc_logits = umma_idesc_16(128, vp, f16, f16);
   a->idesc_dx = umma_idesc_16(128, 64 * a->panels, f16, f16, false, true);
   a->idesc_dw = umma_idesc_16(128, vp, f16, f16, true, true);
@@ -678,7 +678,7 @@ extern "C" int32_t px_head_loss_fwd(const px_head* head, float* norm, float* los
   float2* part = (float2*)at;
   at += up(c.t.tiles_n * h.rows * 8, 1024);
   uint32_t* const dirty = (uint32_t*)(norm + 2 * h.rows);
-  EpiStats epi = {h.target, {h.bias, h.bias_dtype}, part, h.smoothing > 0.f ? (float*)at : nullptr, hit, arrivals, dirty, (int)h.rows, (int)h.classes, uncut_logits(h.c)};
+  EpiStats epi = {h.target, {h.bias, h.bias_dtype}, part, h.smoothing > 0.f ? (float*)at : nullptr, hit, arrivals, dirty, (int)h.rows, (int)h.classes, uncut_logits(h.c, h.dtype == PX_F16)};
   if (const int32_t status = launch_logits(h, 0, h.classes, c, epi, st)) return status;
   JoinArgs j = {part, epi.part_sum, hit, h.target, (float2*)norm, losses, total, inverse, sums, arrivals, dirty, h.ignore, (int)h.rows, (int)h.classes, c.t.tiles_n, mean, h.smoothing};
   return launch_pdl(loss_join_kernel, dim3((unsigned)((h.rows + 31) / 32)), 32 * kJoinWarps, 0, st, j) ? PX_OK : PX_ERR_LAUNCH;
@@ -743,7 +743,7 @@ extern "C" int32_t px_head_loss_bwd(const px_head* head, const float* norm, cons
     el.target = h.target, el.bias = {h.bias ? (const char*)h.bias + first * bias_size : nullptr, h.bias_dtype}, el.norm = (const float2*)norm, el.grad = each ? grad : nullptr, el.scale = out.scale;
     if (dw && i == 0) el.x = (const uint16_t*)h.x, el.x_stride = h.x_stride, el.c = (int)h.c, el.clean = clean, el.dirty = dirty;
     el.part_bias = dbias ? part_bias : nullptr, el.ignore = h.ignore, el.rows = (int)h.rows, el.classes = (int)vc, el.first = (int)first;
-    el.all_classes = (int)h.classes, el.smooth = h.smoothing, el.uncut = uncut_logits(h.c), el.f16 = f16;
+    el.all_classes = (int)h.classes, el.smooth = h.smoothing, el.uncut = uncut_logits(h.c, h.dtype == PX_F16), el.f16 = f16;
     if (const int32_t status = launch_logits(h, first, vc, p.logits, el, st)) return status;
     void* const db = dbias ? (char*)dbias + first * bias_size : nullptr;
     const bool bias_apart = dbias && (!dw || bias_groups > kBiasGroups);

@@ -37,10 +37,11 @@ __device__ __forceinline__ float row_loss(float sum, float ref, float hit, bool 
   return loss < 0.f ? 0.f : loss * 0.6931471805599453f;
 }
 
-// The tensor core cuts an accumulator after each 16 channels, towards zero, by half a step on average: a logit is too small by 2.9e-8 (c / 16 + 1) of itself in the mean,
-// whatever the signs of its terms (what is cut off is in proportion to the sum so far, and that on average to the sum).  This puts it back: the losses of
-// a few rows with 2048 channels were off by 3e-6 of themselves without, those of plain fp32 products by less than 1e-7.
-static inline float uncut_logits(int64_t c) { return 1.f + 2.9e-8f * (float)((c + 15) / 16 + 1); }
+// The tensor core cuts an accumulator after each 16 channels, and what it aligns to it, towards zero.  A logit that grows with its terms comes out too small, in
+// the mean by 1.6e-8 (c / 16 + 1) of itself in bf16 and 2.8e-8 in fp16, whose products are longer (rows that lean towards their class; three times that where
+// all terms are of one sign).  This puts it back: losses of rows by themselves, 256 to 2048 channels, are off by 1e-7 to 5e-7 of their norm in bf16 (with 2.9e-8 by 1.4e-7 to 1.3e-6),
+// 1.4e-7 to 9e-7 in fp16; with 2048 channels 3e-6 without.  Plain fp32 products: 1e-7.
+static inline float uncut_logits(int64_t c, bool f16) { return 1.f + (f16 ? 2.8e-8f : 1.6e-8f) * (float)((c + 15) / 16 + 1); }
 __device__ __forceinline__ void logits_of(const uint32_t (&r)[32], float uncut, float (&v)[32]) {
   const f32x2 u = pair2(uncut, uncut);
 #pragma unroll
