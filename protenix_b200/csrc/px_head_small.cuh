@@ -131,8 +131,8 @@ __global__ void __launch_bounds__(SmallShape<kBackward, kVp>::kThreads, 1) small
 #pragma unroll
           for (int ks = 0; ks < 4; ++ks) umma_bf16(tmem + b * kVp, da + 2 * ks, db + 2 * ks, a.idesc_logits, (p | ks) ? 1u : 0u);
         }
-        umma_commit(&bars.logit_full[b]);
         if (!kBackward) umma_commit(&bars.x_empty[s]);
+        umma_commit(&bars.logit_full[b]);              // last: what is waited for
       }
       __syncwarp();
     };
@@ -161,6 +161,9 @@ __global__ void __launch_bounds__(SmallShape<kBackward, kVp>::kThreads, 1) small
         __syncwarp();
       }
     }
+    // Nothing else waits for the last products of a backward pass that wants no dW: they write tensor memory and arrive on barriers, so this warp stays until
+    // they are through.
+    if (kBackward && ok && mine > 0) mbar_wait_warp(&bars.done, 0, 1024u);
   } else if (warp < 2 + 4 * S::kSets) {
     // rows of the softmax
     const int q = warp & 3, set = (warp - 2) >> 2;
