@@ -42,6 +42,10 @@ class Muon(torch.optim.Optimizer):
     For each parameter p [..., M, N] with gradient g: buf <- momentum buf + g, u = g + momentum buf (``nesterov``) or buf,
     p <- (1 - lr weight_decay) p - lr sqrt(max(1, M / N)) orthogonalize(u).  Parameters of one shape and type are orthogonalised in one call.  For weights
     with two axes or more; biases, norms and tables of embeddings want another optimiser beside it.  fp32, bf16 and fp16 CUDA parameters.
+
+    The momentum is fp32 whatever the parameter's type, in checkpoints too, and u, its orthogonalisation and the new weight are formed in fp32 and rounded
+    once, to the parameter.  What is below half a step of a 16-bit weight (2^-9 to 2^-8 of it in bf16), a small decay beside a small update for one, leaves no
+    trace in it: keep the parameters in fp32 and round them for the forward pass where that matters.
     """
 
     def __init__(self, params: Iterable[torch.Tensor], lr: float = 0.02, momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0,
@@ -69,18 +73,40 @@ class Muon(torch.optim.Optimizer):
                 if p.grad is not None:
                     if p.grad.is_sparse:
                         raise RuntimeError("Muon: sparse gradients are not supported")
+                    if p.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+                        raise RuntimeError(f"Muon: parameters are float32, bfloat16 or float16, got {p.dtype}")
                     sets.setdefault((p.shape, p.dtype, p.device), []).append(p)
             for (shape, dtype, device), params in sets.items():
-                grads = [p.grad for p in params]
-                for p in params:
-                    if "momentum_buffer" not in self.state[p]:
-                        self.state[p]["momentum_buffer"] = torch.zeros_like(p)
-                held = [self.state[p]["momentum_buffer"] for p in params]
+                wide = dtype == torch.float32
+                grads = [p.grad for p in params] if wide else list(torch.stack([p.grad for p in params]).float().unbind(0))
+                held = [self._momentum(p) for p in params]
                 torch._foreach_mul_(held, group["momentum"])
                 torch._foreach_add_(held, grads)
                 update = torch._foreach_add(grads, held, alpha=group["momentum"]) if group["nesterov"] else held
                 turned = orthogonalize(torch.stack(update), group["steps"], group["coefficients"], group["eps"])
-                if group["weight_decay"]:
-                    torch._foreach_mul_(params, 1.0 - group["lr"] * group["weight_decay"])
-                torch._foreach_add_(params, list(turned.unbind(0)), alpha=-group["lr"] * max(1.0, shape[-2] / max(shape[-1], 1)) ** 0.5)
+                keep, by = 1.0 - group["lr"] * group["weight_decay"], -group["lr"] * max(1.0, shape[-2] / max(shape[-1], 1)) ** 0.5
+                if wide:
+                    if group["weight_decay"]:
+                        torch._foreach_mul_(params, keep)
+                    torch._foreach_add_(params, list(turned.unbind(0)), alpha=by)
+                else:
+                    new = torch.stack(params).float().mul_(keep).add_(turned, alpha=by)
+                    torch._foreach_copy_(params, list(new.unbind(0)))
         return loss
+
+    def _momentum(self, p: torch.Tensor) -> torch.Tensor:
+        state = self.state[p]
+        if "momentum_buffer" not in state:
+            state["momentum_buffer"] = torch.zeros_like(p, dtype=torch.float32)
+        elif state["momentum_buffer"].dtype != torch.float32:
+            state["momentum_buffer"] = state["momentum_buffer"].float()
+        return state["momentum_buffer"]
+
+    def load_state_dict(self, state_dict) -> None:
+        """As that of any optimiser, which gives the state the parameters' types; the momentum of 16-bit ones is taken over in fp32."""
+        super().load_state_dict(state_dict)
+        ids = [i for group in state_dict["param_groups"] for i in group["params"]]
+        for i, p in zip(ids, (p for group in self.param_groups for p in group["params"])):
+            held = state_dict["state"].get(i, {}).get("momentum_buffer")
+            if held is not None and p.dtype != torch.float32:
+                self.state[p]["momentum_buffer"] = held.to(device=p.device, dtype=torch.float32, copy=True)
