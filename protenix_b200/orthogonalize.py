@@ -6,6 +6,7 @@ polynomial iteration (Newton-Schulz) needs products only; ``px_orthogonalize`` r
 """
 from __future__ import annotations
 
+import math
 from typing import Iterable, Optional, Sequence, Tuple, Union
 
 import torch
@@ -25,7 +26,7 @@ def orthogonalize(g: torch.Tensor, steps: int = 5, coefficients: Coefficients = 
 
     Products take operands of 22 bits and add in fp32 whatever the type: 16-bit iterates lose up to a third of the result where singular values differ
     much.  Iterates and polynomials of up to 60 are held; an overflow comes out infinite or NaN.  A matrix that is not finite gives NaN, a zero one zero (eps > 0).
-    Not differentiable: g is detached or no_grad is in force.
+    Up to 65535 matrices of 2^20 rows and columns.  Not differentiable: g is detached or no_grad is in force.
     """
     if not g.is_cuda:
         raise RuntimeError("orthogonalize: CUDA tensors only, this package has no CPU path")
@@ -41,7 +42,8 @@ class Muon(torch.optim.Optimizer):
 
     For each parameter p [..., M, N] with gradient g: buf <- momentum buf + g, u = g + momentum buf (``nesterov``) or buf,
     p <- (1 - lr weight_decay) p - lr sqrt(max(1, M / N)) orthogonalize(u).  Parameters of one shape and type are orthogonalised in one call.  For weights
-    with two axes or more; biases, norms and tables of embeddings want another optimiser beside it.  fp32, bf16 and fp16 CUDA parameters.
+    with two axes or more; biases, norms and tables of embeddings want another optimiser beside it.  fp32, bf16 and fp16 CUDA parameters, up to 65535 matrices
+    of a shape and type; a step that is refused has changed nothing.
 
     The momentum is fp32 whatever the parameter's type, in checkpoints too, and u, its orthogonalisation and the new weight are formed in fp32 and rounded
     once, to the parameter.  What is below half a step of a 16-bit weight (2^-9 to 2^-8 of it in bf16), a small decay beside a small update for one, leaves no
@@ -67,16 +69,9 @@ class Muon(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        for group in self.param_groups:
-            sets = {}
-            for p in group["params"]:
-                if p.grad is not None:
-                    if p.grad.is_sparse:
-                        raise RuntimeError("Muon: sparse gradients are not supported")
-                    if p.dtype not in (torch.float32, torch.bfloat16, torch.float16):
-                        raise RuntimeError(f"Muon: parameters are float32, bfloat16 or float16, got {p.dtype}")
-                    sets.setdefault((p.shape, p.dtype, p.device), []).append(p)
-            for (shape, dtype, device), params in sets.items():
+        # what is refused is refused before anything has changed
+        for group, sets in [(group, self._sets(group)) for group in self.param_groups]:
+            for (shape, dtype, _), params in sets.items():
                 wide = dtype == torch.float32
                 grads = [p.grad for p in params] if wide else list(torch.stack([p.grad for p in params]).float().unbind(0))
                 held = [self._momentum(p) for p in params]
@@ -93,6 +88,23 @@ class Muon(torch.optim.Optimizer):
                     new = torch.stack(params).float().mul_(keep).add_(turned, alpha=by)
                     torch._foreach_copy_(params, list(new.unbind(0)))
         return loss
+
+    @staticmethod
+    def _sets(group) -> dict:
+        """The parameters of a group that have a gradient, by shape, type and device."""
+        sets = {}
+        for p in group["params"]:
+            if p.grad is not None:
+                if p.grad.is_sparse:
+                    raise RuntimeError("Muon: sparse gradients are not supported")
+                if p.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+                    raise RuntimeError(f"Muon: parameters are float32, bfloat16 or float16, got {p.dtype}")
+                sets.setdefault((p.shape, p.dtype, p.device), []).append(p)
+        for (shape, _, device), params in sets.items():
+            if shape.numel() and len(params) * math.prod(shape[:-2]) > 65535:
+                raise RuntimeError(f"Muon: at most 65535 matrices of one shape, got {len(params)} parameters of {tuple(shape)}")
+            orthogonalize(torch.empty((0, *shape[-2:]), device=device), group["steps"], group["coefficients"], group["eps"])      # the checks alone
+        return sets
 
     def _momentum(self, p: torch.Tensor) -> torch.Tensor:
         state = self.state[p]
