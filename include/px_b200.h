@@ -454,7 +454,7 @@ PX_API int32_t px_window_bwd(const px_window* w, const px_rows* q, const px_rows
  * Pair j of a head of q [batch][heads][n][d] and k [batch][kv_heads][n][d] turns by positions[batch][row][axis of j] * base^-e: channels (j, j + pairs), or
  * (2 j, 2 j + 1) if interleaved, pairs = the sum of `sections` (the number of pairs of each axis, in their order, on the host), at most d / 2 and 256; the
  * channels behind them stay as they are.  e = j / pairs, or (per_axis) the pair's place in its section over the section's length.  inverse: by the negated angles
- * (the gradient).  Angles are exact modulo a turn for every int64 position; products are fp32, rounded once.  PX_F32, PX_BF16 or PX_F16; strides in elements, of
+ * (the gradient).  Angles are taken modulo a turn with 88 bits of the speed: off by 2^-31 of a turn up to positions of 2^57, by 2^-25 for any int64.  Products are fp32, rounded once.  PX_F32, PX_BF16 or PX_F16; strides in elements, of
  * outputs as of inputs (inputs may repeat rows by strides of zero); 16-byte accesses where strides, pointers and `pairs` allow them.  k NULL with kv_heads 0: q alone.
  * No counterpart in the reference, whose attention takes positions as a bias of pairs. */
 typedef struct {

@@ -1,10 +1,11 @@
 // Rotary positions of several axes: pair j of a head (two channels) turns by the angle position[axis of j] * base^-e_j,
 //   y = (u cos - v sin, v cos + u sin),   the gradient is the same with the angles negated.
 //
-// Memory bound: every element is read and written once, the angles are few.  Angles: a turn is 2^64, a pair's speed a 64-bit fraction of it, and
-// position * speed modulo 2^64 is exact for any position, where fp32 angles are off by 0.06 at position 10^6; its top 32 bits go to
-// sincospif.  A thread forms the sines of kVec pairs (16 bytes of each half) and uses them for all heads of its group; threads beside one another take
-// neighbouring pairs, then neighbouring heads, so that heads inside the rows of a projection are read as whole lines.
+// Memory bound: every element is read and written once, the angles are few.  Angles: a pair's speed is a fraction of a turn with 88 bits, so that position * speed
+// modulo a turn is off by 2^-31 of a turn for positions up to 2^57 and by 2^-25 for any int64 (with 64 bits of the speed by 2^-24 at position 2^40 and by a tenth at
+// 2^60; fp32 angles are off by 0.06 at position 10^6).  Its top 32 bits go to sincospif.  A thread forms the sines of kVec pairs (16 bytes of each half) and uses
+// them for all heads of its group; threads beside one another take neighbouring pairs, then neighbouring heads, so that heads inside the rows of a projection are read as
+// whole lines.
 //
 // 2 x 16384 tokens, 16 + 4 heads of 128, bf16, 336 MB: 60 us (5.6 TB/s; at once on their way 1, 2, 4 heads a thread 66, 60, 59); 5 x 31896, 8 heads of 32, fp32: 56
 // (5.9 TB/s; 59, 56, 59).  With four heads, each vector converted by elements, 116 registers: 101 us.
@@ -34,8 +35,8 @@ struct RotaryArgs {
   int pairs, chunks, d;                // chunks of kVec pairs, then of 2 kVec channels that stay as they are
   int tokens;                          // of a block
   int inverse;
-  uint64_t speed[kRotaryPairs];        // turns a position, times 2^64
-  uint8_t axis[kRotaryPairs];
+  uint64_t speed[kRotaryPairs];        // turns a position, times 2^64, to nearest
+  int32_t rest[kRotaryPairs];          // what that leaves, times 2^96, in the first 24 bits; the axis in the last eight
 };
 
 template <typename T, int kVec>
@@ -70,6 +71,12 @@ __device__ __forceinline__ void rotary_write(RotaryVec<T, kVec>& x, const float*
 #pragma unroll
     for (int j = 0; j < kVec; ++j) x.v[j] = (T)f[j];
   }
+}
+// The fraction of a turn that a position turns by, times 2^32.  Of `rest` only the position's upper half counts: the lower one's part is below 2^-33 of a turn.  Against
+// `speed` alone 2 x 16384 tokens, 16 + 4 heads of 128, bf16 take 59.9 us for 59.6, 20000 tokens of 4 + 4 heads of 256 26.4 for 26.0; with 128 bits of the speed 65 and
+// 38, with a branch for positions beyond 32 bits 70 and 31.
+__device__ __forceinline__ uint32_t rotary_turns(int64_t position, uint64_t speed, int32_t rest) {
+  return (uint32_t)(((uint64_t)position * speed + (uint64_t)((int64_t)(int32_t)(position >> 32) * rest)) >> 32);
 }
 // a b + c d, in the same order in every form of the kernel
 __device__ __forceinline__ float rotary_sum(float a, float b, float c, float d) { return fmaf(a, b, __fmul_rn(c, d)); }
@@ -118,8 +125,8 @@ __device__ __forceinline__ void rotary_heads(const RotaryTensor& t, int64_t b, i
 template <typename T, int kVec, int kHeads, bool kNeighbours>
 __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const __grid_constant__ RotaryArgs a) {
   __shared__ uint64_t speed[kRotaryPairs];
-  __shared__ uint8_t axis[kRotaryPairs];
-  for (int i = threadIdx.x; i < a.pairs; i += kRotaryThreads) speed[i] = a.speed[i], axis[i] = a.axis[i];
+  __shared__ int32_t rest[kRotaryPairs];
+  for (int i = threadIdx.x; i < a.pairs; i += kRotaryThreads) speed[i] = a.speed[i], rest[i] = a.rest[i];
   __syncthreads();
   pdl_wait();
   const int per = a.chunks * a.head_groups, turning = a.pairs / kVec;
@@ -143,9 +150,9 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const __grid_con
       const int64_t* p = a.positions + b * a.pb + row * a.pr;
 #pragma unroll
       for (int j = 0; j < kVec; ++j) {
-        const int pair = kVec * chunk + j;
-        const uint64_t turns = (uint64_t)__ldg(p + axis[pair] * a.pa) * speed[pair];
-        sincospif((float)(int32_t)(turns >> 32) * 4.656612873077393e-10f, &s[j], &c[j]);      // 2^-31: half turns
+        const int pair = kVec * chunk + j, more = rest[pair];
+        const uint32_t turns = rotary_turns(__ldg(p + (more & 255) * a.pa), speed[pair], more & ~255);
+        sincospif((float)(int32_t)turns * 4.656612873077393e-10f, &s[j], &c[j]);      // 2^-31: half turns
         if (a.inverse) s[j] = -s[j];
       }
     }
@@ -158,7 +165,11 @@ template <typename T, int kVec, int kHeads, bool kNeighbours>
 static bool launch_rotary(RotaryArgs& a, int64_t batch, int groups, cudaStream_t st) {
   a.head_groups = groups;
   const int per = a.chunks * groups;
-  a.tokens = (int)std::min<int64_t>(a.n, std::max(1, kRotaryThreads / per));
+  // Lanes that read different arguments take turns, so a block brings the speeds in once for up to four turns of its threads, as long as every SM has 32 blocks:
+  // one head of 64 channels, 3 000 000 tokens, bf16 311 us with one, 279 with four (with eight blocks 5 x 31896 tokens of 8 heads of 32, fp32 53 -> 58).
+  const int once = std::max(1, kRotaryThreads / per);
+  const int64_t turns = std::min<int64_t>(std::max<int64_t>(batch * a.n / once / (32 * sm_count()), 1), 4);
+  a.tokens = (int)std::min<int64_t>(a.n, turns * once);
   const int64_t blocks = (a.n + a.tokens - 1) / a.tokens;
   return launch_pdl(rotary_kernel<T, kVec, kHeads, kNeighbours>, dim3((unsigned)blocks, (unsigned)batch), kRotaryThreads, 0, st, a);
 }
@@ -185,6 +196,57 @@ static bool launch_rotary(RotaryArgs& a, int vec, int64_t batch, cudaStream_t st
 template <typename T>
 static bool launch_rotary(RotaryArgs& a, int vec, bool neighbours, int64_t batch, cudaStream_t st) {
   return neighbours ? launch_rotary<T, true>(a, vec, batch, st) : launch_rotary<T, false>(a, vec, batch, st);
+}
+
+// ---- speeds ----------------------------------------------------------------------------------------------------------
+typedef unsigned __int128 Bits128;
+// m 2^(e - 128), the top bit of m set
+struct Wide {
+  Bits128 m;
+  int e;
+};
+// the upper half of a b, one too small at most
+static Bits128 upper(Bits128 a, Bits128 b) {
+  const uint64_t a1 = (uint64_t)(a >> 64), a0 = (uint64_t)a, b1 = (uint64_t)(b >> 64), b0 = (uint64_t)b;
+  const Bits128 x = (Bits128)a1 * b0, y = (Bits128)a0 * b1, low = ((Bits128)a0 * b0 >> 64) + (uint64_t)x + (uint64_t)y;
+  return (Bits128)a1 * b1 + (x >> 64) + (y >> 64) + (low >> 64);
+}
+static Wide wide(long double v) {
+  int e;
+  const long double f = frexpl(v, &e);      // 64 bits
+  return {(Bits128)(uint64_t)ldexpl(f, 64) << 64, e};
+}
+static Wide times(Wide a, Wide b) {
+  Wide c = {upper(a.m, b.m), a.e + b.e};
+  if (!(c.m >> 127)) c.m <<= 1, --c.e;
+  return c;
+}
+// base^(-1/n): a step of Newton's iteration for r^n = 1 / base from long double's r, whose error e / n, 2^-61 or less of it, leaves its square
+static Wide root_of_inverse(double base, int n) {
+  Wide r = wide(powl((long double)base, -1.0L / n)), power = wide((long double)base), x = r;
+  for (int k = n; k; k >>= 1, x = times(x, x))
+    if (k & 1) power = times(power, x);
+  // power = 1 + e
+  const Bits128 one = (Bits128)1 << 127;
+  const bool above = power.e == 1;
+  const Bits128 e = above ? (power.m - one) << 1 : (Bits128)0 - power.m, change = upper(r.m, e / n);
+  r.m = above ? r.m - change : r.m + change < r.m ? ~(Bits128)0 : r.m + change;
+  return r;
+}
+// The speeds of the pairs, turns times 2^128: each the one before times the ladder's step, cut to 2^-128 of a turn (off by 2^-117 after 256 of them).
+static void rotary_speeds(const px_rotary& r, int pairs, RotaryArgs& a) {
+  const Bits128 turn = (Bits128)0x28be60db9391054aull << 64 | 0x7f09d5f47d4d3770ull;      // 1 / 2 pi
+  Bits128 speed = turn;
+  Wide step = {};
+  int j = 0;
+  for (int i = 0; i < r.axes; ++i) {
+    if (r.per_axis ? r.sections[i] > 0 : i == 0) speed = turn, step = root_of_inverse(r.base, r.per_axis ? r.sections[i] : pairs);
+    for (int e = 0; e < r.sections[i]; ++e, ++j) {
+      const Bits128 near = speed + ((Bits128)1 << 39);                                  // to 88 bits
+      a.speed[j] = (uint64_t)((near + ((Bits128)1 << 63)) >> 64), a.rest[j] = (int32_t)(((uint32_t)(near >> 32) & ~255u) | (uint32_t)i);
+      if (step.e <= 0) speed = step.e > -128 ? upper(speed, step.m) >> -step.e : 0;      // a step of one otherwise
+    }
+  }
 }
 
 }  // namespace px
@@ -231,14 +293,7 @@ extern "C" int32_t px_rotary_turn(const px_rotary* r, const px_rows* q, const px
   a.heads = (int)r->heads, a.kv_heads = (int)r->kv_heads;
   a.pairs = (int)pairs, a.d = (int)r->d;
   a.inverse = inverse != 0;
-  // one power an axis, or one in all; their products are off by 2^-63 a factor
-  const long double turn = 0.159154943091895335768883763372514362034459645740L * 18446744073709551616.0L;      // 2^64 / 2 pi
-  long double speed = turn, step = powl((long double)r->base, -1.0L / pairs);
-  int j = 0;
-  for (int i = 0; i < r->axes; ++i) {
-    if (r->per_axis && r->sections[i]) speed = turn, step = powl((long double)r->base, -1.0L / r->sections[i]);
-    for (int e = 0; e < r->sections[i]; ++e, ++j, speed *= step) a.speed[j] = (uint64_t)llrintl(speed), a.axis[j] = (uint8_t)i;
-  }
+  rotary_speeds(*r, (int)pairs, a);
   const cudaStream_t st = (cudaStream_t)stream;
   const bool ok = r->dtype == PX_F32    ? launch_rotary<float>(a, vec, r->interleaved != 0, r->batch, st)
                   : r->dtype == PX_BF16 ? launch_rotary<bf16>(a, vec, r->interleaved != 0, r->batch, st)

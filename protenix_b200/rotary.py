@@ -19,13 +19,13 @@ def rotary_embedding(q: torch.Tensor, k: Optional[torch.Tensor], positions: torc
     """(q, k) turned by their positions; ``k`` None: q alone.
 
     ``q`` [..., H, N, D] and ``k`` [..., H_kv, N, D], fp32, bf16 or fp16 (views are taken as they are; the outputs lie in memory like
-    them: heads inside the rows where theirs are); ``positions`` [..., N, A], integers of any size and sign, over the batch axes of q or broadcast
+    them: heads inside the rows where theirs are); ``positions`` [..., N, A], integers that int64 holds, over the batch axes of q or broadcast
     along them.  ``sections``: how many pairs of channels each of the A axes turns, in the order of the pairs (default, for one axis:
     all D // 2).  P = sum(sections) pairs are (j, j + P), or with ``interleaved`` (2 j, 2 j + 1); the channels from 2 P on stay as they are.
 
     Pair j turns by positions[axis] * base ** -(j / P): one ladder of speeds through all axes.  ``per_axis``: each axis has the whole ladder,
-    base ** -(i / S) for the i-th of its S pairs.  Angles are exact for far positions, too; products are fp32, rounded once.  Differentiable any
-    number of times in q and k (the operator is linear).
+    base ** -(i / S) for the i-th of its S pairs.  Far positions keep their angles: they are off by 2^-31 of a turn up to 2^57, by 2^-25 up to 2^63.  Products are
+    fp32, rounded once.  Differentiable any number of times in q and k (the operator is linear).
     """
     if not q.is_cuda:
         raise RuntimeError("rotary_embedding: CUDA tensors only, this package has no CPU path")
