@@ -490,8 +490,11 @@ struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
     ctx->saved_data["strides"] = c10::List<int64_t>(c10::ArrayRef<int64_t>(strides));
     ctx->saved_data["base"] = base;
     ctx->saved_data["how"] = (int64_t)interleaved | (int64_t)per_axis << 1 | (int64_t)inverse << 2;
-    if (out.second.defined()) return {out.first, out.second};
-    return {out.first};
+    if (!out.second.defined()) return {out.first};
+    // what does not depend on a leaf asks for no gradient
+    if (!q.requires_grad()) ctx->mark_non_differentiable({out.first});
+    if (!k->requires_grad()) ctx->mark_non_differentiable({out.second});
+    return {out.first, out.second};
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     const int64_t how = ctx->saved_data["how"].toInt();
