@@ -475,7 +475,8 @@ PX_API int32_t px_rotary_turn(const px_rotary* r, const px_rows* q, const px_row
  * (total, with 1 / count or 1 in `inverse` for the backward pass; NULL: not wanted; the mean of nothing is NaN).
  * px_head_loss_bwd writes those of dx [rows][c], dw [classes][c] (type of x, contiguous) and dbias [classes] (type of the bias) that are not NULL, from the gradient of
  * the total (each = 0: one number) or of the rows' losses (each = 1, `inverse` not read).  It forms the logits again, for so many classes at a time
- * that 16 bits a logit stay within 512 MiB (256 classes at least).  Sums are fp32, across rows fp64, and have a fixed order.  c a multiple of 8, pointers aligned
+ * that 16 bits a logit stay within 512 MiB (256 classes at least).  The sum of the losses is fp64.  dx and dw are sums of fp32 accumulators of up to 131072 (PX_BF16) or
+ * 16384 (PX_F16) terms; dbias is fp32 over 32 rows and fp64 over these, with up to 128 channels and classes fp32.  All sums have a fixed order.  c a multiple of 8, pointers aligned
  * to 16 bytes, workspaces to 256.  No counterpart in the reference, whose heads (protenix/model/modules/head.py) leave the loss to torch. */
 typedef struct {
   const void* x;

@@ -10,7 +10,8 @@
 // Four products of 2 N V C where three are the least (the logits are formed twice).
 //
 // dl is formed without the scale of the loss, in [-2, 2] (fp16: times 2^14, so that probabilities down to 2^-28 stay normal numbers); the scale is
-// applied in fp32 where dx and dW are rounded.  Logits, exponentials and all sums are fp32, or fp64 across rows.
+// applied in fp32 where dx and dW are rounded.  Logits, exponentials and their sums are fp32, the sum of the losses fp64; dx and dW fp32 accumulators of bounded length
+// (longest_sum), added up in fp32; db fp32 over 32 rows and fp64 over these (small heads: fp32, px_head_small.cuh).
 //
 // Rows that are ignored take no part whatever they hold: their dl is zero by selection, and where one holds an infinity or a NaN (which a zero
 // weight would not silence) dW takes a copy of x in which those rows are zero; the copy is made only then.  A row of x that is not finite has no
@@ -352,18 +353,18 @@ struct EpiLogitGrad {
 
 // db of a piece: a warp's lanes along the classes, the groups of rows over the warps, in a fixed order.
 __global__ void __launch_bounds__(512) loss_bias_kernel(const float* __restrict__ part, void* __restrict__ db, int type, const LossOut out, int classes, int groups) {
-  __shared__ float x[16][32];
+  __shared__ double x[16][32];
   pdl_wait();
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, v = blockIdx.x * 32 + lane;
   double s = 0.0;
   if (v < classes)
     for (int g = w; g < groups; g += 16) s += part[(int64_t)g * classes + v];
-  x[w][lane] = (float)s;
+  x[w][lane] = s;
   __syncthreads();
   if (w == 0 && v < classes) {
-    float all = 0.f;
+    double all = 0.0;
     for (int i = 0; i < 16; ++i) all += x[i][lane];
-    bias_store(db, type, v, all * out());
+    bias_store(db, type, v, (float)all * out());
   }
 }
 
@@ -490,32 +491,37 @@ typedef GemmShape<1, 128, true, true, 5> Dw128;
 typedef GemmShape<1, 256, true, true, 4> Dw256;
 typedef GemmShape<2, 256, true, true, 5> DwPair;
 
-// A product's tiles, and the parts that a long axis is cut into (at least four steps each) where that shortens the rounds of its tiles: fewer tiles than SMs, or
-// a last round with few.
+// Steps of 64 terms that one accumulator of dx or dW takes.  The tensor core cuts it after each 16 terms: a sum of one sign loses 1.0e-7 (fp16) to 1.15e-7 (bf16) of itself
+// a cut (dW of 131072 to 453000 rows in one accumulator), so what the cuts take off stays below a quarter of half a step of the result.
+static int64_t longest_sum(bool f16) { return f16 ? 256 : 2048; }
+
+// A product's tiles, and the parts that a long axis is cut into: as many as longest_sum() wants (0: not cut), more (of at least four steps each) where that shortens the
+// rounds of its tiles, fewer than SMs or a last round with few.
 struct HeadCut {
   int ctas, kn;
   GemmTiles t;
   int64_t cycles;
 };
-static HeadCut cut_for(int ctas, int kn, int64_t m, int64_t n, int64_t k, bool split) {
+static HeadCut cut_for(int ctas, int kn, int64_t m, int64_t n, int64_t k, int64_t longest) {
   HeadCut c = {ctas, kn, {}, 0};
   const int64_t room = sm_count() / ctas;
   c.t.tiles_m = (int)(up(m, 128 * ctas) / (128 * ctas)), c.t.tiles_n = (int)(up(n, kn) / kn);
   c.t.batch = 1, c.t.splits = 1, c.t.group = 8;
   c.t.nk = c.t.nk_split = (int)(up(k, kGemmK) / kGemmK);
   const int64_t tiles = (int64_t)c.t.tiles_m * c.t.tiles_n, step = ctas == 2 ? 600 : 750;
-  for (int64_t s = 1; s <= (split ? std::min<int64_t>(std::max<int64_t>(room / tiles, 4), c.t.nk / 4) : 1) || s == 1; ++s) {
+  const int64_t least = longest ? (c.t.nk + longest - 1) / longest : 1, most = longest ? std::min<int64_t>(std::max<int64_t>(room / tiles, 4), c.t.nk / 4) : 1;
+  for (int64_t s = least; s <= most || s == least; ++s) {
     const int64_t nk = (c.t.nk + s - 1) / s, parts = (c.t.nk + nk - 1) / nk;
     const int64_t cycles = (tiles * parts + room - 1) / room * (nk * step + 2000) + (parts > 1 ? 4000 + m * n * parts / 400 : 0);
-    if (s == 1 || cycles < c.cycles) c.cycles = cycles, c.t.nk_split = (int)nk, c.t.splits = (int)parts;
+    if (s == least || cycles < c.cycles) c.cycles = cycles, c.t.nk_split = (int)nk, c.t.splits = (int)parts;
   }
   return c;
 }
 // A pair of CTAs asks L2 for a third less and goes through a step in some 600 cycles, where one alone takes 750 (both measured with all SMs at work): dx of 8192
 // rows, 32768 classes and 1024 channels, two rounds of either, 414 us alone.
-static HeadCut cut(int64_t m, int64_t n, int64_t k, bool split, int narrow) {
-  if (n <= narrow || m <= 128) return cut_for(1, n <= narrow ? narrow : 256, m, n, k, split);
-  const HeadCut one = cut_for(1, 256, m, n, k, split), two = cut_for(2, 256, m, n, k, split);
+static HeadCut cut(int64_t m, int64_t n, int64_t k, int64_t longest, int narrow) {
+  if (n <= narrow || m <= 128) return cut_for(1, n <= narrow ? narrow : 256, m, n, k, longest);
+  const HeadCut one = cut_for(1, 256, m, n, k, longest), two = cut_for(2, 256, m, n, k, longest);
   return two.cycles < one.cycles ? two : one;
 }
 
@@ -532,9 +538,10 @@ static HeadPlan head_plan(const px_head& h, bool want_dx, bool want_dw, bool wan
   p.piece = p.pieces == 1 ? h.classes : up((h.classes + p.pieces - 1) / p.pieces, 256);
   p.pieces = (h.classes + p.piece - 1) / p.piece;
   p.ld = up(p.piece, 8);
-  p.logits = cut(h.rows, p.piece, h.c, false, 64);
-  p.dx = cut(h.rows, h.c, p.piece, true, 128);
-  p.dw = cut(p.piece, h.c, h.rows, true, 128);
+  const int64_t longest = longest_sum(h.dtype == PX_F16);
+  p.logits = cut(h.rows, p.piece, h.c, 0, 64);
+  p.dx = cut(h.rows, h.c, p.piece, longest, 128);
+  p.dw = cut(p.piece, h.c, h.rows, longest, 128);
   p.dx_slots = p.dx.t.splits > 1 || p.pieces > 1;
   int64_t at = 0;
   const auto take = [&](int64_t bytes) {
@@ -630,12 +637,17 @@ template <bool kBackward>
 static bool launch_small(const SmallArgs& a, cudaStream_t st) {
   return a.classes <= 64 ? launch_small<kBackward, 64>(a, st) : launch_small<kBackward, 128>(a, st);
 }
+// The rows of a launch are as many as its CTAs' accumulators of dW take; the launches' sums are joined in their order.
 struct SmallPlan {
+  int64_t rows, ctas;                      // of a launch; of all launches
   int64_t scale, found, w, b, bytes;
 };
 static SmallPlan small_plan(const px_head& h) {
-  const int64_t ctas = small_ctas(h.rows), vp = small_vp(h.classes);
+  const int64_t vp = small_vp(h.classes), tiles = up(h.rows, 128) / 128, most = sm_count() * longest_sum(h.dtype == PX_F16) / 2, launches = (tiles + most - 1) / most;
   SmallPlan p;
+  p.rows = (tiles + launches - 1) / launches * 128, p.ctas = 0;
+  for (int64_t row = 0; row < h.rows; row += p.rows) p.ctas += small_ctas(std::min(p.rows, h.rows - row));
+  const int64_t ctas = p.ctas;
   p.scale = 0, p.found = 1024, p.w = p.found + up(kScanBlocks * 4, 1024), p.b = p.w + ctas * 128 * vp * 4, p.bytes = p.b + ctas * 8 * vp * 4;
   return p;
 }
@@ -667,7 +679,7 @@ extern "C" int32_t px_head_loss_fwd(const px_head* head, float* norm, float* los
     if (!launch_small<false>(a, st)) return PX_ERR_LAUNCH;
     return !total || launch_pdl(small_total_kernel, dim3(1), 32, 0, st, (const double2*)workspace, small_ctas(h.rows), total, inverse, (int)mean) ? PX_OK : PX_ERR_LAUNCH;
   }
-  const HeadCut c = cut(h.rows, h.classes, h.c, false, 64);
+  const HeadCut c = cut(h.rows, h.classes, h.c, 0, 64);
   char* at = (char*)workspace;
   uint32_t* arrivals = (uint32_t*)at;
   at += 1024;
@@ -714,17 +726,25 @@ extern "C" int32_t px_head_loss_bwd(const px_head* head, const float* norm, cons
   };
   if (small_head(h.c, h.classes)) {
     const SmallPlan p = small_plan(h);
-    SmallArgs a;
-    if (!small_args(&a, h) || (dx && !out_map(&a.dx, type16(f16), 2, dx, h.c, h.rows, h.c, 1))) return PX_ERR_LAUNCH;
-    a.norm = (float2*)const_cast<float*>(norm), a.want_dx = dx != nullptr;
-    a.part_w = dw ? (float*)(ws + p.w) : nullptr, a.part_b = dbias ? (float*)(ws + p.b) : nullptr;
+    const int64_t vp = small_vp(h.classes);
     if (!scales(p.scale, p.found)) return PX_ERR_LAUNCH;
-    a.out = out;
-    if (!launch_small<true>(a, st)) return PX_ERR_LAUNCH;
+    int64_t slot = 0;
+    for (int64_t row = 0; row < h.rows; row += p.rows) {
+      px_head part = h;
+      part.rows = std::min(p.rows, h.rows - row), part.x = (const uint16_t*)h.x + row * h.x_stride, part.target = h.target + row;
+      SmallArgs a;
+      if (!small_args(&a, part) || (dx && !out_map(&a.dx, type16(f16), 2, (uint16_t*)dx + row * h.c, h.c, part.rows, h.c, 1))) return PX_ERR_LAUNCH;
+      a.norm = (float2*)const_cast<float*>(norm) + row, a.want_dx = dx != nullptr;
+      a.part_w = dw ? (float*)(ws + p.w) + slot * 128 * vp : nullptr, a.part_b = dbias ? (float*)(ws + p.b) + slot * 8 * vp : nullptr;
+      a.out = out;
+      if (each) a.out.grad = grad + row;
+      if (!launch_small<true>(a, st)) return PX_ERR_LAUNCH;
+      slot += small_ctas(part.rows);
+    }
     if (!dw && !dbias) return PX_OK;
-    const int vp = (int)small_vp(h.classes), groups = vp / 32;
-    return launch_pdl(small_join_kernel, dim3((unsigned)(groups * (h.c + 1))), 256, 0, st, (const float*)a.part_w, (const float*)a.part_b, (uint16_t*)dw, dbias,
-                      small_ctas(h.rows), vp, (int)h.c, (int)h.classes, (int)f16, (int)h.bias_dtype)
+    const int groups = (int)vp / 32;
+    return launch_pdl(small_join_kernel, dim3((unsigned)(groups * (h.c + 1))), 256, 0, st, dw ? (const float*)(ws + p.w) : nullptr, dbias ? (const float*)(ws + p.b) : nullptr,
+                      (uint16_t*)dw, dbias, (int)p.ctas, (int)vp, (int)h.c, (int)h.classes, (int)f16, (int)h.bias_dtype)
                ? PX_OK
                : PX_ERR_LAUNCH;
   }
