@@ -473,7 +473,7 @@ PX_API int32_t px_rotary_turn(const px_rotary* r, const px_rows* q, const px_row
  * any gradient, whatever they hold; a target outside the classes makes its row's loss, and the gradients that it enters, NaN.
  * px_head_loss_fwd writes norm [rows + 1][2] (for the backward pass: reference and sum of the exponentials, last what it found in ignored rows), the rows' losses [rows] (NULL: not wanted) and their sum or mean over the rows that count
  * (total, with 1 / count or 1 in `inverse` for the backward pass; NULL: not wanted; the mean of nothing is NaN).
- * px_head_loss_bwd writes those of dx [rows][c], dw [classes][c] (type of x, contiguous) and dbias [classes] (type of the bias) that are not NULL, from the gradient of
+ * px_head_loss_bwd writes those of dx [rows][c], dw [classes][c] (type of x, contiguous) and dbias [classes] (type of the bias) that are not NULL (none over an input), from the gradient of
  * the total (each = 0: one number) or of the rows' losses (each = 1, `inverse` not read).  It forms the logits again, for so many classes at a time
  * that 16 bits a logit stay within 512 MiB (256 classes at least).  The sum of the losses is fp64.  dx and dw are sums of fp32 accumulators of up to 131072 (PX_BF16) or
  * 16384 (PX_F16) terms; dbias is fp32 over 32 rows and fp64 over these, with up to 128 channels and classes fp32.  All sums have a fixed order.  c a multiple of 8, pointers aligned

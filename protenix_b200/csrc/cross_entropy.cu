@@ -14,7 +14,8 @@
 // (longest_sum), added up in fp32; db fp32 over 32 rows and fp64 over these (small heads: fp32, px_head_small.cuh).
 //
 // Rows that are ignored take no part whatever they hold: their dl is zero by selection, and where one holds an infinity or a NaN (which a zero
-// weight would not silence) dW takes a copy of x in which those rows are zero; the copy is made only then.  A row of x that is not finite has no
+// weight would not silence) dW takes a copy of x in which those rows are zero; the copy is made only then, where dx will be (dW is formed before it), or in the
+// workspace of a call that wants no dx.  A row of x that is not finite has no
 // finite logit, so the forward pass sees it in the row's sum; by a pass over the ignored rows and one for the verdict, two more launches, training on
 // 384 rows took 104 us and on 3001 12 us more.
 #include "px_head_small.cuh"
@@ -551,7 +552,7 @@ static HeadPlan head_plan(const px_head& h, bool want_dx, bool want_dw, bool wan
   };
   p.scale = take(sizeof(LossScale));
   p.found = take(kScanBlocks * 4);
-  p.clean = take(want_dw ? h.rows * h.c * 2 : 0);
+  p.clean = take(want_dw && !want_dx ? h.rows * h.c * 2 : 0);
   p.dl = take(h.rows * p.ld * 2);
   p.dx_at = take(want_dx && p.dx_slots ? p.dx.t.splits * h.rows * h.c * 4 : 0);
   p.dw_at = take(want_dw && p.dw.t.splits > 1 ? p.dw.t.splits * p.piece * h.c * 4 : 0);
@@ -750,7 +751,7 @@ extern "C" int32_t px_head_loss_bwd(const px_head* head, const float* norm, cons
   }
   const HeadPlan p = head_plan(h, dx, dw, dbias);
   uint16_t* dl = (uint16_t*)(ws + p.dl);
-  uint16_t* clean = (uint16_t*)(ws + p.clean);
+  uint16_t* clean = dx ? (uint16_t*)dx : (uint16_t*)(ws + p.clean);      // dx is written after the last dW that reads them
   float* part_bias = (float*)(ws + p.db_at);
   const uint32_t* const dirty = (const uint32_t*)(norm + 2 * h.rows);
   const int bias_groups = (int)((h.rows + 31) / 32);
@@ -768,30 +769,6 @@ extern "C" int32_t px_head_loss_bwd(const px_head* head, const float* norm, cons
     void* const db = dbias ? (char*)dbias + first * bias_size : nullptr;
     const bool bias_apart = dbias && (!dw || bias_groups > kBiasGroups);
     if (bias_apart && !launch_pdl(loss_bias_kernel, dim3((unsigned)((vc + 31) / 32)), 512, 0, st, (const float*)part_bias, db, (int)h.bias_dtype, out, (int)vc, bias_groups)) return PX_ERR_LAUNCH;
-    if (dx) {
-      GemmOperands ops = {};
-      if (!gemm_map(&ops.a, f16, dl, vc, h.rows, 1, p.ld, h.rows * p.ld, kGemmM) ||
-          !gemm_map(&ops.b, f16, (const uint16_t*)h.w + first * h.w_stride, h.c, vc, 1, h.w_stride, vc * h.w_stride, kGemmK))
-        return PX_ERR_LAUNCH;
-      GemmTiles t = p.dx.t;
-      t.nk = (int)(up(vc, kGemmK) / kGemmK);
-      if (t.splits == 1) t.nk_split = t.nk;
-      // a last piece may be too short for all splits: the ones that it has leave the others' sums as they are
-      t.splits = (t.nk + t.nk_split - 1) / t.nk_split;
-      int32_t status;
-      if (p.dx_slots) {
-        EpiGrad<true> ep = {};
-        if (!out_map(&ep.map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, ws + p.dx_at, h.c, h.rows, h.c, p.dx.t.splits)) return PX_ERR_LAUNCH;
-        ep.out = out, ep.rows = (int)h.rows, ep.cols = (int)h.c, ep.add = i > 0;
-        status = launch_grad<Dx128, Dx256, DxPair>(ops, f16, p.dx, ep, t, st);
-      } else {
-        EpiGrad<false> ep = {};
-        if (!out_map(&ep.map, type16(f16), 2, dx, h.c, h.rows, h.c, 1)) return PX_ERR_LAUNCH;
-        ep.out = out, ep.target = h.target, ep.ignore = h.ignore, ep.rows = (int)h.rows, ep.cols = (int)h.c, ep.f16 = f16;
-        status = launch_grad<Dx128, Dx256, DxPair>(ops, f16, p.dx, ep, t, st);
-      }
-      if (status) return status;
-    }
     if (dw) {
       uint16_t* to = (uint16_t*)dw + first * h.c;
       GemmOperands ops = {};
@@ -818,6 +795,30 @@ extern "C" int32_t px_head_loss_bwd(const px_head* head, const float* norm, cons
         if (!out_map(&ep.map, type16(f16), 2, to, h.c, vc, h.c, 1)) return PX_ERR_LAUNCH;
         ep.out = out, ep.rows = (int)vc, ep.cols = (int)h.c, ep.f16 = f16;
         status = launch_grad<Dw128, Dw256, DwPair>(ops, f16, p.dw, ep, t, st);
+      }
+      if (status) return status;
+    }
+    if (dx) {
+      GemmOperands ops = {};
+      if (!gemm_map(&ops.a, f16, dl, vc, h.rows, 1, p.ld, h.rows * p.ld, kGemmM) ||
+          !gemm_map(&ops.b, f16, (const uint16_t*)h.w + first * h.w_stride, h.c, vc, 1, h.w_stride, vc * h.w_stride, kGemmK))
+        return PX_ERR_LAUNCH;
+      GemmTiles t = p.dx.t;
+      t.nk = (int)(up(vc, kGemmK) / kGemmK);
+      if (t.splits == 1) t.nk_split = t.nk;
+      // a last piece may be too short for all splits: the ones that it has leave the others' sums as they are
+      t.splits = (t.nk + t.nk_split - 1) / t.nk_split;
+      int32_t status;
+      if (p.dx_slots) {
+        EpiGrad<true> ep = {};
+        if (!out_map(&ep.map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, ws + p.dx_at, h.c, h.rows, h.c, p.dx.t.splits)) return PX_ERR_LAUNCH;
+        ep.out = out, ep.rows = (int)h.rows, ep.cols = (int)h.c, ep.add = i > 0;
+        status = launch_grad<Dx128, Dx256, DxPair>(ops, f16, p.dx, ep, t, st);
+      } else {
+        EpiGrad<false> ep = {};
+        if (!out_map(&ep.map, type16(f16), 2, dx, h.c, h.rows, h.c, 1)) return PX_ERR_LAUNCH;
+        ep.out = out, ep.target = h.target, ep.ignore = h.ignore, ep.rows = (int)h.rows, ep.cols = (int)h.c, ep.f16 = f16;
+        status = launch_grad<Dx128, Dx256, DxPair>(ops, f16, p.dx, ep, t, st);
       }
       if (status) return status;
     }

@@ -104,3 +104,20 @@ def test_small_heads_in_several_launches(rows, reduction):
                                   (dw, dl.t() @ x.detach().double(), dl.abs().t() @ x.detach().double().abs(), 2 * (g.abs()[:, None] * x.detach().double().abs()).sum(0))):
         assert bool(((got.double() - want).abs() <= u * (1 + u) * size + u * want.abs() + 2.0 ** -17 * most + 2.0 ** -25).all())
     assert bool(((db.double() - dl.sum(0)).abs() <= 2.0 ** -14 * g.abs().sum()).all())
+
+
+@pytest.mark.parametrize("rows,c,v", [(300, 264, 300), (9000, 136, 700), (70000, 64, 9000)])
+@pytest.mark.parametrize("which", [(0, 1, 2), (0, 1), (1,), (1, 2), (0,)])
+def test_ignored_rows_that_are_not_finite(rows, c, v, which):
+    """The rows without them are kept where dx will be, or in the workspace of a call without dx; classes in one piece and in several."""
+    x, w, b, t = _inputs(rows, c, v, BF16, seed=2)
+    dirty = x.detach().clone()
+    x.data[t == -100] = 0.0
+    dirty[t == -100] = math.inf
+    dirty.requires_grad_()
+    out = []
+    for y in (x, dirty):
+        leaves = (y, w, b)
+        out.append(torch.autograd.grad(px.linear_cross_entropy(y, w, t, bias=b), [leaves[i] for i in which]))
+    ops.device_error_flags()
+    assert all(bool(g.isfinite().all()) and torch.equal(g, z) for g, z in zip(*out))
