@@ -32,6 +32,10 @@ __host__ __device__ constexpr float uncut(int64_t k, int chunk) { return 1.f + 2
 
 // ---- norm and first iterate ------------------------------------------------------------------------------------------
 constexpr int kNormBlocks = 1024;      // of a matrix, at most
+// Blocks of a matrix, each of which leaves a sum.
+static int norm_parts(int64_t batch, int64_t elements) {
+  return (int)std::min<int64_t>(std::min<int64_t>(kNormBlocks, std::max<int64_t>(8, 8 * sm_count() / batch)), (elements + 2047) / 2048);
+}
 // kVec elements at a time: 16 bytes where matrices begin at a multiple of that (24 x 384 x 1536, bf16: by elements 14 us).
 template <typename T, int kVec>
 __global__ void __launch_bounds__(256) ortho_norm_kernel(const T* __restrict__ g, double* __restrict__ sums, int64_t elements) {
@@ -565,7 +569,7 @@ static OrthoPlan ortho_plan(int64_t batch, int64_t m, int64_t n) {
     at += ortho_up(bytes, 1024);
     return here;
   };
-  p.sums = take(batch * kNormBlocks * 8);
+  p.sums = take(batch * norm_parts(batch, m * n) * 8);
   for (int64_t& x : p.x) x = take(batch * 2 * m * p.ld * 2);
   p.gram = take(batch * 2 * p.s * p.lds * 2);
   p.poly = take(batch * 2 * p.s * p.lds * 2);
@@ -576,8 +580,7 @@ static OrthoPlan ortho_plan(int64_t batch, int64_t m, int64_t n) {
 }
 template <typename T>
 static bool ortho_first(const void* g, double* sums, uint4* planes, int64_t batch, int64_t m, int64_t n, int64_t ld, double eps, cudaStream_t st) {
-  const int64_t blocks_each = std::max<int64_t>(8, 8 * sm_count() / batch);
-  const int parts = (int)std::min<int64_t>(std::min<int64_t>(kNormBlocks, blocks_each), (m * n + 2047) / 2048);
+  const int parts = norm_parts(batch, m * n);
   constexpr int kVec = 16 / sizeof(T);
   const bool wide = m * n % kVec == 0 && ((uintptr_t)g & 15) == 0;
   if (!launch_pdl(wide ? ortho_norm_kernel<T, kVec> : ortho_norm_kernel<T, 1>, dim3(parts, (unsigned)batch), 256, 0, st, (const T*)g, sums, m * n)) return false;
