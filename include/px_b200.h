@@ -501,7 +501,8 @@ PX_API int32_t px_head_loss_bwd(const px_head* head, const float* norm, const fl
  * 1 to 1000 steps, m and n up to 2^20.  Products take operands of 22 bits (two fp16 planes) and add in fp32, whatever the type; iterates and polynomials may grow to
  * 60 (an overflow comes out infinite or NaN).  A matrix that is not finite gives NaN and leaves the others alone.  Workspace aligned to 256 bytes.  No
  * counterpart in the reference. */
-PX_API int64_t px_orthogonalize_workspace_bytes(int64_t batch, int64_t m, int64_t n);
+PX_API int64_t px_orthogonalize_workspace_bytes(int64_t batch, int64_t m, int64_t n); /* for any number of steps */
+PX_API int64_t px_orthogonalize_steps_workspace_bytes(int64_t batch, int64_t m, int64_t n, int32_t steps);
 PX_API int32_t px_orthogonalize(const void* g, void* out, int64_t batch, int64_t m, int64_t n, const float* coefficients, int32_t steps, double eps, int32_t dtype,
                          void* workspace, int64_t workspace_bytes, void* stream);
 

@@ -91,6 +91,7 @@ SIGNATURES = {
     "px_window_workspace_bytes": (I64, [P, I32]),
     "px_window_bwd": (I32, [P, P, P, P, P, P, P, P, P, P, P, P, P, I64, P]),
     "px_orthogonalize_workspace_bytes": (I64, [I64, I64, I64]),
+    "px_orthogonalize_steps_workspace_bytes": (I64, [I64, I64, I64, I32]),
     "px_orthogonalize": (I32, [P, P, I64, I64, I64, P, I32, D, I32, P, I64, P]),
     "px_rotary_turn": (I32, [P, P, P, P, P, I32, P]),
     "px_head_loss_workspace_bytes": (I64, [I64, I64]),

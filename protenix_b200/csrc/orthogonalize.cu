@@ -601,6 +601,13 @@ extern "C" int64_t px_orthogonalize_workspace_bytes(int64_t batch, int64_t m, in
   return batch <= 0 || m <= 0 || n <= 0 ? 0 : ortho_plan(batch, m, n).bytes;
 }
 
+// All steps in one launch take none; 1024 bytes, so that a call has a workspace whatever its form.
+extern "C" int64_t px_orthogonalize_steps_workspace_bytes(int64_t batch, int64_t m, int64_t n, int32_t steps) {
+  if (batch <= 0 || m <= 0 || n <= 0) return 0;
+  int slices;
+  return small_ortho_ctas(batch, std::min(m, n), std::max(m, n), steps, &slices) ? 1024 : ortho_plan(batch, m, n).bytes;
+}
+
 extern "C" int32_t px_orthogonalize(const void* g, void* out, int64_t batch, int64_t m, int64_t n, const float* coefficients, int32_t steps, double eps, int32_t dtype,
                                     void* workspace, int64_t workspace_bytes, void* stream) {
   if (batch < 0 || m < 0 || n < 0 || steps < 1 || !coefficients || !(eps >= 0.0)) return PX_ERR_BAD_ARG;
@@ -608,8 +615,8 @@ extern "C" int32_t px_orthogonalize(const void* g, void* out, int64_t batch, int
   if (batch > 65535 || m > (1 << 20) || n > (1 << 20) || steps > 1000) return PX_ERR_UNSUPPORTED;
   if (batch == 0 || m == 0 || n == 0) return PX_OK;
   if (!g || !out || !workspace || ((uintptr_t)workspace & 255) || (((uintptr_t)g | (uintptr_t)out) & (dtype == PX_F32 ? 3 : 1))) return PX_ERR_BAD_ARG;
+  if (workspace_bytes < px_orthogonalize_steps_workspace_bytes(batch, m, n, steps)) return PX_ERR_WORKSPACE;
   const OrthoPlan p = ortho_plan(batch, m, n);
-  if (workspace_bytes < p.bytes) return PX_ERR_WORKSPACE;
   if (!have_context()) return PX_ERR_LAUNCH;
   const cudaStream_t st = (cudaStream_t)stream;
   int slices = 1;

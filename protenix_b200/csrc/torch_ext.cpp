@@ -64,7 +64,7 @@ constexpr int64_t kCz = 128, kCs = 384, kHeadsSingle = 16, kHeads = 4, kHeadDim 
   X(px_dropout_add) X(px_relpos_codes_bytes) X(px_relpos_workspace_bytes) X(px_relpos_fwd) X(px_relpos_bwd) X(px_window_lse_floats) \
   X(px_window_fwd) X(px_window_workspace_bytes) X(px_window_bwd) X(px_head_loss_workspace_bytes) X(px_head_loss_fwd) \
   X(px_head_loss_bwd_workspace_bytes) X(px_head_loss_bwd) X(px_rotary_turn) \
-  X(px_orthogonalize_workspace_bytes) X(px_orthogonalize)
+  X(px_orthogonalize_workspace_bytes) X(px_orthogonalize_steps_workspace_bytes) X(px_orthogonalize)
 struct Abi {
 #define X(f) decltype(&::f) f = nullptr;
   PX_FUNCTIONS(X)

@@ -591,7 +591,7 @@ Tensor orthogonalize(const Tensor& g_, const std::vector<double>& coefficients, 
   const Tensor g = g_.contiguous(), out = at::empty(g.sizes(), g.options());
   if (batch == 0) return out;
   const std::vector<float> c(coefficients.begin(), coefficients.end());
-  const int64_t bytes = abi.px_orthogonalize_workspace_bytes(batch, m, n);
+  const int64_t bytes = abi.px_orthogonalize_steps_workspace_bytes(batch, m, n, (int32_t)steps);
   const Tensor ws = bytes_like(g, bytes);
   const cudaStream_t st = at::cuda::getCurrentCUDAStream();
   launch("px_orthogonalize", st, [&] {
