@@ -121,3 +121,18 @@ def test_ignored_rows_that_are_not_finite(rows, c, v, which):
         out.append(torch.autograd.grad(px.linear_cross_entropy(y, w, t, bias=b), [leaves[i] for i in which]))
     ops.device_error_flags()
     assert all(bool(g.isfinite().all()) and torch.equal(g, z) for g, z in zip(*out))
+
+
+@pytest.mark.parametrize("c,v", [(64, 90), (136, 300)])
+@pytest.mark.parametrize("reduction", ["none", "mean"])
+@pytest.mark.parametrize("dtype,power", [(BF16, -90), (BF16, -20), (BF16, 20), (BF16, 100), (FP16, -4), (FP16, 8)])
+def test_the_scale_of_the_loss_enters_at_the_end(c, v, reduction, dtype, power):
+    """All three gradients of a loss times a power of two are those of the loss times it, to the bit, where both are normal numbers of their type."""
+    x, w, b, t = _inputs(150, c, v, dtype, seed=4)
+    loss = px.linear_cross_entropy(x, w, t, bias=b, reduction=reduction)
+    up = torch.randn(loss.shape, device="cuda")
+    one = torch.autograd.grad(loss, (x, w, b), up, retain_graph=True)
+    for g, z in zip(torch.autograd.grad(loss, (x, w, b), up * 2.0 ** power), one):
+        least = torch.finfo(z.dtype).tiny
+        normal = (z.abs() >= least) & (g.abs() >= least) & g.isfinite()
+        assert float(normal.float().mean()) > 0.1 and torch.equal(g[normal].double(), z[normal].double() * 2.0 ** power)
