@@ -134,5 +134,5 @@ def test_the_scale_of_the_loss_enters_at_the_end(c, v, reduction, dtype, power):
     one = torch.autograd.grad(loss, (x, w, b), up, retain_graph=True)
     for g, z in zip(torch.autograd.grad(loss, (x, w, b), up * 2.0 ** power), one):
         least = torch.finfo(z.dtype).tiny
-        normal = (z.abs() >= least) & (g.abs() >= least) & g.isfinite()
+        normal = (z.abs() > least) & (g.abs() > least) & g.isfinite()      # the least itself may have come from below, where steps are wider
         assert float(normal.float().mean()) > 0.1 and torch.equal(g[normal].double(), z[normal].double() * 2.0 ** power)
