@@ -37,11 +37,11 @@ __device__ __forceinline__ float row_loss(float sum, float ref, float hit, bool 
   return loss < 0.f ? 0.f : loss * 0.6931471805599453f;
 }
 
-// The tensor core cuts an accumulator after each 16 channels, and what it aligns to it, towards zero.  A logit that grows with its terms comes out too small, in
-// the mean by 1.6e-8 (c / 16 + 1) of itself in bf16 and 2.8e-8 in fp16, whose products are longer (rows that lean towards their class; three times that where
-// all terms are of one sign).  This puts it back: losses of rows by themselves, 256 to 2048 channels, are off by 1e-7 to 5e-7 of their norm in bf16 (with 2.9e-8 by 1.4e-7 to 1.3e-6),
-// 1.4e-7 to 9e-7 in fp16; with 2048 channels 3e-6 without.  Plain fp32 products: 1e-7.
-static inline float uncut_logits(int64_t c, bool f16) { return 1.f + (f16 ? 2.8e-8f : 1.6e-8f) * (float)((c + 15) / 16 + 1); }
+// The tensor core cuts an accumulator after each 16 channels, and what it aligns to it, towards zero: a logit comes out too small, in the mean, of rows that lean
+// towards their class and of logits that are noise alike, by 1.5e-8 to 1.6e-8 (c / 16 + 1) of itself in bf16 and 1.7e-8 to 2.5e-8 in fp16, whose products are longer (512 to
+// 4096 channels).  This puts the mean back, to within 0.4e-8.  Where all terms are of one sign 1e-8 (512 channels) to 4e-8 (4096) is missing in bf16 and 8e-8 to 1e-7 in
+// fp16, of which it is a part; few channels whose sums are exact gain up to 1.2e-7.  Losses of 4096 rows of noise, 4096 channels: 1e-6 off in the mean, 6e-5 without (bf16).
+static inline float uncut_logits(int64_t c, bool f16) { return 1.f + (f16 ? 2.1e-8f : 1.6e-8f) * (float)((c + 15) / 16 + 1); }
 __device__ __forceinline__ void logits_of(const uint32_t (&r)[32], float uncut, float (&v)[32]) {
   const f32x2 u = pair2(uncut, uncut);
 #pragma unroll
