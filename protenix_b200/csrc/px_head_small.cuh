@@ -3,7 +3,7 @@
 // The weight stays in shared memory and the rows go through once.  Forward, a tile of 128 rows: logits = x W^T into tensor memory, a thread a row
 // forms the loss.  Backward: logits again, a thread a row writes dl in 16 bits to shared memory, and both gradients are products with that same
 // tile, dx = dl W (dl along the classes, W across) and dW^T += x^T dl (both across), dW^T staying in tensor memory until the CTA's last tile.  The
-// sums of the CTAs are joined in their order.  Bytes: x once forward; x and dx once backward.  (Through the general path dl would be written and read
+// sums of the CTAs are joined in their order (backward, rows beyond what a CTA's dW^T may add up go through another launch).  Bytes: x once forward; x and dx once backward.  (Through the general path dl would be written and read
 // twice, 16 bits a class: 768^2 rows, 128 channels, 64 classes 664 us in all.)
 //
 // Rows that are ignored: dl zero by selection, and their x is zeroed in shared memory before the product for dW reads it.

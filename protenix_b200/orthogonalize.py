@@ -1,8 +1,11 @@
 """``orthogonalize``: matrices with their singular values driven towards one, and ``Muon``, the optimiser that takes such updates.
 
 The weights of a Pairformer stack are matrices, many of one shape (128 x 128, 512 x 128 and 128 x 512 in the pair path of each block, 384 x 384 to 1536 x
-384 in the single one).  A momentum whose singular values are made alike moves all directions of a weight by the same amount.  The
-polynomial iteration (Newton-Schulz) needs products only; ``px_orthogonalize`` runs it for all matrices of a shape at once.
+384 in the single one).  The stack of this package runs forward only and gives them no gradient: they are updated where other code trains them.  What the operators
+of this package train are the matrices around them: projections, heads, the weight of the position encoding.
+
+A momentum whose singular values are made alike moves all directions of a weight by the same amount.  The polynomial iteration (Newton-Schulz) needs products
+only; ``px_orthogonalize`` runs it for all matrices of a shape at once.
 """
 from __future__ import annotations
 
