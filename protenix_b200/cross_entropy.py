@@ -23,10 +23,10 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     influence.  Any other target makes its row's loss, and the gradients that it enters, NaN.  ``label_smoothing`` e: the
     class counts 1 - e, and each class e / V more.  ``reduction``: "mean" (over the rows that count; of none NaN, with gradients of zero), "sum" or "none".
 
-    Logits, exponentials and their sums are fp32, the sum of the losses fp64; sums of dx and of dW are fp32 in parts of at most 131072 (bf16) or 16384 (fp16) terms,
-    what such a part loses to the tensor core's cuts is below a quarter of the result's rounding.  The gradient of the logits is rounded to x's type where the products for x and
-    weight take it, before the scale of the loss is applied (of losses by row, relative to the largest of their gradients); in fp16 what is below 2^-38 of that vanishes.
-    That of bias is not rounded before its sum.  Differentiable once in x, weight and bias; the gradients have their types and are the same to the bit on each call.
+    Logits, exponentials and their sums are fp32, the sum of the losses fp64.  Sums of dx and of dW are fp32, in parts of at most 131072 (bf16) or 16384 (fp16) terms:
+    what a part loses to the tensor core's cuts is below a quarter of the result's rounding.  The gradient of the logits is rounded to x's type where the
+    products for x and weight take it, before the scale of the loss is applied (of losses by row, relative to the largest of their gradients); in fp16 what is
+    below 2^-38 of that vanishes.  That of bias is not rounded before its sum.  Differentiable once in x, weight and bias; the gradients have their types and are the same to the bit on each call.
     """
     if not x.is_cuda:
         raise RuntimeError("linear_cross_entropy: CUDA tensors only, this package has no CPU path")
