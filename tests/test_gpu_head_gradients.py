@@ -136,3 +136,26 @@ def test_the_scale_of_the_loss_enters_at_the_end(c, v, reduction, dtype, power):
         least = torch.finfo(z.dtype).tiny
         normal = (z.abs() > least) & (g.abs() > least) & g.isfinite()      # the least itself may have come from below, where steps are wider
         assert float(normal.float().mean()) > 0.1 and torch.equal(g[normal].double(), z[normal].double() * 2.0 ** power)
+
+
+@pytest.mark.parametrize("rows,c,v", [(300, 264, 300), (70000, 64, 9000), (300, 64, 50)])
+def test_a_captured_pass_whose_ignored_rows_change(rows, c, v):
+    """Replays find ignored rows that are finite, then not, then finite again, and other rows ignored."""
+    x, w, b, t = _inputs(rows, c, v, BF16, seed=6)
+    fixed, target = x.detach().clone().requires_grad_(), t.clone()
+    for _ in range(2):
+        torch.autograd.grad(px.linear_cross_entropy(fixed, w, target, bias=b), (fixed, w, b))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss = px.linear_cross_entropy(fixed, w, target, bias=b)
+        out = [loss.detach(), *torch.autograd.grad(loss, (fixed, w, b))]
+    for hold, shift in ((0.0, 0), (math.nan, 0), (math.inf, 1), (1.0, 1)):
+        with torch.no_grad():
+            target.copy_(t.roll(shift))
+            fixed.copy_(torch.where((target == -100)[:, None], hold, x))
+        graph.replay()
+        leaves = [l.detach().clone().requires_grad_() for l in (fixed, w, b)]
+        want = px.linear_cross_entropy(leaves[0], leaves[1], target, bias=leaves[2])
+        for a, z in zip(out, [want.detach(), *torch.autograd.grad(want, leaves)]):
+            assert bool(z.isfinite().all()) and torch.equal(a, z)
+    ops.device_error_flags()

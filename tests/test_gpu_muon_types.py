@@ -118,3 +118,29 @@ def test_a_checkpoint_with_a_momentum_in_16_bits():
     p.grad = torch.randn_like(p)
     opt.step()
     assert opt.state[p]["momentum_buffer"].dtype == torch.float32
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_captured_step(dtype):
+    """Replays move the state and the weights as calls do."""
+    params, others = _parameters(dtype), _parameters(dtype)
+    opt, again = px.Muon(params, lr=0.1, weight_decay=0.1), px.Muon(others, lr=0.1, weight_decay=0.1)
+    grads = [torch.zeros_like(p) for p in params]
+    for p, g in zip(params, grads):
+        p.grad = g
+    for o, ps in ((opt, params), (again, others)):
+        for p in ps:
+            p.grad = torch.zeros_like(p) if ps is others else p.grad
+        o.step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for step in range(3):
+        _give(others, step)
+        for g, q in zip(grads, others):
+            g.copy_(q.grad)
+        graph.replay()
+        again.step()
+        assert all(torch.equal(p, q) for p, q in zip(params, others))
+        assert all(torch.equal(opt.state[p]["momentum_buffer"], again.state[q]["momentum_buffer"]) for p, q in zip(params, others))
